@@ -7,6 +7,7 @@ CPU or eager-PyTorch path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import importlib.util
 import sysconfig
@@ -106,6 +107,14 @@ _SIGNATURES = {
                                    _vp, _ll, _ll, _ll, _ll, _vp, _i, _ll, _ll, _ll,
                                    _i, _i, _i, _i, _i, _i, _i, _f, _vp]),
     "dkv_rope_apply": (_i, [_vp, _i, _vp, _ll, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _i]),
+    "dkv_paged_append": (_i, [_vp, _i, _vp, _ll, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp,
+                              _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _f, _vp]),
+    "dkv_paged_workspace_floats": (_ll, [_i, _i, _i, _i, _i, _i]),
+    "dkv_paged_attention": (_i, [_vp, _i, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp, _ll, _i,
+                                 _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _ll, _vp, _i,
+                                 _ll, _ll]),
+    "dkv_sample_tokens": (_i, [_vp, _i, _vp, _ll, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f,
+                               _vp]),
     "dkv_cutoff_kv": (_i, [_vp, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _ll,
                            _vp, _vp, _ll, _vp, _ll, _i, _i, _i]),
 }
@@ -263,6 +272,15 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which t's device is the current one, as a launch on one of its streams needs."""
+    i = t.get_device()
+    return _NO_GUARD if i == torch.cuda.current_device() else torch.cuda.device(i)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

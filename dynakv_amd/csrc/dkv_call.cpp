@@ -106,6 +106,10 @@ PyMethodDef methods[] = {
     DKV_CALL(dkv_gemv),
     DKV_CALL(dkv_gemv_rmsnorm),
     DKV_CALL(dkv_gemv_glu),
+    DKV_CALL(dkv_paged_append),
+    DKV_CALL(dkv_paged_workspace_floats),
+    DKV_CALL(dkv_paged_attention),
+    DKV_CALL(dkv_sample_tokens),
     {nullptr, nullptr, 0, nullptr},
 };
 

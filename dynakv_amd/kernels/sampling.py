@@ -1,0 +1,74 @@
+"""Sampling of the next token from logits (host side of ``dkv_sample.hip``).
+
+The generators take the most probable token (the reference's benchmark decodes greedily,
+``scripts/benchmark_throughput.py:17-30``; its models inherit transformers' ``generate`` with
+temperature, top-k, top-p and min-p). ``sample_tokens`` draws a token per row under these filters from
+a uniform number that the caller gives, so a draw can be repeated and costs one launch.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+MAX_VOCAB = 1 << 19
+
+
+def _setting(value, rows: int, dtype: torch.dtype, device, name: str):
+    """(pointer of a per-row tensor or None, the value for every row)."""
+    if not torch.is_tensor(value):
+        return None, value
+    if value.shape != (rows,) or value.dtype != dtype or not value.is_contiguous():
+        raise ValueError(f"{name} must be a number or a contiguous ({rows},) {dtype} tensor")
+    if value.device != device:
+        raise ValueError(f"{name} must be on the logits' device")
+    return value.data_ptr(), 0
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A token per row: (rows,) int64.
+
+    ``logits`` (rows, V) in bf16, fp16 or fp32 with unit last stride, V <= 524288; ``u`` (rows,)
+    fp32, uniform in [0, 1). Each setting is a number or a (rows,) tensor (``top_k`` int32, the
+    others fp32). With w_i = exp((l_i - max l) / temperature), and tokens in the order of their
+    logits (of equal ones the lowest index first):
+
+    * ``top_k`` keeps the first k (0, negative or >= V: all);
+    * ``top_p`` keeps, of those, the tokens before which less than ``top_p`` of their mass lies
+      (1 or more: all);
+    * ``min_p`` keeps, of those, the ones with w_i >= ``min_p``.
+
+    The first token is always kept. The result is the first token, in the vocabulary's order, up to
+    which the kept mass exceeds u times all of it. ``temperature`` 0 (or below) takes the first
+    token. A logit of -inf is never taken, NaN counts as -inf, +inf ones share the mass among
+    themselves, and a row with no logit above -inf gives -1. Masses are summed in 64-bit fixed
+    point, so a result depends on the row alone."""
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be (rows, V) with unit last stride")
+    rows, V = logits.shape
+    if V == 0:
+        raise ValueError("logits have no vocabulary")
+    if V > MAX_VOCAB:
+        raise NotImplementedError(f"vocabularies of at most {MAX_VOCAB} tokens")
+    dev = logits.device
+    if u.shape != (rows,) or u.dtype != torch.float32 or not u.is_contiguous() or u.device != dev:
+        raise ValueError(f"u must be a contiguous ({rows},) float32 tensor on the logits' device")
+    t_ptr, t = _setting(temperature, rows, torch.float32, dev, "temperature")
+    k_ptr, k = _setting(top_k, rows, torch.int32, dev, "top_k")
+    p_ptr, p = _setting(top_p, rows, torch.float32, dev, "top_p")
+    m_ptr, m = _setting(min_p, rows, torch.float32, dev, "min_p")
+    st = _lib.stream_of(logits)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+    elif out.shape != (rows,) or out.dtype != torch.int64 or not out.is_contiguous() \
+            or out.device != dev:
+        raise ValueError(f"out must be a contiguous ({rows},) int64 tensor on the logits' device")
+    with _lib.on_device(logits):
+        rc = _lib.calls().dkv_sample_tokens(
+            st, _lib.dtype_code(logits.dtype), logits.data_ptr(),
+            logits.stride(0) if rows > 1 else V, rows, V, u.data_ptr(), t_ptr, float(t), k_ptr,
+            int(min(max(k, 0), V)), p_ptr, float(p), m_ptr, float(m), out.data_ptr())
+    _lib.check(rc, "dkv_sample_tokens")
+    return out

@@ -617,6 +617,62 @@ int dkv_gemv_glu(void* stream, int dtype, const void* x, long long x_ld, const v
                  long long delta_ld, const void* norm_w, float eps, void* r_out, long long r_ld,
                  const void* W, long long w_ld, void* h, long long h_ld, int M, int F, int K);
 
+/*
+ * The paged cache (no counterpart in the reference, whose baseline keeps one length for a whole
+ * batch, scripts/benchmark_throughput.py:17-77). A pool holds num_pages pages of page_size tokens
+ * (a power of two from 16 on), keys and values in pools of the same layout: slot s of KV head g of
+ * page j at element j * page_stride + g * head_stride + s * 128, 128 elements. Token t of request b
+ * is in page page_table[b * table_ld + t / page_size], slot t % page_size. A step's rows
+ * q_start[b] .. q_start[b + 1] - 1 (q_start: B + 1 ascending numbers) are the newest tokens of
+ * request b, the last of them at position lens[b] - 1. Table, starts and lengths are device memory,
+ * read and checked on the device: rows outside [0, T), tokens past table_cols pages and page ids
+ * outside the pool are neither read nor written.
+ *
+ * dkv_paged_append: rows of the fused q/k/v projection (Hq query, Hkv key, Hkv value heads of 128,
+ * row stride qkv_ld). Queries and keys, normed first where q_norm / k_norm (128 weights) are given
+ * (x / sqrt(mean(x^2) + eps) * w), are rotated (rotate-half) by position * inv_freq[j] (64 doubles
+ * in HOST memory, read during the call), in fp32 with the angle in 64 bits, and rounded once: the
+ * queries to q_out (strides q_st per row, q_sh per head), the keys to their page. Values are copied.
+ * 16-byte aligned rows; q_out apart from qkv.
+ *
+ * dkv_paged_attention: q (T, Hq, 128), rotated; the row at position t attends its request's tokens
+ * 0 .. t, softmax in fp32; a row with none gives 0; out in dtype or fp32. Hq / Hkv <= 16. max_new
+ * and max_len bound every request's new tokens and length, min_new (from below) the new tokens of a
+ * request that has any: they choose the launch, and what passes them may be left out. The workspace
+ * holds dkv_paged_workspace_floats(...) floats, its first 16384 zero (and left zero); it may be null
+ * where that is 0. Calls that share it must not overlap.
+ */
+int dkv_paged_append(void* stream, int dtype, const void* qkv, long long qkv_ld, void* q_out,
+                     long long q_st, long long q_sh, void* k_pages, void* v_pages,
+                     long long page_stride, long long head_stride, int num_pages, int page_size,
+                     const int* page_table, long long table_ld, int table_cols, const int* q_start,
+                     const int* lens, int B, int T, int Hq, int Hkv, int Dh, const void* q_norm,
+                     const void* k_norm, float eps, const double* inv_freq);
+long long dkv_paged_workspace_floats(int B, int Hq, int Hkv, int max_new, int min_new, int max_len);
+int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st, long long q_sh,
+                        const void* k_pages, const void* v_pages, long long page_stride,
+                        long long head_stride, int num_pages, int page_size,
+                        const int* page_table, long long table_ld, int table_cols,
+                        const int* q_start, const int* lens, int B, int T, int Hq, int Hkv, int Dh,
+                        int max_new, int min_new, int max_len, float scale, float* workspace,
+                        long long workspace_floats, void* out, int out_dtype, long long o_st,
+                        long long o_sh);
+
+/*
+ * dkv_sample_tokens: one token per row of logits (rows, V <= 524288; row stride ld; bf16, fp16 or
+ * fp32) from a uniform number u[row] in [0, 1). Settings per row where the pointer is given, else the
+ * value beside it. With w_i = exp((l_i - max l) / temperature) and tokens in the order of their
+ * logits (of equal ones the lowest index first): top_k keeps the first k (k <= 0: all), top_p those
+ * before which less than p of the kept mass lies (p >= 1: all), min_p those with w_i >= min_p, the
+ * first token always; the result is the first token in index order up to which the kept mass exceeds
+ * u times all of it. temperature <= 0: the first token. NaN counts as -inf; a row of -inf alone
+ * gives -1.
+ */
+int dkv_sample_tokens(void* stream, int dtype, const void* logits, long long ld, int rows, int V,
+                      const float* u, const float* temperature, float temperature_all,
+                      const int* top_k, int top_k_all, const float* top_p, float top_p_all,
+                      const float* min_p, float min_p_all, long long* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,526 @@
+"""The paged cache's operators on the GPU against the formulas in float64.
+
+Every pool starts full of NaN and every table ends in ids outside the pool, so a slot that is read
+without having been written, or a page that is not the request's, shows in the result; every write
+is checked by comparing the whole pool. Tolerances count the roundings (a 16-bit value is off by at
+most half a step, eps / 2 relative): see ``_append_tol`` and ``_attend_tol``."""
+import math
+
+import pytest
+import torch
+
+from dynakv_amd.kernels.paged import PagedBatch, PagedKVCache, paged_append, paged_attention
+
+DH = 128
+BF, FP = torch.bfloat16, torch.float16
+
+
+class Step:
+    """A step's batch and pools: ``new`` and ``lens`` per request, pages in random order."""
+
+    def __init__(self, dev, new, lens, *, hkv=8, ps=16, dtype=BF, seed=0, layout="plain", pad=0,
+                 spare=2, data=True):
+        self.dev, self.new, self.lens, self.hkv, self.ps, self.dtype = dev, new, lens, hkv, ps, dtype
+        g = self.g = torch.Generator().manual_seed(seed)
+        need = [-(-n // ps) for n in lens]
+        pages = sum(need) + spare
+        ids = torch.randperm(pages, generator=g).tolist()
+        cols = max(need) + 2
+        self.table = torch.full((len(new), cols), pages + 7, dtype=torch.int32)  # not in the pool
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = torch.tensor(ids[at:at + n], dtype=torch.int32)
+            at += n
+        self.starts = [0]
+        for n in new:
+            self.starts.append(self.starts[-1] + n)
+        self.rows = self.starts[-1]
+        self.T = self.rows + pad
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+        self.batch = PagedBatch(self.table.to(dev), i32(self.starts), i32(lens), rows=self.rows,
+                                max_new=max(new), max_len=max(lens),
+                                min_new=min([n for n in new if n], default=0))
+        self.k = self.pool(pages, layout)
+        self.v = self.pool(pages, layout)
+        if data:  # the requests' tokens, the step's own included
+            for b, n in enumerate(lens):
+                for t0 in range(0, n, ps):
+                    m = min(ps, n - t0)
+                    page = int(self.table[b, t0 // ps])
+                    for t in (self.k, self.v):
+                        t[page, :, :m] = self.rand(hkv, m, DH)
+
+    def pool(self, pages, layout):
+        nan = float("nan")
+        if layout == "plain":
+            return torch.full((pages, self.hkv, self.ps, DH), nan, dtype=self.dtype, device=self.dev)
+        # heads first, or pages with room between them
+        if layout == "heads_first":
+            return torch.full((self.hkv, pages, self.ps, DH), nan, dtype=self.dtype,
+                              device=self.dev).transpose(0, 1)
+        return torch.full((pages, self.hkv + 1, self.ps + 16, DH), nan, dtype=self.dtype,
+                          device=self.dev)[:, :self.hkv, :self.ps]
+
+    def rand(self, *dims, scale=1.0):
+        return (torch.randn(*dims, generator=self.g) * scale).to(self.dtype).to(self.dev)
+
+    def tokens(self, pool, b, g):
+        """(len, 128) float64: the keys or values of request b, KV head g."""
+        n = self.lens[b]
+        ids = self.table[b, :-(-n // self.ps)].long().to(self.dev)
+        return pool[ids, g].reshape(-1, DH)[:n].double()
+
+
+# ---------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------
+def _turn(y, pos, freq):
+    """(n, heads, 128) rotated at positions (n,), all float64."""
+    ang = pos[:, None, None] * freq
+    a, b = y[..., :64], y[..., 64:]
+    c, s = torch.cos(ang), torch.sin(ang)
+    return torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+
+
+def _append_reference(s, qkv, heads, freq, q_norm=None, k_norm=None, eps=1e-6):
+    """(queries, keys, values) of the step's rows in float64, and the sizes the tolerance uses."""
+    x = qkv[:s.rows].double().reshape(s.rows, -1)[:, :(heads + 2 * s.hkv) * DH]
+    x = x.view(s.rows, heads + 2 * s.hkv, DH)
+    q, k, v = x[:, :heads], x[:, heads:heads + s.hkv], x[:, heads + s.hkv:]
+    norm = lambda t, w: t if w is None else (  # noqa: E731
+        t / torch.sqrt(t.square().mean(-1, keepdim=True) + eps) * w.double())
+    q, k = norm(q, q_norm), norm(k, k_norm)
+    pos = torch.cat([torch.arange(n - m, n, dtype=torch.float64)
+                     for m, n in zip(s.new, s.lens)]).to(s.dev)
+    size = lambda t: (t[..., :64].abs() + t[..., 64:].abs()).repeat(1, 1, 2)  # noqa: E731
+    return _turn(q, pos, freq), _turn(k, pos, freq), v, size(q), size(k)
+
+
+def _append_tol(want, size, dtype):
+    """Half a step of the result; before that fp32 work on the pair: the norm's sum of 128 squares,
+    root, division and two products (a relative 2^-24 each, under 32 of them), the part of a
+    revolution in fp32 (2 pi 2^-25) and the sine and cosine instructions (2^-18 at most is assumed
+    of them), each times the pair's size."""
+    return torch.finfo(dtype).eps / 2 * want.abs() + size * (2.0**-18 + 2.0**-19) + 1e-30
+
+
+def _freq(dev, theta):
+    return torch.tensor([theta ** (-2.0 * j / DH) for j in range(64)], dtype=torch.float64,
+                        device=dev)
+
+
+def _check_append(s, heads, *, theta=500000.0, norms=False, inv_freq=None, qkv=None, out=None,
+                  wide=0):
+    if qkv is None:
+        qkv = s.rand(s.T, (heads + 2 * s.hkv) * DH + wide)
+    qn = kn = None
+    if norms:
+        qn, kn = 1 + s.rand(DH, scale=0.2), 1 + s.rand(DH, scale=0.2)
+    k0, v0, x0 = s.k.clone(), s.v.clone(), qkv.clone()
+    q = paged_append(qkv, s.k, s.v, s.batch, heads=heads,
+                     theta=None if inv_freq is not None else theta, inv_freq=inv_freq, q_norm=qn,
+                     k_norm=kn, out=out)
+    freq = (_freq(s.dev, theta) if inv_freq is None
+            else torch.tensor(inv_freq, dtype=torch.float64, device=s.dev))
+    wq, wk, wv, sq, sk = _append_reference(s, qkv, heads, freq, qn, kn)
+    assert torch.equal(qkv, x0), "the projection was written to"
+    assert bool(((q[:s.rows].double() - wq).abs() <= _append_tol(wq, sq, s.dtype)).all())
+    # the pools: the written slots within their tolerance, every other slot as it was
+    at = 0
+    for b, (m, n) in enumerate(zip(s.new, s.lens)):
+        for t in range(n - m, n):
+            page, slot = int(s.table[b, t // s.ps]), t % s.ps
+            err = (s.k[page, :, slot].double() - wk[at]).abs()
+            assert bool((err <= _append_tol(wk[at], sk[at], s.dtype)).all()), (b, t)
+            assert torch.equal(s.v[page, :, slot].double(), wv[at]), (b, t)
+            k0[page, :, slot], v0[page, :, slot] = s.k[page, :, slot], s.v[page, :, slot]
+            at += 1
+    bits = lambda t: t.contiguous().view(torch.int16)  # noqa: E731  (NaN equals itself)
+    assert torch.equal(bits(s.k), bits(k0)) and torch.equal(bits(s.v), bits(v0))
+    return q
+
+
+APPEND = {
+    # name: (new tokens, lengths, query heads, KV heads, page, dtype, norms, layout)
+    "one_token": ([1], [1], 4, 2, 16, BF, False, "plain"),
+    "step_of_five": ([1] * 5, [33, 1, 16, 17, 250], 32, 8, 16, BF, False, "plain"),
+    "prompts": ([40, 1, 65], [40, 1, 65], 8, 2, 32, FP, True, "plain"),
+    "chunk_far_out": ([33], [100033], 4, 1, 128, FP, False, "plain"),
+    "none_and_some": ([0, 3, 0, 0, 18, 0], [5, 3, 0, 31, 20, 7], 6, 3, 16, BF, True, "plain"),
+    "heads_first": ([9, 2], [30, 50], 14, 2, 16, FP, True, "heads_first"),
+    "pages_apart": ([9, 2], [30, 50], 8, 8, 64, BF, False, "apart"),
+    "many_requests": ([1, 0, 2] * 70, [5, 9, 18] * 70, 2, 1, 16, BF, False, "plain"),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(APPEND))
+def test_append(dev, name):
+    new, lens, hq, hkv, ps, dt, norms, layout = APPEND[name]
+    print(f"[gpu] paged append {name}", flush=True)
+    s = Step(dev, new, lens, hkv=hkv, ps=ps, dtype=dt, layout=layout, seed=3, data=False)
+    _check_append(s, hq, norms=norms)
+
+
+@pytest.mark.gpu
+def test_append_given_frequencies_and_strides(dev):
+    print("[gpu] paged append frequencies, strides", flush=True)
+    inv = [(1.0 if j < 20 else 0.125) * 10000.0 ** (-2.0 * j / DH) for j in range(64)]
+    s = Step(dev, [7, 20], [4000, 20], hkv=2, dtype=FP, seed=4, data=False)
+    whole = torch.full((s.T, 5, 2 * DH), 5.0, dtype=FP, device=dev)
+    out = whole[:, 1:, :DH]  # rows and heads apart
+    q = _check_append(s, 4, inv_freq=inv, out=out, wide=24)
+    assert q.data_ptr() == out.data_ptr()
+    whole[:, 1:, :DH] = 5.0
+    assert bool((whole == 5.0).all())
+
+
+@pytest.mark.gpu
+def test_append_leaves_padding_rows(dev):
+    """Rows behind the last request: their queries keep what ``out`` held, nothing is stored."""
+    print("[gpu] paged append padding", flush=True)
+    s = Step(dev, [3, 0, 4], [20, 4, 4], hkv=2, seed=5, pad=30, data=False)
+    out = torch.full((s.T, 4, DH), 7.0, dtype=BF, device=dev)
+    _check_append(s, 4, out=out, norms=True)
+    assert bool((out[s.rows:] == 7.0).all()) and not bool((out[:s.rows] == 7.0).all())
+
+
+@pytest.mark.gpu
+def test_append_skips_what_has_no_place(dev):
+    """Tokens whose page id is outside the pool, or past the table, are not stored; their queries
+    are rotated all the same. A request whose length is smaller than its rows has its first rows
+    left out."""
+    print("[gpu] paged append bad pages", flush=True)
+    s = Step(dev, [20, 4, 3], [40, 4, 3], hkv=2, seed=6, data=False)
+    table = s.table.clone()
+    table[0, 1], table[1, 0] = -5, 2**30  # tokens 16 .. 31 of request 0, all of request 1
+    lens = torch.tensor([40, 4, 2], dtype=torch.int32, device=dev)
+    batch = PagedBatch(table.to(dev), s.batch.q_start, lens, rows=s.rows, max_new=20, max_len=40)
+    qkv = s.rand(s.T, 8 * DH)
+    q = paged_append(qkv, s.k, s.v, batch, heads=4, theta=1e4,
+                     out=torch.zeros(s.T, 4, DH, dtype=BF, device=dev))
+    written = ~torch.isnan(s.v[:, 0, :, 0])
+    assert int(written.sum()) == (40 - 32) + 0 + 2
+    assert int((~torch.isnan(s.k)).sum()) == 10 * 2 * DH
+    assert bool((q[24] == 0).all()) and bool((q[:24].abs().sum((1, 2)) > 0).all())
+    cut = PagedBatch(s.table[:, :1].contiguous().to(dev), s.batch.q_start, s.batch.lens,
+                     rows=s.rows, max_new=20, max_len=16)
+    s.k.fill_(float("nan")), s.v.fill_(float("nan"))
+    paged_append(qkv, s.k, s.v, cut, heads=4, theta=1e4)
+    assert int((~torch.isnan(s.v[:, 0, :, 0])).sum()) == 0 + 4 + 3
+
+
+# ---------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------
+def _attend_reference(s, q, scale=None):
+    """(rows, heads, 128) float64 and the error bound of the result before its own rounding."""
+    hq = q.shape[1]
+    hpg, scale = hq // s.hkv, scale or 1 / math.sqrt(DH)
+    out = torch.zeros(s.rows, hq, DH, dtype=torch.float64, device=s.dev)
+    tol = torch.zeros_like(out)
+    # a score: 128 products summed in fp32, of size at most a; then the softmax's weight to bf16
+    # (its half step is the larger one; fp16's is smaller) and the rest of the softmax in fp32
+    half = torch.finfo(s.dtype).eps / 2
+    for b, (m, n) in enumerate(zip(s.new, s.lens)):
+        if m == 0:
+            continue
+        r = slice(s.starts[b], s.starts[b] + m)
+        dead = (torch.arange(n, device=s.dev)[None, :]
+                > torch.arange(n - m, n, device=s.dev)[:, None])
+        for h in range(hq):
+            k, v = s.tokens(s.k, b, h // hpg), s.tokens(s.v, b, h // hpg)
+            z = (q[r, h].double() @ k.T) * scale
+            p = torch.softmax(z.masked_fill(dead, -math.inf), -1)
+            a = ((q[r, h].double().abs() @ k.abs().T) * scale).masked_fill(dead, 0).amax(-1)
+            out[r, h] = p @ v
+            rel = half + 2 * 130 * 2.0**-24 * a[:, None] + 2.0**-18
+            tol[r, h] = rel * (p @ v.abs())
+    return out, tol
+
+
+def _check_attend(s, hq, *, scale=None, qscale=1.0, q=None):
+    if q is None:
+        q = s.rand(s.T, hq, DH, scale=qscale)
+    want, tol = _attend_reference(s, q, scale)
+    got = paged_attention(q, s.k, s.v, s.batch, scale=scale, out_dtype=torch.float32)
+    err = (got[:s.rows].double() - want).abs()
+    print(f"[gpu]   err/tol {float((err / (tol + 1e-30)).max()):.3f}", flush=True)
+    assert bool((err <= tol + 1e-30).all())
+    got16 = paged_attention(q, s.k, s.v, s.batch, scale=scale)
+    assert got16.dtype == s.dtype and torch.equal(got16[:s.rows], got[:s.rows].to(s.dtype))
+    return got
+
+
+ATTEND = {
+    # name: (new tokens, lengths, query heads, KV heads, page, dtype, layout)
+    "one_key": ([1], [1], 4, 2, 16, BF, "plain"),
+    "lens_around_tiles": ([1] * 8, [15, 16, 17, 63, 64, 65, 127, 129], 8, 2, 16, BF, "plain"),
+    "step_fp16": ([1] * 5, [1, 300, 77, 1023, 512], 32, 8, 32, FP, "plain"),
+    "step_long": ([1, 1], [8195, 5000], 32, 8, 64, BF, "plain"),
+    "one_long": ([1], [20011], 8, 8, 128, FP, "plain"),
+    "hpg16": ([1, 1, 1], [700, 31, 1500], 32, 2, 16, BF, "plain"),
+    "hpg7_drafts": ([5, 2, 7], [500, 90, 7], 14, 2, 16, FP, "plain"),
+    "drafts_long": ([4, 3], [6000, 4097], 8, 2, 32, BF, "plain"),
+    "hpg3_prompt": ([100, 33], [100, 33], 6, 2, 16, BF, "plain"),
+    "prompt": ([257, 64], [257, 64], 8, 2, 64, FP, "plain"),
+    "prompt_odd": ([333, 1, 190], [333, 1, 190], 4, 4, 128, BF, "plain"),
+    "chunk": ([130, 61], [1500, 61], 8, 2, 16, BF, "plain"),
+    "chunk_long": ([40], [9001], 8, 2, 32, FP, "plain"),
+    "mixed": ([1, 1, 150, 1, 0, 3, 1], [400, 17, 700, 1, 9, 2000, 64], 8, 2, 32, BF, "plain"),
+    "heads_first": ([1, 70], [130, 95], 8, 2, 32, FP, "heads_first"),
+    "pages_apart": ([1, 70, 2], [130, 95, 600], 16, 1, 16, BF, "apart"),
+    "none_at_all": ([0, 2, 0], [5, 2, 0], 4, 1, 16, BF, "plain"),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(ATTEND))
+def test_attention(dev, name):
+    new, lens, hq, hkv, ps, dt, layout = ATTEND[name]
+    print(f"[gpu] paged attention {name}", flush=True)
+    _check_attend(Step(dev, new, lens, hkv=hkv, ps=ps, dtype=dt, layout=layout, seed=11), hq)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 1], [700, 90]), ([80, 5], [300, 200])])
+def test_attention_peaked_and_scaled(dev, new, lens):
+    """A near one-hot softmax (the running maximum rises late), and a scale of its own."""
+    print(f"[gpu] paged attention peaked {new}", flush=True)
+    _check_attend(Step(dev, new, lens, hkv=2, seed=12), 8, qscale=8.0)
+    _check_attend(Step(dev, new, lens, hkv=2, seed=13, dtype=FP), 8, scale=0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1] * 3, [700, 90, 33]), ([80, 5], [300, 200])])
+def test_attention_leaves_padding_rows(dev, new, lens):
+    print(f"[gpu] paged attention padding {new}", flush=True)
+    s = Step(dev, new, lens, hkv=2, seed=14, pad=9)
+    q = s.rand(s.T, 8, DH)
+    want, tol = _attend_reference(s, q)
+    whole = torch.full((s.T, 9, 2 * DH), 3.0, dtype=torch.float32, device=dev)
+    out = whole[:, :8, :DH]
+    got = paged_attention(q, s.k, s.v, s.batch, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert bool(((out[:s.rows].double() - want).abs() <= tol + 1e-30).all())
+    out[:s.rows] = 3.0
+    assert bool((whole == 3.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 3, 60])
+def test_attention_masks_pages_that_are_not_there(dev, new):
+    """A page id outside the pool: its keys are masked. No page at all, or a length of zero: 0."""
+    print(f"[gpu] paged attention bad pages {new}", flush=True)
+    s = Step(dev, [new] * 4, [150, 150, 150, 60], hkv=2, seed=15)
+    q = s.rand(s.T, 4, DH)
+    want, _ = _attend_reference(s, q)
+    s.table[1, 2], s.table[1, 5] = -1, 10**6      # tokens 32 .. 47 and 80 .. 95 of request 1
+    s.table[2] = -1                               # all of request 2
+    lens = torch.tensor([150, 150, 150, 0], dtype=torch.int32, device=dev)
+    batch = PagedBatch(s.table.to(dev), s.batch.q_start, lens, rows=s.rows, max_new=new,
+                       max_len=150, min_new=new)
+    got = paged_attention(q, s.k, s.v, batch, out_dtype=torch.float32)
+    pos = torch.arange(150 - new, 150, device=dev)[:, None]
+    key = torch.arange(150, device=dev)[None]
+    dead = (key > pos) | ((key // 16) == 2) | ((key // 16) == 5)
+    good = [int(i) if 0 <= int(i) < s.k.shape[0] else 0 for i in s.table[1, :10]]
+    for h in range(4):
+        k = s.k[good, h // 2].reshape(-1, DH)[:150].double().nan_to_num()
+        v = s.v[good, h // 2].reshape(-1, DH)[:150].double().nan_to_num()
+        z = (q[new:2 * new, h].double() @ k.T / math.sqrt(DH)).masked_fill(dead, -math.inf)
+        p = torch.softmax(z, -1)
+        tol = 2.0**-7 * (p @ v.abs()) + 1e-30
+        assert bool(((got[new:2 * new, h].double() - p @ v).abs() <= tol).all())
+        err = (got[:new, h].double() - want[:new, h]).abs()
+        assert bool((err <= 2.0**-7 * 4).all())
+    assert bool((got[2 * new:] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 1], [900, 450]), ([90, 2], [350, 200])])
+def test_attention_same_result_every_time(dev, new, lens):
+    print(f"[gpu] paged attention repeat {new}", flush=True)
+    s = Step(dev, new, lens, hkv=2, seed=16)
+    q = s.rand(s.T, 8, DH)
+    first = paged_attention(q, s.k, s.v, s.batch)
+    for _ in range(3):
+        assert torch.equal(paged_attention(q, s.k, s.v, s.batch), first)
+    strided = torch.empty(s.T, 8, 2, DH, dtype=BF, device=dev)[:, :, 1]
+    strided.copy_(q)
+    assert torch.equal(paged_attention(strided, s.k, s.v, s.batch), first)
+
+
+def _random_step(i):
+    g = torch.Generator().manual_seed(500 + i)
+    r = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
+    hkv = [1, 2, 3, 8][r(0, 3)]
+    hq = hkv * [1, 2, 4, 5, 8, 16][r(0, 5)]
+    n = r(1, 6)
+    kind = r(0, 3)
+    new = [[1, r(1, 6), r(1, 200), [0, 1, r(2, 90)][r(0, 2)]][kind] for _ in range(n)]
+    if not any(new):
+        new[0] = 1
+    lens = [m + (0 if r(0, 2) == 0 else int(math.exp(float(torch.rand(1, generator=g)) * 8)))
+            for m in new]
+    return new, lens, hq, hkv, [16, 32, 64, 128, 256][r(0, 4)], [BF, FP][r(0, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(16))
+def test_random_steps(dev, i):
+    """Append, then attention, of a random step."""
+    new, lens, hq, hkv, ps, dt = _random_step(i)
+    print(f"[gpu] random step {i}: {new} {lens} {hq}/{hkv} page {ps} {dt}", flush=True)
+    s = Step(dev, new, lens, hkv=hkv, ps=ps, dtype=dt, seed=600 + i)
+    q = _check_append(s, hq, norms=i % 2 == 0)
+    _check_attend(s, hq, q=q)
+
+
+# ---------------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_chunks_give_what_a_whole_prompt_gives(dev):
+    """Three requests through a cache: prompts in chunks of different sizes beside single tokens,
+    one request ended and its pages reused, one cut back; every output against attention over the
+    request's tokens kept aside."""
+    print("[gpu] paged chunks", flush=True)
+    hq, hkv, theta = 8, 2, 10000.0
+    cache = PagedKVCache(1, 24, hkv, page_size=16, device=dev)
+    cache.k[0].fill_(float("nan")), cache.v[0].fill_(float("nan"))
+    g = torch.Generator().manual_seed(77)
+    rand = lambda n: torch.randn(n, (hq + 2 * hkv) * DH, generator=g).to(BF).to(dev)  # noqa: E731
+    kept: dict = {}
+    a, b, c = cache.add(), cache.add(), cache.add()
+
+    def step(parts):
+        qkv = rand(sum(n for _, n in parts))
+        batch = cache.batch(parts)
+        q = paged_append(qkv, cache.k[0], cache.v[0], batch, heads=hq, theta=theta)
+        o = paged_attention(q, cache.k[0], cache.v[0], batch, out_dtype=torch.float32)
+        at = 0
+        for r, n in parts:
+            kept[r] = torch.cat([kept[r], qkv[at:at + n]]) if r in kept else qkv[at:at + n]
+            total = kept[r].shape[0]
+            assert total == cache.length(r)
+            x = kept[r].double().view(total, hq + 2 * hkv, DH)
+            pos = torch.arange(total, dtype=torch.float64, device=dev)
+            y = _turn(x[:, :hq + hkv], pos, _freq(dev, theta)).to(BF).double()
+            for h in range(hq):
+                z = y[total - n:, h] @ y[:, hq + h // 4].T / math.sqrt(DH)
+                z.masked_fill_(torch.arange(total, device=dev)[None]
+                               > torch.arange(total - n, total, device=dev)[:, None], -math.inf)
+                v = x[:, hq + hkv + h // 4]
+                p = torch.softmax(z, -1)
+                # a key or query may round to the other neighbour: one step of one of 128 products
+                # moves a score by at most 2^-7 |q||k| / sqrt(128); 2^-6 covers it and the weights
+                assert bool(((o[at:at + n, h].double() - p @ v).abs()
+                             <= 2.0**-6 * (p @ v.abs()) + 2.0**-7).all()), (r, total, h)
+            at += n
+
+    step([(a, 70), (b, 5)])
+    step([(b, 40), (a, 1)])
+    step([(a, 1), (c, 100), (b, 1)])
+    cache.truncate(c, 90)
+    kept[c] = kept[c][:90]
+    step([(a, 1), (b, 0), (c, 3)])
+    cache.free(a)
+    d = cache.add()
+    step([(d, 130), (c, 1), (b, 2)])
+    step([(d, 1), (c, 1), (b, 1)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1] * 4, [700, 90, 33, 260]), ([60, 1, 9], [300, 200, 100])])
+def test_captured_step(dev, new, lens):
+    """A captured append and attention, replayed with other inputs, lengths and pages in the same
+    buffers, with eager work between the replays; two graphs replayed at once on two streams."""
+    print(f"[gpu] paged graph {new}", flush=True)
+    side = torch.cuda.Stream()
+    s = [Step(dev, new, lens, hkv=2, seed=21 + i) for i in range(2)]
+    qkv = [t.rand(t.T, 12 * DH) for t in s]
+    one = lambda i: paged_attention(  # noqa: E731
+        paged_append(qkv[i], s[i].k, s[i].v, s[i].batch, heads=8, theta=1e4), s[i].k, s[i].v,
+        s[i].batch)
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        for i in range(2):
+            one(i)
+        torch.cuda.synchronize()
+        for i in range(2):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=side):
+                outs.append(one(i))
+            graphs.append(gr)
+    torch.cuda.synchronize()
+    other = Step(dev, [1], [3000], hkv=2, seed=29)
+    oq = other.rand(1, 8, DH)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        for i in range(2):
+            qkv[i].copy_(s[i].rand(s[i].T, 12 * DH))
+            if rep == 2:  # shorter, and two pages changed places
+                t = s[i]
+                t.lens = [max(m, n - 20) for m, n in zip(t.new, t.lens)]
+                t.batch.lens.copy_(torch.tensor(t.lens, dtype=torch.int32))
+                t.table[0, [0, 1]] = t.table[0, [1, 0]]
+                t.batch.page_table.copy_(t.table)
+        paged_attention(oq, other.k, other.v, other.batch)
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            got, k, v = outs[i].clone(), s[i].k.clone(), s[i].v.clone()
+            assert torch.equal(one(i), got), (rep, i)
+            assert torch.equal(s[i].k.view(torch.int16), k.view(torch.int16))
+            assert torch.equal(s[i].v.view(torch.int16), v.view(torch.int16))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    print("[gpu] paged two streams", flush=True)
+    s = [Step(dev, [1, 2], [1500, 1100 + 300 * i], hkv=2, seed=31 + i) for i in range(2)]
+    q = [t.rand(t.T, 8, DH) for t in s]
+    want = [paged_attention(q[i], s[i].k, s[i].v, s[i].batch) for i in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(paged_attention(q[i], s[i].k, s[i].v, s[i].batch))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            assert torch.equal(o, want[i])
+
+
+@pytest.mark.gpu
+def test_pool_past_32_bits(dev):
+    """Pages whose elements lie past 2^32 bytes of the pool's start."""
+    print("[gpu] paged large pool", flush=True)
+    ps, hkv, pages = 256, 2, 40000  # 5.2 GB each for keys and values
+    k = torch.empty(pages, hkv, ps, DH, dtype=BF, device=dev)
+    v = torch.empty_like(k)
+    g = torch.Generator().manual_seed(41)
+    for new, n in ((1, 700), (70, 700)):
+        ids = torch.tensor([[pages - 1, 3, pages - 900]], dtype=torch.int32)
+        for i in ids[0].tolist():
+            k[i] = torch.randn(hkv, ps, DH, generator=g).to(BF)
+            v[i] = torch.randn(hkv, ps, DH, generator=g).to(BF)
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        batch = PagedBatch(ids.to(dev), i32(0, new), i32(n), rows=new, max_new=new, max_len=n,
+                           min_new=new)
+        small = Step(dev, [new], [n], hkv=hkv, ps=ps, seed=42)
+        qkv = small.rand(new, 8 * DH)
+        order = small.table[0, :3].long().to(dev)
+        small.k[order], small.v[order] = k[ids[0].long().to(dev)], v[ids[0].long().to(dev)]
+        qa = paged_append(qkv, k, v, batch, heads=4, theta=1e4)
+        qb = paged_append(qkv, small.k, small.v, small.batch, heads=4, theta=1e4)
+        assert torch.equal(qa, qb) and torch.equal(k[ids[0].long().to(dev)], small.k[order])
+        assert torch.equal(v[ids[0].long().to(dev)], small.v[order])
+        assert torch.equal(paged_attention(qa, k, v, batch),
+                           paged_attention(qb, small.k, small.v, small.batch))

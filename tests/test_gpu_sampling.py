@@ -1,0 +1,244 @@
+"""Sampling on the GPU against the definition in float64: whole numbers, so equal ones.
+
+The inputs make the filters' borders matter (ties, integers, borders on a tie); where a border falls
+between float64 values no result depends on the last bit of a sum: weights of equal logits are equal,
+and random logits put the nearest border far from any sum's error."""
+import math
+
+import pytest
+import torch
+
+from dynakv_amd.kernels.sampling import sample_tokens
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _one(x, u, t, k, p, mp):
+    """The definition, for one row (float64 on the CPU)."""
+    x = torch.where(torch.isnan(x), -math.inf, x)
+    m = x.max()
+    if m == -math.inf:
+        return -1
+    order = torch.sort(x, descending=True, stable=True).indices
+    if not t > 0:
+        return int(order[0])
+    w = torch.where(x == m, 1.0, torch.exp((x - m) / t))
+    w = torch.where(x == -math.inf, 0.0, w)
+    if k > 0:
+        order = order[:k]
+    if p < 1:
+        c = torch.cumsum(w[order], 0)
+        order = order[:max(1, int((c - w[order] < p * c[-1]).sum()))]
+    kept = order[w[order] >= mp]
+    if len(kept) == 0:
+        kept = order[:1]
+    ids = torch.sort(kept).values
+    c = torch.cumsum(w[ids], 0)
+    i = int((c <= u * c[-1]).sum())
+    if i >= len(ids):
+        i = int((c < c[-1]).sum())
+    return int(ids[i])
+
+
+def _all(x, u, t, k, p, mp):
+    at = lambda v, b: float(v[b]) if torch.is_tensor(v) else float(v)  # noqa: E731
+    x, u = x.double().cpu(), u.double().cpu()
+    t, p, mp = (v.cpu() if torch.is_tensor(v) else torch.tensor(v, dtype=torch.float32).item()
+                for v in (t, p, mp))
+    k = k.cpu() if torch.is_tensor(k) else k
+    return [_one(x[b], float(u[b]), at(t, b), int(at(k, b)), at(p, b), at(mp, b))
+            for b in range(x.shape[0])]
+
+
+def _check(x, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    got = sample_tokens(x, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    assert got.dtype == torch.int64 and got.shape == (x.shape[0],)
+    want = _all(x, u, temperature, top_k, top_p, min_p)
+    assert got.tolist() == want
+    return got
+
+
+def _inputs(dev, rows, V, dtype, seed, scale=2.5):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, V, generator=g) * scale).to(DT[dtype])
+    return x.to(dev), torch.rand(rows, generator=g).to(dev), g
+
+
+SETTINGS = {
+    "plain": {},
+    "cold": dict(temperature=0.3),
+    "hot": dict(temperature=5.0),
+    "greedy": dict(temperature=0.0),
+    "top_k": dict(top_k=40),
+    "top_p": dict(top_p=0.9),
+    "min_p": dict(min_p=0.05),
+    "k_then_p": dict(top_k=100, top_p=0.8, temperature=0.7),
+    "all": dict(top_k=300, top_p=0.95, min_p=0.02, temperature=1.3),
+    "wide": dict(top_p=0.9999, top_k=100000),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("name", list(SETTINGS))
+def test_settings(dev, name, dtype):
+    print(f"[gpu] sample {name} {dtype}", flush=True)
+    for rows, V in ((9, 1000), (3, 32000), (2, 50257)):
+        x, u, _ = _inputs(dev, rows, V, dtype, 7 * V + rows)
+        _check(x, u, **SETTINGS[name])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [1, 2, 7, 63, 64, 65, 511, 513, 1023, 1025, 8191, 131071, 131073,
+                               200003, 524288])
+def test_vocabulary_sizes(dev, V):
+    print(f"[gpu] sample V={V}", flush=True)
+    for dtype in ("bf16", "fp32"):
+        x, u, _ = _inputs(dev, 2, V, dtype, V)
+        _check(x, u, top_p=0.9)
+        _check(x, u, top_k=3)
+        _check(x, u)
+
+
+@pytest.mark.gpu
+def test_settings_of_each_row(dev):
+    print("[gpu] sample per row", flush=True)
+    x, u, g = _inputs(dev, 64, 5003, "fp32", 5)
+    r = lambda lo, hi: (lo + (hi - lo) * torch.rand(64, generator=g)).to(dev)  # noqa: E731
+    t, p, mp = r(0.0, 1.5), r(0.5, 1.1), r(-0.02, 0.1)
+    t[::7] = 0.0
+    t[1] = -1.0
+    k = torch.randint(-1, 60, (64,), generator=g, dtype=torch.int32).to(dev)
+    _check(x, u, temperature=t, top_k=k, top_p=p, min_p=mp)
+    _check(x, u, temperature=t, top_k=5, top_p=p)
+    _check(x, u, top_k=k, min_p=0.2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_ties(dev, dtype):
+    """Few distinct logits: every border falls inside a run of equal ones, the lowest indices of
+    which are kept; equal weights make a mass of exactly p or u a real case."""
+    print(f"[gpu] sample ties {dtype}", flush=True)
+    g = torch.Generator().manual_seed(9)
+    x = torch.randint(-2, 3, (16, 4099), generator=g).to(DT[dtype]).to(dev)
+    u = torch.rand(16, generator=g).to(dev)
+    for kw in (dict(top_k=1), dict(top_k=2), dict(top_k=900), dict(top_k=4098), dict(top_p=0.5),
+               dict(top_p=0.999), dict(top_k=1700, top_p=0.7), dict(min_p=1.0), dict(min_p=0.3),
+               dict(top_p=1e-6), dict(temperature=0.0), {}):
+        _check(x, u, **kw)
+    same = torch.full((8, 1024), 0.5, dtype=DT[dtype], device=dev)
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.9990234375, 0.125, 1 - 2.0**-24, 0.0009765625],
+                     device=dev)
+    assert _check(same, u).tolist() == [0, 256, 512, 768, 1023, 128, 1023, 1]
+    assert _check(same, u, top_k=512).tolist() == [0, 128, 256, 384, 511, 64, 511, 0]
+    assert _check(same, u, top_p=0.5).tolist() == [0, 128, 256, 384, 511, 64, 511, 0]
+    zero = torch.zeros(2, 300, dtype=DT[dtype], device=dev)
+    zero[:, ::2] = -0.0  # equal to 0: the order is the index's
+    assert _check(zero, u[2:4], top_k=10).tolist() == [5, 7]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_what_cannot_be_taken(dev, dtype):
+    print(f"[gpu] sample masked {dtype}", flush=True)
+    inf, nan = math.inf, math.nan
+    x, u, _ = _inputs(dev, 8, 3001, dtype, 21)
+    low = torch.finfo(DT[dtype]).min
+    x[0] = -inf                       # nothing to take
+    x[1] = -inf
+    x[1, 2222] = -3.0                 # one token
+    x[2] = nan
+    x[3] = nan
+    x[3, 17] = 1.0
+    x[4, 100] = inf                   # takes all the mass
+    x[5, [5, 700, 3000]] = inf        # shared
+    x[6] = low                        # the type's lowest value: an ordinary, equal logit
+    x[7, ::2] = -inf
+    x[7, 1::4] = nan
+    for kw in ({}, dict(top_k=50), dict(top_p=0.8), dict(min_p=0.1, top_k=7, top_p=0.9),
+               dict(temperature=0.0), dict(temperature=1e-30), dict(temperature=1e30, top_p=0.7)):
+        got = _check(x, u, **kw).tolist()
+        assert got[0] == -1 and got[1] == 2222 and got[2] == -1 and got[3] == 17 and got[4] == 100
+        assert got[5] in (5, 700, 3000) and got[7] % 4 == 3
+
+
+@pytest.mark.gpu
+def test_extreme_settings(dev):
+    print("[gpu] sample extreme settings", flush=True)
+    x, u, _ = _inputs(dev, 6, 777, "fp32", 31)
+    best = x.argmax(-1).tolist()
+    for kw in (dict(top_p=0.0), dict(top_p=-1.0), dict(min_p=2.0), dict(top_k=1),
+               dict(temperature=-1.0), dict(temperature=1e-38), dict(min_p=1.0)):
+        assert _check(x, u, **kw).tolist() == best
+    full = _check(x, u).tolist()
+    for kw in (dict(top_p=1.0), dict(top_p=3.0), dict(top_k=777), dict(top_k=10**9),
+               dict(top_k=-4), dict(min_p=0.0), dict(min_p=-1.0)):
+        assert _check(x, u, **kw).tolist() == full
+    # numbers that are no uniform ones stay inside what is kept
+    odd = torch.tensor([1.0, 2.0, -1.0, math.nan, math.inf, 0.0], device=dev)
+    got = sample_tokens(x, odd, top_k=5)
+    for b in range(6):
+        assert int(got[b]) in torch.topk(x[b], 5).indices.tolist()
+
+
+@pytest.mark.gpu
+def test_far_apart_logits(dev):
+    """Borders far below the largest logit, and logits of both signs and all sizes."""
+    print("[gpu] sample far apart", flush=True)
+    g = torch.Generator().manual_seed(41)
+    x = (torch.randn(6, 9001, generator=g) * torch.exp(6 * torch.randn(6, 9001, generator=g)))
+    u = torch.rand(6, generator=g).to(dev)
+    for dtype in ("fp32", "bf16"):
+        y = x.clamp(-60000, 60000).to(DT[dtype]).to(dev)
+        for kw in (dict(top_k=4500), dict(top_k=9000), dict(temperature=30000.0, top_p=0.6),
+                   dict(temperature=1e4, top_k=5000, top_p=0.99)):
+            _check(y, u, **kw)
+        _check(y - 70000 if dtype == "fp32" else -y.abs(), u, top_k=4000, temperature=100.0)
+
+
+@pytest.mark.gpu
+def test_strides_and_out(dev):
+    print("[gpu] sample strides", flush=True)
+    for dtype in DT:
+        whole, u, _ = _inputs(dev, 5, 4003, dtype, 51)
+        x = whole[:, 3:3 + 3333]  # rows that start anywhere
+        out = torch.full((5,), -9, dtype=torch.int64, device=dev)
+        got = sample_tokens(x, u, top_p=0.9, out=out)
+        assert got.data_ptr() == out.data_ptr()
+        assert got.tolist() == _all(x, u, 1.0, 0, 0.9, 0.0)
+    assert sample_tokens(whole[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.gpu
+def test_draws_follow_the_weights(dev):
+    """A grid of u over [0, 1): every token is drawn on its share of the grid."""
+    print("[gpu] sample shares", flush=True)
+    n = 4096
+    x = torch.tensor([0.0, 1.0, -1.0, 3.0, 2.0, -math.inf, 0.5], device=dev)
+    u = (torch.arange(n, device=dev, dtype=torch.float32) + 0.5) / n
+    got = sample_tokens(x.expand(n, -1).contiguous(), u, temperature=0.8)
+    share = torch.bincount(got, minlength=7).double() / n
+    want = torch.softmax(x.double() / torch.tensor(0.8, dtype=torch.float32).item(), 0)
+    assert bool(((share - want).abs() <= 1.0 / n + 1e-9).all())
+    assert bool((got[1:] >= got[:-1]).all())
+
+
+@pytest.mark.gpu
+def test_captured_and_repeated(dev):
+    print("[gpu] sample graph", flush=True)
+    x, u, g = _inputs(dev, 12, 32000, "bf16", 61)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        sample_tokens(x, u, top_k=50, top_p=0.9)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            got = sample_tokens(x, u, top_k=50, top_p=0.9)
+    for _ in range(4):
+        x.copy_((torch.randn(12, 32000, generator=g) * 3).to(torch.bfloat16))
+        u.copy_(torch.rand(12, generator=g))
+        gr.replay()
+        torch.cuda.synchronize()
+        assert got.tolist() == sample_tokens(x, u, top_k=50, top_p=0.9).tolist()
+        assert got.tolist() == _all(x, u, 1.0, 50, 0.9, 0.0)

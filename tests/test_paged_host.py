@@ -1,0 +1,194 @@
+"""The paged cache's host side, without a device: pages taken and given back, the batch's buffers,
+and the refusals of the operators (checked before anything touches a device)."""
+import pytest
+import torch
+
+from dynakv_amd import _lib
+from dynakv_amd.kernels.paged import PagedBatch, PagedKVCache, paged_append, paged_attention
+from dynakv_amd.kernels.sampling import sample_tokens
+
+BF = torch.bfloat16
+
+
+def _cache(pages=10, **kw):
+    return PagedKVCache(2, pages, 2, page_size=16, device="cpu", **kw)
+
+
+def test_pages_are_taken_as_tokens_need_them():
+    c = _cache()
+    a, b = c.add(), c.add()
+    batch = c.batch([(a, 17), (b, 16)])
+    assert (c.length(a), c.length(b), c.free_pages) == (17, 16, 7)
+    assert batch.q_start.tolist() == [0, 17, 33] and batch.lens.tolist() == [17, 16]
+    assert (batch.rows, batch.max_new, batch.min_new, batch.max_len) == (33, 17, 16, 17)
+    assert batch.page_table.tolist() == [c.page_ids(a), c.page_ids(b) + [-1]]
+    batch = c.batch([(b, 1), (a, 1)])  # b needs its second page, a has room
+    assert c.free_pages == 6 and batch.page_table.tolist() == [c.page_ids(b), c.page_ids(a)]
+    assert len(set(c.page_ids(a) + c.page_ids(b))) == 4
+    assert batch.lens.tolist() == [17, 18] and batch.q_start.tolist() == [0, 1, 2]
+    assert c.k[0].shape == (10, 2, 16, 128) and len(c.v) == 2
+
+
+def test_pages_come_back():
+    c = _cache(pages=4)
+    a, b = c.add(), c.add()
+    c.batch([(a, 40), (b, 5)])
+    assert c.free_pages == 0
+    held = c.page_ids(a)
+    c.truncate(a, 33)
+    assert c.free_pages == 0 and c.length(a) == 33
+    c.truncate(a, 32)
+    assert c.free_pages == 1 and c.page_ids(a) == held[:2]
+    c.free(a)
+    assert c.free_pages == 3
+    with pytest.raises(ValueError, match="no request"):
+        c.length(a)
+    c.batch([(b, 40)])
+    assert c.length(b) == 45 and c.free_pages == 1
+
+
+def test_a_step_that_does_not_fit_changes_nothing():
+    c = _cache(pages=3)
+    a, b = c.add(), c.add()
+    c.batch([(a, 16)])
+    with pytest.raises(RuntimeError, match="needs 3 pages, 2 are free"):
+        c.batch([(a, 1), (b, 17)])
+    assert (c.length(a), c.length(b), c.free_pages) == (16, 0, 2)
+    with pytest.raises(ValueError, match="once"):
+        c.batch([(a, 1), (a, 1)])
+    with pytest.raises(ValueError, match="negative"):
+        c.batch([(a, -1)])
+    with pytest.raises(ValueError, match="no request"):
+        c.batch([(99, 1)])
+    with pytest.raises(ValueError):
+        c.truncate(a, 17)
+    assert (c.length(a), c.free_pages) == (16, 2)
+
+
+def test_empty_steps():
+    c = _cache()
+    a = c.add()
+    batch = c.batch([])
+    assert batch.requests == 0 and batch.rows == 0 and batch.max_new == 0
+    batch = c.batch([(a, 0)])
+    assert batch.requests == 1 and batch.rows == 0 and batch.page_table.shape == (1, 0)
+
+
+@pytest.mark.parametrize("kw", [dict(page_size=8), dict(page_size=24), dict(page_size=0),
+                                dict(dtype=torch.float32)])
+def test_cache_refusals(kw):
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 4, 2, device="cpu", **kw)
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 0, 2, device="cpu")
+
+
+def _batch(B=2, cols=3, **kw):
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    args = dict(rows=4, max_new=2, max_len=20) | kw
+    return PagedBatch(torch.zeros(B, cols, dtype=torch.int32), i32(0, 2, 4), i32(20, 7), **args)
+
+
+def test_batch_refusals():
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    table, start, lens = torch.zeros(2, 3, dtype=torch.int32), i32(0, 2, 4), i32(20, 7)
+    ok = dict(rows=4, max_new=2, max_len=20)
+    PagedBatch(table, start, lens, **ok)
+    for args, kw in (((table, start[:2], lens), ok), ((table[:1], start, lens), ok),
+                     ((table.long(), start, lens), ok), ((table, start.float(), lens), ok),
+                     ((table.t().contiguous().t(), start, lens), ok),
+                     ((table, torch.zeros(6, dtype=torch.int32)[::2], lens), ok),
+                     ((table, start, lens), ok | dict(max_new=5)),
+                     ((table, start, lens), ok | dict(min_new=3)),
+                     ((table, start, lens), ok | dict(max_len=-1))):
+        with pytest.raises(ValueError):
+            PagedBatch(*args, **kw)
+
+
+def _pages(pages=4, heads=2, size=16, dtype=BF):
+    return torch.zeros(pages, heads, size, 128, dtype=dtype)
+
+
+def test_append_refusals():
+    b, k = _batch(), _pages()
+    qkv = torch.zeros(4, (4 + 4) * 128, dtype=BF)
+    call = lambda **kw: paged_append(**(dict(qkv=qkv, k_pages=k, v_pages=k.clone(), batch=b,  # noqa: E731
+                                             heads=4, theta=1e4) | kw))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        call()
+    for kw in (dict(theta=None), dict(inv_freq=[1.0] * 64), dict(theta=0.0), dict(theta=-2.0),
+               dict(theta=float("inf")), dict(theta=None, inv_freq=[1.0] * 63),
+               dict(theta=None, inv_freq=[float("nan")] * 64),
+               dict(heads=8), dict(heads=0), dict(qkv=qkv[:3]), dict(qkv=qkv.half()),
+               dict(qkv=qkv.t().contiguous().t()), dict(v_pages=_pages(heads=1)),
+               dict(k_pages=_pages(dtype=torch.float16)),
+               dict(k_pages=k.transpose(1, 2).contiguous().transpose(1, 2)),
+               dict(q_norm=torch.ones(64, dtype=BF)), dict(k_norm=torch.ones(128)),
+               dict(eps=-1.0), dict(batch=_batch(max_len=49))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    with pytest.raises(NotImplementedError):
+        call(k_pages=_pages(size=24), v_pages=_pages(size=24))
+
+
+def test_attention_refusals():
+    b, k = _batch(), _pages()
+    q = torch.zeros(4, 4, 128, dtype=BF)
+    call = lambda **kw: paged_attention(**(dict(q=q, k_pages=k, v_pages=k.clone(), batch=b) | kw))  # noqa: E731
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        call()
+    for kw in (dict(q=q[:, :3]), dict(q=q[:, :0]), dict(q=q[:3]), dict(q=q.half()),
+               dict(q=q[..., :64]), dict(out_dtype=torch.float16), dict(q=q[0]),
+               dict(batch=_batch(max_len=49)), dict(v_pages=_pages(pages=5))):
+        with pytest.raises(ValueError):
+            call(**kw)
+
+
+def test_c_entry_refusals():
+    """Bad arguments are refused before any launch; empty work is a no-op."""
+    lib = _lib.load()
+    E, U, OK = _lib.DKV_E_ARG, _lib.DKV_E_UNSUPPORTED, _lib.DKV_OK
+
+    def append(dtype=_lib.DKV_BF16, ps=16, cols=2, ld=2, B=1, T=1, hq=4, hkv=2, dh=128, stride=4096):
+        return lib.dkv_paged_append(None, dtype, None, 1024, None, 512, 128, None, None, stride,
+                                    2048, 4, ps, None, ld, cols, None, None, B, T, hq, hkv, dh,
+                                    None, None, 1e-6, None)
+
+    assert append() == E and append(dtype=0) == U and append(dh=64) == U and append(hq=3) == U
+    assert append(B=-1) == E and append(hkv=0) == E and append(ld=1) == E
+    assert append(ps=24, cols=0) == U and append(ps=8, cols=0) == U
+    assert append(B=0, cols=0) == OK and append(T=0, cols=0) == OK
+    assert append(stride=4, cols=0) == U
+
+    def attend(dtype=_lib.DKV_BF16, scale=0.1, B=1, T=1, hq=4, hkv=2, new=1, odt=_lib.DKV_BF16):
+        return lib.dkv_paged_attention(None, dtype, None, 512, 128, None, None, 4096, 2048, 4, 16,
+                                       None, 0, 0, None, None, B, T, hq, hkv, 128, new, 1, 16,
+                                       scale, None, 0, None, odt, 512, 128)
+
+    assert attend() == E and attend(dtype=0) == U and attend(hq=34) == U and attend(hq=5) == U
+    assert attend(odt=_lib.DKV_F16) == E and attend(B=-1) == E
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert attend(scale=scale) == U
+    assert attend(B=0) == OK and attend(T=0) == OK and attend(new=0) == OK
+
+
+def test_sampling_refusals():
+    x, u = torch.zeros(3, 8), torch.zeros(3)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        sample_tokens(x, u)
+    for args, kw in (((x[0], u), {}), ((x, u[:2]), {}), ((x, u.double()), {}),
+                     ((x[:, :0], u), {}), ((x.t().contiguous().t(), u), {}),
+                     ((x, u), dict(temperature=torch.ones(2))),
+                     ((x, u), dict(top_k=torch.ones(3))),
+                     ((x, u), dict(top_p=torch.ones(3, dtype=torch.float64))),
+                     ((x, u), dict(min_p=torch.ones(6)[::2]))):
+        with pytest.raises(ValueError):
+            sample_tokens(*args, **kw)
+    with pytest.raises(NotImplementedError):
+        sample_tokens(torch.zeros(1, (1 << 19) + 1), u[:1])
+    lib = _lib.load()
+    call = lambda dt, rows, v, ld=8: lib.dkv_sample_tokens(  # noqa: E731
+        None, dt, None, ld, rows, v, None, None, 1.0, None, 0, None, 1.0, None, 0.0, None)
+    assert call(0, 1, 8) == _lib.DKV_E_ARG and call(0, -1, 8) == _lib.DKV_E_ARG
+    assert call(9, 1, 8) == _lib.DKV_E_UNSUPPORTED and call(0, 1, 1 << 20) == _lib.DKV_E_UNSUPPORTED
+    assert call(0, 0, 8) == _lib.DKV_OK and call(0, 1, 0) == _lib.DKV_E_ARG
