@@ -109,7 +109,7 @@ _SIGNATURES = {
     "dkv_rope_apply": (_i, [_vp, _i, _vp, _ll, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _i]),
     "dkv_paged_append": (_i, [_vp, _i, _vp, _ll, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp,
                               _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _f, _vp]),
-    "dkv_paged_workspace_floats": (_ll, [_i, _i, _i, _i, _i, _i]),
+    "dkv_paged_workspace_floats": (_ll, [_i, _i, _i, _i, _i, _i, _i]),
     "dkv_paged_attention": (_i, [_vp, _i, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp, _ll, _i,
                                  _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _ll, _vp, _i,
                                  _ll, _ll]),

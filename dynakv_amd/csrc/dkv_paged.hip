@@ -43,6 +43,18 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedPool& pool, con
   return r;
 }
 
+// The same, for a request that is the whole wave's: in scalar registers.
+__device__ __forceinline__ PagedRequest paged_request_uniform(const PagedPool& pool,
+                                                              const int* q_start, const int* lens,
+                                                              int b, int T) {
+  PagedRequest r = paged_request(pool, q_start, lens, b, T);
+  r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
+  r.n = __builtin_amdgcn_readfirstlane(r.n);
+  r.len = __builtin_amdgcn_readfirstlane(r.len);
+  r.pos0 = __builtin_amdgcn_readfirstlane(r.pos0);
+  return r;
+}
+
 // The page of token t of request b, or -1 where there is none.
 __device__ __forceinline__ int paged_page(const PagedPool& pool, int b, int t) {
   const int c = t >> pool.page_shift;
@@ -194,9 +206,8 @@ __global__ __launch_bounds__(64 * AP_WAVES) void paged_append_kernel(AppendParam
 
 // ---------------------------------------------------------------------------------------
 // Attention of the new tokens over their request's pages: the token at position t attends keys
-// 0 .. t; o = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m), s_k = scale q . k. One wave per row and
-// query head: lane l scores key l of a tile of 64, the maximum and the sum run over the tiles, and
-// lane l sums dims 2l, 2l + 1 of the values.
+// 0 .. t; o = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m), s_k = scale q . k, one pass over the
+// keys with a running maximum and sum.
 // ---------------------------------------------------------------------------------------
 struct AttendParams {
   const uint16_t* q;
@@ -208,68 +219,847 @@ struct AttendParams {
   const int* lens;
   void* out;
   long long o_st, o_sh;
-  int B, T, Hq, Hkv;
-  float scale;
+  int B, T, Hq, Hkv, hpg;
+  float scale_log2;  // softmax scale * log2(e)
+  float* records;    // split records
+  int* counters;     // arrival counters, zero between calls
+  int split;         // whether a request's keys may be split among workgroups
 };
 
+// 16 bytes at byte offset `off` of a buffer resource into LDS at M0 + 16 * lane (inline assembly so
+// that the compiler neither moves LDS accesses across it nor waits for it before later LDS reads;
+// the kernels wait for these loads themselves).
+__device__ __forceinline__ void pg_lds_load16(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_base,
+                                              uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               ::"s"(lds_base), "v"(off), "s"(rsrc)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void pg_wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+typedef __attribute__((address_space(3))) dkv_i16x4 pg_lds_i16x4;
+__device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
+  return __builtin_bit_cast(
+      dkv_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                     (pg_lds_i16x4*)(__attribute__((address_space(3))) uint8_t*)p));
+}
+
+// ---- few rows: single tokens, a few drafted ones ----
+//
+// A request whose new tokens times query heads per KV head fill at most 16 rows. Bound by the keys
+// and values it reads once. A unit is (request, KV head); its keys go to the waves of one
+// workgroup, or of several (parts), in tiles of 16, which lie in one page each. A wave's tile of K
+// and V (4 KB each) lands in its own part of LDS by direct-to-LDS loads, 16-byte pieces XOR-swizzled
+// by token, the next tile's loads in flight meanwhile; the resource of a load ends with the request's
+// tokens, so slots behind them read as zero and cost nothing. S^T = K Q^T and P V on 16x16x32 MFMA
+// with the rows in the operand's columns; the weights go to the products as bf16 hi + lo pairs
+// (fp16: as fp16), 16 tokens filling 32 deep products. Waves are joined in LDS, parts by the
+// unit's last one to arrive.
+//
+// How a step's units are cut: requests have any lengths, which only the device knows, and the launch
+// has a fixed number of workgroups. Every wave finds the smallest part C (tiles) for which
+// sum over units of ceil(tiles / C) parts fit the launch, and takes its own from the running sums.
+constexpr int DW = 4;                       // waves per workgroup
+constexpr int DSLOT = 2;                    // tile slots per wave
+constexpr int DTILE = 16;
+constexpr int DTILE_BYTES = DTILE * PG_DH * 2;
+constexpr int DSLOT_BYTES = 2 * DTILE_BYTES;
+constexpr int DROWS = 16;
+constexpr int DREC = DROWS * (PG_DH + 2);   // floats of a record: m, l and acc[128] of 16 rows
+constexpr int D_COUNTERS = 16384;           // leading workspace ints
+constexpr int D_SPLIT_B = 256;              // requests a wave can hold the lengths of (4 a lane)
+constexpr int D_WGS = 512;                  // two workgroups per CU
+constexpr int D_MIN_TILES = 2 * DW;         // least part
+constexpr float D_RESCALE = 11.5f;          // log2 units the running maximum may be exceeded by
+
+__device__ __forceinline__ int pg_wave_sum(int v) { return dkv_wave_sum_fast_i(v); }
+
 template <int DT, int ODT>
-__global__ __launch_bounds__(64) void paged_attend_kernel(AttendParams p) {
-  __shared__ float sq[PG_DH];
-  __shared__ float sp[64];
-  __shared__ long long sv[64];
-  const int lane = threadIdx.x;
-  const int row = blockIdx.x, h = blockIdx.y, g = h / (p.Hq / p.Hkv);
-  const int b = request_of_row(p.q_start, p.B, row, lane);
-  if (b < 0) return;
-  const PagedRequest r = paged_request(p.pool, p.q_start, p.lens, b, p.T);
-  const int pos = r.pos0 + row - r.row0;
-  const uint16_t* qr = p.q + (long long)row * p.q_st + (long long)h * p.q_sh;
-  sq[2 * lane] = dkv_load_f32<DT>(qr, 2 * lane) * p.scale;
-  sq[2 * lane + 1] = dkv_load_f32<DT>(qr, 2 * lane + 1) * p.scale;
-  __syncthreads();
-  const int end = min(pos + 1, r.len);
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int k0 = 0; k0 < end; k0 += 64) {
-    const int key = k0 + lane;
-    const int page = key < end ? paged_page(p.pool, b, key) : -1;
-    const long long at = page < 0 ? -1
-                                  : (long long)page * p.pool.page_stride +
-                                        (long long)g * p.pool.head_stride +
-                                        (long long)(key & (p.pool.page_size - 1)) * PG_DH;
-    float s = -INFINITY;
-    if (at >= 0) {
-      s = 0.f;
-      for (int d = 0; d < PG_DH; d += 8) {
-        float kv[8];
-        load8<DT>(p.k + at + d, kv);
+__global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t sRing[DW * DSLOT * DSLOT_BYTES];
+  __shared__ int sLast;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+
+  // tiles of a request's keys; 0 for one without rows or with too many
+  auto tiles_of = [&](int b) {
+    if (b >= p.B) return 0;
+    const PagedRequest r = paged_request(p.pool, p.q_start, p.lens, b, p.T);
+    if (r.n <= 0 || r.n * p.hpg > DROWS) return 0;
+    return max(1, (r.len + DTILE - 1) / DTILE);
+  };
+  int b, kvh, part = 0, parts = 1, first = 0;
+  if (p.split) {
+    int t[D_SPLIT_B / 64], total = 0, units = 0;
+    const int used = (p.B + 63) / 64;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(sq[d + e], kv[e], s);
+    for (int j = 0; j < D_SPLIT_B / 64; ++j) {
+      t[j] = j < used ? tiles_of(64 * j + lane) : 0;
+      total += t[j];
+      units += t[j] > 0;
+    }
+    total = pg_wave_sum(total) * p.Hkv;
+    units = pg_wave_sum(units) * p.Hkv;
+    const int G = gridDim.x;  // at least the units
+    // parts of size c; the same in every wave of the launch, whatever the rounding
+    auto parts_of = [&](int tiles, float inv) {
+      return tiles > 0 ? max(1, (int)((float)tiles * inv + 0.999f)) : 0;
+    };
+    // the least c lies between total / G (no rounding up) and total / (G - units) (each unit
+    // rounded up by a whole part)
+    float lo = max((float)total / (float)G, (float)D_MIN_TILES);
+    float hi = G > units ? max((float)total / (float)(G - units), lo) : 1e9f;
+    for (int it = 0; it < 6; ++it) {
+      const float c = it == 0 ? lo : 0.5f * (lo + hi), inv = 1.0f / c;
+      int sum = 0;
+#pragma unroll
+      for (int j = 0; j < D_SPLIT_B / 64; ++j)
+        if (j < used) sum += parts_of(t[j], inv);
+      if (pg_wave_sum(sum) * p.Hkv <= G) {
+        hi = c;
+        if (it == 0) break;
+      } else {
+        lo = c;
       }
     }
+    float inv = 1.0f / hi;
+    {  // hi may still be the untested bound
+      int sum = 0;
+#pragma unroll
+      for (int j = 0; j < D_SPLIT_B / 64; ++j)
+        if (j < used) sum += parts_of(t[j], inv);
+      if (pg_wave_sum(sum) * p.Hkv > G) inv = 0.f;  // one part each
+    }
+    // this workgroup's place in the running sums
+    int base = 0;
+    b = -1;
+#pragma unroll
+    for (int j = 0; j < D_SPLIT_B / 64; ++j) {
+      if (j >= used || b >= 0) continue;
+      const int s = parts_of(t[j], inv) * p.Hkv;
+      int run = s;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(run, o, 64);
+        if (lane >= o) run += x;
+      }
+      const unsigned long long hit = __ballot((int)blockIdx.x < base + run);
+      if (hit) {
+        const int l = __ffsll((long long)hit) - 1;
+        b = 64 * j + l;
+        first = base + __shfl(run - s, l, 64);
+        parts = __shfl(s, l, 64) / p.Hkv;
+      } else {
+        base += __shfl(run, 63, 64);
+      }
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    if (b < 0) return;
+    first = __builtin_amdgcn_readfirstlane(first);
+    parts = __builtin_amdgcn_readfirstlane(parts);
+    const int rel = (int)blockIdx.x - first;
+    kvh = rel / parts;
+    part = rel % parts;
+    first += kvh * parts;
+  } else {
+    b = blockIdx.x / p.Hkv;
+    kvh = blockIdx.x % p.Hkv;
+  }
+  const int n_all = __builtin_amdgcn_readfirstlane(tiles_of(b));
+  if (n_all == 0) return;
+  const PagedRequest r = paged_request_uniform(p.pool, p.q_start, p.lens, b, p.T);
+  const int rows = r.n * p.hpg;
+  const int per = (n_all + parts - 1) / parts;
+  const int t_begin = part * per, t_end = min(n_all, t_begin + per);
+  const int n_iter = max(0, (t_end - t_begin - wave + DW - 1) / DW);
+  auto tix = [&](int j) { return t_begin + wave + DW * j; };
+
+  uint8_t* ring = sRing + wave * DSLOT * DSLOT_BYTES;
+  uint32_t piece_off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 4 * i + (lane >> 4);
+    piece_off[i] = (uint32_t)(t * 256 + 16 * ((lane & 15) ^ t));
+  }
+  int ids = -1;  // lane l: the page of the wave's tile l of the current 64
+  auto fetch_ids = [&](int j) {
+    const int t = tix(j + lane);
+    ids = t < t_end ? paged_page(p.pool, b, t * DTILE) : -1;
+  };
+  auto page_at = [&](int j) { return __builtin_amdgcn_readlane(ids, j & 63); };
+  auto issue = [&](int j) {
+    if (j >= n_iter) return;
+    if ((j & 63) == 0) fetch_ids(j);
+    const int page = page_at(j), tok = tix(j) * DTILE;
+    const long long at = (long long)max(page, 0) * p.pool.page_stride +
+                         (long long)kvh * p.pool.head_stride +
+                         (long long)(tok & (p.pool.page_size - 1)) * PG_DH;
+    const uint32_t bytes = page < 0 ? 0u : (uint32_t)min(r.len - tok, DTILE) * (PG_DH * 2);
+    const __amdgpu_buffer_rsrc_t rk = dkv_make_rsrc(p.k + at, bytes);
+    const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc(p.v + at, bytes);
+    const uint32_t slot = dkv_lds_addr(ring + (j % DSLOT) * DSLOT_BYTES);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pg_lds_load16(rk, slot + 1024 * i, piece_off[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pg_lds_load16(rv, slot + DTILE_BYTES + 1024 * i, piece_off[i]);
+  };
+  int ids_now = -1;  // the ids that the tile being worked on belongs to
+  issue(0);
+  ids_now = ids;
+
+  // query operand: column n = row n (new token n / hpg, head n % hpg; rows past the request's
+  // zero), dims 32c + 8g .. +8
+  dkv_u32x4 bq[4];
+  const bool has = n < rows;
+  const int qi = has ? n / p.hpg : 0;  // the row's new token
+  const uint16_t* qr = p.q + (long long)(r.row0 + qi) * p.q_st +
+                       (long long)(kvh * p.hpg + (has ? n % p.hpg : 0)) * p.q_sh;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const dkv_u32x4 v = *(const dkv_u32x4*)(qr + 32 * c + 8 * g);
+    bq[c] = has ? v : dkv_u32x4{0u, 0u, 0u, 0u};
+  }
+  // settled here (with tile 0), not inside the loop, where the wait would drain the next tile too
+#pragma unroll
+  for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(bq[c]));
+  const int limit = min(r.pos0 + qi, r.len - 1);  // the row's last key
+
+  dkv_f32x4 acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -1.0e30f, l_run = 0.f;  // log2 units; a finite floor: exp2(-inf - floor) is 0
+
+  for (int j = 0; j < n_iter; ++j) {
+    pg_wait_vm<0>();  // tile j
+    if ((j & 63) == 0) ids_now = ids;
+    const int page = __builtin_amdgcn_readlane(ids_now, j & 63);
+    issue(j + 1);
+    const uint8_t* slot = ring + (j % DSLOT) * DSLOT_BYTES;
+    const int key0 = tix(j) * DTILE;
+    dkv_u32x4 xk[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      xk[c] = *(const dkv_u32x4*)(slot + n * 256 + 16 * ((4 * c + g) ^ n));
+    dkv_f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sc = dkv_mfma32<DT>(xk[c], bq[c], sc);
+    // lane (row n, keys 4g + u): scores in log2 units
+    const int last = page < 0 ? -1 : limit - key0 - 4 * g;
+    float z[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) z[u] = u <= last ? sc[u] * p.scale_log2 : -INFINITY;
+    float tmax = dkv_max3(dkv_max3(z[0], z[1], z[2]), z[3], z[3]);
+    tmax = dkv_lane_max32(tmax);
+    tmax = dkv_lane_max16(tmax);
+    if (__ballot(tmax > m_run + D_RESCALE)) {
+      const float m_new = fmaxf(m_run, tmax);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+      m_run = m_new;
+      float au[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) au[u] = __shfl(alpha, 4 * g + u, 64);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[i][u] *= au[u];
+    }
+    float pu[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      pu[u] = __builtin_amdgcn_exp2f(z[u] - m_run);
+      l_run += pu[u];
+    }
+    // P.V: A = P (row n; its 16 tokens twice, as hi and lo parts: k = 8g + e is part e / 4 of token
+    // 4g + e % 4), B = V (the token's value, column = dim 16 blk + n) read transposed: lane (n, g)
+    // reads 8 bytes of token 4g + n / 4 and receives tokens 4g .. 4g + 3 of dim 16 blk + n
+    dkv_u32x4 pa;
+    if constexpr (DT == DKV_BF16) {
+      uint32_t h01, h23, l01, l23;
+      dkv_split_bf16x2(pu[0], pu[1], h01, l01);
+      dkv_split_bf16x2(pu[2], pu[3], h23, l23);
+      pa = dkv_u32x4{h01, h23, l01, l23};
+    } else {
+      pa = dkv_u32x4{dkv_pack_f16x2(pu[0], pu[1]), dkv_pack_f16x2(pu[2], pu[3]), 0u, 0u};
+    }
+    const int vtok = 4 * g + (n >> 2);
+    dkv_u32x2 xv[8];
+#pragma unroll
+    for (int blk = 0; blk < 8; ++blk) {
+      const int piece = 2 * blk + ((n & 3) >> 1);
+      xv[blk] = pg_read_tr(slot + DTILE_BYTES + vtok * 256 + 16 * (piece ^ vtok) + 8 * (n & 1));
+    }
+    if (key0 + DTILE - 1 <= r.pos0 || r.n == 1) {
+#pragma unroll
+      for (int blk = 0; blk < 8; ++blk)
+        acc[blk] = dkv_mfma32<DT>(pa, dkv_u32x4{xv[blk].x, xv[blk].y, xv[blk].x, xv[blk].y},
+                                  acc[blk]);
+    } else {
+      // Keys that some of the rows attend and others do not (they come after them): a product per
+      // new token with the later keys' values cleared, of which its own rows are taken, so that an
+      // infinity or NaN there, whose weight is 0, stays out of the rows before it.
+      for (int i = 0; i < r.n; ++i) {
+        const int cut = r.pos0 + i - key0 - 4 * g;  // the token's last key, from this lane's first
+        const uint32_t m0 = (cut >= 0 ? 0xffffu : 0u) | (cut >= 1 ? 0xffff0000u : 0u);
+        const uint32_t m1 = (cut >= 2 ? 0xffffu : 0u) | (cut >= 3 ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int blk = 0; blk < 8; ++blk) {
+          const uint32_t v0 = xv[blk].x & m0, v1 = xv[blk].y & m1;
+          const dkv_f32x4 o = dkv_mfma32<DT>(pa, dkv_u32x4{v0, v1, v0, v1},
+                                             dkv_f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int x = 4 * g + u - i * p.hpg;
+            if (x >= 0 && x < p.hpg) acc[blk][u] += o[u];
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  pg_wait_vm<0>();  // nothing lands in the ring once it is reused below
+
+  // ---- join the waves through LDS ----
+  float l_tot = l_run;
+  l_tot += __shfl_xor(l_tot, 16, 64);
+  l_tot += __shfl_xor(l_tot, 32, 64);
+  __syncthreads();
+  float* sw = reinterpret_cast<float*>(sRing);  // per wave: 16 m, 16 l, 16 x 128 acc
+  constexpr int WREC = 2 * DROWS + DROWS * PG_DH;
+  static_assert(DW * WREC * 4 <= DW * DSLOT * DSLOT_BYTES, "the epilogue's floats fit the ring");
+  float* my = sw + wave * WREC;
+  if (g == 0) {
+    my[n] = m_run;
+    my[DROWS + n] = l_tot;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) my[2 * DROWS + (4 * g + u) * PG_DH + 16 * i + n] = acc[i][u];
+  __syncthreads();
+  auto joined = [&](int row, int d, float& M, float& L) {  // sum of dim d, with the row's M and L
+    float mw[DW], A = 0.f;
+    M = -INFINITY;
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < DW; ++w) {
+      mw[w] = sw[w * WREC + row];
+      M = fmaxf(M, mw[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < DW; ++w) {
+      const float wt = exp2f(mw[w] - M);
+      L += wt * sw[w * WREC + DROWS + row];
+      A += wt * sw[w * WREC + 2 * DROWS + row * PG_DH + d];
+    }
+    return A;
+  };
+  auto store = [&](int row, int d, float A, float L) {
+    const long long oi = (long long)(r.row0 + row / p.hpg) * p.o_st +
+                         (long long)(kvh * p.hpg + row % p.hpg) * p.o_sh + d;
+    dkv_store_f32<ODT>(p.out, oi, L > 0.f ? A / L : 0.f);
+  };
+  if (parts == 1) {
+    for (int idx = tid; idx < rows * PG_DH; idx += 64 * DW) {
+      float M, L;
+      const float A = joined(idx / PG_DH, idx % PG_DH, M, L);
+      store(idx / PG_DH, idx % PG_DH, A, L);
+    }
+    return;
+  }
+  // this part's record: per row m, l, acc[128]
+  float* rec = p.records + (long long)blockIdx.x * DREC;
+  for (int idx = tid; idx < rows * PG_DH; idx += 64 * DW) {
+    const int row = idx / PG_DH, d = idx % PG_DH;
+    float M, L;
+    const float A = joined(row, d, M, L);
+    float* rr = rec + row * (PG_DH + 2);
+    __hip_atomic_store(rr + 2 + d, A, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (d == 0) {
+      __hip_atomic_store(rr, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(rr + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  // ---- the unit's last part to arrive joins the parts ----
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    const int old = __hip_atomic_fetch_add(p.counters + b * p.Hkv + kvh, 1, __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_AGENT);
+    sLast = old == parts - 1;
+  }
+  __syncthreads();
+  if (!sLast) return;
+  const float* recs = p.records + (long long)first * DREC;
+  auto ld = [&](const float* a) {
+    return __hip_atomic_load(a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  for (int idx = tid; idx < rows * PG_DH; idx += 64 * DW) {
+    const int row = idx / PG_DH, d = idx % PG_DH;
+    float M = -INFINITY, L = 0.f, A = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += 8) {
+      float mb[8], lb[8], xb[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* rr = recs + (long long)min(s0 + u, parts - 1) * DREC + row * (PG_DH + 2);
+        mb[u] = ld(rr);
+        lb[u] = ld(rr + 1);
+        xb[u] = ld(rr + 2 + d);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (s0 + u >= parts) break;
+        const float Mn = fmaxf(M, mb[u]);
+        const float so = exp2f(M - Mn), sn = exp2f(mb[u] - Mn);
+        L = L * so + lb[u] * sn;
+        A = A * so + xb[u] * sn;
+        M = Mn;
+      }
+    }
+    store(row, d, A, L);
+  }
+  if (tid == 0) p.counters[b * p.Hkv + kvh] = 0;
+}
+
+// ---- many rows: prompts and their chunks ----
+//
+// A request's new tokens and a KV head's query heads make rows (token R / hpg, head R % hpg), so the
+// heads that read the same keys share their tiles. One workgroup has BQ = 16 QB NW rows of one
+// request and KV head (NW waves of QB blocks of 16 rows) and all the keys they attend, or, where
+// there are few rows to fill the chip with, one of `splits` ranges of them (records joined by a
+// second launch). Key tiles of 64 are staged in LDS (double-buffered, direct-to-LDS loads, 16-byte
+// pieces XOR-swizzled by key so that neither the row reads of K nor the transposed reads of V meet
+// in a bank); a tile is four blocks of 16 keys, each within one page, and a wave loads one of them
+// (NW = 8: half of one) through a resource that ends with the request's keys. S^T = K Q^T on
+// 16x16x32 MFMA (a lane then holds one row's scores for 16 keys); softmax in fp32, the running
+// maximum raised only when a tile's exceeds it by more than 2^8; P V on 16x16x32 MFMA with the
+// weights rounded once to the cache's type.
+constexpr int CK = 64;                      // keys per tile
+constexpr int CTILE_BYTES = CK * PG_DH * 2;
+constexpr float C_RESCALE = 8.f;            // log2 units
+
+struct ChunkParams {
+  AttendParams a;
+  int bq, splits, few_rows;  // rows of a workgroup; key ranges; rows up to which the other kernel works
+};
+
+// The work item of a workgroup: row tile `rt` of request b. Items are counted request by request,
+// a request's later rows (with more keys) first.
+struct ChunkItem {
+  int b, rt, tiles;
+};
+__device__ __forceinline__ ChunkItem chunk_item(const ChunkParams& p, int item, int lane) {
+  const AttendParams& a = p.a;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int t = 0;
+    if (b0 + lane < a.B) {
+      const PagedRequest r = paged_request(a.pool, a.q_start, a.lens, b0 + lane, a.T);
+      const long long rows = (long long)r.n * a.hpg;
+      t = r.n > 0 && rows > p.few_rows ? (int)((rows + p.bq - 1) / p.bq) : 0;
+    }
+    int run = t;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(run, o, 64);
+      if (lane >= o) run += x;
+    }
+    const unsigned long long hit = __ballot(item < base + run);
+    if (hit) {
+      const int l = __ffsll((long long)hit) - 1;
+      ChunkItem it;
+      it.b = __builtin_amdgcn_readfirstlane(b0 + l);
+      it.tiles = __builtin_amdgcn_readfirstlane(__shfl(t, l, 64));
+      const int before = base + __shfl(run - t, l, 64);
+      it.rt = __builtin_amdgcn_readfirstlane(it.tiles - 1 - (item - before));
+      return it;
+    }
+    base += __shfl(run, 63, 64);
+  }
+  return ChunkItem{-1, 0, 0};
+}
+
+__device__ __forceinline__ float pg_max4(float x) {  // over lanes n, n + 16, n + 32, n + 48
+  return dkv_lane_max16(dkv_lane_max32(x));
+}
+
+// One row over keys k0 .. k1 - 1, by a wave, key by key: for rows whose values came out as infinity or
+// NaN. A product of matrices takes a masked key's value times 0, which is NaN for an infinite one; here
+// a masked key is not touched. Lane l returns dims 2l, 2l + 1.
+template <int DT>
+__device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, int kvh,
+                                              const uint16_t* qr, int k0, int k1, int lane,
+                                              float& m, float& l, float& o0, float& o1) {
+  m = -1.0e30f;
+  l = o0 = o1 = 0.f;
+  for (int t0 = k0; t0 < k1; t0 += 64) {
+    const int key = t0 + lane;
+    const int page = key < k1 ? paged_page(p.pool, b, key) : -1;
+    const long long at = (long long)max(page, 0) * p.pool.page_stride +
+                         (long long)kvh * p.pool.head_stride +
+                         (long long)(key & (p.pool.page_size - 1)) * PG_DH;
+    float s = -INFINITY;
+    if (page >= 0) {
+      s = 0.f;
+      for (int d = 0; d < PG_DH; d += 8) {
+        float kv[8], qv[8];
+        load8<DT>(p.k + at + d, kv);
+        load8<DT>(qr + d, qv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(qv[e], kv[e], s);
+      }
+      s *= p.scale_log2;
+    }
     const float mt = fmaxf(m, dkv_wave_max(s));
-    if (mt == -INFINITY) continue;
-    const float alpha = expf(m - mt);
-    const float pr = at >= 0 ? expf(s - mt) : 0.f;
-    l = l * alpha + dkv_wave_sum(pr);
+    const float alpha = exp2f(m - mt), w = page >= 0 ? exp2f(s - mt) : 0.f;
+    l = l * alpha + dkv_wave_sum(w);
     o0 *= alpha;
     o1 *= alpha;
     m = mt;
-    __syncthreads();
-    sp[lane] = pr;
-    sv[lane] = at;
-    __syncthreads();
-    const int cnt = min(64, end - k0);
-    for (int j = 0; j < cnt; ++j) {
-      if (sv[j] < 0) continue;
-      const float w = sp[j];
-      o0 = fmaf(w, dkv_load_f32<DT>(p.v + sv[j], 2 * lane), o0);
-      o1 = fmaf(w, dkv_load_f32<DT>(p.v + sv[j], 2 * lane + 1), o1);
+    for (int j = 0; j < 64 && t0 + j < k1; ++j) {
+      if (__builtin_amdgcn_readlane(page, j) < 0) continue;
+      const float wj = __shfl(w, j, 64);
+      const long long vj = __shfl(at, j, 64);
+      o0 = fmaf(wj, dkv_load_f32<DT>(p.v + vj, 2 * lane), o0);
+      o1 = fmaf(wj, dkv_load_f32<DT>(p.v + vj, 2 * lane + 1), o1);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const long long oi = (long long)row * p.o_st + (long long)h * p.o_sh + 2 * lane;
-  dkv_store_f32<ODT>(p.out, oi, o0 * inv);
-  dkv_store_f32<ODT>(p.out, oi + 1, o1 * inv);
+}
+
+template <int DT, int ODT, int QB, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(ChunkParams c) {
+  constexpr int QW = 16 * QB;            // rows per wave
+  constexpr int BQ = NW * QW;            // rows per workgroup
+  constexpr int LW = CK / 4 / NW;        // K (or V) loads per wave and tile, 4 keys each
+  __shared__ __attribute__((aligned(1024))) uint8_t sK[2][CTILE_BYTES];
+  __shared__ __attribute__((aligned(1024))) uint8_t sV[2][CTILE_BYTES];
+  const AttendParams& p = c.a;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  // the KV head runs fastest: workgroups go to the 8 XCDs in turn, so that a head's keys and values
+  // stay in one L2 (for 8 heads, or a multiple)
+  const int kvh = __builtin_amdgcn_readfirstlane(blockIdx.x % p.Hkv);
+  const int rest = blockIdx.x / p.Hkv;
+  const int split = rest % c.splits;
+  const ChunkItem it = chunk_item(c, rest / c.splits, lane);
+  const int b = __builtin_amdgcn_readfirstlane(it.b);
+  if (b < 0) return;
+  const PagedRequest r = paged_request_uniform(p.pool, p.q_start, p.lens, b, p.T);
+  const int rows = r.n * p.hpg;
+  const int q0 = __builtin_amdgcn_readfirstlane(it.rt) * BQ;
+  const int wq0 = q0 + QW * wave;  // the wave's first row
+
+  // this lane's rows (operand columns): token and last key
+  dkv_u32x4 qop[QB][4];
+  int limit[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int R = min(wq0 + 16 * qb + n, rows - 1);
+    const int i = R / p.hpg, h = R - i * p.hpg;
+    const uint16_t* qp = p.q + (long long)(r.row0 + i) * p.q_st +
+                         (long long)(kvh * p.hpg + h) * p.q_sh + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qop[qb][s] = *(const dkv_u32x4*)(qp + 32 * s);
+    limit[qb] = min(r.pos0 + i, r.len - 1);
+  }
+  // keys up to the last row's; the wave's first and last row's limits
+  const int k_end = __builtin_amdgcn_readfirstlane(
+      max(0, min(r.len, r.pos0 + (min(q0 + BQ, rows) - 1) / p.hpg + 1)));
+  const int w_first = r.pos0 + min(wq0, rows - 1) / p.hpg;
+  const int w_end = wq0 < rows ? r.pos0 + (min(wq0 + QW, rows) - 1) / p.hpg + 1 : 0;
+  const int all_tiles = (k_end + CK - 1) / CK;
+  const int per = (all_tiles + c.splits - 1) / c.splits;
+  const int t0 = min(all_tiles, split * per), n_tiles = min(all_tiles, t0 + per);
+
+  // pages of the 64 blocks of 16 keys from tile tb on (16 tiles); the next 64 fetched ahead
+  int ids = -1, ids_next = -1;
+  auto fetch_ids = [&](int tb) {
+    const int key = (tb * 4 + lane) * 16;
+    return key < k_end ? paged_page(p.pool, b, key) : -1;
+  };
+  int ids_base = t0;
+  ids = fetch_ids(t0);
+  if (t0 + 16 < n_tiles) ids_next = fetch_ids(t0 + 16);
+  // blocks with keys but no page
+  auto absent_of = [&](int tb) {
+    return __ballot(ids < 0 && (tb * 4 + lane) * 16 < k_end);
+  };
+  unsigned long long absent = absent_of(t0);
+
+  // tile loads: wave w, instruction i stores keys 64 / NW * w + 4 i + lane / 16 of the tile, LDS piece
+  // lane % 16, which holds the key's 16-byte piece (lane % 16) ^ (key % 16)
+  const int blk = wave * (CK / NW) / 16;              // the wave's block of the tile
+  const int sub = (wave * (CK / NW)) & 15;            // its first key in the block
+  uint32_t voff[LW];
+#pragma unroll
+  for (int i = 0; i < LW; ++i) {
+    const int kk = 4 * i + (lane >> 4);
+    voff[i] = (uint32_t)(kk * 256 + 16 * ((lane & 15) ^ ((sub + kk) & 15)));
+  }
+  auto issue = [&](int t, int page) {
+    const int key = t * CK + blk * 16 + sub;
+    const long long at = (long long)max(page, 0) * p.pool.page_stride +
+                         (long long)kvh * p.pool.head_stride +
+                         (long long)(key & (p.pool.page_size - 1)) * PG_DH;
+    const int cnt = __builtin_amdgcn_readfirstlane(
+        page < 0 ? 0 : min(max(k_end - key, 0), CK / NW));  // (a vector instruction clamps)
+    const __amdgpu_buffer_rsrc_t rk = dkv_make_rsrc(p.k + at, (uint32_t)cnt * (PG_DH * 2));
+    const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc(p.v + at, (uint32_t)cnt * (PG_DH * 2));
+    const uint32_t dk = dkv_lds_addr(sK[t & 1]) + CK / NW * wave * 256;
+    const uint32_t dv = dkv_lds_addr(sV[t & 1]) + CK / NW * wave * 256;
+#pragma unroll
+    for (int i = 0; i < LW; ++i) pg_lds_load16(rk, dk + 1024 * i, voff[i]);
+#pragma unroll
+    for (int i = 0; i < LW; ++i) pg_lds_load16(rv, dv + 1024 * i, voff[i]);
+  };
+
+  dkv_f32x4 acc[QB][8];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[qb][i] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run[QB], l_run[QB];  // log2 units
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    m_run[qb] = -1.0e30f;
+    l_run[qb] = 0.f;
+  }
+
+  // S^T of key block kb: A = K rows (lane: key 16kb + n, dims 32s + 8g .. +8), B = Q^T; lane (row n,
+  // g) then holds keys 16kb + 4g + u, unscaled
+  const uint32_t krd = n * 256 + 16 * (g ^ n);
+  typedef __attribute__((address_space(3))) dkv_u32x4 lds_u32x4;
+  // transposed V reads: lane 4i + q of each 16 reads key 16kb + 4g + i, dims 16db + 4q .. +3; lane i
+  // then holds dim 16db + i of keys 4g .. 4g + 3
+  const uint32_t vrd =
+      (4 * g + (n >> 2)) * 256 + 16 * (((n & 3) >> 1) ^ (4 * g + (n >> 2))) + 8 * (n & 1);
+
+  if (t0 < n_tiles) issue(t0, __builtin_amdgcn_readlane(ids, blk));
+  for (int t = t0; t < n_tiles; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // tile t is in LDS for every wave; tile t - 1's buffer is free
+    const uint32_t gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
+    if (t + 1 < n_tiles) {
+      if (t + 1 == ids_base + 16) {
+        ids_base += 16;
+        ids = ids_next;
+        absent = absent_of(ids_base);
+        if (ids_base + 16 < n_tiles) ids_next = fetch_ids(ids_base + 16);
+      }
+      issue(t + 1, __builtin_amdgcn_readlane(ids, 4 * (t + 1 - ids_base) + blk));
+    }
+    const int key0 = t * CK;
+    if (key0 >= w_end) continue;  // every key of the tile is past the wave's rows
+    const uint32_t kt = dkv_lds_addr(sK[t & 1]);
+    const uint32_t vt = dkv_lds_addr(sV[t & 1]) + vrd;
+    dkv_f32x4 z[QB][4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const dkv_u32x4 a = *(const lds_u32x4*)(((kt + krd) ^ (64 * s)) + 4096 * kb);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_mfma32<DT>(a, qop[qb][s], z[qb][kb]);
+      }
+    }
+    if (key0 + CK - 1 > w_first || key0 + CK > r.len || gone) {
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          const int last = (gone >> kb) & 1u ? -1 : limit[qb] - key0 - 16 * kb - 4 * g;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (u > last) z[qb][kb][u] = -INFINITY;
+        }
+    }
+    // V operands of key blocks 0 and 1: read ahead of the softmax
+    dkv_u32x2 vx[8][2];
+    auto vread = [&](int j, int db) {
+      const uint32_t src = (vt ^ (32 * db)) + 8192 * j;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+        vx[db][kk] = __builtin_bit_cast(
+            dkv_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds_i16x4*)(src + 4096 * kk)));
+    };
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int db = 0; db < 8; ++db) vread(0, db);
+    __builtin_amdgcn_sched_barrier(0);
+    float tmax[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      float m[4];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+        m[kb] = dkv_max3(dkv_max3(z[qb][kb][0], z[qb][kb][1], z[qb][kb][2]), z[qb][kb][3],
+                         z[qb][kb][3]);
+      tmax[qb] = pg_max4(dkv_max3(dkv_max3(m[0], m[1], m[2]), m[3], m[3])) * p.scale_log2;
+    }
+    if (__ballot(tmax[0] > m_run[0] + C_RESCALE || tmax[QB - 1] > m_run[QB - 1] + C_RESCALE)) {
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        const float m_new = dkv_max2(m_run[qb], tmax[qb]);
+        const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+        m_run[qb] = m_new;
+        l_run[qb] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) acc[qb][i][u] *= alpha;
+      }
+    }
+    // P of key blocks 2j and 2j + 1: the products' k = 8g .. 8g + 3 are key block 2j's keys 4g .. 4g
+    // + 3, k = 8g + 4 .. 8g + 7 key block 2j + 1's
+    dkv_u32x4 bp[2][QB];
+    auto probs = [&](int j, int kk, int qb) {
+      float pu[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        pu[u] = __builtin_amdgcn_exp2f(
+            __builtin_fmaf(z[qb][2 * j + kk][u], p.scale_log2, -m_run[qb]));
+        l_run[qb] += pu[u];
+      }
+      typedef __attribute__((ext_vector_type(2))) float f32x2;
+      if constexpr (DT == DKV_BF16) {
+        bp[j][qb][2 * kk] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector(f32x2{pu[0], pu[1]}, dkv_bf16x2));
+        bp[j][qb][2 * kk + 1] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector(f32x2{pu[2], pu[3]}, dkv_bf16x2));
+      } else {
+        bp[j][qb][2 * kk] = dkv_pack_f16x2(pu[0], pu[1]);
+        bp[j][qb][2 * kk + 1] = dkv_pack_f16x2(pu[2], pu[3]);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < 2 * QB; ++i) probs(0, i & 1, i >> 1);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        __builtin_amdgcn_sched_barrier(0);
+        const dkv_u32x4 aop = {vx[db][0].x, vx[db][0].y, vx[db][1].x, vx[db][1].y};
+        if (j == 0) vread(1, db);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) acc[qb][db] = dkv_mfma32<DT>(aop, bp[j][qb], acc[qb][db]);
+        if (j == 0 && db % (4 / QB) == 4 / QB - 1)
+          probs(1, db / (4 / QB) % 2, db / (8 / QB));
+      }
+    }
+  }
+
+  // acc rows are dims, columns rows of the request: lane (row n, g) holds dims 16db + 4g + u
+  float* rec0 = p.records + ((long long)(rest / c.splits * p.Hkv + kvh) * c.splits + split) * BQ *
+                                (PG_DH + 2);
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    float l = l_run[qb];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const int R = wq0 + 16 * qb + n;
+    const int i = R / p.hpg, h = R - i * p.hpg;
+    // the largest magnitude, infinite or NaN where a value is (a sum of products by 0)
+    float odd = l * 0.f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) odd = fmaf(acc[qb][db][u], 0.f, odd);
+    unsigned long long bad = __ballot(R < rows && !(odd == 0.f));
+    bad = (bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xffffull;  // by row
+    const bool good = R < rows && !((bad >> n) & 1);
+    if (c.splits == 1) {
+      if (good) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const long long ob = (long long)(r.row0 + i) * p.o_st +
+                             (long long)(kvh * p.hpg + h) * p.o_sh;
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            dkv_store_f32<ODT>(p.out, ob + 16 * db + 4 * g + u, acc[qb][db][u] * inv);
+      }
+    } else if (good) {
+      float* rec = rec0 + (long long)(QW * wave + 16 * qb + n) * (PG_DH + 2);
+      if (g == 0) {
+        rec[0] = m_run[qb];
+        rec[1] = l;
+      }
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) rec[2 + 16 * db + 4 * g + u] = acc[qb][db][u];
+    }
+    while (bad) {  // rows with an infinity or NaN, key by key
+      const int x = __ffsll((long long)bad) - 1;
+      bad &= bad - 1;
+      const int Rx = wq0 + 16 * qb + x, ix = Rx / p.hpg, hx = Rx - ix * p.hpg;
+      const uint16_t* qx = p.q + (long long)(r.row0 + ix) * p.q_st +
+                           (long long)(kvh * p.hpg + hx) * p.q_sh;
+      float mx, lx, o0, o1;
+      attend_row_apart<DT>(p, b, kvh, qx, t0 * CK, min(n_tiles * CK, min(r.pos0 + ix + 1, r.len)),
+                           lane, mx, lx, o0, o1);
+      if (c.splits == 1) {
+        const float inv = lx > 0.f ? 1.f / lx : (lx == 0.f ? 0.f : lx);
+        const long long ob = (long long)(r.row0 + ix) * p.o_st +
+                             (long long)(kvh * p.hpg + hx) * p.o_sh + 2 * lane;
+        dkv_store_f32<ODT>(p.out, ob, o0 * inv);
+        dkv_store_f32<ODT>(p.out, ob + 1, o1 * inv);
+      } else {
+        float* rec = rec0 + (long long)(QW * wave + 16 * qb + x) * (PG_DH + 2);
+        if (lane == 0) {
+          rec[0] = mx;
+          rec[1] = lx;
+        }
+        rec[2 + 2 * lane] = o0;
+        rec[3 + 2 * lane] = o1;
+      }
+    }
+  }
+}
+
+// The key ranges' records of one row joined: one wave per row, lane l dims 2l, 2l + 1.
+template <int DT, int ODT>
+__global__ __launch_bounds__(256) void paged_join_kernel(ChunkParams c) {
+  const AttendParams& p = c.a;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int groups = c.bq / 4;  // workgroups per (item, KV head)
+  const int x = blockIdx.x * 4 + wave;
+  const int ik = blockIdx.x / groups, row = x % c.bq;
+  const int kvh = ik % p.Hkv;
+  const ChunkItem it = chunk_item(c, ik / p.Hkv, lane);
+  if (it.b < 0) return;
+  const PagedRequest r = paged_request(p.pool, p.q_start, p.lens, it.b, p.T);
+  const int R = it.rt * c.bq + row;
+  if (R >= r.n * p.hpg) return;
+  const float* rec = p.records + (long long)ik * c.splits * c.bq * (PG_DH + 2) +
+                     (long long)row * (PG_DH + 2);
+  const long long step = (long long)c.bq * (PG_DH + 2);
+  float M = -1.0e30f;
+  for (int s = 0; s < c.splits; ++s) M = fmaxf(M, rec[s * step]);
+  float L = 0.f, a0 = 0.f, a1 = 0.f;
+  for (int s = 0; s < c.splits; ++s) {
+    const float* q = rec + s * step;
+    const float l = q[1];
+    if (l == 0.f) continue;  // a range without keys for the row
+    const float w = exp2f(q[0] - M);
+    L += w * l;
+    a0 += w * q[2 + 2 * lane];
+    a1 += w * q[3 + 2 * lane];
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  const int i = R / p.hpg, h = R - i * p.hpg;
+  const long long ob = (long long)(r.row0 + i) * p.o_st +
+                       (long long)(kvh * p.hpg + h) * p.o_sh + 2 * lane;
+  dkv_store_f32<ODT>(p.out, ob, a0 * inv);
+  dkv_store_f32<ODT>(p.out, ob + 1, a1 * inv);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -349,10 +1139,99 @@ extern "C" int dkv_paged_append(void* stream, int dtype, const void* qkv, long l
   return DKV_OK;
 }
 
-extern "C" long long dkv_paged_workspace_floats(int B, int Hq, int Hkv, int max_new, int min_new,
-                                                int max_len) {
-  (void)B, (void)Hq, (void)Hkv, (void)max_new, (void)min_new, (void)max_len;
-  return 0;
+namespace {
+
+// The launches of a call, from its bounds alone.
+struct AttendPlan {
+  bool few, many;          // kernels that run
+  int few_wgs, few_split;
+  int qb, nw, bq, items, splits;
+  long long floats;        // workspace (0: none)
+};
+
+// The shape of the many-row kernel by the number of 128-row workgroups, as the prefill attention's:
+// more than two rounds of the 512 that fit the chip take two row blocks per wave, up to that one
+// block and 8 waves, one workgroup per CU or fewer 64 rows. Fewer 64-row workgroups than CUs: the
+// keys of each are cut into ranges of at least 4 tiles.
+AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, int max_len) {
+  AttendPlan a = {};
+  const int hpg = Hq / Hkv;
+  const long long units = (long long)B * Hkv;
+  a.few = (long long)(min_new > 1 ? min_new : 1) * hpg <= DROWS;
+  a.many = (long long)max_new * hpg > DROWS;
+  long long floats = 0;
+  if (a.few) {
+    const long long tiles = ((long long)max_len + DTILE - 1) / DTILE;
+    const long long most = units * ((tiles + D_MIN_TILES - 1) / D_MIN_TILES);
+    long long wgs = units;
+    if (B <= D_SPLIT_B && units <= D_COUNTERS) {
+      if (wgs < D_WGS) wgs = most < D_WGS ? (most > units ? most : units) : D_WGS;
+      a.few_split = wgs > units;
+    }
+    a.few_wgs = (int)wgs;
+    if (a.few_split) floats = wgs * DREC;
+  }
+  if (a.many) {
+    auto items = [&](int bq) {  // sum over requests of ceil(rows / bq), at most
+      const long long rows = (long long)T * hpg, each = ((long long)max_new * hpg + bq - 1) / bq;
+      const long long x = rows / bq + B, y = each * B;
+      return x < y ? x : y;
+    };
+    const long long wg128 = items(128) * Hkv;
+    a.qb = wg128 > 1024 ? 2 : 1;
+    a.nw = wg128 > 1024 ? 4 : wg128 > 256 ? 8 : 4;
+    a.bq = 16 * a.qb * a.nw;
+    a.items = (int)items(a.bq);
+    a.splits = 1;
+    const long long wgs = (long long)a.items * Hkv;
+    if (a.bq == 64 && wgs < 256) {
+      const long long tiles = ((long long)max_len + CK - 1) / CK;
+      long long n = (512 + wgs - 1) / wgs;
+      if (n > tiles / 4) n = tiles / 4;
+      a.splits = (int)(n < 1 ? 1 : n);
+    }
+    if (a.splits > 1) {
+      const long long f = wgs * a.splits * a.bq * (PG_DH + 2);
+      if (f > floats) floats = f;
+    }
+  }
+  a.floats = floats ? D_COUNTERS + floats : 0;
+  return a;
+}
+
+template <int DT, int ODT>
+void launch_attend(const AttendPlan& a, const ChunkParams& c, hipStream_t st) {
+  if (a.few)
+    hipLaunchKernelGGL((paged_few_kernel<DT, ODT>), dim3((unsigned)a.few_wgs), dim3(64 * DW), 0, st,
+                       c.a);
+  if (!a.many) return;
+  const dim3 grid((unsigned)(a.items * c.a.Hkv * a.splits));
+  if (a.qb == 2)
+    hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 2, 4>), grid, dim3(256), 0, st, c);
+  else if (a.nw == 8)
+    hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 8>), grid, dim3(512), 0, st, c);
+  else
+    hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 4>), grid, dim3(256), 0, st, c);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((paged_join_kernel<DT, ODT>),
+                       dim3((unsigned)(a.items * c.a.Hkv * (a.bq / 4))), dim3(256), 0, st, c);
+}
+
+bool attend_sizes_ok(int B, int T, int Hq, int Hkv, int max_new) {
+  // rows and work items are counted in 32 bits
+  return (long long)T * (Hq / Hkv) + 4096 < 0x7fffffffLL &&
+         (long long)max_new * (Hq / Hkv) + 4096 < 0x7fffffffLL &&
+         (((long long)T * (Hq / Hkv)) / 64 + B) * Hkv * 32 < 0x7fffffffLL;
+}
+
+}  // namespace
+
+extern "C" long long dkv_paged_workspace_floats(int B, int T, int Hq, int Hkv, int max_new,
+                                                int min_new, int max_len) {
+  if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_new <= 0 || max_len < 0)
+    return 0;
+  if (!attend_sizes_ok(B, T, Hq, Hkv, max_new)) return 0;
+  return attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len).floats;
 }
 
 extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st,
@@ -370,16 +1249,19 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || max_new < 0 || min_new < 0 || max_len < 0)
     return DKV_E_ARG;
   if (Dh != PG_DH || Hq % Hkv != 0 || Hq / Hkv > 16) return DKV_E_UNSUPPORTED;
-  AttendParams p;
+  ChunkParams c;
+  AttendParams& p = c.a;
   const int rc = fill_pool(p.pool, page_stride, head_stride, num_pages, page_size, page_table,
                            table_ld, table_cols, Hkv);
   if (rc != DKV_OK) return rc;
   if (B == 0 || T == 0 || max_new == 0) return DKV_OK;
-  if (!q || !k_pages || !v_pages || !q_start || !lens || !out) return DKV_E_ARG;
+  if (!q || !k_pages || !v_pages || !q_start || !lens || !out || num_pages == 0) return DKV_E_ARG;
   if (q_st < 0 || q_sh < 0 || o_st < 0 || o_sh < PG_DH) return DKV_E_ARG;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || (q_st & 7) || (q_sh & 7))
     return DKV_E_UNSUPPORTED;
-  (void)workspace, (void)workspace_floats;
+  if (!attend_sizes_ok(B, T, Hq, Hkv, max_new)) return DKV_E_UNSUPPORTED;
+  const AttendPlan plan = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len);
+  if (plan.floats > 0 && (!workspace || workspace_floats < plan.floats)) return DKV_E_WORKSPACE;
   p.q = (const uint16_t*)q;
   p.q_st = q_st;
   p.q_sh = q_sh;
@@ -394,24 +1276,26 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   p.T = T;
   p.Hq = Hq;
   p.Hkv = Hkv;
-  p.scale = scale;
-  if (Hq > 65535) return DKV_E_UNSUPPORTED;
+  p.hpg = Hq / Hkv;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.counters = reinterpret_cast<int*>(workspace);
+  p.records = workspace ? workspace + D_COUNTERS : nullptr;
+  p.split = plan.few_split;
+  c.bq = plan.bq;
+  c.splits = plan.splits;
+  c.few_rows = plan.few ? DROWS : 0;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)T, (unsigned)Hq);
-#define PG_LAUNCH(DT, ODT) \
-  hipLaunchKernelGGL((paged_attend_kernel<DT, ODT>), grid, dim3(64), 0, st, p)
   if (dtype == DKV_BF16) {
     if (out_dtype == DKV_F32)
-      PG_LAUNCH(DKV_BF16, DKV_F32);
+      launch_attend<DKV_BF16, DKV_F32>(plan, c, st);
     else
-      PG_LAUNCH(DKV_BF16, DKV_BF16);
+      launch_attend<DKV_BF16, DKV_BF16>(plan, c, st);
   } else {
     if (out_dtype == DKV_F32)
-      PG_LAUNCH(DKV_F16, DKV_F32);
+      launch_attend<DKV_F16, DKV_F32>(plan, c, st);
     else
-      PG_LAUNCH(DKV_F16, DKV_F16);
+      launch_attend<DKV_F16, DKV_F16>(plan, c, st);
   }
-#undef PG_LAUNCH
   DKV_HIP_CHECK_LAUNCH();
   return DKV_OK;
 }

@@ -32,7 +32,7 @@ from .. import _lib
 from .decode import workspace
 
 HEAD_DIM = 128
-MAX_HEADS_PER_KV = 16
+_COUNTERS = 16384  # leading floats of the attention's workspace: its arrival counters
 
 
 class PagedBatch:
@@ -262,8 +262,8 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             out.stride(0), out.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
             k_pages.stride(0), k_pages.stride(1), k_pages.shape[0], ps, t.data_ptr(),
             max(t.stride(0), t.shape[1]), t.shape[1], batch.q_start.data_ptr(),
-            batch.lens.data_ptr(), batch.requests, T, heads, hkv, HEAD_DIM, _lib.ptr(q_norm),
-            _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs))
+            batch.lens.data_ptr(), batch.requests, batch.rows, heads, hkv, HEAD_DIM,
+            _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs))
     _lib.check(rc, "dkv_paged_append")
     return out
 
@@ -303,15 +303,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lib = _lib.calls()
     t = batch.page_table
     with _lib.on_device(q):
-        need = lib.dkv_paged_workspace_floats(batch.requests, hq, hkv, batch.max_new,
+        need = lib.dkv_paged_workspace_floats(batch.requests, batch.rows, hq, hkv, batch.max_new,
                                               batch.min_new, batch.max_len)
         ws = _attention_workspace(q.device, st, need) if need else None
         rc = lib.dkv_paged_attention(
             st, _lib.dtype_code(q.dtype), q.data_ptr(), q.stride(0), q.stride(1),
             k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
             k_pages.shape[0], ps, t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[1],
-            batch.q_start.data_ptr(), batch.lens.data_ptr(), batch.requests, T, hq, hkv, HEAD_DIM,
-            batch.max_new, batch.min_new, batch.max_len, sc, _lib.ptr(ws),
+            batch.q_start.data_ptr(), batch.lens.data_ptr(), batch.requests, batch.rows, hq, hkv,
+            HEAD_DIM, batch.max_new, batch.min_new, batch.max_len, sc, _lib.ptr(ws),
             ws.numel() if need else 0, out.data_ptr(), _lib.dtype_code(odt), out.stride(0),
             out.stride(1))
     _lib.check(rc, "dkv_paged_attention")
@@ -323,5 +323,7 @@ def _attention_workspace(device: torch.device, stream: int, floats: int) -> torc
     share its workspace, in that stream's order. A call under capture gets one of its own in the
     graph's pool, cleared by the graph itself: two captured graphs may be replayed at once."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(floats, dtype=torch.float32, device=device)
+        ws = torch.empty(floats, dtype=torch.float32, device=device)
+        ws[:_COUNTERS].zero_()
+        return ws
     return workspace(device, stream, floats)

@@ -648,7 +648,8 @@ int dkv_paged_append(void* stream, int dtype, const void* qkv, long long qkv_ld,
                      const int* page_table, long long table_ld, int table_cols, const int* q_start,
                      const int* lens, int B, int T, int Hq, int Hkv, int Dh, const void* q_norm,
                      const void* k_norm, float eps, const double* inv_freq);
-long long dkv_paged_workspace_floats(int B, int Hq, int Hkv, int max_new, int min_new, int max_len);
+long long dkv_paged_workspace_floats(int B, int T, int Hq, int Hkv, int max_new, int min_new,
+                                     int max_len);
 int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st, long long q_sh,
                         const void* k_pages, const void* v_pages, long long page_stride,
                         long long head_stride, int num_pages, int page_size,

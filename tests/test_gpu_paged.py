@@ -338,6 +338,33 @@ def test_attention_masks_pages_that_are_not_there(dev, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("new,n,hkv", [(4, 300, 2), (60, 60, 2), (60, 3000, 2), (700, 700, 8)])
+def test_attention_keeps_later_tokens_out(dev, new, n, hkv, value):
+    """An infinity or NaN in a new token's key and value: the tokens before it, that do not attend
+    it, have the result they have without it; the ones from it on have it in theirs."""
+    print(f"[gpu] paged attention later {value} {new}", flush=True)
+    s = Step(dev, [new, 1], [n, 40], hkv=hkv, seed=17)
+    q = s.rand(s.T, 4 * hkv, DH)
+    clean = paged_attention(q, s.k, s.v, s.batch, out_dtype=torch.float32)
+    _, tol = _attend_reference(s, q)
+    bad = n - new + new // 2  # the position of the token
+    page, slot = int(s.table[0, bad // 16]), bad % 16
+    s.v[page, :, slot, ::3] = value
+    got = paged_attention(q, s.k, s.v, s.batch, out_dtype=torch.float32)
+    before, after = slice(0, new // 2), slice(new // 2, new)
+    assert bool(((got[before] - clean[before]).abs() <= 2 * tol[before]).all())
+    assert torch.equal(got[new:], clean[new:])
+    assert not bool(torch.isfinite(got[after][..., ::3]).any())
+    # the dims beside it are what they were (a sum of their own)
+    assert bool(((got[after] - clean[after]).abs() <= 2 * tol[after])[..., 1::3].all())
+    s.k[page, :, slot] = value
+    got = paged_attention(q, s.k, s.v, s.batch, out_dtype=torch.float32)
+    assert bool(((got[before] - clean[before]).abs() <= 2 * tol[before]).all())
+    assert torch.equal(got[new:], clean[new:])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new,lens", [([1, 1], [900, 450]), ([90, 2], [350, 200])])
 def test_attention_same_result_every_time(dev, new, lens):
     print(f"[gpu] paged attention repeat {new}", flush=True)
