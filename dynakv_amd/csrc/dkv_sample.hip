@@ -8,10 +8,18 @@
 // and how many of its equals are (the lowest indices). The answer is the first token, in the
 // vocabulary's order, up to which the kept mass exceeds u times all of it.
 //
-// Weights are held in 64-bit fixed point, 44 bits after the point, computed in 64-bit floating
-// point: sums of them are the same in any order (the histograms add by atomics), and a token is
-// decided by u * mass against a running sum, where 32 bits would pick another token than the
-// formula's in one draw of a few thousand.
+// Weights are held in 64-bit fixed point, 44 bits after the point: sums of them are the same in any
+// order (the histogram adds by atomics), and a token is decided by u * mass against a running sum,
+// where 32 bits would pick another token than the formula's in one draw of a few thousand. With
+// x = 64 log2(e) (max l - l) / t in 64-bit floating point, i = floor(x):
+//   w = 2^(-i/64) (1 - d),  d = 1 - 2^(-(x - i)/64) < 0.011,
+// d to 32 bits after the point, 2^(-j/64) from a table of 64.
+//
+// One workgroup of 1024 threads per row, which goes over the row four times (from the caches after the
+// first): the maximum; a histogram of the tokens by i (counts and sums of d in one 64-bit number, so that a bin's mass is
+// known), in which the borders' bins are found; the tokens of a border's bin sorted in LDS; the kept
+// mass of every 512 tokens (256 in fp32), in the vocabulary's order; the token. Bound by vector
+// instructions: a row's 128256 tokens in one CU take 0.85 us an instruction.
 #include "dkv_common.h"
 
 namespace {
@@ -22,7 +30,12 @@ constexpr int SM_THREADS = 1024;
 constexpr int SM_WAVES = SM_THREADS / 64;
 constexpr int SM_POINT = 44;             // bits after the point of a weight
 constexpr int SM_MAX_V = 1 << 19;        // weights of at most 1: sums below 2^63
-constexpr int SM_BINS = 2048;
+constexpr int SM_AHEAD = 4;              // 16-byte pieces that a thread has in flight
+constexpr int SM_BINS = 4096;            // bins of 1/64 in log2 of the weight; the last: the rest
+constexpr int SM_CAND = 2048;            // tokens of a border's bin that are sorted
+constexpr int SM_CHUNKS = SM_WAVES * (SM_MAX_V / 4 / SM_THREADS + 1);  // 1 KB pieces of a row
+constexpr int SM_COUNT = 45;             // a bin: the count from this bit on, below it the sum of d
+constexpr double SM_ONE = 17592186044416.0;  // 2^44
 
 struct SampleParams {
   const void* logits;
@@ -38,41 +51,15 @@ struct SampleParams {
   long long* out;
 };
 
-// A logit as a number that orders as the logits do: NaN as -infinity, -0 as +0.
-__device__ __forceinline__ float sm_clean(float f) {
-  return f != f ? -INFINITY : f + 0.0f;
-}
+// A logit as a number that orders as the logits do (-0 as +0).
 __device__ __forceinline__ uint32_t sm_key(float f) {
-  const uint32_t b = __float_as_uint(f);
+  const uint32_t b = __float_as_uint(f + 0.0f);
   return b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u);
 }
-
-__device__ __forceinline__ u64 sm_weight(float l, float m, double c) {
-  if (l == m) return 1ULL << SM_POINT;
-  const double y = ((double)l - (double)m) * c;  // c = log2(e) / t
-  if (!(y > -(double)(SM_POINT + 2))) return 0;
-  const double n = rint(y), g = (y - n) * 0.69314718055994530942;
-  double s = 1.0 / 479001600.0;  // sum of g^k / k!, k <= 12: |g| <= ln 2 / 2, 2e-16 left out
-  s = fma(s, g, 1.0 / 39916800.0);
-  s = fma(s, g, 1.0 / 3628800.0);
-  s = fma(s, g, 1.0 / 362880.0);
-  s = fma(s, g, 1.0 / 40320.0);
-  s = fma(s, g, 1.0 / 5040.0);
-  s = fma(s, g, 1.0 / 720.0);
-  s = fma(s, g, 1.0 / 120.0);
-  s = fma(s, g, 1.0 / 24.0);
-  s = fma(s, g, 1.0 / 6.0);
-  s = fma(s, g, 0.5);
-  s = fma(s, g, 1.0);
-  s = fma(s, g, 1.0);
-  return (u64)llrint(ldexp(s, (int)n + SM_POINT));
+__device__ __forceinline__ float sm_unkey(uint32_t k) {
+  return __uint_as_float(k ^ ((int)k < 0 ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ u64 sm_wave_sum(u64 v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 __device__ __forceinline__ u64 sm_wave_scan(u64 v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -81,191 +68,500 @@ __device__ __forceinline__ u64 sm_wave_scan(u64 v, int lane) {  // inclusive
   }
   return v;
 }
+__device__ __forceinline__ double sm_wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
 
-// What is kept: every token above `key`, and the first `ties` of those at it.
+// What is kept: every token above `key`, and those at it up to index `last`.
 struct Border {
-  uint32_t key;
-  int ties;
+  float at;
+  int last;
 };
 
 template <int DT>
 __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
-  __shared__ u64 sMass[SM_BINS];
-  __shared__ uint32_t sCount[SM_BINS];
+  constexpr int E = DT == DKV_F32 ? 4 : 8;  // elements of a 16-byte piece
+  __shared__ u64 sHist[SM_BINS];
+  __shared__ u64 sCand[SM_CAND];
+  __shared__ u64 sSort[SM_CAND];
+  __shared__ u64 sChunk[SM_CHUNKS];
+  __shared__ double sRoot[64];
   __shared__ u64 sWave[SM_WAVES];
-  __shared__ uint32_t sWaveN[SM_WAVES];
+  __shared__ u64 sWave2[SM_WAVES];
+  __shared__ float sMax[SM_WAVES];
   __shared__ u64 sPick[4];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int sN;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int V = p.V;
   const char* base = (const char*)p.logits + (long long)row * p.ld * (DT == DKV_F32 ? 4 : 2);
-  auto logit = [&](int i) { return sm_clean(dkv_load_f32<DT>(base, i)); };
   const float t = p.temperature ? p.temperature[row] : p.temperature_all;
   const int k = p.top_k ? p.top_k[row] : p.top_k_all;
   const float tp = p.top_p ? p.top_p[row] : p.top_p_all;
   const float mp = p.min_p ? p.min_p[row] : p.min_p_all;
-  const int V = p.V;
 
-  // the largest logit and the first index of it
-  u64 best = 0;
-  for (int i = tid; i < V; i += SM_THREADS)
-    best = max(best, ((u64)sm_key(logit(i)) << 32) | (uint32_t)~i);
+  // ---- the row: pieces of 16 aligned bytes, a wave's consecutive ----
+  const int head = (int)((uintptr_t)base & 15) / (16 / E);  // elements of the first piece before it
+  const int pieces = (V + head + E - 1) / E;
+  const int per_wave = (pieces + SM_THREADS - 1) / SM_THREADS;  // of 64 pieces each
+  auto first_of = [&](int c) { return ((wave * per_wave + c) * 64 + lane) * E - head; };
+  // piece c of the thread as its words; elements outside the row are -infinity
+  auto load = [&](int c) {
+    const int i0 = first_of(c);
+    constexpr uint32_t none = DT == DKV_F32 ? 0xff800000u
+                              : DT == DKV_BF16 ? 0xff80ff80u
+                                               : 0xfc00fc00u;
+    dkv_u32x4 v = {none, none, none, none};
+    if (i0 >= 0 && i0 + E <= V) {
+      v = *(const dkv_u32x4*)(base + (long long)i0 * (16 / E));
+    } else if (i0 + E > 0 && i0 < V) {  // the first or the last piece
+      uint32_t w[4] = {none, none, none, none};
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
-  if (lane == 0) sWave[wave] = best;
+      for (int e = 0; e < E; ++e) {
+        if (i0 + e < 0 || i0 + e >= V) continue;
+        if constexpr (E == 4) {
+          w[e] = ((const uint32_t*)base)[i0 + e];
+        } else {
+          const uint32_t x = ((const uint16_t*)base)[i0 + e];
+          w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | (x << 16) : (w[e / 2] & 0xffff0000u) | x;
+        }
+      }
+      v = dkv_u32x4{w[0], w[1], w[2], w[3]};
+    }
+    return v;
+  };
+  // In a row with logits of +infinity those share the mass: they are read as 0, the others as
+  // -infinity.
+  bool infinite = false;
+  auto remap = [&](dkv_u32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == DKV_F32) {
+        v[i] = v[i] == 0x7f800000u ? 0u : 0xff800000u;
+      } else {
+        constexpr uint32_t inf = DT == DKV_BF16 ? 0x7f80u : 0x7c00u;
+        v[i] = ((v[i] & 0xffffu) == inf ? 0u : inf | 0x8000u) |
+               ((v[i] >> 16) == inf ? 0u : (inf | 0x8000u) << 16);
+      }
+    }
+    return v;
+  };
+  auto value = [&](const dkv_u32x4& v, int e) {
+    if constexpr (DT == DKV_F32)
+      return __uint_as_float(v[e]);
+    else if constexpr (DT == DKV_BF16)
+      return __uint_as_float(e & 1 ? v[e / 2] & 0xffff0000u : v[e / 2] << 16);
+    else
+      return dkv_f16_bits_to_f32(e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xffffu);
+  };
+  auto load_again = [&](int c) {
+    const dkv_u32x4 v = load(c);
+    return infinite ? remap(v) : v;
+  };
+  // f(c, its first token, the piece) for each of the thread's pieces, in order
+  auto each = [&](auto&& f) {
+#pragma unroll 1
+    for (int c = 0; c < per_wave; c += SM_AHEAD) {
+      dkv_u32x4 v[SM_AHEAD];
+#pragma unroll
+      for (int q = 0; q < SM_AHEAD; ++q)
+        if (c + q < per_wave) v[q] = load_again(c + q);
+#pragma unroll
+      for (int q = 0; q < SM_AHEAD; ++q)
+        if (c + q < per_wave) f(c + q, first_of(c + q), v[q]);
+    }
+  };
+
+  // ---- the largest logit ----
+  float m = -INFINITY;
+  each([&](int, int, const dkv_u32x4& v) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, value(v, e));  // (a NaN is passed over)
+  });
+  m = dkv_wave_max(m);
+  if (lane == 0) sMax[wave] = m;
+  if (tid == 0) sN = 0x7fffffff;
+  if (tid < 64) sRoot[tid] = exp2(-(double)tid / 64.0);
   __syncthreads();
-  for (int w = 0; w < SM_WAVES; ++w) best = max(best, sWave[w]);
-  __syncthreads();
-  const int arg = (int)~(uint32_t)best;
-  const float m = logit(arg);
+  for (int w = 0; w < SM_WAVES; ++w) m = fmaxf(m, sMax[w]);
   if (m == -INFINITY) {
     if (tid == 0) p.out[row] = -1;
     return;
   }
   if (!(t > 0.f) || k == 1 || tp <= 0.f || mp > 1.f) {  // the first token alone
-    if (tid == 0) p.out[row] = arg;
+    int at = 0x7fffffff;
+    each([&](int c, int i0, const dkv_u32x4& v) {
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (value(v, e) == m) at = min(at, i0 + e);
+    });
+    if (at != 0x7fffffff) atomicMin(&sN, at);
+    __syncthreads();
+    if (tid == 0) p.out[row] = sN;
     return;
   }
-  const double c = 1.4426950408889634074 / (double)t;
+  if (m == INFINITY) {
+    infinite = true;
+    m = 0.f;
+  }
+  const double c64 = 64.0 * 1.4426950408889634074 / (double)fminf(fmaxf(t, 1e-30f), 1e30f);
 
-  // The border by digits of the keys (11, 11, 10 bits): a histogram of the tokens that share the
-  // digits found so far, counts and masses, and the bin in which the k-th token (by_mass: the
-  // first token before which the mass reaches P) lies. Every thread gets the same answer.
-  auto find = [&](bool by_mass, u64 want, double P, u64& mass_above) {
-    Border r = {0, 0};
-    u64 above = 0;  // mass or count above the bins of this level
-    u64 m_above = 0;
+  // bin and d (32 bits after the point) of a logit
+  auto split = [&](float l, int& i, uint32_t& d) {
+    const double x = fmin(((double)m - (double)l) * c64, (double)(SM_BINS - 1));
+    i = (int)x;
+    const float f = (float)(x - (double)i);
+    // 2^32 (1 - 2^(-f/64)): with g = ln2 / 64, g f - (g f)^2 / 2 + (g f)^3 / 6 - (g f)^4 / 24
+    constexpr double g = 0.69314718055994530942 / 64, one = 4294967296.0;
+    const float s =
+        f * (float)(g * one) +
+        f * f * ((float)(-g * g / 2 * one) +
+                 f * ((float)(g * g * g / 6 * one) + f * (float)(-g * g * g * g / 24 * one)));
+    d = (uint32_t)fmaxf(s, 0.f);
+  };
+  // the weight of a logit, a whole number (of 2^-44) in a double
+  auto weight = [&](float l) {
+    int i;
+    uint32_t d;
+    split(l, i, d);
+    const double w = sRoot[i & 63] * fma((double)d, -1.0 / 4294967296.0, 1.0);
+    return i == SM_BINS - 1 ? 0.0 : rint(ldexp(w, SM_POINT - (i >> 6)));
+  };
+  auto bin_of = [&](float l) {
+    return (int)fmin(((double)m - (double)l) * c64, (double)(SM_BINS - 1));
+  };
+  // the mass of a bin
+  auto bin_mass = [&](int i, u64 h) {
+    const double n = (double)(h >> SM_COUNT);
+    const double d = (double)(h & ((1ULL << SM_COUNT) - 1)) * (1.0 / 4294967296.0);
+    return i == SM_BINS - 1 ? 0ULL
+                            : (u64)rint(ldexp(sRoot[i & 63] * (n - d), SM_POINT - (i >> 6)));
+  };
+
+  const bool by_k = k > 0 && k < V, by_p = tp < 1.f;
+  Border keep = {-INFINITY, -1};
+  u64 kept = 0;  // the mass of what is kept so far
+
+  // ---- the border inside a bin: its tokens sorted ----
+  // j > 0: up to the j-th of them; else those before which (with `before`) less than P lies. Returns
+  // false where they are too many. `mass`: what is kept of the bin.
+  auto in_bin = [&](int bin, u64 j, u64 before, double P, Border& r, u64& mass) {
+    __syncthreads();
+    if (tid == 0) sN = 0;
+    __syncthreads();
+    const float c32 = (float)c64, mid = (float)bin + 0.5f;
+    each([&](int c, int i0, const dkv_u32x4& v) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float l = value(v, e);
+        const float x = (m - l) * c32;
+        if (!(fabsf(x - mid) > 0.52f) || bin == SM_BINS - 1) {  // near it, or not to be told
+          const int i = i0 + e;
+          if (i >= 0 && i < V && l == l && bin_of(l) == bin) {
+            const int at = atomicAdd(&sN, 1);
+            if (at < SM_CAND) sCand[at] = ((u64)sm_key(l) << 32) | (uint32_t)~i;
+          }
+        }
+      }
+    });
+    __syncthreads();
+    const int n = sN;
+    if (n > SM_CAND) return false;
+    for (int a = tid; a < n; a += SM_THREADS) {
+      const u64 x = sCand[a];
+      int rank = 0;
+      for (int b = 0; b < n; ++b) rank += sCand[b] > x;
+      sSort[rank] = x;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      u64 run = 0;
+      int last = -1;
+      for (int a = 0; a < n; a += 64) {
+        const int at = a + lane;
+        const u64 w = at < n ? (u64)weight(sm_unkey((uint32_t)(sSort[at] >> 32))) : 0;
+        const u64 sum = sm_wave_scan(w, lane);
+        const bool in = at < n && (j ? (u64)at < j : (double)(before + run + sum - w) < P);
+        const u64 hit = __ballot(in);
+        if (!hit) break;
+        const int l = 63 - __clzll((long long)hit);
+        last = a + l;
+        run += __shfl(sum, l, 64);
+        if (l < 63) break;
+      }
+      if (lane == 0) {
+        sPick[0] = last >= 0 ? sSort[last] : 0;
+        sPick[1] = run;
+      }
+    }
+    __syncthreads();
+    // (no token at all: the j-th is a NaN; everything above them is kept)
+    r.at = sPick[0] ? sm_unkey((uint32_t)(sPick[0] >> 32)) : -INFINITY;
+    r.last = (int)~(uint32_t)sPick[0];
+    mass = sPick[1];
+    return true;
+  };
+
+  // ---- the border by digits of the keys (11, 11, 10 bits): for a bin of too many tokens ----
+  // Level by level the bin in which the border lies, among the tokens that share the digits found so
+  // far; then the index of the last of the equal ones that are kept. Clears the histogram.
+  auto by_digits = [&](u64 want, double P, Border& r, u64& mass_kept) {
+    u64 above = 0, m_above = 0;
     uint32_t found = 0;
+    u64 ties = 0;
     for (int level = 0; level < 3; ++level) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
       const int bits = level == 2 ? 10 : 11;
-      for (int i = tid; i < SM_BINS; i += SM_THREADS) sMass[i] = 0, sCount[i] = 0;
       __syncthreads();
-      for (int i = tid; i < V; i += SM_THREADS) {
-        const float l = logit(i);
-        const uint32_t key = sm_key(l);
-        if (level && (key >> (shift + bits)) != found) continue;
-        const int bin = (int)((key >> shift) & ((1u << bits) - 1));
-        atomicAdd(&sCount[bin], 1u);
-        atomicAdd(&sMass[bin], sm_weight(l, m, c));
-      }
+      for (int i = tid; i < SM_BINS; i += SM_THREADS) sHist[i] = 0;
       __syncthreads();
-      // thread 0 walks the bins from the top
-      if (tid == 0) {
-        u64 cum = above, mass = m_above;
-        int at = -1;
-        u64 cum_at = 0, mass_at = 0;
-        for (int bin = (1 << bits) - 1; bin >= 0; --bin) {
-          if (!sCount[bin]) continue;
-          if (by_mass ? (double)cum < P : cum < want) {
-            at = bin;
-            cum_at = cum;
-            mass_at = mass;
-          } else {
-            break;
-          }
-          cum += by_mass ? sMass[bin] : sCount[bin];
-          mass += sMass[bin];
+      each([&](int c, int i0, const dkv_u32x4& v) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float l = fmaxf(value(v, e), -INFINITY);
+          const int i = i0 + e;
+          if (i < 0 || i >= V) continue;
+          const uint32_t key = sm_key(l);
+          if (level && (key >> (shift + bits)) != found) continue;
+          const int bin = (int)((key >> shift) & ((1u << bits) - 1));
+          atomicAdd(&sHist[bin], (u64)weight(l));
+          atomicAdd(&sHist[2048 + bin], 1ULL);
         }
-        sPick[0] = (u64)(uint32_t)at;
-        sPick[1] = cum_at;
+      });
+      __syncthreads();
+      if (tid == 0) {  // the bins from the top
+        u64 cnt = above, mass = m_above, cnt_at = 0, mass_at = 0;
+        int at = 0;
+        for (int bin = (1 << bits) - 1; bin >= 0; --bin) {
+          if (!sHist[2048 + bin]) continue;
+          if (!(want ? cnt < want : (double)mass < P)) break;
+          at = bin;
+          cnt_at = cnt;
+          mass_at = mass;
+          cnt += sHist[2048 + bin];
+          mass += sHist[bin];
+        }
+        sPick[0] = (u64)at;
+        sPick[1] = cnt_at;
         sPick[2] = mass_at;
-        sPick[3] = at >= 0 ? sCount[at] : 0;
+        sPick[3] = sHist[2048 + at];
       }
       __syncthreads();
       found = (found << bits) | (uint32_t)sPick[0];
       above = sPick[1];
       m_above = sPick[2];
-      r.ties = (int)sPick[3];
-      __syncthreads();
+      ties = sPick[3];
     }
-    r.key = found;
-    const uint32_t b = found ^ ((int)found < 0 ? 0x80000000u : 0xffffffffu);
-    const u64 w = sm_weight(__uint_as_float(b), m, c);
-    if (!by_mass) {
-      r.ties = (int)min((u64)r.ties, want - above);
+    r.at = sm_unkey(found);
+    const u64 w = (u64)weight(r.at);
+    if (want) {
+      ties = min(ties, want - above);
     } else if (w > 0) {
-      // the ties before which less than P lies
-      int lo = 1, hi = r.ties;
+      u64 lo = 1, hi = ties;  // the equal ones before which less than P lies
       while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if ((double)(above + (u64)(mid - 1) * w) < P)
+        const u64 mid = (lo + hi + 1) / 2;
+        if ((double)(m_above + (mid - 1) * w) < P)
           lo = mid;
         else
           hi = mid - 1;
       }
-      r.ties = lo;
+      ties = lo;
     }
-    mass_above = m_above + (u64)r.ties * w;  // the mass kept
-    return r;
+    mass_kept = m_above + ties * w;
+    // the index of the last of them: equal ones by piece row, in order
+    __syncthreads();
+    for (int i = tid; i < SM_CHUNKS; i += SM_THREADS) sChunk[i] = 0;
+    __syncthreads();
+    each([&](int c, int i0, const dkv_u32x4& v) {
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = i0 + e;
+        n += i >= 0 && i < V && fmaxf(value(v, e), -INFINITY) == r.at;
+      }
+      if (n) atomicAdd(&sChunk[wave * per_wave + c], (u64)n);
+    });
+    __syncthreads();
+    if (tid == 0) {
+      u64 cnt = 0;
+      int at = 0;
+      for (; at < SM_WAVES * per_wave - 1 && cnt + sChunk[at] < ties; ++at) cnt += sChunk[at];
+      sPick[0] = (u64)at;
+      sPick[1] = ties - cnt;  // the one of them in that piece row
+    }
+    __syncthreads();
+    if ((int)sPick[0] / per_wave == wave) {
+      const int c = (int)sPick[0] % per_wave;
+      const dkv_u32x4 v = load_again(c);
+      const int i0 = first_of(c);
+      uint32_t mask = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = i0 + e;
+        if (i >= 0 && i < V && fmaxf(value(v, e), -INFINITY) == r.at) mask |= 1u << e;
+      }
+      const u64 run = sm_wave_scan((u64)__popc(mask), lane), want_at = sPick[1];
+      const u64 before = run - (u64)__popc(mask);
+      if (before < want_at && want_at <= run) {
+        for (u64 x = before + 1; x < want_at; ++x) mask &= mask - 1;
+        sPick[2] = (u64)(i0 + __ffs((int)mask) - 1);
+      }
+    }
+    __syncthreads();
+    r.last = (int)sPick[2];
+    __syncthreads();
   };
 
-  Border keep = {0, 0x7fffffff};
-  u64 kept = 0;
-  const bool by_k = k > 0 && k < V, by_p = tp < 1.f;
-  if (by_k) keep = find(false, (u64)k, 0.0, kept);
-  if (by_p) {
-    if (!by_k) {
-      u64 s = 0;
-      for (int i = tid; i < V; i += SM_THREADS) s += sm_weight(logit(i), m, c);
-      s = sm_wave_sum(s);
-      if (lane == 0) sWave[wave] = s;
-      __syncthreads();
-      for (int w = 0; w < SM_WAVES; ++w) kept += sWave[w];
-      __syncthreads();
+  if (by_k || by_p) {
+    // ---- the histogram ----
+    for (int i = tid; i < SM_BINS; i += SM_THREADS) sHist[i] = 0;
+    __syncthreads();
+    each([&](int c, int i0, const dkv_u32x4& v) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float l = fmaxf(value(v, e), -INFINITY);
+        int i;
+        uint32_t d;
+        split(l, i, d);
+        if (i < SM_BINS - 1) atomicAdd(&sHist[i], (1ULL << SM_COUNT) | d);
+      }
+    });
+    __syncthreads();
+    // running counts and masses: thread i has bins 4i .. 4i + 3 (the last bin is the rest)
+    u64 cnt[4], mass[4], nsum = 0, msum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const u64 h = sHist[4 * tid + q];
+      cnt[q] = h >> SM_COUNT;
+      mass[q] = bin_mass(4 * tid + q, h);
+      nsum += cnt[q];
+      msum += mass[q];
     }
-    const double P = (double)tp * (double)kept;
-    keep = find(true, 0, P, kept);
+    u64 nrun = sm_wave_scan(nsum, lane), mrun = sm_wave_scan(msum, lane);
+    if (lane == 63) {
+      sWave[wave] = nrun;
+      sWave2[wave] = mrun;
+    }
+    __syncthreads();
+    u64 total = 0;
+    nrun -= nsum;
+    mrun -= msum;
+    for (int w = 0; w < SM_WAVES; ++w) {
+      if (w < wave) {
+        nrun += sWave[w];
+        mrun += sWave2[w];
+      }
+      total += sWave2[w];
+    }
+    kept = total;
+    bool digits = false;
+#pragma unroll 1
+    for (int step = 0; step < 2; ++step) {  // top-k, then top-p of what it keeps
+      if (step == 0 ? !by_k : !by_p) continue;
+      const u64 want = step == 0 ? (u64)k : 0;
+      const double P = step == 0 ? 0.0 : (double)tp * (double)kept;
+      bool found = false;
+      __syncthreads();
+      if (!digits) {
+        if (tid == 0) sPick[0] = step == 0 ? SM_BINS - 1 : SM_BINS, sPick[1] = sPick[2] = 0;
+        __syncthreads();
+        u64 n = nrun, s = mrun;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bool rest = 4 * tid + q == SM_BINS - 1;
+          const bool here = step == 0 ? n < want && (rest || want <= n + cnt[q])
+                                      : cnt[q] && (double)s < P && P <= (double)(s + mass[q]);
+          if (here) {
+            sPick[0] = (u64)(4 * tid + q);
+            sPick[1] = n;
+            sPick[2] = s;
+          }
+          n += cnt[q];
+          s += mass[q];
+        }
+        __syncthreads();
+        const int bin = (int)sPick[0];
+        const u64 j = want - sPick[1], above = sPick[2];
+        u64 in = 0;
+        Border r;
+        if (bin < SM_BINS && in_bin(bin, step == 0 ? j : 0, above, P, r, in)) {
+          keep = r;
+          kept = above + in;
+          found = true;
+        }
+      }
+      if (!found) {
+        by_digits(want, P, keep, kept);
+        digits = true;
+      }
+    }
   }
-  const double floor_w = mp > 0.f ? (double)mp * (double)(1ULL << SM_POINT) : 0.0;
 
-  // The kept mass in the vocabulary's order: wave w takes the w-th part of the row.
-  const int part = (V + SM_WAVES - 1) / SM_WAVES;
-  const int i0 = min(V, wave * part), i1 = min(V, i0 + part);
-  // ties up to the part
-  uint32_t nt = 0;
-  for (int i = i0 + lane; i < i1; i += 64) nt += sm_key(logit(i)) == keep.key;
-  nt = (uint32_t)sm_wave_sum(nt);
-  if (lane == 0) sWaveN[wave] = nt;
-  __syncthreads();
-  uint32_t ties0 = 0;
-  for (int w = 0; w < wave; ++w) ties0 += sWaveN[w];
-  auto part_mass = [&](u64 target, bool pick, u64 before) {
-    u64 sum = before;
-    uint32_t ties = ties0;
-    for (int j = i0; j < i1; j += 64) {
-      const int i = j + lane;
-      const float l = i < i1 ? logit(i) : -INFINITY;
-      const uint32_t key = i < i1 ? sm_key(l) : 0u;
-      const u64 same = __ballot(i < i1 && key == keep.key);
-      const uint32_t rank = ties + (uint32_t)__popcll(same & ((1ULL << lane) - 1));
-      ties += (uint32_t)__popcll(same);
-      u64 w = 0;
-      if (i < i1 && (key > keep.key || (key == keep.key && rank < (uint32_t)keep.ties))) {
-        w = sm_weight(l, m, c);
-        if ((double)w < floor_w) w = 0;
-      }
-      const u64 run = sm_wave_scan(w, lane);
-      if (pick) {
-        const u64 hit = __ballot(sum + run > target);
-        if (hit) return (u64)(j + __ffsll((long long)hit) - 1);
-      }
-      sum += __shfl(run, 63, 64);
+  // ---- the kept mass of each row of 64 pieces ----
+  const double floor_w = mp > 0.f ? (double)mp * SM_ONE : 0.0;
+  auto mass_of = [&](float l, int i) {
+    double w = 0.0;
+    if (l > keep.at || (l == keep.at && i <= keep.last)) {
+      w = weight(l);
+      w = w >= floor_w ? w : 0.0;
     }
-    return pick ? (u64)-1 : sum;
+    return w;
   };
-  const u64 mine = part_mass(0, false, 0);
-  if (lane == 0) sWave[wave] = mine;
   __syncthreads();
-  u64 all = 0, before = 0;
+  each([&](int c, int i0, const dkv_u32x4& v) {
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s += mass_of(value(v, e), i0 + e);
+    }
+    s = sm_wave_sum(s);  // 512 whole numbers of at most 2^44: exact
+    if (lane == 0) sChunk[wave * per_wave + c] = (u64)s;
+  });
+  __syncthreads();
+  // ---- the row of pieces in which u * mass lies ----
+  const int rows = SM_WAVES * per_wave;
+  const int share = (rows + SM_THREADS - 1) / SM_THREADS;
+  u64 own = 0;
+  for (int i = tid * share; i < min(rows, (tid + 1) * share); ++i) own += sChunk[i];
+  u64 run = sm_wave_scan(own, lane);
+  if (lane == 63) sWave[wave] = run;
+  __syncthreads();
+  u64 all = 0;
+  run -= own;
   for (int w = 0; w < SM_WAVES; ++w) {
-    if (w < wave) before += sWave[w];
+    if (w < wave) run += sWave[w];
     all += sWave[w];
   }
   const float uu = p.u[row];
   const double U = uu > 0.f ? (double)uu * (double)all : 0.0;
   const u64 target = U < (double)all ? min((u64)U, all - 1) : all - 1;
-  if (before <= target && target < before + mine) {
-    const u64 i = part_mass(target, true, before);
-    if (lane == 0) p.out[row] = (long long)i;
+  for (int i = tid * share; i < min(rows, (tid + 1) * share); ++i) {
+    if (run <= target && target < run + sChunk[i]) {
+      sPick[0] = (u64)i;
+      sPick[1] = run;
+    }
+    run += sChunk[i];
+  }
+  __syncthreads();
+  // ---- and the token ----
+  const int hit = (int)sPick[0];
+  if (hit / per_wave == wave) {
+    const int c = hit % per_wave;
+    const dkv_u32x4 v = load_again(c);
+    const int i0 = first_of(c);
+    u64 w[E], s = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += w[e] = (u64)mass_of(value(v, e), i0 + e);
+    u64 at = sPick[1] + sm_wave_scan(s, lane) - s;
+    if (at <= target && target < at + s) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (at <= target && target < at + w[e]) p.out[row] = (long long)(i0 + e);
+        at += w[e];
+      }
+    }
   }
 }
 
