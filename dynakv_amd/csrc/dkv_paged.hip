@@ -254,8 +254,8 @@ __device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
 // and V (4 KB each) lands in its own part of LDS by direct-to-LDS loads, 16-byte pieces XOR-swizzled
 // by token, the next tile's loads in flight meanwhile; the resource of a load ends with the request's
 // tokens, so slots behind them read as zero and cost nothing. S^T = K Q^T and P V on 16x16x32 MFMA
-// with the rows in the operand's columns; the weights go to the products as bf16 hi + lo pairs
-// (fp16: as fp16), 16 tokens filling 32 deep products. Waves are joined in LDS, parts by the
+// with the rows in the operand's columns; the weights go to the products as 16-bit hi + lo
+// pairs, which the 32 deep products of 16 tokens have room for. Waves are joined in LDS, parts by the
 // unit's last one to arrive.
 //
 // How a step's units are cut: requests have any lengths, which only the device knows, and the launch
@@ -483,7 +483,11 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
       dkv_split_bf16x2(pu[2], pu[3], h23, l23);
       pa = dkv_u32x4{h01, h23, l01, l23};
     } else {
-      pa = dkv_u32x4{dkv_pack_f16x2(pu[0], pu[1]), dkv_pack_f16x2(pu[2], pu[3]), 0u, 0u};
+      float lo[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) lo[u] = pu[u] - (float)(_Float16)pu[u];
+      pa = dkv_u32x4{dkv_pack_f16x2(pu[0], pu[1]), dkv_pack_f16x2(pu[2], pu[3]),
+                     dkv_pack_f16x2(lo[0], lo[1]), dkv_pack_f16x2(lo[2], lo[3])};
     }
     const int vtok = 4 * g + (n >> 2);
     dkv_u32x2 xv[8];
@@ -1149,10 +1153,20 @@ struct AttendPlan {
   long long floats;        // workspace (0: none)
 };
 
-// The shape of the many-row kernel by the number of 128-row workgroups, as the prefill attention's:
-// more than two rounds of the 512 that fit the chip take two row blocks per wave, up to that one
-// block and 8 waves, one workgroup per CU or fewer 64 rows. Fewer 64-row workgroups than CUs: the
-// keys of each are cut into ranges of at least 4 tiles.
+// The shape of the many-row kernel, by the workgroups that the rows fill (rows that the host counts
+// as if requests' tiles were full; 512 workgroups fit the chip at a time, 256 of 8 waves), and the key
+// tiles of the longest request. us on MI355X, bf16, 32 query and 8 KV heads; shape: row blocks x
+// waves / key ranges (workgroups):
+//  * more than 1024 of 128 rows: 2x4, each key operand read from LDS serves two products. Four
+//    2048-token prompts 169 2x4/1, 178 1x8/1, 213 1x4/1.
+//  * up to 256 of 128 rows and long keys: ranges that fill the chip once, at least 24 tiles each.
+//    512 tokens at 8192: 88.8 2x4/4 (512), 102 2x4/3, 105 1x4/2, 173 1x4/1. 846 tokens of two
+//    requests at up to 6001: 103 2x4/2, 109 2x4/4, 125 1x4/1.
+//  * so few rows that 64-row tiles, too, leave half the chip idle: those, ranges of 8 tiles or more.
+//    64 tokens at 32768: 73 1x4/16, 82 2x4/16. 200 at 2000: 29.7 1x4/4, 31.5 1x4/2, 35.0 1x4/5 (520).
+//  * otherwise one range: above 256 of 128 rows 1x8 (eight 300-token prompts 25.6, against 27.1 1x4,
+//    28.3 2x4), else 1x4 (512 tokens at 1024: 22.6, against 27.0 1x8 and 36 2x4/2: a range more
+//    costs its records, 66 KB a workgroup, written and read).
 AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, int max_len) {
   AttendPlan a = {};
   const int hpg = Hq / Hkv;
@@ -1177,19 +1191,29 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
       const long long x = rows / bq + B, y = each * B;
       return x < y ? x : y;
     };
-    const long long wg128 = items(128) * Hkv;
-    a.qb = wg128 > 1024 ? 2 : 1;
-    a.nw = wg128 > 1024 ? 4 : wg128 > 256 ? 8 : 4;
+    const long long tiles = ((long long)max_len + CK - 1) / CK;
+    auto full = [&](int bq) {  // workgroups of full tiles
+      const long long x = ((long long)T * hpg + bq - 1) / bq, y = items(bq);
+      return (x < y ? x : y) * Hkv;
+    };
+    const long long wg128 = full(128), wg64 = full(64);
+    auto ranges = [&](long long wgs, long long least) {
+      const long long n = 512 / wgs, most = (tiles + least / 2) / least;
+      return (int)(n < most ? n : most);
+    };
+    a.splits = 1;
+    if (wg128 > 1024) {
+      a.qb = 2, a.nw = 4;
+    } else if (wg64 >= 256 && wg128 <= 256 && ranges(wg128, 24) > 1) {
+      a.qb = 2, a.nw = 4, a.splits = ranges(wg128, 24);
+    } else if (wg64 < 256 && ranges(wg64, 8) > 1) {
+      a.qb = 1, a.nw = 4, a.splits = ranges(wg64, 8);
+    } else {
+      a.qb = 1, a.nw = wg128 > 256 ? 8 : 4;
+    }
     a.bq = 16 * a.qb * a.nw;
     a.items = (int)items(a.bq);
-    a.splits = 1;
     const long long wgs = (long long)a.items * Hkv;
-    if (a.bq == 64 && wgs < 256) {
-      const long long tiles = ((long long)max_len + CK - 1) / CK;
-      long long n = (512 + wgs - 1) / wgs;
-      if (n > tiles / 4) n = tiles / 4;
-      a.splits = (int)(n < 1 ? 1 : n);
-    }
     if (a.splits > 1) {
       const long long f = wgs * a.splits * a.bq * (PG_DH + 2);
       if (f > floats) floats = f;
