@@ -43,11 +43,8 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedPool& pool, con
   return r;
 }
 
-// The same, for a request that is the whole wave's: in scalar registers.
-__device__ __forceinline__ PagedRequest paged_request_uniform(const PagedPool& pool,
-                                                              const int* q_start, const int* lens,
-                                                              int b, int T) {
-  PagedRequest r = paged_request(pool, q_start, lens, b, T);
+// The same in scalar registers, for a request that is the whole wave's.
+__device__ __forceinline__ PagedRequest uniform(PagedRequest r) {
   r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
   r.n = __builtin_amdgcn_readfirstlane(r.n);
   r.len = __builtin_amdgcn_readfirstlane(r.len);
@@ -224,16 +221,25 @@ struct AttendParams {
   float* records;    // split records
   int* counters;     // arrival counters, zero between calls
   int split;         // whether a request's keys may be split among workgroups
+  int out_wide;      // output rows begin at multiples of four values, aligned as such
 };
 
 // 16 bytes at byte offset `off` of a buffer resource into LDS at M0 + 16 * lane (inline assembly so
 // that the compiler neither moves LDS accesses across it nor waits for it before later LDS reads;
 // the kernels wait for these loads themselves).
+// ONCE: data that no other workgroup reads, passed by the caches (two requests of 65533 tokens, single
+// new ones: 89 us, 6.0 TB/s, against 101 us without; 16 of 8192: 88 against 101).
+template <bool ONCE>
 __device__ __forceinline__ void pg_lds_load16(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_base,
                                               uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               ::"s"(lds_base), "v"(off), "s"(rsrc)
-               : "memory", "m0");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+                 ::"s"(lds_base), "v"(off), "s"(rsrc)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 ::"s"(lds_base), "v"(off), "s"(rsrc)
+                 : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void pg_wait_vm() {
@@ -261,7 +267,6 @@ __device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
 // How a step's units are cut: requests have any lengths, which only the device knows, and the launch
 // has a fixed number of workgroups. Every wave finds the smallest part C (tiles) for which
 // sum over units of ceil(tiles / C) parts fit the launch, and takes its own from the running sums.
-constexpr int DW = 4;                       // waves per workgroup
 constexpr int DSLOT = 2;                    // tile slots per wave
 constexpr int DTILE = 16;
 constexpr int DTILE_BYTES = DTILE * PG_DH * 2;
@@ -270,40 +275,44 @@ constexpr int DROWS = 16;
 constexpr int DREC = DROWS * (PG_DH + 2);   // floats of a record: m, l and acc[128] of 16 rows
 constexpr int D_COUNTERS = 16384;           // leading workspace ints
 constexpr int D_SPLIT_B = 256;              // requests a wave can hold the lengths of (4 a lane)
-constexpr int D_WGS = 512;                  // two workgroups per CU
-constexpr int D_MIN_TILES = 2 * DW;         // least part
+constexpr int D_WGS = 256;                  // workgroups of 8 waves: one per CU
+constexpr int D_MIN_TILES = 16;             // least part
 constexpr float D_RESCALE = 11.5f;          // log2 units the running maximum may be exceeded by
 
 __device__ __forceinline__ int pg_wave_sum(int v) { return dkv_wave_sum_fast_i(v); }
 
-template <int DT, int ODT>
-__global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
-  __shared__ __attribute__((aligned(256))) uint8_t sRing[DW * DSLOT * DSLOT_BYTES];
-  __shared__ int sLast;
+// Workgroup `wg` of `wgs`, of DW waves; `sRing`: DW * DSLOT * DSLOT_BYTES of LDS, `sLast` an int of it.
+template <int DT, int ODT, int DW>
+__device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs, uint8_t* sRing,
+                                         int* sLast) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
 
   // tiles of a request's keys; 0 for one without rows or with too many
-  auto tiles_of = [&](int b) {
-    if (b >= p.B) return 0;
-    const PagedRequest r = paged_request(p.pool, p.q_start, p.lens, b, p.T);
+  auto tiles_of = [&](const PagedRequest& r) {
     if (r.n <= 0 || r.n * p.hpg > DROWS) return 0;
     return max(1, (r.len + DTILE - 1) / DTILE);
   };
+  PagedRequest r;
   int b, kvh, part = 0, parts = 1, first = 0;
   if (p.split) {
+    PagedRequest rs[D_SPLIT_B / 64];
     int t[D_SPLIT_B / 64], total = 0, units = 0;
     const int used = (p.B + 63) / 64;
 #pragma unroll
     for (int j = 0; j < D_SPLIT_B / 64; ++j) {
-      t[j] = j < used ? tiles_of(64 * j + lane) : 0;
+      t[j] = 0;
+      if (64 * j + lane < p.B) {
+        rs[j] = paged_request(p.pool, p.q_start, p.lens, 64 * j + lane, p.T);
+        t[j] = tiles_of(rs[j]);
+      }
       total += t[j];
       units += t[j] > 0;
     }
     total = pg_wave_sum(total) * p.Hkv;
     units = pg_wave_sum(units) * p.Hkv;
-    const int G = gridDim.x;  // at least the units
+    const int G = wgs;  // at least the units
     // parts of size c; the same in every wave of the launch, whatever the rounding
     auto parts_of = [&](int tiles, float inv) {
       return tiles > 0 ? max(1, (int)((float)tiles * inv + 0.999f)) : 0;
@@ -346,12 +355,16 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
         const int x = __shfl_up(run, o, 64);
         if (lane >= o) run += x;
       }
-      const unsigned long long hit = __ballot((int)blockIdx.x < base + run);
+      const unsigned long long hit = __ballot(wg < base + run);
       if (hit) {
         const int l = __ffsll((long long)hit) - 1;
         b = 64 * j + l;
         first = base + __shfl(run - s, l, 64);
         parts = __shfl(s, l, 64) / p.Hkv;
+        r.row0 = __shfl(rs[j].row0, l, 64);
+        r.n = __shfl(rs[j].n, l, 64);
+        r.len = __shfl(rs[j].len, l, 64);
+        r.pos0 = __shfl(rs[j].pos0, l, 64);
       } else {
         base += __shfl(run, 63, 64);
       }
@@ -360,17 +373,18 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
     if (b < 0) return;
     first = __builtin_amdgcn_readfirstlane(first);
     parts = __builtin_amdgcn_readfirstlane(parts);
-    const int rel = (int)blockIdx.x - first;
+    const int rel = wg - first;
     kvh = rel / parts;
     part = rel % parts;
     first += kvh * parts;
   } else {
-    b = blockIdx.x / p.Hkv;
-    kvh = blockIdx.x % p.Hkv;
+    b = wg / p.Hkv;
+    kvh = wg % p.Hkv;
+    r = paged_request(p.pool, p.q_start, p.lens, b, p.T);
   }
-  const int n_all = __builtin_amdgcn_readfirstlane(tiles_of(b));
+  r = uniform(r);
+  const int n_all = tiles_of(r);
   if (n_all == 0) return;
-  const PagedRequest r = paged_request_uniform(p.pool, p.q_start, p.lens, b, p.T);
   const int rows = r.n * p.hpg;
   const int per = (n_all + parts - 1) / parts;
   const int t_begin = part * per, t_end = min(n_all, t_begin + per);
@@ -384,16 +398,14 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
     const int t = 4 * i + (lane >> 4);
     piece_off[i] = (uint32_t)(t * 256 + 16 * ((lane & 15) ^ t));
   }
-  int ids = -1;  // lane l: the page of the wave's tile l of the current 64
-  auto fetch_ids = [&](int j) {
-    const int t = tix(j + lane);
-    ids = t < t_end ? paged_page(p.pool, b, t * DTILE) : -1;
-  };
-  auto page_at = [&](int j) { return __builtin_amdgcn_readlane(ids, j & 63); };
-  auto issue = [&](int j) {
-    if (j >= n_iter) return;
-    if ((j & 63) == 0) fetch_ids(j);
-    const int page = page_at(j), tok = tix(j) * DTILE;
+  int ids = -1;  // lane l: the page of the wave's tile l of the 64 being issued
+  auto issue = [&](int j) {  // the tile's loads; returns its page (scalar)
+    if (j >= n_iter) return -1;
+    if ((j & 63) == 0) {
+      const int t = tix(j + lane);
+      ids = t < t_end ? paged_page(p.pool, b, t * DTILE) : -1;
+    }
+    const int page = __builtin_amdgcn_readlane(ids, j & 63), tok = tix(j) * DTILE;
     const long long at = (long long)max(page, 0) * p.pool.page_stride +
                          (long long)kvh * p.pool.head_stride +
                          (long long)(tok & (p.pool.page_size - 1)) * PG_DH;
@@ -402,13 +414,14 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
     const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc(p.v + at, bytes);
     const uint32_t slot = dkv_lds_addr(ring + (j % DSLOT) * DSLOT_BYTES);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pg_lds_load16(rk, slot + 1024 * i, piece_off[i]);
+    for (int i = 0; i < 4; ++i) pg_lds_load16<true>(rk, slot + 1024 * i, piece_off[i]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pg_lds_load16(rv, slot + DTILE_BYTES + 1024 * i, piece_off[i]);
+    for (int i = 0; i < 4; ++i) pg_lds_load16<true>(rv, slot + DTILE_BYTES + 1024 * i, piece_off[i]);
+    return page;
   };
-  int ids_now = -1;  // the ids that the tile being worked on belongs to
-  issue(0);
-  ids_now = ids;
+  int pages[DSLOT];  // of tiles j, j + 1, ...
+#pragma unroll
+  for (int i = 0; i + 1 < DSLOT; ++i) pages[i] = issue(i);
 
   // query operand: column n = row n (new token n / hpg, head n % hpg; rows past the request's
   // zero), dims 32c + 8g .. +8
@@ -433,10 +446,14 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
   float m_run = -1.0e30f, l_run = 0.f;  // log2 units; a finite floor: exp2(-inf - floor) is 0
 
   for (int j = 0; j < n_iter; ++j) {
-    pg_wait_vm<0>();  // tile j
-    if ((j & 63) == 0) ids_now = ids;
-    const int page = __builtin_amdgcn_readlane(ids_now, j & 63);
-    issue(j + 1);
+    if (DSLOT == 3 && j + 1 < n_iter)
+      pg_wait_vm<8>();  // tile j, while tile j + 1's loads are on their way
+    else
+      pg_wait_vm<0>();
+    const int page = pages[0];
+#pragma unroll
+    for (int i = 0; i + 2 < DSLOT; ++i) pages[i] = pages[i + 1];
+    pages[DSLOT - 2] = issue(j + DSLOT - 1);
     const uint8_t* slot = ring + (j % DSLOT) * DSLOT_BYTES;
     const int key0 = tix(j) * DTILE;
     dkv_u32x4 xk[4];
@@ -576,18 +593,20 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
     }
     return;
   }
-  // this part's record: per row m, l, acc[128]
-  float* rec = p.records + (long long)blockIdx.x * DREC;
-  for (int idx = tid; idx < rows * PG_DH; idx += 64 * DW) {
-    const int row = idx / PG_DH, d = idx % PG_DH;
+  // This part's record: per row m and l, then acc[128], as pairs (8-byte accesses that all XCDs see).
+  auto put = [&](float* a, float x, float y) {
+    __hip_atomic_store((unsigned long long*)a,
+                       __float_as_uint(x) | ((unsigned long long)__float_as_uint(y) << 32),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  float* rec = p.records + (long long)wg * DREC;
+  for (int idx = tid; idx < rows * (PG_DH / 2); idx += 64 * DW) {
+    const int row = idx / (PG_DH / 2), d = 2 * (idx % (PG_DH / 2));
     float M, L;
-    const float A = joined(row, d, M, L);
+    const float x = joined(row, d, M, L), y = joined(row, d + 1, M, L);
     float* rr = rec + row * (PG_DH + 2);
-    __hip_atomic_store(rr + 2 + d, A, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (d == 0) {
-      __hip_atomic_store(rr, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(rr + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    put(rr + 2 + d, x, y);
+    if (d == 0) put(rr, M, L);
   }
   // ---- the unit's last part to arrive joins the parts ----
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -595,39 +614,51 @@ __global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
   if (tid == 0) {
     const int old = __hip_atomic_fetch_add(p.counters + b * p.Hkv + kvh, 1, __ATOMIC_RELAXED,
                                            __HIP_MEMORY_SCOPE_AGENT);
-    sLast = old == parts - 1;
+    *sLast = old == parts - 1;
   }
   __syncthreads();
-  if (!sLast) return;
+  if (!*sLast) return;
   const float* recs = p.records + (long long)first * DREC;
-  auto ld = [&](const float* a) {
-    return __hip_atomic_load(a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  auto get = [&](const float* a) {
+    return __hip_atomic_load((const unsigned long long*)a, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
   };
-  for (int idx = tid; idx < rows * PG_DH; idx += 64 * DW) {
-    const int row = idx / PG_DH, d = idx % PG_DH;
-    float M = -INFINITY, L = 0.f, A = 0.f;
-    for (int s0 = 0; s0 < parts; s0 += 8) {
-      float mb[8], lb[8], xb[8];
+  constexpr int AHEAD = 8;  // parts whose loads are on their way together
+  for (int idx = tid; idx < rows * (PG_DH / 2); idx += 64 * DW) {
+    const int row = idx / (PG_DH / 2), d = 2 * (idx % (PG_DH / 2));
+    float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += AHEAD) {
+      unsigned long long ml[AHEAD], xy[AHEAD];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float* rr = recs + (long long)min(s0 + u, parts - 1) * DREC + row * (PG_DH + 2);
-        mb[u] = ld(rr);
-        lb[u] = ld(rr + 1);
-        xb[u] = ld(rr + 2 + d);
+      for (int u = 0; u < AHEAD; ++u) {
+        if (s0 + u >= parts) break;
+        const float* rr = recs + (long long)(s0 + u) * DREC + row * (PG_DH + 2);
+        ml[u] = get(rr);
+        xy[u] = get(rr + 2 + d);
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < AHEAD; ++u) {
         if (s0 + u >= parts) break;
-        const float Mn = fmaxf(M, mb[u]);
-        const float so = exp2f(M - Mn), sn = exp2f(mb[u] - Mn);
-        L = L * so + lb[u] * sn;
-        A = A * so + xb[u] * sn;
+        const float mu = __uint_as_float((uint32_t)ml[u]);
+        const float Mn = fmaxf(M, mu);
+        const float so = exp2f(M - Mn), sn = exp2f(mu - Mn);
+        L = L * so + __uint_as_float((uint32_t)(ml[u] >> 32)) * sn;
+        A0 = A0 * so + __uint_as_float((uint32_t)xy[u]) * sn;
+        A1 = A1 * so + __uint_as_float((uint32_t)(xy[u] >> 32)) * sn;
         M = Mn;
       }
     }
-    store(row, d, A, L);
+    store(row, d, A0, L);
+    store(row, d + 1, A1, L);
   }
   if (tid == 0) p.counters[b * p.Hkv + kvh] = 0;
+}
+
+template <int DT, int ODT>
+__global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t sRing[8 * DSLOT * DSLOT_BYTES];
+  __shared__ int sLast;
+  few_rows<DT, ODT, 8>(p, blockIdx.x, gridDim.x, sRing, &sLast);
 }
 
 // ---- many rows: prompts and their chunks ----
@@ -649,21 +680,24 @@ constexpr float C_RESCALE = 8.f;            // log2 units
 
 struct ChunkParams {
   AttendParams a;
+  float* records;
   int bq, splits, few_rows;  // rows of a workgroup; key ranges; rows up to which the other kernel works
 };
 
 // The work item of a workgroup: row tile `rt` of request b. Items are counted request by request,
 // a request's later rows (with more keys) first.
 struct ChunkItem {
-  int b, rt, tiles;
+  int b, rt;  // b < 0: none
+  PagedRequest r;
 };
 __device__ __forceinline__ ChunkItem chunk_item(const ChunkParams& p, int item, int lane) {
   const AttendParams& a = p.a;
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     int t = 0;
+    PagedRequest r = {0, 0, 0, 0};
     if (b0 + lane < a.B) {
-      const PagedRequest r = paged_request(a.pool, a.q_start, a.lens, b0 + lane, a.T);
+      r = paged_request(a.pool, a.q_start, a.lens, b0 + lane, a.T);
       const long long rows = (long long)r.n * a.hpg;
       t = r.n > 0 && rows > p.few_rows ? (int)((rows + p.bq - 1) / p.bq) : 0;
     }
@@ -678,14 +712,35 @@ __device__ __forceinline__ ChunkItem chunk_item(const ChunkParams& p, int item, 
       const int l = __ffsll((long long)hit) - 1;
       ChunkItem it;
       it.b = __builtin_amdgcn_readfirstlane(b0 + l);
-      it.tiles = __builtin_amdgcn_readfirstlane(__shfl(t, l, 64));
-      const int before = base + __shfl(run - t, l, 64);
-      it.rt = __builtin_amdgcn_readfirstlane(it.tiles - 1 - (item - before));
+      it.rt = __builtin_amdgcn_readfirstlane(base + __shfl(run, l, 64) - 1 - item);
+      it.r.row0 = __shfl(r.row0, l, 64);
+      it.r.n = __shfl(r.n, l, 64);
+      it.r.len = __shfl(r.len, l, 64);
+      it.r.pos0 = __shfl(r.pos0, l, 64);
+      it.r = uniform(it.r);
       return it;
     }
     base += __shfl(run, 63, 64);
   }
-  return ChunkItem{-1, 0, 0};
+  return ChunkItem{-1, 0, {0, 0, 0, 0}};
+}
+
+// Four neighbouring values of the output, as one store where its rows allow it.
+template <int ODT>
+__device__ __forceinline__ void store4(const AttendParams& p, long long at, dkv_f32x4 v) {
+  if (!p.out_wide) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) dkv_store_f32<ODT>(p.out, at + u, v[u]);
+  } else if constexpr (ODT == DKV_F32) {
+    *(dkv_f32x4*)((float*)p.out + at) = v;
+  } else if constexpr (ODT == DKV_BF16) {
+    *(dkv_u32x2*)((uint16_t*)p.out + at) =
+        dkv_u32x2{dkv_f32_to_bf16_bits(v[0]) | (dkv_f32_to_bf16_bits(v[1]) << 16),
+                  dkv_f32_to_bf16_bits(v[2]) | (dkv_f32_to_bf16_bits(v[3]) << 16)};
+  } else {
+    *(dkv_u32x2*)((uint16_t*)p.out + at) =
+        dkv_u32x2{dkv_pack_f16x2(v[0], v[1]), dkv_pack_f16x2(v[2], v[3])};
+  }
 }
 
 __device__ __forceinline__ float pg_max4(float x) {  // over lanes n, n + 16, n + 32, n + 48
@@ -735,26 +790,28 @@ __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, i
   }
 }
 
+// Workgroup `wg`; `sKV`: 4 * CTILE_BYTES of LDS, 1 KB aligned (the operand reads form their
+// addresses by exclusive-or): two K tiles, two V tiles.
 template <int DT, int ODT, int QB, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(ChunkParams c) {
+__device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t* sKV) {
   constexpr int QW = 16 * QB;            // rows per wave
   constexpr int BQ = NW * QW;            // rows per workgroup
   constexpr int LW = CK / 4 / NW;        // K (or V) loads per wave and tile, 4 keys each
-  __shared__ __attribute__((aligned(1024))) uint8_t sK[2][CTILE_BYTES];
-  __shared__ __attribute__((aligned(1024))) uint8_t sV[2][CTILE_BYTES];
+  auto sK = [&](int i) { return sKV + i * CTILE_BYTES; };
+  auto sV = [&](int i) { return sKV + (2 + i) * CTILE_BYTES; };
   const AttendParams& p = c.a;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   // the KV head runs fastest: workgroups go to the 8 XCDs in turn, so that a head's keys and values
   // stay in one L2 (for 8 heads, or a multiple)
-  const int kvh = __builtin_amdgcn_readfirstlane(blockIdx.x % p.Hkv);
-  const int rest = blockIdx.x / p.Hkv;
+  const int kvh = __builtin_amdgcn_readfirstlane(wg % p.Hkv);
+  const int rest = wg / p.Hkv;
   const int split = rest % c.splits;
   const ChunkItem it = chunk_item(c, rest / c.splits, lane);
   const int b = __builtin_amdgcn_readfirstlane(it.b);
   if (b < 0) return;
-  const PagedRequest r = paged_request_uniform(p.pool, p.q_start, p.lens, b, p.T);
+  const PagedRequest r = uniform(it.r);
   const int rows = r.n * p.hpg;
   const int q0 = __builtin_amdgcn_readfirstlane(it.rt) * BQ;
   const int wq0 = q0 + QW * wave;  // the wave's first row
@@ -815,12 +872,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(C
         page < 0 ? 0 : min(max(k_end - key, 0), CK / NW));  // (a vector instruction clamps)
     const __amdgpu_buffer_rsrc_t rk = dkv_make_rsrc(p.k + at, (uint32_t)cnt * (PG_DH * 2));
     const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc(p.v + at, (uint32_t)cnt * (PG_DH * 2));
-    const uint32_t dk = dkv_lds_addr(sK[t & 1]) + CK / NW * wave * 256;
-    const uint32_t dv = dkv_lds_addr(sV[t & 1]) + CK / NW * wave * 256;
+    const uint32_t dk = dkv_lds_addr(sK(t & 1)) + CK / NW * wave * 256;
+    const uint32_t dv = dkv_lds_addr(sV(t & 1)) + CK / NW * wave * 256;
 #pragma unroll
-    for (int i = 0; i < LW; ++i) pg_lds_load16(rk, dk + 1024 * i, voff[i]);
+    for (int i = 0; i < LW; ++i) pg_lds_load16<false>(rk, dk + 1024 * i, voff[i]);
 #pragma unroll
-    for (int i = 0; i < LW; ++i) pg_lds_load16(rv, dv + 1024 * i, voff[i]);
+    for (int i = 0; i < LW; ++i) pg_lds_load16<false>(rv, dv + 1024 * i, voff[i]);
   };
 
   dkv_f32x4 acc[QB][8];
@@ -860,8 +917,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(C
     }
     const int key0 = t * CK;
     if (key0 >= w_end) continue;  // every key of the tile is past the wave's rows
-    const uint32_t kt = dkv_lds_addr(sK[t & 1]);
-    const uint32_t vt = dkv_lds_addr(sV[t & 1]) + vrd;
+    const uint32_t kt = dkv_lds_addr(sK(t & 1));
+    const uint32_t vt = dkv_lds_addr(sV(t & 1)) + vrd;
     dkv_f32x4 z[QB][4];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
@@ -960,9 +1017,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(C
     }
   }
 
-  // acc rows are dims, columns rows of the request: lane (row n, g) holds dims 16db + 4g + u
-  float* rec0 = p.records + ((long long)(rest / c.splits * p.Hkv + kvh) * c.splits + split) * BQ *
-                                (PG_DH + 2);
+  // acc rows are dims, columns rows of the request: lane (row n, g) holds dims 16db + 4g + u. A
+  // range's record: acc[BQ][128], then m and l of each row.
+  float* rec = c.records + ((long long)(rest / c.splits * p.Hkv + kvh) * c.splits + split) * BQ *
+                               (PG_DH + 2);
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     float l = l_run[qb];
@@ -986,20 +1044,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(C
                              (long long)(kvh * p.hpg + h) * p.o_sh;
 #pragma unroll
         for (int db = 0; db < 8; ++db)
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            dkv_store_f32<ODT>(p.out, ob + 16 * db + 4 * g + u, acc[qb][db][u] * inv);
+          store4<ODT>(p, ob + 16 * db + 4 * g, acc[qb][db] * inv);
       }
     } else if (good) {
-      float* rec = rec0 + (long long)(QW * wave + 16 * qb + n) * (PG_DH + 2);
-      if (g == 0) {
-        rec[0] = m_run[qb];
-        rec[1] = l;
-      }
+      const int x = QW * wave + 16 * qb + n;
+      if (g == 0) *(float2*)(rec + BQ * PG_DH + 2 * x) = float2{m_run[qb], l};
 #pragma unroll
       for (int db = 0; db < 8; ++db)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) rec[2 + 16 * db + 4 * g + u] = acc[qb][db][u];
+        *(dkv_f32x4*)(rec + x * PG_DH + 16 * db + 4 * g) = acc[qb][db];
     }
     while (bad) {  // rows with an infinity or NaN, key by key
       const int x = __ffsll((long long)bad) - 1;
@@ -1017,53 +1069,74 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(C
         dkv_store_f32<ODT>(p.out, ob, o0 * inv);
         dkv_store_f32<ODT>(p.out, ob + 1, o1 * inv);
       } else {
-        float* rec = rec0 + (long long)(QW * wave + 16 * qb + x) * (PG_DH + 2);
-        if (lane == 0) {
-          rec[0] = mx;
-          rec[1] = lx;
-        }
-        rec[2 + 2 * lane] = o0;
-        rec[3 + 2 * lane] = o1;
+        const int y = QW * wave + 16 * qb + x;
+        if (lane == 0) *(float2*)(rec + BQ * PG_DH + 2 * y) = float2{mx, lx};
+        *(float2*)(rec + y * PG_DH + 2 * lane) = float2{o0, o1};
       }
     }
   }
 }
 
-// The key ranges' records of one row joined: one wave per row, lane l dims 2l, 2l + 1.
+template <int DT, int ODT, int QB, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(ChunkParams c) {
+  __shared__ __attribute__((aligned(1024))) uint8_t sKV[4 * CTILE_BYTES];
+  many_rows<DT, ODT, QB, NW>(c, blockIdx.x, sKV);
+}
+
+// Both kinds of requests in one launch: the ones of few rows, bound by memory, beside the others,
+// bound by their products. Workgroups of the two kinds are handed out in turn, so that a CU has one of
+// each.
+template <int DT, int ODT, int QB>
+__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(ChunkParams c, int few, int many) {
+  static_assert(4 * DSLOT * DSLOT_BYTES <= 4 * CTILE_BYTES, "one workgroup shape");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * CTILE_BYTES];
+  __shared__ int sLast;
+  const int x = blockIdx.x, both = 2 * min(few, many);
+  const int i = x < both ? x >> 1 : x - both / 2;
+  if (x < both ? (x & 1) == 0 : few > many)
+    few_rows<DT, ODT, 4>(c.a, i, few, smem, &sLast);
+  else
+    many_rows<DT, ODT, QB, 4>(c, i, smem);
+}
+
+// The key ranges' records of a row joined: 32 rows per workgroup, 8 threads of 16 dims each.
 template <int DT, int ODT>
 __global__ __launch_bounds__(256) void paged_join_kernel(ChunkParams c) {
   const AttendParams& p = c.a;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int groups = c.bq / 4;  // workgroups per (item, KV head)
-  const int x = blockIdx.x * 4 + wave;
-  const int ik = blockIdx.x / groups, row = x % c.bq;
+  const int groups = c.bq / 32;  // workgroups per (item, KV head)
+  const int ik = blockIdx.x / groups;
+  const int row = blockIdx.x % groups * 32 + (threadIdx.x >> 3), d0 = 4 * (threadIdx.x & 7);
+  const float* rec = c.records + (long long)ik * c.splits * c.bq * (PG_DH + 2);
+  const long long step = (long long)c.bq * (PG_DH + 2);
   const int kvh = ik % p.Hkv;
-  const ChunkItem it = chunk_item(c, ik / p.Hkv, lane);
+  const ChunkItem it = chunk_item(c, ik / p.Hkv, threadIdx.x & 63);
   if (it.b < 0) return;
-  const PagedRequest r = paged_request(p.pool, p.q_start, p.lens, it.b, p.T);
+  const PagedRequest& r = it.r;
   const int R = it.rt * c.bq + row;
   if (R >= r.n * p.hpg) return;
-  const float* rec = p.records + (long long)ik * c.splits * c.bq * (PG_DH + 2) +
-                     (long long)row * (PG_DH + 2);
-  const long long step = (long long)c.bq * (PG_DH + 2);
-  float M = -1.0e30f;
-  for (int s = 0; s < c.splits; ++s) M = fmaxf(M, rec[s * step]);
-  float L = 0.f, a0 = 0.f, a1 = 0.f;
+  float M = -1.0e30f, L = 0.f;
+  dkv_f32x4 a[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) a[q] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < c.splits; ++s) {
-    const float* q = rec + s * step;
-    const float l = q[1];
-    if (l == 0.f) continue;  // a range without keys for the row
-    const float w = exp2f(q[0] - M);
-    L += w * l;
-    a0 += w * q[2 + 2 * lane];
-    a1 += w * q[3 + 2 * lane];
+    const float2 ml = *(const float2*)(rec + s * step + c.bq * PG_DH + 2 * row);
+    dkv_f32x4 x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      x[q] = *(const dkv_f32x4*)(rec + s * step + row * PG_DH + 32 * q + d0);
+    if (ml.y == 0.f) continue;  // a range without keys for the row
+    const float Mn = fmaxf(M, ml.x), so = exp2f(M - Mn), sn = exp2f(ml.x - Mn);
+    M = Mn;
+    L = L * so + ml.y * sn;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) a[q] = a[q] * so + x[q] * sn;
   }
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
   const int i = R / p.hpg, h = R - i * p.hpg;
   const long long ob = (long long)(r.row0 + i) * p.o_st +
-                       (long long)(kvh * p.hpg + h) * p.o_sh + 2 * lane;
-  dkv_store_f32<ODT>(p.out, ob, a0 * inv);
-  dkv_store_f32<ODT>(p.out, ob + 1, a1 * inv);
+                       (long long)(kvh * p.hpg + h) * p.o_sh + d0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) store4<ODT>(p, ob + 32 * q, a[q] * inv);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -1150,6 +1223,7 @@ struct AttendPlan {
   bool few, many;          // kernels that run
   int few_wgs, few_split;
   int qb, nw, bq, items, splits;
+  long long many_at;       // the many-row kind's records, in floats from the others'
   long long floats;        // workspace (0: none)
 };
 
@@ -1172,8 +1246,8 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
   const int hpg = Hq / Hkv;
   const long long units = (long long)B * Hkv;
   a.few = (long long)(min_new > 1 ? min_new : 1) * hpg <= DROWS;
-  a.many = (long long)max_new * hpg > DROWS;
   long long floats = 0;
+  a.many = (long long)max_new * hpg > DROWS;
   if (a.few) {
     const long long tiles = ((long long)max_len + DTILE - 1) / DTILE;
     const long long most = units * ((tiles + D_MIN_TILES - 1) / D_MIN_TILES);
@@ -1198,7 +1272,7 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
     };
     const long long wg128 = full(128), wg64 = full(64);
     auto ranges = [&](long long wgs, long long least) {
-      const long long n = 512 / wgs, most = (tiles + least / 2) / least;
+      const long long n = (a.few ? 256 : 512) / wgs, most = (tiles + least / 2) / least;
       return (int)(n < most ? n : most);
     };
     a.splits = 1;
@@ -1209,14 +1283,14 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
     } else if (wg64 < 256 && ranges(wg64, 8) > 1) {
       a.qb = 1, a.nw = 4, a.splits = ranges(wg64, 8);
     } else {
-      a.qb = 1, a.nw = wg128 > 256 ? 8 : 4;
+      a.qb = 1, a.nw = wg128 > 256 && !a.few ? 8 : 4;
     }
     a.bq = 16 * a.qb * a.nw;
     a.items = (int)items(a.bq);
     const long long wgs = (long long)a.items * Hkv;
-    if (a.splits > 1) {
-      const long long f = wgs * a.splits * a.bq * (PG_DH + 2);
-      if (f > floats) floats = f;
+    if (a.splits > 1) {  // its records behind the other kind's
+      a.many_at = (floats + 3) / 4 * 4;
+      floats = a.many_at + wgs * a.splits * a.bq * (PG_DH + 2);
     }
   }
   a.floats = floats ? D_COUNTERS + floats : 0;
@@ -1225,20 +1299,29 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
 
 template <int DT, int ODT>
 void launch_attend(const AttendPlan& a, const ChunkParams& c, hipStream_t st) {
-  if (a.few)
-    hipLaunchKernelGGL((paged_few_kernel<DT, ODT>), dim3((unsigned)a.few_wgs), dim3(64 * DW), 0, st,
-                       c.a);
-  if (!a.many) return;
-  const dim3 grid((unsigned)(a.items * c.a.Hkv * a.splits));
-  if (a.qb == 2)
-    hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 2, 4>), grid, dim3(256), 0, st, c);
-  else if (a.nw == 8)
-    hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 8>), grid, dim3(512), 0, st, c);
-  else
-    hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 4>), grid, dim3(256), 0, st, c);
-  if (a.splits > 1)
+  const int many = a.items * c.a.Hkv * a.splits;
+  if (a.few && a.many) {
+    const dim3 grid((unsigned)(a.few_wgs + many));
+    if (a.qb == 2)
+      hipLaunchKernelGGL((paged_mixed_kernel<DT, ODT, 2>), grid, dim3(256), 0, st, c, a.few_wgs,
+                         many);
+    else
+      hipLaunchKernelGGL((paged_mixed_kernel<DT, ODT, 1>), grid, dim3(256), 0, st, c, a.few_wgs,
+                         many);
+  } else if (a.few) {
+    hipLaunchKernelGGL((paged_few_kernel<DT, ODT>), dim3((unsigned)a.few_wgs), dim3(512), 0, st, c.a);
+  } else {
+    const dim3 grid((unsigned)many);
+    if (a.qb == 2)
+      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 2, 4>), grid, dim3(256), 0, st, c);
+    else if (a.nw == 8)
+      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 8>), grid, dim3(512), 0, st, c);
+    else
+      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 4>), grid, dim3(256), 0, st, c);
+  }
+  if (a.many && a.splits > 1)
     hipLaunchKernelGGL((paged_join_kernel<DT, ODT>),
-                       dim3((unsigned)(a.items * c.a.Hkv * (a.bq / 4))), dim3(256), 0, st, c);
+                       dim3((unsigned)(a.items * c.a.Hkv * (a.bq / 32))), dim3(256), 0, st, c);
 }
 
 bool attend_sizes_ok(int B, int T, int Hq, int Hkv, int max_new) {
@@ -1305,6 +1388,10 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   p.counters = reinterpret_cast<int*>(workspace);
   p.records = workspace ? workspace + D_COUNTERS : nullptr;
   p.split = plan.few_split;
+  p.out_wide = !(((uintptr_t)out | (uintptr_t)o_st * dkv_elt_size(out_dtype) |
+                  (uintptr_t)o_sh * dkv_elt_size(out_dtype)) &
+                 (uintptr_t)(4 * dkv_elt_size(out_dtype) - 1));
+  c.records = workspace ? workspace + D_COUNTERS + plan.many_at : nullptr;
   c.bq = plan.bq;
   c.splits = plan.splits;
   c.few_rows = plan.few ? DROWS : 0;
