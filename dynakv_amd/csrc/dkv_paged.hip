@@ -313,9 +313,12 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     total = pg_wave_sum(total) * p.Hkv;
     units = pg_wave_sum(units) * p.Hkv;
     const int G = wgs;  // at least the units
-    // parts of size c; the same in every wave of the launch, whatever the rounding
+    // Parts of size c; the same in every wave of the launch, whatever the rounding. At most 0.65
+    // sqrt(tiles): a part costs its join what two tiles cost (one user of 8192 tokens: 15.6 us in 16
+    // parts, 18.0 in 32; of 2048 tokens: 12.6 in 4, 11.5 in 8).
     auto parts_of = [&](int tiles, float inv) {
-      return tiles > 0 ? max(1, (int)((float)tiles * inv + 0.999f)) : 0;
+      const float most = 0.65f * __builtin_amdgcn_sqrtf((float)tiles) + 0.5f;
+      return tiles > 0 ? max(1, (int)fminf((float)tiles * inv + 0.999f, most)) : 0;
     };
     // the least c lies between total / G (no rounding up) and total / (G - units) (each unit
     // rounded up by a whole part)
@@ -1272,7 +1275,9 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
     };
     const long long wg128 = full(128), wg64 = full(64);
     auto ranges = [&](long long wgs, long long least) {
-      const long long n = (a.few ? 256 : 512) / wgs, most = (tiles + least / 2) / least;
+      // (beside the other kind, about half the chip: 12 single tokens and 512 at 2048, 16 and 4
+      // heads: 34 us with two ranges, 42 with one or three, 49 in a launch of its own)
+      const long long n = a.few ? (256 + wgs / 2) / wgs : 512 / wgs, most = (tiles + least / 2) / least;
       return (int)(n < most ? n : most);
     };
     a.splits = 1;
