@@ -20,6 +20,10 @@ only the forward math):
   skinny GEMM (``kernels/model_ops.py``), with the residual add and the RMSNorm before them
   folded into its x staging for one or two rows, and the SwiGLU product is one kernel --
   the same stages serve the dense baseline.
+* ``PagedLlama.generate``: the same weights over a paged uncompressed cache
+  (``kernels/paged.py``), for prompts of different lengths that come and go: prompts go through
+  in chunks beside the other requests' single tokens. Generation is greedy, or drawn by a
+  ``Sampler`` (``kernels/sampling.py``), which the other generators take too.
 * ``DenseLlama.generate``: the uncompressed-cache baseline of the same weights (K/V kept in
   full in a preallocated cache; decode attention by the same split kernel over that cache read
   as a packed cache with all 128 dims per token and an identity basis, prefill attention by
@@ -42,8 +46,10 @@ from .kernels.cutoff import CutoffHead
 from .kernels.decode import dense_append_, dense_decode_attention, grouped_decode_attention
 from .kernels.layer import DecodeLayerPlan
 from .kernels.model_ops import linear, rmsnorm_glu, rmsnorm_linear
+from .kernels.paged import PagedKVCache, paged_append, paged_attention
 from .kernels.prefill import coef_prefill_attention, rope_dense_
 from .kernels.router import KernelPolicy
+from .kernels.sampling import sample_tokens
 
 
 @dataclass(frozen=True)
@@ -57,6 +63,9 @@ class LlamaShape:
     vocab: int = 128256
     theta: float = 500000.0
     eps: float = 1e-5
+    # norms of each query and key head before the rotation (the reference's second model family,
+    # custom_qwen3.py): PagedLlama alone takes such a shape
+    qk_norm: bool = False
 
 
 @dataclass
@@ -78,6 +87,8 @@ class LayerWeights:
     k_basis: torch.Tensor  # (G, R, Dh) rank-major
     v_basis: torch.Tensor
     cutoff: CutoffHead = field(repr=False)
+    q_norm: torch.Tensor | None = None  # (Dh,) weights of the head norms, where the shape has them
+    k_norm: torch.Tensor | None = None
 
 
 def _orthogonal(n: int, count: int, gen: torch.Generator, device) -> torch.Tensor:
@@ -148,7 +159,27 @@ class RandomLlama:
                 k_basis=Uk.transpose(1, 2).contiguous().to(dtype),
                 v_basis=Uv.transpose(1, 2).contiguous().to(dtype),
                 cutoff=CutoffHead(cut[0], bias[0], cut[1], bias[1], groups=G)))
+        if s.qk_norm:  # (drawn last: the other weights are those of the shape without norms)
+            for lw in self.layers:
+                lw.q_norm, lw.k_norm = 1 + rnd(Dh), 1 + rnd(Dh)
 
+
+class Sampler:
+    """Draws tokens from logits: a generator's replacement for its argmax. The settings are those of
+    ``sample_tokens``, numbers or a tensor with an entry per row; the uniform numbers come from a
+    generator of its own, so a seed gives the same draws for the same logits."""
+
+    def __init__(self, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0,
+                 device="cuda"):
+        self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self._gen = torch.Generator(device=device)
+        self._gen.manual_seed(seed)
+
+    def __call__(self, logits: torch.Tensor) -> torch.Tensor:
+        """``logits`` (..., V) -> tokens (...)."""
+        rows = logits.reshape(-1, logits.shape[-1])
+        u = torch.rand(rows.shape[0], generator=self._gen, device=logits.device)
+        return sample_tokens(rows, u, **self.settings).view(logits.shape[:-1])
 
 
 
@@ -159,7 +190,11 @@ def _rope_q(q: torch.Tensor, pos0: int, theta: float) -> torch.Tensor:
 
 
 class _Generator:
+    takes_qk_norm = False
+
     def __init__(self, model: RandomLlama):
+        if model.shape.qk_norm and not self.takes_qk_norm:
+            raise ValueError(f"{type(self).__name__} has no query and key norms")
         self.m = model
         self.s = model.shape
 
@@ -185,19 +220,22 @@ class _Generator:
             delta = linear(h, lw.w_down)
         return x + delta
 
-    def generate(self, prompt: torch.Tensor, new_tokens: int) -> dict:
-        """Greedy decode; returns tokens, timings and cache bytes."""
+    def generate(self, prompt: torch.Tensor, new_tokens: int,
+                 sampler: Sampler | None = None) -> dict:
+        """Greedy decode (or tokens drawn by ``sampler``); returns tokens, timings and cache
+        bytes."""
+        pick = sampler if sampler is not None else lambda logits: logits.argmax(-1)
         torch.cuda.synchronize(self.m.device)
         t0 = time.perf_counter()
         x = self.prefill(prompt)
-        tok = self.logits(x[:, -1:]).argmax(-1)  # (B, 1)
+        tok = pick(self.logits(x[:, -1:]))  # (B, 1)
         out = [tok]
         torch.cuda.synchronize(self.m.device)
         t1 = time.perf_counter()
         pos = prompt.shape[1]
         for _ in range(new_tokens - 1):
             x = self.decode(tok, pos)
-            tok = self.logits(x).argmax(-1)
+            tok = pick(self.logits(x))
             out.append(tok)
             pos += 1
         torch.cuda.synchronize(self.m.device)
@@ -411,3 +449,97 @@ class DenseLlama(_Generator):
         s = self.s
         rows = self.k[0].shape[0] if self.k else 0
         return 2 * s.layers * rows * self.len * s.head_dim * self.m.embed.element_size()
+
+
+class PagedLlama(_Generator):
+    """The same weights over a paged uncompressed cache: requests of different lengths, whose
+    prompts go through in chunks beside the other requests' single tokens.
+
+    ``pages`` pages of ``page_size`` tokens per layer are shared by all requests. ``add`` starts a
+    request, ``step`` feeds tokens to some of them and returns the logits after each one's last
+    token, ``end`` gives a request's pages back; ``generate`` is the loop over them."""
+
+    takes_qk_norm = True
+
+    def __init__(self, model: RandomLlama, pages: int, page_size: int = 64):
+        super().__init__(model)
+        s = self.s
+        self.cache = PagedKVCache(s.layers, pages, s.kv_heads, page_size=page_size,
+                                  dtype=model.dtype, device=model.device)
+
+    def add(self) -> int:
+        return self.cache.add()
+
+    def end(self, request: int) -> None:
+        self.cache.free(request)
+
+    def step(self, feed: list[tuple[int, torch.Tensor]]) -> torch.Tensor:
+        """Feed each (request, (n,) tokens), n >= 1; returns (requests, vocab) logits."""
+        s = self.s
+        if not feed or any(t.dim() != 1 or t.shape[0] < 1 for _, t in feed):
+            raise ValueError("a step feeds at least one token to each of its requests")
+        batch = self.cache.batch((r, t.shape[0]) for r, t in feed)
+        x = F.embedding(torch.cat([t for _, t in feed]), self.m.embed).unsqueeze(0)
+
+        def attn(i, lw, y):
+            q = paged_append(y[0], self.cache.k[i], self.cache.v[i], batch, heads=s.heads,
+                             theta=s.theta, q_norm=lw.q_norm, k_norm=lw.k_norm, eps=s.eps)
+            a = paged_attention(q, self.cache.k[i], self.cache.v[i], batch)
+            return a.view(1, -1, s.hidden)
+
+        x = self._run(x, attn, "w_qkv")[0]
+        return self.logits(x[batch.q_start[1:].long() - 1])
+
+    def generate(self, prompts: list[torch.Tensor], new_tokens: int,
+                 sampler: Sampler | None = None, chunk: int = 512) -> dict:
+        """``new_tokens`` tokens for each of the (n,) prompts (n >= 1), greedily or drawn by
+        ``sampler``; a step takes at most ``chunk`` tokens of prompts, in the prompts' order, beside
+        a token of each request that is generating. Returns the tokens (prompts, new_tokens), the
+        wall time and the most pages held."""
+        if chunk < 1 or new_tokens < 1 or not prompts:
+            raise ValueError("need prompts, a positive chunk and a positive number of tokens")
+        if any(p.dim() != 1 or p.shape[0] < 1 for p in prompts):
+            raise ValueError("prompts are (n,) tokens, n >= 1")
+        pick = sampler if sampler is not None else lambda logits: logits.argmax(-1)
+        torch.cuda.synchronize(self.m.device)
+        t0 = time.perf_counter()
+        ids: list = [self.add() for _ in prompts]  # None once ended
+        fed = [0] * len(prompts)                   # prompt tokens gone through
+        out: list[list[torch.Tensor]] = [[] for _ in prompts]
+        held = 0
+        try:
+            while any(len(o) < new_tokens for o in out):
+                room, feed, who = chunk, [], []
+                for j, p in enumerate(prompts):
+                    n = min(room, p.shape[0] - fed[j])
+                    if n > 0:
+                        feed.append((ids[j], p[fed[j]:fed[j] + n]))
+                        room -= n
+                        fed[j] += n
+                    elif fed[j] == p.shape[0] and len(out[j]) < new_tokens:
+                        feed.append((ids[j], out[j][-1]))
+                    else:
+                        continue
+                    who.append(j)
+                tok = pick(self.step(feed))
+                held = max(held, self.cache.pages - self.cache.free_pages)
+                for i, j in enumerate(who):
+                    if fed[j] == prompts[j].shape[0]:  # its whole prompt has gone through
+                        out[j].append(tok[i:i + 1])
+                        if len(out[j]) == new_tokens:
+                            self.end(ids[j])
+                            ids[j] = None
+        finally:
+            for r in ids:
+                if r is not None:
+                    self.end(r)
+        torch.cuda.synchronize(self.m.device)
+        t = time.perf_counter() - t0
+        return {"tokens": torch.stack([torch.cat(o) for o in out]), "seconds": t,
+                "tokens_per_s": len(prompts) * new_tokens / t, "pages": held}
+
+    def kv_bytes(self) -> int:
+        """Bytes of the pages that requests hold, over all layers."""
+        k = self.cache.k[0]
+        held = self.cache.pages - self.cache.free_pages
+        return 2 * len(self.cache.k) * held * k[0].numel() * k.element_size()
