@@ -11,9 +11,9 @@
 // Weights are held in 64-bit fixed point, 44 bits after the point: sums of them are the same in any
 // order (the histogram adds by atomics), and a token is decided by u * mass against a running sum,
 // where 32 bits would pick another token than the formula's in one draw of a few thousand. With
-// x = 64 log2(e) (max l - l) / t in 64-bit floating point, i = floor(x):
+// x = 64 log2(e) (max l - l) / t as a sum of two 32-bit numbers p + r, i = floor(p):
 //   w = 2^(-i/64) (1 - d),  d = 1 - 2^(-(x - i)/64) < 0.011,
-// d to 32 bits after the point, 2^(-j/64) from a table of 64.
+// d to 31 bits after the point, 2^(-j/64) from a table of 64.
 //
 // One workgroup of 1024 threads per row, which goes over the row four times (from the caches after the
 // first): the maximum; a histogram of the tokens by i (counts and sums of d in one 64-bit number, so that a bin's mass is
@@ -34,7 +34,8 @@ constexpr int SM_AHEAD = 4;              // 16-byte pieces that a thread has in 
 constexpr int SM_BINS = 4096;            // bins of 1/64 in log2 of the weight; the last: the rest
 constexpr int SM_CAND = 2048;            // tokens of a border's bin that are sorted
 constexpr int SM_CHUNKS = SM_WAVES * (SM_MAX_V / 4 / SM_THREADS + 1);  // 1 KB pieces of a row
-constexpr int SM_COUNT = 45;             // a bin: the count from this bit on, below it the sum of d
+constexpr int SM_COUNT = 44;             // a bin: the count from this bit on, below it the sum of d
+constexpr uint32_t SM_OFF = 1u << 13;    // added to d, which may be as low as -2^-19
 constexpr double SM_ONE = 17592186044416.0;  // 2^44
 
 struct SampleParams {
@@ -68,9 +69,28 @@ __device__ __forceinline__ u64 sm_wave_scan(u64 v, int lane) {  // inclusive
   }
   return v;
 }
-__device__ __forceinline__ double sm_wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+template <int CTRL>
+__device__ __forceinline__ u64 sm_dpp(u64 v) {
+  return (uint32_t)dkv_dpp_i32<CTRL>((int)(uint32_t)v) |
+         ((u64)(uint32_t)dkv_dpp_i32<CTRL>((int)(uint32_t)(v >> 32)) << 32);
+}
+__device__ __forceinline__ u64 sm_wave_sum(u64 v) {  // as dkv_wave_sum_fast
+  v += sm_dpp<0xb1>(v);
+  v += sm_dpp<0x4e>(v);
+  v += sm_dpp<0x141>(v);
+  v += sm_dpp<0x140>(v);
+  {
+    const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    v = (a[0] | ((u64)b[0] << 32)) + (a[1] | ((u64)b[1] << 32));
+  }
+  {
+    const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    v = (a[0] | ((u64)b[0] << 32)) + (a[1] | ((u64)b[1] << 32));
+  }
   return v;
 }
 
@@ -87,7 +107,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
   __shared__ u64 sCand[SM_CAND];
   __shared__ u64 sSort[SM_CAND];
   __shared__ u64 sChunk[SM_CHUNKS];
-  __shared__ double sRoot[64];
+  __shared__ uint32_t sRoot[64];
   __shared__ u64 sWave[SM_WAVES];
   __shared__ u64 sWave2[SM_WAVES];
   __shared__ float sMax[SM_WAVES];
@@ -183,7 +203,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
   m = dkv_wave_max(m);
   if (lane == 0) sMax[wave] = m;
   if (tid == 0) sN = 0x7fffffff;
-  if (tid < 64) sRoot[tid] = exp2(-(double)tid / 64.0);
+  if (tid < 64) sRoot[tid] = (uint32_t)rint(exp2(31.0 - (double)tid / 64.0));
   __syncthreads();
   for (int w = 0; w < SM_WAVES; ++w) m = fmaxf(m, sMax[w]);
   if (m == -INFINITY) {
@@ -208,58 +228,68 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
   }
   const double c64 = 64.0 * 1.4426950408889634074 / (double)fminf(fmaxf(t, 1e-30f), 1e30f);
 
-  // bin and d (32 bits after the point) of a logit
-  auto split = [&](float l, int& i, uint32_t& d) {
-    const double x = fmin(((double)m - (double)l) * c64, (double)(SM_BINS - 1));
-    i = (int)x;
-    const float f = (float)(x - (double)i);
-    // 2^32 (1 - 2^(-f/64)): with g = ln2 / 64, g f - (g f)^2 / 2 + (g f)^3 / 6 - (g f)^4 / 24
-    constexpr double g = 0.69314718055994530942 / 64, one = 4294967296.0;
-    const float s =
-        f * (float)(g * one) +
-        f * f * ((float)(-g * g / 2 * one) +
-                 f * ((float)(g * g * g / 6 * one) + f * (float)(-g * g * g * g / 24 * one)));
-    d = (uint32_t)fmaxf(s, 0.f);
+  const float c_hi = (float)c64, c_lo = (float)(c64 - (double)c_hi);
+
+  // The bin of a logit; `d`: 2^31 d + SM_OFF. (NaN: the last bin.) Of max l - l, which is rounded,
+  // fp32 logits take what the rounding left; 16-bit ones are exact but for some next to 0.
+  auto bin_at = [&](float l, float& dl, float& x) {
+    dl = m - l;
+    x = fminf(dl * c_hi, (float)(SM_BINS - 1));
+    return (int)x;
   };
-  // the weight of a logit, a whole number (of 2^-44) in a double
+  auto bin_of = [&](float l) {
+    float dl, x;
+    return bin_at(l, dl, x);
+  };
+  auto split = [&](float l, int& i, uint32_t& d) {
+    float dl, x;
+    i = bin_at(l, dl, x);
+    float r = fmaf(dl, c_lo, fmaf(dl, c_hi, -x));
+    if constexpr (DT == DKV_F32) r = fmaf((m - dl) - l, c_hi, r);
+    const float f = __builtin_amdgcn_fractf(x) + r;
+    // 2^31 (1 - 2^(-f/64)): with g = ln2 / 64, g f - (g f)^2 / 2 + (g f)^3 / 6 - (g f)^4 / 24
+    constexpr double g = 0.69314718055994530942 / 64, one = 2147483648.0;
+    const float s = fmaf(
+        f, fmaf(f, fmaf(f, fmaf(f, (float)(-g * g * g * g / 24 * one), (float)(g * g * g / 6 * one)),
+                        (float)(-g * g / 2 * one)),
+                (float)(g * one)),
+        (float)SM_OFF);
+    d = (uint32_t)s;
+  };
+  // the weight of a logit, in 2^-44
   auto weight = [&](float l) {
     int i;
     uint32_t d;
     split(l, i, d);
-    const double w = sRoot[i & 63] * fma((double)d, -1.0 / 4294967296.0, 1.0);
-    return i == SM_BINS - 1 ? 0.0 : rint(ldexp(w, SM_POINT - (i >> 6)));
-  };
-  auto bin_of = [&](float l) {
-    return (int)fmin(((double)m - (double)l) * c64, (double)(SM_BINS - 1));
+    const u64 w = (u64)sRoot[i & 63] * (u64)(uint32_t)((1u << 31) + SM_OFF - d);  // 2^62 w
+    return i == SM_BINS - 1 ? 0ULL : w >> min((62 - SM_POINT) + (i >> 6), 63);
   };
   // the mass of a bin
   auto bin_mass = [&](int i, u64 h) {
     const double n = (double)(h >> SM_COUNT);
-    const double d = (double)(h & ((1ULL << SM_COUNT) - 1)) * (1.0 / 4294967296.0);
-    return i == SM_BINS - 1 ? 0ULL
-                            : (u64)rint(ldexp(sRoot[i & 63] * (n - d), SM_POINT - (i >> 6)));
+    const double d = (double)(h & ((1ULL << SM_COUNT) - 1)) - n * (double)SM_OFF;
+    const double w = (double)sRoot[i & 63] * (n - d * (1.0 / 2147483648.0));  // 2^31 w
+    return i == SM_BINS - 1 ? 0ULL : (u64)rint(ldexp(w, SM_POINT - 31 - (i >> 6)));
   };
 
   const bool by_k = k > 0 && k < V, by_p = tp < 1.f;
   Border keep = {-INFINITY, -1};
   u64 kept = 0;  // the mass of what is kept so far
 
-  // ---- the border inside a bin: its tokens sorted ----
-  // j > 0: up to the j-th of them; else those before which (with `before`) less than P lies. Returns
-  // false where they are too many. `mass`: what is kept of the bin.
-  auto in_bin = [&](int bin, u64 j, u64 before, double P, Border& r, u64& mass) {
+  // ---- the borders inside bins: the n tokens of bins b0 .. b1 (at most SM_CAND) sorted ----
+  int sorted = 0;
+  auto sort_bins = [&](int b0, int b1) {
     __syncthreads();
     if (tid == 0) sN = 0;
     __syncthreads();
-    const float c32 = (float)c64, mid = (float)bin + 0.5f;
     each([&](int c, int i0, const dkv_u32x4& v) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float l = value(v, e);
-        const float x = (m - l) * c32;
-        if (!(fabsf(x - mid) > 0.52f) || bin == SM_BINS - 1) {  // near it, or not to be told
+        const int bin = bin_of(l);
+        if (bin >= b0 && bin <= b1) {
           const int i = i0 + e;
-          if (i >= 0 && i < V && l == l && bin_of(l) == bin) {
+          if (i >= 0 && i < V && l == l) {
             const int at = atomicAdd(&sN, 1);
             if (at < SM_CAND) sCand[at] = ((u64)sm_key(l) << 32) | (uint32_t)~i;
           }
@@ -267,23 +297,29 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
       }
     });
     __syncthreads();
-    const int n = sN;
-    if (n > SM_CAND) return false;
-    for (int a = tid; a < n; a += SM_THREADS) {
+    sorted = sN;
+    if (sorted > SM_CAND) return false;
+    for (int a = tid; a < sorted; a += SM_THREADS) {
       const u64 x = sCand[a];
       int rank = 0;
-      for (int b = 0; b < n; ++b) rank += sCand[b] > x;
+      for (int b = 0; b < sorted; ++b) rank += sCand[b] > x;
       sSort[rank] = x;
     }
+    __syncthreads();
+    return true;
+  };
+  // Up to the j-th of the sorted tokens (j > 0), or those before which, with `before`, less than P
+  // lies; `mass`: theirs.
+  auto border_in = [&](u64 j, u64 before, double P, Border& r, u64& mass) {
     __syncthreads();
     if (wave == 0) {
       u64 run = 0;
       int last = -1;
-      for (int a = 0; a < n; a += 64) {
+      for (int a = 0; a < sorted; a += 64) {
         const int at = a + lane;
-        const u64 w = at < n ? (u64)weight(sm_unkey((uint32_t)(sSort[at] >> 32))) : 0;
+        const u64 w = at < sorted ? weight(sm_unkey((uint32_t)(sSort[at] >> 32))) : 0;
         const u64 sum = sm_wave_scan(w, lane);
-        const bool in = at < n && (j ? (u64)at < j : (double)(before + run + sum - w) < P);
+        const bool in = at < sorted && (j ? (u64)at < j : (double)(before + run + sum - w) < P);
         const u64 hit = __ballot(in);
         if (!hit) break;
         const int l = 63 - __clzll((long long)hit);
@@ -301,7 +337,6 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
     r.at = sPick[0] ? sm_unkey((uint32_t)(sPick[0] >> 32)) : -INFINITY;
     r.last = (int)~(uint32_t)sPick[0];
     mass = sPick[1];
-    return true;
   };
 
   // ---- the border by digits of the keys (11, 11, 10 bits): for a bin of too many tokens ----
@@ -326,7 +361,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
           const uint32_t key = sm_key(l);
           if (level && (key >> (shift + bits)) != found) continue;
           const int bin = (int)((key >> shift) & ((1u << bits) - 1));
-          atomicAdd(&sHist[bin], (u64)weight(l));
+          atomicAdd(&sHist[bin], weight(l));
           atomicAdd(&sHist[2048 + bin], 1ULL);
         }
       });
@@ -355,7 +390,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
       ties = sPick[3];
     }
     r.at = sm_unkey(found);
-    const u64 w = (u64)weight(r.at);
+    const u64 w = weight(r.at);
     if (want) {
       ties = min(ties, want - above);
     } else if (w > 0) {
@@ -421,10 +456,9 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
     each([&](int c, int i0, const dkv_u32x4& v) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float l = fmaxf(value(v, e), -INFINITY);
         int i;
         uint32_t d;
-        split(l, i, d);
+        split(value(v, e), i, d);
         if (i < SM_BINS - 1) atomicAdd(&sHist[i], (1ULL << SM_COUNT) | d);
       }
     });
@@ -456,43 +490,62 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
       total += sWave2[w];
     }
     kept = total;
-    bool digits = false;
+    // The bin of a border: where the k-th token is (want), or the last one before which less than P
+    // lies; the count and the mass above it. SM_BINS: none.
+    auto find = [&](u64 want, double P, u64& n_above, u64& m_above) {
+      __syncthreads();
+      if (tid == 0) sPick[0] = want ? SM_BINS - 1 : SM_BINS, sPick[1] = sPick[2] = 0;
+      __syncthreads();
+      u64 n = nrun, s = mrun;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool rest = 4 * tid + q == SM_BINS - 1;
+        const bool here = want ? n < want && (rest || want <= n + cnt[q])
+                               : cnt[q] && (double)s < P && P <= (double)(s + mass[q]);
+        if (here) {
+          sPick[0] = (u64)(4 * tid + q);
+          sPick[1] = n;
+          sPick[2] = s;
+        }
+        n += cnt[q];
+        s += mass[q];
+      }
+      __syncthreads();
+      n_above = sPick[1];
+      m_above = sPick[2];
+      return (int)sPick[0];
+    };
+    bool digits = false, done = false;
+    u64 n_k = 0, m_k = 0;
+    const int bin_k = by_k ? find((u64)k, 0.0, n_k, m_k) : SM_BINS;
+    if (by_k && by_p && bin_k < SM_BINS - 1) {
+      // What top-k keeps has a mass between m_k and that with its bin's; the bins in which the border
+      // of top-p can lie then, sorted with top-k's where they are few: one pass for both.
+      u64 n_p, m_p;
+      const int bin_p = find(0, (double)tp * (double)max(m_k, 1ULL), n_p, m_p);
+      const u64 h = sHist[bin_k] >> SM_COUNT;
+      if (bin_p <= bin_k && n_k + h - n_p <= SM_CAND && sort_bins(bin_p, bin_k)) {
+        u64 in;
+        border_in((u64)k - n_p, 0, 0.0, keep, in);
+        kept = m_p + in;
+        const double P = (double)tp * (double)kept;
+        border_in(0, m_p, P, keep, in);
+        kept = m_p + in;
+        done = true;
+      }
+    }
 #pragma unroll 1
-    for (int step = 0; step < 2; ++step) {  // top-k, then top-p of what it keeps
+    for (int step = 0; step < 2 && !done; ++step) {  // top-k, then top-p of what it keeps
       if (step == 0 ? !by_k : !by_p) continue;
       const u64 want = step == 0 ? (u64)k : 0;
       const double P = step == 0 ? 0.0 : (double)tp * (double)kept;
-      bool found = false;
-      __syncthreads();
-      if (!digits) {
-        if (tid == 0) sPick[0] = step == 0 ? SM_BINS - 1 : SM_BINS, sPick[1] = sPick[2] = 0;
-        __syncthreads();
-        u64 n = nrun, s = mrun;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const bool rest = 4 * tid + q == SM_BINS - 1;
-          const bool here = step == 0 ? n < want && (rest || want <= n + cnt[q])
-                                      : cnt[q] && (double)s < P && P <= (double)(s + mass[q]);
-          if (here) {
-            sPick[0] = (u64)(4 * tid + q);
-            sPick[1] = n;
-            sPick[2] = s;
-          }
-          n += cnt[q];
-          s += mass[q];
-        }
-        __syncthreads();
-        const int bin = (int)sPick[0];
-        const u64 j = want - sPick[1], above = sPick[2];
-        u64 in = 0;
-        Border r;
-        if (bin < SM_BINS && in_bin(bin, step == 0 ? j : 0, above, P, r, in)) {
-          keep = r;
-          kept = above + in;
-          found = true;
-        }
-      }
-      if (!found) {
+      u64 n_above = 0, above = 0;
+      const int bin = digits ? SM_BINS : find(want, P, n_above, above);
+      if (bin < SM_BINS && sort_bins(bin, bin)) {
+        u64 in;
+        border_in(want ? want - n_above : 0, above, P, keep, in);
+        kept = above + in;
+      } else {
         by_digits(want, P, keep, kept);
         digits = true;
       }
@@ -500,24 +553,38 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
   }
 
   // ---- the kept mass of each row of 64 pieces ----
-  const double floor_w = mp > 0.f ? (double)mp * SM_ONE : 0.0;
-  auto mass_of = [&](float l, int i) {
-    double w = 0.0;
-    if (l > keep.at || (l == keep.at && i <= keep.last)) {
-      w = weight(l);
-      w = w >= floor_w ? w : 0.0;
-    }
-    return w;
-  };
+  const u64 floor_w = mp > 0.f ? (u64)ceil((double)mp * SM_ONE) : 0;
+  auto is_kept = [&](float l, int i) { return l > keep.at || (l == keep.at && i <= keep.last); };
+  auto floored = [&](u64 w) { return w >= floor_w ? w : 0ULL; };
   __syncthreads();
   each([&](int c, int i0, const dkv_u32x4& v) {
-    double s = 0.0;
+    u64 s = 0;
+    if (!by_k && !by_p) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      s += mass_of(value(v, e), i0 + e);
+      for (int e = 0; e < E; ++e) {
+        const float l = value(v, e);
+        s += l > -INFINITY ? floored(weight(l)) : 0ULL;
+      }
+    } else {
+      // the few that are kept, one of each lane's at a time
+      uint32_t mask = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float l = value(v, e);
+        mask |= l >= keep.at && is_kept(l, i0 + e) ? 1u << e : 0u;
+      }
+      while (__ballot(mask != 0)) {
+        const int e = mask ? __ffs((int)mask) - 1 : 0;
+        float l = value(v, 0);
+#pragma unroll
+        for (int x = 1; x < E; ++x) l = e == x ? value(v, x) : l;
+        const u64 w = floored(weight(l));
+        s += mask ? w : 0ULL;
+        mask &= mask - 1;
+      }
     }
-    s = sm_wave_sum(s);  // 512 whole numbers of at most 2^44: exact
-    if (lane == 0) sChunk[wave * per_wave + c] = (u64)s;
+    s = sm_wave_sum(s);
+    if (lane == 0) sChunk[wave * per_wave + c] = s;
   });
   __syncthreads();
   // ---- the row of pieces in which u * mass lies ----
@@ -553,7 +620,11 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
     const int i0 = first_of(c);
     u64 w[E], s = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += w[e] = (u64)mass_of(value(v, e), i0 + e);
+    for (int e = 0; e < E; ++e) {
+      const float l = value(v, e);
+      w[e] = is_kept(l, i0 + e) ? floored(weight(l)) : 0ULL;
+      s += w[e];
+    }
     u64 at = sPick[1] + sm_wave_scan(s, lane) - s;
     if (at <= target && target < at + s) {
 #pragma unroll
