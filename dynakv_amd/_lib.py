@@ -7,7 +7,6 @@ CPU or eager-PyTorch path.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import importlib.util
 import sysconfig
@@ -274,13 +273,15 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-_NO_GUARD = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def on_device(t: torch.Tensor):
-    """Context in which t's device is the current one, as a launch on one of its streams needs."""
-    i = t.get_device()
-    return _NO_GUARD if i == torch.cuda.current_device() else torch.cuda.device(i)
+def call_on(device: int, fn, *args):
+    """fn(*args) with ``device`` as the current one, as a launch on one of its streams needs."""
+    if _current_device() == device:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

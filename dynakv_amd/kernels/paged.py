@@ -32,6 +32,7 @@ from .. import _lib
 from .decode import workspace
 
 HEAD_DIM = 128
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _COUNTERS = 16384  # leading floats of the attention's workspace: its arrival counters
 
 
@@ -48,28 +49,32 @@ class PagedBatch:
     tokens past ``max_new`` or keys past ``max_len`` may be left out."""
 
     __slots__ = ("page_table", "q_start", "lens", "rows", "max_new", "max_len", "min_new",
-                 "requests")
+                 "requests", "device", "_table_args", "_row_args")
 
     def __init__(self, page_table: torch.Tensor, q_start: torch.Tensor, lens: torch.Tensor, *,
                  rows: int, max_new: int, max_len: int, min_new: int = 1):
-        if page_table.dim() != 2 or q_start.dim() != 1 or lens.dim() != 1:
+        shape, n_start, n_lens = page_table.shape, q_start.shape, lens.shape
+        if len(shape) != 2 or len(n_start) != 1 or len(n_lens) != 1:
             raise ValueError("page_table must be (B, P), q_start (B + 1,), lens (B,)")
-        B = lens.shape[0]
-        if page_table.shape[0] != B or q_start.shape[0] != B + 1:
+        B, cols = shape
+        if n_lens[0] != B or n_start[0] != B + 1:
             raise ValueError("page_table, q_start and lens disagree on the number of requests")
         if not (page_table.dtype == q_start.dtype == lens.dtype == torch.int32):
             raise ValueError("page_table, q_start and lens must be int32")
-        if (not q_start.is_contiguous() or not lens.is_contiguous()
-                or (page_table.shape[1] > 1 and page_table.stride(1) != 1)
-                or (B > 1 and page_table.stride(0) < page_table.shape[1])):
+        ld, unit = page_table.stride()
+        if (not q_start.is_contiguous() or not lens.is_contiguous() or (cols > 1 and unit != 1)
+                or (B > 1 and ld < cols)):
             raise ValueError("page_table rows, q_start and lens must be contiguous")
         if not (page_table.device == q_start.device == lens.device):
             raise ValueError("page_table, q_start and lens must be on one device")
         if not (0 <= min_new <= max_new <= rows and max_len >= 0):
             raise ValueError("need 0 <= min_new <= max_new <= rows and max_len >= 0")
         self.page_table, self.q_start, self.lens = page_table, q_start, lens
-        self.requests = B
+        self.requests, self.device = B, page_table.get_device()
         self.rows, self.max_new, self.max_len, self.min_new = rows, max_new, max_len, min_new
+        # what every call passes of the batch: its buffers stay where they are
+        self._table_args = (page_table.data_ptr(), max(ld, cols), cols)
+        self._row_args = (q_start.data_ptr(), lens.data_ptr(), B, rows)
 
 
 class PagedKVCache:
@@ -173,9 +178,14 @@ class PagedKVCache:
 
 @functools.lru_cache(maxsize=64)
 def _frequencies(values) -> ctypes.Array:
-    """64 host doubles: radians per position of each pair (dims j and j + 64)."""
+    """64 host doubles, radians per position of each pair (dims j and j + 64), of a theta or as
+    given."""
     if isinstance(values, float):
+        if not (values > 0.0 and math.isfinite(values)):
+            raise ValueError("theta must be positive and finite")
         values = tuple(values ** (-2.0 * j / HEAD_DIM) for j in range(HEAD_DIM // 2))
+    if len(values) != HEAD_DIM // 2 or not all(math.isfinite(f) for f in values):
+        raise ValueError(f"inv_freq must hold {HEAD_DIM // 2} finite numbers")
     return (ctypes.c_double * (HEAD_DIM // 2))(*values)
 
 
@@ -183,39 +193,33 @@ def _frequency_address(theta: float | None, inv_freq: Sequence[float] | None) ->
     if (theta is None) == (inv_freq is None):
         raise ValueError("give theta or inv_freq, one of them")
     if theta is not None:
-        theta = float(theta)
-        if not (theta > 0.0 and math.isfinite(theta)):
-            raise ValueError("theta must be positive and finite")
-        return _frequencies(theta)
+        return _frequencies(float(theta))
     if torch.is_tensor(inv_freq):
         if inv_freq.is_cuda:
             raise ValueError("inv_freq is a host sequence (a device tensor would be read back)")
         inv_freq = inv_freq.tolist()
-    inv_freq = tuple(float(f) for f in inv_freq)
-    if len(inv_freq) != HEAD_DIM // 2 or not all(math.isfinite(f) for f in inv_freq):
-        raise ValueError(f"inv_freq must hold {HEAD_DIM // 2} finite numbers")
-    return _frequencies(inv_freq)
+    return _frequencies(tuple(float(f) for f in inv_freq))
 
 
-def _pool_checks(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch,
-                 dtype: torch.dtype) -> tuple[int, int]:
-    """(KV heads, page size) of the pools, checked against each other and the batch."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != HEAD_DIM:
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, dtype: torch.dtype,
+           device: int) -> tuple:
+    """(KV heads, the pools' arguments of a call), checked against each other and the batch."""
+    shape, st = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or shape[3] != HEAD_DIM:
         raise ValueError("k_pages / v_pages must be (pages, kv_heads, page_size, 128), alike")
-    st = k_pages.stride()
     if st != v_pages.stride() or st[3] != 1 or st[2] != HEAD_DIM:
         raise ValueError("pages must hold a head's tokens back to back, with one layout for K and V")
     if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise ValueError("page and input dtypes differ")
-    if not (k_pages.device == v_pages.device == batch.lens.device):
-        raise ValueError("pages and batch must be on one device")
-    hkv, ps = k_pages.shape[1], k_pages.shape[2]
+    if not (k_pages.get_device() == v_pages.get_device() == batch.device == device):
+        raise ValueError("inputs, pages and batch must be on one device")
+    pages, hkv, ps, _ = shape
     if ps < 16 or ps & (ps - 1):
         raise NotImplementedError("page_size must be a power of two of at least 16")
-    if batch.max_len > batch.page_table.shape[1] * ps:
+    if batch.max_len > batch._table_args[2] * ps:
         raise ValueError(f"max_len {batch.max_len} is past the page table "
-                         f"({batch.page_table.shape[1]} pages of {ps})")
-    return hkv, ps
+                         f"({batch._table_args[2]} pages of {ps})")
+    return hkv, (k_pages.data_ptr(), v_pages.data_ptr(), st[0], st[1], pages, ps)
 
 
 def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -232,39 +236,35 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ((128,) of qkv's dtype) each query / key head is first normed, x / sqrt(mean(x^2) + eps) * w.
     Everything in fp32, rounded once where it is stored. ``out``: where the queries go (T, heads,
     128), unit last stride; not qkv's own memory. A token whose page is not there is not stored."""
-    if qkv.dim() != 2 or qkv.stride(1) != 1:
+    shape, st = qkv.shape, qkv.stride()
+    if len(shape) != 2 or st[1] != 1:
         raise ValueError("qkv must be (T, W) with unit last stride")
-    hkv, ps = _pool_checks(k_pages, v_pages, batch, qkv.dtype)
-    T = qkv.shape[0]
-    if heads <= 0 or qkv.shape[1] < (heads + 2 * hkv) * HEAD_DIM:
+    T, width = shape
+    dt, dev = qkv.dtype, qkv.get_device()
+    hkv, pools = _pools(k_pages, v_pages, batch, dt, dev)
+    if heads <= 0 or width < (heads + 2 * hkv) * HEAD_DIM:
         raise ValueError(f"qkv must hold {heads} + 2 * {hkv} heads of {HEAD_DIM}")
     if batch.rows > T:
         raise ValueError(f"the batch has {batch.rows} rows, qkv {T}")
-    if qkv.device != k_pages.device:
-        raise ValueError("qkv and pages must be on one device")
     for w in (q_norm, k_norm):
-        if w is not None and (w.shape != (HEAD_DIM,) or w.dtype != qkv.dtype
-                              or not w.is_contiguous() or w.device != qkv.device):
+        if w is not None and (w.shape != (HEAD_DIM,) or w.dtype != dt or not w.is_contiguous()
+                              or w.get_device() != dev):
             raise ValueError("norm weights must be contiguous (128,) vectors of qkv's dtype")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     freqs = _frequency_address(theta, inv_freq)
-    st = _lib.stream_of(qkv)
+    stream = _lib.stream_of(qkv)
     if out is None:
-        out = torch.empty((T, heads, HEAD_DIM), dtype=qkv.dtype, device=qkv.device)
-    elif (out.shape != (T, heads, HEAD_DIM) or out.stride(2) != 1 or out.dtype != qkv.dtype
-          or out.device != qkv.device):
+        out = torch.empty((T, heads, HEAD_DIM), dtype=dt, device=qkv.device)
+    elif (out.shape != (T, heads, HEAD_DIM) or out.stride(2) != 1 or out.dtype != dt
+          or out.get_device() != dev):
         raise ValueError("out must be (T, heads, 128) of qkv's dtype with unit last stride")
-    t = batch.page_table
-    with _lib.on_device(qkv):
-        rc = _lib.calls().dkv_paged_append(
-            st, _lib.dtype_code(qkv.dtype), qkv.data_ptr(), qkv.stride(0), out.data_ptr(),
-            out.stride(0), out.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
-            k_pages.stride(0), k_pages.stride(1), k_pages.shape[0], ps, t.data_ptr(),
-            max(t.stride(0), t.shape[1]), t.shape[1], batch.q_start.data_ptr(),
-            batch.lens.data_ptr(), batch.requests, batch.rows, heads, hkv, HEAD_DIM,
-            _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs))
-    _lib.check(rc, "dkv_paged_append")
+    o_st = out.stride()
+    _lib.check(_lib.call_on(
+        dev, _lib.calls().dkv_paged_append, stream, _lib.dtype_code(dt), qkv.data_ptr(), st[0],
+        out.data_ptr(), o_st[0], o_st[1], *pools, *batch._table_args, *batch._row_args, heads, hkv,
+        HEAD_DIM, _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs)),
+        "dkv_paged_append")
     return out
 
 
@@ -278,43 +278,38 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     token at position t attends its request's tokens 0 .. t (the pages hold them all: the step's own
     are appended first); one that has none to attend gives 0. ``scale`` defaults to 1 / sqrt(128).
     The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``."""
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM:
+    shape, st = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != HEAD_DIM:
         raise ValueError("q must be (T, heads, 128)")
-    hkv, ps = _pool_checks(k_pages, v_pages, batch, q.dtype)
-    T, hq, _ = q.shape
+    T, hq, _ = shape
+    dt, dev = q.dtype, q.get_device()
+    hkv, pools = _pools(k_pages, v_pages, batch, dt, dev)
     if hq % hkv or hq == 0:
         raise ValueError(f"{hq} query heads do not divide among {hkv} KV heads")
     if batch.rows > T:
         raise ValueError(f"the batch has {batch.rows} rows, q {T}")
-    if q.device != k_pages.device:
-        raise ValueError("q and pages must be on one device")
-    if q.stride(2) != 1 or q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+    if st[2] != 1 or q.data_ptr() % 16 or st[0] % 8 or st[1] % 8:
         q = q.contiguous()
-    odt = out_dtype if out_dtype is not None else (out.dtype if out is not None else q.dtype)
-    if odt not in (q.dtype, torch.float32):
+        st = q.stride()
+    odt = out_dtype if out_dtype is not None else (out.dtype if out is not None else dt)
+    if odt != dt and odt != torch.float32:
         raise ValueError("out_dtype must be the query dtype or float32")
-    st = _lib.stream_of(q)
+    stream = _lib.stream_of(q)
     if out is None:
-        out = torch.empty((T, hq, HEAD_DIM), dtype=odt, device=q.device)
-    elif (out.shape != (T, hq, HEAD_DIM) or out.dtype != odt or out.stride(2) != 1
-          or out.device != q.device):
+        out = torch.empty(shape, dtype=odt, device=q.device)
+    elif (out.shape != shape or out.dtype != odt or out.stride(2) != 1
+          or out.get_device() != dev):
         raise ValueError("out must be (T, heads, 128) with unit last stride and the requested dtype")
-    sc = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    o_st = out.stride()
     lib = _lib.calls()
-    t = batch.page_table
-    with _lib.on_device(q):
-        need = lib.dkv_paged_workspace_floats(batch.requests, batch.rows, hq, hkv, batch.max_new,
-                                              batch.min_new, batch.max_len)
-        ws = _attention_workspace(q.device, st, need) if need else None
-        rc = lib.dkv_paged_attention(
-            st, _lib.dtype_code(q.dtype), q.data_ptr(), q.stride(0), q.stride(1),
-            k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
-            k_pages.shape[0], ps, t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[1],
-            batch.q_start.data_ptr(), batch.lens.data_ptr(), batch.requests, batch.rows, hq, hkv,
-            HEAD_DIM, batch.max_new, batch.min_new, batch.max_len, sc, _lib.ptr(ws),
-            ws.numel() if need else 0, out.data_ptr(), _lib.dtype_code(odt), out.stride(0),
-            out.stride(1))
-    _lib.check(rc, "dkv_paged_attention")
+    bounds = batch.max_new, batch.min_new, batch.max_len
+    need = lib.dkv_paged_workspace_floats(batch.requests, batch.rows, hq, hkv, *bounds)
+    ws = _attention_workspace(q.device, stream, need) if need else None
+    _lib.check(_lib.call_on(
+        dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), st[0], st[1],
+        *pools, *batch._table_args, *batch._row_args, hq, hkv, HEAD_DIM, *bounds,
+        _SCALE if scale is None else float(scale), _lib.ptr(ws), ws.numel() if need else 0,
+        out.data_ptr(), _lib.dtype_code(odt), o_st[0], o_st[1]), "dkv_paged_attention")
     return out
 
 

@@ -15,13 +15,13 @@ from .. import _lib
 MAX_VOCAB = 1 << 19
 
 
-def _setting(value, rows: int, dtype: torch.dtype, device, name: str):
+def _setting(value, rows: int, dtype: torch.dtype, device: int, name: str):
     """(pointer of a per-row tensor or None, the value for every row)."""
-    if not torch.is_tensor(value):
+    if not isinstance(value, torch.Tensor):
         return None, value
     if value.shape != (rows,) or value.dtype != dtype or not value.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous ({rows},) {dtype} tensor")
-    if value.device != device:
+    if value.get_device() != device:
         raise ValueError(f"{name} must be on the logits' device")
     return value.data_ptr(), 0
 
@@ -45,30 +45,31 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     token. A logit of -inf is never taken, NaN counts as -inf, +inf ones share the mass among
     themselves, and a row with no logit above -inf gives -1. Masses are summed in 64-bit fixed
     point, so a result depends on the row alone."""
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    shape, st = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and st[1] != 1):
         raise ValueError("logits must be (rows, V) with unit last stride")
-    rows, V = logits.shape
+    rows, V = shape
     if V == 0:
         raise ValueError("logits have no vocabulary")
     if V > MAX_VOCAB:
         raise NotImplementedError(f"vocabularies of at most {MAX_VOCAB} tokens")
-    dev = logits.device
-    if u.shape != (rows,) or u.dtype != torch.float32 or not u.is_contiguous() or u.device != dev:
+    dev = logits.get_device()
+    if (u.shape != (rows,) or u.dtype != torch.float32 or not u.is_contiguous()
+            or u.get_device() != dev):
         raise ValueError(f"u must be a contiguous ({rows},) float32 tensor on the logits' device")
     t_ptr, t = _setting(temperature, rows, torch.float32, dev, "temperature")
     k_ptr, k = _setting(top_k, rows, torch.int32, dev, "top_k")
     p_ptr, p = _setting(top_p, rows, torch.float32, dev, "top_p")
     m_ptr, m = _setting(min_p, rows, torch.float32, dev, "min_p")
-    st = _lib.stream_of(logits)
+    stream = _lib.stream_of(logits)
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=dev)
-    elif out.shape != (rows,) or out.dtype != torch.int64 or not out.is_contiguous() \
-            or out.device != dev:
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    elif (out.shape != (rows,) or out.dtype != torch.int64 or not out.is_contiguous()
+          or out.get_device() != dev):
         raise ValueError(f"out must be a contiguous ({rows},) int64 tensor on the logits' device")
-    with _lib.on_device(logits):
-        rc = _lib.calls().dkv_sample_tokens(
-            st, _lib.dtype_code(logits.dtype), logits.data_ptr(),
-            logits.stride(0) if rows > 1 else V, rows, V, u.data_ptr(), t_ptr, float(t), k_ptr,
-            int(min(max(k, 0), V)), p_ptr, float(p), m_ptr, float(m), out.data_ptr())
-    _lib.check(rc, "dkv_sample_tokens")
+    _lib.check(_lib.call_on(
+        dev, _lib.calls().dkv_sample_tokens, stream, _lib.dtype_code(logits.dtype),
+        logits.data_ptr(), st[0] if rows > 1 else V, rows, V, u.data_ptr(), t_ptr, float(t), k_ptr,
+        int(min(max(k, 0), V)), p_ptr, float(p), m_ptr, float(m), out.data_ptr()),
+        "dkv_sample_tokens")
     return out
