@@ -15,11 +15,16 @@
 //   w = 2^(-i/64) (1 - d),  d = 1 - 2^(-(x - i)/64) < 0.011,
 // d to 31 bits after the point, 2^(-j/64) from a table of 64.
 //
-// One workgroup of 1024 threads per row, which goes over the row four times (from the caches after the
-// first): the maximum; a histogram of the tokens by i (counts and sums of d in one 64-bit number, so that a bin's mass is
-// known), in which the borders' bins are found; the tokens of a border's bin sorted in LDS; the kept
-// mass of every 512 tokens (256 in fp32), in the vocabulary's order; the token. Bound by vector
-// instructions: a row's 128256 tokens in one CU take 0.85 us an instruction.
+// A row goes by three times (from the caches after the first): for the maximum; for a histogram of the
+// tokens by i, counts and sums of d in one 64-bit number, so that a bin's mass is known and with it the
+// bins of the borders; for the mass of every 512 tokens (256 in fp32) above those bins, in the
+// vocabulary's order, and the tokens inside them, which are sorted and those kept added. Then the 512
+// and the token in which u times the mass lies are known. A bin of too many tokens (equal logits, a
+// border 64 halvings down) goes through a search by the digits of the logits instead.
+//
+// Bound by vector instructions: a row of 128256 in one CU takes 0.85 us an instruction, of which the
+// histogram has 22 a token. One workgroup takes a row where there are rows for half the CUs; fewer rows
+// are cut into parts, a launch for each of the three passes.
 #include "dkv_common.h"
 
 namespace {
@@ -33,7 +38,7 @@ constexpr int SM_MAX_V = 1 << 19;        // weights of at most 1: sums below 2^6
 constexpr int SM_AHEAD = 4;              // 16-byte pieces that a thread has in flight
 constexpr int SM_BINS = 4096;            // bins of 1/64 in log2 of the weight; the last: the rest
 constexpr int SM_CAND = 2048;            // tokens of a border's bin that are sorted
-constexpr int SM_CHUNKS = SM_WAVES * (SM_MAX_V / 4 / SM_THREADS + 1);  // 1 KB pieces of a row
+constexpr int SM_CHUNKS = SM_MAX_V / 4 / 64 + 2;  // rows of 64 pieces (1 KB) of a row of logits
 constexpr int SM_COUNT = 44;             // a bin: the count from this bit on, below it the sum of d
 constexpr uint32_t SM_OFF = 1u << 13;    // added to d, which may be as low as -2^-19
 constexpr double SM_ONE = 17592186044416.0;  // 2^44
@@ -50,6 +55,23 @@ struct SampleParams {
   float temperature_all, top_p_all, min_p_all;
   int top_k_all;
   long long* out;
+  u64* ws;    // SM_WS words a row where rows are cut
+  int parts;  // workgroups of a row
+};
+
+// A cut row's words in the workspace: the parts' maxima, the number of listed tokens and of parts that
+// are done, the histogram, the tokens of the borders' bins, the masses of the rows of pieces.
+constexpr int SM_PARTS = 16;
+constexpr int SM_WS_N = SM_PARTS, SM_WS_HIST = 32, SM_WS_CAND = SM_WS_HIST + SM_BINS,
+              SM_WS_CHUNK = SM_WS_CAND + SM_CAND, SM_WS = SM_WS_CHUNK + SM_CHUNKS;
+static_assert(SM_WS % 2 == 0 && SM_WS_HIST % 2 == 0, "16-byte accesses");
+
+struct SampleShared {
+  __attribute__((aligned(16))) u64 hist[SM_BINS];
+  u64 cand[SM_CAND], sort[SM_CAND], chunk[SM_CHUNKS];
+  u64 wave[SM_WAVES], wave2[SM_WAVES], pick[4];
+  uint32_t root[64];
+  int n, last;
 };
 
 // A logit as a number that orders as the logits do (-0 as +0).
@@ -61,18 +83,26 @@ __device__ __forceinline__ float sm_unkey(uint32_t k) {
   return __uint_as_float(k ^ ((int)k < 0 ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ u64 sm_wave_scan(u64 v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 x = __shfl_up(v, o, 64);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
 template <int CTRL>
 __device__ __forceinline__ u64 sm_dpp(u64 v) {
   return (uint32_t)dkv_dpp_i32<CTRL>((int)(uint32_t)v) |
          ((u64)(uint32_t)dkv_dpp_i32<CTRL>((int)(uint32_t)(v >> 32)) << 32);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 sm_dpp_rows(u64 v) {  // 0 into the rows that are not meant
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false) |
+         ((u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf,
+                                                     false)
+          << 32);
+}
+__device__ __forceinline__ u64 sm_wave_scan(u64 v) {  // inclusive, as dkv_wave_scan_fast
+  v += sm_dpp<0x111>(v);
+  v += sm_dpp<0x112>(v);
+  v += sm_dpp<0x114>(v);
+  v += sm_dpp<0x118>(v);
+  v += sm_dpp_rows<0x142, 0xa>(v);
+  v += sm_dpp_rows<0x143, 0xc>(v);
+  return v;
 }
 __device__ __forceinline__ u64 sm_wave_sum(u64 v) {  // as dkv_wave_sum_fast
   v += sm_dpp<0xb1>(v);
@@ -94,42 +124,74 @@ __device__ __forceinline__ u64 sm_wave_sum(u64 v) {  // as dkv_wave_sum_fast
   return v;
 }
 
-// What is kept: every token above `key`, and those at it up to index `last`.
+// What is kept: every token above `at`, and those at it up to index `last`.
 struct Border {
   float at;
   int last;
 };
 
-template <int DT>
-__global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
-  constexpr int E = DT == DKV_F32 ? 4 : 8;  // elements of a 16-byte piece
-  __shared__ u64 sHist[SM_BINS];
-  __shared__ u64 sCand[SM_CAND];
-  __shared__ u64 sSort[SM_CAND];
-  __shared__ u64 sChunk[SM_CHUNKS];
-  __shared__ uint32_t sRoot[64];
-  __shared__ u64 sWave[SM_WAVES];
-  __shared__ u64 sWave2[SM_WAVES];
-  __shared__ float sMax[SM_WAVES];
-  __shared__ u64 sPick[4];
-  __shared__ int sN;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int V = p.V;
-  const char* base = (const char*)p.logits + (long long)row * p.ld * (DT == DKV_F32 ? 4 : 2);
-  const float t = p.temperature ? p.temperature[row] : p.temperature_all;
-  const int k = p.top_k ? p.top_k[row] : p.top_k_all;
-  const float tp = p.top_p ? p.top_p[row] : p.top_p_all;
-  const float mp = p.min_p ? p.min_p[row] : p.min_p_all;
+__device__ __forceinline__ u64 sm_get(const u64* a) {
+  return __hip_atomic_load(a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void sm_put(u64* a, u64 v) {
+  __hip_atomic_store(a, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
-  // ---- the row: pieces of 16 aligned bytes, a wave's consecutive ----
-  const int head = (int)((uintptr_t)base & 15) / (16 / E);  // elements of the first piece before it
-  const int pieces = (V + head + E - 1) / E;
-  const int per_wave = (pieces + SM_THREADS - 1) / SM_THREADS;  // of 64 pieces each
-  auto first_of = [&](int c) { return ((wave * per_wave + c) * 64 + lane) * E - head; };
-  // piece c of the thread as its words; elements outside the row are -infinity
-  auto load = [&](int c) {
-    const int i0 = first_of(c);
+// One workgroup's work on a row.
+template <int DT>
+struct RowSampler {
+  static constexpr int E = DT == DKV_F32 ? 4 : 8;  // elements of a 16-byte piece
+  const SampleParams& p;
+  SampleShared& s;
+  const int row, tid, lane, wave, V;
+  const char* base;
+  int head, rows64;  // elements of the first aligned piece before the row; its rows of 64 pieces
+  int r0, r1;        // the wave's rows of pieces
+  float t, tp, mp, u;
+  int k;
+  bool by_k, by_p;
+  bool infinite = false;
+  float m, c_hi, c_lo;  // largest logit; 64 log2(e) / t
+  u64 floor_w;
+  Border keep = {-INFINITY, -1};
+  u64 kept = 0;  // the mass of what is kept so far
+  // the histogram's running counts and masses before the thread's bins 4 tid .. 4 tid + 3, and theirs
+  u64 n_run, m_run, cnt[4], mass[4];
+
+  __device__ __forceinline__ RowSampler(const SampleParams& p_, SampleShared& s_, int row_)
+      : p(p_), s(s_), row(row_), tid(threadIdx.x), lane(threadIdx.x & 63),
+        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), V(p_.V) {
+    base = (const char*)p.logits + (long long)row * p.ld * (16 / E);
+    head = (int)((uintptr_t)base & 15) / (16 / E);
+    rows64 = (V + head + E * 64 - 1) / (E * 64);
+    t = p.temperature ? p.temperature[row] : p.temperature_all;
+    k = p.top_k ? p.top_k[row] : p.top_k_all;
+    tp = p.top_p ? p.top_p[row] : p.top_p_all;
+    mp = p.min_p ? p.min_p[row] : p.min_p_all;
+    u = p.u[row];
+    by_k = k > 0 && k < V;
+    by_p = tp < 1.f;
+    floor_w = mp > 0.f && mp <= 1.f ? (u64)ceil((double)mp * SM_ONE) : 0;
+    if (tid < 64) s.root[tid] = (uint32_t)rint(exp2(31.0 - (double)tid / 64.0));
+  }
+  // only the first token is kept
+  __device__ __forceinline__ bool greedy() const {
+    return !(t > 0.f) || k == 1 || tp <= 0.f || mp > 1.f;
+  }
+  // the workgroup takes part `part` of `parts` of the row
+  __device__ __forceinline__ void take(int part, int parts) {
+    const int per = (rows64 + parts - 1) / parts;
+    const int a = min(rows64, part * per), b = min(rows64, a + per);
+    const int pw = (b - a + SM_WAVES - 1) / SM_WAVES;
+    r0 = min(b, a + wave * pw);
+    r1 = min(b, r0 + pw);
+  }
+
+  // ---- the row: pieces of 16 aligned bytes, 64 to a row of pieces ----
+  __device__ __forceinline__ int first_of(int R) const { return (R * 64 + lane) * E - head; }
+  // the lane's piece of row R as its words; elements outside the row of logits are -infinity
+  __device__ __forceinline__ dkv_u32x4 load(int R) const {
+    const int i0 = first_of(R);
     constexpr uint32_t none = DT == DKV_F32 ? 0xff800000u
                               : DT == DKV_BF16 ? 0xff80ff80u
                                                : 0xfc00fc00u;
@@ -150,176 +212,295 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
       }
       v = dkv_u32x4{w[0], w[1], w[2], w[3]};
     }
-    return v;
-  };
-  // In a row with logits of +infinity those share the mass: they are read as 0, the others as
-  // -infinity.
-  bool infinite = false;
-  auto remap = [&](dkv_u32x4 v) {
+    if (infinite) {  // logits of +infinity share the mass: they are read as 0, the others as -infinity
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == DKV_F32) {
-        v[i] = v[i] == 0x7f800000u ? 0u : 0xff800000u;
-      } else {
-        constexpr uint32_t inf = DT == DKV_BF16 ? 0x7f80u : 0x7c00u;
-        v[i] = ((v[i] & 0xffffu) == inf ? 0u : inf | 0x8000u) |
-               ((v[i] >> 16) == inf ? 0u : (inf | 0x8000u) << 16);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == DKV_F32) {
+          v[i] = v[i] == 0x7f800000u ? 0u : 0xff800000u;
+        } else {
+          constexpr uint32_t inf = DT == DKV_BF16 ? 0x7f80u : 0x7c00u;
+          v[i] = ((v[i] & 0xffffu) == inf ? 0u : inf | 0x8000u) |
+                 ((v[i] >> 16) == inf ? 0u : (inf | 0x8000u) << 16);
+        }
       }
     }
     return v;
-  };
-  auto value = [&](const dkv_u32x4& v, int e) {
+  }
+  static __device__ __forceinline__ float value(const dkv_u32x4& v, int e) {
     if constexpr (DT == DKV_F32)
       return __uint_as_float(v[e]);
     else if constexpr (DT == DKV_BF16)
       return __uint_as_float(e & 1 ? v[e / 2] & 0xffff0000u : v[e / 2] << 16);
     else
       return dkv_f16_bits_to_f32(e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xffffu);
-  };
-  auto load_again = [&](int c) {
-    const dkv_u32x4 v = load(c);
-    return infinite ? remap(v) : v;
-  };
-  // f(c, its first token, the piece) for each of the thread's pieces, in order
-  auto each = [&](auto&& f) {
+  }
+  // f(R, first token of the lane's piece, the piece) for each of the wave's rows of pieces, in order
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll 1
-    for (int c = 0; c < per_wave; c += SM_AHEAD) {
+    for (int R = r0; R < r1; R += SM_AHEAD) {
       dkv_u32x4 v[SM_AHEAD];
 #pragma unroll
       for (int q = 0; q < SM_AHEAD; ++q)
-        if (c + q < per_wave) v[q] = load_again(c + q);
+        if (R + q < r1) v[q] = load(R + q);
 #pragma unroll
       for (int q = 0; q < SM_AHEAD; ++q)
-        if (c + q < per_wave) f(c + q, first_of(c + q), v[q]);
+        if (R + q < r1) f(R + q, first_of(R + q), v[q]);
     }
-  };
-
-  // ---- the largest logit ----
-  float m = -INFINITY;
-  each([&](int, int, const dkv_u32x4& v) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, value(v, e));  // (a NaN is passed over)
-  });
-  m = dkv_wave_max(m);
-  if (lane == 0) sMax[wave] = m;
-  if (tid == 0) sN = 0x7fffffff;
-  if (tid < 64) sRoot[tid] = (uint32_t)rint(exp2(31.0 - (double)tid / 64.0));
-  __syncthreads();
-  for (int w = 0; w < SM_WAVES; ++w) m = fmaxf(m, sMax[w]);
-  if (m == -INFINITY) {
-    if (tid == 0) p.out[row] = -1;
-    return;
   }
-  if (!(t > 0.f) || k == 1 || tp <= 0.f || mp > 1.f) {  // the first token alone
-    int at = 0x7fffffff;
-    each([&](int c, int i0, const dkv_u32x4& v) {
+
+  // ---- the largest logit of the workgroup's part, or for a greedy row that and its first index, as
+  // (key, ~index) ----
+  __device__ __forceinline__ u64 largest() {
+    float x = -INFINITY;
+    each([&](int, int, const dkv_u32x4& v) {
 #pragma unroll
-      for (int e = E - 1; e >= 0; --e)
-        if (value(v, e) == m) at = min(at, i0 + e);
+      for (int e = 0; e < E; ++e) x = fmaxf(x, value(v, e));  // (a NaN is passed over)
     });
-    if (at != 0x7fffffff) atomicMin(&sN, at);
+    x = dkv_wave_max(x);
+    u64 best = (u64)sm_key(x) << 32;
+    if (greedy()) {  // of the waves with the largest, each the first index of its own
+      int at = 0x7fffffff;
+      each([&](int, int i0, const dkv_u32x4& v) {
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if (value(v, e) == x) at = min(at, i0 + e);
+      });
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+      best |= (uint32_t)~at;
+    }
     __syncthreads();
-    if (tid == 0) p.out[row] = sN;
-    return;
+    if (lane == 0) s.wave[wave] = best;
+    __syncthreads();
+    for (int w = 0; w < SM_WAVES; ++w) best = max(best, s.wave[w]);
+    __syncthreads();
+    return best;
   }
-  if (m == INFINITY) {
-    infinite = true;
-    m = 0.f;
+  // Takes the row's largest logit; false where that decides the row (the answer is written, by one).
+  __device__ __forceinline__ bool begin(u64 best, bool write) {
+    m = sm_unkey((uint32_t)(best >> 32));
+    if (m == -INFINITY || greedy()) {
+      if (write && tid == 0) p.out[row] = m == -INFINITY ? -1 : (long long)~(uint32_t)best;
+      return false;
+    }
+    if (m == INFINITY) {
+      infinite = true;
+      m = 0.f;
+    }
+    const double c64 = 64.0 * 1.4426950408889634074 / (double)fminf(fmaxf(t, 1e-30f), 1e30f);
+    c_hi = (float)c64;
+    c_lo = (float)(c64 - (double)c_hi);
+    return true;
   }
-  const double c64 = 64.0 * 1.4426950408889634074 / (double)fminf(fmaxf(t, 1e-30f), 1e30f);
 
-  const float c_hi = (float)c64, c_lo = (float)(c64 - (double)c_hi);
-
-  // The bin of a logit; `d`: 2^31 d + SM_OFF. (NaN: the last bin.) Of max l - l, which is rounded,
-  // fp32 logits take what the rounding left; 16-bit ones are exact but for some next to 0.
-  auto bin_at = [&](float l, float& dl, float& x) {
+  // x of a logit, up to that of the last bin (that of a NaN); `dl`: max l - l as it was rounded
+  __device__ __forceinline__ float x_of(float l, float& dl) const {
     dl = m - l;
-    x = fminf(dl * c_hi, (float)(SM_BINS - 1));
-    return (int)x;
-  };
-  auto bin_of = [&](float l) {
-    float dl, x;
-    return bin_at(l, dl, x);
-  };
-  auto split = [&](float l, int& i, uint32_t& d) {
-    float dl, x;
-    i = bin_at(l, dl, x);
+    return fminf(dl * c_hi, (float)(SM_BINS - 1));
+  }
+  // The bin of a logit; `d`: 2^31 d + SM_OFF. Of max l - l fp32 logits take what the rounding left;
+  // 16-bit ones are exact but for some next to 0.
+  __device__ __forceinline__ int split(float l, uint32_t& d) const {
+    float dl;
+    const float x = x_of(l, dl);
     float r = fmaf(dl, c_lo, fmaf(dl, c_hi, -x));
     if constexpr (DT == DKV_F32) r = fmaf((m - dl) - l, c_hi, r);
     const float f = __builtin_amdgcn_fractf(x) + r;
     // 2^31 (1 - 2^(-f/64)): with g = ln2 / 64, g f - (g f)^2 / 2 + (g f)^3 / 6 - (g f)^4 / 24
     constexpr double g = 0.69314718055994530942 / 64, one = 2147483648.0;
-    const float s = fmaf(
+    const float y = fmaf(
         f, fmaf(f, fmaf(f, fmaf(f, (float)(-g * g * g * g / 24 * one), (float)(g * g * g / 6 * one)),
                         (float)(-g * g / 2 * one)),
                 (float)(g * one)),
         (float)SM_OFF);
-    d = (uint32_t)s;
-  };
+    d = (uint32_t)y;
+    return (int)x;
+  }
   // the weight of a logit, in 2^-44
-  auto weight = [&](float l) {
-    int i;
+  __device__ __forceinline__ u64 weight(float l) const {
     uint32_t d;
-    split(l, i, d);
-    const u64 w = (u64)sRoot[i & 63] * (u64)(uint32_t)((1u << 31) + SM_OFF - d);  // 2^62 w
+    const int i = split(l, d);
+    const u64 w = (u64)s.root[i & 63] * (u64)(uint32_t)((1u << 31) + SM_OFF - d);  // 2^62 w
     return i == SM_BINS - 1 ? 0ULL : w >> min((62 - SM_POINT) + (i >> 6), 63);
-  };
+  }
+  __device__ __forceinline__ u64 floored(u64 w) const { return w >= floor_w ? w : 0ULL; }
   // the mass of a bin
-  auto bin_mass = [&](int i, u64 h) {
+  __device__ __forceinline__ u64 bin_mass(int i, u64 h) const {
     const double n = (double)(h >> SM_COUNT);
     const double d = (double)(h & ((1ULL << SM_COUNT) - 1)) - n * (double)SM_OFF;
-    const double w = (double)sRoot[i & 63] * (n - d * (1.0 / 2147483648.0));  // 2^31 w
+    const double w = (double)s.root[i & 63] * (n - d * (1.0 / 2147483648.0));  // 2^31 w
     return i == SM_BINS - 1 ? 0ULL : (u64)rint(ldexp(w, SM_POINT - 31 - (i >> 6)));
-  };
+  }
+  __device__ __forceinline__ bool is_kept(float l, int i) const {
+    return l > keep.at || (l == keep.at && i <= keep.last);
+  }
 
-  const bool by_k = k > 0 && k < V, by_p = tp < 1.f;
-  Border keep = {-INFINITY, -1};
-  u64 kept = 0;  // the mass of what is kept so far
-
-  // ---- the borders inside bins: the n tokens of bins b0 .. b1 (at most SM_CAND) sorted ----
-  int sorted = 0;
-  auto sort_bins = [&](int b0, int b1) {
+  // ---- the histogram of the workgroup's part (the last bin, the rest, is left out) ----
+  __device__ __forceinline__ void histogram() {
+    for (int i = tid; i < SM_BINS; i += SM_THREADS) s.hist[i] = 0;
     __syncthreads();
-    if (tid == 0) sN = 0;
-    __syncthreads();
-    each([&](int c, int i0, const dkv_u32x4& v) {
+    each([&](int, int, const dkv_u32x4& v) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float l = value(v, e);
-        const int bin = bin_of(l);
-        if (bin >= b0 && bin <= b1) {
-          const int i = i0 + e;
-          if (i >= 0 && i < V && l == l) {
-            const int at = atomicAdd(&sN, 1);
-            if (at < SM_CAND) sCand[at] = ((u64)sm_key(l) << 32) | (uint32_t)~i;
-          }
-        }
+        uint32_t d;
+        const int i = split(value(v, e), d);
+        if (i < SM_BINS - 1) atomicAdd(&s.hist[i], (1ULL << SM_COUNT) | d);
       }
     });
     __syncthreads();
-    sorted = sN;
-    if (sorted > SM_CAND) return false;
-    for (int a = tid; a < sorted; a += SM_THREADS) {
-      const u64 x = sCand[a];
-      int rank = 0;
-      for (int b = 0; b < sorted; ++b) rank += sCand[b] > x;
-      sSort[rank] = x;
+  }
+  // running counts and masses over the histogram; the total mass is what is kept at first
+  __device__ __forceinline__ void run_sums() {
+    u64 n_sum = 0, m_sum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const u64 h = s.hist[4 * tid + q];
+      cnt[q] = h >> SM_COUNT;
+      mass[q] = bin_mass(4 * tid + q, h);
+      n_sum += cnt[q];
+      m_sum += mass[q];
+    }
+    n_run = sm_wave_scan(n_sum);
+    m_run = sm_wave_scan(m_sum);
+    if (lane == 63) {
+      s.wave[wave] = n_run;
+      s.wave2[wave] = m_run;
     }
     __syncthreads();
-    return true;
-  };
-  // Up to the j-th of the sorted tokens (j > 0), or those before which, with `before`, less than P
-  // lies; `mass`: theirs.
-  auto border_in = [&](u64 j, u64 before, double P, Border& r, u64& mass) {
+    n_run -= n_sum;
+    m_run -= m_sum;
+    kept = 0;
+    for (int w = 0; w < SM_WAVES; ++w) {
+      if (w < wave) {
+        n_run += s.wave[w];
+        m_run += s.wave2[w];
+      }
+      kept += s.wave2[w];
+    }
+  }
+  // The bin of a border: where the k-th token is (want), or the last one before which less than P lies;
+  // the count and the mass above it. SM_BINS: none.
+  __device__ __forceinline__ int find(u64 want, double P, u64& n_above, u64& m_above) {
+    __syncthreads();
+    if (tid == 0) s.pick[0] = want ? SM_BINS - 1 : SM_BINS, s.pick[1] = s.pick[2] = 0;
+    __syncthreads();
+    u64 n = n_run, x = m_run;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool rest = 4 * tid + q == SM_BINS - 1;
+      const bool here = want ? n < want && (rest || want <= n + cnt[q])
+                             : cnt[q] && (double)x < P && P <= (double)(x + mass[q]);
+      if (here) {
+        s.pick[0] = (u64)(4 * tid + q);
+        s.pick[1] = n;
+        s.pick[2] = x;
+      }
+      n += cnt[q];
+      x += mass[q];
+    }
+    __syncthreads();
+    n_above = s.pick[1];
+    m_above = s.pick[2];
+    return (int)s.pick[0];
+  }
+  // The bins b0 .. b1 in which the borders lie, and the count and the mass above them, if one list can
+  // hold their tokens. Both borders: what top-k keeps has a mass between that above its bin and that
+  // with it, which bounds top-p's bin from above.
+  __device__ __forceinline__ bool bins(int& b0, int& b1, u64& n_above, u64& m_above) {
+    if (!by_k) {
+      b0 = b1 = find(0, (double)tp * (double)kept, n_above, m_above);
+      return b0 < SM_BINS && (s.hist[b0] >> SM_COUNT) <= SM_CAND;
+    }
+    u64 n_k, m_k;
+    b0 = b1 = find((u64)k, 0.0, n_k, m_k);
+    if (b1 == SM_BINS - 1) return false;
+    const u64 n_end = n_k + (s.hist[b1] >> SM_COUNT);
+    n_above = n_k;
+    m_above = m_k;
+    if (by_p) {
+      b0 = find(0, (double)tp * (double)max(m_k, 1ULL), n_above, m_above);
+      if (b0 > b1) return false;
+    }
+    return n_end - n_above <= SM_CAND;
+  }
+
+  // ---- the mass of each row of pieces, to put(R, mass) ----
+  // LISTED: of the tokens above bin b0; those of bins b0 .. b1 go to list(key and ~index). Otherwise of
+  // the tokens that are kept.
+  template <bool LISTED, class Put, class List>
+  __device__ __forceinline__ void masses(int b0, int b1, Put&& put, List&& list) {
+    const float x0 = (float)b0, x1 = b1 == SM_BINS - 1 ? INFINITY : (float)(b1 + 1);
+    each([&](int R, int i0, const dkv_u32x4& v) {
+      u64 sum = 0;
+      if (!by_k && !by_p) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float l = value(v, e);
+          sum += l > -INFINITY ? floored(weight(l)) : 0ULL;
+        }
+      } else {
+        uint32_t mask = 0, in = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float l = value(v, e);
+          if constexpr (LISTED) {
+            float dl;
+            const float x = x_of(l, dl);
+            mask |= x < x0 ? 1u << e : 0u;
+            in |= x < x1 ? 1u << e : 0u;
+          } else {
+            mask |= l >= keep.at && is_kept(l, i0 + e) ? 1u << e : 0u;
+          }
+        }
+        auto pick = [&](uint32_t bits) {
+          const int e = bits ? __ffs((int)bits) - 1 : 0;
+          float l = value(v, 0);
+#pragma unroll
+          for (int x = 1; x < E; ++x) l = e == x ? value(v, x) : l;
+          return l;
+        };
+        in &= ~mask;
+        while (__ballot(mask != 0)) {  // one of each lane's at a time
+          const u64 w = floored(weight(pick(mask)));
+          sum += mask ? w : 0ULL;
+          mask &= mask - 1;
+        }
+        if constexpr (LISTED) {
+          while (in) {
+            const float l = pick(in);
+            const int i = i0 + __ffs((int)in) - 1;
+            if (i >= 0 && i < V && l == l) list(((u64)sm_key(l) << 32) | (uint32_t)~i);
+            in &= in - 1;
+          }
+        }
+      }
+      sum = sm_wave_sum(sum);
+      if (lane == 0) put(R, sum);
+    });
+  }
+  // the n tokens of s.cand in order
+  __device__ __forceinline__ void sort(int n) {
+    for (int a = tid; a < n; a += SM_THREADS) {
+      const u64 x = s.cand[a];
+      int rank = 0;
+      for (int b = 0; b < n; ++b) rank += s.cand[b] > x;
+      s.sort[rank] = x;
+    }
+    __syncthreads();
+  }
+  // Up to the j-th of the n sorted tokens (j > 0), or those before which, with `before`, less than P
+  // lies; returns their mass.
+  __device__ __forceinline__ u64 border_in(int n, u64 j, u64 before, double P) {
     __syncthreads();
     if (wave == 0) {
       u64 run = 0;
       int last = -1;
-      for (int a = 0; a < sorted; a += 64) {
+      for (int a = 0; a < n; a += 64) {
         const int at = a + lane;
-        const u64 w = at < sorted ? weight(sm_unkey((uint32_t)(sSort[at] >> 32))) : 0;
-        const u64 sum = sm_wave_scan(w, lane);
-        const bool in = at < sorted && (j ? (u64)at < j : (double)(before + run + sum - w) < P);
+        const u64 w = at < n ? weight(sm_unkey((uint32_t)(s.sort[at] >> 32))) : 0;
+        const u64 sum = sm_wave_scan(w);
+        const bool in = at < n && (j ? (u64)at < j : (double)(before + run + sum - w) < P);
         const u64 hit = __ballot(in);
         if (!hit) break;
         const int l = 63 - __clzll((long long)hit);
@@ -328,31 +509,44 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
         if (l < 63) break;
       }
       if (lane == 0) {
-        sPick[0] = last >= 0 ? sSort[last] : 0;
-        sPick[1] = run;
+        s.pick[0] = last >= 0 ? s.sort[last] : 0;
+        s.pick[1] = run;
       }
     }
     __syncthreads();
     // (no token at all: the j-th is a NaN; everything above them is kept)
-    r.at = sPick[0] ? sm_unkey((uint32_t)(sPick[0] >> 32)) : -INFINITY;
-    r.last = (int)~(uint32_t)sPick[0];
-    mass = sPick[1];
-  };
+    keep.at = s.pick[0] ? sm_unkey((uint32_t)(s.pick[0] >> 32)) : -INFINITY;
+    keep.last = (int)~(uint32_t)s.pick[0];
+    return s.pick[1];
+  }
+  // The borders among the n sorted tokens, above which count and mass are given; the kept ones' masses
+  // join their rows of pieces.
+  __device__ __forceinline__ void borders(int n, u64 n_above, u64 m_above) {
+    if (by_k) kept = m_above + border_in(n, (u64)k - n_above, 0, 0.0);
+    if (by_p) kept = m_above + border_in(n, 0, m_above, (double)tp * (double)kept);
+    for (int a = tid; a < n; a += SM_THREADS) {
+      const float l = sm_unkey((uint32_t)(s.sort[a] >> 32));
+      const int i = (int)~(uint32_t)s.sort[a];
+      if (is_kept(l, i)) atomicAdd(&s.chunk[(i + head) / (E * 64)], floored(weight(l)));
+    }
+    __syncthreads();
+  }
 
   // ---- the border by digits of the keys (11, 11, 10 bits): for a bin of too many tokens ----
   // Level by level the bin in which the border lies, among the tokens that share the digits found so
   // far; then the index of the last of the equal ones that are kept. Clears the histogram.
-  auto by_digits = [&](u64 want, double P, Border& r, u64& mass_kept) {
+  __device__ __forceinline__ void by_digits(u64 want, double P) {
     u64 above = 0, m_above = 0;
     uint32_t found = 0;
     u64 ties = 0;
+#pragma unroll 1
     for (int level = 0; level < 3; ++level) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
       const int bits = level == 2 ? 10 : 11;
       __syncthreads();
-      for (int i = tid; i < SM_BINS; i += SM_THREADS) sHist[i] = 0;
+      for (int i = tid; i < SM_BINS; i += SM_THREADS) s.hist[i] = 0;
       __syncthreads();
-      each([&](int c, int i0, const dkv_u32x4& v) {
+      each([&](int, int i0, const dkv_u32x4& v) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float l = fmaxf(value(v, e), -INFINITY);
@@ -361,36 +555,36 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
           const uint32_t key = sm_key(l);
           if (level && (key >> (shift + bits)) != found) continue;
           const int bin = (int)((key >> shift) & ((1u << bits) - 1));
-          atomicAdd(&sHist[bin], weight(l));
-          atomicAdd(&sHist[2048 + bin], 1ULL);
+          atomicAdd(&s.hist[bin], weight(l));
+          atomicAdd(&s.hist[2048 + bin], 1ULL);
         }
       });
       __syncthreads();
       if (tid == 0) {  // the bins from the top
-        u64 cnt = above, mass = m_above, cnt_at = 0, mass_at = 0;
+        u64 n = above, x = m_above, n_at = 0, x_at = 0;
         int at = 0;
         for (int bin = (1 << bits) - 1; bin >= 0; --bin) {
-          if (!sHist[2048 + bin]) continue;
-          if (!(want ? cnt < want : (double)mass < P)) break;
+          if (!s.hist[2048 + bin]) continue;
+          if (!(want ? n < want : (double)x < P)) break;
           at = bin;
-          cnt_at = cnt;
-          mass_at = mass;
-          cnt += sHist[2048 + bin];
-          mass += sHist[bin];
+          n_at = n;
+          x_at = x;
+          n += s.hist[2048 + bin];
+          x += s.hist[bin];
         }
-        sPick[0] = (u64)at;
-        sPick[1] = cnt_at;
-        sPick[2] = mass_at;
-        sPick[3] = sHist[2048 + at];
+        s.pick[0] = (u64)at;
+        s.pick[1] = n_at;
+        s.pick[2] = x_at;
+        s.pick[3] = s.hist[2048 + at];
       }
       __syncthreads();
-      found = (found << bits) | (uint32_t)sPick[0];
-      above = sPick[1];
-      m_above = sPick[2];
-      ties = sPick[3];
+      found = (found << bits) | (uint32_t)s.pick[0];
+      above = s.pick[1];
+      m_above = s.pick[2];
+      ties = s.pick[3];
     }
-    r.at = sm_unkey(found);
-    const u64 w = weight(r.at);
+    keep.at = sm_unkey(found);
+    const u64 w = weight(keep.at);
     if (want) {
       ties = min(ties, want - above);
     } else if (w > 0) {
@@ -404,229 +598,119 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
       }
       ties = lo;
     }
-    mass_kept = m_above + ties * w;
-    // the index of the last of them: equal ones by piece row, in order
-    __syncthreads();
-    for (int i = tid; i < SM_CHUNKS; i += SM_THREADS) sChunk[i] = 0;
-    __syncthreads();
-    each([&](int c, int i0, const dkv_u32x4& v) {
-      int n = 0;
+    kept = m_above + ties * w;
+    // the index of the last of them: equal ones by row of pieces, in order
+    auto equal = [&](int i0, const dkv_u32x4& v) {
+      uint32_t mask = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int i = i0 + e;
-        n += i >= 0 && i < V && fmaxf(value(v, e), -INFINITY) == r.at;
+        if (i >= 0 && i < V && fmaxf(value(v, e), -INFINITY) == keep.at) mask |= 1u << e;
       }
-      if (n) atomicAdd(&sChunk[wave * per_wave + c], (u64)n);
+      return mask;
+    };
+    __syncthreads();
+    for (int i = tid; i < rows64; i += SM_THREADS) s.chunk[i] = 0;
+    __syncthreads();
+    each([&](int R, int i0, const dkv_u32x4& v) {
+      const uint32_t mask = equal(i0, v);
+      if (mask) atomicAdd(&s.chunk[R], (u64)__popc(mask));
     });
     __syncthreads();
     if (tid == 0) {
-      u64 cnt = 0;
+      u64 n = 0;
       int at = 0;
-      for (; at < SM_WAVES * per_wave - 1 && cnt + sChunk[at] < ties; ++at) cnt += sChunk[at];
-      sPick[0] = (u64)at;
-      sPick[1] = ties - cnt;  // the one of them in that piece row
+      for (; at < rows64 - 1 && n + s.chunk[at] < ties; ++at) n += s.chunk[at];
+      s.pick[0] = (u64)at;
+      s.pick[1] = ties - n;  // the one of them in that row of pieces
     }
     __syncthreads();
-    if ((int)sPick[0] / per_wave == wave) {
-      const int c = (int)sPick[0] % per_wave;
-      const dkv_u32x4 v = load_again(c);
-      const int i0 = first_of(c);
-      uint32_t mask = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = i0 + e;
-        if (i >= 0 && i < V && fmaxf(value(v, e), -INFINITY) == r.at) mask |= 1u << e;
-      }
-      const u64 run = sm_wave_scan((u64)__popc(mask), lane), want_at = sPick[1];
+    if (wave == 0) {
+      const int R = (int)s.pick[0], i0 = first_of(R);
+      uint32_t mask = equal(i0, load(R));
+      const u64 run = sm_wave_scan((u64)__popc(mask)), at = s.pick[1];
       const u64 before = run - (u64)__popc(mask);
-      if (before < want_at && want_at <= run) {
-        for (u64 x = before + 1; x < want_at; ++x) mask &= mask - 1;
-        sPick[2] = (u64)(i0 + __ffs((int)mask) - 1);
+      if (before < at && at <= run) {
+        for (u64 x = before + 1; x < at; ++x) mask &= mask - 1;
+        s.pick[2] = (u64)(i0 + __ffs((int)mask) - 1);
       }
     }
     __syncthreads();
-    r.last = (int)sPick[2];
+    keep.last = (int)s.pick[2];
     __syncthreads();
-  };
+  }
 
-  if (by_k || by_p) {
-    // ---- the histogram ----
-    for (int i = tid; i < SM_BINS; i += SM_THREADS) sHist[i] = 0;
-    __syncthreads();
-    each([&](int c, int i0, const dkv_u32x4& v) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        int i;
-        uint32_t d;
-        split(value(v, e), i, d);
-        if (i < SM_BINS - 1) atomicAdd(&sHist[i], (1ULL << SM_COUNT) | d);
-      }
-    });
-    __syncthreads();
-    // running counts and masses: thread i has bins 4i .. 4i + 3 (the last bin is the rest)
-    u64 cnt[4], mass[4], nsum = 0, msum = 0;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const u64 h = sHist[4 * tid + q];
-      cnt[q] = h >> SM_COUNT;
-      mass[q] = bin_mass(4 * tid + q, h);
-      nsum += cnt[q];
-      msum += mass[q];
-    }
-    u64 nrun = sm_wave_scan(nsum, lane), mrun = sm_wave_scan(msum, lane);
-    if (lane == 63) {
-      sWave[wave] = nrun;
-      sWave2[wave] = mrun;
-    }
-    __syncthreads();
-    u64 total = 0;
-    nrun -= nsum;
-    mrun -= msum;
-    for (int w = 0; w < SM_WAVES; ++w) {
-      if (w < wave) {
-        nrun += sWave[w];
-        mrun += sWave2[w];
-      }
-      total += sWave2[w];
-    }
-    kept = total;
-    // The bin of a border: where the k-th token is (want), or the last one before which less than P
-    // lies; the count and the mass above it. SM_BINS: none.
-    auto find = [&](u64 want, double P, u64& n_above, u64& m_above) {
-      __syncthreads();
-      if (tid == 0) sPick[0] = want ? SM_BINS - 1 : SM_BINS, sPick[1] = sPick[2] = 0;
-      __syncthreads();
-      u64 n = nrun, s = mrun;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bool rest = 4 * tid + q == SM_BINS - 1;
-        const bool here = want ? n < want && (rest || want <= n + cnt[q])
-                               : cnt[q] && (double)s < P && P <= (double)(s + mass[q]);
-        if (here) {
-          sPick[0] = (u64)(4 * tid + q);
-          sPick[1] = n;
-          sPick[2] = s;
-        }
-        n += cnt[q];
-        s += mass[q];
-      }
-      __syncthreads();
-      n_above = sPick[1];
-      m_above = sPick[2];
-      return (int)sPick[0];
-    };
-    bool digits = false, done = false;
-    u64 n_k = 0, m_k = 0;
-    const int bin_k = by_k ? find((u64)k, 0.0, n_k, m_k) : SM_BINS;
-    if (by_k && by_p && bin_k < SM_BINS - 1) {
-      // What top-k keeps has a mass between m_k and that with its bin's; the bins in which the border
-      // of top-p can lie then, sorted with top-k's where they are few: one pass for both.
-      u64 n_p, m_p;
-      const int bin_p = find(0, (double)tp * (double)max(m_k, 1ULL), n_p, m_p);
-      const u64 h = sHist[bin_k] >> SM_COUNT;
-      if (bin_p <= bin_k && n_k + h - n_p <= SM_CAND && sort_bins(bin_p, bin_k)) {
-        u64 in;
-        border_in((u64)k - n_p, 0, 0.0, keep, in);
-        kept = m_p + in;
-        const double P = (double)tp * (double)kept;
-        border_in(0, m_p, P, keep, in);
-        kept = m_p + in;
-        done = true;
-      }
-    }
+  // ---- the borders one after the other, and the masses of what is kept: where one list does not
+  // do. The workgroup has the whole row and its histogram. ----
+  __device__ __forceinline__ void one_by_one() {
+    bool digits = false;
 #pragma unroll 1
-    for (int step = 0; step < 2 && !done; ++step) {  // top-k, then top-p of what it keeps
+    for (int step = 0; step < 2; ++step) {  // top-k, then top-p of what it keeps
       if (step == 0 ? !by_k : !by_p) continue;
       const u64 want = step == 0 ? (u64)k : 0;
       const double P = step == 0 ? 0.0 : (double)tp * (double)kept;
-      u64 n_above = 0, above = 0;
-      const int bin = digits ? SM_BINS : find(want, P, n_above, above);
-      if (bin < SM_BINS && sort_bins(bin, bin)) {
-        u64 in;
-        border_in(want ? want - n_above : 0, above, P, keep, in);
-        kept = above + in;
+      u64 n_above = 0, m_above = 0;
+      const int bin = digits ? SM_BINS : find(want, P, n_above, m_above);
+      if (bin < SM_BINS) {
+        __syncthreads();
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        masses<true>(bin, bin, [](int, u64) {}, [&](u64 x) {
+          const int at = atomicAdd(&s.n, 1);
+          if (at < SM_CAND) s.cand[at] = x;
+        });
+        __syncthreads();
+      }
+      if (bin < SM_BINS && s.n <= SM_CAND) {
+        const int n = s.n;
+        sort(n);
+        kept = m_above + border_in(n, want ? want - n_above : 0, m_above, P);
       } else {
-        by_digits(want, P, keep, kept);
+        by_digits(want, P);
         digits = true;
       }
     }
+    __syncthreads();
+    masses<false>(0, 0, [&](int R, u64 w) { s.chunk[R] = w; }, [](u64) {});
+    __syncthreads();
   }
 
-  // ---- the kept mass of each row of 64 pieces ----
-  const u64 floor_w = mp > 0.f ? (u64)ceil((double)mp * SM_ONE) : 0;
-  auto is_kept = [&](float l, int i) { return l > keep.at || (l == keep.at && i <= keep.last); };
-  auto floored = [&](u64 w) { return w >= floor_w ? w : 0ULL; };
-  __syncthreads();
-  each([&](int c, int i0, const dkv_u32x4& v) {
-    u64 s = 0;
-    if (!by_k && !by_p) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float l = value(v, e);
-        s += l > -INFINITY ? floored(weight(l)) : 0ULL;
-      }
-    } else {
-      // the few that are kept, one of each lane's at a time
-      uint32_t mask = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float l = value(v, e);
-        mask |= l >= keep.at && is_kept(l, i0 + e) ? 1u << e : 0u;
-      }
-      while (__ballot(mask != 0)) {
-        const int e = mask ? __ffs((int)mask) - 1 : 0;
-        float l = value(v, 0);
-#pragma unroll
-        for (int x = 1; x < E; ++x) l = e == x ? value(v, x) : l;
-        const u64 w = floored(weight(l));
-        s += mask ? w : 0ULL;
-        mask &= mask - 1;
-      }
+  // ---- the token in which u times the mass lies ----
+  __device__ __forceinline__ void finish() {
+    const int share = (rows64 + SM_THREADS - 1) / SM_THREADS;
+    u64 own = 0;
+    for (int i = tid * share; i < min(rows64, (tid + 1) * share); ++i) own += s.chunk[i];
+    u64 run = sm_wave_scan(own);
+    if (lane == 63) s.wave[wave] = run;
+    __syncthreads();
+    u64 all = 0;
+    run -= own;
+    for (int w = 0; w < SM_WAVES; ++w) {
+      if (w < wave) run += s.wave[w];
+      all += s.wave[w];
     }
-    s = sm_wave_sum(s);
-    if (lane == 0) sChunk[wave * per_wave + c] = s;
-  });
-  __syncthreads();
-  // ---- the row of pieces in which u * mass lies ----
-  const int rows = SM_WAVES * per_wave;
-  const int share = (rows + SM_THREADS - 1) / SM_THREADS;
-  u64 own = 0;
-  for (int i = tid * share; i < min(rows, (tid + 1) * share); ++i) own += sChunk[i];
-  u64 run = sm_wave_scan(own, lane);
-  if (lane == 63) sWave[wave] = run;
-  __syncthreads();
-  u64 all = 0;
-  run -= own;
-  for (int w = 0; w < SM_WAVES; ++w) {
-    if (w < wave) run += sWave[w];
-    all += sWave[w];
-  }
-  const float uu = p.u[row];
-  const double U = uu > 0.f ? (double)uu * (double)all : 0.0;
-  const u64 target = U < (double)all ? min((u64)U, all - 1) : all - 1;
-  for (int i = tid * share; i < min(rows, (tid + 1) * share); ++i) {
-    if (run <= target && target < run + sChunk[i]) {
-      sPick[0] = (u64)i;
-      sPick[1] = run;
+    const double U = u > 0.f ? (double)u * (double)all : 0.0;
+    const u64 target = U < (double)all ? min((u64)U, all - 1) : all - 1;
+    for (int i = tid * share; i < min(rows64, (tid + 1) * share); ++i) {
+      if (run <= target && target < run + s.chunk[i]) {
+        s.pick[0] = (u64)i;
+        s.pick[1] = run;
+      }
+      run += s.chunk[i];
     }
-    run += sChunk[i];
-  }
-  __syncthreads();
-  // ---- and the token ----
-  const int hit = (int)sPick[0];
-  if (hit / per_wave == wave) {
-    const int c = hit % per_wave;
-    const dkv_u32x4 v = load_again(c);
-    const int i0 = first_of(c);
-    u64 w[E], s = 0;
+    __syncthreads();
+    if (wave != 0) return;
+    const int R = (int)s.pick[0], i0 = first_of(R);
+    const dkv_u32x4 v = load(R);
+    u64 w[E], sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float l = value(v, e);
       w[e] = is_kept(l, i0 + e) ? floored(weight(l)) : 0ULL;
-      s += w[e];
+      sum += w[e];
     }
-    u64 at = sPick[1] + sm_wave_scan(s, lane) - s;
-    if (at <= target && target < at + s) {
+    u64 at = s.pick[1] + sm_wave_scan(sum) - sum;
+    if (at <= target && target < at + sum) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         if (at <= target && target < at + w[e]) p.out[row] = (long long)(i0 + e);
@@ -634,20 +718,166 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(SampleParams p) {
       }
     }
   }
+};
+
+// A row per workgroup.
+template <int DT>
+__global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(SampleParams p) {
+  __shared__ SampleShared s;
+  RowSampler<DT> r(p, s, blockIdx.x);
+  r.take(0, 1);
+  if (!r.begin(r.largest(), true)) return;
+  if (r.by_k || r.by_p) {
+    r.histogram();
+    r.run_sums();
+    int b0, b1;
+    u64 n_above, m_above;
+    if (r.bins(b0, b1, n_above, m_above)) {
+      if (threadIdx.x == 0) s.n = 0;
+      __syncthreads();
+      r.template masses<true>(b0, b1, [&](int R, u64 w) { s.chunk[R] = w; },
+                              [&](u64 x) { s.cand[atomicAdd(&s.n, 1)] = x; });
+      __syncthreads();
+      const int n = s.n;
+      r.sort(n);
+      r.borders(n, n_above, m_above);
+    } else {
+      r.one_by_one();
+    }
+  } else {
+    r.template masses<false>(0, 0, [&](int R, u64 w) { s.chunk[R] = w; }, [](u64) {});
+    __syncthreads();
+  }
+  r.finish();
+}
+
+// A part of a row per workgroup, a launch per pass: 0 the maxima (and a clear workspace), 1 the
+// histogram, 2 the masses, after which the row's last workgroup to arrive ends it.
+template <int DT, int PASS>
+__global__ __launch_bounds__(SM_THREADS) void sample_parts_kernel(SampleParams p) {
+  __shared__ SampleShared s;
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x;
+  u64* ws = p.ws + (long long)row * SM_WS;
+  RowSampler<DT> r(p, s, row);
+  r.take(part, p.parts);
+  if constexpr (PASS == 0) {
+    const u64 best = r.largest();
+    if (tid == 0) ws[part] = best;
+    if (part == 0 && tid == 0) ws[SM_WS_N] = 0;
+    for (int i = part * SM_THREADS + tid; i < SM_BINS; i += p.parts * SM_THREADS)
+      ws[SM_WS_HIST + i] = 0;
+    return;
+  }
+  u64 best = (tid & 63) < p.parts ? ws[tid & 63] : 0;
+  dkv_u64x2 h[2];  // the histogram's bins 4 tid .. 4 tid + 3
+  if constexpr (PASS == 2) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) h[q] = ((const dkv_u64x2*)(ws + SM_WS_HIST))[2 * tid + q];
+  }
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
+  best = __shfl(best, 0, 64);
+  __syncthreads();  // (the table of roots)
+  if (!r.begin(best, PASS == 1 && part == 0)) return;
+  const bool filters = r.by_k || r.by_p;
+  if constexpr (PASS == 1) {
+    if (!filters) return;
+    r.histogram();
+    for (int i = tid; i < SM_BINS; i += SM_THREADS)
+      if (s.hist[i]) atomicAdd(&ws[SM_WS_HIST + i], s.hist[i]);
+    return;
+  }
+  int b0 = 0, b1 = 0;
+  u64 n_above = 0, m_above = 0;
+  bool listed = false;
+  if (filters) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) ((dkv_u64x2*)s.hist)[2 * tid + q] = h[q];
+    __syncthreads();
+    r.run_sums();
+    listed = r.bins(b0, b1, n_above, m_above);
+    if (!listed) {  // one workgroup goes on with the whole row
+      if (part) return;
+      r.take(0, 1);
+      r.one_by_one();
+      r.finish();
+      return;
+    }
+  }
+  uint32_t* counts = (uint32_t*)(ws + SM_WS_N);  // listed tokens, parts that are done
+  auto put = [&](int R, u64 w) { sm_put(ws + SM_WS_CHUNK + R, w); };
+  if (listed)
+    r.template masses<true>(b0, b1, put, [&](u64 x) {
+      sm_put(ws + SM_WS_CAND + atomicAdd(&counts[0], 1u), x);
+    });
+  else
+    r.template masses<false>(0, 0, put, [](u64) {});
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) s.last = atomicAdd(&counts[1], 1u) == (uint32_t)p.parts - 1;
+  __syncthreads();
+  if (!s.last) return;
+  const int n = listed ? (int)__hip_atomic_load(&counts[0], __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT)
+                       : 0;
+  for (int i = tid; i < r.rows64; i += SM_THREADS) s.chunk[i] = sm_get(ws + SM_WS_CHUNK + i);
+  for (int i = tid; i < n; i += SM_THREADS) s.cand[i] = sm_get(ws + SM_WS_CAND + i);
+  __syncthreads();
+  if (listed) {
+    r.sort(n);
+    r.borders(n, n_above, m_above);
+  }
+  r.finish();
+}
+
+// Workgroups of a row: rows for half the CUs have one each, fewer are cut so that the workgroups fill
+// the chip, if each of the 16 waves would have ten rows of pieces or more. The launches and the parts'
+// meeting cost 8 us. us, top-p, cut / whole: one row of 128256 bf16 24.0 / 58.8, 100 rows 51 / 64; 37
+// rows of 50257 fp32 27.6 / 34.5; one row of 32000 bf16 21.2 / 23.5 but with top-k 19.7 / 18.4; 64 rows of
+// 32000 fp32 27.4 / 25.6.
+int sample_parts(int rows, int V, int dtype) {
+  const int tokens = (dtype == DKV_F32 ? 4 : 8) * 64;
+  const int rows64 = (V + tokens - 1) / tokens;
+  if (rows64 < 10 * SM_WAVES || rows < 1) return 1;
+  int n = 256 / rows;
+  if (n > SM_PARTS) n = SM_PARTS;
+  if (n > rows64 / (2 * SM_WAVES)) n = rows64 / (2 * SM_WAVES);
+  return n < 1 ? 1 : n;
+}
+
+template <int DT>
+void launch_sample(const SampleParams& p, int rows, hipStream_t st) {
+  const dim3 block(SM_THREADS), grid((unsigned)(rows * p.parts));
+  if (p.parts == 1) {
+    hipLaunchKernelGGL(sample_rows_kernel<DT>, grid, block, 0, st, p);
+    return;
+  }
+  hipLaunchKernelGGL((sample_parts_kernel<DT, 0>), grid, block, 0, st, p);
+  hipLaunchKernelGGL((sample_parts_kernel<DT, 1>), grid, block, 0, st, p);
+  hipLaunchKernelGGL((sample_parts_kernel<DT, 2>), grid, block, 0, st, p);
 }
 
 }  // namespace
+
+extern "C" long long dkv_sample_workspace_bytes(int dtype, int rows, int V) {
+  if (rows <= 0 || V <= 0 || V > SM_MAX_V) return 0;
+  return sample_parts(rows, V, dtype) > 1 ? (long long)rows * SM_WS * (long long)sizeof(u64) : 0;
+}
 
 extern "C" int dkv_sample_tokens(void* stream, int dtype, const void* logits, long long ld,
                                  int rows, int V, const float* u, const float* temperature,
                                  float temperature_all, const int* top_k, int top_k_all,
                                  const float* top_p, float top_p_all, const float* min_p,
-                                 float min_p_all, long long* out) {
+                                 float min_p_all, void* workspace, long long workspace_bytes,
+                                 long long* out) {
   if (dtype != DKV_F16 && dtype != DKV_BF16 && dtype != DKV_F32) return DKV_E_UNSUPPORTED;
   if (rows < 0 || V <= 0) return DKV_E_ARG;
   if (V > SM_MAX_V) return DKV_E_UNSUPPORTED;
   if (rows == 0) return DKV_OK;
   if (!logits || !u || !out || ld < 0 || (rows > 1 && ld < V)) return DKV_E_ARG;
+  const long long need = dkv_sample_workspace_bytes(dtype, rows, V);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return DKV_E_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return DKV_E_UNSUPPORTED;
   SampleParams p;
   p.logits = logits;
   p.ld = ld;
@@ -662,14 +892,15 @@ extern "C" int dkv_sample_tokens(void* stream, int dtype, const void* logits, lo
   p.top_p_all = top_p_all;
   p.min_p_all = min_p_all;
   p.out = out;
+  p.ws = (u64*)workspace;
+  p.parts = sample_parts(rows, V, dtype);
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)rows), block(SM_THREADS);
   if (dtype == DKV_F32)
-    hipLaunchKernelGGL(sample_kernel<DKV_F32>, grid, block, 0, st, p);
+    launch_sample<DKV_F32>(p, rows, st);
   else if (dtype == DKV_BF16)
-    hipLaunchKernelGGL(sample_kernel<DKV_BF16>, grid, block, 0, st, p);
+    launch_sample<DKV_BF16>(p, rows, st);
   else
-    hipLaunchKernelGGL(sample_kernel<DKV_F16>, grid, block, 0, st, p);
+    launch_sample<DKV_F16>(p, rows, st);
   DKV_HIP_CHECK_LAUNCH();
   return DKV_OK;
 }

@@ -667,12 +667,15 @@ int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st, 
  * before which less than p of the kept mass lies (p >= 1: all), min_p those with w_i >= min_p, the
  * first token always; the result is the first token in index order up to which the kept mass exceeds
  * u times all of it. temperature <= 0: the first token. NaN counts as -inf; a row of -inf alone
- * gives -1.
+ * gives -1. The workspace holds dkv_sample_workspace_bytes(...) bytes, with any contents, 16-byte
+ * aligned; it may be null where that is 0. Calls that share it must not overlap.
  */
+long long dkv_sample_workspace_bytes(int dtype, int rows, int V);
 int dkv_sample_tokens(void* stream, int dtype, const void* logits, long long ld, int rows, int V,
                       const float* u, const float* temperature, float temperature_all,
                       const int* top_k, int top_k_all, const float* top_p, float top_p_all,
-                      const float* min_p, float min_p_all, long long* out);
+                      const float* min_p, float min_p_all,
+                      void* workspace, long long workspace_bytes, long long* out);
 
 #ifdef __cplusplus
 }

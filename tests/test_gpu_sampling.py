@@ -83,7 +83,8 @@ SETTINGS = {
 @pytest.mark.parametrize("name", list(SETTINGS))
 def test_settings(dev, name, dtype):
     print(f"[gpu] sample {name} {dtype}", flush=True)
-    for rows, V in ((9, 1000), (3, 32000), (2, 50257)):
+    # short rows and many rows have a workgroup each, the others several
+    for rows, V in ((9, 1000), (3, 32000), (2, 50257), (40, 20000), (150, 9001)):
         x, u, _ = _inputs(dev, rows, V, dtype, 7 * V + rows)
         _check(x, u, **SETTINGS[name])
 
@@ -123,6 +124,9 @@ def test_ties(dev, dtype):
     g = torch.Generator().manual_seed(9)
     x = torch.randint(-2, 3, (16, 4099), generator=g).to(DT[dtype]).to(dev)
     u = torch.rand(16, generator=g).to(dev)
+    wide = torch.randint(-2, 3, (3, 60001), generator=g).to(DT[dtype]).to(dev)
+    for kw in (dict(top_k=9000), dict(top_p=0.6), dict(top_k=40000, top_p=0.7), {}):
+        _check(wide, u[:3], **kw)
     for kw in (dict(top_k=1), dict(top_k=2), dict(top_k=900), dict(top_k=4098), dict(top_p=0.5),
                dict(top_p=0.999), dict(top_k=1700, top_p=0.7), dict(min_p=1.0), dict(min_p=0.3),
                dict(top_p=1e-6), dict(temperature=0.0), {}):

@@ -188,7 +188,7 @@ def test_sampling_refusals():
         sample_tokens(torch.zeros(1, (1 << 19) + 1), u[:1])
     lib = _lib.load()
     call = lambda dt, rows, v, ld=8: lib.dkv_sample_tokens(  # noqa: E731
-        None, dt, None, ld, rows, v, None, None, 1.0, None, 0, None, 1.0, None, 0.0, None)
+        None, dt, None, ld, rows, v, None, None, 1.0, None, 0, None, 1.0, None, 0.0, None, 0, None)
     assert call(0, 1, 8) == _lib.DKV_E_ARG and call(0, -1, 8) == _lib.DKV_E_ARG
     assert call(9, 1, 8) == _lib.DKV_E_UNSUPPORTED and call(0, 1, 1 << 20) == _lib.DKV_E_UNSUPPORTED
     assert call(0, 0, 8) == _lib.DKV_OK and call(0, 1, 0) == _lib.DKV_E_ARG
