@@ -676,7 +676,17 @@ __global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
 // (NW = 8: half of one) through a resource that ends with the request's keys. S^T = K Q^T on
 // 16x16x32 MFMA (a lane then holds one row's scores for 16 keys); softmax in fp32, the running
 // maximum raised only when a tile's exceeds it by more than 2^8; P V on 16x16x32 MFMA with the
-// weights rounded once to the cache's type.
+// weights rounded once to the cache's type and summed as rounded: a weight is off by at most half a
+// step, as the output is by its own rounding, and as the errors are of either sign, together they
+// come to 1.25 to 1.4 times the output's alone (measured against 64 bits; a second product with what
+// the rounding left would take half as many products again, which are the prompts' bound).
+//
+// Bound by the SIMDs' issue slots: per wave and tile (QB = 2) 66 products of 16 cycles beside ~190
+// vector instructions, 32 of them exponentials of 16 cycles; two waves a SIMD fill one's products with
+// the other's vector work in part. Four prompts of 2048 tokens (32 and 8 heads): 166 us, 0.83 PFLOP/s,
+// one of 8192: 513 us, 1.07 PFLOP/s, where a large library product reaches 1.23. (Sums by additions and
+// equal priorities: 169 and 527.) A deeper ring (four tiles of 64 or 32 keys) gains nothing: 1x4, 512
+// tokens at 1024: 23.0 us with two tiles of 64 or four, 27.2 with four of 32.
 constexpr int CK = 64;                      // keys per tile
 constexpr int CTILE_BYTES = CK * PG_DH * 2;
 constexpr float C_RESCALE = 8.f;            // log2 units
@@ -888,11 +898,16 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[qb][i] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run[QB], l_run[QB];  // log2 units
+  // running maxima (log2 units), and the sums of the weights as one more row of P V: a product with
+  // ones, of the weights as they were rounded (every element holds it)
+  float m_run[QB];
+  dkv_f32x4 sum[QB];
+  constexpr uint32_t one2 = DT == DKV_BF16 ? 0x3f803f80u : 0x3c003c00u;
+  const dkv_u32x4 ones = {one2, one2, one2, one2};
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     m_run[qb] = -1.0e30f;
-    l_run[qb] = 0.f;
+    sum[qb] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   // S^T of key block kb: A = K rows (lane: key 16kb + n, dims 32s + 8g .. +8), B = Q^T; lane (row n,
@@ -923,6 +938,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     const uint32_t kt = dkv_lds_addr(sK(t & 1));
     const uint32_t vt = dkv_lds_addr(sV(t & 1)) + vrd;
     dkv_f32x4 z[QB][4];
+    __builtin_amdgcn_s_setprio(1);  // (the SIMD's other wave has its vector work meanwhile)
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
 #pragma unroll
@@ -934,6 +950,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_mfma32<DT>(a, qop[qb][s], z[qb][kb]);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     if (key0 + CK - 1 > w_first || key0 + CK > r.len || gone) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
@@ -974,7 +991,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         const float m_new = dkv_max2(m_run[qb], tmax[qb]);
         const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
         m_run[qb] = m_new;
-        l_run[qb] *= alpha;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[qb][u] *= alpha;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -990,7 +1008,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       for (int u = 0; u < 4; ++u) {
         pu[u] = __builtin_amdgcn_exp2f(
             __builtin_fmaf(z[qb][2 * j + kk][u], p.scale_log2, -m_run[qb]));
-        l_run[qb] += pu[u];
       }
       typedef __attribute__((ext_vector_type(2))) float f32x2;
       if constexpr (DT == DKV_BF16) {
@@ -1014,6 +1031,10 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         if (j == 0) vread(1, db);
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) acc[qb][db] = dkv_mfma32<DT>(aop, bp[j][qb], acc[qb][db]);
+        if (db == 7) {
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) sum[qb] = dkv_mfma32<DT>(ones, bp[j][qb], sum[qb]);
+        }
         if (j == 0 && db % (4 / QB) == 4 / QB - 1)
           probs(1, db / (4 / QB) % 2, db / (8 / QB));
       }
@@ -1026,9 +1047,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
                                (PG_DH + 2);
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    float l = l_run[qb];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    const float l = sum[qb][0];
     const int R = wq0 + 16 * qb + n;
     const int i = R / p.hpg, h = R - i * p.hpg;
     // the largest magnitude, infinite or NaN where a value is (a sum of products by 0)
