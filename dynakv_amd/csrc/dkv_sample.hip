@@ -35,7 +35,7 @@ constexpr int SM_THREADS = 1024;
 constexpr int SM_WAVES = SM_THREADS / 64;
 constexpr int SM_POINT = 44;             // bits after the point of a weight
 constexpr int SM_MAX_V = 1 << 19;        // weights of at most 1: sums below 2^63
-constexpr int SM_AHEAD = 4;              // 16-byte pieces that a thread has in flight
+constexpr int SM_AHEAD = 2;              // 16-byte pieces that a thread has in flight
 constexpr int SM_BINS = 4096;            // bins of 1/64 in log2 of the weight; the last: the rest
 constexpr int SM_CAND = 2048;            // tokens of a border's bin that are sorted
 constexpr int SM_CHUNKS = SM_MAX_V / 4 / 64 + 2;  // rows of 64 pieces (1 KB) of a row of logits
@@ -67,7 +67,7 @@ constexpr int SM_WS_N = SM_PARTS, SM_WS_HIST = 32, SM_WS_CAND = SM_WS_HIST + SM_
 static_assert(SM_WS % 2 == 0 && SM_WS_HIST % 2 == 0, "16-byte accesses");
 
 struct SampleShared {
-  __attribute__((aligned(16))) u64 hist[SM_BINS];
+  __attribute__((aligned(16))) u64 hist[SM_BINS + 64];  // and 64 that catch the rest
   u64 cand[SM_CAND], sort[SM_CAND], chunk[SM_CHUNKS];
   u64 wave[SM_WAVES], wave2[SM_WAVES], pick[4];
   uint32_t root[64];
@@ -307,13 +307,9 @@ struct RowSampler {
     float r = fmaf(dl, c_lo, fmaf(dl, c_hi, -x));
     if constexpr (DT == DKV_F32) r = fmaf((m - dl) - l, c_hi, r);
     const float f = __builtin_amdgcn_fractf(x) + r;
-    // 2^31 (1 - 2^(-f/64)): with g = ln2 / 64, g f - (g f)^2 / 2 + (g f)^3 / 6 - (g f)^4 / 24
-    constexpr double g = 0.69314718055994530942 / 64, one = 2147483648.0;
-    const float y = fmaf(
-        f, fmaf(f, fmaf(f, fmaf(f, (float)(-g * g * g * g / 24 * one), (float)(g * g * g / 6 * one)),
-                        (float)(-g * g / 2 * one)),
-                (float)(g * one)),
-        (float)SM_OFF);
+    // 2^31 (1 - 2^(-f/64)) by the cubic of least error over 0 .. 1 through 0 (0.02 of a unit; the
+    // coefficients' own rounding 0.4)
+    const float y = fmaf(f, fmaf(f, fmaf(f, 452.14603f, -125946.242f), 23258160.f), (float)SM_OFF);
     d = (uint32_t)y;
     return (int)x;
   }
@@ -336,7 +332,9 @@ struct RowSampler {
     return l > keep.at || (l == keep.at && i <= keep.last);
   }
 
-  // ---- the histogram of the workgroup's part (the last bin, the rest, is left out) ----
+  // ---- the histogram of the workgroup's part ----
+  // The last bin, the rest, stays empty: such a token goes to its lane's bin behind it (a branch around
+  // the addition keeps the eight tokens of a piece from being worked on together).
   __device__ __forceinline__ void histogram() {
     for (int i = tid; i < SM_BINS; i += SM_THREADS) s.hist[i] = 0;
     __syncthreads();
@@ -345,7 +343,7 @@ struct RowSampler {
       for (int e = 0; e < E; ++e) {
         uint32_t d;
         const int i = split(value(v, e), d);
-        if (i < SM_BINS - 1) atomicAdd(&s.hist[i], (1ULL << SM_COUNT) | d);
+        atomicAdd(&s.hist[i < SM_BINS - 1 ? i : SM_BINS + lane], (1ULL << SM_COUNT) | d);
       }
     });
     __syncthreads();
@@ -440,6 +438,7 @@ struct RowSampler {
           sum += l > -INFINITY ? floored(weight(l)) : 0ULL;
         }
       } else {
+        // bit E - 1 - e of a mask: token e; a bit is the sign of a difference
         uint32_t mask = 0, in = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -447,18 +446,22 @@ struct RowSampler {
           if constexpr (LISTED) {
             float dl;
             const float x = x_of(l, dl);
-            mask |= x < x0 ? 1u << e : 0u;
-            in |= x < x1 ? 1u << e : 0u;
+            mask = __builtin_amdgcn_alignbit(mask, __float_as_uint(x - x0), 31);
+            in = __builtin_amdgcn_alignbit(in, __float_as_uint(x - x1), 31);
           } else {
-            mask |= l >= keep.at && is_kept(l, i0 + e) ? 1u << e : 0u;
+            mask = mask << 1 | (l >= keep.at && is_kept(l, i0 + e) ? 1u : 0u);
           }
         }
+        auto token = [&](uint32_t bits) { return E - 1 - (__ffs((int)bits) - 1); };
         auto pick = [&](uint32_t bits) {
-          const int e = bits ? __ffs((int)bits) - 1 : 0;
-          float l = value(v, 0);
-#pragma unroll
-          for (int x = 1; x < E; ++x) l = e == x ? value(v, x) : l;
-          return l;
+          const int e = bits ? token(bits) : 0, w = DT == DKV_F32 ? e : e >> 1;
+          const uint32_t a = w & 1 ? v[1] : v[0], b = w & 1 ? v[3] : v[2], x = w & 2 ? b : a;
+          if constexpr (DT == DKV_F32)
+            return __uint_as_float(x);
+          else if constexpr (DT == DKV_BF16)
+            return __uint_as_float(e & 1 ? x & 0xffff0000u : x << 16);
+          else
+            return dkv_f16_bits_to_f32((e & 1 ? x >> 16 : x) & 0xffffu);
         };
         in &= ~mask;
         while (__ballot(mask != 0)) {  // one of each lane's at a time
@@ -469,7 +472,7 @@ struct RowSampler {
         if constexpr (LISTED) {
           while (in) {
             const float l = pick(in);
-            const int i = i0 + __ffs((int)in) - 1;
+            const int i = i0 + token(in);
             if (i >= 0 && i < V && l == l) list(((u64)sm_key(l) << 32) | (uint32_t)~i);
             in &= in - 1;
           }
