@@ -206,6 +206,8 @@ __global__ __launch_bounds__(64 * AP_WAVES) void paged_append_kernel(AppendParam
 // 0 .. t; o = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m), s_k = scale q . k, one pass over the
 // keys with a running maximum and sum.
 // ---------------------------------------------------------------------------------------
+// A running maximum of no keys: finite, so that exp2(-inf - it) is 0, and below every other score.
+constexpr float PG_NO_MAX = -3.4028234663852886e38f;
 struct AttendParams {
   const uint16_t* q;
   long long q_st, q_sh;
@@ -241,10 +243,7 @@ __device__ __forceinline__ void pg_lds_load16(__amdgpu_buffer_rsrc_t rsrc, uint3
                  ::"s"(lds_base), "v"(off), "s"(rsrc)
                  : "memory", "m0");
 }
-template <int N>
-__device__ __forceinline__ void pg_wait_vm() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
+__device__ __forceinline__ void pg_wait_vm() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 typedef __attribute__((address_space(3))) dkv_i16x4 pg_lds_i16x4;
 __device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
   return __builtin_bit_cast(
@@ -422,9 +421,7 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     for (int i = 0; i < 4; ++i) pg_lds_load16<true>(rv, slot + DTILE_BYTES + 1024 * i, piece_off[i]);
     return page;
   };
-  int pages[DSLOT];  // of tiles j, j + 1, ...
-#pragma unroll
-  for (int i = 0; i + 1 < DSLOT; ++i) pages[i] = issue(i);
+  int page_next = issue(0);
 
   // query operand: column n = row n (new token n / hpg, head n % hpg; rows past the request's
   // zero), dims 32c + 8g .. +8
@@ -446,17 +443,12 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   dkv_f32x4 acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -1.0e30f, l_run = 0.f;  // log2 units; a finite floor: exp2(-inf - floor) is 0
+  float m_run = PG_NO_MAX, l_run = 0.f;  // log2 units
 
   for (int j = 0; j < n_iter; ++j) {
-    if (DSLOT == 3 && j + 1 < n_iter)
-      pg_wait_vm<8>();  // tile j, while tile j + 1's loads are on their way
-    else
-      pg_wait_vm<0>();
-    const int page = pages[0];
-#pragma unroll
-    for (int i = 0; i + 2 < DSLOT; ++i) pages[i] = pages[i + 1];
-    pages[DSLOT - 2] = issue(j + DSLOT - 1);
+    pg_wait_vm();
+    const int page = page_next;
+    page_next = issue(j + 1);
     const uint8_t* slot = ring + (j % DSLOT) * DSLOT_BYTES;
     const int key0 = tix(j) * DTILE;
     dkv_u32x4 xk[4];
@@ -546,7 +538,7 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
-  pg_wait_vm<0>();  // nothing lands in the ring once it is reused below
+  pg_wait_vm();  // nothing lands in the ring once it is reused below
 
   // ---- join the waves through LDS ----
   float l_tot = l_run;
@@ -586,7 +578,7 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   auto store = [&](int row, int d, float A, float L) {
     const long long oi = (long long)(r.row0 + row / p.hpg) * p.o_st +
                          (long long)(kvh * p.hpg + row % p.hpg) * p.o_sh + d;
-    dkv_store_f32<ODT>(p.out, oi, L > 0.f ? A / L : 0.f);
+    dkv_store_f32<ODT>(p.out, oi, L == 0.f ? 0.f : A / L);  // (a NaN among the weights stays)
   };
   if (parts == 1) {
     for (int idx = tid; idx < rows * PG_DH; idx += 64 * DW) {
@@ -612,7 +604,7 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     if (d == 0) put(rr, M, L);
   }
   // ---- the unit's last part to arrive joins the parts ----
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  pg_wait_vm();
   __syncthreads();
   if (tid == 0) {
     const int old = __hip_atomic_fetch_add(p.counters + b * p.Hkv + kvh, 1, __ATOMIC_RELAXED,
@@ -761,13 +753,13 @@ __device__ __forceinline__ float pg_max4(float x) {  // over lanes n, n + 16, n 
 }
 
 // One row over keys k0 .. k1 - 1, by a wave, key by key: for rows whose values came out as infinity or
-// NaN. A product of matrices takes a masked key's value times 0, which is NaN for an infinite one; here
+// NaN, or whose scores are too large for one fused multiplication and subtraction. A product of matrices takes a masked key's value times 0, which is NaN for an infinite one; here
 // a masked key is not touched. Lane l returns dims 2l, 2l + 1.
 template <int DT>
 __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, int kvh,
                                               const uint16_t* qr, int k0, int k1, int lane,
                                               float& m, float& l, float& o0, float& o1) {
-  m = -1.0e30f;
+  m = PG_NO_MAX;
   l = o0 = o1 = 0.f;
   for (int t0 = k0; t0 < k1; t0 += 64) {
     const int key = t0 + lane;
@@ -906,7 +898,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const dkv_u32x4 ones = {one2, one2, one2, one2};
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    m_run[qb] = -1.0e30f;
+    m_run[qb] = PG_NO_MAX;
     sum[qb] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
@@ -921,7 +913,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
 
   if (t0 < n_tiles) issue(t0, __builtin_amdgcn_readlane(ids, blk));
   for (int t = t0; t < n_tiles; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    pg_wait_vm();
     __syncthreads();  // tile t is in LDS for every wave; tile t - 1's buffer is free
     const uint32_t gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
     if (t + 1 < n_tiles) {
@@ -1056,7 +1048,10 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     for (int db = 0; db < 8; ++db)
 #pragma unroll
       for (int u = 0; u < 4; ++u) odd = fmaf(acc[qb][db][u], 0.f, odd);
-    unsigned long long bad = __ballot(R < rows && !(odd == 0.f));
+    // (Or a sum below that of the largest score's weight alone, which is at least 1 as rounded: scores
+    // past 2^24, whose product with the scale and the rounded maximum differ by more than their sum.)
+    const bool low = l < 0.5f && min(limit[qb] + 1, n_tiles * CK) > t0 * CK;
+    unsigned long long bad = __ballot(R < rows && (!(odd == 0.f) || low));
     bad = (bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xffffull;  // by row
     const bool good = R < rows && !((bad >> n) & 1);
     if (c.splits == 1) {
@@ -1075,7 +1070,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       for (int db = 0; db < 8; ++db)
         *(dkv_f32x4*)(rec + x * PG_DH + 16 * db + 4 * g) = acc[qb][db];
     }
-    while (bad) {  // rows with an infinity or NaN, key by key
+    while (bad) {  // key by key
       const int x = __ffsll((long long)bad) - 1;
       bad &= bad - 1;
       const int Rx = wq0 + 16 * qb + x, ix = Rx / p.hpg, hx = Rx - ix * p.hpg;
@@ -1136,7 +1131,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(ChunkParams c) {
   const PagedRequest& r = it.r;
   const int R = it.rt * c.bq + row;
   if (R >= r.n * p.hpg) return;
-  float M = -1.0e30f, L = 0.f;
+  float M = PG_NO_MAX, L = 0.f;
   dkv_f32x4 a[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) a[q] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1170,6 +1165,7 @@ int fill_pool(PagedPool& pool, long long page_stride, long long head_stride, int
   if (head_stride < (long long)page_size * PG_DH && Hkv > 1) return DKV_E_ARG;
   if (page_stride < 0 || head_stride < 0) return DKV_E_ARG;
   if ((page_stride & 7) || (head_stride & 7)) return DKV_E_UNSUPPORTED;
+  if (page_stride < (long long)page_size * PG_DH && num_pages > 1) return DKV_E_ARG;
   if (cols > 0 && !table) return DKV_E_ARG;
   if ((long long)cols * page_size > 0x7fffffffLL - 4096) return DKV_E_UNSUPPORTED;
   pool.page_stride = page_stride;

@@ -37,7 +37,8 @@ _COUNTERS = 16384  # leading floats of the attention's workspace: its arrival co
 
 
 class PagedBatch:
-    """The requests of one step, on the device.
+    """The requests of one step, on the device. Its buffers' contents may change, the buffers and
+    the bounds are fixed.
 
     ``page_table`` (B, P) int32: the pages of request b in order (entries behind its last page are
     not read; an id outside the pool is a page that is not there: its keys are masked, its tokens
@@ -69,12 +70,16 @@ class PagedBatch:
             raise ValueError("page_table, q_start and lens must be on one device")
         if not (0 <= min_new <= max_new <= rows and max_len >= 0):
             raise ValueError("need 0 <= min_new <= max_new <= rows and max_len >= 0")
-        self.page_table, self.q_start, self.lens = page_table, q_start, lens
-        self.requests, self.device = B, page_table.get_device()
-        self.rows, self.max_new, self.max_len, self.min_new = rows, max_new, max_len, min_new
-        # what every call passes of the batch: its buffers stay where they are
-        self._table_args = (page_table.data_ptr(), max(ld, cols), cols)
-        self._row_args = (q_start.data_ptr(), lens.data_ptr(), B, rows)
+        for name, value in zip(self.__slots__, (
+                page_table, q_start, lens, rows, max_new, max_len, min_new, B,
+                page_table.get_device(),
+                # what every call passes of the batch: its buffers stay where they are
+                (page_table.data_ptr(), max(ld, cols), cols),
+                (q_start.data_ptr(), lens.data_ptr(), B, rows))):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("a PagedBatch is fixed: change what its buffers hold, or make another")
 
 
 class PagedKVCache:
@@ -222,6 +227,14 @@ def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, dtyp
     return hkv, (k_pages.data_ptr(), v_pages.data_ptr(), st[0], st[1], pages, ps)
 
 
+def _row_strides(t: torch.Tensor) -> tuple[int, int]:
+    """The row and head strides of (T, heads, 128); those of a size of one are any number."""
+    T, heads, _ = t.shape
+    st = t.stride()
+    sh = st[1] if heads > 1 else HEAD_DIM
+    return (st[0] if T > 1 else sh * heads), sh
+
+
 def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  batch: PagedBatch, *, heads: int, theta: float | None = None,
                  inv_freq: Sequence[float] | None = None, q_norm: torch.Tensor | None = None,
@@ -235,7 +248,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``inv_freq`` (scaled frequencies), the angle formed in 64 bits. With ``q_norm`` / ``k_norm``
     ((128,) of qkv's dtype) each query / key head is first normed, x / sqrt(mean(x^2) + eps) * w.
     Everything in fp32, rounded once where it is stored. ``out``: where the queries go (T, heads,
-    128), unit last stride; not qkv's own memory. A token whose page is not there is not stored."""
+    128), unit last stride (qkv's own query columns will do). A token whose page is not there is not stored."""
     shape, st = qkv.shape, qkv.stride()
     if len(shape) != 2 or st[1] != 1:
         raise ValueError("qkv must be (T, W) with unit last stride")
@@ -259,10 +272,10 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     elif (out.shape != (T, heads, HEAD_DIM) or out.stride(2) != 1 or out.dtype != dt
           or out.get_device() != dev):
         raise ValueError("out must be (T, heads, 128) of qkv's dtype with unit last stride")
-    o_st = out.stride()
+    o_st = _row_strides(out)
     _lib.check(_lib.call_on(
-        dev, _lib.calls().dkv_paged_append, stream, _lib.dtype_code(dt), qkv.data_ptr(), st[0],
-        out.data_ptr(), o_st[0], o_st[1], *pools, *batch._table_args, *batch._row_args, heads, hkv,
+        dev, _lib.calls().dkv_paged_append, stream, _lib.dtype_code(dt), qkv.data_ptr(),
+        st[0] if T > 1 else width, out.data_ptr(), *o_st, *pools, *batch._table_args, *batch._row_args, heads, hkv,
         HEAD_DIM, _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs)),
         "dkv_paged_append")
     return out
@@ -277,8 +290,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q`` (T, heads, 128), rotated; query head h reads KV head ``h // (heads / kv_heads)``. The new
     token at position t attends its request's tokens 0 .. t (the pages hold them all: the step's own
     are appended first); one that has none to attend gives 0. ``scale`` defaults to 1 / sqrt(128).
-    The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``."""
-    shape, st = q.shape, q.stride()
+    The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``;
+    ``out`` may be q itself."""
+    shape = q.shape
     if len(shape) != 3 or shape[2] != HEAD_DIM:
         raise ValueError("q must be (T, heads, 128)")
     T, hq, _ = shape
@@ -288,9 +302,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"{hq} query heads do not divide among {hkv} KV heads")
     if batch.rows > T:
         raise ValueError(f"the batch has {batch.rows} rows, q {T}")
-    if st[2] != 1 or q.data_ptr() % 16 or st[0] % 8 or st[1] % 8:
-        q = q.contiguous()
-        st = q.stride()
+    st = _row_strides(q)
+    if q.stride(2) != 1 or q.data_ptr() % 16 or st[0] % 8 or st[1] % 8:
+        q = q.clone(memory_format=torch.contiguous_format)
+        st = _row_strides(q)
     odt = out_dtype if out_dtype is not None else (out.dtype if out is not None else dt)
     if odt != dt and odt != torch.float32:
         raise ValueError("out_dtype must be the query dtype or float32")
@@ -300,16 +315,16 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     elif (out.shape != shape or out.dtype != odt or out.stride(2) != 1
           or out.get_device() != dev):
         raise ValueError("out must be (T, heads, 128) with unit last stride and the requested dtype")
-    o_st = out.stride()
+    o_st = _row_strides(out)
     lib = _lib.calls()
     bounds = batch.max_new, batch.min_new, batch.max_len
     need = lib.dkv_paged_workspace_floats(batch.requests, batch.rows, hq, hkv, *bounds)
     ws = _attention_workspace(q.device, stream, need) if need else None
     _lib.check(_lib.call_on(
-        dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), st[0], st[1],
+        dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), *st,
         *pools, *batch._table_args, *batch._row_args, hq, hkv, HEAD_DIM, *bounds,
         _SCALE if scale is None else float(scale), _lib.ptr(ws), ws.numel() if need else 0,
-        out.data_ptr(), _lib.dtype_code(odt), o_st[0], o_st[1]), "dkv_paged_attention")
+        out.data_ptr(), _lib.dtype_code(odt), *o_st), "dkv_paged_attention")
     return out
 
 
@@ -317,7 +332,7 @@ def _attention_workspace(device: torch.device, stream: int, floats: int) -> torc
     """Split records and arrival counters (zero before and after a call). Eager calls of a stream
     share its workspace, in that stream's order. A call under capture gets one of its own in the
     graph's pool, cleared by the graph itself: two captured graphs may be replayed at once."""
-    if torch.cuda.is_current_stream_capturing():
+    if _lib.call_on(device.index, torch.cuda.is_current_stream_capturing):
         ws = torch.empty(floats, dtype=torch.float32, device=device)
         ws[:_COUNTERS].zero_()
         return ws

@@ -176,10 +176,11 @@ class Sampler:
         self._gen.manual_seed(seed)
 
     def __call__(self, logits: torch.Tensor) -> torch.Tensor:
-        """``logits`` (..., V) -> tokens (...)."""
+        """``logits`` (..., V) -> tokens (...). Of a row without a token to take (all NaN or
+        -infinity) token 0, as the tokens are looked up next: ``sample_tokens`` tells them by -1."""
         rows = logits.reshape(-1, logits.shape[-1])
         u = torch.rand(rows.shape[0], generator=self._gen, device=logits.device)
-        return sample_tokens(rows, u, **self.settings).view(logits.shape[:-1])
+        return sample_tokens(rows, u, **self.settings).clamp_(min=0).view(logits.shape[:-1])
 
 
 

@@ -551,3 +551,231 @@ def test_pool_past_32_bits(dev):
         assert torch.equal(v[ids[0].long().to(dev)], small.v[order])
         assert torch.equal(paged_attention(qa, k, v, batch),
                            paged_attention(qb, small.k, small.v, small.batch))
+
+
+MANY = {
+    # more requests than one wave holds the lengths of: a workgroup each, single or with prompts beside
+    "single": ([1, 1, 0] * 100, [40, 300, 7] * 100, 8, 2, 16),
+    "mixed": ([1, 40, 0, 2] * 70, [90, 41, 5, 700] * 70, 8, 2, 32),
+    "prompts": ([17, 40] * 140, [17, 60] * 140, 4, 2, 16),
+    # more (request, KV head) units than counters
+    "units": ([1] * 256, [20, 70] * 128, 65, 65, 16),
+    "large_pages": ([1, 90, 1], [3000, 1500, 1025], 8, 2, 1024),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(MANY))
+def test_attention_many_requests_and_large_pages(dev, name):
+    new, lens, hq, hkv, ps = MANY[name]
+    print(f"[gpu] paged attention many {name}", flush=True)
+    s = Step(dev, new, lens, hkv=hkv, ps=ps, seed=51)
+    q = s.rand(s.T, hq, DH)
+    got = paged_attention(q, s.k, s.v, s.batch, out_dtype=torch.float32)
+    want, tol = _attend_reference(_First(s, 6), q)
+    n = want.shape[0]
+    assert bool(((got[:n].double() - want).abs() <= tol + 1e-30).all())
+    # the requests behind: the same keys alone give the same within both bounds
+    for b in {len(new) - 1, len(new) // 2}:
+        one = PagedBatch(s.batch.page_table[b:b + 1], torch.tensor([0, new[b]], dtype=torch.int32,
+                                                                   device=dev),
+                         s.batch.lens[b:b + 1], rows=new[b], max_new=new[b], max_len=lens[b],
+                         min_new=new[b])
+        r = slice(s.starts[b], s.starts[b + 1])
+        alone = paged_attention(q[r], s.k, s.v, one, out_dtype=torch.float32)
+        size = max(float(s.tokens(s.v, b, g).abs().max()) for g in range(hkv)) if new[b] else 0.0
+        assert bool(((got[r] - alone).abs() <= 2 * (2.0**-8 + 2.0**-12) * size).all())
+
+
+class _First:
+    """The first requests of a step, for the reference."""
+
+    def __init__(self, s, n):
+        self.s, self.new, self.lens = s, s.new[:n], s.lens[:n]
+        self.rows, self.starts = s.starts[len(self.new)], s.starts
+
+    def __getattr__(self, name):
+        return getattr(self.s, name)
+
+
+@pytest.mark.gpu
+def test_steps_of_nothing(dev):
+    print("[gpu] paged empty steps", flush=True)
+    cache = PagedKVCache(1, 4, 2, page_size=16, device=dev)
+    a = cache.add()
+    for step in ([], [(a, 0)]):
+        batch = cache.batch(step)
+        qkv = torch.randn(3, 8 * DH, device=dev).to(BF)  # rows of no request
+        out = torch.full((3, 4, DH), 2.0, dtype=BF, device=dev)
+        q = paged_append(qkv, cache.k[0], cache.v[0], batch, heads=4, theta=1e4, out=out)
+        o = paged_attention(q, cache.k[0], cache.v[0], batch, out=out)
+        assert bool((o == 2.0).all())
+        none = paged_append(qkv[:0], cache.k[0], cache.v[0], batch, heads=4, theta=1e4)
+        assert paged_attention(none, cache.k[0], cache.v[0], batch).shape == (0, 4, DH)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 1], [700, 90]), ([3, 2], [300, 900]),
+                                      ([80, 5, 1], [300, 200, 50]), ([40], [5000])])
+def test_in_place(dev, new, lens):
+    """The queries rotated in the projection's own columns, the output written over the queries."""
+    print(f"[gpu] paged in place {new}", flush=True)
+    s = Step(dev, new, lens, hkv=2, seed=52)
+    qkv = s.rand(s.T, 12 * DH)
+    q = paged_append(qkv, s.k, s.v, s.batch, heads=8, theta=1e4)
+    k, v = s.k.clone(), s.v.clone()
+    o = paged_attention(q, s.k, s.v, s.batch)
+    mine = qkv[:, :8 * DH].view(s.T, 8, DH)
+    assert paged_append(qkv, s.k, s.v, s.batch, heads=8, theta=1e4, out=mine) is mine
+    assert torch.equal(mine, q)
+    assert torch.equal(s.k.view(torch.int16), k.view(torch.int16))
+    assert torch.equal(s.v.view(torch.int16), v.view(torch.int16))
+    assert paged_attention(mine, s.k, s.v, s.batch, out=mine) is mine
+    assert torch.equal(mine, o)
+
+
+@pytest.mark.gpu
+def test_strides_of_single_rows_and_shared_queries(dev):
+    print("[gpu] paged odd strides", flush=True)
+    s = Step(dev, [1], [77], hkv=2, seed=53)
+    row = s.rand(1, 12 * DH)
+    odd = torch.empty(12 * DH, 1, dtype=BF, device=dev).t()  # a row stride of 1
+    odd.copy_(row)
+    q = paged_append(row, s.k, s.v, s.batch, heads=8, theta=1e4)
+    out = torch.empty_strided((1, 8, DH), (3, DH, 1), dtype=BF, device=dev)
+    assert torch.equal(paged_append(odd, s.k, s.v, s.batch, heads=8, theta=1e4, out=out), q)
+    want = paged_attention(q, s.k, s.v, s.batch)
+    got = torch.empty_strided((1, 8, DH), (3, DH, 1), dtype=torch.float32, device=dev)
+    paged_attention(out, s.k, s.v, s.batch, out=got)
+    assert torch.equal(got.to(BF), want)
+    for new, lens in (([2, 1], [90, 33]), ([70, 1], [90, 33])):
+        s = Step(dev, new, lens, hkv=2, seed=54)
+        one = s.rand(s.T, 1, DH).expand(s.T, 8, DH)
+        want = paged_attention(one.contiguous(), s.k, s.v, s.batch)
+        assert torch.equal(paged_attention(one, s.k, s.v, s.batch), want)
+        # heads first, in fp32, at an odd offset: rows that 16 bytes do not divide
+        wide = torch.full((8, s.T, DH + 1), 5.0, dtype=torch.float32, device=dev)
+        out = wide[..., 1:].transpose(0, 1)
+        paged_attention(one, s.k, s.v, s.batch, out=out)
+        assert torch.equal(out.to(BF), want) and bool((wide[..., 0] == 5.0).all())
+        # queries whose rows are not aligned
+        skew = torch.empty(s.T * 8 * DH + 3, dtype=BF, device=dev)[3:].view(s.T, 8, DH)
+        skew.copy_(one)
+        assert torch.equal(paged_attention(skew, s.k, s.v, s.batch), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 3, 60])
+def test_lengths_past_the_table_and_shared_pages(dev, new):
+    """A length the table has no room for ends with it, and a page that two requests hold (or one
+    of them twice) is read by both."""
+    print(f"[gpu] paged shared pages {new}", flush=True)
+    s = Step(dev, [new, new], [128, 96], hkv=2, seed=55)
+    q = s.rand(s.T, 4, DH)
+    s.table[1, :6] = s.table[0, :6]
+    s.table[1, 3] = s.table[1, 2]
+    table = s.table[:, :8].contiguous().to(dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    batch = PagedBatch(table, s.batch.q_start, i32(128 + 40, 96), rows=s.rows, max_new=new,
+                       max_len=128, min_new=new)
+    got = paged_attention(q, s.k, s.v, batch, out_dtype=torch.float32)
+    for b, n, end in ((0, 128, 168), (1, 96, 96)):
+        ids = s.table[b, :n // 16].long().to(dev)
+        pos = torch.arange(end - new, end, device=dev)[:, None]
+        dead = torch.arange(n, device=dev)[None] > pos
+        r = slice(b * new, (b + 1) * new)
+        for h in range(4):
+            k, v = (x[ids, h // 2].reshape(-1, DH).double() for x in (s.k, s.v))
+            z = (q[r, h].double() @ k.T / math.sqrt(DH)).masked_fill(dead, -math.inf)
+            p = torch.softmax(z, -1)
+            assert bool(((got[r, h].double() - p @ v).abs() <= 2.0**-7 * (p @ v.abs())).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 1], [700, 90]), ([3], [40]), ([80, 1], [300, 50]),
+                                      ([40], [5000])])
+def test_attention_scores_of_any_size(dev, new, lens):
+    """Scores far below zero (all of them), a NaN score (its row is NaN), an infinite one."""
+    print(f"[gpu] paged attention scores {new}", flush=True)
+    s = Step(dev, new, lens, hkv=2, seed=56)
+    q = torch.zeros(s.T, 8, DH, dtype=BF, device=dev)
+    q[..., 0] = 2.0**60
+    ids = [int(s.table[b, t]) for b, n in enumerate(lens) for t in range(-(-n // 16))]
+    s.k[ids] = 0.0
+    s.k[ids, :, :, 0] = -(2.0**62)
+    first = int(s.table[0, 0])
+    s.k[first, :, 0, 0] = -(2.0**61)  # the largest of request 0: its first key
+    got = paged_attention(q, s.k, s.v, s.batch)
+    want = s.v[first, :, 0].repeat_interleave(4, 0)
+    assert torch.equal(got[:new[0]], want.expand(new[0], 8, DH))
+    # all alike: the mean of the values
+    if len(new) > 1:
+        r, n = s.starts[1], lens[1]
+        mean = torch.stack([s.tokens(s.v, 1, h // 4)[:n - new[1] + 1].mean(0) for h in range(8)])
+        size = torch.stack([s.tokens(s.v, 1, h // 4)[:n - new[1] + 1].abs().mean(0)
+                            for h in range(8)])
+        assert bool(((got[r].double() - mean).abs() <= 2.0**-7 * size).all())
+    q = s.rand(s.T, 8, DH)
+    base = paged_attention(q, s.k, s.v, s.batch)
+    for value in (math.nan, math.inf):
+        bad = q.clone()
+        bad[0, 3, 5] = value
+        got = paged_attention(bad, s.k, s.v, s.batch)
+        if value != value:
+            assert bool(torch.isnan(got[0, 3]).all())
+        got[0, 3] = base[0, 3]
+        assert torch.equal(got, base)
+    k = s.k.clone()
+    k[first, 0, 0] = math.nan  # a key that every row of request 0 attends
+    got = paged_attention(q, k, s.v, s.batch)
+    assert bool(torch.isnan(got[:new[0], :4]).all())
+    got[:new[0], :4] = base[:new[0], :4]
+    assert torch.equal(got, base)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("odd", [dict(min_new=5), dict(max_len=20000), dict(max_new=80)])
+def test_attention_loose_bounds(dev, odd):
+    """Bounds choose the launch alone: any that hold give the same within the roundings, and a least
+    number of new tokens that does not hold costs no row."""
+    print(f"[gpu] paged attention bounds {odd}", flush=True)
+    s = Step(dev, [1, 40, 0, 4], [700, 90, 12, 3000], hkv=2, seed=57)
+    q = s.rand(s.T, 8, DH)
+    want, tol = _attend_reference(s, q)
+    table = torch.cat([s.table, torch.full((4, 1300), -1, dtype=torch.int32)], 1).to(dev)
+    rows = max(s.rows, odd.get("max_new", 0))
+    q2 = torch.cat([q, s.rand(rows - s.rows, 8, DH)])
+    batch = PagedBatch(table, s.batch.q_start, s.batch.lens,
+                       **(dict(rows=rows, max_new=40, max_len=3000, min_new=1) | odd))
+    got = paged_attention(q2, s.k, s.v, batch, out_dtype=torch.float32)[:s.rows]
+    assert bool(((got.double() - want).abs() <= tol + 1e-30).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 1], [700, 90]), ([3], [400]), ([80, 1], [300, 50]),
+                                      ([40], [5000]), ([257], [257])])
+@pytest.mark.parametrize("size", [2.0**13, 2.0**30, 2.0**50])
+def test_attention_scores_far_apart(dev, new, lens, size):
+    """Scores so large that the softmax is one key's: the output is that key's value exactly, for each
+    row whose two largest scores differ by more than fp32 sums can be off by."""
+    print(f"[gpu] paged attention far apart {new} {size}", flush=True)
+    s = Step(dev, new, lens, hkv=2, seed=58)
+    ids = sorted({int(i) for b, n in enumerate(lens) for i in s.table[b, :-(-n // 16)]})
+    s.k[ids] = s.k[ids] * size
+    q = s.rand(s.T, 8, DH, scale=size)
+    got = paged_attention(q, s.k, s.v, s.batch)
+    checked = 0
+    for b, (m, n) in enumerate(zip(new, lens)):
+        pos = torch.arange(n - m, n, device=dev)[:, None]
+        dead = torch.arange(n, device=dev)[None] > pos
+        r = slice(s.starts[b], s.starts[b] + m)
+        for h in range(8):
+            k, v = s.tokens(s.k, b, h // 4), s.tokens(s.v, b, h // 4)
+            z = (q[r, h].double() @ k.T / math.sqrt(DH)).masked_fill(dead, -math.inf)
+            a = (q[r, h].double().abs() @ k.T.abs() / math.sqrt(DH)).masked_fill(dead, 0).amax(-1)
+            top, at = torch.cat([z, z[:, :1] * 0 - math.inf], 1).topk(2)
+            # off by 130 roundings each, and 40 more halvings than bf16 can show
+            sure = top[:, 0] - top[:, 1] > 2 * 130 * 2.0**-24 * a + 40
+            assert torch.equal(got[r, h][sure], v.to(BF)[at[:, 0]][sure]), (b, h)
+            checked += int(sure.sum())
+    assert checked > 0.9 * s.rows * 8

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from dynakv_amd.kernels.sampling import sample_tokens
 from dynakv_amd.model import (CompressedLlama, DenseLlama, LlamaShape, PagedLlama, RandomLlama,
                               Sampler)
 
@@ -138,3 +139,14 @@ def test_other_models_refuse_qk_norm():
     for kind in (CompressedLlama, DenseLlama):
         with pytest.raises(ValueError, match="query and key norms"):
             kind(M())
+
+
+@pytest.mark.gpu
+def test_a_sampler_gives_tokens_that_can_be_looked_up(dev):
+    """A row of NaN or -infinity has no token (-1): the generators' sampler gives token 0 for it."""
+    print("[gpu] sampler without tokens", flush=True)
+    logits = torch.randn(4, 50, device=dev)
+    logits[1], logits[2] = float("nan"), float("-inf")
+    assert sample_tokens(logits, torch.full((4,), 0.5, device=dev)).tolist()[1:3] == [-1, -1]
+    t = Sampler(seed=3, device=dev)(logits)
+    assert t[1:3].tolist() == [0, 0] and int(t.min()) >= 0

@@ -105,6 +105,15 @@ def test_batch_refusals():
             PagedBatch(*args, **kw)
 
 
+def test_a_batch_is_fixed():
+    """Its launch arguments are taken when it is made: only the buffers' contents may change."""
+    b = _batch()
+    for name, value in (("lens", b.lens.clone()), ("rows", 3), ("max_len", 40), ("other", 1)):
+        with pytest.raises(AttributeError):
+            setattr(b, name, value)
+    assert b.rows == 4 and b.max_len == 20 and b.requests == 2
+
+
 def _pages(pages=4, heads=2, size=16, dtype=BF):
     return torch.zeros(pages, heads, size, 128, dtype=dtype)
 
@@ -159,6 +168,8 @@ def test_c_entry_refusals():
     assert append(ps=24, cols=0) == U and append(ps=8, cols=0) == U
     assert append(B=0, cols=0) == OK and append(T=0, cols=0) == OK
     assert append(stride=4, cols=0) == U
+    # pages on top of each other
+    assert append(stride=0, cols=0) == E and append(stride=1024, cols=0) == E
 
     def attend(dtype=_lib.DKV_BF16, scale=0.1, B=1, T=1, hq=4, hkv=2, new=1, odt=_lib.DKV_BF16):
         return lib.dkv_paged_attention(None, dtype, None, 512, 128, None, None, 4096, 2048, 4, 16,
