@@ -7,4 +7,9 @@ Modules mirror the reference package ``src/dynakv/kernels/``:
 * :mod:`.fused` -- ``fused_attention_dispatch`` (short-cache route)
 * :mod:`.two_stage` -- ``abx_sparse`` and ``avx`` (long-cache route)
 * :mod:`.decode` -- the native multi-group split-K entry used by the benchmark
+
+Beside them, for serving without compression:
+
+* :mod:`.paged` -- a paged cache for requests of different lengths, its append and its attention
+* :mod:`.sampling` -- tokens drawn from logits
 """

@@ -24,6 +24,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 from typing import Iterable, Sequence
 
 import torch
@@ -49,8 +50,10 @@ class PagedBatch:
     any. The host never reads the device buffers, so the bounds are the caller's to keep: new
     tokens past ``max_new`` or keys past ``max_len`` may be left out."""
 
-    __slots__ = ("page_table", "q_start", "lens", "rows", "max_new", "max_len", "min_new",
-                 "requests", "device", "_table_args", "_row_args")
+    __slots__ = ("_page_table", "_q_start", "_lens", "_rows", "_max_new", "_max_len", "_min_new",
+                 "_requests", "_device", "_table_args", "_row_args")
+    page_table, q_start, lens, rows, max_new, max_len, min_new, requests = (
+        property(operator.attrgetter(name)) for name in __slots__[:8])
 
     def __init__(self, page_table: torch.Tensor, q_start: torch.Tensor, lens: torch.Tensor, *,
                  rows: int, max_new: int, max_len: int, min_new: int = 1):
@@ -66,20 +69,17 @@ class PagedBatch:
         if (not q_start.is_contiguous() or not lens.is_contiguous() or (cols > 1 and unit != 1)
                 or (B > 1 and ld < cols)):
             raise ValueError("page_table rows, q_start and lens must be contiguous")
-        if not (page_table.device == q_start.device == lens.device):
+        device = page_table.get_device()
+        if not (device == q_start.get_device() == lens.get_device()):
             raise ValueError("page_table, q_start and lens must be on one device")
         if not (0 <= min_new <= max_new <= rows and max_len >= 0):
             raise ValueError("need 0 <= min_new <= max_new <= rows and max_len >= 0")
-        for name, value in zip(self.__slots__, (
-                page_table, q_start, lens, rows, max_new, max_len, min_new, B,
-                page_table.get_device(),
-                # what every call passes of the batch: its buffers stay where they are
-                (page_table.data_ptr(), max(ld, cols), cols),
-                (q_start.data_ptr(), lens.data_ptr(), B, rows))):
-            object.__setattr__(self, name, value)
-
-    def __setattr__(self, name, value):
-        raise AttributeError("a PagedBatch is fixed: change what its buffers hold, or make another")
+        self._page_table, self._q_start, self._lens = page_table, q_start, lens
+        self._requests, self._device = B, device
+        self._rows, self._max_new, self._max_len, self._min_new = rows, max_new, max_len, min_new
+        # what every call passes of the batch: its buffers stay where they are
+        self._table_args = (page_table.data_ptr(), max(ld, cols), cols)
+        self._row_args = (q_start.data_ptr(), lens.data_ptr(), B, rows)
 
 
 class PagedKVCache:
@@ -216,13 +216,13 @@ def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, dtyp
         raise ValueError("pages must hold a head's tokens back to back, with one layout for K and V")
     if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise ValueError("page and input dtypes differ")
-    if not (k_pages.get_device() == v_pages.get_device() == batch.device == device):
+    if not (k_pages.get_device() == v_pages.get_device() == batch._device == device):
         raise ValueError("inputs, pages and batch must be on one device")
     pages, hkv, ps, _ = shape
     if ps < 16 or ps & (ps - 1):
         raise NotImplementedError("page_size must be a power of two of at least 16")
-    if batch.max_len > batch._table_args[2] * ps:
-        raise ValueError(f"max_len {batch.max_len} is past the page table "
+    if batch._max_len > batch._table_args[2] * ps:
+        raise ValueError(f"max_len {batch._max_len} is past the page table "
                          f"({batch._table_args[2]} pages of {ps})")
     return hkv, (k_pages.data_ptr(), v_pages.data_ptr(), st[0], st[1], pages, ps)
 
@@ -257,8 +257,8 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     hkv, pools = _pools(k_pages, v_pages, batch, dt, dev)
     if heads <= 0 or width < (heads + 2 * hkv) * HEAD_DIM:
         raise ValueError(f"qkv must hold {heads} + 2 * {hkv} heads of {HEAD_DIM}")
-    if batch.rows > T:
-        raise ValueError(f"the batch has {batch.rows} rows, qkv {T}")
+    if batch._rows > T:
+        raise ValueError(f"the batch has {batch._rows} rows, qkv {T}")
     for w in (q_norm, k_norm):
         if w is not None and (w.shape != (HEAD_DIM,) or w.dtype != dt or not w.is_contiguous()
                               or w.get_device() != dev):
@@ -268,11 +268,12 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     freqs = _frequency_address(theta, inv_freq)
     stream = _lib.stream_of(qkv)
     if out is None:
-        out = torch.empty((T, heads, HEAD_DIM), dtype=dt, device=qkv.device)
+        out, o_st = qkv.new_empty(T, heads, HEAD_DIM), (heads * HEAD_DIM, HEAD_DIM)
     elif (out.shape != (T, heads, HEAD_DIM) or out.stride(2) != 1 or out.dtype != dt
           or out.get_device() != dev):
         raise ValueError("out must be (T, heads, 128) of qkv's dtype with unit last stride")
-    o_st = _row_strides(out)
+    else:
+        o_st = _row_strides(out)
     _lib.check(_lib.call_on(
         dev, _lib.calls().dkv_paged_append, stream, _lib.dtype_code(dt), qkv.data_ptr(),
         st[0] if T > 1 else width, out.data_ptr(), *o_st, *pools, *batch._table_args, *batch._row_args, heads, hkv,
@@ -292,7 +293,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     are appended first); one that has none to attend gives 0. ``scale`` defaults to 1 / sqrt(128).
     The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``;
     ``out`` may be q itself."""
-    shape = q.shape
+    shape, st = q.shape, q.stride()
     if len(shape) != 3 or shape[2] != HEAD_DIM:
         raise ValueError("q must be (T, heads, 128)")
     T, hq, _ = shape
@@ -300,28 +301,28 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     hkv, pools = _pools(k_pages, v_pages, batch, dt, dev)
     if hq % hkv or hq == 0:
         raise ValueError(f"{hq} query heads do not divide among {hkv} KV heads")
-    if batch.rows > T:
-        raise ValueError(f"the batch has {batch.rows} rows, q {T}")
-    st = _row_strides(q)
-    if q.stride(2) != 1 or q.data_ptr() % 16 or st[0] % 8 or st[1] % 8:
-        q = q.clone(memory_format=torch.contiguous_format)
-        st = _row_strides(q)
+    if batch._rows > T:
+        raise ValueError(f"the batch has {batch._rows} rows, q {T}")
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or q.data_ptr() % 16:
+        q, st = q.clone(memory_format=torch.contiguous_format), (hq * HEAD_DIM, HEAD_DIM)
     odt = out_dtype if out_dtype is not None else (out.dtype if out is not None else dt)
     if odt != dt and odt != torch.float32:
         raise ValueError("out_dtype must be the query dtype or float32")
     stream = _lib.stream_of(q)
     if out is None:
-        out = torch.empty(shape, dtype=odt, device=q.device)
+        out = torch.empty_like(q, dtype=odt, memory_format=torch.contiguous_format)
+        o_st = hq * HEAD_DIM, HEAD_DIM
     elif (out.shape != shape or out.dtype != odt or out.stride(2) != 1
           or out.get_device() != dev):
         raise ValueError("out must be (T, heads, 128) with unit last stride and the requested dtype")
-    o_st = _row_strides(out)
+    else:
+        o_st = _row_strides(out)
     lib = _lib.calls()
-    bounds = batch.max_new, batch.min_new, batch.max_len
-    need = lib.dkv_paged_workspace_floats(batch.requests, batch.rows, hq, hkv, *bounds)
+    bounds = batch._max_new, batch._min_new, batch._max_len
+    need = lib.dkv_paged_workspace_floats(batch._requests, batch._rows, hq, hkv, *bounds)
     ws = _attention_workspace(q.device, stream, need) if need else None
     _lib.check(_lib.call_on(
-        dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), *st,
+        dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), st[0], st[1],
         *pools, *batch._table_args, *batch._row_args, hq, hkv, HEAD_DIM, *bounds,
         _SCALE if scale is None else float(scale), _lib.ptr(ws), ws.numel() if need else 0,
         out.data_ptr(), _lib.dtype_code(odt), *o_st), "dkv_paged_attention")

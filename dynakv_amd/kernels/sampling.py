@@ -63,14 +63,14 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     m_ptr, m = _setting(min_p, rows, torch.float32, dev, "min_p")
     stream = _lib.stream_of(logits)
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+        out = torch.empty_like(u, dtype=torch.int64)
     elif (out.shape != (rows,) or out.dtype != torch.int64 or not out.is_contiguous()
           or out.get_device() != dev):
         raise ValueError(f"out must be a contiguous ({rows},) int64 tensor on the logits' device")
     lib, code = _lib.calls(), _lib.dtype_code(logits.dtype)
     # a workspace of the call's own, in its stream's order: nothing of it outlives the call
     need = lib.dkv_sample_workspace_bytes(code, rows, V)
-    ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    ws = logits.new_empty(need, dtype=torch.uint8) if need else None
     _lib.check(_lib.call_on(
         dev, lib.dkv_sample_tokens, stream, code, logits.data_ptr(), st[0] if rows > 1 else V,
         rows, V, u.data_ptr(), t_ptr, float(t), k_ptr, int(min(max(k, 0), V)), p_ptr, float(p),
