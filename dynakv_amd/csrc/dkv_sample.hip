@@ -42,6 +42,10 @@ constexpr int SM_CHUNKS = SM_MAX_V / 4 / 64 + 2;  // rows of 64 pieces (1 KB) of
 constexpr int SM_COUNT = 44;             // a bin: the count from this bit on, below it the sum of d
 constexpr uint32_t SM_OFF = 1u << 13;    // added to d, which may be as low as -2^-19
 constexpr double SM_ONE = 17592186044416.0;  // 2^44
+constexpr int SM_KEYS = 1 << 15;         // bins of one logit value each (16-bit types)
+constexpr int SM_TABLE = SM_KEYS / 2 - 2;  // weights of such values that a table holds
+constexpr int SM_TIES = 54;              // a chunk: the tokens at the border from this bit on, below it mass
+constexpr u64 SM_MASS = (1ULL << SM_TIES) - 1;
 
 struct SampleParams {
   const void* logits;
@@ -66,12 +70,34 @@ constexpr int SM_WS_N = SM_PARTS, SM_WS_HIST = 32, SM_WS_CAND = SM_WS_HIST + SM_
               SM_WS_CHUNK = SM_WS_CAND + SM_CAND, SM_WS = SM_WS_CHUNK + SM_CHUNKS;
 static_assert(SM_WS % 2 == 0 && SM_WS_HIST % 2 == 0, "16-byte accesses");
 
+template <int DT>
 struct SampleShared {
-  __attribute__((aligned(16))) u64 hist[SM_BINS + 64];  // and 64 that catch the rest
-  u64 cand[SM_CAND], sort[SM_CAND], chunk[SM_CHUNKS];
+  union {
+    struct {
+      __attribute__((aligned(16))) u64 hist[SM_BINS + 64];  // and 64 that catch the rest
+      u64 cand[SM_CAND], sort[SM_CAND];
+    };
+    __attribute__((aligned(16))) uint32_t bins[DT == DKV_F32 ? 4 : SM_KEYS];
+    u64 table[DT == DKV_F32 ? 2 : SM_KEYS / 2];
+  };
+  u64 chunk[SM_CHUNKS];
   u64 wave[SM_WAVES], wave2[SM_WAVES], pick[4];
   uint32_t root[64];
   int n, last;
+};
+
+// 2^(31 - j/64), rounded
+__device__ const uint32_t sm_root[64] = {
+    0x80000000u, 0x7e9f0606u, 0x7d41d96eu, 0x7be86fbau, 0x7a92be8bu, 0x7940bb9eu, 0x77f25cceu,
+    0x76a7980fu, 0x75606374u, 0x741cb528u, 0x72dc8374u, 0x719fc4b9u, 0x70666f76u, 0x6f307a41u,
+    0x6dfddbccu, 0x6cce8ae1u, 0x6ba27e65u, 0x6a79ad56u, 0x69540ec9u, 0x683199edu, 0x6712460bu,
+    0x65f60a7fu, 0x64dcdec3u, 0x63c6ba64u, 0x62b39509u, 0x61a3666du, 0x60962665u, 0x5f8bccdbu,
+    0x5e8451d0u, 0x5d7fad59u, 0x5c7dd7a4u, 0x5b7ec8f2u, 0x5a82799au, 0x5988e209u, 0x5891fac1u,
+    0x579dbc57u, 0x56ac1f75u, 0x55bd1cdbu, 0x54d0ad5au, 0x53e6c9dau, 0x52ff6b55u, 0x521a8ad7u,
+    0x51382182u, 0x50582888u, 0x4f7a9930u, 0x4e9f6cd4u, 0x4dc69cddu, 0x4cf022cau, 0x4c1bf829u,
+    0x4b4a169cu, 0x4a7a77d4u, 0x49ad1598u, 0x48e1e9bau, 0x4818ee22u, 0x47521cc6u, 0x468d6faeu,
+    0x45cae0f2u, 0x450a6abbu, 0x444c0740u, 0x438fb0cbu, 0x42d561b4u, 0x421d1462u, 0x4166c34cu,
+    0x40b268fau,
 };
 
 // A logit as a number that orders as the logits do (-0 as +0).
@@ -124,6 +150,28 @@ __device__ __forceinline__ u64 sm_wave_sum(u64 v) {  // as dkv_wave_sum_fast
   return v;
 }
 
+// lane `lane`'s value, for all (the lane is the whole wave's)
+__device__ __forceinline__ u64 sm_lane(u64 v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
+         ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32);
+}
+__device__ __forceinline__ u64 sm_first(u64 v) { return sm_lane(v, 0); }
+
+// the sums of two waves' values, halfway: of lanes l and l + 32 (a in the lower half, b in the upper);
+// of rows of 16 lanes 2r and 2r + 1 (a in row 2r, b in row 2r + 1)
+__device__ __forceinline__ u64 sm_meet32(u64 a, u64 b) {
+  const auto x = __builtin_amdgcn_permlane32_swap((uint32_t)a, (uint32_t)b, false, false);
+  const auto y =
+      __builtin_amdgcn_permlane32_swap((uint32_t)(a >> 32), (uint32_t)(b >> 32), false, false);
+  return (x[0] | ((u64)y[0] << 32)) + (x[1] | ((u64)y[1] << 32));
+}
+__device__ __forceinline__ u64 sm_meet16(u64 a, u64 b) {
+  const auto x = __builtin_amdgcn_permlane16_swap((uint32_t)a, (uint32_t)b, false, false);
+  const auto y =
+      __builtin_amdgcn_permlane16_swap((uint32_t)(a >> 32), (uint32_t)(b >> 32), false, false);
+  return (x[0] | ((u64)y[0] << 32)) + (x[1] | ((u64)y[1] << 32));
+}
+
 // What is kept: every token above `at`, and those at it up to index `last`.
 struct Border {
   float at;
@@ -142,12 +190,13 @@ template <int DT>
 struct RowSampler {
   static constexpr int E = DT == DKV_F32 ? 4 : 8;  // elements of a 16-byte piece
   const SampleParams& p;
-  SampleShared& s;
+  SampleShared<DT>& s;
   const int row, tid, lane, wave, V;
   const char* base;
   int head, rows64;  // elements of the first aligned piece before the row; its rows of 64 pieces
   int r0, r1;        // the wave's rows of pieces
   float t, tp, mp, u;
+  uint32_t root;
   int k;
   bool by_k, by_p;
   bool infinite = false;
@@ -158,7 +207,7 @@ struct RowSampler {
   // the histogram's running counts and masses before the thread's bins 4 tid .. 4 tid + 3, and theirs
   u64 n_run, m_run, cnt[4], mass[4];
 
-  __device__ __forceinline__ RowSampler(const SampleParams& p_, SampleShared& s_, int row_)
+  __device__ __forceinline__ RowSampler(const SampleParams& p_, SampleShared<DT>& s_, int row_)
       : p(p_), s(s_), row(row_), tid(threadIdx.x), lane(threadIdx.x & 63),
         wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), V(p_.V) {
     base = (const char*)p.logits + (long long)row * p.ld * (16 / E);
@@ -172,7 +221,11 @@ struct RowSampler {
     by_k = k > 0 && k < V;
     by_p = tp < 1.f;
     floor_w = mp > 0.f && mp <= 1.f ? (u64)ceil((double)mp * SM_ONE) : 0;
-    if (tid < 64) s.root[tid] = (uint32_t)rint(exp2(31.0 - (double)tid / 64.0));
+    root = sm_root[lane];
+  }
+  // (after the first loads are under way; seen after the next barrier)
+  __device__ __forceinline__ void keep_root() {
+    if (wave == 0) s.root[lane] = root;
   }
   // only the first token is kept
   __device__ __forceinline__ bool greedy() const {
@@ -270,12 +323,15 @@ struct RowSampler {
       for (int o = 32; o >= 1; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
       best |= (uint32_t)~at;
     }
-    __syncthreads();
+    keep_root();
     if (lane == 0) s.wave[wave] = best;
     __syncthreads();
-    for (int w = 0; w < SM_WAVES; ++w) best = max(best, s.wave[w]);
-    __syncthreads();
-    return best;
+    best = s.wave[lane & (SM_WAVES - 1)];
+    best = max(best, sm_dpp<0xb1>(best));
+    best = max(best, sm_dpp<0x4e>(best));
+    best = max(best, sm_dpp<0x141>(best));
+    best = max(best, sm_dpp<0x140>(best));
+    return sm_first(best);
   }
   // Takes the row's largest logit; false where that decides the row (the answer is written, by one).
   __device__ __forceinline__ bool begin(u64 best, bool write) {
@@ -359,23 +415,22 @@ struct RowSampler {
       n_sum += cnt[q];
       m_sum += mass[q];
     }
-    n_run = sm_wave_scan(n_sum);
-    m_run = sm_wave_scan(m_sum);
-    if (lane == 63) {
-      s.wave[wave] = n_run;
-      s.wave2[wave] = m_run;
-    }
+    u64 n_all;
+    n_run = before(n_sum, s.wave, n_all);
+    m_run = before(m_sum, s.wave2, kept);
+  }
+  // the threads' sums before the thread's own, and that of all; `at`: a word for each wave
+  __device__ __forceinline__ u64 before(u64 own, u64* at, u64& all) const {
+    const u64 run = sm_wave_scan(own);
+    if (lane == 63) at[wave] = run;
     __syncthreads();
-    n_run -= n_sum;
-    m_run -= m_sum;
-    kept = 0;
-    for (int w = 0; w < SM_WAVES; ++w) {
-      if (w < wave) {
-        n_run += s.wave[w];
-        m_run += s.wave2[w];
-      }
-      kept += s.wave2[w];
-    }
+    u64 x = at[lane & (SM_WAVES - 1)];  // (a row of 16 lanes: each wave's)
+    x += sm_dpp<0x111>(x);
+    x += sm_dpp<0x112>(x);
+    x += sm_dpp<0x114>(x);
+    x += sm_dpp<0x118>(x);
+    all = sm_lane(x, SM_WAVES - 1);
+    return (wave ? sm_lane(x, wave - 1) : 0ULL) + run - own;
   }
   // The bin of a border: where the k-th token is (want), or the last one before which less than P lies;
   // the count and the mass above it. SM_BINS: none.
@@ -481,6 +536,11 @@ struct RowSampler {
       sum = sm_wave_sum(sum);
       if (lane == 0) put(R, sum);
     });
+  }
+  // u times the mass, in whole units of it
+  __device__ __forceinline__ u64 target_of(u64 all) const {
+    const double U = u > 0.f ? (double)u * (double)all : 0.0;
+    return U < (double)all ? min((u64)U, all - 1) : all - 1;
   }
   // the n tokens of s.cand in order
   __device__ __forceinline__ void sort(int n) {
@@ -678,28 +738,315 @@ struct RowSampler {
     __syncthreads();
   }
 
+  // ---- 16-bit logits, the row in one workgroup: by their values ----
+  // A row has few distinct logits, so a bin each: its tokens are counted, its weight is worked out once
+  // and, for the masses, read from a table; a border is a bin and the tokens at it (the first of them in
+  // the vocabulary's order are kept), and nothing is sorted.
+  // A bin is the logit's key: its bits without the sign, up to 2^-20 (bf16) or 2^-8 (fp16) all 0, signed.
+  // What is next to 0 thus shares a bin with it (halvings of the logit down to 2^-126 would be most of
+  // the bins): its tokens' weights differ from that of 0 and are put right one by one.
+  static constexpr int NEAR = DT == DKV_BF16 ? (127 - 20) << 7 : (15 - 8) << 10;
+  static constexpr int INF = DT == DKV_BF16 ? 0x7f80 : 0x7c00;
+  typedef short s2 __attribute__((ext_vector_type(2)));
+  typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+  int k_max, k_lo;   // the largest logit's key, and the key of bin 0; bins 0 .. 63 catch what has no weight
+  int near_n = 0;    // tokens next to 0
+  u64 near_m = 0;    // what their weights are above those of as many at 0 (modulo 2^64)
+  static __device__ __forceinline__ s2 keys(uint32_t v) {
+    const u2 t = __builtin_bit_cast(u2, v & 0x7fff7fffu);
+    const u2 u = __builtin_elementwise_sub_sat(t, u2{(unsigned short)NEAR, (unsigned short)NEAR});
+    const s2 sign = __builtin_bit_cast(s2, v) >> 15;
+    return (__builtin_bit_cast(s2, u) ^ sign) - sign;
+  }
+  static __device__ __forceinline__ float of_key(int key) {
+    const uint32_t b = (key < 0 ? 0x8000u : 0u) | (key ? (uint32_t)(abs(key) + NEAR) : 0u);
+    return DT == DKV_BF16 ? __uint_as_float(b << 16) : dkv_f16_bits_to_f32(b);
+  }
+  static __device__ __forceinline__ int key_of(float l) {  // (towards 0)
+    uint32_t b = __float_as_uint(l) >> 16;
+    if constexpr (DT == DKV_F16)
+      b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(l, -65504.f), 0.f));
+    return keys(b)[0];
+  }
+  // Whether the row's range of logits has bins.
+  __device__ __forceinline__ bool by_values_fits() {
+    k_max = key_of(m);
+    // no weight at x = SM_BINS - 1; the key is off by less than 2
+    const int low = key_of(fmaxf(m - (float)SM_BINS / c_hi, -3.4028234663852886e38f)) - 2;
+    k_lo = max(low, -(INF - NEAR) + 1) - 64;
+    return k_max - k_lo <= SM_KEYS - 2;
+  }
+  static __device__ __forceinline__ bool is_near(const dkv_u32x4& v, int e) {
+    return ((v[e / 2] >> (16 * (e & 1))) & 0x7fffu) - 1 < (uint32_t)NEAR;
+  }
+  // f(logit) for the piece's tokens next to 0
+  template <class F>
+  __device__ __forceinline__ void next_to_0(const dkv_u32x4& v, F&& f) const {
+    u2 least = {0xffff, 0xffff};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // (0 itself wraps)
+      least = __builtin_elementwise_min(
+          least, __builtin_bit_cast(u2, v[i] & 0x7fff7fffu) - u2{1, 1});
+    if (min(least[0], least[1]) >= NEAR) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (is_near(v, e)) f(value(v, e));
+  }
+  __device__ __forceinline__ void count_values() {
+    const int range = k_max - k_lo;
+    for (int i = 4 * tid; i <= range; i += 4 * SM_THREADS)
+      *(dkv_u32x4*)&s.bins[i] = dkv_u32x4{0u, 0u, 0u, 0u};
+    if (tid == 0) s.n = 0, s.pick[3] = 0;
+    __syncthreads();
+    const s2 lo = {(short)k_lo, (short)k_lo}, own = {(short)lane, (short)lane};
+    each([&](int, int, const dkv_u32x4& v) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const s2 k = __builtin_elementwise_max(__builtin_elementwise_sub_sat(keys(v[i]), lo), own);
+        const uint32_t b = __builtin_bit_cast(uint32_t, k);
+        atomicAdd(&s.bins[b & 0xffffu], 1u);
+        atomicAdd(&s.bins[b >> 16], 1u);
+      }
+    });
+    __syncthreads();
+    if (count_at(-k_lo)) {  // tokens at 0, or next to it
+      const u64 w0 = weight(0.f);
+      each([&](int, int i0, const dkv_u32x4& v) {
+        next_to_0(v, [&](float l) {
+          atomicAdd(&s.pick[3], weight(l) - w0);
+          atomicAdd(&s.n, 1);
+        });
+      });
+      __syncthreads();
+      near_n = s.n;
+      near_m = s.pick[3];
+    }
+  }
+  __device__ __forceinline__ uint32_t count_at(int bin) const {
+    return bin >= 64 && bin <= k_max - k_lo ? s.bins[bin] : 0u;
+  }
+  __device__ __forceinline__ u64 mass_at(int bin, uint32_t n) const {
+    return (u64)n * weight(of_key(bin + k_lo)) + (bin == -k_lo ? near_m : 0ULL);
+  }
+  // Bins in order: d of them below the largest logit's. `end`, `end_n`: the last of them that are taken
+  // and its tokens that are (top-k's border).
+  __device__ __forceinline__ uint32_t count_d(int d, int end, uint32_t end_n) const {
+    const uint32_t n = count_at(k_max - k_lo - d);
+    return d < end ? n : d == end ? min(n, end_n) : 0u;
+  }
+  __device__ __forceinline__ u64 mass_d(int d, uint32_t n) const {
+    return n ? mass_at(k_max - k_lo - d, n) : 0ULL;
+  }
+  // A border among the bins up to `end`, which is moved to it: thread t has bins per * t .. per * (t +
+  // 1) - 1 (per odd: no two lanes in a bank); the one whose counts (BY_MASS: masses) the border lies in
+  // writes its number, and its bins are looked at by lane.
+  template <bool BY_MASS>
+  __device__ __forceinline__ bool border(int& end, uint32_t& end_n) {
+    const int per = ((end + SM_THREADS) / SM_THREADS) | 1;
+    u64 own = 0, all;
+    for (int d = per * tid; d < min(per * (tid + 1), end + 1); ++d) {
+      const uint32_t n = count_d(d, end, end_n);
+      own += BY_MASS ? mass_d(d, n) : (u64)n;
+    }
+    if (tid == 0) s.pick[0] = ~0ULL;
+    const u64 run = before(own, BY_MASS ? s.wave2 : s.wave, all);
+    const double P = (double)tp * (double)all;
+    auto early = [&](u64 x) { return BY_MASS ? (double)x < P : x < (u64)k; };
+    if (own && early(run) && !early(run + own)) {
+      s.pick[0] = (u64)tid;
+      s.pick[1] = run;
+    }
+    __syncthreads();
+    const u64 who = s.pick[0], run0 = s.pick[1];
+    if (who == ~0ULL) return false;
+    __syncthreads();
+    if (wave == 0) {
+      const int d = per * (int)who + lane;
+      const uint32_t n = lane < per ? count_d(d, end, end_n) : 0u;
+      const u64 x = BY_MASS ? mass_d(d, n) : (u64)n;
+      const u64 first = run0 + sm_wave_scan(x) - x;
+      const unsigned long long hit = __ballot(n && early(first));
+      if (lane == 63 - __clzll((long long)hit)) {
+        u64 j = n;
+        if constexpr (BY_MASS) {
+          const u64 w = weight(of_key(k_max - d));
+          if (w) {  // those before which less than P lies
+            j = min(j, (u64)fmax((P - (double)first) / (double)w, 1.0));
+            while (j > 1 && !early(first + (j - 1) * w)) --j;
+            while (j < n && early(first + j * w)) ++j;
+          }
+        } else {
+          j = min(j, (u64)k - first);
+        }
+        s.pick[2] = (u64)d;
+        s.pick[3] = j;
+      }
+    }
+    __syncthreads();
+    end = (int)s.pick[2];
+    end_n = (uint32_t)s.pick[3];
+    return true;
+  }
+  // The piece's tokens less than n keys below the largest: their masses, and those at n as at_border.
+  template <bool TABLE, class F>
+  __device__ __forceinline__ void value_weights(const dkv_u32x4& v, uint32_t n, u64 at_border,
+                                                F&& f) const {
+    const u2 top = {(unsigned short)k_max, (unsigned short)k_max};
+    const u2 end = {(unsigned short)(n + 1), (unsigned short)(n + 1)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (a NaN's is larger than n)
+      const u2 d = top - __builtin_bit_cast(u2, keys(v[i]));
+      if constexpr (TABLE) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(d, end));
+        f(2 * i, s.table[b & 0xffffu]);
+        f(2 * i + 1, s.table[b >> 16]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          f(2 * i + q,
+            d[q] < n ? floored(weight(value(v, 2 * i + q))) : d[q] == n ? at_border : 0ULL);
+      }
+    }
+  }
+  // The masses of the rows of pieces, and the number of tokens at the border (`ties` of which are kept,
+  // of weight tie_w), then the token in which u times the mass lies.
+  template <bool TABLE>
+  __device__ __forceinline__ void by_weights(uint32_t n, u64 ties, u64 tie_w) {
+    const u64 at_border = ties ? 1ULL << SM_TIES : 0ULL, w0 = floored(weight(0.f));
+    if constexpr (TABLE) {
+      __syncthreads();  // (the bins' memory)
+      for (uint32_t i = tid; i < n; i += SM_THREADS)
+        s.table[i] = floored(weight(of_key(k_max - (int)i)));
+      if (tid < 2) s.table[n + tid] = tid ? 0ULL : at_border;
+      __syncthreads();
+    }
+    const bool near = TABLE && near_n && k_max >= 0 && (uint32_t)k_max < n;
+    auto sum_of = [&](const dkv_u32x4& v) {
+      u64 sum = 0;
+      value_weights<TABLE>(v, n, at_border, [&](int, u64 w) { sum += w; });
+      if (near) next_to_0(v, [&](float l) { sum += floored(weight(l)) - w0; });
+      return sum;
+    };
+    // four rows' sums are brought together in a step of two halves, one of two rows of 16, four within
+    // those: row R + 2 ((lane / 16) % 2) + lane / 32 of the four
+#pragma unroll 1
+    for (int R = r0; R < r1; R += 4) {
+      dkv_u32x4 v[4];
+      u64 x[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = load(min(R + q, r1 - 1));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = R + q < r1 ? sum_of(v[q]) : 0ULL;
+      u64 sum = sm_meet16(sm_meet32(x[0], x[1]), sm_meet32(x[2], x[3]));
+      sum += sm_dpp<0xb1>(sum);
+      sum += sm_dpp<0x4e>(sum);
+      sum += sm_dpp<0x141>(sum);
+      sum += sm_dpp<0x140>(sum);
+      const int at = R + (lane >> 4 & 1) * 2 + (lane >> 5);
+      if ((lane & 15) == 0 && at < r1) s.chunk[at] = sum;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    // one wave does the rest: lane l has rows of pieces share * l .. share * (l + 1) - 1
+    const int share = (rows64 + 63) / 64, c0 = lane * share, c1 = min(rows64, c0 + share);
+    u64 own = 0, at = 0;
+    for (int i = c0; i < c1; ++i) {
+      own += s.chunk[i] & SM_MASS;
+      at += s.chunk[i] >> SM_TIES;
+    }
+    u64 tie0 = 0;  // tokens at the border before the lane's
+    if (ties) {
+      tie0 = sm_wave_scan(at) - at;
+      own += (min(tie0 + at, ties) - min(tie0, ties)) * tie_w;
+    }
+    u64 run = sm_wave_scan(own);
+    const u64 target = target_of(sm_lane(run, 63));
+    const unsigned long long hit = __ballot(run > target);
+    const int who = __ffsll((long long)hit) - 1;
+    run = sm_lane(run - own, who);
+    tie0 = sm_lane(tie0, who);
+    int R = who * share;
+    for (;; ++R) {
+      const u64 c = s.chunk[R], t = c >> SM_TIES;
+      const u64 x = (c & SM_MASS) + (min(tie0 + t, ties) - min(tie0, ties)) * tie_w;
+      if (run + x > target || R == rows64 - 1) break;
+      run += x;
+      tie0 += t;
+    }
+    R = __builtin_amdgcn_readfirstlane(R);
+    const int i0 = first_of(R);
+    const dkv_u32x4 v = load(R);
+    u64 w[E], t = 0, sum = 0;
+    value_weights<TABLE>(v, n, at_border, [&](int e, u64 x) {
+      w[e] = x;
+      t += x >> SM_TIES;
+    });
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (is_near(v, e) ) w[e] = floored(weight(value(v, e)));
+    }
+    if (ties) {
+      tie0 += sm_wave_scan(t) - t;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (w[e] >> SM_TIES) w[e] = tie0++ < ties ? tie_w : 0ULL;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e];
+    run += sm_wave_scan(sum) - sum;
+    if (run <= target && target < run + sum) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (run <= target && target < run + w[e]) p.out[row] = (long long)(i0 + e);
+        run += w[e];
+      }
+    }
+  }
+  // The whole of it; false where the borders are among the tokens next to 0.
+  __device__ __forceinline__ bool by_values() {
+    int end = k_max - k_lo - 64;  // the last bin that has a weight
+    uint32_t end_n = 0;           // its tokens that are kept, where it is a border
+    bool found = false;
+    if (by_k || by_p) {
+      count_values();
+      end_n = ~0u;
+      if (by_k && border<false>(end, end_n)) {
+        found = true;
+        if (end == k_max && near_n) return false;
+      }
+      if (by_p && border<true>(end, end_n)) {
+        found = true;
+        if (end == k_max && near_n) return false;
+      }
+    } else {
+      near_n = 1;  // (unknown)
+    }
+    const uint32_t n = found ? (uint32_t)end : (uint32_t)(end + 1);
+    const u64 ties = found ? end_n : 0ULL, tie_w = floored(weight(of_key(k_max - end)));
+    if (n <= (uint32_t)min(SM_TABLE, V))
+      by_weights<true>(n, ties, tie_w);
+    else
+      by_weights<false>(n, ties, tie_w);
+    return true;
+  }
+
   // ---- the token in which u times the mass lies ----
   __device__ __forceinline__ void finish() {
     const int share = (rows64 + SM_THREADS - 1) / SM_THREADS;
-    u64 own = 0;
-    for (int i = tid * share; i < min(rows64, (tid + 1) * share); ++i) own += s.chunk[i];
-    u64 run = sm_wave_scan(own);
-    if (lane == 63) s.wave[wave] = run;
-    __syncthreads();
-    u64 all = 0;
-    run -= own;
-    for (int w = 0; w < SM_WAVES; ++w) {
-      if (w < wave) run += s.wave[w];
-      all += s.wave[w];
-    }
-    const double U = u > 0.f ? (double)u * (double)all : 0.0;
-    const u64 target = U < (double)all ? min((u64)U, all - 1) : all - 1;
-    for (int i = tid * share; i < min(rows64, (tid + 1) * share); ++i) {
-      if (run <= target && target < run + s.chunk[i]) {
+    const int c0 = tid * share, c1 = min(rows64, c0 + share);
+    u64 own = 0, all;
+    for (int i = c0; i < c1; ++i) own += s.chunk[i];
+    u64 run = before(own, s.wave, all);
+    const u64 target = target_of(all);
+    for (int i = c0; i < c1; ++i) {
+      const u64 c = s.chunk[i];
+      if (run <= target && target < run + c) {
         s.pick[0] = (u64)i;
         s.pick[1] = run;
       }
-      run += s.chunk[i];
+      run += c;
     }
     __syncthreads();
     if (wave != 0) return;
@@ -726,10 +1073,12 @@ struct RowSampler {
 // A row per workgroup.
 template <int DT>
 __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(SampleParams p) {
-  __shared__ SampleShared s;
+  __shared__ SampleShared<DT> s;
   RowSampler<DT> r(p, s, blockIdx.x);
   r.take(0, 1);
   if (!r.begin(r.largest(), true)) return;
+  if constexpr (DT != DKV_F32)
+    if (r.by_values_fits() && r.by_values()) return;
   if (r.by_k || r.by_p) {
     r.histogram();
     r.run_sums();
@@ -758,7 +1107,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(SampleParams p)
 // histogram, 2 the masses, after which the row's last workgroup to arrive ends it.
 template <int DT, int PASS>
 __global__ __launch_bounds__(SM_THREADS) void sample_parts_kernel(SampleParams p) {
-  __shared__ SampleShared s;
+  __shared__ SampleShared<DT> s;
   const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x;
   u64* ws = p.ws + (long long)row * SM_WS;
   RowSampler<DT> r(p, s, row);
@@ -777,6 +1126,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_parts_kernel(SampleParams p
 #pragma unroll
     for (int q = 0; q < 2; ++q) h[q] = ((const dkv_u64x2*)(ws + SM_WS_HIST))[2 * tid + q];
   }
+  r.keep_root();
 #pragma unroll
   for (int o = 8; o >= 1; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
   best = __shfl(best, 0, 64);

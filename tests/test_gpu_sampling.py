@@ -246,3 +246,67 @@ def test_captured_and_repeated(dev):
         torch.cuda.synchronize()
         assert got.tolist() == sample_tokens(x, u, top_k=50, top_p=0.9).tolist()
         assert got.tolist() == _all(x, u, 1.0, 50, 0.9, 0.0)
+
+
+def _row(kind, V, g):
+    x = torch.randn(V, generator=g)
+    if kind == "tiny":            # all next to 0: 1 - 2^-30 and the like
+        return x * 1e-7
+    if kind == "near":            # some next to 0, beside zeros of both signs and ordinary ones
+        x = x * 2
+        x[::5], x[1::7], x[2::7] = x[::5] * 1e-5, 0.0, -0.0
+        return x
+    if kind == "near_below":      # those next to 0 are the largest
+        return torch.where(x > 0.5, x * 1e-6, -x.abs() * 4)
+    if kind == "zeros":           # half of them 0
+        return torch.where(x > 0, 0.0, x * 3)
+    if kind == "below":           # all far below 0
+        return x * 3 - 300.0
+    if kind == "above":
+        return x * 2 + 1000.0
+    if kind == "spread":          # more values than there are bins
+        return torch.exp(x * 4) * x.sign()
+    if kind == "masked":          # most of them at the type's lowest value, some -infinity
+        return torch.where(x > 1.0, x * 2, torch.where(x > 0, -65504.0, -math.inf))
+    if kind == "equal":
+        return torch.full((V,), -3.25)
+    if kind == "nan":             # of both signs
+        x = x * 2.5
+        x[::3], x[1::9] = math.nan, -math.nan
+        return x
+    if kind == "infinite":
+        x[::11] = math.inf
+        return x
+    return x * 2.5
+
+
+KINDS = ["tiny", "near", "near_below", "zeros", "below", "above", "spread", "masked", "equal", "nan",
+         "infinite", "plain"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("kind", KINDS)
+def test_logits_of_every_kind(dev, kind, dtype):
+    """Where 16-bit logits are counted by value: what lies next to 0, ranges with more values than
+    bins, constants; each filter, cold and hot."""
+    print(f"[gpu] sample logits {kind} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(61)
+    for V in (777, 20000):
+        x = torch.stack([_row(kind, V, g) for _ in range(6)]).to(DT[dtype]).to(dev)
+        u = torch.rand(6, generator=g).to(dev)
+        for t in (1.0, 0.05, 40.0):
+            _check(x, u, temperature=t)
+            _check(x, u, temperature=t, top_k=V // 3)
+            _check(x, u, temperature=t, top_p=0.97)
+            _check(x, u, temperature=t, top_p=0.5, top_k=V // 2, min_p=0.3)
+        _check(x, u, top_k=V - 1, top_p=0.999999)
+    # long rows in a workgroup each
+    x = torch.stack([_row(kind, 90001, g) for _ in range(2)]).to(DT[dtype]).to(dev)
+    x, u = x.repeat(70, 1), torch.rand(140, generator=g).to(dev)
+    got = [sample_tokens(x, u, **kw).tolist() for kw in ({}, dict(top_p=0.9), dict(top_k=1000))]
+    few = torch.cat([torch.arange(4), torch.arange(137, 140)])
+    for kw, t in zip(((0, 1.0), (0, 0.9), (1000, 1.0)), got):
+        p = torch.tensor(kw[1], dtype=torch.float32).item()
+        want = _all(x[few.to(dev)], u[few.to(dev)], 1.0, kw[0], p, 0.0)
+        assert [t[int(i)] for i in few] == want
