@@ -738,6 +738,70 @@ struct RowSampler {
     __syncthreads();
   }
 
+  // ---- the token in which u times the mass lies ----
+  // s.chunk: the masses of the rows of pieces, and from bit SM_TIES on the tokens at a border, the first
+  // `ties` of which are kept, of weight tie_w each. weights(piece, its first token, w): the same of a
+  // piece's tokens. One wave's work: lane l has rows share * l .. share * (l + 1) - 1.
+  template <class F>
+  __device__ __forceinline__ void finish(u64 ties, u64 tie_w, F&& weights) const {
+    if (wave != 0) return;
+    const int share = (rows64 + 63) / 64, c0 = lane * share, c1 = min(rows64, c0 + share);
+    u64 own = 0, at = 0;
+    for (int i = c0; i < c1; ++i) {
+      own += s.chunk[i] & SM_MASS;
+      at += s.chunk[i] >> SM_TIES;
+    }
+    u64 tie0 = 0;  // tokens at the border before the lane's
+    if (ties) {
+      tie0 = sm_wave_scan(at) - at;
+      own += (min(tie0 + at, ties) - min(tie0, ties)) * tie_w;
+    }
+    u64 run = sm_wave_scan(own);
+    const u64 target = target_of(sm_lane(run, 63));
+    const int who = __ffsll((long long)__ballot(run > target)) - 1;
+    run = sm_lane(run - own, who);
+    tie0 = sm_lane(tie0, who);
+    int R = who * share;
+    for (;; ++R) {
+      const u64 c = s.chunk[R], t = c >> SM_TIES;
+      const u64 x = (c & SM_MASS) + (min(tie0 + t, ties) - min(tie0, ties)) * tie_w;
+      if (run + x > target || R == rows64 - 1) break;
+      run += x;
+      tie0 += t;
+    }
+    R = __builtin_amdgcn_readfirstlane(R);
+    const int i0 = first_of(R);
+    u64 w[E], t = 0, sum = 0;
+    weights(load(R), i0, w);
+    if (ties) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) t += w[e] >> SM_TIES;
+      tie0 += sm_wave_scan(t) - t;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (w[e] >> SM_TIES) w[e] = tie0++ < ties ? tie_w : 0ULL;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e];
+    run += sm_wave_scan(sum) - sum;
+    if (run <= target && target < run + sum) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (run <= target && target < run + w[e]) p.out[row] = (long long)(i0 + e);
+        run += w[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void finish() const {
+    finish(0, 0, [&](const dkv_u32x4& v, int i0, u64 (&w)[E]) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float l = value(v, e);
+        w[e] = is_kept(l, i0 + e) ? floored(weight(l)) : 0ULL;
+      }
+    });
+  }
+
   // ---- 16-bit logits, the row in one workgroup: by their values ----
   // A row has few distinct logits, so a bin each: its tokens are counted, its weight is worked out once
   // and, for the masses, read from a table; a border is a bin and the tokens at it (the first of them in
@@ -947,62 +1011,14 @@ struct RowSampler {
       if ((lane & 15) == 0 && at < r1) s.chunk[at] = sum;
     }
     __syncthreads();
-    if (wave != 0) return;
-    // one wave does the rest: lane l has rows of pieces share * l .. share * (l + 1) - 1
-    const int share = (rows64 + 63) / 64, c0 = lane * share, c1 = min(rows64, c0 + share);
-    u64 own = 0, at = 0;
-    for (int i = c0; i < c1; ++i) {
-      own += s.chunk[i] & SM_MASS;
-      at += s.chunk[i] >> SM_TIES;
-    }
-    u64 tie0 = 0;  // tokens at the border before the lane's
-    if (ties) {
-      tie0 = sm_wave_scan(at) - at;
-      own += (min(tie0 + at, ties) - min(tie0, ties)) * tie_w;
-    }
-    u64 run = sm_wave_scan(own);
-    const u64 target = target_of(sm_lane(run, 63));
-    const unsigned long long hit = __ballot(run > target);
-    const int who = __ffsll((long long)hit) - 1;
-    run = sm_lane(run - own, who);
-    tie0 = sm_lane(tie0, who);
-    int R = who * share;
-    for (;; ++R) {
-      const u64 c = s.chunk[R], t = c >> SM_TIES;
-      const u64 x = (c & SM_MASS) + (min(tie0 + t, ties) - min(tie0, ties)) * tie_w;
-      if (run + x > target || R == rows64 - 1) break;
-      run += x;
-      tie0 += t;
-    }
-    R = __builtin_amdgcn_readfirstlane(R);
-    const int i0 = first_of(R);
-    const dkv_u32x4 v = load(R);
-    u64 w[E], t = 0, sum = 0;
-    value_weights<TABLE>(v, n, at_border, [&](int e, u64 x) {
-      w[e] = x;
-      t += x >> SM_TIES;
-    });
-    if (near) {
+    finish(ties, tie_w, [&](const dkv_u32x4& v, int, u64 (&w)[E]) {
+      value_weights<TABLE>(v, n, at_border, [&](int e, u64 x) { w[e] = x; });
+      if (near) {
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (is_near(v, e) ) w[e] = floored(weight(value(v, e)));
-    }
-    if (ties) {
-      tie0 += sm_wave_scan(t) - t;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (w[e] >> SM_TIES) w[e] = tie0++ < ties ? tie_w : 0ULL;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum += w[e];
-    run += sm_wave_scan(sum) - sum;
-    if (run <= target && target < run + sum) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (run <= target && target < run + w[e]) p.out[row] = (long long)(i0 + e);
-        run += w[e];
+        for (int e = 0; e < E; ++e)
+          if (is_near(v, e)) w[e] = floored(weight(value(v, e)));
       }
-    }
+    });
   }
   // The whole of it; false where the borders are among the tokens next to 0.
   __device__ __forceinline__ bool by_values() {
@@ -1030,43 +1046,6 @@ struct RowSampler {
     else
       by_weights<false>(n, ties, tie_w);
     return true;
-  }
-
-  // ---- the token in which u times the mass lies ----
-  __device__ __forceinline__ void finish() {
-    const int share = (rows64 + SM_THREADS - 1) / SM_THREADS;
-    const int c0 = tid * share, c1 = min(rows64, c0 + share);
-    u64 own = 0, all;
-    for (int i = c0; i < c1; ++i) own += s.chunk[i];
-    u64 run = before(own, s.wave, all);
-    const u64 target = target_of(all);
-    for (int i = c0; i < c1; ++i) {
-      const u64 c = s.chunk[i];
-      if (run <= target && target < run + c) {
-        s.pick[0] = (u64)i;
-        s.pick[1] = run;
-      }
-      run += c;
-    }
-    __syncthreads();
-    if (wave != 0) return;
-    const int R = (int)s.pick[0], i0 = first_of(R);
-    const dkv_u32x4 v = load(R);
-    u64 w[E], sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float l = value(v, e);
-      w[e] = is_kept(l, i0 + e) ? floored(weight(l)) : 0ULL;
-      sum += w[e];
-    }
-    u64 at = s.pick[1] + sm_wave_scan(sum) - sum;
-    if (at <= target && target < at + sum) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (at <= target && target < at + w[e]) p.out[row] = (long long)(i0 + e);
-        at += w[e];
-      }
-    }
   }
 };
 
@@ -1185,9 +1164,11 @@ __global__ __launch_bounds__(SM_THREADS) void sample_parts_kernel(SampleParams p
 
 // Workgroups of a row: rows for half the CUs have one each, fewer are cut so that the workgroups fill
 // the chip, if each of the 16 waves would have ten rows of pieces or more. The launches and the parts'
-// meeting cost 8 us. us, top-p, cut / whole: one row of 128256 bf16 24.0 / 58.8, 100 rows 51 / 64; 37
-// rows of 50257 fp32 27.6 / 34.5; one row of 32000 bf16 21.2 / 23.5 but with top-k 19.7 / 18.4; 64 rows of
-// 32000 fp32 27.4 / 25.6.
+// meeting cost 8 us. us, top-p, cut / whole: 37 rows of 50257 fp32 27.6 / 34.5, 64 rows of 32000 fp32
+// 27.4 / 25.6. 16-bit rows in one workgroup go by their values, which parts do not, and are cut into
+// six or more: bf16, top-k, top-p and both, one row of 128256 (7 parts) 21.6, 27.4, 22.7 / 26.5, 28.9,
+// 28.5; of 84000 (5) 21.7, 27.6, 22.4 / 20.8, 23.3, 23.0; 64 rows of 128256 (4) 30.7, 39.4, 32.2 / 30.6,
+// 32.8, 32.3.
 int sample_parts(int rows, int V, int dtype) {
   const int tokens = (dtype == DKV_F32 ? 4 : 8) * 64;
   const int rows64 = (V + tokens - 1) / tokens;
@@ -1195,7 +1176,7 @@ int sample_parts(int rows, int V, int dtype) {
   int n = 256 / rows;
   if (n > SM_PARTS) n = SM_PARTS;
   if (n > rows64 / (2 * SM_WAVES)) n = rows64 / (2 * SM_WAVES);
-  return n < 1 ? 1 : n;
+  return n < (dtype == DKV_F32 ? 2 : 6) ? 1 : n;
 }
 
 template <int DT>
