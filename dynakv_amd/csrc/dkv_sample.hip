@@ -411,7 +411,7 @@ struct RowSampler {
     for (int q = 0; q < 4; ++q) {
       const u64 h = s.hist[4 * tid + q];
       cnt[q] = h >> SM_COUNT;
-      mass[q] = bin_mass(4 * tid + q, h);
+      mass[q] = h ? bin_mass(4 * tid + q, h) : 0ULL;  // (most waves have none)
       n_sum += cnt[q];
       m_sum += mass[q];
     }
