@@ -17,6 +17,7 @@ import torch
 
 # the CPython binding's file beside the library, named for the interpreter it was built for
 CALL_NAME = "_dkv_call" + sysconfig.get_config_var("EXT_SUFFIX")
+TENSOR_NAME = "_dkv_tensor" + sysconfig.get_config_var("EXT_SUFFIX")
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libdynakv_amd.so"
 
 DKV_F32, DKV_F16, DKV_BF16 = 0, 1, 2
@@ -142,6 +143,7 @@ class DecodeLayerArgs(C.Structure):
 _lock = threading.Lock()
 _lib = None
 _calls = None
+_tensor_calls = False  # not looked for yet
 
 
 class DynaKVError(RuntimeError):
@@ -189,6 +191,32 @@ def calls():
             else:
                 _calls = lib
     return _calls
+
+
+def tensor_calls():
+    """The ``_dkv_tensor`` module, which makes the paged operators' ordinary calls from torch's tensors
+    and answers None to any other; None where there is none for this interpreter and torch beside the
+    library (the operators then make every call by themselves, with the same results)."""
+    global _tensor_calls
+    if _tensor_calls is not False:
+        return _tensor_calls
+    path = LIB_PATH.with_name(TENSOR_NAME)
+    if path.exists():
+        load()
+    with _lock:
+        if _tensor_calls is False:
+            mod = None
+            if path.exists():
+                spec = importlib.util.spec_from_file_location("_dkv_tensor", path)
+                try:
+                    mod = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(mod)
+                except ImportError:  # another torch's
+                    mod = None
+                if mod is not None and torch.__version__.split("+")[0] != mod.torch_version:
+                    mod = None
+            _tensor_calls = mod
+    return _tensor_calls
 
 
 def exported_symbols() -> list[str]:
@@ -275,6 +303,17 @@ def stream_of(t: torch.Tensor) -> int:
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def is_current(device: int) -> bool:
+    """Whether ``device`` is a GPU and the current one."""
+    return device >= 0 and _current_device() == device
+
+
+def stream_on(device: int) -> int:
+    """Raw hipStream_t of torch's current stream on a device."""
+    return (_raw_stream(device) if _raw_stream is not None
+            else torch.cuda.current_stream(device).cuda_stream)
 
 
 def call_on(device: int, fn, *args):

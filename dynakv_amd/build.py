@@ -4,7 +4,9 @@ Plain ``hipcc`` per source file (in parallel), then one link step, then the CPyt
 per-call entry points (``dkv_call.cpp``, ``dynakv_amd/lib/_dkv_call.<interpreter tag>.so``) linked
 against it. Both are built in-tree so they travel with the repository snapshot to the GPU host. The
 binding needs the interpreter's C headers; without them it is left out and the ctypes binding serves
-(the same functions, about 5 us more per call).
+(the same functions, about 5 us more per call). A second module (``dkv_tensor.cpp``) reads torch's
+tensors for the paged operators' calls; without torch's C++ headers it is left out and the wrappers'
+own checks serve (about 4 us more per call).
 
 Usage: ``python -m dynakv_amd.build`` (or ``dynakv_amd.build.build()``).
 """
@@ -12,6 +14,7 @@ Usage: ``python -m dynakv_amd.build`` (or ``dynakv_amd.build.build()``).
 from __future__ import annotations
 
 import concurrent.futures as _cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -24,6 +27,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libdynakv_amd.so"
 CALL_PATH = LIB_DIR / ("_dkv_call" + sysconfig.get_config_var("EXT_SUFFIX"))
+TENSOR_PATH = LIB_DIR / ("_dkv_tensor" + sysconfig.get_config_var("EXT_SUFFIX"))
 OBJ_DIR = PKG_DIR / "_build"
 SOURCES = ("dkv_append.hip", "dkv_generic.hip", "dkv_splitk.hip", "dkv_cutoff.hip",
            "dkv_prefill.hip", "dkv_layer.hip", "dkv_model.hip", "dkv_joint.hip", "dkv_dense.hip",
@@ -83,6 +87,30 @@ def _build_binding(verbose: bool) -> None:
     os.replace(tmp, CALL_PATH)
 
 
+def _build_tensor_binding(verbose: bool) -> None:
+    """The CPython module that takes torch's tensors, found beside the library at run time."""
+    headers = Path(sysconfig.get_paths()["include"])
+    spec = importlib.util.find_spec("torch")
+    torch_dir = Path(spec.origin).parent if spec and spec.origin else PKG_DIR
+    TENSOR_PATH.unlink(missing_ok=True)
+    if not (headers / "Python.h").exists() \
+            or not (torch_dir / "include/torch/csrc/autograd/python_variable.h").exists():
+        if verbose:
+            print(f"[dynakv_amd] no Python.h or torch headers under {headers}, {torch_dir}: tensor "
+                  "module left out", file=sys.stderr)
+        return
+    tmp = TENSOR_PATH.with_suffix(".so.tmp")
+    cmd = [_hipcc(), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wno-cast-function-type",
+           "-I", str(headers), "-I", str(torch_dir / "include"),
+           "-I", str(torch_dir / "include/torch/csrc/api/include"),
+           str(CSRC / "dkv_tensor.cpp"), "-o", str(tmp), f"-L{LIB_DIR}", "-l:libdynakv_amd.so",
+           f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"binding failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, TENSOR_PATH)
+
+
 def build(verbose: bool = True) -> Path:
     """Compile every HIP source and link the shared library. Always rebuilds."""
     OBJ_DIR.mkdir(exist_ok=True)
@@ -99,6 +127,7 @@ def build(verbose: bool = True) -> Path:
         raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
     _build_binding(verbose)
+    _build_tensor_binding(verbose)
     if verbose:
         print(f"[dynakv_amd] built {LIB_PATH}", file=sys.stderr)
     return LIB_PATH

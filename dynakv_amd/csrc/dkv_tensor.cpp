@@ -1,0 +1,201 @@
+// The paged operators' calls on torch tensors: module _dkv_tensor.
+//
+// A step of single tokens makes two calls a layer whose kernels take 4 to 6 us, and a call's checks of
+// its tensors, one attribute at a time from Python, take 5 us more than its launch. Here a call that is
+// as it should be and ordinary is checked, its output made and its entry point called; any other call
+// (an argument to refuse, an output to write to, a workspace, a copy to align) returns None, and the
+// Python function, which has every check and its message, does it.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
+
+#include <climits>
+
+#include "../../include/dynakv_amd.h"
+
+namespace {
+
+constexpr long long HEAD_DIM = 128;
+
+const at::Tensor* tensor(PyObject* o) {
+  return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+}
+
+bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+bool int32_on(const at::Tensor& t, c10::Device d) {
+  return t.scalar_type() == at::kInt && t.device() == d && t.layout() == at::kStrided;
+}
+
+// None, or the C types of a call's integers.
+bool ints(PyObject* const* args, Py_ssize_t n, long long* v) {
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    v[i] = PyLong_AsLongLong(args[i]);
+    if (v[i] == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+  }
+  return true;
+}
+
+// What PagedBatch holds for the calls: table pointer, row stride, columns, row starts, lengths,
+// requests, rows, max_new, min_new, max_len, device.
+struct Batch {
+  long long v[11];
+  bool read(PyObject* t) {
+    return PyTuple_Check(t) && PyTuple_GET_SIZE(t) == 11 &&
+           ints(&PyTuple_GET_ITEM(t, 0), 11, v);
+  }
+  const int* table() const { return reinterpret_cast<const int*>(v[0]); }
+  const int* starts() const { return reinterpret_cast<const int*>(v[3]); }
+  const int* lens() const { return reinterpret_cast<const int*>(v[4]); }
+  long long ld() const { return v[1]; }
+  int cols() const { return (int)v[2]; }
+  int requests() const { return (int)v[5]; }
+  int rows() const { return (int)v[6]; }
+  int max_new() const { return (int)v[7]; }
+  int min_new() const { return (int)v[8]; }
+  int max_len() const { return (int)v[9]; }
+};
+
+// Pools alike, of x's type and on its device, which is the batch's.
+bool pools(const at::Tensor& k, const at::Tensor& v, const at::Tensor& x, const Batch& b) {
+  if (k.dim() != 4 || v.dim() != 4 || k.sizes() != v.sizes() || k.strides() != v.strides())
+    return false;
+  const auto dt = x.scalar_type();
+  if ((dt != at::kBFloat16 && dt != at::kHalf) || k.scalar_type() != dt || v.scalar_type() != dt)
+    return false;
+  if (!x.is_cuda() || x.get_device() != b.v[10] || k.device() != x.device() ||
+      v.device() != x.device())
+    return false;
+  const long long ps = k.size(2);
+  return k.size(3) == HEAD_DIM && k.stride(3) == 1 && k.stride(2) == HEAD_DIM && ps >= 16 &&
+         (ps & (ps - 1)) == 0 && b.max_len() <= b.cols() * ps && k.size(0) <= INT_MAX &&
+         k.size(1) > 0 && k.size(1) <= 65536;
+}
+
+int code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? DKV_BF16 : DKV_F16; }
+
+// (page_table, q_start, lens, rows, max_new, max_len, min_new) -> the tuple above
+PyObject* paged_batch(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  long long v[4];
+  if (n != 7 || !ints(args + 3, 4, v)) Py_RETURN_NONE;
+  const at::Tensor *t = tensor(args[0]), *s = tensor(args[1]), *l = tensor(args[2]);
+  if (!t || !s || !l || t->dim() != 2 || s->dim() != 1 || l->dim() != 1) Py_RETURN_NONE;
+  const long long B = t->size(0), cols = t->size(1), ld = t->stride(0);
+  const c10::Device d = t->device();
+  if (l->size(0) != B || s->size(0) != B + 1 || !int32_on(*t, d) || !int32_on(*s, d) ||
+      !int32_on(*l, d) || !s->is_contiguous() || !l->is_contiguous() ||
+      (cols > 1 && t->stride(1) != 1) || (B > 1 && ld < cols))
+    Py_RETURN_NONE;
+  if (!(0 <= v[3] && v[3] <= v[1] && v[1] <= v[0] && v[0] <= INT_MAX && 0 <= v[2] &&
+        v[2] <= INT_MAX))
+    Py_RETURN_NONE;
+  return Py_BuildValue("(NLLNNLLLLLi)", PyLong_FromVoidPtr(t->data_ptr()), ld > cols ? ld : cols, cols,
+                       PyLong_FromVoidPtr(s->data_ptr()), PyLong_FromVoidPtr(l->data_ptr()), B, v[0],
+                       v[1], v[3], v[2], d.is_cuda() ? (int)t->get_device() : -1);
+}
+
+// (stream, qkv, k_pages, v_pages, batch, heads, frequencies, q_norm, k_norm, eps)
+PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Batch b;
+  long long heads, freq;
+  if (n != 10 || !b.read(args[4]) || !ints(args + 5, 1, &heads) || !ints(args + 6, 1, &freq))
+    Py_RETURN_NONE;
+  const at::Tensor *x = tensor(args[1]), *k = tensor(args[2]), *v = tensor(args[3]);
+  const double eps = PyFloat_Check(args[9]) ? PyFloat_AS_DOUBLE(args[9]) : -1.0;
+  if (!x || !k || !v || x->dim() != 2 || !(eps >= 0.0) || heads <= 0 || !pools(*k, *v, *x, b))
+    Py_RETURN_NONE;
+  const long long T = x->size(0), hkv = k->size(1), ld = x->stride(0);
+  if (x->stride(1) != 1 || heads > 65536 || x->size(1) < (heads + 2 * hkv) * HEAD_DIM ||
+      ld < x->size(1) || b.rows() > T || !aligned16(*x))
+    Py_RETURN_NONE;
+  const void* norm[2];
+  for (int i = 0; i < 2; ++i) {
+    norm[i] = nullptr;
+    if (args[7 + i] == Py_None) continue;
+    const at::Tensor* w = tensor(args[7 + i]);
+    if (!w || w->dim() != 1 || w->size(0) != HEAD_DIM || w->stride(0) != 1 ||
+        w->scalar_type() != x->scalar_type() || w->device() != x->device())
+      Py_RETURN_NONE;
+    norm[i] = w->data_ptr();
+  }
+  at::Tensor out = at::empty({T, heads, HEAD_DIM}, x->options());
+  int rc;
+  void* const stream = PyLong_AsVoidPtr(args[0]);
+  Py_BEGIN_ALLOW_THREADS;
+  rc = dkv_paged_append(
+      stream, code(*x), x->data_ptr(), ld, out.data_ptr(), heads * HEAD_DIM, HEAD_DIM,
+      k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1), (int)k->size(0), (int)k->size(2),
+      b.table(), b.ld(), b.cols(), b.starts(), b.lens(), b.requests(), b.rows(), (int)heads, (int)hkv,
+      (int)HEAD_DIM, norm[0], norm[1], (float)eps, reinterpret_cast<const double*>(freq));
+  Py_END_ALLOW_THREADS;
+  if (rc != DKV_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (stream, q, k_pages, v_pages, batch, scale)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Batch b;
+  if (n != 6 || !b.read(args[4]) || !PyFloat_Check(args[5])) Py_RETURN_NONE;
+  const at::Tensor *q = tensor(args[1]), *k = tensor(args[2]), *v = tensor(args[3]);
+  if (!q || !k || !v || q->dim() != 3 || q->size(2) != HEAD_DIM || !pools(*k, *v, *q, b))
+    Py_RETURN_NONE;
+  const long long T = q->size(0), hq = q->size(1), hkv = k->size(1);
+  const long long st = q->stride(0), sh = q->stride(1);
+  if (hq <= 0 || hq > 65536 || hq % hkv || q->stride(2) != 1 || (st & 7) || (sh & 7) ||
+      b.rows() > T || !aligned16(*q) ||
+      dkv_paged_workspace_floats(b.requests(), b.rows(), (int)hq, (int)hkv, b.max_new(), b.min_new(),
+                                 b.max_len()) > 0)
+    Py_RETURN_NONE;
+  at::Tensor out = at::empty({T, hq, HEAD_DIM}, q->options());
+  int rc;
+  const float scale = (float)PyFloat_AS_DOUBLE(args[5]);
+  void* const stream = PyLong_AsVoidPtr(args[0]);
+  Py_BEGIN_ALLOW_THREADS;
+  rc = dkv_paged_attention(
+      stream, code(*q), q->data_ptr(), st, sh, k->data_ptr(), v->data_ptr(),
+      k->stride(0), k->stride(1), (int)k->size(0), (int)k->size(2), b.table(), b.ld(), b.cols(),
+      b.starts(), b.lens(), b.requests(), b.rows(), (int)hq, (int)hkv, (int)HEAD_DIM, b.max_new(),
+      b.min_new(), b.max_len(), scale, nullptr, 0, out.data_ptr(), code(*q),
+      hq * HEAD_DIM, HEAD_DIM);
+  Py_END_ALLOW_THREADS;
+  if (rc != DKV_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (a C++ exception, of a tensor without memory or an allocation that failed: the Python function's)
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  try {
+    return F(self, args, n);
+  } catch (const std::exception&) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
+#define DKV_ENTRY(name) \
+  {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<name>)), METH_FASTCALL, nullptr}
+
+PyMethodDef methods[] = {DKV_ENTRY(paged_batch), DKV_ENTRY(paged_append), DKV_ENTRY(paged_attention),
+                         {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_dkv_tensor", nullptr, -1, methods,
+                      nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__dkv_tensor(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -51,12 +51,26 @@ class PagedBatch:
     tokens past ``max_new`` or keys past ``max_len`` may be left out."""
 
     __slots__ = ("_page_table", "_q_start", "_lens", "_rows", "_max_new", "_max_len", "_min_new",
-                 "_requests", "_device", "_table_args", "_row_args")
+                 "_requests", "_args")
     page_table, q_start, lens, rows, max_new, max_len, min_new, requests = (
         property(operator.attrgetter(name)) for name in __slots__[:8])
 
     def __init__(self, page_table: torch.Tensor, q_start: torch.Tensor, lens: torch.Tensor, *,
                  rows: int, max_new: int, max_len: int, min_new: int = 1):
+        self._page_table, self._q_start, self._lens = page_table, q_start, lens
+        self._rows, self._max_new, self._max_len, self._min_new = rows, max_new, max_len, min_new
+        # what every call passes of the batch (its buffers stay where they are): table pointer, row
+        # stride and columns, row starts, lengths, requests, rows, bounds, device
+        fast = _lib.tensor_calls()
+        self._args = None if fast is None else fast.paged_batch(
+            page_table, q_start, lens, rows, max_new, max_len, min_new)
+        if self._args is None:
+            self._args = self._checked()
+        self._requests = self._args[5]
+
+    def _checked(self) -> tuple:
+        page_table, q_start, lens = self._page_table, self._q_start, self._lens
+        rows, max_new, max_len, min_new = self._rows, self._max_new, self._max_len, self._min_new
         shape, n_start, n_lens = page_table.shape, q_start.shape, lens.shape
         if len(shape) != 2 or len(n_start) != 1 or len(n_lens) != 1:
             raise ValueError("page_table must be (B, P), q_start (B + 1,), lens (B,)")
@@ -74,12 +88,8 @@ class PagedBatch:
             raise ValueError("page_table, q_start and lens must be on one device")
         if not (0 <= min_new <= max_new <= rows and max_len >= 0):
             raise ValueError("need 0 <= min_new <= max_new <= rows and max_len >= 0")
-        self._page_table, self._q_start, self._lens = page_table, q_start, lens
-        self._requests, self._device = B, device
-        self._rows, self._max_new, self._max_len, self._min_new = rows, max_new, max_len, min_new
-        # what every call passes of the batch: its buffers stay where they are
-        self._table_args = (page_table.data_ptr(), max(ld, cols), cols)
-        self._row_args = (q_start.data_ptr(), lens.data_ptr(), B, rows)
+        return (page_table.data_ptr(), max(ld, cols), cols, q_start.data_ptr(), lens.data_ptr(), B,
+                rows, max_new, min_new, max_len, device)
 
 
 class PagedKVCache:
@@ -216,14 +226,14 @@ def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, dtyp
         raise ValueError("pages must hold a head's tokens back to back, with one layout for K and V")
     if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise ValueError("page and input dtypes differ")
-    if not (k_pages.get_device() == v_pages.get_device() == batch._device == device):
+    if not (k_pages.get_device() == v_pages.get_device() == batch._args[10] == device):
         raise ValueError("inputs, pages and batch must be on one device")
     pages, hkv, ps, _ = shape
     if ps < 16 or ps & (ps - 1):
         raise NotImplementedError("page_size must be a power of two of at least 16")
-    if batch._max_len > batch._table_args[2] * ps:
+    if batch._max_len > batch._args[2] * ps:
         raise ValueError(f"max_len {batch._max_len} is past the page table "
-                         f"({batch._table_args[2]} pages of {ps})")
+                         f"({batch._args[2]} pages of {ps})")
     return hkv, (k_pages.data_ptr(), v_pages.data_ptr(), st[0], st[1], pages, ps)
 
 
@@ -249,6 +259,13 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ((128,) of qkv's dtype) each query / key head is first normed, x / sqrt(mean(x^2) + eps) * w.
     Everything in fp32, rounded once where it is stored. ``out``: where the queries go (T, heads,
     128), unit last stride (qkv's own query columns will do). A token whose page is not there is not stored."""
+    freqs = _frequency_address(theta, inv_freq)
+    fast = _lib.tensor_calls()
+    if fast is not None and out is None and _lib.is_current(batch._args[10]):
+        out = fast.paged_append(_lib.stream_on(batch._args[10]), qkv, k_pages, v_pages, batch._args,
+                                heads, ctypes.addressof(freqs), q_norm, k_norm, eps)
+        if out is not None:
+            return out
     shape, st = qkv.shape, qkv.stride()
     if len(shape) != 2 or st[1] != 1:
         raise ValueError("qkv must be (T, W) with unit last stride")
@@ -265,7 +282,6 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             raise ValueError("norm weights must be contiguous (128,) vectors of qkv's dtype")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    freqs = _frequency_address(theta, inv_freq)
     stream = _lib.stream_of(qkv)
     if out is None:
         out, o_st = qkv.new_empty(T, heads, HEAD_DIM), (heads * HEAD_DIM, HEAD_DIM)
@@ -276,7 +292,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         o_st = _row_strides(out)
     _lib.check(_lib.call_on(
         dev, _lib.calls().dkv_paged_append, stream, _lib.dtype_code(dt), qkv.data_ptr(),
-        st[0] if T > 1 else width, out.data_ptr(), *o_st, *pools, *batch._table_args, *batch._row_args, heads, hkv,
+        st[0] if T > 1 else width, out.data_ptr(), *o_st, *pools, *batch._args[:7], heads, hkv,
         HEAD_DIM, _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs)),
         "dkv_paged_append")
     return out
@@ -293,6 +309,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     are appended first); one that has none to attend gives 0. ``scale`` defaults to 1 / sqrt(128).
     The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``;
     ``out`` may be q itself."""
+    fast = _lib.tensor_calls()
+    if (fast is not None and out is None and out_dtype is None
+            and _lib.is_current(batch._args[10])):
+        out = fast.paged_attention(_lib.stream_on(batch._args[10]), q, k_pages, v_pages, batch._args,
+                                   _SCALE if scale is None else scale)
+        if out is not None:
+            return out
     shape, st = q.shape, q.stride()
     if len(shape) != 3 or shape[2] != HEAD_DIM:
         raise ValueError("q must be (T, heads, 128)")
@@ -318,12 +341,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     else:
         o_st = _row_strides(out)
     lib = _lib.calls()
-    bounds = batch._max_new, batch._min_new, batch._max_len
+    bounds = batch._args[7:10]
     need = lib.dkv_paged_workspace_floats(batch._requests, batch._rows, hq, hkv, *bounds)
     ws = _attention_workspace(q.device, stream, need) if need else None
     _lib.check(_lib.call_on(
         dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), st[0], st[1],
-        *pools, *batch._table_args, *batch._row_args, hq, hkv, HEAD_DIM, *bounds,
+        *pools, *batch._args[:7], hq, hkv, HEAD_DIM, *bounds,
         _SCALE if scale is None else float(scale), _lib.ptr(ws), ws.numel() if need else 0,
         out.data_ptr(), _lib.dtype_code(odt), *o_st), "dkv_paged_attention")
     return out

@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from dynakv_amd import _lib
 from dynakv_amd.kernels.paged import PagedBatch, PagedKVCache, paged_append, paged_attention
 
 DH = 128
@@ -779,3 +780,33 @@ def test_attention_scores_far_apart(dev, new, lens, size):
             assert torch.equal(got[r, h][sure], v.to(BF)[at[:, 0]][sure]), (b, h)
             checked += int(sure.sum())
     assert checked > 0.9 * s.rows * 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_same_with_and_without_the_tensor_module(dev, dtype, monkeypatch):
+    print(f"[gpu] paged without the tensor module {dtype}", flush=True)
+    s = [Step(dev, new, lens, hkv=2, seed=59, dtype=dtype, pad=2)
+         for new, lens in (([1], [90]), ([1, 1], [700, 90]), ([40, 3], [60, 9]), ([0, 2], [4, 7]))]
+    inputs = [(t.rand(t.T, 12 * DH), 1 + t.rand(DH, scale=0.2)) for t in s]
+
+    def run():
+        out = []
+        for t, (qkv, w) in zip(s, inputs):
+            q = paged_append(qkv, t.k, t.v, t.batch, heads=8, theta=1e4)
+            q2 = paged_append(qkv, t.k, t.v, t.batch, heads=8, inv_freq=[0.5] * 64, q_norm=w, k_norm=w,
+                              eps=1e-5)
+            o = paged_attention(q2, t.k, t.v, t.batch)
+            out += [x[:t.rows] for x in (q, q2, o, paged_attention(q, t.k, t.v, t.batch, scale=0.2))]
+        return [x.clone() for x in out] + [t.k.view(torch.int16).clone() for t in s]
+
+    fast = run()
+    monkeypatch.setattr(_lib, "_tensor_calls", None)
+    for a, b in zip(run(), fast):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        monkeypatch.setattr(_lib, "_tensor_calls", False)
+        torch.cuda.synchronize()
+        for a, b in zip(run(), fast):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()

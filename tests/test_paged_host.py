@@ -203,3 +203,33 @@ def test_sampling_refusals():
     assert call(0, 1, 8) == _lib.DKV_E_ARG and call(0, -1, 8) == _lib.DKV_E_ARG
     assert call(9, 1, 8) == _lib.DKV_E_UNSUPPORTED and call(0, 1, 1 << 20) == _lib.DKV_E_UNSUPPORTED
     assert call(0, 0, 8) == _lib.DKV_OK and call(0, 1, 0) == _lib.DKV_E_ARG
+
+
+def test_without_the_tensor_module(monkeypatch):
+    """What a batch holds for its calls is the same, and so is what is refused."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    table = torch.zeros(3, 9, dtype=torch.int32)
+    makes = [lambda: PagedBatch(table[:2, :5], start, lens, rows=4, max_new=3, max_len=20, min_new=2),
+             lambda: PagedBatch(table[:1, :1], start[:2], lens[:1], rows=0, max_new=0, max_len=0,
+                                min_new=0),
+             lambda: PagedBatch(table[:0], start[:1], lens[:0], rows=7, max_new=1, max_len=5)]
+    start, lens = i32(0, 2, 4), i32(20, 7)
+    assert _lib.tensor_calls() is not None  # built here
+    fast = [m() for m in makes]
+    monkeypatch.setattr(_lib, "_tensor_calls", None)
+    for m, f in zip(makes, fast):
+        assert m()._args == f._args and m().requests == f.requests
+    test_batch_refusals()
+    test_append_refusals()
+    test_attention_refusals()
+
+
+def test_tensor_module_of_another_torch(monkeypatch, tmp_path):
+    """It is left alone: the operators make their calls by themselves."""
+    monkeypatch.setattr(_lib, "_tensor_calls", False)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    assert _lib.tensor_calls() is None
+    monkeypatch.setattr(_lib, "_tensor_calls", False)
+    monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "none.so")
+    assert _lib.tensor_calls() is None
+    _batch()
