@@ -3,7 +3,7 @@
 // A step of single tokens makes two calls a layer whose kernels take 4 to 6 us, and a call's checks of
 // its tensors, one attribute at a time from Python, take 5 us more than its launch. Here a call that is
 // as it should be and ordinary is checked, its output made and its entry point called; any other call
-// (an argument to refuse, an output to write to, a workspace, a copy to align) returns None, and the
+// (an argument to refuse, an output to write to, a copy to align) returns None, and the
 // Python function, which has every check and its message, does it.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -139,21 +139,37 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
-// (stream, q, k_pages, v_pages, batch, scale)
+// (stream, q, k_pages, v_pages, batch, scale, workspace): workspace(q, stream, floats) gives a tensor
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Batch b;
-  if (n != 6 || !b.read(args[4]) || !PyFloat_Check(args[5])) Py_RETURN_NONE;
+  if (n != 7 || !b.read(args[4]) || !PyFloat_Check(args[5])) Py_RETURN_NONE;
   const at::Tensor *q = tensor(args[1]), *k = tensor(args[2]), *v = tensor(args[3]);
   if (!q || !k || !v || q->dim() != 3 || q->size(2) != HEAD_DIM || !pools(*k, *v, *q, b))
     Py_RETURN_NONE;
   const long long T = q->size(0), hq = q->size(1), hkv = k->size(1);
   const long long st = q->stride(0), sh = q->stride(1);
   if (hq <= 0 || hq > 65536 || hq % hkv || q->stride(2) != 1 || (st & 7) || (sh & 7) ||
-      b.rows() > T || !aligned16(*q) ||
-      dkv_paged_workspace_floats(b.requests(), b.rows(), (int)hq, (int)hkv, b.max_new(), b.min_new(),
-                                 b.max_len()) > 0)
+      b.rows() > T || !aligned16(*q))
     Py_RETURN_NONE;
   at::Tensor out = at::empty({T, hq, HEAD_DIM}, q->options());
+  const long long need = dkv_paged_workspace_floats(b.requests(), b.rows(), (int)hq, (int)hkv,
+                                                    b.max_new(), b.min_new(), b.max_len());
+  float* ws = nullptr;
+  long long ws_floats = 0;
+  PyObject* held = nullptr;  // until the launch
+  if (need > 0) {
+    PyObject* floats = PyLong_FromLongLong(need);
+    held = floats ? PyObject_CallFunctionObjArgs(args[6], args[1], args[0], floats, nullptr) : nullptr;
+    Py_XDECREF(floats);
+    const at::Tensor* t = held ? tensor(held) : nullptr;
+    if (!t) {
+      Py_XDECREF(held);
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    ws = static_cast<float*>(t->data_ptr());
+    ws_floats = t->numel();
+  }
   int rc;
   const float scale = (float)PyFloat_AS_DOUBLE(args[5]);
   void* const stream = PyLong_AsVoidPtr(args[0]);
@@ -162,9 +178,10 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       stream, code(*q), q->data_ptr(), st, sh, k->data_ptr(), v->data_ptr(),
       k->stride(0), k->stride(1), (int)k->size(0), (int)k->size(2), b.table(), b.ld(), b.cols(),
       b.starts(), b.lens(), b.requests(), b.rows(), (int)hq, (int)hkv, (int)HEAD_DIM, b.max_new(),
-      b.min_new(), b.max_len(), scale, nullptr, 0, out.data_ptr(), code(*q),
+      b.min_new(), b.max_len(), scale, ws, ws_floats, out.data_ptr(), code(*q),
       hq * HEAD_DIM, HEAD_DIM);
   Py_END_ALLOW_THREADS;
+  Py_XDECREF(held);
   if (rc != DKV_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
 }

@@ -313,7 +313,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if (fast is not None and out is None and out_dtype is None
             and _lib.is_current(batch._args[10])):
         out = fast.paged_attention(_lib.stream_on(batch._args[10]), q, k_pages, v_pages, batch._args,
-                                   _SCALE if scale is None else scale)
+                                   _SCALE if scale is None else scale, _attention_workspace)
         if out is not None:
             return out
     shape, st = q.shape, q.stride()
@@ -343,7 +343,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lib = _lib.calls()
     bounds = batch._args[7:10]
     need = lib.dkv_paged_workspace_floats(batch._requests, batch._rows, hq, hkv, *bounds)
-    ws = _attention_workspace(q.device, stream, need) if need else None
+    ws = _attention_workspace(q, stream, need) if need else None
     _lib.check(_lib.call_on(
         dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), st[0], st[1],
         *pools, *batch._args[:7], hq, hkv, HEAD_DIM, *bounds,
@@ -352,12 +352,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
-def _attention_workspace(device: torch.device, stream: int, floats: int) -> torch.Tensor:
+def _attention_workspace(q: torch.Tensor, stream: int, floats: int) -> torch.Tensor:
     """Split records and arrival counters (zero before and after a call). Eager calls of a stream
     share its workspace, in that stream's order. A call under capture gets one of its own in the
     graph's pool, cleared by the graph itself: two captured graphs may be replayed at once."""
-    if _lib.call_on(device.index, torch.cuda.is_current_stream_capturing):
-        ws = torch.empty(floats, dtype=torch.float32, device=device)
+    if _lib.call_on(q.get_device(), torch.cuda.is_current_stream_capturing):
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device)
         ws[:_COUNTERS].zero_()
         return ws
-    return workspace(device, stream, floats)
+    return workspace(q.device, stream, floats)
