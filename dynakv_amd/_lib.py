@@ -194,7 +194,7 @@ def calls():
 
 
 def tensor_calls():
-    """The ``_dkv_tensor`` module, which makes the paged operators' ordinary calls from torch's tensors
+    """The ``_dkv_tensor`` module, which makes the serving operators' ordinary calls from torch's tensors
     and answers None to any other; None where there is none for this interpreter and torch beside the
     library (the operators then make every call by themselves, with the same results)."""
     global _tensor_calls

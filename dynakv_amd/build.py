@@ -5,7 +5,7 @@ per-call entry points (``dkv_call.cpp``, ``dynakv_amd/lib/_dkv_call.<interpreter
 against it. Both are built in-tree so they travel with the repository snapshot to the GPU host. The
 binding needs the interpreter's C headers; without them it is left out and the ctypes binding serves
 (the same functions, about 5 us more per call). A second module (``dkv_tensor.cpp``) reads torch's
-tensors for the paged operators' calls; without torch's C++ headers it is left out and the wrappers'
+tensors for the serving operators' calls; without torch's C++ headers it is left out and the wrappers'
 own checks serve (about 4 us more per call).
 
 Usage: ``python -m dynakv_amd.build`` (or ``dynakv_amd.build.build()``).

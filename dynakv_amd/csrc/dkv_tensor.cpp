@@ -1,4 +1,4 @@
-// The paged operators' calls on torch tensors: module _dkv_tensor.
+// The serving operators' calls on torch tensors: module _dkv_tensor.
 //
 // A step of single tokens makes two calls a layer whose kernels take 4 to 6 us, and a call's checks of
 // its tensors, one attribute at a time from Python, take 5 us more than its launch. Here a call that is
@@ -186,6 +186,64 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// A setting of the sampling: a contiguous tensor with an entry per row, or a number for all rows.
+bool setting(PyObject* o, const at::Tensor& u, at::ScalarType type, const void*& rows, double& all) {
+  rows = nullptr;
+  all = 0.0;
+  if (PyFloat_Check(o)) {
+    all = PyFloat_AS_DOUBLE(o);
+    return type == at::kFloat;
+  }
+  if (PyLong_Check(o)) {
+    long long x;
+    if (!ints(&o, 1, &x) || x < INT_MIN || x > INT_MAX) return false;
+    all = (double)x;
+    return true;
+  }
+  const at::Tensor* t = tensor(o);
+  if (!t || t->dim() != 1 || t->size(0) != u.size(0) || t->scalar_type() != type ||
+      !t->is_contiguous() || t->device() != u.device())
+    return false;
+  rows = t->data_ptr();
+  return true;
+}
+
+// (stream, device, logits, u, temperature, top_k, top_p, min_p)
+PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  long long dev;
+  if (n != 8 || !ints(args + 1, 1, &dev)) Py_RETURN_NONE;
+  const at::Tensor *x = tensor(args[2]), *u = tensor(args[3]);
+  if (!x || !u || x->dim() != 2 || u->dim() != 1 || !x->is_cuda() || x->get_device() != dev ||
+      u->device() != x->device() || u->scalar_type() != at::kFloat || !u->is_contiguous())
+    Py_RETURN_NONE;
+  const long long rows = x->size(0), V = x->size(1);
+  const auto dt = x->scalar_type();
+  if (rows != u->size(0) || rows > INT_MAX || V < 1 || V > (1 << 19) || (V > 1 && x->stride(1) != 1) ||
+      (dt != at::kBFloat16 && dt != at::kHalf && dt != at::kFloat))
+    Py_RETURN_NONE;
+  const void* by_row[4];
+  double all[4];
+  for (int i = 0; i < 4; ++i)
+    if (!setting(args[4 + i], *u, i == 1 ? at::kInt : at::kFloat, by_row[i], all[i])) Py_RETURN_NONE;
+  const int code = dt == at::kBFloat16 ? DKV_BF16 : dt == at::kHalf ? DKV_F16 : DKV_F32;
+  at::Tensor out = at::empty({rows}, x->options().dtype(at::kLong)), ws;
+  const long long need = dkv_sample_workspace_bytes(code, (int)rows, (int)V);
+  if (need > 0) ws = at::empty({need}, x->options().dtype(at::kByte));
+  int rc;
+  void* const stream = PyLong_AsVoidPtr(args[0]);
+  const int top_k = (int)(all[1] < 0.0 ? 0.0 : all[1] > (double)V ? (double)V : all[1]);
+  Py_BEGIN_ALLOW_THREADS;
+  rc = dkv_sample_tokens(
+      stream, code, x->data_ptr(), rows > 1 ? x->stride(0) : V, (int)rows, (int)V,
+      static_cast<const float*>(u->data_ptr()), static_cast<const float*>(by_row[0]), (float)all[0],
+      static_cast<const int*>(by_row[1]), top_k, static_cast<const float*>(by_row[2]), (float)all[2],
+      static_cast<const float*>(by_row[3]), (float)all[3], need > 0 ? ws.data_ptr() : nullptr, need,
+      static_cast<long long*>(out.data_ptr()));
+  Py_END_ALLOW_THREADS;
+  if (rc != DKV_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
 // (a C++ exception, of a tensor without memory or an allocation that failed: the Python function's)
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
@@ -201,7 +259,7 @@ PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<name>)), METH_FASTCALL, nullptr}
 
 PyMethodDef methods[] = {DKV_ENTRY(paged_batch), DKV_ENTRY(paged_append), DKV_ENTRY(paged_attention),
-                         {nullptr, nullptr, 0, nullptr}};
+                         DKV_ENTRY(sample_tokens), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_dkv_tensor", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

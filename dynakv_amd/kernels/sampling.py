@@ -45,6 +45,14 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     token. A logit of -inf is never taken, NaN counts as -inf, +inf ones share the mass among
     themselves, and a row with no logit above -inf gives -1. Masses are summed in 64-bit fixed
     point, so a result depends on the row alone."""
+    fast = _lib.tensor_calls()
+    if fast is not None and out is None:
+        dev = logits.get_device()
+        if _lib.is_current(dev):
+            out = fast.sample_tokens(_lib.stream_on(dev), dev, logits, u, temperature, top_k, top_p,
+                                     min_p)
+            if out is not None:
+                return out
     shape, st = logits.shape, logits.stride()
     if len(shape) != 2 or (shape[1] > 1 and st[1] != 1):
         raise ValueError("logits must be (rows, V) with unit last stride")

@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from dynakv_amd import _lib
 from dynakv_amd.kernels.sampling import sample_tokens
 
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
@@ -310,3 +311,27 @@ def test_logits_of_every_kind(dev, kind, dtype):
         p = torch.tensor(kw[1], dtype=torch.float32).item()
         want = _all(x[few.to(dev)], u[few.to(dev)], 1.0, kw[0], p, 0.0)
         assert [t[int(i)] for i in few] == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_same_with_and_without_the_tensor_module(dev, dtype, monkeypatch):
+    print(f"[gpu] sample without the tensor module {dtype}", flush=True)
+    inputs = [_inputs(dev, rows, V, dtype, V) for rows, V in ((1, 1), (5, 999), (3, 131072), (0, 5))]
+
+    def run():
+        out = []
+        for x, u, _ in inputs:
+            n = x.shape[0]
+            each = [torch.full((n,), v, device=dev) for v in (0.7, 0.8, 0.01)]
+            k = torch.full((n,), 50, dtype=torch.int32, device=dev)
+            out += [sample_tokens(x, u), sample_tokens(x, u, top_k=10**12),
+                    sample_tokens(x, u, temperature=1, top_k=-3, top_p=0.9, min_p=0.1),
+                    sample_tokens(x, u, temperature=each[0], top_k=k, top_p=each[1], min_p=each[2]),
+                    sample_tokens(x[:, :max(1, x.shape[1] - 1)], u, top_k=7)]
+        return out
+
+    fast = run()
+    monkeypatch.setattr(_lib, "_tensor_calls", None)
+    for a, b in zip(run(), fast):
+        assert a.dtype == b.dtype == torch.int64 and torch.equal(a, b)
