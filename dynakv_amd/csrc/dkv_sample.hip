@@ -344,10 +344,13 @@ struct RowSampler {
       infinite = true;
       m = 0.f;
     }
+    set_scale();
+    return true;
+  }
+  __device__ __forceinline__ void set_scale() {
     const double c64 = 64.0 * 1.4426950408889634074 / (double)fminf(fmaxf(t, 1e-30f), 1e30f);
     c_hi = (float)c64;
     c_lo = (float)(c64 - (double)c_hi);
-    return true;
   }
 
   // x of a logit, up to that of the last bin (that of a NaN); `dl`: max l - l as it was rounded
@@ -813,7 +816,11 @@ struct RowSampler {
   static constexpr int INF = DT == DKV_BF16 ? 0x7f80 : 0x7c00;
   typedef short s2 __attribute__((ext_vector_type(2)));
   typedef unsigned short u2 __attribute__((ext_vector_type(2)));
-  int k_max, k_lo;   // the largest logit's key, and the key of bin 0; bins 0 .. 63 catch what has no weight
+  // keys of 4096 (bf16) or 64 (fp16): rows without larger logits are counted before their largest is
+  // known
+  static constexpr int LIMIT = DT == DKV_BF16 ? ((127 + 12) << 7) - NEAR : ((15 + 6) << 10) - NEAR;
+  int k_max, k_lo;   // the largest logit's key, and the key of bin 0; bins 0 .. 63 catch what lies below
+  int k_low;         // the lowest key that has a weight, or less
   int near_n = 0;    // tokens next to 0
   u64 near_m = 0;    // what their weights are above those of as many at 0 (modulo 2^64)
   static __device__ __forceinline__ s2 keys(uint32_t v) {
@@ -832,18 +839,22 @@ struct RowSampler {
       b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaxf(l, -65504.f), 0.f));
     return keys(b)[0];
   }
-  // Whether the row's range of logits has bins.
-  __device__ __forceinline__ bool by_values_fits() {
-    k_max = key_of(m);
+  __device__ __forceinline__ void set_low() {
     // no weight at x = SM_BINS - 1; the key is off by less than 2
     const int low = key_of(fmaxf(m - (float)SM_BINS / c_hi, -3.4028234663852886e38f)) - 2;
-    k_lo = max(low, -(INF - NEAR) + 1) - 64;
+    k_low = max(low, -(INF - NEAR) + 1);
+  }
+  // Whether the row's range of logits has bins, below its largest logit.
+  __device__ __forceinline__ bool by_values_fits() {
+    k_max = key_of(m);
+    set_low();
+    k_lo = k_low - 64;
     return k_max - k_lo <= SM_KEYS - 2;
   }
   static __device__ __forceinline__ bool is_near(const dkv_u32x4& v, int e) {
     return ((v[e / 2] >> (16 * (e & 1))) & 0x7fffu) - 1 < (uint32_t)NEAR;
   }
-  // f(logit) for the piece's tokens next to 0
+  // f(logit) for the tokens of the piece that are next to 0 and not 0
   template <class F>
   __device__ __forceinline__ void next_to_0(const dkv_u32x4& v, F&& f) const {
     u2 least = {0xffff, 0xffff};
@@ -856,35 +867,64 @@ struct RowSampler {
     for (int e = 0; e < E; ++e)
       if (is_near(v, e)) f(value(v, e));
   }
-  __device__ __forceinline__ void count_values() {
-    const int range = k_max - k_lo;
-    for (int i = 4 * tid; i <= range; i += 4 * SM_THREADS)
+  // The tokens by their key, from k_lo on; what is above bin `top` goes to it.
+  __device__ __forceinline__ void count_values(int top) {
+    for (int i = 4 * tid; i <= top; i += 4 * SM_THREADS)
       *(dkv_u32x4*)&s.bins[i] = dkv_u32x4{0u, 0u, 0u, 0u};
-    if (tid == 0) s.n = 0, s.pick[3] = 0;
     __syncthreads();
-    const s2 lo = {(short)k_lo, (short)k_lo}, own = {(short)lane, (short)lane};
+    const s2 lo = {(short)k_lo, (short)k_lo}, own = {(short)lane, (short)lane},
+             end = {(short)top, (short)top};
     each([&](int, int, const dkv_u32x4& v) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const s2 k = __builtin_elementwise_max(__builtin_elementwise_sub_sat(keys(v[i]), lo), own);
+        const s2 k = __builtin_elementwise_min(
+            __builtin_elementwise_max(__builtin_elementwise_sub_sat(keys(v[i]), lo), own), end);
         const uint32_t b = __builtin_bit_cast(uint32_t, k);
         atomicAdd(&s.bins[b & 0xffffu], 1u);
         atomicAdd(&s.bins[b >> 16], 1u);
       }
     });
     __syncthreads();
-    if (count_at(-k_lo)) {  // tokens at 0, or next to it
-      const u64 w0 = weight(0.f);
-      each([&](int, int i0, const dkv_u32x4& v) {
-        next_to_0(v, [&](float l) {
-          atomicAdd(&s.pick[3], weight(l) - w0);
-          atomicAdd(&s.n, 1);
-        });
+  }
+  // The same before the row's largest logit is known, which is then the last bin that is not empty;
+  // false where it has to be found by itself.
+  __device__ __forceinline__ bool count_first() {
+    constexpr int TOP = 2 * LIMIT + 65;  // above LIMIT: too large, infinite or NaN
+    k_lo = -LIMIT - 64;
+    keep_root();
+    count_values(TOP);
+    int best = 0;
+    for (int i = 64 + tid; i < TOP; i += SM_THREADS) best = s.bins[i] ? i : best;
+    best = (int)dkv_wave_max_fast((float)best);
+    if (lane == 0) s.wave[wave] = (u64)best;
+    __syncthreads();
+    best = (int)dkv_wave_max_fast((float)s.wave[lane & (SM_WAVES - 1)]);
+    const uint32_t over = s.bins[TOP];
+    __syncthreads();
+    best = __builtin_amdgcn_readfirstlane(best);
+    k_max = best + k_lo;
+    if (over || best < 64 || k_max == 0) return false;
+    m = of_key(k_max);
+    set_scale();
+    set_low();
+    return k_low >= -LIMIT;
+  }
+  // the weights of tokens next to 0
+  __device__ __forceinline__ void weigh_near() {
+    if (!count_at(-k_lo) || k_low > 0) return;
+    const u64 w0 = weight(0.f);
+    __syncthreads();
+    if (tid == 0) s.n = 0, s.pick[3] = 0;
+    __syncthreads();
+    each([&](int, int, const dkv_u32x4& v) {
+      next_to_0(v, [&](float l) {
+        atomicAdd(&s.pick[3], weight(l) - w0);
+        atomicAdd(&s.n, 1);
       });
-      __syncthreads();
-      near_n = s.n;
-      near_m = s.pick[3];
-    }
+    });
+    __syncthreads();
+    near_n = s.n;
+    near_m = s.pick[3];
   }
   __device__ __forceinline__ uint32_t count_at(int bin) const {
     return bin >= 64 && bin <= k_max - k_lo ? s.bins[bin] : 0u;
@@ -1020,13 +1060,13 @@ struct RowSampler {
       }
     });
   }
-  // The whole of it; false where the borders are among the tokens next to 0.
+  // The whole of it, of a row that is counted; false where the borders are among the tokens next to 0.
   __device__ __forceinline__ bool by_values() {
-    int end = k_max - k_lo - 64;  // the last bin that has a weight
-    uint32_t end_n = 0;           // its tokens that are kept, where it is a border
+    int end = k_max - k_low;  // the last bin that has a weight
+    uint32_t end_n = 0;       // its tokens that are kept, where it is a border
     bool found = false;
     if (by_k || by_p) {
-      count_values();
+      weigh_near();
       end_n = ~0u;
       if (by_k && border<false>(end, end_n)) {
         found = true;
@@ -1055,9 +1095,15 @@ __global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(SampleParams p)
   __shared__ SampleShared<DT> s;
   RowSampler<DT> r(p, s, blockIdx.x);
   r.take(0, 1);
-  if (!r.begin(r.largest(), true)) return;
   if constexpr (DT != DKV_F32)
-    if (r.by_values_fits() && r.by_values()) return;
+    if ((r.by_k || r.by_p) && !r.greedy() && r.count_first() && r.by_values()) return;
+  if (!r.begin(r.largest(), true)) return;
+  if constexpr (DT != DKV_F32) {
+    if (r.by_values_fits()) {
+      if (r.by_k || r.by_p) r.count_values(r.k_max - r.k_lo + 1);
+      if (r.by_values()) return;
+    }
+  }
   if (r.by_k || r.by_p) {
     r.histogram();
     r.run_sums();
