@@ -71,6 +71,10 @@ __device__ __forceinline__ int paged_page(const PagedPool& pool, int b, int t) {
 // 2^-8 of a radian, as much as a bf16 rounding; reduced to one revolution it fits 32 bits.
 // One wave per row and 8 heads: lane (head h = lane / 8, piece c = lane % 8) holds dims
 // 8c .. 8c + 7 and 64 + 8c .. 64 + 8c + 7, so both halves of its eight pairs.
+//
+// Bound by memory where there is much to do: 8192 tokens of 32 + 2 x 8 heads with norms 44.9 us, 4.5 TB/s
+// of reads and writes (a large copy has 4.8); 16 tokens 4.0 us, the chain of loads to the page id.
+// Stores past the caches (non-temporal) take 3 us off the former and add 9 to the attention after it.
 // ---------------------------------------------------------------------------------------
 struct AppendParams {
   const uint16_t* qkv;
@@ -261,7 +265,8 @@ __device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
 // tokens, so slots behind them read as zero and cost nothing. S^T = K Q^T and P V on 16x16x32 MFMA
 // with the rows in the operand's columns; the weights go to the products as 16-bit hi + lo
 // pairs, which the 32 deep products of 16 tokens have room for. Waves are joined in LDS, parts by the
-// unit's last one to arrive.
+// unit's last one to arrive. 16 requests of 2K to 8K tokens (8 KV heads) 61 us, 5.7 TB/s; two of 65533
+// 86 us, 6.0 TB/s; one of 96 5.5 us, the latency of lengths, page ids, one tile and the joins.
 //
 // How a step's units are cut: requests have any lengths, which only the device knows, and the launch
 // has a fixed number of workgroups. Every wave finds the smallest part C (tiles) for which

@@ -15,16 +15,20 @@
 //   w = 2^(-i/64) (1 - d),  d = 1 - 2^(-(x - i)/64) < 0.011,
 // d to 31 bits after the point, 2^(-j/64) from a table of 64.
 //
-// A row goes by three times (from the caches after the first): for the maximum; for a histogram of the
-// tokens by i, counts and sums of d in one 64-bit number, so that a bin's mass is known and with it the
-// bins of the borders; for the mass of every 512 tokens (256 in fp32) above those bins, in the
-// vocabulary's order, and the tokens inside them, which are sorted and those kept added. Then the 512
-// and the token in which u times the mass lies are known. A bin of too many tokens (equal logits, a
-// border 64 halvings down) goes through a search by the digits of the logits instead.
-//
-// Bound by vector instructions: a row of 128256 in one CU takes 0.85 us an instruction, of which the
-// histogram has 22 a token. One workgroup takes a row where there are rows for half the CUs; fewer rows
-// are cut into parts, a launch for each of the three passes.
+// Two ways through a row:
+//  * 16-bit logits, a workgroup per row: by their values. A bin for each value (those next to 0 share
+//    one), so the row is read twice: for the counts, from which the borders follow with one weight a
+//    bin, and for the mass of every 512 tokens, by a table of the weights. Then the 512 and the token in
+//    which u times the mass lies are known. us, 256 rows of 128256 bf16 with top-p: 34.5, of which the
+//    first reading takes 10 at the rate of the memory, the second 9 (11 vector instructions a token and
+//    a table read); 90 by bins of the weights' logarithm as below.
+//  * otherwise by the logarithm of the weights: for the maximum; for a histogram of the tokens by i,
+//    counts and sums of d in one 64-bit number, so that a bin's mass is known and with it the bins of the
+//    borders; for the mass of every 512 tokens (256 in fp32) above those bins, and the tokens inside
+//    them, which are sorted and those kept added. A bin of too many tokens (equal logits, a border 64
+//    halvings down) goes through a search by the digits of the logits instead. Bound by vector
+//    instructions where a row has one CU (17 a token for the histogram), else by latency. Few rows are
+//    cut into parts, a launch for each of the three passes; 37 rows of 50257 fp32: 27 us.
 #include "dkv_common.h"
 
 namespace {
@@ -1212,9 +1216,8 @@ __global__ __launch_bounds__(SM_THREADS) void sample_parts_kernel(SampleParams p
 // the chip, if each of the 16 waves would have ten rows of pieces or more. The launches and the parts'
 // meeting cost 8 us. us, top-p, cut / whole: 37 rows of 50257 fp32 27.6 / 34.5, 64 rows of 32000 fp32
 // 27.4 / 25.6. 16-bit rows in one workgroup go by their values, which parts do not, and are cut into
-// six or more: bf16, top-k, top-p and both, one row of 128256 (7 parts) 21.6, 27.4, 22.7 / 26.5, 28.9,
-// 28.5; of 84000 (5) 21.7, 27.6, 22.4 / 20.8, 23.3, 23.0; 64 rows of 128256 (4) 30.7, 39.4, 32.2 / 30.6,
-// 32.8, 32.3.
+// eight or more: bf16, top-k, top-p and both, one row of 200000 (12 parts) 20.7, 28.5, 22.3 / 33.2, 35.7,
+// 35.3; of 128256 (7) 21.0, 27.5, 21.9 / 23.7, 26.4, 25.6; 16 such rows 23.2, 29.9, 25.5 / 24.3, 26.9, 26.4.
 int sample_parts(int rows, int V, int dtype) {
   const int tokens = (dtype == DKV_F32 ? 4 : 8) * 64;
   const int rows64 = (V + tokens - 1) / tokens;
@@ -1222,7 +1225,7 @@ int sample_parts(int rows, int V, int dtype) {
   int n = 256 / rows;
   if (n > SM_PARTS) n = SM_PARTS;
   if (n > rows64 / (2 * SM_WAVES)) n = rows64 / (2 * SM_WAVES);
-  return n < (dtype == DKV_F32 ? 2 : 6) ? 1 : n;
+  return n < (dtype == DKV_F32 ? 2 : 8) ? 1 : n;
 }
 
 template <int DT>

@@ -3,7 +3,8 @@
 The generators take the most probable token (the reference's benchmark decodes greedily,
 ``scripts/benchmark_throughput.py:17-30``; its models inherit transformers' ``generate`` with
 temperature, top-k, top-p and min-p). ``sample_tokens`` draws a token per row under these filters from
-a uniform number that the caller gives, so a draw can be repeated and costs one launch.
+a uniform number that the caller gives, so a draw can be repeated; it is one launch, or three where
+few rows of a large vocabulary are cut among workgroups.
 """
 
 from __future__ import annotations
@@ -43,8 +44,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     The first token is always kept. The result is the first token, in the vocabulary's order, up to
     which the kept mass exceeds u times all of it. ``temperature`` 0 (or below) takes the first
     token. A logit of -inf is never taken, NaN counts as -inf, +inf ones share the mass among
-    themselves, and a row with no logit above -inf gives -1. Masses are summed in 64-bit fixed
-    point, so a result depends on the row alone."""
+    themselves, and a row with no logit above -inf gives -1. Masses are sums in 64-bit fixed
+    point, so the same call gives the same tokens every time."""
     fast = _lib.tensor_calls()
     if fast is not None and out is None:
         dev = logits.get_device()
