@@ -16,6 +16,17 @@ namespace {
 
 constexpr int PG_DH = 128;
 
+// x / d for 0 <= x < 2^31, by a product: m = ceil(2^32 / d) gives the quotient or one more.
+struct Divisor {
+  uint32_t d, m;
+};
+Divisor divisor(int d) { return {(uint32_t)d, d > 1 ? (uint32_t)((0x100000000ULL + d - 1) / d) : 0u}; }
+__device__ __forceinline__ int quot(const Divisor& v, int x) {
+  uint32_t q = __umulhi((uint32_t)x, v.m);
+  q -= q * v.d > (uint32_t)x;
+  return v.d == 1 ? x : (int)q;
+}
+
 struct PagedPool {
   long long page_stride, head_stride;  // elements
   int num_pages, page_size, page_shift;
@@ -223,6 +234,7 @@ struct AttendParams {
   void* out;
   long long o_st, o_sh;
   int B, T, Hq, Hkv, hpg;
+  Divisor by_hpg, by_hkv;
   float scale_log2;  // softmax scale * log2(e)
   float* records;    // split records
   int* counters;     // arrival counters, zero between calls
@@ -284,6 +296,19 @@ constexpr int D_MIN_TILES = 16;             // least part
 constexpr float D_RESCALE = 11.5f;          // log2 units the running maximum may be exceeded by
 
 __device__ __forceinline__ int pg_wave_sum(int v) { return dkv_wave_sum_fast_i(v); }
+__device__ __forceinline__ int pg_wave_scan(int v) {  // inclusive, as dkv_wave_scan_fast
+  v += dkv_dpp_i32<0x111>(v);
+  v += dkv_dpp_i32<0x112>(v);
+  v += dkv_dpp_i32<0x114>(v);
+  v += dkv_dpp_i32<0x118>(v);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+__device__ __forceinline__ PagedRequest pg_lane(const PagedRequest& r, int l) {  // lane l's, for all
+  return {__builtin_amdgcn_readlane(r.row0, l), __builtin_amdgcn_readlane(r.n, l),
+          __builtin_amdgcn_readlane(r.len, l), __builtin_amdgcn_readlane(r.pos0, l)};
+}
 
 // Workgroup `wg` of `wgs`, of DW waves; `sRing`: DW * DSLOT * DSLOT_BYTES of LDS, `sLast` an int of it.
 template <int DT, int ODT, int DW>
@@ -356,24 +381,16 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     for (int j = 0; j < D_SPLIT_B / 64; ++j) {
       if (j >= used || b >= 0) continue;
       const int s = parts_of(t[j], inv) * p.Hkv;
-      int run = s;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(run, o, 64);
-        if (lane >= o) run += x;
-      }
+      const int run = pg_wave_scan(s);
       const unsigned long long hit = __ballot(wg < base + run);
       if (hit) {
         const int l = __ffsll((long long)hit) - 1;
         b = 64 * j + l;
-        first = base + __shfl(run - s, l, 64);
-        parts = __shfl(s, l, 64) / p.Hkv;
-        r.row0 = __shfl(rs[j].row0, l, 64);
-        r.n = __shfl(rs[j].n, l, 64);
-        r.len = __shfl(rs[j].len, l, 64);
-        r.pos0 = __shfl(rs[j].pos0, l, 64);
+        first = base + __builtin_amdgcn_readlane(run - s, l);
+        parts = quot(p.by_hkv, __builtin_amdgcn_readlane(s, l));
+        r = pg_lane(rs[j], l);
       } else {
-        base += __shfl(run, 63, 64);
+        base += __builtin_amdgcn_readlane(run, 63);
       }
     }
     b = __builtin_amdgcn_readfirstlane(b);
@@ -385,8 +402,8 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     part = rel % parts;
     first += kvh * parts;
   } else {
-    b = wg / p.Hkv;
-    kvh = wg % p.Hkv;
+    b = quot(p.by_hkv, wg);
+    kvh = wg - b * p.Hkv;
     r = paged_request(p.pool, p.q_start, p.lens, b, p.T);
   }
   r = uniform(r);
@@ -432,9 +449,9 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   // zero), dims 32c + 8g .. +8
   dkv_u32x4 bq[4];
   const bool has = n < rows;
-  const int qi = has ? n / p.hpg : 0;  // the row's new token
+  const int qi = has ? quot(p.by_hpg, n) : 0;  // the row's new token
   const uint16_t* qr = p.q + (long long)(r.row0 + qi) * p.q_st +
-                       (long long)(kvh * p.hpg + (has ? n % p.hpg : 0)) * p.q_sh;
+                       (long long)(kvh * p.hpg + (has ? n - qi * p.hpg : 0)) * p.q_sh;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const dkv_u32x4 v = *(const dkv_u32x4*)(qr + 32 * c + 8 * g);
@@ -581,8 +598,9 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     return A;
   };
   auto store = [&](int row, int d, float A, float L) {
-    const long long oi = (long long)(r.row0 + row / p.hpg) * p.o_st +
-                         (long long)(kvh * p.hpg + row % p.hpg) * p.o_sh + d;
+    const int i = quot(p.by_hpg, row);
+    const long long oi = (long long)(r.row0 + i) * p.o_st +
+                         (long long)((kvh - i) * p.hpg + row) * p.o_sh + d;
     dkv_store_f32<ODT>(p.out, oi, L == 0.f ? 0.f : A / L);  // (a NaN among the weights stays)
   };
   if (parts == 1) {
@@ -691,7 +709,9 @@ constexpr float C_RESCALE = 8.f;            // log2 units
 struct ChunkParams {
   AttendParams a;
   float* records;
-  int bq, splits, few_rows;  // rows of a workgroup; key ranges; rows up to which the other kernel works
+  // rows of a workgroup and their log2; key ranges; rows up to which the other kernel works
+  int bq, bq_shift, splits, few_rows;
+  Divisor by_splits;
 };
 
 // The work item of a workgroup: row tile `rt` of request b. Items are counted request by request,
@@ -708,48 +728,54 @@ __device__ __forceinline__ ChunkItem chunk_item(const ChunkParams& p, int item, 
     PagedRequest r = {0, 0, 0, 0};
     if (b0 + lane < a.B) {
       r = paged_request(a.pool, a.q_start, a.lens, b0 + lane, a.T);
-      const long long rows = (long long)r.n * a.hpg;
-      t = r.n > 0 && rows > p.few_rows ? (int)((rows + p.bq - 1) / p.bq) : 0;
+      const int rows = r.n * a.hpg;
+      t = r.n > 0 && rows > p.few_rows ? (rows + p.bq - 1) >> p.bq_shift : 0;
     }
-    int run = t;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(run, o, 64);
-      if (lane >= o) run += x;
-    }
+    const int run = pg_wave_scan(t);
     const unsigned long long hit = __ballot(item < base + run);
     if (hit) {
       const int l = __ffsll((long long)hit) - 1;
       ChunkItem it;
-      it.b = __builtin_amdgcn_readfirstlane(b0 + l);
-      it.rt = __builtin_amdgcn_readfirstlane(base + __shfl(run, l, 64) - 1 - item);
-      it.r.row0 = __shfl(r.row0, l, 64);
-      it.r.n = __shfl(r.n, l, 64);
-      it.r.len = __shfl(r.len, l, 64);
-      it.r.pos0 = __shfl(r.pos0, l, 64);
-      it.r = uniform(it.r);
+      it.b = b0 + l;
+      it.rt = base + __builtin_amdgcn_readlane(run, l) - 1 - item;
+      it.r = pg_lane(r, l);
       return it;
     }
-    base += __shfl(run, 63, 64);
+    base += __builtin_amdgcn_readlane(run, 63);
   }
   return ChunkItem{-1, 0, {0, 0, 0, 0}};
 }
 
-// Four neighbouring values of the output, as one store where its rows allow it.
-template <int ODT>
+// Four neighbouring values of the output, WIDE as one store.
+template <int ODT, bool WIDE>
 __device__ __forceinline__ void store4(const AttendParams& p, long long at, dkv_f32x4 v) {
-  if (!p.out_wide) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  if constexpr (!WIDE) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) dkv_store_f32<ODT>(p.out, at + u, v[u]);
   } else if constexpr (ODT == DKV_F32) {
     *(dkv_f32x4*)((float*)p.out + at) = v;
   } else if constexpr (ODT == DKV_BF16) {
-    *(dkv_u32x2*)((uint16_t*)p.out + at) =
-        dkv_u32x2{dkv_f32_to_bf16_bits(v[0]) | (dkv_f32_to_bf16_bits(v[1]) << 16),
-                  dkv_f32_to_bf16_bits(v[2]) | (dkv_f32_to_bf16_bits(v[3]) << 16)};
+    *(dkv_u32x2*)((uint16_t*)p.out + at) = dkv_u32x2{
+        __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[0], v[1]}, dkv_bf16x2)),
+        __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2], v[3]}, dkv_bf16x2))};
   } else {
+    // (the quotient in fp32 first, as the fp32 output has it: not one instruction to fp16)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) asm("" : "+v"(v[u]));
     *(dkv_u32x2*)((uint16_t*)p.out + at) =
         dkv_u32x2{dkv_pack_f16x2(v[0], v[1]), dkv_pack_f16x2(v[2], v[3])};
+  }
+}
+// f(db) at dims 16 db + 0 .. 3 from `at` on, by wide stores where the output's rows allow it
+template <int ODT, class F>
+__device__ __forceinline__ void store_dims(const AttendParams& p, long long at, F&& f) {
+  if (p.out_wide) {
+#pragma unroll
+    for (int db = 0; db < 8; ++db) store4<ODT, true>(p, at + 16 * db, f(db));
+  } else {
+#pragma unroll
+    for (int db = 0; db < 8; ++db) store4<ODT, false>(p, at + 16 * db, f(db));
   }
 }
 
@@ -815,10 +841,11 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const int n = lane & 15, g = lane >> 4;
   // the KV head runs fastest: workgroups go to the 8 XCDs in turn, so that a head's keys and values
   // stay in one L2 (for 8 heads, or a multiple)
-  const int kvh = __builtin_amdgcn_readfirstlane(wg % p.Hkv);
-  const int rest = wg / p.Hkv;
-  const int split = rest % c.splits;
-  const ChunkItem it = chunk_item(c, rest / c.splits, lane);
+  const int rest = __builtin_amdgcn_readfirstlane(quot(p.by_hkv, wg));
+  const int kvh = wg - rest * p.Hkv;
+  const int item = __builtin_amdgcn_readfirstlane(quot(c.by_splits, rest));
+  const int split = rest - item * c.splits;
+  const ChunkItem it = chunk_item(c, item, lane);
   const int b = __builtin_amdgcn_readfirstlane(it.b);
   if (b < 0) return;
   const PagedRequest r = uniform(it.r);
@@ -832,7 +859,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int R = min(wq0 + 16 * qb + n, rows - 1);
-    const int i = R / p.hpg, h = R - i * p.hpg;
+    const int i = quot(p.by_hpg, R), h = R - i * p.hpg;
     const uint16_t* qp = p.q + (long long)(r.row0 + i) * p.q_st +
                          (long long)(kvh * p.hpg + h) * p.q_sh + 8 * g;
 #pragma unroll
@@ -841,11 +868,11 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   }
   // keys up to the last row's; the wave's first and last row's limits
   const int k_end = __builtin_amdgcn_readfirstlane(
-      max(0, min(r.len, r.pos0 + (min(q0 + BQ, rows) - 1) / p.hpg + 1)));
-  const int w_first = r.pos0 + min(wq0, rows - 1) / p.hpg;
-  const int w_end = wq0 < rows ? r.pos0 + (min(wq0 + QW, rows) - 1) / p.hpg + 1 : 0;
+      max(0, min(r.len, r.pos0 + quot(p.by_hpg, min(q0 + BQ, rows) - 1) + 1)));
+  const int w_first = r.pos0 + quot(p.by_hpg, min(wq0, rows - 1));
+  const int w_end = wq0 < rows ? r.pos0 + quot(p.by_hpg, min(wq0 + QW, rows) - 1) + 1 : 0;
   const int all_tiles = (k_end + CK - 1) / CK;
-  const int per = (all_tiles + c.splits - 1) / c.splits;
+  const int per = quot(c.by_splits, all_tiles + c.splits - 1);
   const int t0 = min(all_tiles, split * per), n_tiles = min(all_tiles, t0 + per);
 
   // pages of the 64 blocks of 16 keys from tile tb on (16 tiles); the next 64 fetched ahead
@@ -1040,19 +1067,20 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
 
   // acc rows are dims, columns rows of the request: lane (row n, g) holds dims 16db + 4g + u. A
   // range's record: acc[BQ][128], then m and l of each row.
-  float* rec = c.records + ((long long)(rest / c.splits * p.Hkv + kvh) * c.splits + split) * BQ *
+  float* rec = c.records + ((long long)(item * p.Hkv + kvh) * c.splits + split) * BQ *
                                (PG_DH + 2);
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const float l = sum[qb][0];
     const int R = wq0 + 16 * qb + n;
-    const int i = R / p.hpg, h = R - i * p.hpg;
-    // the largest magnitude, infinite or NaN where a value is (a sum of products by 0)
-    float odd = l * 0.f;
+    const int i = quot(p.by_hpg, R), h = R - i * p.hpg;
+    // 0, or NaN where a value is infinite or NaN
+    float od[4] = {l * 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int db = 0; db < 8; ++db)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) odd = fmaf(acc[qb][db][u], 0.f, odd);
+      for (int u = 0; u < 4; ++u) od[u] = fmaf(acc[qb][db][u], 0.f, od[u]);
+    const float odd = (od[0] + od[1]) + (od[2] + od[3]);
     // (Or a sum below that of the largest score's weight alone, which is at least 1 as rounded: scores
     // past 2^24, whose product with the scale and the rounded maximum differ by more than their sum.)
     const bool low = l < 0.5f && min(limit[qb] + 1, n_tiles * CK) > t0 * CK;
@@ -1064,9 +1092,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         const float inv = l > 0.f ? 1.f / l : 0.f;
         const long long ob = (long long)(r.row0 + i) * p.o_st +
                              (long long)(kvh * p.hpg + h) * p.o_sh;
-#pragma unroll
-        for (int db = 0; db < 8; ++db)
-          store4<ODT>(p, ob + 16 * db + 4 * g, acc[qb][db] * inv);
+        store_dims<ODT>(p, ob + 4 * g, [&](int db) { return acc[qb][db] * inv; });
       }
     } else if (good) {
       const int x = QW * wave + 16 * qb + n;
@@ -1078,7 +1104,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     while (bad) {  // key by key
       const int x = __ffsll((long long)bad) - 1;
       bad &= bad - 1;
-      const int Rx = wq0 + 16 * qb + x, ix = Rx / p.hpg, hx = Rx - ix * p.hpg;
+      const int Rx = wq0 + 16 * qb + x, ix = quot(p.by_hpg, Rx), hx = Rx - ix * p.hpg;
       const uint16_t* qx = p.q + (long long)(r.row0 + ix) * p.q_st +
                            (long long)(kvh * p.hpg + hx) * p.q_sh;
       float mx, lx, o0, o1;
@@ -1154,11 +1180,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(ChunkParams c) {
     for (int q = 0; q < 4; ++q) a[q] = a[q] * so + x[q] * sn;
   }
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-  const int i = R / p.hpg, h = R - i * p.hpg;
+  const int i = quot(p.by_hpg, R), h = R - i * p.hpg;
   const long long ob = (long long)(r.row0 + i) * p.o_st +
                        (long long)(kvh * p.hpg + h) * p.o_sh + d0;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) store4<ODT>(p, ob + 32 * q, a[q] * inv);
+  for (int q = 0; q < 4; ++q) {
+    if (p.out_wide)
+      store4<ODT, true>(p, ob + 32 * q, a[q] * inv);
+    else
+      store4<ODT, false>(p, ob + 32 * q, a[q] * inv);
+  }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -1409,6 +1440,8 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.hpg = Hq / Hkv;
+  p.by_hpg = divisor(p.hpg);
+  p.by_hkv = divisor(Hkv);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.counters = reinterpret_cast<int*>(workspace);
   p.records = workspace ? workspace + D_COUNTERS : nullptr;
@@ -1418,7 +1451,9 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
                  (uintptr_t)(4 * dkv_elt_size(out_dtype) - 1));
   c.records = workspace ? workspace + D_COUNTERS + plan.many_at : nullptr;
   c.bq = plan.bq;
+  c.bq_shift = plan.many ? __builtin_ctz((unsigned)plan.bq) : 0;
   c.splits = plan.splits;
+  c.by_splits = divisor(plan.many ? plan.splits : 1);
   c.few_rows = plan.few ? DROWS : 0;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DKV_BF16) {
