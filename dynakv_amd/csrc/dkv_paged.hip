@@ -853,19 +853,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const int q0 = __builtin_amdgcn_readfirstlane(it.rt) * BQ;
   const int wq0 = q0 + QW * wave;  // the wave's first row
 
-  // this lane's rows (operand columns): token and last key
-  dkv_u32x4 qop[QB][4];
-  int limit[QB];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int R = min(wq0 + 16 * qb + n, rows - 1);
-    const int i = quot(p.by_hpg, R), h = R - i * p.hpg;
-    const uint16_t* qp = p.q + (long long)(r.row0 + i) * p.q_st +
-                         (long long)(kvh * p.hpg + h) * p.q_sh + 8 * g;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) qop[qb][s] = *(const dkv_u32x4*)(qp + 32 * s);
-    limit[qb] = min(r.pos0 + i, r.len - 1);
-  }
   // keys up to the last row's; the wave's first and last row's limits
   const int k_end = __builtin_amdgcn_readfirstlane(
       max(0, min(r.len, r.pos0 + quot(p.by_hpg, min(q0 + BQ, rows) - 1) + 1)));
@@ -882,8 +869,21 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     return key < k_end ? paged_page(p.pool, b, key) : -1;
   };
   int ids_base = t0;
-  ids = fetch_ids(t0);
+  ids = fetch_ids(t0);  // (before the queries, which the first tiles' loads need not wait for)
   if (t0 + 16 < n_tiles) ids_next = fetch_ids(t0 + 16);
+  // this lane's rows (operand columns): token and last key
+  dkv_u32x4 qop[QB][4];
+  int limit[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int R = min(wq0 + 16 * qb + n, rows - 1);
+    const int i = quot(p.by_hpg, R), h = R - i * p.hpg;
+    const uint16_t* qp = p.q + (long long)(r.row0 + i) * p.q_st +
+                         (long long)(kvh * p.hpg + h) * p.q_sh + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qop[qb][s] = *(const dkv_u32x4*)(qp + 32 * s);
+    limit[qb] = min(r.pos0 + i, r.len - 1);
+  }
   // blocks with keys but no page
   auto absent_of = [&](int tb) {
     return __ballot(ids < 0 && (tb * 4 + lane) * 16 < k_end);
