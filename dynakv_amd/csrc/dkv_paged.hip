@@ -944,6 +944,12 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       (4 * g + (n >> 2)) * 256 + 16 * (((n & 3) >> 1) ^ (4 * g + (n >> 2))) + 8 * (n & 1);
 
   if (t0 < n_tiles) issue(t0, __builtin_amdgcn_readlane(ids, blk));
+  // settled here, not inside the loop, where the compiler's waits for them would be waits for the next
+  // tile, which it does not know of
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(qop[qb][s]));
   for (int t = t0; t < n_tiles; ++t) {
     pg_wait_vm();
     __syncthreads();  // tile t is in LDS for every wave; tile t - 1's buffer is free
