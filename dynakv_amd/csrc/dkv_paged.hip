@@ -242,22 +242,38 @@ struct AttendParams {
   int out_wide;      // output rows begin at multiples of four values, aligned as such
 };
 
-// 16 bytes at byte offset `off` of a buffer resource into LDS at M0 + 16 * lane (inline assembly so
-// that the compiler neither moves LDS accesses across it nor waits for it before later LDS reads;
-// the kernels wait for these loads themselves).
+// N loads of 16 bytes a lane, at byte offset off[i] + 1024 i of a buffer resource, into LDS at lds_base +
+// 1024 i + 16 * lane (an instruction's offset counts on both sides, so that M0 is set once; one block of
+// inline assembly, so that the compiler does not change M0 in between, neither moves LDS accesses across
+// it nor waits for it before later LDS reads; the kernels wait for these loads themselves).
 // ONCE: data that no other workgroup reads, passed by the caches (two requests of 65533 tokens, single
 // new ones: 89 us, 6.0 TB/s, against 101 us without; 16 of 8192: 88 against 101).
-template <bool ONCE>
-__device__ __forceinline__ void pg_lds_load16(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_base,
-                                              uint32_t off) {
-  if constexpr (ONCE)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
-                 ::"s"(lds_base), "v"(off), "s"(rsrc)
-                 : "memory", "m0");
+template <bool ONCE, int N>
+__device__ __forceinline__ void pg_lds_loads(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_base,
+                                             const uint32_t (&off)[N]) {
+  static_assert(N == 2 || N == 4, "");
+  if constexpr (ONCE && N == 4)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %5, 0 offen nt lds\n\t"
+        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 nt lds\n\t"
+        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 nt lds\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 nt lds" ::"s"(lds_base),
+        "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(rsrc)
+        : "memory", "m0");
+  else if constexpr (N == 4)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 lds\n\t"
+        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 lds\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 lds" ::"s"(lds_base),
+        "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(rsrc)
+        : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 ::"s"(lds_base), "v"(off), "s"(rsrc)
-                 : "memory", "m0");
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds" ::"s"(lds_base),
+        "v"(off[0]), "v"(off[1]), "s"(rsrc)
+        : "memory", "m0");
 }
 __device__ __forceinline__ void pg_wait_vm() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 typedef __attribute__((address_space(3))) dkv_i16x4 pg_lds_i16x4;
@@ -420,7 +436,7 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 4 * i + (lane >> 4);
-    piece_off[i] = (uint32_t)(t * 256 + 16 * ((lane & 15) ^ t));
+    piece_off[i] = (uint32_t)((lane >> 4) * 256 + 16 * ((lane & 15) ^ t));
   }
   int ids = -1;  // lane l: the page of the wave's tile l of the 64 being issued
   auto issue = [&](int j) {  // the tile's loads; returns its page (scalar)
@@ -437,10 +453,8 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     const __amdgpu_buffer_rsrc_t rk = dkv_make_rsrc(p.k + at, bytes);
     const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc(p.v + at, bytes);
     const uint32_t slot = dkv_lds_addr(ring + (j % DSLOT) * DSLOT_BYTES);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pg_lds_load16<true>(rk, slot + 1024 * i, piece_off[i]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pg_lds_load16<true>(rv, slot + DTILE_BYTES + 1024 * i, piece_off[i]);
+    pg_lds_loads<true>(rk, slot, piece_off);
+    pg_lds_loads<true>(rv, slot + DTILE_BYTES, piece_off);
     return page;
   };
   int page_next = issue(0);
@@ -898,23 +912,23 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
 #pragma unroll
   for (int i = 0; i < LW; ++i) {
     const int kk = 4 * i + (lane >> 4);
-    voff[i] = (uint32_t)(kk * 256 + 16 * ((lane & 15) ^ ((sub + kk) & 15)));
+    voff[i] = (uint32_t)((lane >> 4) * 256 + 16 * ((lane & 15) ^ ((sub + kk) & 15)));
   }
-  auto issue = [&](int t, int page) {
-    const int key = t * CK + blk * 16 + sub;
+  const uint16_t* k_head = p.k + (long long)kvh * p.pool.head_stride;
+  const uint16_t* v_head = p.v + (long long)kvh * p.pool.head_stride;
+  const int key_in_tile = blk * 16 + sub, slot_mask = p.pool.page_size - 1;
+  auto issue = [&](int t, int page) {  // (scalar work, a wave's by itself: every instruction counts)
+    const int key = t * CK + key_in_tile;
     const long long at = (long long)max(page, 0) * p.pool.page_stride +
-                         (long long)kvh * p.pool.head_stride +
-                         (long long)(key & (p.pool.page_size - 1)) * PG_DH;
-    const int cnt = __builtin_amdgcn_readfirstlane(
-        page < 0 ? 0 : min(max(k_end - key, 0), CK / NW));  // (a vector instruction clamps)
-    const __amdgpu_buffer_rsrc_t rk = dkv_make_rsrc(p.k + at, (uint32_t)cnt * (PG_DH * 2));
-    const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc(p.v + at, (uint32_t)cnt * (PG_DH * 2));
-    const uint32_t dk = dkv_lds_addr(sK(t & 1)) + CK / NW * wave * 256;
-    const uint32_t dv = dkv_lds_addr(sV(t & 1)) + CK / NW * wave * 256;
-#pragma unroll
-    for (int i = 0; i < LW; ++i) pg_lds_load16<false>(rk, dk + 1024 * i, voff[i]);
-#pragma unroll
-    for (int i = 0; i < LW; ++i) pg_lds_load16<false>(rv, dv + 1024 * i, voff[i]);
+                         (long long)((key & slot_mask) * PG_DH);
+    int keys;  // as scalar instructions: the compiler would clamp in a vector register
+    asm("s_max_i32 %0, %1, 0" : "=s"(keys) : "s"(k_end - key) : "scc");
+    asm("s_min_i32 %0, %1, %2" : "=s"(keys) : "s"(keys), "n"(CK / NW) : "scc");
+    const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys * (PG_DH * 2);
+    pg_lds_loads<false>(dkv_make_rsrc(k_head + at, bytes),
+                        dkv_lds_addr(sK(t & 1)) + CK / NW * wave * 256, voff);
+    pg_lds_loads<false>(dkv_make_rsrc(v_head + at, bytes),
+                        dkv_lds_addr(sV(t & 1)) + CK / NW * wave * 256, voff);
   };
 
   dkv_f32x4 acc[QB][8];
