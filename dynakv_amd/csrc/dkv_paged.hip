@@ -712,10 +712,11 @@ __global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
 //
 // Bound by the SIMDs' issue slots: per wave and tile (QB = 2) 66 products of 16 cycles beside ~190
 // vector instructions, 32 of them exponentials of 16 cycles; two waves a SIMD fill one's products with
-// the other's vector work in part. Four prompts of 2048 tokens (32 and 8 heads): 166 us, 0.83 PFLOP/s,
-// one of 8192: 513 us, 1.07 PFLOP/s, where a large library product reaches 1.23. (Sums by additions and
-// equal priorities: 169 and 527.) A deeper ring (four tiles of 64 or 32 keys) gains nothing: 1x4, 512
-// tokens at 1024: 23.0 us with two tiles of 64 or four, 27.2 with four of 32.
+// the other's vector work in part. Four prompts of 2048 tokens (32 and 8 heads): 159 us, 0.86 PFLOP/s
+// (a workgroup's start and end are as long as three of its 17 tiles), one of 8192: 500 us, 1.10 PFLOP/s,
+// where a large library product reaches 1.23. (Sums by additions and equal priorities: 2% more.) Key
+// tiles of 32 and three waves a SIMD: the same at 8192, 10% slower on chunks. Deeper rings of tiles, the
+// scores of the next tile among this one's softmax, K operands read before the next tile's loads: nothing.
 constexpr int CK = 64;                      // keys per tile
 constexpr int CTILE_BYTES = CK * PG_DH * 2;
 constexpr float C_RESCALE = 8.f;            // log2 units
@@ -798,7 +799,8 @@ __device__ __forceinline__ float pg_max4(float x) {  // over lanes n, n + 16, n 
 }
 
 // One row over keys k0 .. k1 - 1, by a wave, key by key: for rows whose values came out as infinity or
-// NaN, or whose scores are too large for one fused multiplication and subtraction. A product of matrices takes a masked key's value times 0, which is NaN for an infinite one; here
+// NaN, or whose scores are too large for one fused multiplication and subtraction. A product of
+// matrices takes a masked key's value times 0, which is NaN for an infinite one; here
 // a masked key is not touched. Lane l returns dims 2l, 2l + 1.
 template <int DT>
 __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, int kvh,
@@ -1306,14 +1308,15 @@ struct AttendPlan {
 // tiles of the longest request. us on MI355X, bf16, 32 query and 8 KV heads; shape: row blocks x
 // waves / key ranges (workgroups):
 //  * more than 1024 of 128 rows: 2x4, each key operand read from LDS serves two products. Four
-//    2048-token prompts 169 2x4/1, 178 1x8/1, 213 1x4/1.
+//    2048-token prompts 156 2x4/1, 167 1x8/1, 188 1x4/1.
 //  * up to 256 of 128 rows and long keys: ranges that fill the chip once, at least 24 tiles each.
-//    512 tokens at 8192: 88.8 2x4/4 (512), 102 2x4/3, 105 1x4/2, 173 1x4/1. 846 tokens of two
-//    requests at up to 6001: 103 2x4/2, 109 2x4/4, 125 1x4/1.
+//    512 tokens at 8192: 77.7 2x4/4 (512), 87 2x4/3, 89.4 1x4/2, 125 1x4/1. 846 tokens of two
+//    requests at up to 6001: 87.3 2x4/2, 89.4 2x4/4, 101 1x4/1.
 //  * so few rows that 64-row tiles, too, leave half the chip idle: those, ranges of 8 tiles or more.
-//    64 tokens at 32768: 73 1x4/16, 82 2x4/16. 200 at 2000: 29.7 1x4/4, 31.5 1x4/2, 35.0 1x4/5 (520).
-//  * otherwise one range: above 256 of 128 rows 1x8 (eight 300-token prompts 25.6, against 27.1 1x4,
-//    28.3 2x4), else 1x4 (512 tokens at 1024: 22.6, against 27.0 1x8 and 36 2x4/2: a range more
+//    64 tokens at 32768: 61.9 1x4/16, 65.1 2x4/16. 200 at 2000: 26.7 1x4/4, 27.5 1x4/2, 31.7 1x4/5
+//    (520).
+//  * otherwise one range: above 256 of 128 rows 1x8 (eight 300-token prompts 22.7, against 23.5 1x4,
+//    25.5 2x4), else 1x4 (512 tokens at 1024: 20.1, against 24.4 1x8 and 29 2x4/2: a range more
 //    costs its records, 66 KB a workgroup, written and read).
 AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, int max_len) {
   AttendPlan a = {};
@@ -1347,7 +1350,8 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
     const long long wg128 = full(128), wg64 = full(64);
     auto ranges = [&](long long wgs, long long least) {
       // (beside the other kind, about half the chip: 12 single tokens and 512 at 2048, 16 and 4
-      // heads: 34 us with two ranges, 42 with one or three, 49 in a launch of its own)
+      // heads: 30 us with two ranges; 42 with one or three and 49 in a launch of its own, where two
+      // took 34)
       const long long n = a.few ? (256 + wgs / 2) / wgs : 512 / wgs, most = (tiles + least / 2) / least;
       return (int)(n < most ? n : most);
     };
