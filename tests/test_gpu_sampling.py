@@ -335,3 +335,22 @@ def test_same_with_and_without_the_tensor_module(dev, dtype, monkeypatch):
     monkeypatch.setattr(_lib, "_tensor_calls", None)
     for a, b in zip(run(), fast):
         assert a.dtype == b.dtype == torch.int64 and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_borders_among_many_equal_logits(dev, dtype):
+    """Thousands of equal logits at the border beside some next to them, of both signs: the search by
+    digits, for top-k, top-p and both."""
+    print(f"[gpu] sample many equal {dtype}", flush=True)
+    g = torch.Generator().manual_seed(71)
+    for V in (9001, 30000):
+        x = torch.randn(5, V, generator=g) * 2.5
+        x[torch.rand(5, V, generator=g) < 0.9] = 0.0
+        x[1, ::13], x[2, ::17], x[3] = 1e-6, -1e-6, x[3] - 7.75
+        x[4, ::3] = -0.0
+        x = x.to(DT[dtype]).to(dev)
+        u = torch.rand(5, generator=g).to(dev)
+        for kw in (dict(top_p=0.9), dict(top_p=0.5), dict(top_k=V // 2), dict(top_k=V - 50),
+                   dict(top_k=V // 2, top_p=0.8), dict(temperature=0.3, top_p=0.99, top_k=V // 3)):
+            _check(x, u, **kw)
