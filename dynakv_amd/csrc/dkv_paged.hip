@@ -223,6 +223,16 @@ __global__ __launch_bounds__(64 * AP_WAVES) void paged_append_kernel(AppendParam
 // ---------------------------------------------------------------------------------------
 // A running maximum of no keys: finite, so that exp2(-inf - it) is 0, and below every other score.
 constexpr float PG_NO_MAX = -3.4028234663852886e38f;
+// Weights are powers of two measured from a row's reference (log2 units), which is PG_BIAS below a running
+// maximum and raised when a score exceeds that by more than the kernel's rescale step. fp16's step is
+// 2^-24 for all numbers below 2^-14, so its weights are kept as large as it can hold: the largest of a row at
+// 2^12 to 2^15, so that the others have all their bits down to 2^-26 of it (18 nats) and some to 2^-36.
+// With the largest at 1 to 2^8, 4000 keys 18 nats below one whose value is 0 came out up to 11% off in
+// chunks, 1.7% for single tokens; with this 2e-5 and 2e-6, in the same time. The power cancels in the
+// division; maxima in records are references. bf16 has fp32's range.
+template <int DT>
+constexpr float PG_BIAS = DT == DKV_F16 ? 12.f : 0.f;
+constexpr float PG_F16_RESCALE = 3.f;  // 2^(12 + 3) and a rounding below fp16's 65504
 struct AttendParams {
   const uint16_t* q;
   long long q_st, q_sh;
@@ -309,7 +319,8 @@ constexpr int D_COUNTERS = 16384;           // leading workspace ints
 constexpr int D_SPLIT_B = 256;              // requests a wave can hold the lengths of (4 a lane)
 constexpr int D_WGS = 256;                  // workgroups of 8 waves: one per CU
 constexpr int D_MIN_TILES = 16;             // least part
-constexpr float D_RESCALE = 11.5f;          // log2 units the running maximum may be exceeded by
+template <int DT>                           // log2 units the running maximum may be exceeded by
+constexpr float D_RESCALE = DT == DKV_F16 ? PG_F16_RESCALE : 11.5f;
 
 __device__ __forceinline__ int pg_wave_sum(int v) { return dkv_wave_sum_fast_i(v); }
 __device__ __forceinline__ int pg_wave_scan(int v) {  // inclusive, as dkv_wave_scan_fast
@@ -479,7 +490,7 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   dkv_f32x4 acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = PG_NO_MAX, l_run = 0.f;  // log2 units
+  float m_run = PG_NO_MAX, l_run = 0.f;  // the row's reference (log2 units) and sum
 
   for (int j = 0; j < n_iter; ++j) {
     pg_wait_vm();
@@ -502,8 +513,8 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     float tmax = dkv_max3(dkv_max3(z[0], z[1], z[2]), z[3], z[3]);
     tmax = dkv_lane_max32(tmax);
     tmax = dkv_lane_max16(tmax);
-    if (__ballot(tmax > m_run + D_RESCALE)) {
-      const float m_new = fmaxf(m_run, tmax);
+    if (__ballot(tmax > m_run + (PG_BIAS<DT> + D_RESCALE<DT>))) {
+      const float m_new = fmaxf(m_run, tmax - PG_BIAS<DT>);
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       l_run *= alpha;
       m_run = m_new;
@@ -704,11 +715,12 @@ __global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
 // in a bank); a tile is four blocks of 16 keys, each within one page, and a wave loads one of them
 // (NW = 8: half of one) through a resource that ends with the request's keys. S^T = K Q^T on
 // 16x16x32 MFMA (a lane then holds one row's scores for 16 keys); softmax in fp32, the running
-// maximum raised only when a tile's exceeds it by more than 2^8; P V on 16x16x32 MFMA with the
-// weights rounded once to the cache's type and summed as rounded: a weight is off by at most half a
-// step, as the output is by its own rounding, and as the errors are of either sign, together they
-// come to 1.25 to 1.4 times the output's alone (measured against 64 bits; a second product with what
-// the rounding left would take half as many products again, which are the prompts' bound).
+// maximum raised only when a tile's exceeds it by more than 2^8 (fp16: 2^3); P V on 16x16x32 MFMA with
+// the weights rounded once to the cache's type and summed as rounded: a weight is off by at most half a
+// step (fp16: or 2^-37 of the row's largest, above), as the output is by its own rounding, and as the
+// errors are of either sign, together they come to 1.25 to 1.4 times the output's alone (normal scores,
+// measured against 64 bits; a second product with what the rounding left would take half as many products
+// again, which are the prompts' bound).
 //
 // Bound by the SIMDs' issue slots: per wave and tile (QB = 2) 66 products of 16 cycles beside ~190
 // vector instructions, 32 of them exponentials of 16 cycles; two waves a SIMD fill one's products with
@@ -719,7 +731,8 @@ __global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
 // scores of the next tile among this one's softmax, K operands read before the next tile's loads: nothing.
 constexpr int CK = 64;                      // keys per tile
 constexpr int CTILE_BYTES = CK * PG_DH * 2;
-constexpr float C_RESCALE = 8.f;            // log2 units
+template <int DT>                           // log2 units the running maximum may be exceeded by
+constexpr float C_RESCALE = DT == DKV_F16 ? PG_F16_RESCALE : 8.f;
 
 struct ChunkParams {
   AttendParams a;
@@ -938,8 +951,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[qb][i] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
-  // running maxima (log2 units), and the sums of the weights as one more row of P V: a product with
-  // ones, of the weights as they were rounded (every element holds it)
+  // the rows' references (log2 units), and the sums of the weights as one more row of P V: a product
+  // with ones, of the weights as they were rounded (every element holds it)
   float m_run[QB];
   dkv_f32x4 sum[QB];
   constexpr uint32_t one2 = DT == DKV_BF16 ? 0x3f803f80u : 0x3c003c00u;
@@ -1031,10 +1044,11 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
                          z[qb][kb][3]);
       tmax[qb] = pg_max4(dkv_max3(dkv_max3(m[0], m[1], m[2]), m[3], m[3])) * p.scale_log2;
     }
-    if (__ballot(tmax[0] > m_run[0] + C_RESCALE || tmax[QB - 1] > m_run[QB - 1] + C_RESCALE)) {
+    constexpr float RAISE = PG_BIAS<DT> + C_RESCALE<DT>;
+    if (__ballot(tmax[0] > m_run[0] + RAISE || tmax[QB - 1] > m_run[QB - 1] + RAISE)) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        const float m_new = dkv_max2(m_run[qb], tmax[qb]);
+        const float m_new = dkv_max2(m_run[qb], tmax[qb] - PG_BIAS<DT>);
         const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
         m_run[qb] = m_new;
 #pragma unroll
@@ -1103,9 +1117,11 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
 #pragma unroll
       for (int u = 0; u < 4; ++u) od[u] = fmaf(acc[qb][db][u], 0.f, od[u]);
     const float odd = (od[0] + od[1]) + (od[2] + od[3]);
-    // (Or a sum below that of the largest score's weight alone, which is at least 1 as rounded: scores
-    // past 2^24, whose product with the scale and the rounded maximum differ by more than their sum.)
-    const bool low = l < 0.5f && min(limit[qb] + 1, n_tiles * CK) > t0 * CK;
+    // (Or a sum below that of the largest score's weight alone, which is at least 2^PG_BIAS as rounded:
+    // scores past 2^24, whose product with the scale and the rounded maximum differ by more than their sum.)
+    constexpr float LOW = DT == DKV_F16 ? 2048.f : 0.5f;  // half of it
+    static_assert(PG_BIAS<DKV_F16> == 12.f && PG_BIAS<DKV_BF16> == 0.f, "");
+    const bool low = l < LOW && min(limit[qb] + 1, n_tiles * CK) > t0 * CK;
     unsigned long long bad = __ballot(R < rows && (!(odd == 0.f) || low));
     bad = (bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xffffull;  // by row
     const bool good = R < rows && !((bad >> n) & 1);

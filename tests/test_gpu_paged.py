@@ -810,3 +810,35 @@ def test_same_with_and_without_the_tensor_module(dev, dtype, monkeypatch):
         for a, b in zip(run(), fast):
             assert torch.equal(a, b)
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [14, 16, 18])
+@pytest.mark.parametrize("new,lens", [([1, 1], [4000, 9001]), ([3], [4000]), ([40], [4000]),
+                                      ([300, 1], [4000, 700]), ([70], [70])])
+def test_fp16_weights_far_below_the_largest(dev, new, lens, gap):
+    """A first key ``gap`` nats above all others, whose value is 0: the output is the others', whose
+    weights are 2^-20 to 2^-26 of the largest. An fp16 weight's step is 2^-24 below 2^-14, so a row's
+    largest weight is kept at 2^12 or more: a weight is off by at most 2^-25 of 2^12, or by its own half
+    step, which ``_attend_reference`` counts."""
+    print(f"[gpu] paged attention far below {new} {gap}", flush=True)
+    s = Step(dev, new, lens, hkv=2, seed=61, dtype=FP)
+    q = s.rand(s.T, 8, DH, scale=0.3)
+    q[..., 0] = 8.0
+    for b, n in enumerate(lens):
+        ids = s.table[b, :-(-n // 16)].tolist()
+        s.k[ids, :, :, 0] = torch.where(s.k[ids, :, :, 0].isnan(), s.k[ids, :, :, 0], 0.0)
+        s.v[ids] += 0.5
+        s.k[ids[0], :, 0] = 0.0
+        s.k[ids[0], :, 0, 0] = gap * math.sqrt(DH) / 8.0
+        s.v[ids[0], :, 0] = 0.0
+    want, tol = _attend_reference(s, q)
+    for b, (m, n) in enumerate(zip(new, lens)):  # the largest weight is at most 1
+        for h in range(8):
+            size = s.tokens(s.v, b, h // 4).abs().sum(0)
+            tol[s.starts[b]:s.starts[b] + m, h] += 2.0**-37 * size
+    got = paged_attention(q, s.k, s.v, s.batch, out_dtype=torch.float32)
+    err = (got.double() - want).abs()
+    print(f"[gpu]   err/tol {float((err / (tol + 1e-30)).max()):.3f}", flush=True)
+    assert bool((err <= tol + 1e-30).all())
+    assert torch.equal(paged_attention(q, s.k, s.v, s.batch), got.to(FP))
