@@ -12,6 +12,8 @@
 #include "dkv_common.h"
 #include "dkv_mfma_ops.h"
 
+#include <mutex>
+
 namespace {
 
 constexpr int PG_DH = 128;
@@ -1393,9 +1395,19 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
   return a;
 }
 
+// The lock of a workspace, under which every call that has one makes its launches: of two, the second
+// reads what the first left, and threads may make calls on one stream, in whose workspace they follow
+// each other.
+std::mutex& launch_lock(const void* workspace) {
+  static std::mutex locks[16];
+  return locks[((uintptr_t)workspace >> 9) % 16];
+}
+
 template <int DT, int ODT>
 void launch_attend(const AttendPlan& a, const ChunkParams& c, hipStream_t st) {
   const int many = a.items * c.a.Hkv * a.splits;
+  std::unique_lock<std::mutex> together(launch_lock(c.a.counters), std::defer_lock);
+  if (a.floats > 0) together.lock();
   if (a.few && a.many) {
     const dim3 grid((unsigned)(a.few_wgs + many));
     if (a.qb == 2)

@@ -47,19 +47,20 @@ def rope_table(device: torch.device, stream: int, theta: float, seq_len: int):
     return ent
 
 
-def workspace(device: torch.device, stream: int, floats: int) -> torch.Tensor:
+def workspace(device: torch.device, stream: int, floats: int,
+              cache: dict = _WS_CACHE) -> torch.Tensor:
     """Split-K workspace of at least ``floats`` floats (cached per device and stream). It is
     zero-filled when allocated: its leading merge counters must start at zero, and every call
     leaves them zero. It grows at least twofold; a replaced workspace stays allocated
     (``_lib.retire``: graphs captured with it keep using it)."""
     key = (device.index, stream)
-    t = _WS_CACHE.get(key)
+    t = cache.get(key)
     if t is None or t.numel() < floats:
         old = t
         grow = 2 * old.numel() if old is not None else 0
         t = torch.zeros(max(int(floats), grow, 1 << 16), dtype=torch.float32, device=device)
         _lib.retire(old)
-        _WS_CACHE[key] = t
+        cache[key] = t
     return t
 
 

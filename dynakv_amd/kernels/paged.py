@@ -35,6 +35,7 @@ from .decode import workspace
 HEAD_DIM = 128
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _COUNTERS = 16384  # leading floats of the attention's workspace: its arrival counters
+_WORKSPACES: dict = {}  # (device, stream) -> the attention's workspace
 
 
 class PagedBatch:
@@ -353,11 +354,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 def _attention_workspace(q: torch.Tensor, stream: int, floats: int) -> torch.Tensor:
-    """Split records and arrival counters (zero before and after a call). Eager calls of a stream
-    share its workspace, in that stream's order. A call under capture gets one of its own in the
+    """Split records and arrival counters (zero before and after a call). Eager calls of a stream, from
+    any threads, share its workspace, in that stream's order: a call of two launches makes them
+    together, and no other operator writes there. A call under capture gets one of its own in the
     graph's pool, cleared by the graph itself: two captured graphs may be replayed at once."""
     if _lib.call_on(q.get_device(), torch.cuda.is_current_stream_capturing):
         ws = torch.empty(floats, dtype=torch.float32, device=q.device)
         ws[:_COUNTERS].zero_()
         return ws
-    return workspace(q.device, stream, floats)
+    return workspace(q.device, stream, floats, _WORKSPACES)

@@ -5,6 +5,7 @@ without having been written, or a page that is not the request's, shows in the r
 is checked by comparing the whole pool. Tolerances count the roundings (a 16-bit value is off by at
 most half a step, eps / 2 relative): see ``_append_tol`` and ``_attend_tol``."""
 import math
+import threading
 
 import pytest
 import torch
@@ -842,3 +843,29 @@ def test_fp16_weights_far_below_the_largest(dev, new, lens, gap):
     print(f"[gpu]   err/tol {float((err / (tol + 1e-30)).max()):.3f}", flush=True)
     assert bool((err <= tol + 1e-30).all())
     assert torch.equal(paged_attention(q, s.k, s.v, s.batch), got.to(FP))
+
+
+@pytest.mark.gpu
+def test_threads_on_one_stream(dev):
+    """Calls from several threads on one stream, of one launch and of two (key ranges and their join):
+    each has its own result."""
+    print("[gpu] paged threads", flush=True)
+    s = [Step(dev, new, lens, hkv=2, seed=63 + i) for i, (new, lens) in enumerate(
+        (([40], [3000]), ([64], [2500]), ([1, 1, 40], [900, 450, 2000]), ([1, 1], [2000, 700])))]
+    q = [t.rand(t.T, 8, DH) for t in s]
+    want = [paged_attention(q[i], t.k, t.v, t.batch) for i, t in enumerate(s)]
+    torch.cuda.synchronize()
+    got = [[] for _ in s]
+
+    def run(i):
+        for _ in range(60):
+            got[i].append(paged_attention(q[i], s[i].k, s[i].v, s[i].batch))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(s))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(len(s)):
+        assert len(got[i]) == 60 and all(torch.equal(o, want[i]) for o in got[i]), i

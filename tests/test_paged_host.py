@@ -1,9 +1,14 @@
 """The paged cache's host side, without a device: pages taken and given back, the batch's buffers,
 and the refusals of the operators (checked before anything touches a device)."""
+import shutil
+import subprocess
+import sys
+
 import pytest
 import torch
 
 from dynakv_amd import _lib
+from dynakv_amd.kernels import decode, paged
 from dynakv_amd.kernels.paged import PagedBatch, PagedKVCache, paged_append, paged_attention
 from dynakv_amd.kernels.sampling import sample_tokens
 
@@ -233,3 +238,95 @@ def test_tensor_module_of_another_torch(monkeypatch, tmp_path):
     monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "none.so")
     assert _lib.tensor_calls() is None
     _batch()
+
+
+def test_the_attention_has_a_workspace_of_its_own(monkeypatch):
+    """Other operators' calls, which another thread may make between its two launches, do not write
+    there."""
+    monkeypatch.setattr(_lib, "call_on", lambda device, fn, *args: False)  # no capture
+    monkeypatch.setattr(paged, "_WORKSPACES", {}, raising=False)
+    q = torch.zeros(1, 1, 128, dtype=BF)
+    mine = paged._attention_workspace(q, 77, 1 << 17)
+    assert mine is paged._attention_workspace(q, 77, 1 << 16) and not mine.any()
+    assert mine.data_ptr() != decode.workspace(q.device, 77, 1 << 17).data_ptr()
+    assert mine is not paged._attention_workspace(q, 78, 1 << 16)
+    decode._WS_CACHE.pop((q.device.index, 77))
+
+
+_RECORDER = r"""
+#include <pthread.h>
+#include <stddef.h>
+#include <stdint.h>
+#include <time.h>
+typedef struct { uint32_t x, y, z; } dims;
+static pthread_mutex_t lock = PTHREAD_MUTEX_INITIALIZER;
+static const void* seen[4096];
+static int n;
+int hipGetLastError(void) { return 0; }
+int __hipPushCallConfiguration(dims grid, dims block, size_t lds, void* stream) { return 0; }
+int __hipPopCallConfiguration(dims* grid, dims* block, size_t* lds, void** stream) { return 0; }
+/* a launch takes a millisecond; its first argument's first member, q, tells the call */
+int hipLaunchKernel(const void* f, dims grid, dims block, void** args, size_t lds, void* stream) {
+  pthread_mutex_lock(&lock);
+  if (n < 4096) seen[n++] = *(const void**)args[0];
+  pthread_mutex_unlock(&lock);
+  struct timespec t = {0, 1000000};
+  nanosleep(&t, 0);
+  return 0;
+}
+int launches(const void** out) {
+  for (int i = 0; i < n; ++i) out[i] = seen[i];
+  return n;
+}
+"""
+
+_THREADS = r"""
+import ctypes, sys, threading
+rec = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)  # found before the runtime's own
+lib = ctypes.CDLL(sys.argv[2])
+L, F = ctypes.c_longlong, ctypes.c_float
+lib.dkv_paged_workspace_floats.restype = L
+floats = lib.dkv_paged_workspace_floats(1, 64, 32, 8, 64, 64, 32768)
+assert floats > 16384 and lib.dkv_paged_workspace_floats(1, 1, 32, 8, 1, 1, 32768) > 16384
+P = ctypes.c_void_p
+
+def calls(q, workspace, times, new):
+    for _ in range(times):
+        rc = lib.dkv_paged_attention(
+            P(0), 2, P(q), L(4096), L(128), P(1 << 30), P(1 << 31), L(65536), L(8192), 1000, 64,
+            P(1 << 20), L(512), 512, P(1 << 21), P(1 << 22), 1, new, 32, 8, 128, new, new, 32768, F(0.1),
+            P(workspace), L(floats), P(1 << 23), 2, L(4096), L(128))
+        assert rc == 0, rc
+
+# threads on one stream share its workspace: 1 .. 3 make two launches a call, 4 and 5 one
+threads = [threading.Thread(target=calls, args=((i + 1) << 32, 1 << 24, 8, 64 if i < 3 else 1))
+           for i in range(5)]
+for t in threads: t.start()
+for t in threads: t.join()
+seen = (P * 4096)()
+n = rec.launches(seen)
+assert n == 3 * 8 * 2 + 2 * 8, n
+order = [(s or 0) >> 32 for s in seen[:n]]
+i = 0
+while i < n:
+    two = order[i] <= 3
+    assert not two or order[i] == order[i + 1], order
+    i += 2 if two else 1
+print("together")
+"""
+
+
+def test_launches_of_a_call_stay_together(tmp_path):
+    """Calls of one stream share its workspace, from any thread: what a call's first launch leaves there
+    its second one reads, so no other call's launch may come between them. Launches are recorded in place
+    of being made, in a process of its own."""
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    (tmp_path / "rec.c").write_text(_RECORDER)
+    rec = tmp_path / "librec.so"
+    subprocess.run([cc, "-shared", "-fPIC", "-O1", str(tmp_path / "rec.c"), "-o", str(rec), "-lpthread"],
+                   check=True)
+    run = subprocess.run([sys.executable, "-c", _THREADS, str(rec), str(_lib.LIB_PATH)],
+                         capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and "together" in run.stdout, run.stdout + run.stderr
