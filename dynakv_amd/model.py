@@ -35,6 +35,7 @@ from __future__ import annotations
 import math
 import time
 from dataclasses import dataclass, field
+from typing import Sequence
 
 import torch
 import torch.nn.functional as F
@@ -166,8 +167,9 @@ class RandomLlama:
 
 class Sampler:
     """Draws tokens from logits: a generator's replacement for its argmax. The settings are those of
-    ``sample_tokens``, numbers or a tensor with an entry per row; the uniform numbers come from a
-    generator of its own, so a seed gives the same draws for the same logits."""
+    ``sample_tokens``, numbers or a tensor with an entry per row (of a batch, or of the requests that
+    are generated for); the uniform numbers come from a generator of its own, so a seed gives the same
+    draws for the same logits."""
 
     def __init__(self, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0,
                  device="cuda"):
@@ -175,13 +177,54 @@ class Sampler:
         self._gen = torch.Generator(device=device)
         self._gen.manual_seed(seed)
 
-    def __call__(self, logits: torch.Tensor) -> torch.Tensor:
-        """``logits`` (..., V) -> tokens (...). Of a row without a token to take (all NaN or
-        -infinity) token 0, as the tokens are looked up next: ``sample_tokens`` tells them by -1."""
+    def __call__(self, logits: torch.Tensor, *, requests: Sequence[int] | None = None,
+                 u: torch.Tensor | None = None) -> torch.Tensor:
+        """``logits`` (..., V) -> tokens (...). ``requests``: the request of each row, whose entries the
+        settings' tensors are taken from (else row i has entry i); ``u``: the rows' uniform numbers (else
+        the generator's next ones). Of a row without a token to take (all NaN or -infinity) token 0, as
+        the tokens are looked up next: ``sample_tokens`` tells them by -1."""
         rows = logits.reshape(-1, logits.shape[-1])
-        u = torch.rand(rows.shape[0], generator=self._gen, device=logits.device)
-        return sample_tokens(rows, u, **self.settings).clamp_(min=0).view(logits.shape[:-1])
+        settings = self.settings
+        if requests is not None:
+            settings = self._of(requests, rows)
+        if u is None:
+            u = self.uniform(rows.shape[0], logits.device)
+        return sample_tokens(rows, u, **settings).clamp_(min=0).view(logits.shape[:-1])
 
+    def uniform(self, n: int, device) -> torch.Tensor:
+        """The generator's next ``n`` numbers."""
+        return torch.rand(n, generator=self._gen, device=device)
+
+    def check(self, requests: int) -> None:
+        """Raises where a setting's tensor has not an entry for each of so many requests."""
+        for name, v in self.settings.items():
+            if torch.is_tensor(v) and v.shape != (requests,):
+                raise ValueError(f"{name} must be a number or have an entry for each of the {requests} "
+                                 "requests")
+
+    def _of(self, requests: Sequence[int], rows: torch.Tensor) -> dict:
+        if len(requests) != rows.shape[0]:
+            raise ValueError(f"{len(requests)} requests for {rows.shape[0]} rows of logits")
+        at = None
+        settings = dict(self.settings)
+        for name, v in settings.items():
+            if not torch.is_tensor(v):
+                continue
+            if v.dim() != 1 or not all(0 <= r < v.shape[0] for r in requests):
+                raise ValueError(f"{name} has no entry for one of the requests {list(requests)}")
+            if list(requests) != list(range(v.shape[0])):
+                at = _index(requests, v.device) if at is None else at
+                settings[name] = v.index_select(0, at)
+        return settings
+
+
+
+def _index(numbers: Sequence[int], device) -> torch.Tensor:
+    """Host numbers as an index on the device (a copy that the host does not wait for)."""
+    t = torch.tensor(numbers, dtype=torch.long)
+    if torch.device(device).type == "cuda":
+        t = t.pin_memory()
+    return t.to(device, non_blocking=True)
 
 
 def _rope_q(q: torch.Tensor, pos0: int, theta: float) -> torch.Tensor:
@@ -495,13 +538,15 @@ class PagedLlama(_Generator):
                  sampler: Sampler | None = None, chunk: int = 512) -> dict:
         """``new_tokens`` tokens for each of the (n,) prompts (n >= 1), greedily or drawn by
         ``sampler``; a step takes at most ``chunk`` tokens of prompts, in the prompts' order, beside
-        a token of each request that is generating. Returns the tokens (prompts, new_tokens), the
-        wall time and the most pages held."""
+        a token of each request that is generating. Settings of the sampler with an entry per request
+        are the prompts' in their order, and a request's i-th token is drawn by a uniform number of its
+        own, whichever requests share its step. Returns the tokens (prompts, new_tokens), the wall time
+        and the most pages held."""
         if chunk < 1 or new_tokens < 1 or not prompts:
             raise ValueError("need prompts, a positive chunk and a positive number of tokens")
         if any(p.dim() != 1 or p.shape[0] < 1 for p in prompts):
             raise ValueError("prompts are (n,) tokens, n >= 1")
-        pick = sampler if sampler is not None else lambda logits: logits.argmax(-1)
+        pick = self._pick(sampler, len(prompts), new_tokens)
         torch.cuda.synchronize(self.m.device)
         t0 = time.perf_counter()
         ids: list = [self.add() for _ in prompts]  # None once ended
@@ -522,14 +567,19 @@ class PagedLlama(_Generator):
                     else:
                         continue
                     who.append(j)
-                tok = pick(self.step(feed))
+                logits = self.step(feed)
                 held = max(held, self.cache.pages - self.cache.free_pages)
-                for i, j in enumerate(who):
-                    if fed[j] == prompts[j].shape[0]:  # its whole prompt has gone through
-                        out[j].append(tok[i:i + 1])
-                        if len(out[j]) == new_tokens:
-                            self.end(ids[j])
-                            ids[j] = None
+                done = [i for i, j in enumerate(who) if fed[j] == prompts[j].shape[0]]
+                if not done:  # no request's whole prompt has gone through
+                    continue
+                if len(done) < len(who):
+                    logits = logits.index_select(0, _index(done, logits.device))
+                tok = pick(logits, [(who[i], len(out[who[i]])) for i in done])
+                for i, j in enumerate(who[i] for i in done):
+                    out[j].append(tok[i:i + 1])
+                    if len(out[j]) == new_tokens:
+                        self.end(ids[j])
+                        ids[j] = None
         finally:
             for r in ids:
                 if r is not None:
@@ -538,6 +588,27 @@ class PagedLlama(_Generator):
         t = time.perf_counter() - t0
         return {"tokens": torch.stack([torch.cat(o) for o in out]), "seconds": t,
                 "tokens_per_s": len(prompts) * new_tokens / t, "pages": held}
+
+    def _pick(self, sampler: Sampler | None, requests: int, new_tokens: int):
+        """(logits, (request, index of its token) of each row) -> tokens."""
+        if sampler is None:
+            return lambda logits, at: logits.argmax(-1)
+        if not isinstance(sampler, Sampler):  # any function of logits
+            return lambda logits, at: sampler(logits)
+        sampler.check(requests)
+        # row i: the numbers of the requests' i-th tokens, drawn when the first of them is
+        u = torch.empty(new_tokens, requests, dtype=torch.float32, device=self.m.device)
+        drawn = 0
+
+        def pick(logits, at):
+            nonlocal drawn
+            while drawn <= max(i for _, i in at):
+                u[drawn] = sampler.uniform(requests, u.device)
+                drawn += 1
+            mine = u.view(-1).index_select(0, _index([i * requests + j for j, i in at], u.device))
+            return sampler(logits, requests=[j for j, _ in at], u=mine)
+
+        return pick
 
     def kv_bytes(self) -> int:
         """Bytes of the pages that requests hold, over all layers."""

@@ -150,3 +150,59 @@ def test_a_sampler_gives_tokens_that_can_be_looked_up(dev):
     assert sample_tokens(logits, torch.full((4,), 0.5, device=dev)).tolist()[1:3] == [-1, -1]
     t = Sampler(seed=3, device=dev)(logits)
     assert t[1:3].tolist() == [0, 0] and int(t.min()) >= 0
+
+
+@pytest.mark.gpu
+def test_generate_with_settings_of_each_request(dev, monkeypatch):
+    """Settings with an entry per request hold for that request in every step, whichever others are in
+    it, and its uniform numbers are its own: the same for every size of chunk."""
+    print("[gpu] sampled generate, settings of each request", flush=True)
+    m = RandomLlama(LlamaShape(**KW), device=dev, seed=9, std=0.05)
+    p = PagedLlama(m, pages=20, page_size=16)
+    g = torch.Generator().manual_seed(10)
+    prompts = [torch.randint(0, 1000, (n,), generator=g).to(dev) for n in (50, 3, 21, 40)]
+    f32 = lambda *v: torch.tensor(v, dtype=torch.float32, device=dev)  # noqa: E731
+    setting = dict(temperature=f32(0.0, 50.0, 1.0, 1.0), top_p=f32(1.0, 1.0, 1.0, 0.0),
+                   top_k=torch.tensor([0, 0, 1, 0], dtype=torch.int32, device=dev))
+    for chunk in (512, 16):
+        got = p.generate(prompts, 5, Sampler(seed=3, **setting), chunk=chunk)["tokens"]
+        assert got.shape == (4, 5) and p.cache.free_pages == 20
+        near = []
+        for j, t in enumerate(prompts):
+            want = [_logits(m, torch.cat([t, got[j, :i]]))[-1] for i in range(5)]
+            near.append([float(w[got[j, i]]) >= float(w.max()) - 0.05 * float(w.abs().max())
+                         for i, w in enumerate(want)])
+        # greedy by temperature, by top-k, by top-p; and one that is nearly uniform over 1000 tokens
+        assert all(near[0]) and all(near[2]) and all(near[3]) and not all(near[1])
+    # tokens that the uniform numbers alone decide
+    seen = []
+
+    def by_u(logits, u, **kw):
+        seen.append((logits.shape[0], {k: v.tolist() for k, v in kw.items() if torch.is_tensor(v)}))
+        return (u * 1000).long()
+
+    monkeypatch.setattr("dynakv_amd.model.sample_tokens", by_u)
+    runs = [p.generate(prompts, 5, Sampler(seed=4, **setting), chunk=c)["tokens"]
+            for c in (512, 16, 1, 512)]
+    for r in runs[1:]:
+        assert torch.equal(r, runs[0])
+    assert len(set(runs[0].flatten().tolist())) > 15
+    top_p = setting["top_p"].tolist()
+    for rows, kw in seen:
+        assert rows > 0 and all(len(v) == rows for v in kw.values())
+    assert seen[0][1]["top_p"] == top_p
+    # one entry too few: refused before anything is fed
+    with pytest.raises(ValueError, match="entry"):
+        p.generate(prompts[:3], 5, Sampler(seed=3, **setting))
+    assert p.cache.free_pages == 20
+    # as a callable of its own: rows of some requests
+    logits = torch.randn(2, 1000, device=dev)
+    monkeypatch.undo()
+    s = Sampler(seed=3, **setting)
+    assert torch.equal(s(logits, requests=[2, 0]), logits.argmax(-1))
+    with pytest.raises(ValueError):
+        s(logits, requests=[2, 4])
+    with pytest.raises(ValueError):
+        s(logits, requests=[0, -1])
+    with pytest.raises(ValueError):
+        s(logits, requests=[0])
