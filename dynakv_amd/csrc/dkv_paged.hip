@@ -1234,6 +1234,45 @@ __global__ __launch_bounds__(256) void paged_join_kernel(ChunkParams c) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// T x H segments of `len` bytes, segment (i, h) at `at` + i st + h sh; a stride of a size of one is any.
+struct Segments {
+  long long at, st, sh, len;
+  int T, H;
+  long long end() const { return at + (T - 1) * st + (H - 1) * sh + len; }
+};
+// Whether a segment of a and one of b, of the same strides, have a byte in common (of one array with
+// itself: two of its segments).
+bool segments_meet(const Segments& a, const Segments& b, bool itself = false) {
+  const long long st = a.T > 1 ? a.st : 0;
+  for (int dh = 1 - a.H; dh < b.H; ++dh) {
+    // the least di for which b's segment ends behind the start of a's
+    const long long x = b.at - a.at + dh * b.sh;
+    long long di = 1 - a.T;
+    if (st > 0 && x + di * st + b.len <= 0) di += (-b.len - x - di * st) / st + 1;
+    if (itself && dh == 0 && di <= 0) di = 1;
+    if (di < a.T && x + di * st + b.len > 0 && x + di * st < a.len) return true;
+  }
+  return false;
+}
+// Whether an output's rows may be written while an operator reads `in`: apart from it (or, with its
+// strides, between its rows), or in its place, row for row; no two of them on top of each other.
+bool output_apart(const Segments& out, const Segments& in, bool in_place) {
+  const bool nested =  // (the usual layouts: rows of heads, or heads of rows)
+      (out.sh >= out.len && (out.T == 1 || out.st >= (out.H - 1) * out.sh + out.len)) ||
+      (out.st >= out.len && (out.H == 1 || out.sh >= (out.T - 1) * out.st + out.len));
+  if (!nested && segments_meet(out, out, true)) return false;
+  if (in_place || out.end() <= in.at || in.end() <= out.at) return true;
+  const bool alike = (out.T == 1 || out.st == in.st) &&
+                     ((out.H == 1 && in.H == 1) || (out.H == in.H ? out.sh == in.sh : in.H == 1));
+  if (alike && out.H == in.H) return !segments_meet(in, out);
+  if (!alike) return false;
+  for (int h = 0; h < out.H; ++h) {
+    const Segments one = {out.at + h * out.sh, out.st, 0, out.len, out.T, 1};
+    if (segments_meet(in, one)) return false;
+  }
+  return true;
+}
+
 int fill_pool(PagedPool& pool, long long page_stride, long long head_stride, int num_pages,
               int page_size, const int* table, long long table_ld, int cols, int Hkv) {
   if (num_pages < 0 || cols < 0 || table_ld < cols) return DKV_E_ARG;
@@ -1275,6 +1314,13 @@ extern "C" int dkv_paged_append(void* stream, int dtype, const void* qkv, long l
   if (B == 0 || T == 0) return DKV_OK;
   if (!qkv || !q_out || !k_pages || !v_pages || !q_start || !lens || !inv_freq) return DKV_E_ARG;
   if (qkv_ld < (long long)(Hq + 2 * Hkv) * PG_DH || q_sh < PG_DH || q_st < PG_DH) return DKV_E_ARG;
+  const bool in_place =
+      qkv == q_out && (T == 1 || q_st == qkv_ld) && (Hq == 1 || q_sh == PG_DH);
+  if (!output_apart({(long long)(uintptr_t)q_out, 2 * q_st, 2 * q_sh, 2 * PG_DH, T, Hq},
+                    {(long long)(uintptr_t)qkv, 2 * qkv_ld, 0,
+                     2LL * (Hq + 2 * Hkv) * PG_DH, T, 1},
+                    in_place))
+    return DKV_E_ARG;
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) ||
       (qkv_ld & 7) || (q_st & 7) || (q_sh & 7) || (q_norm && !aligned16(q_norm)) ||
       (k_norm && !aligned16(k_norm)))
@@ -1472,6 +1518,12 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   if (B == 0 || T == 0 || max_new == 0) return DKV_OK;
   if (!q || !k_pages || !v_pages || !q_start || !lens || !out || num_pages == 0) return DKV_E_ARG;
   if (q_st < 0 || q_sh < 0 || o_st < 0 || o_sh < PG_DH) return DKV_E_ARG;
+  const int oz = dkv_elt_size(out_dtype);
+  const bool in_place = q == out && out_dtype == dtype && (T == 1 || q_st == o_st) &&
+                        (Hq == 1 || q_sh == o_sh);
+  if (!output_apart({(long long)(uintptr_t)out, oz * o_st, oz * o_sh, oz * PG_DH, T, Hq},
+                    {(long long)(uintptr_t)q, 2 * q_st, 2 * q_sh, 2 * PG_DH, T, Hq}, in_place))
+    return DKV_E_ARG;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || (q_st & 7) || (q_sh & 7))
     return DKV_E_UNSUPPORTED;
   if (!attend_sizes_ok(B, T, Hq, Hkv, max_new)) return DKV_E_UNSUPPORTED;

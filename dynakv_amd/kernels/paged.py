@@ -259,7 +259,8 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``inv_freq`` (scaled frequencies), the angle formed in 64 bits. With ``q_norm`` / ``k_norm``
     ((128,) of qkv's dtype) each query / key head is first normed, x / sqrt(mean(x^2) + eps) * w.
     Everything in fp32, rounded once where it is stored. ``out``: where the queries go (T, heads,
-    128), unit last stride (qkv's own query columns will do). A token whose page is not there is not stored."""
+    128), unit last stride: qkv's own query columns, or memory apart from it. A token whose page is not
+    there is not stored."""
     freqs = _frequency_address(theta, inv_freq)
     fast = _lib.tensor_calls()
     if fast is not None and out is None and _lib.is_current(batch._args[10]):
@@ -309,7 +310,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     token at position t attends its request's tokens 0 .. t (the pages hold them all: the step's own
     are appended first); one that has none to attend gives 0. ``scale`` defaults to 1 / sqrt(128).
     The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``;
-    ``out`` may be q itself."""
+    ``out`` may be q itself, or memory apart from it."""
     fast = _lib.tensor_calls()
     if (fast is not None and out is None and out_dtype is None
             and _lib.is_current(batch._args[10])):

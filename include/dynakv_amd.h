@@ -633,10 +633,12 @@ int dkv_gemv_glu(void* stream, int dtype, const void* x, long long x_ld, const v
  * (x / sqrt(mean(x^2) + eps) * w), are rotated (rotate-half) by position * inv_freq[j] (64 doubles
  * in HOST memory, read during the call), in fp32 with the angle in 64 bits, and rounded once: the
  * queries to q_out (strides q_st per row, q_sh per head), the keys to their page. Values are copied.
- * 16-byte aligned rows; q_out apart from qkv.
+ * 16-byte aligned rows; q_out apart from qkv, or qkv's own query columns (an output that meets its input
+ * in another way, or whose rows meet each other, is refused, here and below).
  *
  * dkv_paged_attention: q (T, Hq, 128), rotated; the row at position t attends its request's tokens
- * 0 .. t, softmax in fp32; a row with none gives 0; out in dtype or fp32. Hq / Hkv <= 16. max_new
+ * 0 .. t, softmax in fp32; a row with none gives 0; out in dtype or fp32, apart from q, or (in dtype, with
+ * q's strides) q itself. Hq / Hkv <= 16. max_new
  * and max_len bound every request's new tokens and length, min_new (from below) the new tokens of a
  * request that has any: they choose the launch, and what passes them may be left out. The workspace
  * holds dkv_paged_workspace_floats(...) floats, its first 16384 zero (and left zero); it may be null

@@ -253,6 +253,48 @@ def test_the_attention_has_a_workspace_of_its_own(monkeypatch):
     decode._WS_CACHE.pop((q.device.index, 77))
 
 
+def test_outputs_on_top_of_inputs_or_themselves():
+    """An output may be its operator's queries, place for place, or memory that no row of theirs and no
+    other row of its own has: anything else is refused, as rows are written while others are read. (No
+    call here gets to its launch: weights off their alignment, or no workspace, are refused next.)"""
+    lib = _lib.load()
+    E, U, WS = _lib.DKV_E_ARG, _lib.DKV_E_UNSUPPORTED, _lib.DKV_E_WORKSPACE
+    at, far = 1 << 32, (1 << 32) + (1 << 24)
+
+    def append(q_out, q_st, q_sh, T=4, hq=4):  # a projection of (T, 1024), 8 heads
+        return lib.dkv_paged_append(None, _lib.DKV_BF16, at, 1024, q_out, q_st, q_sh, at << 1, at << 2,
+                                    4096, 2048, 4, 16, at << 3, 2, 2, at << 3, at << 3, 1, T, hq,
+                                    (8 - hq) // 2, 128, at + 2, None, 1e-6, at)
+
+    for q_out, st, sh in ((at, 1024, 128), (far, 512, 128), (far, 128, 512), (far, 640, 128),
+                          (far, 1024, 256), (at - 4096, 512, 128), (at + 8192, 512, 128)):
+        assert append(q_out, st, sh) == U, (q_out - at, st, sh)
+    for q_out, st, sh in ((at + 16, 1024, 128), (at + 2048, 1024, 128), (at + 1024, 1024, 128),
+                          (at - 256, 1024, 128), (at, 512, 128), (at, 1024, 256), (at - 4080, 512, 128),
+                          (at + 8176, 512, 128), (far, 128, 128), (far, 256, 128), (far, 384, 384),
+                          (far, 504, 128), (far, 128, 504)):
+        assert append(q_out, st, sh) == E, (q_out - at, st, sh)
+    assert append(at, 8, 128, T=1) == E and append(at, 512, 128, T=1) == U  # (a row is a row)
+    assert append(at + 256, 512, 128, T=1) == E
+
+    def attend(out, o_st, o_sh, q_st=512, q_sh=128, T=4, hq=4, odt=_lib.DKV_BF16):
+        return lib.dkv_paged_attention(None, _lib.DKV_BF16, at, q_st, q_sh, at << 1, at << 2, 4096,
+                                       2048, 4, 16, at << 3, 4096, 4096, at << 3, at << 3, 1, T, hq, 2,
+                                       128, T, 1, 65536, 0.1, None, 0, out, odt, o_st, o_sh)
+
+    f32 = _lib.DKV_F32
+    for args in ((at, 512, 128), (far, 512, 128), (far, 128, 512), (far, 512, 128, 512, 128, 4, 4, f32),
+                 (far, 512, 128, 0, 0), (at, 1024, 128, 1024), (at + 1024, 1024, 128, 1024),
+                 (at, 1024, 256, 1024, 256), (at + 256, 1024, 256, 1024, 256), (at, 128, 512, 128, 512),
+                 (at + 4096, 512, 128), (at - 4096, 512, 128), (at, 77, 128, 96, 128, 1)):
+        assert attend(*args) == WS, args
+    for args in ((at + 16, 512, 128), (at + 256, 512, 128), (at + 1024, 512, 128), (at - 256, 512, 128),
+                 (at, 512, 128, 512, 128, 4, 4, f32), (at, 1024, 128), (at, 128, 512),
+                 (at + 1008, 1024, 128, 1024), (at, 512, 128, 0, 0), (at + 4080, 512, 128),
+                 (far, 0, 128), (far, 256, 128), (far, 128, 256), (far, 504, 128)):
+        assert attend(*args) == E, args
+
+
 _RECORDER = r"""
 #include <pthread.h>
 #include <stddef.h>
