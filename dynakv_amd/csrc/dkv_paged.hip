@@ -739,8 +739,9 @@ constexpr float C_RESCALE = DT == DKV_F16 ? PG_F16_RESCALE : 8.f;
 struct ChunkParams {
   AttendParams a;
   float* records;
-  // rows of a workgroup and their log2; key ranges; rows up to which the other kernel works
-  int bq, bq_shift, splits, few_rows;
+  // rows of a workgroup and their log2; row tiles that have key ranges, and how many (further tiles
+  // have one, and no record); rows up to which the other kernel works
+  int bq, bq_shift, items, splits, few_rows;
   Divisor by_splits;
 };
 
@@ -874,8 +875,11 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   // stay in one L2 (for 8 heads, or a multiple)
   const int rest = __builtin_amdgcn_readfirstlane(quot(p.by_hkv, wg));
   const int kvh = wg - rest * p.Hkv;
-  const int item = __builtin_amdgcn_readfirstlane(quot(c.by_splits, rest));
-  const int split = rest - item * c.splits;
+  const bool cut = rest < c.items * c.splits;
+  const int splits = cut ? c.splits : 1;
+  const int item = cut ? __builtin_amdgcn_readfirstlane(quot(c.by_splits, rest))
+                       : rest - c.items * (c.splits - 1);
+  const int split = cut ? rest - item * c.splits : 0;
   const ChunkItem it = chunk_item(c, item, lane);
   const int b = __builtin_amdgcn_readfirstlane(it.b);
   if (b < 0) return;
@@ -890,7 +894,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const int w_first = r.pos0 + quot(p.by_hpg, min(wq0, rows - 1));
   const int w_end = wq0 < rows ? r.pos0 + quot(p.by_hpg, min(wq0 + QW, rows) - 1) + 1 : 0;
   const int all_tiles = (k_end + CK - 1) / CK;
-  const int per = quot(c.by_splits, all_tiles + c.splits - 1);
+  const int per = cut ? quot(c.by_splits, all_tiles + c.splits - 1) : all_tiles;
   const int t0 = min(all_tiles, split * per), n_tiles = min(all_tiles, t0 + per);
 
   // pages of the 64 blocks of 16 keys from tile tb on (16 tiles); the next 64 fetched ahead
@@ -1127,7 +1131,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     unsigned long long bad = __ballot(R < rows && (!(odd == 0.f) || low));
     bad = (bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & 0xffffull;  // by row
     const bool good = R < rows && !((bad >> n) & 1);
-    if (c.splits == 1) {
+    if (splits == 1) {
       if (good) {
         const float inv = l > 0.f ? 1.f / l : 0.f;
         const long long ob = (long long)(r.row0 + i) * p.o_st +
@@ -1150,7 +1154,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       float mx, lx, o0, o1;
       attend_row_apart<DT>(p, b, kvh, qx, t0 * CK, min(n_tiles * CK, min(r.pos0 + ix + 1, r.len)),
                            lane, mx, lx, o0, o1);
-      if (c.splits == 1) {
+      if (splits == 1) {
         const float inv = lx > 0.f ? 1.f / lx : (lx == 0.f ? 0.f : lx);
         const long long ob = (long long)(r.row0 + ix) * p.o_st +
                              (long long)(kvh * p.hpg + hx) * p.o_sh + 2 * lane;
@@ -1362,7 +1366,8 @@ namespace {
 struct AttendPlan {
   bool few, many;          // kernels that run
   int few_wgs, few_split;
-  int qb, nw, bq, items, splits;
+  int qb, nw, bq, splits;
+  int items, more;         // row tiles cut into key ranges, and further ones that are not
   long long many_at;       // the many-row kind's records, in floats from the others'
   long long floats;        // workspace (0: none)
 };
@@ -1431,10 +1436,18 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
     }
     a.bq = 16 * a.qb * a.nw;
     a.items = (int)items(a.bq);
-    const long long wgs = (long long)a.items * Hkv;
     if (a.splits > 1) {  // its records behind the other kind's
+      // Of tiles that requests of min_new tokens (and more rows than the other kind's) can have: a step's
+      // other requests have no token. The tiles that only a step which breaks min_new has come after them.
+      const long long least = a.few ? DROWS / hpg + 1 : min_new;
+      const long long n = T / least < B ? (T >= least ? T / least : 1) : B;
+      const long long x = (long long)T * hpg / a.bq + n;
+      const long long y = ((long long)max_new * hpg + a.bq - 1) / a.bq * n;
+      const int all = a.items;
+      a.items = (int)(x < y ? x : y);
+      a.more = all - a.items;
       a.many_at = (floats + 3) / 4 * 4;
-      floats = a.many_at + wgs * a.splits * a.bq * (PG_DH + 2);
+      floats = a.many_at + (long long)a.items * Hkv * a.splits * a.bq * (PG_DH + 2);
     }
   }
   a.floats = floats ? D_COUNTERS + floats : 0;
@@ -1451,7 +1464,7 @@ std::mutex& launch_lock(const void* workspace) {
 
 template <int DT, int ODT>
 void launch_attend(const AttendPlan& a, const ChunkParams& c, hipStream_t st) {
-  const int many = a.items * c.a.Hkv * a.splits;
+  const int many = (a.items * a.splits + a.more) * c.a.Hkv;
   std::unique_lock<std::mutex> together(launch_lock(c.a.counters), std::defer_lock);
   if (a.floats > 0) together.lock();
   if (a.few && a.many) {
@@ -1556,6 +1569,7 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   c.records = workspace ? workspace + D_COUNTERS + plan.many_at : nullptr;
   c.bq = plan.bq;
   c.bq_shift = plan.many ? __builtin_ctz((unsigned)plan.bq) : 0;
+  c.items = plan.items;
   c.splits = plan.splits;
   c.by_splits = divisor(plan.many ? plan.splits : 1);
   c.few_rows = plan.few ? DROWS : 0;

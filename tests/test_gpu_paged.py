@@ -869,3 +869,21 @@ def test_threads_on_one_stream(dev):
     torch.cuda.synchronize()
     for i in range(len(s)):
         assert len(got[i]) == 60 and all(torch.equal(o, want[i]) for o in got[i]), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens,bounds", [
+    ([0] * 30 + [64] + [0] * 9, [40] * 30 + [3000] + [700] * 9, {}),
+    ([0] * 30 + [64, 1] + [0] * 9, [40] * 30 + [3000, 90] + [700] * 9, {}),
+    # a least number of new tokens that does not hold: more row tiles than it allows for
+    ([1] * 20 + [64], [500, 17] * 10 + [3000], dict(min_new=64)),
+])
+def test_attention_beside_requests_of_no_new_token(dev, new, lens, bounds):
+    print(f"[gpu] paged attention idle requests {len(new)} {bounds}", flush=True)
+    s = Step(dev, new, lens, hkv=2, seed=67)
+    q = s.rand(s.T, 8, DH)
+    want, tol = _attend_reference(s, q)
+    batch = PagedBatch(s.batch.page_table, s.batch.q_start, s.batch.lens, **(dict(
+        rows=s.rows, max_new=64, max_len=3000, min_new=s.batch.min_new) | bounds))
+    got = paged_attention(q, s.k, s.v, batch, out_dtype=torch.float32)
+    assert bool(((got.double() - want).abs() <= tol + 1e-30).all())

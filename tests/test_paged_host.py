@@ -240,6 +240,21 @@ def test_tensor_module_of_another_torch(monkeypatch, tmp_path):
     _batch()
 
 
+@pytest.mark.parametrize("heads,kv", [(32, 8), (16, 1), (8, 8)])
+def test_requests_without_new_tokens_need_no_workspace(heads, kv):
+    """A chunk beside requests that have no token in the step: the records are those of the requests
+    that can have rows, by the step's rows and the least number of new tokens."""
+    floats = lambda B, T, new, least: _lib.load().dkv_paged_workspace_floats(  # noqa: E731
+        B, T, heads, kv, new, least, 32768)
+    alone = floats(1, 64, 64, 64)
+    assert alone > 16384
+    for B in (2, 64, 1024):
+        assert floats(B, 64, 64, 64) == alone
+        # single tokens are allowed: requests of more than 16 rows are still few
+        few = 64 // (16 // (heads // kv) + 1)
+        assert floats(B, 64, 64, 1) <= floats(1, 64, 64, 1) * (1 + few) + 256 * 16 * 130
+
+
 def test_the_attention_has_a_workspace_of_its_own(monkeypatch):
     """Other operators' calls, which another thread may make between its two launches, do not write
     there."""
