@@ -47,7 +47,7 @@ from .kernels.cutoff import CutoffHead
 from .kernels.decode import dense_append_, dense_decode_attention, grouped_decode_attention
 from .kernels.layer import DecodeLayerPlan
 from .kernels.model_ops import linear, rmsnorm_glu, rmsnorm_linear
-from .kernels.paged import PagedKVCache, paged_append, paged_attention
+from .kernels.paged import PagedBatch, PagedKVCache, paged_append, paged_attention
 from .kernels.prefill import coef_prefill_attention, rope_dense_
 from .kernels.router import KernelPolicy
 from .kernels.sampling import sample_tokens
@@ -518,11 +518,21 @@ class PagedLlama(_Generator):
         self.cache.free(request)
 
     def step(self, feed: list[tuple[int, torch.Tensor]]) -> torch.Tensor:
-        """Feed each (request, (n,) tokens), n >= 1; returns (requests, vocab) logits."""
-        s = self.s
+        """Feed each (request, (n,) tokens), n >= 1; returns (requests, vocab) logits. A step that raises
+        leaves the requests as long as they were."""
         if not feed or any(t.dim() != 1 or t.shape[0] < 1 for _, t in feed):
             raise ValueError("a step feeds at least one token to each of its requests")
+        before = [(r, self.cache.length(r)) for r, _ in feed]
         batch = self.cache.batch((r, t.shape[0]) for r, t in feed)
+        try:
+            return self._step(feed, batch)
+        except BaseException:
+            for r, n in before:
+                self.cache.truncate(r, n)
+            raise
+
+    def _step(self, feed: list[tuple[int, torch.Tensor]], batch: PagedBatch) -> torch.Tensor:
+        s = self.s
         x = F.embedding(torch.cat([t for _, t in feed]), self.m.embed).unsqueeze(0)
 
         def attn(i, lw, y):

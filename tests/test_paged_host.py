@@ -11,6 +11,7 @@ from dynakv_amd import _lib
 from dynakv_amd.kernels import decode, paged
 from dynakv_amd.kernels.paged import PagedBatch, PagedKVCache, paged_append, paged_attention
 from dynakv_amd.kernels.sampling import sample_tokens
+from dynakv_amd.model import LlamaShape, PagedLlama
 
 BF = torch.bfloat16
 
@@ -387,3 +388,33 @@ def test_launches_of_a_call_stay_together(tmp_path):
     run = subprocess.run([sys.executable, "-c", _THREADS, str(rec), str(_lib.LIB_PATH)],
                          capture_output=True, text=True, timeout=120)
     assert run.returncode == 0 and "together" in run.stdout, run.stdout + run.stderr
+
+
+class _Weights:
+    """What a PagedLlama takes of a model before its first kernel."""
+
+    shape = LlamaShape(hidden=256, layers=2, heads=2, kv_heads=2, head_dim=128, ffn=64, vocab=50)
+    dtype, device = BF, torch.device("cpu")
+    embed = torch.zeros(50, 256, dtype=BF)
+    layers: list = []
+
+
+def test_a_step_that_fails_changes_nothing():
+    """Tokens that cannot be looked up (floats here): the requests have the lengths and pages they
+    had, so that the step can be given again."""
+    p = PagedLlama(_Weights(), pages=8, page_size=16)
+    a, b = p.add(), p.add()
+    p.cache.batch([(a, 20)])
+    ids = p.cache.page_ids(a)
+    for tokens in ([torch.zeros(5), torch.zeros(40)], [torch.zeros(5, dtype=torch.long), torch.ones(40)]):
+        with pytest.raises(Exception):
+            p.step([(a, tokens[0]), (b, tokens[1])])
+        assert (p.cache.length(a), p.cache.length(b), p.cache.free_pages) == (20, 0, 6)
+        assert p.cache.page_ids(a) == ids
+    with pytest.raises(ValueError, match="no request"):
+        p.step([(a, torch.zeros(1)), (9, torch.zeros(1))])
+    with pytest.raises(ValueError, match="once"):
+        p.step([(a, torch.zeros(1)), (a, torch.zeros(1))])
+    with pytest.raises(RuntimeError, match="pages"):
+        p.step([(a, torch.zeros(200))])
+    assert (p.cache.length(a), p.cache.free_pages) == (20, 6)
