@@ -107,9 +107,10 @@ class PagedKVCache:
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"unsupported dtype {dtype}")
         self.page_size, self.pages = page_size, pages
-        self.device = torch.device(device)
         dims = (pages, kv_heads, page_size, HEAD_DIM)
-        self.k = [torch.empty(dims, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.k = [torch.empty(dims, dtype=dtype, device=device)]
+        self.device = self.k[0].device  # ("cuda": the device that is current now)
+        self.k += [torch.empty(dims, dtype=dtype, device=self.device) for _ in range(layers - 1)]
         self.v = [torch.empty(dims, dtype=dtype, device=self.device) for _ in range(layers)]
         self._free = list(range(pages - 1, -1, -1))
         self._held: dict[int, list[int]] = {}

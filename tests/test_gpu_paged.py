@@ -887,3 +887,14 @@ def test_attention_beside_requests_of_no_new_token(dev, new, lens, bounds):
         rows=s.rows, max_new=64, max_len=3000, min_new=s.batch.min_new) | bounds))
     got = paged_attention(q, s.k, s.v, batch, out_dtype=torch.float32)
     assert bool(((got.double() - want).abs() <= tol + 1e-30).all())
+
+
+@pytest.mark.gpu
+def test_a_cache_stays_on_its_device(dev):
+    """A cache made for "cuda" is on the device that was current then, and its batches go there whichever
+    is current later."""
+    print("[gpu] paged cache device", flush=True)
+    cache = PagedKVCache(1, 4, 2, page_size=16, device="cuda")
+    assert cache.device == cache.k[0].device and cache.device.index is not None
+    a = cache.add()
+    assert cache.batch([(a, 3)]).page_table.device == cache.device
