@@ -1517,7 +1517,7 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
                                    int max_len, float scale, float* workspace,
                                    long long workspace_floats, void* out, int out_dtype,
                                    long long o_st, long long o_sh) {
-  if (!(scale > 0.f) || !(scale < INFINITY)) return DKV_E_UNSUPPORTED;
+  if (!(scale > 0.f) || !(scale * 1.4426950408889634f < INFINITY)) return DKV_E_UNSUPPORTED;
   if (dtype != DKV_F16 && dtype != DKV_BF16) return DKV_E_UNSUPPORTED;
   if (out_dtype != dtype && out_dtype != DKV_F32) return DKV_E_ARG;
   if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || max_new < 0 || min_new < 0 || max_len < 0)

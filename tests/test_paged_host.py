@@ -418,3 +418,14 @@ def test_a_step_that_fails_changes_nothing():
     with pytest.raises(RuntimeError, match="pages"):
         p.step([(a, torch.zeros(200))])
     assert (p.cache.length(a), p.cache.free_pages) == (20, 6)
+
+
+def test_attention_scale_too_large_for_its_logarithm():
+    """The scores are in units of log2: a scale whose product with log2(e) is past fp32 is refused (the
+    call that is not is refused next, for its lack of a workspace)."""
+    at = 1 << 32
+    attend = lambda scale: _lib.load().dkv_paged_attention(  # noqa: E731
+        None, _lib.DKV_BF16, at, 512, 128, at << 1, at << 2, 4096, 2048, 4, 16, at << 3, 4096, 4096,
+        at << 3, at << 3, 1, 4, 4, 2, 128, 4, 1, 65536, scale, None, 0, at, _lib.DKV_BF16, 512, 128)
+    assert attend(2.3e38) == _lib.DKV_E_WORKSPACE and attend(1e-30) == _lib.DKV_E_WORKSPACE
+    assert attend(2.4e38) == _lib.DKV_E_UNSUPPORTED and attend(3.4e38) == _lib.DKV_E_UNSUPPORTED
