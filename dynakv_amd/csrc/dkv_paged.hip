@@ -1541,6 +1541,7 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
     return DKV_E_UNSUPPORTED;
   if (!attend_sizes_ok(B, T, Hq, Hkv, max_new)) return DKV_E_UNSUPPORTED;
   const AttendPlan plan = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len);
+  if (!aligned16(workspace)) return DKV_E_UNSUPPORTED;
   if (plan.floats > 0 && (!workspace || workspace_floats < plan.floats)) return DKV_E_WORKSPACE;
   p.q = (const uint16_t*)q;
   p.q_st = q_st;

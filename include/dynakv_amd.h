@@ -641,8 +641,8 @@ int dkv_gemv_glu(void* stream, int dtype, const void* x, long long x_ld, const v
  * q's strides) q itself. Hq / Hkv <= 16. max_new
  * and max_len bound every request's new tokens and length, min_new (from below) the new tokens of a
  * request that has any: they choose the launch, and what passes them may be left out. The workspace
- * holds dkv_paged_workspace_floats(...) floats, its first 16384 zero (and left zero); it may be null
- * where that is 0. Calls that share it must not overlap on the device: those of one stream may share it,
+ * holds dkv_paged_workspace_floats(...) floats, its first 16384 zero (and left zero), 16-byte
+ * aligned; it may be null where that is 0. Calls that share it must not overlap on the device: those of one stream may share it,
  * from any threads (a call of two launches makes them together).
  */
 int dkv_paged_append(void* stream, int dtype, const void* qkv, long long qkv_ld, void* q_out,

@@ -429,3 +429,15 @@ def test_attention_scale_too_large_for_its_logarithm():
         at << 3, at << 3, 1, 4, 4, 2, 128, 4, 1, 65536, scale, None, 0, at, _lib.DKV_BF16, 512, 128)
     assert attend(2.3e38) == _lib.DKV_E_WORKSPACE and attend(1e-30) == _lib.DKV_E_WORKSPACE
     assert attend(2.4e38) == _lib.DKV_E_UNSUPPORTED and attend(3.4e38) == _lib.DKV_E_UNSUPPORTED
+
+
+def test_attention_workspace_alignment():
+    """Records are read and written 8 and 16 bytes at a time: a workspace that is not aligned to 16 is
+    refused (before one that is too small, as all of these are)."""
+    at = 1 << 32
+    attend = lambda ws: _lib.load().dkv_paged_attention(  # noqa: E731
+        None, _lib.DKV_BF16, at, 512, 128, at << 1, at << 2, 4096, 2048, 4, 16, at << 3, 4096, 4096,
+        at << 3, at << 3, 1, 4, 4, 2, 128, 4, 1, 65536, 0.1, ws, 0, at, _lib.DKV_BF16, 512, 128)
+    assert attend(at) == _lib.DKV_E_WORKSPACE and attend(None) == _lib.DKV_E_WORKSPACE
+    for off in (2, 4, 8):
+        assert attend(at + off) == _lib.DKV_E_UNSUPPORTED
