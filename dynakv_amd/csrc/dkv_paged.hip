@@ -85,7 +85,7 @@ __device__ __forceinline__ int paged_page(const PagedPool& pool, int b, int t) {
 // One wave per row and 8 heads: lane (head h = lane / 8, piece c = lane % 8) holds dims
 // 8c .. 8c + 7 and 64 + 8c .. 64 + 8c + 7, so both halves of its eight pairs.
 //
-// Bound by memory where there is much to do: 8192 tokens of 32 + 2 x 8 heads with norms 44.9 us, 4.5 TB/s
+// Bound by memory where there is much to do: 8192 tokens of 32 + 2 x 8 heads with norms 44.6 us, 4.5 TB/s
 // of reads and writes (a large copy has 4.8); 16 tokens 4.0 us, the chain of loads to the page id.
 // Stores past the caches (non-temporal) take 3 us off the former and add 9 to the attention after it.
 // ---------------------------------------------------------------------------------------
@@ -305,12 +305,15 @@ __device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
 // tokens, so slots behind them read as zero and cost nothing. S^T = K Q^T and P V on 16x16x32 MFMA
 // with the rows in the operand's columns; the weights go to the products as 16-bit hi + lo
 // pairs, which the 32 deep products of 16 tokens have room for. Waves are joined in LDS, parts by the
-// unit's last one to arrive. 16 requests of 2K to 8K tokens (8 KV heads) 61 us, 5.7 TB/s; two of 65533
-// 86 us, 6.0 TB/s; one of 96 5.5 us, the latency of lengths, page ids, one tile and the joins.
+// unit's last one to arrive. 16 requests of 2K to 8K tokens (8 KV heads) 63 us, 5.6 TB/s; two of 65533
+// 89 us, 6.0 TB/s; one of 96 5.0 us, the latency of lengths, page ids, one tile and the joins.
 //
-// How a step's units are cut: requests have any lengths, which only the device knows, and the launch
-// has a fixed number of workgroups. Every wave finds the smallest part C (tiles) for which
-// sum over units of ceil(tiles / C) parts fit the launch, and takes its own from the running sums.
+// How a step's units are cut, where there are fewer than D_WGS: requests have any lengths, which only
+// the device knows, and the launch has a fixed number of workgroups. Every wave finds the smallest part C
+// (tiles) for which sum over units of ceil(tiles / C) parts fit the launch, and takes its own from the
+// running sums. From D_WGS units on (32 requests of 8 KV heads) a unit is one workgroup's, whatever its
+// length: 32 requests of 8192 tokens 159 us (6.7 TB/s, partly from the memory-side cache), 33 of them 226,
+// a second round of workgroups; one of 65536 beside 39 of 500 570 us, beside 20 of 500, in parts, 66.
 constexpr int DSLOT = 2;                    // tile slots per wave
 constexpr int DTILE = 16;
 constexpr int DTILE_BYTES = DTILE * PG_DH * 2;
@@ -318,8 +321,9 @@ constexpr int DSLOT_BYTES = 2 * DTILE_BYTES;
 constexpr int DROWS = 16;
 constexpr int DREC = DROWS * (PG_DH + 2);   // floats of a record: m, l and acc[128] of 16 rows
 constexpr int D_COUNTERS = 16384;           // leading workspace ints
-constexpr int D_SPLIT_B = 256;              // requests a wave can hold the lengths of (4 a lane)
 constexpr int D_WGS = 256;                  // workgroups of 8 waves: one per CU
+constexpr int D_SPLIT_B = 256;              // requests a wave can hold the lengths of (4 a lane)
+static_assert(D_WGS <= D_SPLIT_B && D_WGS <= D_COUNTERS, "units that are cut: fewer than D_WGS");
 constexpr int D_MIN_TILES = 16;             // least part
 template <int DT>                           // log2 units the running maximum may be exceeded by
 constexpr float D_RESCALE = DT == DKV_F16 ? PG_F16_RESCALE : 11.5f;
@@ -713,20 +717,20 @@ __global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
 // request and KV head (NW waves of QB blocks of 16 rows) and all the keys they attend, or, where
 // there are few rows to fill the chip with, one of `splits` ranges of them (records joined by a
 // second launch). Key tiles of 64 are staged in LDS (double-buffered, direct-to-LDS loads, 16-byte
-// pieces XOR-swizzled by key so that neither the row reads of K nor the transposed reads of V meet
-// in a bank); a tile is four blocks of 16 keys, each within one page, and a wave loads one of them
+// pieces XOR-swizzled by key so that the row reads of K do not meet in a bank; of the transposed reads of
+// V those of keys 2i and 2i + 1 do, two cycles a read by SQ_LDS_BANK_CONFLICT); a tile is four blocks of 16 keys, each within one page, and a wave loads one of them
 // (NW = 8: half of one) through a resource that ends with the request's keys. S^T = K Q^T on
 // 16x16x32 MFMA (a lane then holds one row's scores for 16 keys); softmax in fp32, the running
 // maximum raised only when a tile's exceeds it by more than 2^8 (fp16: 2^3); P V on 16x16x32 MFMA with
 // the weights rounded once to the cache's type and summed as rounded: a weight is off by at most half a
-// step (fp16: or 2^-37 of the row's largest, above), as the output is by its own rounding, and as the
-// errors are of either sign, together they come to 1.25 to 1.4 times the output's alone (normal scores,
-// measured against 64 bits; a second product with what the rounding left would take half as many products
-// again, which are the prompts' bound).
+// step (fp16: or 2^-37 of the row's largest, above), and a row, which its sum divides, by at most two half
+// steps of sum p |v|; as the errors are of either sign, with the output's own rounding they come to 1.25
+// to 1.4 times that alone (normal scores, measured against 64 bits; a second product with what the
+// rounding left would take half as many products again, which are the prompts' bound).
 //
-// Bound by the SIMDs' issue slots: per wave and tile (QB = 2) 66 products of 16 cycles beside ~190
+// Bound by the SIMDs' issue slots: per wave and tile (QB = 2) 68 products of 16 cycles beside ~190
 // vector instructions, 32 of them exponentials of 16 cycles; two waves a SIMD fill one's products with
-// the other's vector work in part. Four prompts of 2048 tokens (32 and 8 heads): 159 us, 0.86 PFLOP/s
+// the other's vector work in part. Four prompts of 2048 tokens (32 and 8 heads): 158 us, 0.87 PFLOP/s
 // (a workgroup's start and end are as long as three of its 17 tiles), one of 8192: 500 us, 1.10 PFLOP/s,
 // where a large library product reaches 1.23. (Sums by additions and equal priorities: 2% more.) Key
 // tiles of 32 and three waves a SIMD: the same at 8192, 10% slower on chunks. Deeper rings of tiles, the
@@ -817,7 +821,9 @@ __device__ __forceinline__ float pg_max4(float x) {  // over lanes n, n + 16, n 
 // One row over keys k0 .. k1 - 1, by a wave, key by key: for rows whose values came out as infinity or
 // NaN, or whose scores are too large for one fused multiplication and subtraction. A product of
 // matrices takes a masked key's value times 0, which is NaN for an infinite one; here
-// a masked key is not touched. Lane l returns dims 2l, 2l + 1.
+// a masked key is not touched. Lane l returns dims 2l, 2l + 1. Slow, and for every row that attends such
+// a value: one NaN in the first value of a KV head makes 512 tokens at 8192 take 16 ms (80 us without), a
+// prompt of 2048 8.8 ms (59 us).
 template <int DT>
 __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, int kvh,
                                               const uint16_t* qr, int k0, int k1, int lane,
@@ -1377,7 +1383,7 @@ struct AttendPlan {
 // tiles of the longest request. us on MI355X, bf16, 32 query and 8 KV heads; shape: row blocks x
 // waves / key ranges (workgroups):
 //  * more than 1024 of 128 rows: 2x4, each key operand read from LDS serves two products. Four
-//    2048-token prompts 156 2x4/1, 167 1x8/1, 188 1x4/1.
+//    2048-token prompts 158 2x4/1, 167 1x8/1, 188 1x4/1.
 //  * up to 256 of 128 rows and long keys: ranges that fill the chip once, at least 24 tiles each.
 //    512 tokens at 8192: 77.7 2x4/4 (512), 87 2x4/3, 89.4 1x4/2, 125 1x4/1. 846 tokens of two
 //    requests at up to 6001: 87.3 2x4/2, 89.4 2x4/4, 101 1x4/1.
@@ -1398,10 +1404,8 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
     const long long tiles = ((long long)max_len + DTILE - 1) / DTILE;
     const long long most = units * ((tiles + D_MIN_TILES - 1) / D_MIN_TILES);
     long long wgs = units;
-    if (B <= D_SPLIT_B && units <= D_COUNTERS) {
-      if (wgs < D_WGS) wgs = most < D_WGS ? (most > units ? most : units) : D_WGS;
-      a.few_split = wgs > units;
-    }
+    if (wgs < D_WGS) wgs = most < D_WGS ? (most > units ? most : units) : D_WGS;
+    a.few_split = wgs > units;
     a.few_wgs = (int)wgs;
     if (a.few_split) floats = wgs * DREC;
   }
@@ -1420,7 +1424,8 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
     auto ranges = [&](long long wgs, long long least) {
       // (beside the other kind, about half the chip: 12 single tokens and 512 at 2048, 16 and 4
       // heads: 30 us with two ranges; 42 with one or three and 49 in a launch of its own, where two
-      // took 34)
+      // took 34. How many workgroups the other kind has does not count: 512 at 8192 beside one token,
+      // or with a least number of new tokens that allows one, 128 us, alone 80)
       const long long n = a.few ? (256 + wgs / 2) / wgs : 512 / wgs, most = (tiles + least / 2) / least;
       return (int)(n < most ? n : most);
     };

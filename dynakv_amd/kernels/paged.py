@@ -49,7 +49,9 @@ class PagedBatch:
     ``q_start[B]``; ``max_new`` and ``max_len``: at least the largest number of new tokens and the
     largest length; ``min_new``: at most the smallest number of new tokens of a request that has
     any. The host never reads the device buffers, so the bounds are the caller's to keep: new
-    tokens past ``max_new`` or keys past ``max_len`` may be left out."""
+    tokens past ``max_new`` or keys past ``max_len`` may be left out. They choose the launch: a step
+    without single tokens is faster with its own ``min_new`` than with 1, which allows for some (512
+    tokens at 8192: 80 us against 128)."""
 
     __slots__ = ("_page_table", "_q_start", "_lens", "_rows", "_max_new", "_max_len", "_min_new",
                  "_requests", "_args")
@@ -309,7 +311,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     ``q`` (T, heads, 128), rotated; query head h reads KV head ``h // (heads / kv_heads)``. The new
     token at position t attends its request's tokens 0 .. t (the pages hold them all: the step's own
-    are appended first); one that has none to attend gives 0. ``scale`` defaults to 1 / sqrt(128).
+    are appended first); one that has none to attend (or scores of -infinity alone) gives 0. ``scale`` defaults to 1 / sqrt(128).
     The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``;
     ``out`` may be q itself, or memory apart from it."""
     fast = _lib.tensor_calls()

@@ -637,7 +637,7 @@ int dkv_gemv_glu(void* stream, int dtype, const void* x, long long x_ld, const v
  * in another way, or whose rows meet each other, is refused, here and below).
  *
  * dkv_paged_attention: q (T, Hq, 128), rotated; the row at position t attends its request's tokens
- * 0 .. t, softmax in fp32; a row with none gives 0; out in dtype or fp32, apart from q, or (in dtype, with
+ * 0 .. t, softmax in fp32; a row with none (or with scores of -infinity alone) gives 0; out in dtype or fp32, apart from q, or (in dtype, with
  * q's strides) q itself. Hq / Hkv <= 16. max_new
  * and max_len bound every request's new tokens and length, min_new (from below) the new tokens of a
  * request that has any: they choose the launch, and what passes them may be left out. The workspace
