@@ -113,6 +113,14 @@ _SIGNATURES = {
     "dkv_paged_attention": (_i, [_vp, _i, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp, _ll, _i,
                                  _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _ll, _vp, _i,
                                  _ll, _ll]),
+    "dkv_paged_append8": (_i, [_vp, _i, _vp, _ll, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp,
+                               _vp, _ll, _ll, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp,
+                               _f, _vp]),
+    "dkv_paged_attention8": (_i, [_vp, _i, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _i, _i, _vp, _vp, _ll,
+                                  _ll, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f,
+                                  _vp, _ll, _vp, _i, _ll, _ll]),
+    "dkv_paged_values": (_i, [_vp, _i, _vp, _vp, _ll, _ll, _i, _i, _i, _i, _vp, _vp, _ll, _ll, _vp,
+                              _i, _vp, _vp]),
     "dkv_sample_workspace_bytes": (_ll, [_i, _i, _i]),
     "dkv_sample_tokens": (_i, [_vp, _i, _vp, _ll, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f,
                                _vp, _ll, _vp]),

@@ -109,6 +109,9 @@ PyMethodDef methods[] = {
     DKV_CALL(dkv_paged_append),
     DKV_CALL(dkv_paged_workspace_floats),
     DKV_CALL(dkv_paged_attention),
+    DKV_CALL(dkv_paged_append8),
+    DKV_CALL(dkv_paged_attention8),
+    DKV_CALL(dkv_paged_values),
     DKV_CALL(dkv_sample_workspace_bytes),
     DKV_CALL(dkv_sample_tokens),
     {nullptr, nullptr, 0, nullptr},

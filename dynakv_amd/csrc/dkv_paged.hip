@@ -1,77 +1,12 @@
 // The paged cache: the append of a step's keys and values, and the attention of its new tokens.
 //
-// A pool of pages holds the keys (and another the values) of requests of different lengths: page
-// j, KV head g, slot s at element j * page_stride + g * head_stride + s * 128, 128 elements each,
-// with page_size slots per page (a power of two from 16 on). Token t of request b is in page
-// table[b][t / page_size], slot t % page_size. A step brings rows q_start[b] .. q_start[b + 1] - 1
-// of request b: its newest tokens, the last of them at position lens[b] - 1.
-//
-// Everything that decides an address is read on the device and checked there: rows outside
-// [0, T), positions outside the table and page ids outside the pool are neither read nor written
-// (an absent key is masked, an absent place is not stored to).
-#include "dkv_common.h"
-#include "dkv_mfma_ops.h"
+// The pool, a step's rows and what is checked of them: dkv_paged.h.
+#include "dkv_paged.h"
 
 #include <mutex>
+#include <type_traits>
 
 namespace {
-
-constexpr int PG_DH = 128;
-
-// x / d for 0 <= x < 2^31, by a product: m = ceil(2^32 / d) gives the quotient or one more.
-struct Divisor {
-  uint32_t d, m;
-};
-Divisor divisor(int d) { return {(uint32_t)d, d > 1 ? (uint32_t)((0x100000000ULL + d - 1) / d) : 0u}; }
-__device__ __forceinline__ int quot(const Divisor& v, int x) {
-  uint32_t q = __umulhi((uint32_t)x, v.m);
-  q -= q * v.d > (uint32_t)x;
-  return v.d == 1 ? x : (int)q;
-}
-
-struct PagedPool {
-  long long page_stride, head_stride;  // elements
-  int num_pages, page_size, page_shift;
-  const int* table;  // (B, cols), row stride ld
-  long long table_ld;
-  int cols;
-};
-
-// One request of the step, clamped to what the buffers hold.
-struct PagedRequest {
-  int row0, n;  // its rows of the step
-  int len;      // keys it attends (the last row's), at most what the table has room for
-  int pos0;     // position of its first row (negative where the lengths do not fit the rows)
-};
-
-__device__ __forceinline__ PagedRequest paged_request(const PagedPool& pool, const int* q_start,
-                                                      const int* lens, int b, int T) {
-  PagedRequest r;
-  const int a = q_start[b], e = q_start[b + 1], len = lens[b];
-  r.row0 = max(a, 0);
-  r.n = min(e, T) - r.row0;
-  r.pos0 = len - (e - a) + (r.row0 - a);
-  const long long room = (long long)pool.cols << pool.page_shift;
-  r.len = (int)min((long long)max(len, 0), room);
-  return r;
-}
-
-// The same in scalar registers, for a request that is the whole wave's.
-__device__ __forceinline__ PagedRequest uniform(PagedRequest r) {
-  r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
-  r.n = __builtin_amdgcn_readfirstlane(r.n);
-  r.len = __builtin_amdgcn_readfirstlane(r.len);
-  r.pos0 = __builtin_amdgcn_readfirstlane(r.pos0);
-  return r;
-}
-
-// The page of token t of request b, or -1 where there is none.
-__device__ __forceinline__ int paged_page(const PagedPool& pool, int b, int t) {
-  const int c = t >> pool.page_shift;
-  if (t < 0 || c >= pool.cols) return -1;
-  const int id = pool.table[(long long)b * pool.table_ld + c];
-  return id >= 0 && id < pool.num_pages ? id : -1;
-}
 
 // ---------------------------------------------------------------------------------------
 // Append: per row of the fused q/k/v projection and head, optionally the RMS norm of the head's
@@ -106,46 +41,6 @@ struct AppendParams {
   double rev[PG_DH / 2];  // revolutions per position of each pair
 };
 
-template <int DT>
-__device__ __forceinline__ void load8(const uint16_t* p, float (&f)[8]) {
-  const dkv_u32x4 v = *(const dkv_u32x4*)p;
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    f[2 * k] = dkv_elt_to_f32<DT>(w[k] & 0xffffu);
-    f[2 * k + 1] = dkv_elt_to_f32<DT>(w[k] >> 16);
-  }
-}
-template <int DT>
-__device__ __forceinline__ dkv_u32x4 round8(const float (&f)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if constexpr (DT == DKV_BF16)
-      w[k] = dkv_f32_to_bf16_bits(f[2 * k]) | (dkv_f32_to_bf16_bits(f[2 * k + 1]) << 16);
-    else
-      w[k] = dkv_f32_to_f16_bits(f[2 * k]) | (dkv_f32_to_f16_bits(f[2 * k + 1]) << 16);
-  }
-  return dkv_u32x4{w[0], w[1], w[2], w[3]};
-}
-
-// The request of row `row`: the last one that starts at or before it (64 starts per step, one per
-// lane), or -1 for a row of no request.
-__device__ __forceinline__ int request_of_row(const int* q_start, int B, int row, int lane) {
-  if (row < q_start[0] || row >= q_start[B]) return -1;
-  int lo = 0, n = B;
-  while (n > 1) {
-    const int step = (n + 63) / 64;
-    const int i = lo + lane * step;
-    const bool at = lane * step < n && q_start[min(i, B - 1)] <= row;
-    const int cnt = max(1, __popcll(__ballot(at)));
-    const int skip = (cnt - 1) * step;
-    lo += skip;
-    n = min(step, n - skip);
-  }
-  return lo;
-}
-
 constexpr int AP_WAVES = 4;
 
 template <int DT>
@@ -164,7 +59,7 @@ __global__ __launch_bounds__(64 * AP_WAVES) void paged_append_kernel(AppendParam
   const int a0 = p.q_start[b], a1 = p.q_start[b + 1];
   const int pos = p.lens[b] - (a1 - a0) + (row - a0);
   if (pos < 0 || h >= heads) return;
-  const uint16_t* src = p.qkv + (long long)row * p.qkv_ld + (long long)h * PG_DH + 8 * c;
+  const uint16_t* src = p.qkv + (long long)row * p.qkv_ld + (long long)h * PG_DH;
   const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
   uint16_t* dst;
   if (is_q) {
@@ -179,41 +74,14 @@ __global__ __launch_bounds__(64 * AP_WAVES) void paged_append_kernel(AppendParam
   }
   if (is_v) {
     if (dst) {
-      *(dkv_u32x4*)(dst + 8 * c) = *(const dkv_u32x4*)src;
-      *(dkv_u32x4*)(dst + 64 + 8 * c) = *(const dkv_u32x4*)(src + 64);
+      *(dkv_u32x4*)(dst + 8 * c) = *(const dkv_u32x4*)(src + 8 * c);
+      *(dkv_u32x4*)(dst + 64 + 8 * c) = *(const dkv_u32x4*)(src + 64 + 8 * c);
     }
     return;
   }
-  float x[8], y[8];
-  load8<DT>(src, x);
-  load8<DT>(src + 64, y);
-  const uint16_t* nw = is_q ? p.q_norm : p.k_norm;
-  if (nw) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
-#pragma unroll
-    for (int o = 1; o <= 4; o <<= 1) ss += __shfl_xor(ss, o, 64);
-    const float inv = 1.0f / sqrtf(ss * (1.0f / PG_DH) + p.eps);
-    float wx[8], wy[8];
-    load8<DT>(nw + 8 * c, wx);
-    load8<DT>(nw + 64 + 8 * c, wy);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = x[e] * inv * wx[e];
-      y[e] = y[e] * inv * wy[e];
-    }
-  }
-  if (!dst) return;
   float ox[8], oy[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const double r = (double)pos * p.rev[8 * c + e];
-    const float f = (float)(r - floor(r));  // part of a revolution: 0 .. 1
-    const float sn = __builtin_amdgcn_sinf(f), cs = __builtin_amdgcn_cosf(f);
-    ox[e] = x[e] * cs - y[e] * sn;
-    oy[e] = y[e] * cs + x[e] * sn;
-  }
+  paged_turn<DT>(src, is_q ? p.q_norm : p.k_norm, p.eps, pos, p.rev, c, ox, oy);
+  if (!dst) return;
   *(dkv_u32x4*)(dst + 8 * c) = round8<DT>(ox);
   *(dkv_u32x4*)(dst + 64 + 8 * c) = round8<DT>(oy);
 }
@@ -245,6 +113,7 @@ struct AttendParams {
   const int* lens;
   void* out;
   long long o_st, o_sh;
+  PagedScales scales;  // of 8-bit pages, whose codes k and v then are
   int B, T, Hq, Hkv, hpg;
   Divisor by_hpg, by_hkv;
   float scale_log2;  // softmax scale * log2(e)
@@ -280,6 +149,12 @@ __device__ __forceinline__ void pg_lds_loads(__amdgpu_buffer_rsrc_t rsrc, uint32
         "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 lds" ::"s"(lds_base),
         "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(rsrc)
         : "memory", "m0");
+  else if constexpr (ONCE)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
+        "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds" ::"s"(lds_base),
+        "v"(off[0]), "v"(off[1]), "s"(rsrc)
+        : "memory", "m0");
   else
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
@@ -294,6 +169,16 @@ __device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
       dkv_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                      (pg_lds_i16x4*)(__attribute__((address_space(3))) uint8_t*)p));
 }
+typedef __attribute__((ext_vector_type(2))) int pg_i32x2;
+typedef __attribute__((address_space(3))) pg_i32x2 pg_lds_i32x2;
+__device__ __forceinline__ dkv_u32x2 pg_read_tr8(const uint8_t* p) {
+  return __builtin_bit_cast(
+      dkv_u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                     (pg_lds_i32x2*)(__attribute__((address_space(3))) uint8_t*)p));
+}
+// The piece of a token's codes that lies at piece i of its 128 bytes of LDS is i ^ swizzle8(token): the
+// pieces of 16 tokens that one read takes lie in all banks.
+__device__ __forceinline__ int swizzle8(int t) { return (t ^ (t >> 3)) & 7; }
 
 // ---- few rows: single tokens, a few drafted ones ----
 //
@@ -315,8 +200,9 @@ __device__ __forceinline__ dkv_u32x2 pg_read_tr(const uint8_t* p) {
 // length: 32 requests of 8192 tokens 159 us (6.7 TB/s, partly from the memory-side cache), 33 of them 226,
 // a second round of workgroups; one of 65536 beside 39 of 500 570 us, beside 20 of 500, in parts, 66.
 constexpr int DSLOT = 2;                    // tile slots per wave
-constexpr int DTILE = 16;
-constexpr int DTILE_BYTES = DTILE * PG_DH * 2;
+template <bool Q8>
+constexpr int DTILE = Q8 ? 32 : 16;
+constexpr int DTILE_BYTES = 16 * PG_DH * 2;
 constexpr int DSLOT_BYTES = 2 * DTILE_BYTES;
 constexpr int DROWS = 16;
 constexpr int DREC = DROWS * (PG_DH + 2);   // floats of a record: m, l and acc[128] of 16 rows
@@ -344,17 +230,19 @@ __device__ __forceinline__ PagedRequest pg_lane(const PagedRequest& r, int l) { 
 }
 
 // Workgroup `wg` of `wgs`, of DW waves; `sRing`: DW * DSLOT * DSLOT_BYTES of LDS, `sLast` an int of it.
-template <int DT, int ODT, int DW>
+template <int DT, int ODT, bool Q8, int DW>
 __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs, uint8_t* sRing,
                                          int* sLast) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
+  constexpr int TILE = DTILE<Q8>;
+  constexpr int BLOCKS = TILE / PG_BLOCK;
 
   // tiles of a request's keys; 0 for one without rows or with too many
   auto tiles_of = [&](const PagedRequest& r) {
     if (r.n <= 0 || r.n * p.hpg > DROWS) return 0;
-    return max(1, (r.len + DTILE - 1) / DTILE);
+    return max(1, (r.len + TILE - 1) / TILE);
   };
   PagedRequest r;
   int b, kvh, part = 0, parts = 1, first = 0;
@@ -449,32 +337,83 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   auto tix = [&](int j) { return t_begin + wave + DW * j; };
 
   uint8_t* ring = sRing + wave * DSLOT * DSLOT_BYTES;
+  // 16-byte pieces of the tokens (16 of 16-bit ones, 8 of codes), XOR-swizzled by the token
   uint32_t piece_off[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int t = 4 * i + (lane >> 4);
-    piece_off[i] = (uint32_t)((lane >> 4) * 256 + 16 * ((lane & 15) ^ t));
-  }
-  int ids = -1;  // lane l: the page of the wave's tile l of the 64 being issued
-  auto issue = [&](int j) {  // the tile's loads; returns its page (scalar)
-    if (j >= n_iter) return -1;
-    if ((j & 63) == 0) {
-      const int t = tix(j + lane);
-      ids = t < t_end ? paged_page(p.pool, b, t * DTILE) : -1;
+    if constexpr (Q8) {
+      const int t = 8 * i + (lane >> 3);
+      piece_off[i] = (uint32_t)((lane >> 3) * PG_DH + 16 * ((lane & 7) ^ swizzle8(t)));
+    } else {
+      const int t = 4 * i + (lane >> 4);
+      piece_off[i] = (uint32_t)((lane >> 4) * 256 + 16 * ((lane & 15) ^ t));
     }
-    const int page = __builtin_amdgcn_readlane(ids, j & 63), tok = tix(j) * DTILE;
-    const long long at = (long long)max(page, 0) * p.pool.page_stride +
-                         (long long)kvh * p.pool.head_stride +
-                         (long long)(tok & (p.pool.page_size - 1)) * PG_DH;
-    const uint32_t bytes = page < 0 ? 0u : (uint32_t)min(r.len - tok, DTILE) * (PG_DH * 2);
-    const __amdgpu_buffer_rsrc_t rk = dkv_make_rsrc(p.k + at, bytes);
-    const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc(p.v + at, bytes);
-    const uint32_t slot = dkv_lds_addr(ring + (j % DSLOT) * DSLOT_BYTES);
-    pg_lds_loads<true>(rk, slot, piece_off);
-    pg_lds_loads<true>(rv, slot + DTILE_BYTES, piece_off);
-    return page;
+  }
+  // Lane l: the page of block l % BLOCKS of the wave's tile l / BLOCKS of the ones being issued; for codes
+  // its scales too, keys' below values' (1 where the block has no token).
+  constexpr int AHEAD_TILES = 64 / BLOCKS;
+  int ids = -1;
+  uint32_t scales = 0x7f7f;
+  auto fetch_ids = [&](int j) {
+    const int t = tix(j + lane / BLOCKS);
+    ids = t < t_end ? paged_page(p.pool, b, t * TILE + lane % BLOCKS * PG_BLOCK) : -1;
   };
-  int page_next = issue(0);
+  auto fetch_scales = [&](int j) {
+    const int tok = tix(j + lane / BLOCKS) * TILE + lane % BLOCKS * PG_BLOCK;
+    scales = 0x7f7f;
+    if (ids >= 0 && tok < r.len) {
+      const long long at = (long long)ids * p.scales.page_stride +
+                           (long long)kvh * p.scales.head_stride +
+                           (tok & (p.pool.page_size - 1)) / PG_BLOCK;
+      scales = p.scales.k[at] | (uint32_t)p.scales.v[at] << 8;
+    }
+  };
+  struct Tile {
+    int page[BLOCKS];
+    uint32_t scales[BLOCKS];
+  };
+  auto tile_of = [&](int j) {
+    Tile t;
+#pragma unroll
+    for (int h = 0; h < BLOCKS; ++h) {
+      t.page[h] = __builtin_amdgcn_readlane(ids, j % AHEAD_TILES * BLOCKS + h);
+      if constexpr (Q8)
+        t.scales[h] = __builtin_amdgcn_readlane(scales, j % AHEAD_TILES * BLOCKS + h);
+    }
+    return t;
+  };
+  auto issue = [&](int j) {  // the tile's loads
+    const int tok0 = tix(j) * TILE;
+    const uint32_t slot = dkv_lds_addr(ring + (j % DSLOT) * DSLOT_BYTES);
+#pragma unroll
+    for (int h = 0; h < BLOCKS; ++h) {
+      const int page = __builtin_amdgcn_readlane(ids, j % AHEAD_TILES * BLOCKS + h);
+      const int tok = tok0 + h * PG_BLOCK;
+      const long long at = (long long)max(page, 0) * p.pool.page_stride +
+                           (long long)kvh * p.pool.head_stride +
+                           (long long)(tok & (p.pool.page_size - 1)) * PG_DH;
+      constexpr int SIZE = Q8 ? 1 : 2;
+      int tokens = min(r.len - tok, PG_BLOCK);
+      if constexpr (Q8)  // (as a scalar instruction: the compiler would clamp in a vector register)
+        asm("s_max_i32 %0, %1, 0" : "=s"(tokens) : "s"(tokens) : "scc");
+      const uint32_t bytes = page < 0 ? 0u : (uint32_t)tokens * (PG_DH * SIZE);
+      const __amdgpu_buffer_rsrc_t rk = dkv_make_rsrc((const uint8_t*)p.k + at * SIZE, bytes);
+      const __amdgpu_buffer_rsrc_t rv = dkv_make_rsrc((const uint8_t*)p.v + at * SIZE, bytes);
+      if constexpr (Q8) {
+        const uint32_t off[2] = {piece_off[2 * h], piece_off[2 * h + 1]};
+        pg_lds_loads<true>(rk, slot + 2048 * h, off);
+        pg_lds_loads<true>(rv, slot + DTILE_BYTES + 2048 * h, off);
+      } else {
+        pg_lds_loads<true>(rk, slot, piece_off);
+        pg_lds_loads<true>(rv, slot + DTILE_BYTES, piece_off);
+      }
+    }
+  };
+  if (n_iter > 0) {
+    fetch_ids(0);
+    issue(0);
+    if constexpr (Q8) fetch_scales(0);
+  }
 
   // query operand: column n = row n (new token n / hpg, head n % hpg; rows past the request's
   // zero), dims 32c + 8g .. +8
@@ -485,12 +424,15 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
                        (long long)(kvh * p.hpg + (has ? n - qi * p.hpg : 0)) * p.q_sh;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const dkv_u32x4 v = *(const dkv_u32x4*)(qr + 32 * c + 8 * g);
+    // (of codes a lane reads 16 bytes at a time, dims 64 (c / 2) + 16 g and on, for two products)
+    const dkv_u32x4 v =
+        *(const dkv_u32x4*)(qr + (Q8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g));
     bq[c] = has ? v : dkv_u32x4{0u, 0u, 0u, 0u};
   }
   // settled here (with tile 0), not inside the loop, where the wait would drain the next tile too
 #pragma unroll
   for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(bq[c]));
+  if constexpr (Q8) asm volatile("" : "+v"(scales));
   const int limit = min(r.pos0 + qi, r.len - 1);  // the row's last key
 
   dkv_f32x4 acc[8];
@@ -498,25 +440,57 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   for (int i = 0; i < 8; ++i) acc[i] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = PG_NO_MAX, l_run = 0.f;  // the row's reference (log2 units) and sum
 
+  Tile next = tile_of(0);
   for (int j = 0; j < n_iter; ++j) {
     pg_wait_vm();
-    const int page = page_next;
-    page_next = issue(j + 1);
+    const Tile tile = next;
+    if (j + 1 < n_iter) {
+      const bool refill = (j + 1) % AHEAD_TILES == 0;
+      if (refill) fetch_ids(j + 1);
+      issue(j + 1);
+      if constexpr (Q8) {
+        if (refill) {
+          fetch_scales(j + 1);
+          asm volatile("" : "+v"(scales));  // (settled here, as the queries)
+        }
+      }
+      next = tile_of(j + 1);
+    }
     const uint8_t* slot = ring + (j % DSLOT) * DSLOT_BYTES;
-    const int key0 = tix(j) * DTILE;
-    dkv_u32x4 xk[4];
+    const int key0 = tix(j) * TILE;
+    // lane (row n, keys 16h + 4g + u): scores in log2 units
+    float z[BLOCKS][4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      xk[c] = *(const dkv_u32x4*)(slot + n * 256 + 16 * ((4 * c + g) ^ n));
-    dkv_f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < BLOCKS; ++h) {
+      dkv_u32x4 xk[4];
+      if constexpr (Q8) {
+        const int t = 16 * h + n;
+        const float s = pg_scale(tile.scales[h] & 0xffu);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) sc = dkv_mfma32<DT>(xk[c], bq[c], sc);
-    // lane (row n, keys 4g + u): scores in log2 units
-    const int last = page < 0 ? -1 : limit - key0 - 4 * g;
-    float z[4];
+        for (int c = 0; c < 2; ++c) {
+          const dkv_u32x4 w =
+              *(const dkv_u32x4*)(slot + t * PG_DH + 16 * ((4 * c + g) ^ swizzle8(t)));
 #pragma unroll
-    for (int u = 0; u < 4; ++u) z[u] = u <= last ? sc[u] * p.scale_log2 : -INFINITY;
-    float tmax = dkv_max3(dkv_max3(z[0], z[1], z[2]), z[3], z[3]);
+          for (int e = 0; e < 2; ++e)
+            xk[2 * c + e] = dkv_u32x4{
+                pg_pair<DT, false>(w[2 * e], s), pg_pair<DT, true>(w[2 * e], s),
+                pg_pair<DT, false>(w[2 * e + 1], s), pg_pair<DT, true>(w[2 * e + 1], s)};
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          xk[c] = *(const dkv_u32x4*)(slot + n * 256 + 16 * ((4 * c + g) ^ n));
+      }
+      dkv_f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sc = dkv_mfma32<DT>(xk[c], bq[c], sc);
+      const int last = tile.page[h] < 0 ? -1 : limit - key0 - 16 * h - 4 * g;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) z[h][u] = u <= last ? sc[u] * p.scale_log2 : -INFINITY;
+    }
+    float tmax = dkv_max3(dkv_max3(z[0][0], z[0][1], z[0][2]), z[0][3], z[0][3]);
+    if constexpr (Q8)
+      tmax = dkv_max3(dkv_max3(z[1][0], z[1][1], z[1][2]), z[1][3], tmax);
     tmax = dkv_lane_max32(tmax);
     tmax = dkv_lane_max16(tmax);
     if (__ballot(tmax > m_run + (PG_BIAS<DT> + D_RESCALE<DT>))) {
@@ -532,53 +506,93 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[i][u] *= au[u];
     }
-    float pu[4];
+    float pu[BLOCKS][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      pu[u] = __builtin_amdgcn_exp2f(z[u] - m_run);
-      l_run += pu[u];
-    }
-    // P.V: A = P (row n; its 16 tokens twice, as hi and lo parts: k = 8g + e is part e / 4 of token
-    // 4g + e % 4), B = V (the token's value, column = dim 16 blk + n) read transposed: lane (n, g)
-    // reads 8 bytes of token 4g + n / 4 and receives tokens 4g .. 4g + 3 of dim 16 blk + n
-    dkv_u32x4 pa;
-    if constexpr (DT == DKV_BF16) {
-      uint32_t h01, h23, l01, l23;
-      dkv_split_bf16x2(pu[0], pu[1], h01, l01);
-      dkv_split_bf16x2(pu[2], pu[3], h23, l23);
-      pa = dkv_u32x4{h01, h23, l01, l23};
-    } else {
-      float lo[4];
+    for (int h = 0; h < BLOCKS; ++h)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) lo[u] = pu[u] - (float)(_Float16)pu[u];
-      pa = dkv_u32x4{dkv_pack_f16x2(pu[0], pu[1]), dkv_pack_f16x2(pu[2], pu[3]),
-                     dkv_pack_f16x2(lo[0], lo[1]), dkv_pack_f16x2(lo[2], lo[3])};
+      for (int u = 0; u < 4; ++u) {
+        pu[h][u] = __builtin_amdgcn_exp2f(z[h][u] - m_run);
+        l_run += pu[h][u];
+      }
+    // P.V. 16-bit values: A = P (row n; its 16 tokens twice, as hi and lo parts: k = 8g + e is part e / 4
+    // of token 4g + e % 4), B = V (the token's value, column = dim 16 blk + n) read transposed: lane
+    // (n, g) reads 8 bytes of token 4g + n / 4 and receives tokens 4g .. 4g + 3 of dim 16 blk + n.
+    // Codes: k = 8g + e is token 4g + e % 4 of the tile's block e / 4, a product with the hi parts and
+    // one with the lo parts; lane (n, g) reads 8 codes of such a token (e = n / 2) and receives the
+    // eight tokens' of dim 16 blk + n.
+    dkv_u32x4 pa[BLOCKS];
+    {
+      dkv_u32x2 hi[BLOCKS], lo[BLOCKS];
+#pragma unroll
+      for (int h = 0; h < BLOCKS; ++h) {
+        if constexpr (DT == DKV_BF16) {
+          uint32_t h01, h23, l01, l23;
+          dkv_split_bf16x2(pu[h][0], pu[h][1], h01, l01);
+          dkv_split_bf16x2(pu[h][2], pu[h][3], h23, l23);
+          hi[h] = dkv_u32x2{h01, h23};
+          lo[h] = dkv_u32x2{l01, l23};
+        } else {
+          float d[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) d[u] = pu[h][u] - (float)(_Float16)pu[h][u];
+          hi[h] = dkv_u32x2{dkv_pack_f16x2(pu[h][0], pu[h][1]), dkv_pack_f16x2(pu[h][2], pu[h][3])};
+          lo[h] = dkv_u32x2{dkv_pack_f16x2(d[0], d[1]), dkv_pack_f16x2(d[2], d[3])};
+        }
+      }
+      if constexpr (Q8) {
+        pa[0] = dkv_u32x4{hi[0].x, hi[0].y, hi[1].x, hi[1].y};
+        pa[1] = dkv_u32x4{lo[0].x, lo[0].y, lo[1].x, lo[1].y};
+      } else {
+        pa[0] = dkv_u32x4{hi[0].x, hi[0].y, lo[0].x, lo[0].y};
+      }
     }
-    const int vtok = 4 * g + (n >> 2);
+    // the products of dims 16 blk .. +15 with the values xv (dwords: as the lane received them)
+    auto values = [&](dkv_u32x2 xv, dkv_f32x4 c) {
+      if constexpr (Q8) {
+        const float s0 = pg_scale(tile.scales[0] >> 8), s1 = pg_scale(tile.scales[1] >> 8);
+        const dkv_u32x4 v = {pg_pair<DT, false>(xv.x, s0), pg_pair<DT, true>(xv.x, s0),
+                             pg_pair<DT, false>(xv.y, s1), pg_pair<DT, true>(xv.y, s1)};
+        return dkv_mfma32<DT>(pa[1], v, dkv_mfma32<DT>(pa[0], v, c));
+      } else {
+        return dkv_mfma32<DT>(pa[0], dkv_u32x4{xv.x, xv.y, xv.x, xv.y}, c);
+      }
+    };
     dkv_u32x2 xv[8];
 #pragma unroll
     for (int blk = 0; blk < 8; ++blk) {
-      const int piece = 2 * blk + ((n & 3) >> 1);
-      xv[blk] = pg_read_tr(slot + DTILE_BYTES + vtok * 256 + 16 * (piece ^ vtok) + 8 * (n & 1));
+      if constexpr (Q8) {
+        const int e = n >> 1, t = 16 * (e >> 2) + 4 * g + (e & 3);
+        xv[blk] = pg_read_tr8(slot + DTILE_BYTES + t * PG_DH + 16 * (blk ^ swizzle8(t)) +
+                              8 * (n & 1));
+      } else {
+        const int vtok = 4 * g + (n >> 2), piece = 2 * blk + ((n & 3) >> 1);
+        xv[blk] = pg_read_tr(slot + DTILE_BYTES + vtok * 256 + 16 * (piece ^ vtok) + 8 * (n & 1));
+      }
     }
-    if (key0 + DTILE - 1 <= r.pos0 || r.n == 1) {
+    if (key0 + TILE - 1 <= r.pos0 || r.n == 1) {
 #pragma unroll
-      for (int blk = 0; blk < 8; ++blk)
-        acc[blk] = dkv_mfma32<DT>(pa, dkv_u32x4{xv[blk].x, xv[blk].y, xv[blk].x, xv[blk].y},
-                                  acc[blk]);
+      for (int blk = 0; blk < 8; ++blk) acc[blk] = values(xv[blk], acc[blk]);
     } else {
       // Keys that some of the rows attend and others do not (they come after them): a product per
       // new token with the later keys' values cleared, of which its own rows are taken, so that an
       // infinity or NaN there, whose weight is 0, stays out of the rows before it.
       for (int i = 0; i < r.n; ++i) {
         const int cut = r.pos0 + i - key0 - 4 * g;  // the token's last key, from this lane's first
-        const uint32_t m0 = (cut >= 0 ? 0xffffu : 0u) | (cut >= 1 ? 0xffff0000u : 0u);
-        const uint32_t m1 = (cut >= 2 ? 0xffffu : 0u) | (cut >= 3 ? 0xffff0000u : 0u);
+        uint32_t m0, m1;
+        if constexpr (Q8) {
+          auto first = [](int k) {  // the first k + 1 of four codes
+            return k < 0 ? 0u : 0xffffffffu >> (8 * (3 - min(k, 3)));
+          };
+          m0 = first(cut);
+          m1 = first(cut - 16);
+        } else {
+          m0 = (cut >= 0 ? 0xffffu : 0u) | (cut >= 1 ? 0xffff0000u : 0u);
+          m1 = (cut >= 2 ? 0xffffu : 0u) | (cut >= 3 ? 0xffff0000u : 0u);
+        }
 #pragma unroll
         for (int blk = 0; blk < 8; ++blk) {
-          const uint32_t v0 = xv[blk].x & m0, v1 = xv[blk].y & m1;
-          const dkv_f32x4 o = dkv_mfma32<DT>(pa, dkv_u32x4{v0, v1, v0, v1},
-                                             dkv_f32x4{0.f, 0.f, 0.f, 0.f});
+          const dkv_f32x4 o =
+              values(dkv_u32x2{xv[blk].x & m0, xv[blk].y & m1}, dkv_f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int x = 4 * g + u - i * p.hpg;
@@ -703,11 +717,11 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   if (tid == 0) p.counters[b * p.Hkv + kvh] = 0;
 }
 
-template <int DT, int ODT>
+template <int DT, int ODT, bool Q8>
 __global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
   __shared__ __attribute__((aligned(256))) uint8_t sRing[8 * DSLOT * DSLOT_BYTES];
   __shared__ int sLast;
-  few_rows<DT, ODT, 8>(p, blockIdx.x, gridDim.x, sRing, &sLast);
+  few_rows<DT, ODT, Q8, 8>(p, blockIdx.x, gridDim.x, sRing, &sLast);
 }
 
 // ---- many rows: prompts and their chunks ----
@@ -824,7 +838,7 @@ __device__ __forceinline__ float pg_max4(float x) {  // over lanes n, n + 16, n 
 // a masked key is not touched. Lane l returns dims 2l, 2l + 1. Slow, and for every row that attends such
 // a value: one NaN in the first value of a KV head makes 512 tokens at 8192 take 16 ms (80 us without), a
 // prompt of 2048 8.8 ms (59 us).
-template <int DT>
+template <int DT, bool Q8>
 __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, int kvh,
                                               const uint16_t* qr, int k0, int k1, int lane,
                                               float& m, float& l, float& o0, float& o1) {
@@ -836,12 +850,24 @@ __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, i
     const long long at = (long long)max(page, 0) * p.pool.page_stride +
                          (long long)kvh * p.pool.head_stride +
                          (long long)(key & (p.pool.page_size - 1)) * PG_DH;
-    float s = -INFINITY;
+    float s = -INFINITY, by_k = 1.f, by_v = 1.f;
+    if constexpr (Q8) {
+      if (page >= 0) {
+        const long long sa = (long long)page * p.scales.page_stride +
+                             (long long)kvh * p.scales.head_stride +
+                             (key & (p.pool.page_size - 1)) / PG_BLOCK;
+        by_k = pg_scale(p.scales.k[sa]);
+        by_v = pg_scale(p.scales.v[sa]);
+      }
+    }
     if (page >= 0) {
       s = 0.f;
       for (int d = 0; d < PG_DH; d += 8) {
         float kv[8], qv[8];
-        load8<DT>(p.k + at + d, kv);
+        if constexpr (Q8)
+          pg_codes8((const uint8_t*)p.k + at + d, by_k, kv);
+        else
+          load8<DT>(p.k + at + d, kv);
         load8<DT>(qr + d, qv);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s = fmaf(qv[e], kv[e], s);
@@ -858,15 +884,22 @@ __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, i
       if (__builtin_amdgcn_readlane(page, j) < 0) continue;
       const float wj = __shfl(w, j, 64);
       const long long vj = __shfl(at, j, 64);
-      o0 = fmaf(wj, dkv_load_f32<DT>(p.v + vj, 2 * lane), o0);
-      o1 = fmaf(wj, dkv_load_f32<DT>(p.v + vj, 2 * lane + 1), o1);
+      if constexpr (Q8) {
+        const float by = __shfl(by_v, j, 64);
+        const uint32_t w = *(const uint16_t*)((const uint8_t*)p.v + vj + 2 * lane);
+        o0 = fmaf(wj, __builtin_amdgcn_cvt_f32_fp8(w, 0) * by, o0);
+        o1 = fmaf(wj, __builtin_amdgcn_cvt_f32_fp8(w, 1) * by, o1);
+      } else {
+        o0 = fmaf(wj, dkv_load_f32<DT>(p.v + vj, 2 * lane), o0);
+        o1 = fmaf(wj, dkv_load_f32<DT>(p.v + vj, 2 * lane + 1), o1);
+      }
     }
   }
 }
 
 // Workgroup `wg`; `sKV`: 4 * CTILE_BYTES of LDS, 1 KB aligned (the operand reads form their
 // addresses by exclusive-or): two K tiles, two V tiles.
-template <int DT, int ODT, int QB, int NW>
+template <int DT, int ODT, bool Q8, int QB, int NW>
 __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t* sKV) {
   constexpr int QW = 16 * QB;            // rows per wave
   constexpr int BQ = NW * QW;            // rows per workgroup
@@ -929,7 +962,22 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   auto absent_of = [&](int tb) {
     return __ballot(ids < 0 && (tb * 4 + lane) * 16 < k_end);
   };
-  unsigned long long absent = absent_of(t0);
+  unsigned long long absent = absent_of(t0), absent_next = 0;
+
+  // scales of codes, as the pages: keys' below values' (1 where the block has no key)
+  uint32_t scales = 0x7f7f, scales_next = 0x7f7f;
+  auto fetch_scales = [&](int tb, int page) {
+    const int key = (tb * 4 + lane) * 16;
+    uint32_t s = 0x7f7f;
+    if (page >= 0 && key < r.len) {
+      const long long at = (long long)page * p.scales.page_stride +
+                           (long long)kvh * p.scales.head_stride +
+                           (key & (p.pool.page_size - 1)) / PG_BLOCK;
+      s = p.scales.k[at] | (uint32_t)p.scales.v[at] << 8;
+    }
+    return s;
+  };
+  if constexpr (Q8) scales = fetch_scales(t0, ids);
 
   // tile loads: wave w, instruction i stores keys 64 / NW * w + 4 i + lane / 16 of the tile, LDS piece
   // lane % 16, which holds the key's 16-byte piece (lane % 16) ^ (key % 16)
@@ -958,6 +1006,48 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
                         dkv_lds_addr(sV(t & 1)) + CK / NW * wave * 256, voff);
   };
 
+  // Codes go through registers: a wave's part of a tile is fetched (two loads of 16 codes a lane, or one)
+  // while the tile before it is worked on, and stored to LDS as the 16-bit numbers that codes times scale
+  // are, where the products find them as they would a 16-bit cache's.
+  constexpr int CW = (LW + 1) / 2;
+  dkv_u32x4 ck[CW], cv[CW];
+  uint32_t c_scales = 0x7f7f;
+  auto fetch = [&](int t, int page, uint32_t s) {
+    const int key = t * CK + key_in_tile;
+    const long long at = (long long)max(page, 0) * p.pool.page_stride +
+                         (long long)((key & slot_mask) * PG_DH);
+    const int keys = min(max(k_end - key, 0), CK / NW);
+    const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys * PG_DH;
+    const __amdgpu_buffer_rsrc_t rk =
+        dkv_make_rsrc((const uint8_t*)p.k + (long long)kvh * p.pool.head_stride + at, bytes);
+    const __amdgpu_buffer_rsrc_t rv =
+        dkv_make_rsrc((const uint8_t*)p.v + (long long)kvh * p.pool.head_stride + at, bytes);
+    c_scales = s;
+#pragma unroll
+    for (int i = 0; i < CW; ++i) {
+      ck[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, 1024 * i + 16 * lane, 0, 0);
+      cv[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, 1024 * i + 16 * lane, 0, 0);
+    }
+  };
+  auto place = [&](int t) {  // the fetched part, into tile t's buffers
+    const float sk = pg_scale(c_scales & 0xffu), sv = pg_scale(c_scales >> 8);
+#pragma unroll
+    for (int i = 0; i < CW; ++i) {
+      const int kk = sub + 8 * i + (lane >> 3);  // key of the block
+      const uint32_t row = (uint32_t)(blk * 16 + kk) * 256;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t to = row + 16 * ((2 * (lane & 7) + e) ^ kk);
+        auto wide = [&](const dkv_u32x4& w, float s) {
+          return dkv_u32x4{pg_pair<DT, false>(w[2 * e], s), pg_pair<DT, true>(w[2 * e], s),
+                           pg_pair<DT, false>(w[2 * e + 1], s), pg_pair<DT, true>(w[2 * e + 1], s)};
+        };
+        *(dkv_u32x4*)(sK(t & 1) + to) = wide(ck[i], sk);
+        *(dkv_u32x4*)(sV(t & 1) + to) = wide(cv[i], sv);
+      }
+    }
+  };
+
   dkv_f32x4 acc[QB][8];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb)
@@ -984,7 +1074,17 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const uint32_t vrd =
       (4 * g + (n >> 2)) * 256 + 16 * (((n & 3) >> 1) ^ (4 * g + (n >> 2))) + 8 * (n & 1);
 
-  if (t0 < n_tiles) issue(t0, __builtin_amdgcn_readlane(ids, blk));
+  if constexpr (Q8) {
+    if (t0 < n_tiles) {
+      fetch(t0, __builtin_amdgcn_readlane(ids, blk), __builtin_amdgcn_readlane(scales, blk));
+      place(t0);
+    }
+    if (t0 + 1 < n_tiles)
+      fetch(t0 + 1, __builtin_amdgcn_readlane(ids, 4 + blk),
+            __builtin_amdgcn_readlane(scales, 4 + blk));
+  } else {
+    if (t0 < n_tiles) issue(t0, __builtin_amdgcn_readlane(ids, blk));
+  }
   // settled here, not inside the loop, where the compiler's waits for them would be waits for the next
   // tile, which it does not know of
 #pragma unroll
@@ -992,9 +1092,31 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
 #pragma unroll
     for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(qop[qb][s]));
   for (int t = t0; t < n_tiles; ++t) {
-    pg_wait_vm();
+    if constexpr (!Q8) pg_wait_vm();
     __syncthreads();  // tile t is in LDS for every wave; tile t - 1's buffer is free
-    const uint32_t gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
+    uint32_t gone;
+    if constexpr (Q8) {
+      if (t == ids_base + 16) {
+        ids_base += 16;
+        absent = absent_next;
+      }
+      gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
+      if (t + 1 < n_tiles) place(t + 1);
+      if (t + 2 < n_tiles) {
+        // (pages and scales of the next 16 tiles, two tiles before the products are at them)
+        const int u = t + 2 - t0;
+        if ((u & 15) == 0) {
+          ids = ids_next;
+          scales = scales_next;
+          absent_next = absent_of(t + 2);
+          if (t + 2 + 16 < n_tiles) ids_next = fetch_ids(t + 2 + 16);
+        }
+        if ((u & 15) == 8 && t + 2 + 8 < n_tiles) scales_next = fetch_scales(t + 2 + 8, ids_next);
+        fetch(t + 2, __builtin_amdgcn_readlane(ids, 4 * (u & 15) + blk),
+              __builtin_amdgcn_readlane(scales, 4 * (u & 15) + blk));
+      }
+    } else {
+    gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
     if (t + 1 < n_tiles) {
       if (t + 1 == ids_base + 16) {
         ids_base += 16;
@@ -1003,6 +1125,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         if (ids_base + 16 < n_tiles) ids_next = fetch_ids(ids_base + 16);
       }
       issue(t + 1, __builtin_amdgcn_readlane(ids, 4 * (t + 1 - ids_base) + blk));
+    }
     }
     const int key0 = t * CK;
     if (key0 >= w_end) continue;  // every key of the tile is past the wave's rows
@@ -1158,7 +1281,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       const uint16_t* qx = p.q + (long long)(r.row0 + ix) * p.q_st +
                            (long long)(kvh * p.hpg + hx) * p.q_sh;
       float mx, lx, o0, o1;
-      attend_row_apart<DT>(p, b, kvh, qx, t0 * CK, min(n_tiles * CK, min(r.pos0 + ix + 1, r.len)),
+      attend_row_apart<DT, Q8>(p, b, kvh, qx, t0 * CK, min(n_tiles * CK, min(r.pos0 + ix + 1, r.len)),
                            lane, mx, lx, o0, o1);
       if (splits == 1) {
         const float inv = lx > 0.f ? 1.f / lx : (lx == 0.f ? 0.f : lx);
@@ -1175,16 +1298,16 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   }
 }
 
-template <int DT, int ODT, int QB, int NW>
+template <int DT, int ODT, bool Q8, int QB, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : 2) void paged_chunk_kernel(ChunkParams c) {
   __shared__ __attribute__((aligned(1024))) uint8_t sKV[4 * CTILE_BYTES];
-  many_rows<DT, ODT, QB, NW>(c, blockIdx.x, sKV);
+  many_rows<DT, ODT, Q8, QB, NW>(c, blockIdx.x, sKV);
 }
 
 // Both kinds of requests in one launch: the ones of few rows, bound by memory, beside the others,
 // bound by their products. Workgroups of the two kinds are handed out in turn, so that a CU has one of
 // each.
-template <int DT, int ODT, int QB>
+template <int DT, int ODT, bool Q8, int QB>
 __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(ChunkParams c, int few, int many) {
   static_assert(4 * DSLOT * DSLOT_BYTES <= 4 * CTILE_BYTES, "one workgroup shape");
   __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * CTILE_BYTES];
@@ -1192,9 +1315,9 @@ __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(ChunkParams c, int 
   const int x = blockIdx.x, both = 2 * min(few, many);
   const int i = x < both ? x >> 1 : x - both / 2;
   if (x < both ? (x & 1) == 0 : few > many)
-    few_rows<DT, ODT, 4>(c.a, i, few, smem, &sLast);
+    few_rows<DT, ODT, Q8, 4>(c.a, i, few, smem, &sLast);
   else
-    many_rows<DT, ODT, QB, 4>(c, i, smem);
+    many_rows<DT, ODT, Q8, QB, 4>(c, i, smem);
 }
 
 // The key ranges' records of a row joined: 32 rows per workgroup, 8 threads of 16 dims each.
@@ -1240,68 +1363,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(ChunkParams c) {
     else
       store4<ODT, false>(p, ob + 32 * q, a[q] * inv);
   }
-}
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-// T x H segments of `len` bytes, segment (i, h) at `at` + i st + h sh; a stride of a size of one is any.
-struct Segments {
-  long long at, st, sh, len;
-  int T, H;
-  long long end() const { return at + (T - 1) * st + (H - 1) * sh + len; }
-};
-// Whether a segment of a and one of b, of the same strides, have a byte in common (of one array with
-// itself: two of its segments).
-bool segments_meet(const Segments& a, const Segments& b, bool itself = false) {
-  const long long st = a.T > 1 ? a.st : 0;
-  for (int dh = 1 - a.H; dh < b.H; ++dh) {
-    // the least di for which b's segment ends behind the start of a's
-    const long long x = b.at - a.at + dh * b.sh;
-    long long di = 1 - a.T;
-    if (st > 0 && x + di * st + b.len <= 0) di += (-b.len - x - di * st) / st + 1;
-    if (itself && dh == 0 && di <= 0) di = 1;
-    if (di < a.T && x + di * st + b.len > 0 && x + di * st < a.len) return true;
-  }
-  return false;
-}
-// Whether an output's rows may be written while an operator reads `in`: apart from it (or, with its
-// strides, between its rows), or in its place, row for row; no two of them on top of each other.
-bool output_apart(const Segments& out, const Segments& in, bool in_place) {
-  const bool nested =  // (the usual layouts: rows of heads, or heads of rows)
-      (out.sh >= out.len && (out.T == 1 || out.st >= (out.H - 1) * out.sh + out.len)) ||
-      (out.st >= out.len && (out.H == 1 || out.sh >= (out.T - 1) * out.st + out.len));
-  if (!nested && segments_meet(out, out, true)) return false;
-  if (in_place || out.end() <= in.at || in.end() <= out.at) return true;
-  const bool alike = (out.T == 1 || out.st == in.st) &&
-                     ((out.H == 1 && in.H == 1) || (out.H == in.H ? out.sh == in.sh : in.H == 1));
-  if (alike && out.H == in.H) return !segments_meet(in, out);
-  if (!alike) return false;
-  for (int h = 0; h < out.H; ++h) {
-    const Segments one = {out.at + h * out.sh, out.st, 0, out.len, out.T, 1};
-    if (segments_meet(in, one)) return false;
-  }
-  return true;
-}
-
-int fill_pool(PagedPool& pool, long long page_stride, long long head_stride, int num_pages,
-              int page_size, const int* table, long long table_ld, int cols, int Hkv) {
-  if (num_pages < 0 || cols < 0 || table_ld < cols) return DKV_E_ARG;
-  if (page_size < 16 || (page_size & (page_size - 1))) return DKV_E_UNSUPPORTED;
-  if (head_stride < (long long)page_size * PG_DH && Hkv > 1) return DKV_E_ARG;
-  if (page_stride < 0 || head_stride < 0) return DKV_E_ARG;
-  if ((page_stride & 7) || (head_stride & 7)) return DKV_E_UNSUPPORTED;
-  if (page_stride < (long long)page_size * PG_DH && num_pages > 1) return DKV_E_ARG;
-  if (cols > 0 && !table) return DKV_E_ARG;
-  if ((long long)cols * page_size > 0x7fffffffLL - 4096) return DKV_E_UNSUPPORTED;
-  pool.page_stride = page_stride;
-  pool.head_stride = head_stride;
-  pool.num_pages = num_pages;
-  pool.page_size = page_size;
-  pool.page_shift = __builtin_ctz((unsigned)page_size);
-  pool.table = table;
-  pool.table_ld = table_ld;
-  pool.cols = cols;
-  return DKV_OK;
 }
 
 }  // namespace
@@ -1393,7 +1454,8 @@ struct AttendPlan {
 //  * otherwise one range: above 256 of 128 rows 1x8 (eight 300-token prompts 22.7, against 23.5 1x4,
 //    25.5 2x4), else 1x4 (512 tokens at 1024: 20.1, against 24.4 1x8 and 29 2x4/2: a range more
 //    costs its records, 66 KB a workgroup, written and read).
-AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, int max_len) {
+AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, int max_len,
+                       bool q8) {
   AttendPlan a = {};
   const int hpg = Hq / Hkv;
   const long long units = (long long)B * Hkv;
@@ -1401,7 +1463,8 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
   long long floats = 0;
   a.many = (long long)max_new * hpg > DROWS;
   if (a.few) {
-    const long long tiles = ((long long)max_len + DTILE - 1) / DTILE;
+    const int tile = q8 ? DTILE<true> : DTILE<false>;
+    const long long tiles = ((long long)max_len + tile - 1) / tile;
     const long long most = units * ((tiles + D_MIN_TILES - 1) / D_MIN_TILES);
     long long wgs = units;
     if (wgs < D_WGS) wgs = most < D_WGS ? (most > units ? most : units) : D_WGS;
@@ -1467,7 +1530,7 @@ std::mutex& launch_lock(const void* workspace) {
   return locks[((uintptr_t)workspace >> 9) % 16];
 }
 
-template <int DT, int ODT>
+template <int DT, int ODT, bool Q8>
 void launch_attend(const AttendPlan& a, const ChunkParams& c, hipStream_t st) {
   const int many = (a.items * a.splits + a.more) * c.a.Hkv;
   std::unique_lock<std::mutex> together(launch_lock(c.a.counters), std::defer_lock);
@@ -1475,21 +1538,21 @@ void launch_attend(const AttendPlan& a, const ChunkParams& c, hipStream_t st) {
   if (a.few && a.many) {
     const dim3 grid((unsigned)(a.few_wgs + many));
     if (a.qb == 2)
-      hipLaunchKernelGGL((paged_mixed_kernel<DT, ODT, 2>), grid, dim3(256), 0, st, c, a.few_wgs,
+      hipLaunchKernelGGL((paged_mixed_kernel<DT, ODT, Q8, 2>), grid, dim3(256), 0, st, c, a.few_wgs,
                          many);
     else
-      hipLaunchKernelGGL((paged_mixed_kernel<DT, ODT, 1>), grid, dim3(256), 0, st, c, a.few_wgs,
+      hipLaunchKernelGGL((paged_mixed_kernel<DT, ODT, Q8, 1>), grid, dim3(256), 0, st, c, a.few_wgs,
                          many);
   } else if (a.few) {
-    hipLaunchKernelGGL((paged_few_kernel<DT, ODT>), dim3((unsigned)a.few_wgs), dim3(512), 0, st, c.a);
+    hipLaunchKernelGGL((paged_few_kernel<DT, ODT, Q8>), dim3((unsigned)a.few_wgs), dim3(512), 0, st, c.a);
   } else {
     const dim3 grid((unsigned)many);
     if (a.qb == 2)
-      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 2, 4>), grid, dim3(256), 0, st, c);
+      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, Q8, 2, 4>), grid, dim3(256), 0, st, c);
     else if (a.nw == 8)
-      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 8>), grid, dim3(512), 0, st, c);
+      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, Q8, 1, 8>), grid, dim3(512), 0, st, c);
     else
-      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, 1, 4>), grid, dim3(256), 0, st, c);
+      hipLaunchKernelGGL((paged_chunk_kernel<DT, ODT, Q8, 1, 4>), grid, dim3(256), 0, st, c);
   }
   if (a.many && a.splits > 1)
     hipLaunchKernelGGL((paged_join_kernel<DT, ODT>),
@@ -1510,18 +1573,22 @@ extern "C" long long dkv_paged_workspace_floats(int B, int T, int Hq, int Hkv, i
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_new <= 0 || max_len < 0)
     return 0;
   if (!attend_sizes_ok(B, T, Hq, Hkv, max_new)) return 0;
-  return attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len).floats;
+  // (for either kind of pages)
+  const long long a = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len, false).floats;
+  const long long c = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len, true).floats;
+  return a > c ? a : c;
 }
 
-extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st,
-                                   long long q_sh, const void* k_pages, const void* v_pages,
-                                   long long page_stride, long long head_stride, int num_pages,
-                                   int page_size, const int* page_table, long long table_ld,
-                                   int table_cols, const int* q_start, const int* lens, int B,
-                                   int T, int Hq, int Hkv, int Dh, int max_new, int min_new,
-                                   int max_len, float scale, float* workspace,
-                                   long long workspace_floats, void* out, int out_dtype,
-                                   long long o_st, long long o_sh) {
+namespace {
+
+// The attention over 16-bit pages, or (with scales) over 8-bit ones.
+int attention(void* stream, int dtype, const void* q, long long q_st, long long q_sh,
+              const void* k_pages, const void* v_pages, long long page_stride, long long head_stride,
+              int num_pages, int page_size, const PagedScales* scales, const int* page_table,
+              long long table_ld, int table_cols, const int* q_start, const int* lens, int B, int T,
+              int Hq, int Hkv, int Dh, int max_new, int min_new, int max_len, float scale,
+              float* workspace, long long workspace_floats, void* out, int out_dtype, long long o_st,
+              long long o_sh) {
   if (!(scale > 0.f) || !(scale * 1.4426950408889634f < INFINITY)) return DKV_E_UNSUPPORTED;
   if (dtype != DKV_F16 && dtype != DKV_BF16) return DKV_E_UNSUPPORTED;
   if (out_dtype != dtype && out_dtype != DKV_F32) return DKV_E_ARG;
@@ -1531,7 +1598,7 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   ChunkParams c;
   AttendParams& p = c.a;
   const int rc = fill_pool(p.pool, page_stride, head_stride, num_pages, page_size, page_table,
-                           table_ld, table_cols, Hkv);
+                           table_ld, table_cols, Hkv, scales ? 16 : 8);
   if (rc != DKV_OK) return rc;
   if (B == 0 || T == 0 || max_new == 0) return DKV_OK;
   if (!q || !k_pages || !v_pages || !q_start || !lens || !out || num_pages == 0) return DKV_E_ARG;
@@ -1545,7 +1612,11 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || (q_st & 7) || (q_sh & 7))
     return DKV_E_UNSUPPORTED;
   if (!attend_sizes_ok(B, T, Hq, Hkv, max_new)) return DKV_E_UNSUPPORTED;
-  const AttendPlan plan = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len);
+  if (scales) {
+    const int rs = check_scales(*scales, num_pages, page_size, Hkv);
+    if (rs != DKV_OK) return rs;
+  }
+  const AttendPlan plan = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len, scales != nullptr);
   if (!aligned16(workspace)) return DKV_E_UNSUPPORTED;
   if (plan.floats > 0 && (!workspace || workspace_floats < plan.floats)) return DKV_E_WORKSPACE;
   p.q = (const uint16_t*)q;
@@ -1553,6 +1624,7 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   p.q_sh = q_sh;
   p.k = (const uint16_t*)k_pages;
   p.v = (const uint16_t*)v_pages;
+  p.scales = scales ? *scales : PagedScales{nullptr, nullptr, 0, 0};
   p.q_start = q_start;
   p.lens = lens;
   p.out = out;
@@ -1580,17 +1652,61 @@ extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long 
   c.by_splits = divisor(plan.many ? plan.splits : 1);
   c.few_rows = plan.few ? DROWS : 0;
   hipStream_t st = (hipStream_t)stream;
+  auto launch = [&](auto dt, auto odt) {
+    if (scales)
+      launch_attend<decltype(dt)::value, decltype(odt)::value, true>(plan, c, st);
+    else
+      launch_attend<decltype(dt)::value, decltype(odt)::value, false>(plan, c, st);
+  };
+  using BF16 = std::integral_constant<int, DKV_BF16>;
+  using F16 = std::integral_constant<int, DKV_F16>;
+  using F32 = std::integral_constant<int, DKV_F32>;
   if (dtype == DKV_BF16) {
     if (out_dtype == DKV_F32)
-      launch_attend<DKV_BF16, DKV_F32>(plan, c, st);
+      launch(BF16{}, F32{});
     else
-      launch_attend<DKV_BF16, DKV_BF16>(plan, c, st);
+      launch(BF16{}, BF16{});
   } else {
     if (out_dtype == DKV_F32)
-      launch_attend<DKV_F16, DKV_F32>(plan, c, st);
+      launch(F16{}, F32{});
     else
-      launch_attend<DKV_F16, DKV_F16>(plan, c, st);
+      launch(F16{}, F16{});
   }
   DKV_HIP_CHECK_LAUNCH();
   return DKV_OK;
+}
+
+}  // namespace
+
+extern "C" int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st,
+                                   long long q_sh, const void* k_pages, const void* v_pages,
+                                   long long page_stride, long long head_stride, int num_pages,
+                                   int page_size, const int* page_table, long long table_ld,
+                                   int table_cols, const int* q_start, const int* lens, int B,
+                                   int T, int Hq, int Hkv, int Dh, int max_new, int min_new,
+                                   int max_len, float scale, float* workspace,
+                                   long long workspace_floats, void* out, int out_dtype,
+                                   long long o_st, long long o_sh) {
+  return attention(stream, dtype, q, q_st, q_sh, k_pages, v_pages, page_stride, head_stride,
+                   num_pages, page_size, nullptr, page_table, table_ld, table_cols, q_start, lens, B,
+                   T, Hq, Hkv, Dh, max_new, min_new, max_len, scale, workspace, workspace_floats, out,
+                   out_dtype, o_st, o_sh);
+}
+
+extern "C" int dkv_paged_attention8(void* stream, int dtype, const void* q, long long q_st,
+                                    long long q_sh, const void* k_pages, const void* v_pages,
+                                    long long page_stride, long long head_stride, int num_pages,
+                                    int page_size, const void* k_scale, const void* v_scale,
+                                    long long scale_page_stride, long long scale_head_stride,
+                                    const int* page_table, long long table_ld, int table_cols,
+                                    const int* q_start, const int* lens, int B, int T, int Hq, int Hkv,
+                                    int Dh, int max_new, int min_new, int max_len, float scale,
+                                    float* workspace, long long workspace_floats, void* out,
+                                    int out_dtype, long long o_st, long long o_sh) {
+  const PagedScales scales = {(const uint8_t*)k_scale, (const uint8_t*)v_scale, scale_page_stride,
+                              scale_head_stride};
+  return attention(stream, dtype, q, q_st, q_sh, k_pages, v_pages, page_stride, head_stride,
+                   num_pages, page_size, &scales, page_table, table_ld, table_cols, q_start, lens, B,
+                   T, Hq, Hkv, Dh, max_new, min_new, max_len, scale, workspace, workspace_floats, out,
+                   out_dtype, o_st, o_sh);
 }

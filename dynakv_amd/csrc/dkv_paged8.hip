@@ -1,0 +1,570 @@
+// Pages of 8 bits: the append of a step's keys and values to them, and pages read back as values.
+// The layout of codes and scales: dkv_paged.h. The attention over them: dkv_paged.hip.
+#include "dkv_paged.h"
+
+namespace {
+
+constexpr float E4M3_MAX = 448.f;
+// Exponents a block may get: those for which every code times 2^e is a number of the model's type (in
+// bf16 a normal one), so that the attention reads exactly what was stored.
+template <int DT>
+constexpr int E_LOW = DT == DKV_F16 ? -15 : -110;
+template <int DT>
+constexpr int E_HIGH = DT == DKV_F16 ? 7 : 119;
+
+// ---------------------------------------------------------------------------------------
+// Append to 8-bit pages. Queries as in the 16-bit append. Keys y (normed, rotated) and values y of one
+// block (16 tokens, one head) get one exponent
+//   e = least with max |y| <= 448 2^e, within E_LOW .. E_HIGH, and at least the block's old one where it
+//       holds earlier tokens of the request (its first slots), whose codes are then rounded again,
+//   c = y / 2^e rounded to the nearest e4m3 (ties to even), at most 448.
+// Scales are powers of two: a code moved to a larger one only loses what falls below 2^-9 of it, so
+// tokens that come one by one are held as those that come at once are, but for a last bit down there;
+// a value's relative error is that of e4m3 (2^-4) from 2^-15 of the block's largest on. Values that
+// are infinite or NaN are held as NaN and have no say in e.
+//
+// Keys are computed in 64 bits: which code a value gets turns over at borders, and 32-bit arithmetic with
+// the sine instruction put 350 of 8 million keys on another side of one.
+//
+// A wave has one block and head: lane (token i = lane / 8 of eight, twice; piece c = lane % 8) holds dims
+// 8c .. 8c + 7 and 64 + 8c .. 64 + 8c + 7. Eight waves (K heads, then V heads) share the block's sines and
+// cosines in LDS. Queries go to further workgroups of the launch, a wave per row and 8 heads.
+// ---------------------------------------------------------------------------------------
+struct Append8Params {
+  const uint16_t* qkv;
+  long long qkv_ld;
+  uint16_t* q_out;
+  long long q_st, q_sh;
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  long long scale_page, scale_head;  // strides of the scales
+  PagedPool pool;
+  const int* q_start;
+  const int* lens;
+  int B, T, Hq, Hkv;
+  int kv_wgs;      // leading workgroups: blocks times groups of eight units
+  Divisor by_groups, by_q_groups;
+  const uint16_t* q_norm;  // (128,), or null: no norm
+  const uint16_t* k_norm;
+  float eps;
+  double rev[PG_DH / 2];  // revolutions per position of each pair
+};
+
+constexpr int A8_WAVES = 8;
+constexpr int A8_ROW = 72;  // pairs of doubles a token's sines and cosines take in LDS
+
+// A block with new tokens: tokens t_lo .. t_hi - 1 of request b, all in block [base, base + 16).
+struct NewBlock {
+  int b;  // < 0: none
+  int base, t_lo, t_hi;
+  int row_of_0;  // row of token t: row_of_0 + t
+};
+// The item-th block with new tokens, request by request.
+__device__ __forceinline__ NewBlock new_block(const Append8Params& p, int item, int lane) {
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    int count = 0, lo = 0, hi = 0, off = 0;
+    if (b0 + lane < p.B) {
+      const PagedRequest r = paged_request(p.pool, p.q_start, p.lens, b0 + lane, p.T);
+      lo = max(r.pos0, 0);
+      hi = (int)min((long long)r.pos0 + r.n, (long long)p.pool.cols << p.pool.page_shift);
+      off = r.row0 - r.pos0;
+      if (r.n > 0 && hi > lo) count = (hi - 1) / PG_BLOCK - lo / PG_BLOCK + 1;
+    }
+    int run = count;  // inclusive scan
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(run, o, 64);
+      if (lane >= o) run += x;
+    }
+    const unsigned long long hit = __ballot(item < before + run);
+    if (hit) {
+      const int l = __ffsll((long long)hit) - 1;
+      NewBlock n;
+      n.b = b0 + l;
+      const int first = __builtin_amdgcn_readlane(lo, l);
+      const int j = item - before - __builtin_amdgcn_readlane(run - count, l);
+      n.base = (first / PG_BLOCK + j) * PG_BLOCK;
+      n.t_lo = max(first, n.base);
+      n.t_hi = min(__builtin_amdgcn_readlane(hi, l), n.base + PG_BLOCK);
+      n.row_of_0 = __builtin_amdgcn_readlane(off, l);
+      return n;
+    }
+    before += __builtin_amdgcn_readlane(run, 63);
+  }
+  return NewBlock{-1, 0, 0, 0, 0};
+}
+
+// cos and sin of f revolutions, 0 <= f < 1: reduced to an eighth of one, then the series (the first term
+// left out is below 2^-53).
+__device__ __forceinline__ double2 cos_sin_rev(double f) {
+  const double q = rint(4.0 * f);
+  const double x = (f - 0.25 * q) * 6.283185307179586477, z = x * x;
+  double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;
+  s = fma(s, z, 1.0 / 6227020800.0);
+  s = fma(s, z, -1.0 / 39916800.0);
+  s = fma(s, z, 1.0 / 362880.0);
+  s = fma(s, z, -1.0 / 5040.0);
+  s = fma(s, z, 1.0 / 120.0);
+  s = fma(s, z, -1.0 / 6.0);
+  s = fma(s * z, x, x);
+  c = fma(c, z, -1.0 / 87178291200.0);
+  c = fma(c, z, 1.0 / 479001600.0);
+  c = fma(c, z, -1.0 / 3628800.0);
+  c = fma(c, z, 1.0 / 40320.0);
+  c = fma(c, z, -1.0 / 720.0);
+  c = fma(c, z, 1.0 / 24.0);
+  c = fma(c, z, -0.5);
+  c = fma(c, z, 1.0);
+  const int n = (int)q & 3;
+  const double a = n & 1 ? s : c, b = n & 1 ? c : s;
+  return double2{n == 1 || n == 2 ? -a : a, n >= 2 ? -b : b};
+}
+
+// The least e with m <= 448 2^e = 1.75 2^(e + 8) (m = 0: very low).
+__device__ __forceinline__ int exponent_of(double m) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, m);
+  const bool above = (bits & 0xfffffffffffffULL) > 0xc000000000000ULL;
+  return (int)(bits >> 52) - 1023 - 8 + above;
+}
+__device__ __forceinline__ double pow2(int e) {
+  return __builtin_bit_cast(double, (unsigned long long)(1023 + e) << 52);
+}
+
+// f rounded to e4m3, four to a dword; what is not finite becomes NaN.
+__device__ __forceinline__ uint32_t encode4(const float* f) {
+  float x[4];
+  bool odd = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = __builtin_amdgcn_fmed3f(f[k], -E4M3_MAX, E4M3_MAX);
+    odd = odd || !(fabsf(f[k]) < INFINITY);
+  }
+  uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+  if (odd) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (!(fabsf(f[k]) < INFINITY)) w = (w & ~(0xffu << (8 * k))) | (0x7fu << (8 * k));
+  }
+  return w;
+}
+__device__ __forceinline__ dkv_u32x2 encode8(const float* f) {
+  return dkv_u32x2{encode4(f), encode4(f + 4)};
+}
+// d as a float from which e4m3 rounds as it would from d: where rounding to fp32 landed on a border
+// between two codes (or on a code, which has no more bits), a step to d's side of it.
+__device__ __forceinline__ float float_for_e4m3(double d) {
+  const float f = (float)d;
+  const uint32_t bits = __float_as_uint(f);
+  if ((bits & 0x7ffffu) == 0 && (double)f != d)  // (a NaN stays one)
+    return __uint_as_float(fabs(d) < fabs((double)f) ? bits - 1 : bits + 1);
+  return f;
+}
+
+template <int DT>
+__device__ __forceinline__ void append8_block(const Append8Params& p, int wg, double2* sTrig) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane >> 3, c = lane & 7;
+  const int groups = (int)p.by_groups.d;
+  const int item = __builtin_amdgcn_readfirstlane(quot(p.by_groups, wg));
+  const int unit0 = (wg - item * groups) * A8_WAVES, unit = unit0 + wave;
+  const NewBlock n = new_block(p, item, lane);
+  if (n.b < 0) return;
+  const int page = __builtin_amdgcn_readfirstlane(paged_page(p.pool, n.b, n.base));
+  if (page < 0) return;
+  const bool is_k = unit < p.Hkv, there = unit < 2 * p.Hkv;
+  const int head = is_k ? unit : unit - p.Hkv, slot0 = n.base & (p.pool.page_size - 1);
+  uint8_t* codes = (is_k ? p.k : p.v) + (long long)page * p.pool.page_stride +
+                   (long long)head * p.pool.head_stride + (long long)slot0 * PG_DH + 8 * c;
+  uint8_t* scale = (is_k ? p.k_scale : p.v_scale) + (long long)page * p.scale_page +
+                   (long long)head * p.scale_head + slot0 / PG_BLOCK;
+  // the new rows, and the earlier tokens' codes
+  dkv_u32x4 xa[2], xb[2];
+  dkv_u32x2 oa[2], ob[2];
+  bool isnew[2], isold[2];
+  uint32_t old_byte = 127;
+  const bool has_old = n.t_lo > n.base;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int t = n.base + 8 * s + i;
+    isnew[s] = there && t >= n.t_lo && t < n.t_hi;
+    isold[s] = there && t < n.t_lo;
+    xa[s] = xb[s] = dkv_u32x4{0u, 0u, 0u, 0u};
+    oa[s] = ob[s] = dkv_u32x2{0u, 0u};
+    if (isnew[s]) {
+      const uint16_t* src = p.qkv + (long long)(n.row_of_0 + t) * p.qkv_ld +
+                            (long long)(p.Hq + unit) * PG_DH + 8 * c;
+      xa[s] = *(const dkv_u32x4*)src;
+      xb[s] = *(const dkv_u32x4*)(src + 64);
+    }
+    if (isold[s]) {
+      oa[s] = *(const dkv_u32x2*)(codes + (8 * s + i) * PG_DH);
+      ob[s] = *(const dkv_u32x2*)(codes + (8 * s + i) * PG_DH + 64);
+    }
+  }
+  if (there && has_old) old_byte = *scale;
+  if (unit0 < p.Hkv) {  // some of the waves have keys
+    const int first = n.t_lo - n.base, pairs = (n.t_hi - n.t_lo) * (PG_DH / 2);
+    for (int x = tid; x < pairs; x += 64 * A8_WAVES) {
+      const int t = first + x / (PG_DH / 2), j = x % (PG_DH / 2);
+      const double r = (double)(n.base + t) * p.rev[j];
+      // (read below by piece j / 8 of the lanes, element j % 8)
+      sTrig[t * A8_ROW + (j % 8) * 8 + j / 8] = cos_sin_rev(r - floor(r));
+    }
+    __syncthreads();
+  }
+  if (!there) return;
+
+  float f[2][16];  // y, or y scaled
+  double y[2][16];
+  double big = 0.0;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[s][2 * e] = dkv_elt_to_f32<DT>(xa[s][e] & 0xffffu);
+      f[s][2 * e + 1] = dkv_elt_to_f32<DT>(xa[s][e] >> 16);
+      f[s][8 + 2 * e] = dkv_elt_to_f32<DT>(xb[s][e] & 0xffffu);
+      f[s][8 + 2 * e + 1] = dkv_elt_to_f32<DT>(xb[s][e] >> 16);
+    }
+  }
+  if (is_k) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (n.base + 8 * s + 8 <= n.t_lo || n.base + 8 * s >= n.t_hi) {  // (the wave's)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[s][e] = 0.0;
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[s][e] = (double)f[s][e];
+      if (p.k_norm) {
+        double ss = 0.0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ss = fma(y[s][e], y[s][e], ss);
+#pragma unroll
+        for (int o = 1; o <= 4; o <<= 1) ss += __shfl_xor(ss, o, 64);
+        const double inv = 1.0 / sqrt(ss * (1.0 / PG_DH) + (double)p.eps);
+        float wx[8], wy[8];
+        load8<DT>(p.k_norm + 8 * c, wx);
+        load8<DT>(p.k_norm + 64 + 8 * c, wy);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y[s][e] = y[s][e] * inv * (double)wx[e];
+          y[s][8 + e] = y[s][8 + e] * inv * (double)wy[e];
+        }
+      }
+      if (isnew[s]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const double2 cs = sTrig[(8 * s + i) * A8_ROW + 8 * e + c];
+          const double u = y[s][e], w = y[s][8 + e];
+          y[s][e] = fma(u, cs.x, -(w * cs.y));
+          y[s][8 + e] = fma(w, cs.x, u * cs.y);
+          big = fmax(big, fmax(fabs(y[s][e]), fabs(y[s][8 + e])));
+        }
+      }
+    }
+    if (!(big < INFINITY)) {  // without what is not finite
+      big = 0.0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (isnew[s] && fabs(y[s][e]) < INFINITY) big = fmax(big, fabs(y[s][e]));
+    }
+  } else {
+    float m = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(f[s][e]));
+    if (!(m < INFINITY)) {
+      m = 0.f;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (fabsf(f[s][e]) < INFINITY) m = fmaxf(m, fabsf(f[s][e]));
+    }
+    big = (double)m;
+  }
+  const int need = (int)dkv_wave_max_fast((float)exponent_of(big));  // (small whole numbers)
+  const int old_e = min(max((int)old_byte - 127, E_LOW<DT>), E_HIGH<DT>);
+  int e_new = min(max(need, E_LOW<DT>), E_HIGH<DT>);
+  if (has_old) e_new = max(e_new, old_e);
+  e_new = __builtin_amdgcn_readfirstlane(e_new);
+
+  if (is_k) {
+    const double by = pow2(-e_new);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[s][e] = float_for_e4m3(y[s][e] * by);
+  } else {
+    const float by = __uint_as_float((uint32_t)(127 - e_new) << 23);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[s][e] *= by;
+  }
+  const bool lower = has_old && e_new > old_e;
+  const float down = lower ? __uint_as_float((uint32_t)max(127 + old_e - e_new, 0) << 23) : 1.f;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    uint8_t* at = codes + (8 * s + i) * PG_DH;
+    if (isnew[s]) {
+      *(dkv_u32x2*)at = encode8(f[s]);
+      *(dkv_u32x2*)(at + 64) = encode8(f[s] + 8);
+    } else if (isold[s] && lower) {
+      float g[16];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        g[4 * h] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 0) * down;
+        g[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 1) * down;
+        g[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 2) * down;
+        g[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 3) * down;
+        g[8 + 4 * h] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 0) * down;
+        g[8 + 4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 1) * down;
+        g[8 + 4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 2) * down;
+        g[8 + 4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 3) * down;
+      }
+      *(dkv_u32x2*)at = encode8(g);
+      *(dkv_u32x2*)(at + 64) = encode8(g + 8);
+    }
+  }
+  if (lane == 0) *scale = (uint8_t)(127 + e_new);
+}
+
+template <int DT>
+__global__ __launch_bounds__(64 * A8_WAVES) void paged_append8_kernel(Append8Params p) {
+  __shared__ double2 sTrig[PG_BLOCK * A8_ROW];
+  if ((int)blockIdx.x < p.kv_wgs) {
+    append8_block<DT>(p, blockIdx.x, sTrig);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = (int)(blockIdx.x - p.kv_wgs) * A8_WAVES + wave;
+  const int row = quot(p.by_q_groups, item);
+  const int h = (item - row * (int)p.by_q_groups.d) * 8 + (lane >> 3), c = lane & 7;
+  if (row >= p.T) return;
+  const int b = request_of_row(p.q_start, p.B, row, lane);
+  if (b < 0) return;
+  const int a0 = p.q_start[b], a1 = p.q_start[b + 1];
+  const int pos = p.lens[b] - (a1 - a0) + (row - a0);
+  if (pos < 0 || h >= p.Hq) return;
+  float ox[8], oy[8];
+  paged_turn<DT>(p.qkv + (long long)row * p.qkv_ld + (long long)h * PG_DH, p.q_norm, p.eps, pos,
+                 p.rev, c, ox, oy);
+  uint16_t* dst = p.q_out + (long long)row * p.q_st + (long long)h * p.q_sh;
+  *(dkv_u32x4*)(dst + 8 * c) = round8<DT>(ox);
+  *(dkv_u32x4*)(dst + 64 + 8 * c) = round8<DT>(oy);
+}
+
+// ---------------------------------------------------------------------------------------
+// Pages read back: value = code * scale, of all pages or of those that `ids` names (one outside the pool
+// gives zeros), keys and values to (pages, heads, page_size, 128) each. Bound by memory. A thread turns 16
+// codes (one token's piece) into 32 or 64 bytes.
+// ---------------------------------------------------------------------------------------
+struct ValuesParams {
+  const uint8_t* k;
+  const uint8_t* v;
+  PagedScales scales;
+  long long page_stride, head_stride;
+  int num_pages, page_shift, Hkv;
+  const int* ids;  // null: page i
+  Divisor by_hkv;
+  long long pieces;  // 16 codes each
+  void* k_out;
+  void* v_out;
+};
+constexpr int V_THREADS = 256, V_EACH = 4;
+
+template <int ODT>
+__global__ __launch_bounds__(V_THREADS) void paged_values_kernel(ValuesParams p) {
+  const bool is_v = blockIdx.y != 0;
+  const uint8_t* pool = is_v ? p.v : p.k;
+  const uint8_t* scales = is_v ? p.scales.v : p.scales.k;
+  uint8_t* out = (uint8_t*)(is_v ? p.v_out : p.k_out);
+  const long long at0 = (long long)blockIdx.x * (V_THREADS * V_EACH) + threadIdx.x;
+  dkv_u32x4 codes[V_EACH];
+  uint32_t byte[V_EACH];
+#pragma unroll
+  for (int u = 0; u < V_EACH; ++u) {
+    const long long at = at0 + u * V_THREADS;
+    codes[u] = dkv_u32x4{0u, 0u, 0u, 0u};
+    byte[u] = 127;
+    if (at >= p.pieces) continue;
+    const int row = (int)(at >> (p.page_shift + 3));  // page and head
+    const int i = quot(p.by_hkv, row), h = row - i * p.Hkv;
+    const int slot = (int)(at >> 3) & ((1 << p.page_shift) - 1), piece = (int)at & 7;
+    const int page = p.ids ? p.ids[i] : i;
+    if (page < 0 || page >= p.num_pages) continue;
+    codes[u] = *(const dkv_u32x4*)(pool + (long long)page * p.page_stride +
+                                   (long long)h * p.head_stride + slot * PG_DH + 16 * piece);
+    byte[u] = scales[(long long)page * p.scales.page_stride + (long long)h * p.scales.head_stride +
+                     slot / PG_BLOCK];
+  }
+#pragma unroll
+  for (int u = 0; u < V_EACH; ++u) {
+    const long long at = at0 + u * V_THREADS;
+    if (at >= p.pieces) continue;
+    const float s = pg_scale(byte[u]);
+    if constexpr (ODT == DKV_F32) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        dkv_f32x4 x;
+        x[0] = __builtin_amdgcn_cvt_f32_fp8(codes[u][d], 0) * s;
+        x[1] = __builtin_amdgcn_cvt_f32_fp8(codes[u][d], 1) * s;
+        x[2] = __builtin_amdgcn_cvt_f32_fp8(codes[u][d], 2) * s;
+        x[3] = __builtin_amdgcn_cvt_f32_fp8(codes[u][d], 3) * s;
+        *(dkv_f32x4*)(out + at * 64 + 16 * d) = x;
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const uint32_t a = codes[u][2 * d], b = codes[u][2 * d + 1];
+        *(dkv_u32x4*)(out + at * 32 + 16 * d) =
+            dkv_u32x4{pg_pair<ODT, false>(a, s), pg_pair<ODT, true>(a, s), pg_pair<ODT, false>(b, s),
+                      pg_pair<ODT, true>(b, s)};
+      }
+    }
+  }
+}
+
+bool ranges_meet(const void* a, long long an, const void* b, long long bn) {
+  return (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
+}  // namespace
+
+extern "C" int dkv_paged_append8(void* stream, int dtype, const void* qkv, long long qkv_ld,
+                                 void* q_out, long long q_st, long long q_sh, void* k_pages,
+                                 void* v_pages, long long page_stride, long long head_stride,
+                                 int num_pages, int page_size, void* k_scale, void* v_scale,
+                                 long long scale_page_stride, long long scale_head_stride,
+                                 const int* page_table, long long table_ld, int table_cols,
+                                 const int* q_start, const int* lens, int B, int T, int Hq, int Hkv,
+                                 int Dh, const void* q_norm, const void* k_norm, float eps,
+                                 const double* inv_freq) {
+  if (dtype != DKV_F16 && dtype != DKV_BF16) return DKV_E_UNSUPPORTED;
+  if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0) return DKV_E_ARG;
+  if (Dh != PG_DH || Hq % Hkv != 0) return DKV_E_UNSUPPORTED;
+  Append8Params p;
+  int rc = fill_pool(p.pool, page_stride, head_stride, num_pages, page_size, page_table, table_ld,
+                     table_cols, Hkv, 16);
+  if (rc != DKV_OK) return rc;
+  if (B == 0 || T == 0) return DKV_OK;
+  if (!qkv || !q_out || !k_pages || !v_pages || !q_start || !lens || !inv_freq) return DKV_E_ARG;
+  rc = check_scales({(const uint8_t*)k_scale, (const uint8_t*)v_scale, scale_page_stride,
+                     scale_head_stride},
+                    num_pages, page_size, Hkv);
+  if (rc != DKV_OK) return rc;
+  if (qkv_ld < (long long)(Hq + 2 * Hkv) * PG_DH || q_sh < PG_DH || q_st < PG_DH) return DKV_E_ARG;
+  const bool in_place =
+      qkv == q_out && (T == 1 || q_st == qkv_ld) && (Hq == 1 || q_sh == PG_DH);
+  if (!output_apart({(long long)(uintptr_t)q_out, 2 * q_st, 2 * q_sh, 2 * PG_DH, T, Hq},
+                    {(long long)(uintptr_t)qkv, 2 * qkv_ld, 0,
+                     2LL * (Hq + 2 * Hkv) * PG_DH, T, 1},
+                    in_place))
+    return DKV_E_ARG;
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) ||
+      (qkv_ld & 7) || (q_st & 7) || (q_sh & 7) || (q_norm && !aligned16(q_norm)) ||
+      (k_norm && !aligned16(k_norm)))
+    return DKV_E_UNSUPPORTED;
+  p.qkv = (const uint16_t*)qkv;
+  p.qkv_ld = qkv_ld;
+  p.q_out = (uint16_t*)q_out;
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.k = (uint8_t*)k_pages;
+  p.v = (uint8_t*)v_pages;
+  p.k_scale = (uint8_t*)k_scale;
+  p.v_scale = (uint8_t*)v_scale;
+  p.scale_page = scale_page_stride;
+  p.scale_head = scale_head_stride;
+  p.q_start = q_start;
+  p.lens = lens;
+  p.B = B;
+  p.T = T;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.q_norm = (const uint16_t*)q_norm;
+  p.k_norm = (const uint16_t*)k_norm;
+  p.eps = eps;
+  for (int j = 0; j < PG_DH / 2; ++j) p.rev[j] = inv_freq[j] * 0.15915494309189533577;
+  // n new tokens touch at most n blocks and at most n / 16 + 2
+  const long long some = T / PG_BLOCK + 2LL * (B < T ? B : T), blocks = some < T ? some : T;
+  const int groups = (2 * Hkv + A8_WAVES - 1) / A8_WAVES, q_groups = (Hq + 7) / 8;
+  const long long q_items = (long long)T * q_groups;
+  const long long wgs = blocks * groups + (q_items + A8_WAVES - 1) / A8_WAVES;
+  if (wgs > 0x7fffffffLL || q_items > 0x7fffffffLL - A8_WAVES) return DKV_E_UNSUPPORTED;
+  p.kv_wgs = (int)(blocks * groups);
+  p.by_groups = divisor(groups);
+  p.by_q_groups = divisor(q_groups);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DKV_BF16)
+    hipLaunchKernelGGL(paged_append8_kernel<DKV_BF16>, dim3((unsigned)wgs), dim3(64 * A8_WAVES), 0, st,
+                       p);
+  else
+    hipLaunchKernelGGL(paged_append8_kernel<DKV_F16>, dim3((unsigned)wgs), dim3(64 * A8_WAVES), 0, st,
+                       p);
+  DKV_HIP_CHECK_LAUNCH();
+  return DKV_OK;
+}
+
+extern "C" int dkv_paged_values(void* stream, int out_dtype, const void* k_pages, const void* v_pages,
+                                long long page_stride, long long head_stride, int num_pages,
+                                int page_size, int Hkv, int Dh, const void* k_scale,
+                                const void* v_scale, long long scale_page_stride,
+                                long long scale_head_stride, const int* ids, int n, void* k_out,
+                                void* v_out) {
+  if (out_dtype != DKV_F16 && out_dtype != DKV_BF16 && out_dtype != DKV_F32) return DKV_E_UNSUPPORTED;
+  if (Hkv <= 0 || n < 0 || (!ids && n > num_pages)) return DKV_E_ARG;
+  if (Dh != PG_DH) return DKV_E_UNSUPPORTED;
+  PagedPool pool;
+  int rc = fill_pool(pool, page_stride, head_stride, num_pages, page_size, nullptr, 0, 0, Hkv, 16);
+  if (rc != DKV_OK) return rc;
+  if (n == 0) return DKV_OK;
+  if (!k_pages || !v_pages || !k_out || !v_out) return DKV_E_ARG;
+  rc = check_scales({(const uint8_t*)k_scale, (const uint8_t*)v_scale, scale_page_stride,
+                     scale_head_stride},
+                    num_pages, page_size, Hkv);
+  if (rc != DKV_OK) return rc;
+  if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(k_out) || !aligned16(v_out))
+    return DKV_E_UNSUPPORTED;
+  const long long bytes = (long long)n * Hkv * page_size * PG_DH * dkv_elt_size(out_dtype);
+  if (ranges_meet(k_out, bytes, v_out, bytes)) return DKV_E_ARG;
+  if ((long long)n * Hkv > 0x7fffffffLL) return DKV_E_UNSUPPORTED;
+  ValuesParams p;
+  p.k = (const uint8_t*)k_pages;
+  p.v = (const uint8_t*)v_pages;
+  p.scales = {(const uint8_t*)k_scale, (const uint8_t*)v_scale, scale_page_stride, scale_head_stride};
+  p.page_stride = page_stride;
+  p.head_stride = head_stride;
+  p.num_pages = num_pages;
+  p.page_shift = pool.page_shift;
+  p.Hkv = Hkv;
+  p.ids = ids;
+  p.by_hkv = divisor(Hkv);
+  p.pieces = (long long)n * Hkv * page_size * (PG_DH / 16);
+  p.k_out = k_out;
+  p.v_out = v_out;
+  const long long wgs = (p.pieces + V_THREADS * V_EACH - 1) / (V_THREADS * V_EACH);
+  if (wgs > 0x7fffffffLL) return DKV_E_UNSUPPORTED;
+  const dim3 grid((unsigned)wgs, 2);
+  hipStream_t st = (hipStream_t)stream;
+  if (out_dtype == DKV_BF16)
+    hipLaunchKernelGGL(paged_values_kernel<DKV_BF16>, grid, dim3(V_THREADS), 0, st, p);
+  else if (out_dtype == DKV_F16)
+    hipLaunchKernelGGL(paged_values_kernel<DKV_F16>, grid, dim3(V_THREADS), 0, st, p);
+  else
+    hipLaunchKernelGGL(paged_values_kernel<DKV_F32>, grid, dim3(V_THREADS), 0, st, p);
+  DKV_HIP_CHECK_LAUNCH();
+  return DKV_OK;
+}

@@ -63,21 +63,47 @@ struct Batch {
   int max_len() const { return (int)v[9]; }
 };
 
-// Pools alike, of x's type and on its device, which is the batch's.
-bool pools(const at::Tensor& k, const at::Tensor& v, const at::Tensor& x, const Batch& b) {
+// Pages alike, of type dt on device d.
+bool pages(const at::Tensor& k, const at::Tensor& v, at::ScalarType dt, c10::Device d) {
   if (k.dim() != 4 || v.dim() != 4 || k.sizes() != v.sizes() || k.strides() != v.strides())
     return false;
-  const auto dt = x.scalar_type();
-  if ((dt != at::kBFloat16 && dt != at::kHalf) || k.scalar_type() != dt || v.scalar_type() != dt)
-    return false;
-  if (!x.is_cuda() || x.get_device() != b.v[10] || k.device() != x.device() ||
-      v.device() != x.device())
+  if (k.scalar_type() != dt || v.scalar_type() != dt || !d.is_cuda() || k.device() != d ||
+      v.device() != d)
     return false;
   const long long ps = k.size(2);
   return k.size(3) == HEAD_DIM && k.stride(3) == 1 && k.stride(2) == HEAD_DIM && ps >= 16 &&
-         (ps & (ps - 1)) == 0 && b.max_len() <= b.cols() * ps && k.size(0) <= INT_MAX &&
-         k.size(1) > 0 && k.size(1) <= 65536;
+         (ps & (ps - 1)) == 0 && k.size(0) <= INT_MAX && ps <= INT_MAX && k.size(1) > 0 &&
+         k.size(1) <= 65536;
 }
+
+// The scales of 8-bit pages, alike: (pages, heads, page_size / 16).
+bool scales(const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& k) {
+  return ks.dim() == 3 && vs.dim() == 3 && ks.sizes() == vs.sizes() && ks.strides() == vs.strides() &&
+         ks.scalar_type() == at::kFloat8_e8m0fnu && vs.scalar_type() == at::kFloat8_e8m0fnu &&
+         ks.device() == k.device() && vs.device() == k.device() && ks.size(0) == k.size(0) &&
+         ks.size(1) == k.size(1) && ks.size(2) == k.size(2) / 16 &&
+         (ks.size(2) == 1 || ks.stride(2) == 1);
+}
+
+// Pools of a call on x, whose device is the batch's: pages of x's type, or with their scales (else None,
+// null here) of 8 bits.
+struct Pools {
+  const at::Tensor *k, *v, *ks, *vs;
+  bool read(PyObject* k_pages, PyObject* v_pages, PyObject* k_scale, PyObject* v_scale,
+            const at::Tensor& x, const Batch& b) {
+    k = tensor(k_pages), v = tensor(v_pages), ks = vs = nullptr;
+    const auto dt = x.scalar_type();
+    if (!k || !v || (dt != at::kBFloat16 && dt != at::kHalf) || !x.is_cuda() ||
+        x.get_device() != b.v[10])
+      return false;
+    if (k_scale != Py_None || v_scale != Py_None) {
+      ks = tensor(k_scale), vs = tensor(v_scale);
+      if (!ks || !vs) return false;
+    }
+    return pages(*k, *v, ks ? at::kFloat8_e4m3fn : dt, x.device()) &&
+           (!ks || scales(*ks, *vs, *k)) && b.max_len() <= b.cols() * k->size(2);
+  }
+};
 
 int code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? DKV_BF16 : DKV_F16; }
 
@@ -101,16 +127,19 @@ PyObject* paged_batch(PyObject*, PyObject* const* args, Py_ssize_t n) {
                        v[1], v[3], v[2], d.is_cuda() ? (int)t->get_device() : -1);
 }
 
-// (stream, qkv, k_pages, v_pages, batch, heads, frequencies, q_norm, k_norm, eps)
+// (stream, qkv, k_pages, v_pages, batch, heads, frequencies, q_norm, k_norm, eps, k_scale, v_scale)
 PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Batch b;
   long long heads, freq;
-  if (n != 10 || !b.read(args[4]) || !ints(args + 5, 1, &heads) || !ints(args + 6, 1, &freq))
+  if (n != 12 || !b.read(args[4]) || !ints(args + 5, 1, &heads) || !ints(args + 6, 1, &freq))
     Py_RETURN_NONE;
-  const at::Tensor *x = tensor(args[1]), *k = tensor(args[2]), *v = tensor(args[3]);
+  const at::Tensor* x = tensor(args[1]);
   const double eps = PyFloat_Check(args[9]) ? PyFloat_AS_DOUBLE(args[9]) : -1.0;
-  if (!x || !k || !v || x->dim() != 2 || !(eps >= 0.0) || heads <= 0 || !pools(*k, *v, *x, b))
+  Pools pool;
+  if (!x || x->dim() != 2 || !(eps >= 0.0) || heads <= 0 ||
+      !pool.read(args[2], args[3], args[10], args[11], *x, b))
     Py_RETURN_NONE;
+  const at::Tensor *k = pool.k, *v = pool.v;
   const long long T = x->size(0), hkv = k->size(1), ld = x->stride(0);
   if (x->stride(1) != 1 || heads > 65536 || x->size(1) < (heads + 2 * hkv) * HEAD_DIM ||
       ld < x->size(1) || b.rows() > T || !aligned16(*x))
@@ -129,23 +158,35 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int rc;
   void* const stream = PyLong_AsVoidPtr(args[0]);
   Py_BEGIN_ALLOW_THREADS;
-  rc = dkv_paged_append(
-      stream, code(*x), x->data_ptr(), ld, out.data_ptr(), heads * HEAD_DIM, HEAD_DIM,
-      k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1), (int)k->size(0), (int)k->size(2),
-      b.table(), b.ld(), b.cols(), b.starts(), b.lens(), b.requests(), b.rows(), (int)heads, (int)hkv,
-      (int)HEAD_DIM, norm[0], norm[1], (float)eps, reinterpret_cast<const double*>(freq));
+  if (pool.ks)
+    rc = dkv_paged_append8(
+        stream, code(*x), x->data_ptr(), ld, out.data_ptr(), heads * HEAD_DIM, HEAD_DIM,
+        k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1), (int)k->size(0), (int)k->size(2),
+        pool.ks->data_ptr(), pool.vs->data_ptr(), pool.ks->stride(0), pool.ks->stride(1), b.table(),
+        b.ld(), b.cols(), b.starts(), b.lens(), b.requests(), b.rows(), (int)heads, (int)hkv,
+        (int)HEAD_DIM, norm[0], norm[1], (float)eps, reinterpret_cast<const double*>(freq));
+  else
+    rc = dkv_paged_append(
+        stream, code(*x), x->data_ptr(), ld, out.data_ptr(), heads * HEAD_DIM, HEAD_DIM,
+        k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1), (int)k->size(0), (int)k->size(2),
+        b.table(), b.ld(), b.cols(), b.starts(), b.lens(), b.requests(), b.rows(), (int)heads,
+        (int)hkv, (int)HEAD_DIM, norm[0], norm[1], (float)eps, reinterpret_cast<const double*>(freq));
   Py_END_ALLOW_THREADS;
   if (rc != DKV_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
 }
 
-// (stream, q, k_pages, v_pages, batch, scale, workspace): workspace(q, stream, floats) gives a tensor
+// (stream, q, k_pages, v_pages, batch, scale, workspace, k_scale, v_scale): workspace(q, stream, floats)
+// gives a tensor
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Batch b;
-  if (n != 7 || !b.read(args[4]) || !PyFloat_Check(args[5])) Py_RETURN_NONE;
-  const at::Tensor *q = tensor(args[1]), *k = tensor(args[2]), *v = tensor(args[3]);
-  if (!q || !k || !v || q->dim() != 3 || q->size(2) != HEAD_DIM || !pools(*k, *v, *q, b))
+  if (n != 9 || !b.read(args[4]) || !PyFloat_Check(args[5])) Py_RETURN_NONE;
+  const at::Tensor* q = tensor(args[1]);
+  Pools pool;
+  if (!q || q->dim() != 3 || q->size(2) != HEAD_DIM ||
+      !pool.read(args[2], args[3], args[7], args[8], *q, b))
     Py_RETURN_NONE;
+  const at::Tensor *k = pool.k, *v = pool.v;
   const long long T = q->size(0), hq = q->size(1), hkv = k->size(1);
   const long long st = q->stride(0), sh = q->stride(1);
   if (hq <= 0 || hq > 65536 || hq % hkv || q->stride(2) != 1 || (st & 7) || (sh & 7) ||
@@ -174,16 +215,61 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const float scale = (float)PyFloat_AS_DOUBLE(args[5]);
   void* const stream = PyLong_AsVoidPtr(args[0]);
   Py_BEGIN_ALLOW_THREADS;
-  rc = dkv_paged_attention(
-      stream, code(*q), q->data_ptr(), st, sh, k->data_ptr(), v->data_ptr(),
-      k->stride(0), k->stride(1), (int)k->size(0), (int)k->size(2), b.table(), b.ld(), b.cols(),
-      b.starts(), b.lens(), b.requests(), b.rows(), (int)hq, (int)hkv, (int)HEAD_DIM, b.max_new(),
-      b.min_new(), b.max_len(), scale, ws, ws_floats, out.data_ptr(), code(*q),
-      hq * HEAD_DIM, HEAD_DIM);
+  if (pool.ks)
+    rc = dkv_paged_attention8(
+        stream, code(*q), q->data_ptr(), st, sh, k->data_ptr(), v->data_ptr(), k->stride(0),
+        k->stride(1), (int)k->size(0), (int)k->size(2), pool.ks->data_ptr(), pool.vs->data_ptr(),
+        pool.ks->stride(0), pool.ks->stride(1), b.table(), b.ld(), b.cols(), b.starts(), b.lens(),
+        b.requests(), b.rows(), (int)hq, (int)hkv, (int)HEAD_DIM, b.max_new(), b.min_new(),
+        b.max_len(), scale, ws, ws_floats, out.data_ptr(), code(*q), hq * HEAD_DIM, HEAD_DIM);
+  else
+    rc = dkv_paged_attention(
+        stream, code(*q), q->data_ptr(), st, sh, k->data_ptr(), v->data_ptr(), k->stride(0),
+        k->stride(1), (int)k->size(0), (int)k->size(2), b.table(), b.ld(), b.cols(), b.starts(),
+        b.lens(), b.requests(), b.rows(), (int)hq, (int)hkv, (int)HEAD_DIM, b.max_new(), b.min_new(),
+        b.max_len(), scale, ws, ws_floats, out.data_ptr(), code(*q), hq * HEAD_DIM, HEAD_DIM);
   Py_END_ALLOW_THREADS;
   Py_XDECREF(held);
   if (rc != DKV_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
+}
+
+// (stream, k_pages, v_pages, k_scale, v_scale, page ids, dtype code) -> (k, v)
+PyObject* paged_values(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  long long dt;
+  if (n != 7 || !ints(args + 6, 1, &dt)) Py_RETURN_NONE;
+  const at::Tensor *k = tensor(args[1]), *v = tensor(args[2]), *ks = tensor(args[3]),
+                   *vs = tensor(args[4]), *ids = nullptr;
+  if (!k || !v || !ks || !vs || !pages(*k, *v, at::kFloat8_e4m3fn, k->device()) ||
+      !scales(*ks, *vs, *k))
+    Py_RETURN_NONE;
+  long long count = k->size(0);
+  if (args[5] != Py_None) {
+    ids = tensor(args[5]);
+    if (!ids || ids->dim() != 1 || !int32_on(*ids, k->device()) || !ids->is_contiguous() ||
+        ids->size(0) > INT_MAX)
+      Py_RETURN_NONE;
+    count = ids->size(0);
+  }
+  const auto type = dt == DKV_BF16 ? at::kBFloat16 : dt == DKV_F16 ? at::kHalf : at::kFloat;
+  at::Tensor out[2];
+  for (at::Tensor& t : out)
+    t = at::empty({count, k->size(1), k->size(2), HEAD_DIM}, k->options().dtype(type));
+  int rc;
+  void* const stream = PyLong_AsVoidPtr(args[0]);
+  Py_BEGIN_ALLOW_THREADS;
+  rc = dkv_paged_values(stream, (int)dt, k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1),
+                        (int)k->size(0), (int)k->size(2), (int)k->size(1), (int)HEAD_DIM,
+                        ks->data_ptr(), vs->data_ptr(), ks->stride(0), ks->stride(1),
+                        ids ? static_cast<const int*>(ids->data_ptr()) : nullptr, (int)count,
+                        out[0].data_ptr(), out[1].data_ptr());
+  Py_END_ALLOW_THREADS;
+  if (rc != DKV_OK) Py_RETURN_NONE;
+  PyObject *a = THPVariable_Wrap(std::move(out[0])), *b = THPVariable_Wrap(std::move(out[1]));
+  PyObject* both = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return both;
 }
 
 // A setting of the sampling: a contiguous tensor with an entry per row, or a number for all rows.
@@ -259,7 +345,7 @@ PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<name>)), METH_FASTCALL, nullptr}
 
 PyMethodDef methods[] = {DKV_ENTRY(paged_batch), DKV_ENTRY(paged_append), DKV_ENTRY(paged_attention),
-                         DKV_ENTRY(sample_tokens), {nullptr, nullptr, 0, nullptr}};
+                         DKV_ENTRY(paged_values), DKV_ENTRY(sample_tokens), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_dkv_tensor", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

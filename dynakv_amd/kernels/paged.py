@@ -13,6 +13,10 @@ and a request that ends gives its memory back. Here the keys and values are in p
 * ``paged_attention`` lets every new token attend its request's tokens up to itself: prompts, chunks
   and single tokens in one call.
 
+A cache of dtype ``torch.float8_e4m3fn`` holds half the bytes: pages of e4m3 codes, and for every block
+of 16 tokens of a page's head a power of two (``torch.float8_e8m0fnu``) that they are multiplied by. Both
+operators then take the scales beside the pages, and ``paged_values`` reads pages back.
+
 Rows of a step are its requests' new tokens, one request after the other. Rows behind the last
 request are neither read nor written (a batch padded for a captured graph); a request may have no
 new token. Everything the device buffers of a ``PagedBatch`` hold may change between replays of a
@@ -33,6 +37,8 @@ from .. import _lib
 from .decode import workspace
 
 HEAD_DIM = 128
+BLOCK = 16  # tokens of a page's head that share a scale in 8-bit pages
+CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _COUNTERS = 16384  # leading floats of the attention's workspace: its arrival counters
 _WORKSPACES: dict = {}  # (device, stream) -> the attention's workspace
@@ -98,7 +104,10 @@ class PagedBatch:
 class PagedKVCache:
     """A pool of ``pages`` pages of ``page_size`` tokens for every layer (``k[i]`` and ``v[i]``:
     (pages, kv_heads, page_size, 128)), and the requests that hold them. A page id means the same
-    page in every layer, so one ``PagedBatch`` serves a whole step."""
+    page in every layer, so one ``PagedBatch`` serves a whole step.
+
+    ``dtype`` bf16, fp16, or float8_e4m3fn for pages of 8 bits with scales ``k_scale[i]`` and
+    ``v_scale[i]``: (pages, kv_heads, page_size / 16) (else None)."""
 
     def __init__(self, layers: int, pages: int, kv_heads: int, *, page_size: int = 64,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -106,7 +115,7 @@ class PagedKVCache:
             raise ValueError("page_size must be a power of two of at least 16")
         if layers < 1 or pages < 1 or kv_heads < 1:
             raise ValueError("layers, pages and kv_heads must be positive")
-        if dtype not in (torch.bfloat16, torch.float16):
+        if dtype not in (torch.bfloat16, torch.float16, CODES):
             raise ValueError(f"unsupported dtype {dtype}")
         self.page_size, self.pages = page_size, pages
         dims = (pages, kv_heads, page_size, HEAD_DIM)
@@ -114,6 +123,13 @@ class PagedKVCache:
         self.device = self.k[0].device  # ("cuda": the device that is current now)
         self.k += [torch.empty(dims, dtype=dtype, device=self.device) for _ in range(layers - 1)]
         self.v = [torch.empty(dims, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.k_scale: list = [None] * layers
+        self.v_scale: list = [None] * layers
+        if dtype == CODES:
+            dims = (pages, kv_heads, page_size // BLOCK)
+            for scales in (self.k_scale, self.v_scale):
+                scales[:] = [torch.zeros(dims, dtype=torch.uint8, device=self.device).view(SCALES)
+                             for _ in range(layers)]
         self._free = list(range(pages - 1, -1, -1))
         self._held: dict[int, list[int]] = {}
         self._len: dict[int, int] = {}
@@ -220,9 +236,8 @@ def _frequency_address(theta: float | None, inv_freq: Sequence[float] | None) ->
     return _frequencies(tuple(float(f) for f in inv_freq))
 
 
-def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, dtype: torch.dtype,
-           device: int) -> tuple:
-    """(KV heads, the pools' arguments of a call), checked against each other and the batch."""
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, device: int) -> tuple:
+    """(KV heads, the pools' arguments of a call), checked against each other."""
     shape, st = k_pages.shape, k_pages.stride()
     if len(shape) != 4 or shape != v_pages.shape or shape[3] != HEAD_DIM:
         raise ValueError("k_pages / v_pages must be (pages, kv_heads, page_size, 128), alike")
@@ -230,15 +245,50 @@ def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, dtyp
         raise ValueError("pages must hold a head's tokens back to back, with one layout for K and V")
     if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise ValueError("page and input dtypes differ")
-    if not (k_pages.get_device() == v_pages.get_device() == batch._args[10] == device):
+    if not (k_pages.get_device() == v_pages.get_device() == device):
         raise ValueError("inputs, pages and batch must be on one device")
     pages, hkv, ps, _ = shape
     if ps < 16 or ps & (ps - 1):
         raise NotImplementedError("page_size must be a power of two of at least 16")
-    if batch._max_len > batch._args[2] * ps:
-        raise ValueError(f"max_len {batch._max_len} is past the page table "
-                         f"({batch._args[2]} pages of {ps})")
     return hkv, (k_pages.data_ptr(), v_pages.data_ptr(), st[0], st[1], pages, ps)
+
+
+def _scales(k_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> tuple:
+    """The scales' arguments of a call, checked against the pages."""
+    pages, hkv, ps, _ = k_pages.shape
+    shape, st = (pages, hkv, ps // BLOCK), k_scale.stride()
+    if k_scale.shape != shape or v_scale.shape != shape:
+        raise ValueError(f"k_scale / v_scale must be (pages, kv_heads, page_size / {BLOCK})")
+    if k_scale.dtype != SCALES or v_scale.dtype != SCALES:
+        raise ValueError(f"scales must be {SCALES}")
+    if st != v_scale.stride() or (shape[2] > 1 and st[2] != 1):
+        raise ValueError("scales must have unit last stride, and one layout for K and V")
+    if not (k_scale.get_device() == v_scale.get_device() == k_pages.get_device()):
+        raise ValueError("pages and scales must be on one device")
+    return k_scale.data_ptr(), v_scale.data_ptr(), st[0], st[1]
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, dtype: torch.dtype,
+           device: int, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> tuple:
+    """(KV heads, the pools' arguments of a call, whether the pages have scales), checked against
+    each other and the batch."""
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("give k_scale and v_scale, or neither")
+    coded = k_scale is not None
+    if coded:
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"unsupported dtype {dtype}")
+    elif k_pages.dtype == CODES:
+        raise ValueError("8-bit pages need k_scale and v_scale")
+    hkv, args = _pages(k_pages, v_pages, CODES if coded else dtype, device)
+    if batch._args[10] != device:
+        raise ValueError("inputs, pages and batch must be on one device")
+    if batch._max_len > batch._args[2] * k_pages.shape[2]:
+        raise ValueError(f"max_len {batch._max_len} is past the page table "
+                         f"({batch._args[2]} pages of {k_pages.shape[2]})")
+    if coded:
+        args += _scales(k_pages, k_scale, v_scale)
+    return hkv, args, coded
 
 
 def _row_strides(t: torch.Tensor) -> tuple[int, int]:
@@ -253,6 +303,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                  batch: PagedBatch, *, heads: int, theta: float | None = None,
                  inv_freq: Sequence[float] | None = None, q_norm: torch.Tensor | None = None,
                  k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                 k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """Write a step's keys and values to their pages; returns its queries (T, heads, 128).
 
@@ -263,12 +314,22 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ((128,) of qkv's dtype) each query / key head is first normed, x / sqrt(mean(x^2) + eps) * w.
     Everything in fp32, rounded once where it is stored. ``out``: where the queries go (T, heads,
     128), unit last stride: qkv's own query columns, or memory apart from it. A token whose page is not
-    there is not stored."""
+    there is not stored.
+
+    8-bit pages come with their ``k_scale`` and ``v_scale``. The step's keys (computed in 64 bits) and
+    values of a block of 16 tokens are held as code * scale, scale the least power of two with |y| <=
+    448 scale and code y / scale rounded to the nearest e4m3 (ties to even). A block that holds earlier
+    tokens of the request keeps its scale where that is larger, and else has their codes rounded again
+    to the new one (a request cut back by ``truncate`` into a block leaves that block's scale). Scales
+    are 2^-15 to 2^7 for fp16 and 2^-110 to 2^119 for bf16, so that every value held is one of qkv's
+    type: what is past 448 times the largest is held as that, and what is infinite or NaN as NaN.
+    Requests of one call must not share such a block."""
     freqs = _frequency_address(theta, inv_freq)
     fast = _lib.tensor_calls()
     if fast is not None and out is None and _lib.is_current(batch._args[10]):
         out = fast.paged_append(_lib.stream_on(batch._args[10]), qkv, k_pages, v_pages, batch._args,
-                                heads, ctypes.addressof(freqs), q_norm, k_norm, eps)
+                                heads, ctypes.addressof(freqs), q_norm, k_norm, eps, k_scale,
+                                v_scale)
         if out is not None:
             return out
     shape, st = qkv.shape, qkv.stride()
@@ -276,7 +337,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise ValueError("qkv must be (T, W) with unit last stride")
     T, width = shape
     dt, dev = qkv.dtype, qkv.get_device()
-    hkv, pools = _pools(k_pages, v_pages, batch, dt, dev)
+    hkv, pools, coded = _pools(k_pages, v_pages, batch, dt, dev, k_scale, v_scale)
     if heads <= 0 or width < (heads + 2 * hkv) * HEAD_DIM:
         raise ValueError(f"qkv must hold {heads} + 2 * {hkv} heads of {HEAD_DIM}")
     if batch._rows > T:
@@ -295,16 +356,17 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise ValueError("out must be (T, heads, 128) of qkv's dtype with unit last stride")
     else:
         o_st = _row_strides(out)
+    name = "dkv_paged_append8" if coded else "dkv_paged_append"
     _lib.check(_lib.call_on(
-        dev, _lib.calls().dkv_paged_append, stream, _lib.dtype_code(dt), qkv.data_ptr(),
+        dev, getattr(_lib.calls(), name), stream, _lib.dtype_code(dt), qkv.data_ptr(),
         st[0] if T > 1 else width, out.data_ptr(), *o_st, *pools, *batch._args[:7], heads, hkv,
-        HEAD_DIM, _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs)),
-        "dkv_paged_append")
+        HEAD_DIM, _lib.ptr(q_norm), _lib.ptr(k_norm), float(eps), ctypes.addressof(freqs)), name)
     return out
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     batch: PagedBatch, *, scale: float | None = None,
+                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                     out: torch.Tensor | None = None,
                     out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Attention of a step's new tokens over their requests' pages (T, heads, 128).
@@ -313,12 +375,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     token at position t attends its request's tokens 0 .. t (the pages hold them all: the step's own
     are appended first); one that has none to attend (or scores of -infinity alone) gives 0. ``scale`` defaults to 1 / sqrt(128).
     The output is in q's dtype, or in fp32 before that rounding with ``out_dtype=torch.float32``;
-    ``out`` may be q itself, or memory apart from it."""
+    ``out`` may be q itself, or memory apart from it. 8-bit pages come with their ``k_scale`` and
+    ``v_scale``; keys and values are then code * scale, in q's type."""
     fast = _lib.tensor_calls()
     if (fast is not None and out is None and out_dtype is None
             and _lib.is_current(batch._args[10])):
         out = fast.paged_attention(_lib.stream_on(batch._args[10]), q, k_pages, v_pages, batch._args,
-                                   _SCALE if scale is None else scale, _attention_workspace)
+                                   _SCALE if scale is None else scale, _attention_workspace, k_scale,
+                                   v_scale)
         if out is not None:
             return out
     shape, st = q.shape, q.stride()
@@ -326,7 +390,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("q must be (T, heads, 128)")
     T, hq, _ = shape
     dt, dev = q.dtype, q.get_device()
-    hkv, pools = _pools(k_pages, v_pages, batch, dt, dev)
+    hkv, pools, coded = _pools(k_pages, v_pages, batch, dt, dev, k_scale, v_scale)
     if hq % hkv or hq == 0:
         raise ValueError(f"{hq} query heads do not divide among {hkv} KV heads")
     if batch._rows > T:
@@ -349,12 +413,47 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     bounds = batch._args[7:10]
     need = lib.dkv_paged_workspace_floats(batch._requests, batch._rows, hq, hkv, *bounds)
     ws = _attention_workspace(q, stream, need) if need else None
+    name = "dkv_paged_attention8" if coded else "dkv_paged_attention"
     _lib.check(_lib.call_on(
-        dev, lib.dkv_paged_attention, stream, _lib.dtype_code(dt), q.data_ptr(), st[0], st[1],
+        dev, getattr(lib, name), stream, _lib.dtype_code(dt), q.data_ptr(), st[0], st[1],
         *pools, *batch._args[:7], hq, hkv, HEAD_DIM, *bounds,
         _SCALE if scale is None else float(scale), _lib.ptr(ws), ws.numel() if need else 0,
-        out.data_ptr(), _lib.dtype_code(odt), *o_st), "dkv_paged_attention")
+        out.data_ptr(), _lib.dtype_code(odt), *o_st), name)
     return out
+
+
+def paged_values(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor,
+                 v_scale: torch.Tensor, *, pages: torch.Tensor | None = None,
+                 dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that 8-bit pages hold, code * scale: two tensors (n, kv_heads, page_size,
+    128) of ``dtype`` (bf16, fp16 or fp32; rounded where it is not one of its numbers).
+
+    ``pages`` (n,) int32: which ones, on the pages' device (an id outside the pool gives zeros);
+    all by default. To hand a request to a 16-bit cache, to keep it elsewhere, to look at it."""
+    fast = _lib.tensor_calls()
+    dev = k_pages.get_device()
+    if fast is not None and _lib.is_current(dev):
+        out = fast.paged_values(_lib.stream_on(dev), k_pages, v_pages, k_scale, v_scale, pages,
+                                _lib.dtype_code(dtype))
+        if out is not None:
+            return out
+    hkv, pools = _pages(k_pages, v_pages, CODES, dev)
+    scales = _scales(k_pages, k_scale, v_scale)
+    ps = k_pages.shape[2]
+    n = k_pages.shape[0]
+    if pages is not None:
+        if pages.dim() != 1 or pages.dtype != torch.int32 or not pages.is_contiguous():
+            raise ValueError("pages must be a contiguous (n,) int32 tensor")
+        if pages.get_device() != dev:
+            raise ValueError("pages and their ids must be on one device")
+        n = pages.shape[0]
+    code, stream = _lib.dtype_code(dtype), _lib.stream_of(k_pages)
+    k = torch.empty((n, hkv, ps, HEAD_DIM), dtype=dtype, device=k_pages.device)
+    v = torch.empty_like(k)
+    _lib.check(_lib.call_on(
+        dev, _lib.calls().dkv_paged_values, stream, code, *pools, hkv, HEAD_DIM, *scales,
+        _lib.ptr(pages), n, k.data_ptr(), v.data_ptr()), "dkv_paged_values")
+    return k, v
 
 
 def _attention_workspace(q: torch.Tensor, stream: int, floats: int) -> torch.Tensor:

@@ -663,6 +663,48 @@ int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st, 
                         long long o_sh);
 
 /*
+ * The same over pages of 8 bits. Codes are e4m3 bytes laid out as the elements above (strides in bytes,
+ * multiples of 16), and the 16 slots of a block (16 i .. 16 i + 15 of a page's head) share a scale
+ * 2^(byte - 127) (255: NaN), byte i of (page, head) in k_scale / v_scale, strides scale_page_stride and
+ * scale_head_stride. The value is code * scale.
+ *
+ * dkv_paged_append8: queries as dkv_paged_append. The new keys (computed in 64 bits) and values of a
+ * block get the least scale with |y| <= 448 scale (fp16: 2^-15 to 2^7, bf16: 2^-110 to 2^119; what is past
+ * 448 times the largest is held as that), or the block's own where that is larger and the block holds
+ * earlier tokens of the request, whose codes are otherwise rounded again to the new scale; y / scale is
+ * rounded to the nearest code (ties to even). What is infinite or NaN is held as NaN. New tokens of one
+ * call must not share a block with another request's.
+ *
+ * dkv_paged_attention8: dkv_paged_attention over the pages' values; its workspace is the same.
+ *
+ * dkv_paged_values: the values of pages ids[0 .. n - 1] (device; zeros for one outside the pool), or of the
+ * pages 0 .. n - 1 where ids is null, to k_out and v_out, each (n, Hkv, page_size, 128) of out_dtype,
+ * contiguous, 16-byte aligned, apart from each other.
+ */
+int dkv_paged_append8(void* stream, int dtype, const void* qkv, long long qkv_ld, void* q_out,
+                      long long q_st, long long q_sh, void* k_pages, void* v_pages,
+                      long long page_stride, long long head_stride, int num_pages, int page_size,
+                      void* k_scale, void* v_scale, long long scale_page_stride,
+                      long long scale_head_stride, const int* page_table, long long table_ld,
+                      int table_cols, const int* q_start, const int* lens, int B, int T, int Hq,
+                      int Hkv, int Dh, const void* q_norm, const void* k_norm, float eps,
+                      const double* inv_freq);
+int dkv_paged_attention8(void* stream, int dtype, const void* q, long long q_st, long long q_sh,
+                         const void* k_pages, const void* v_pages, long long page_stride,
+                         long long head_stride, int num_pages, int page_size, const void* k_scale,
+                         const void* v_scale, long long scale_page_stride,
+                         long long scale_head_stride, const int* page_table, long long table_ld,
+                         int table_cols, const int* q_start, const int* lens, int B, int T, int Hq,
+                         int Hkv, int Dh, int max_new, int min_new, int max_len, float scale,
+                         float* workspace, long long workspace_floats, void* out, int out_dtype,
+                         long long o_st, long long o_sh);
+int dkv_paged_values(void* stream, int out_dtype, const void* k_pages, const void* v_pages,
+                     long long page_stride, long long head_stride, int num_pages, int page_size,
+                     int Hkv, int Dh, const void* k_scale, const void* v_scale,
+                     long long scale_page_stride, long long scale_head_stride, const int* ids, int n,
+                     void* k_out, void* v_out);
+
+/*
  * dkv_sample_tokens: one token per row of logits (rows, V <= 524288; row stride ld; bf16, fp16 or
  * fp32) from a uniform number u[row] in [0, 1). Settings per row where the pointer is given, else the
  * value beside it. With w_i = exp((l_i - max l) / temperature) and tokens in the order of their
