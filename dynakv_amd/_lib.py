@@ -124,6 +124,8 @@ _SIGNATURES = {
     "dkv_sample_workspace_bytes": (_ll, [_i, _i, _i]),
     "dkv_sample_tokens": (_i, [_vp, _i, _vp, _ll, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f,
                                _vp, _ll, _vp]),
+    "dkv_adjust_logits": (_i, [_vp, _i, _vp, _ll, _i, _i, _vp, _i, _ll, _i, _vp, _i, _vp, _i, _vp, _f,
+                               _vp, _f, _vp, _f, _vp, _ll, _vp, _ll, _i, _vp, _ll]),
     "dkv_cutoff_kv": (_i, [_vp, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _ll,
                            _vp, _vp, _ll, _vp, _ll, _i, _i, _i]),
 }

@@ -31,7 +31,8 @@ TENSOR_PATH = LIB_DIR / ("_dkv_tensor" + sysconfig.get_config_var("EXT_SUFFIX"))
 OBJ_DIR = PKG_DIR / "_build"
 SOURCES = ("dkv_append.hip", "dkv_generic.hip", "dkv_splitk.hip", "dkv_cutoff.hip",
            "dkv_prefill.hip", "dkv_layer.hip", "dkv_model.hip", "dkv_joint.hip", "dkv_dense.hip",
-           "dkv_recon.hip", "dkv_paged.hip", "dkv_paged8.hip", "dkv_sample.hip")
+           "dkv_recon.hip", "dkv_paged.hip", "dkv_paged8.hip", "dkv_sample.hip",
+           "dkv_logits.hip")
 ARCH = os.environ.get("DYNAKV_AMD_ARCH", "gfx950")
 
 COMMON_FLAGS = [

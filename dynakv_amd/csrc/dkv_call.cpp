@@ -114,6 +114,7 @@ PyMethodDef methods[] = {
     DKV_CALL(dkv_paged_values),
     DKV_CALL(dkv_sample_workspace_bytes),
     DKV_CALL(dkv_sample_tokens),
+    DKV_CALL(dkv_adjust_logits),
     {nullptr, nullptr, 0, nullptr},
 };
 

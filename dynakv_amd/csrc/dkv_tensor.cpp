@@ -330,6 +330,97 @@ PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// A (rows, n) tensor of a type, on a device, with unit last stride.
+const at::Tensor* matrix(PyObject* o, long long rows, c10::Device d) {
+  const at::Tensor* t = tensor(o);
+  return t && t->dim() == 2 && t->size(0) == rows && t->device() == d && t->size(1) <= INT_MAX &&
+                 (t->size(1) <= 1 || t->stride(1) == 1)
+             ? t
+             : nullptr;
+}
+
+// (stream, device, logits, tokens, prompt_lens, lens, repetition, frequency, presence, bias_ids, bias,
+// allowed) -> True
+PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  long long dev;
+  if (n != 12 || !ints(args + 1, 1, &dev)) Py_RETURN_NONE;
+  const at::Tensor* x = tensor(args[2]);
+  if (!x || x->dim() != 2 || !x->is_cuda() || x->get_device() != dev) Py_RETURN_NONE;
+  const long long rows = x->size(0), V = x->size(1);
+  const auto dt = x->scalar_type();
+  if (rows > INT_MAX || V > INT_MAX || (V > 1 && x->stride(1) != 1) ||
+      (rows > 1 && x->stride(0) < V) ||
+      (dt != at::kBFloat16 && dt != at::kHalf && dt != at::kFloat))
+    Py_RETURN_NONE;
+  const c10::Device d = x->device();
+  const at::Tensor *tokens = nullptr, *ids = nullptr, *bias = nullptr, *allowed = nullptr;
+  long long N = 0;
+  if (args[3] != Py_None) {
+    tokens = matrix(args[3], rows, d);
+    if (!tokens || (tokens->scalar_type() != at::kInt && tokens->scalar_type() != at::kLong))
+      Py_RETURN_NONE;
+    N = tokens->size(1);
+  } else if (args[4] != Py_None || args[5] != Py_None) {
+    Py_RETURN_NONE;
+  }
+  const void* by_row[5] = {};
+  double all[5] = {0.0, (double)N, 1.0, 0.0, 0.0};
+  const double none[5] = {0.0, 0.0, 1.0, 0.0, 0.0};
+  for (int i = 0; i < 5; ++i) {
+    PyObject* o = args[4 + i];
+    if (i < 2) {
+      if (o == Py_None) continue;
+      if (PyFloat_Check(o)) Py_RETURN_NONE;
+    }
+    const at::Tensor* t = tensor(o);
+    if (t && (t->dim() != 1 || t->size(0) != rows || t->device() != d ||
+              t->scalar_type() != (i < 2 ? at::kInt : at::kFloat) || !t->is_contiguous()))
+      Py_RETURN_NONE;
+    if (t) {
+      by_row[i] = t->data_ptr();
+      all[i] = none[i];
+    } else if (PyFloat_Check(o)) {
+      all[i] = PyFloat_AS_DOUBLE(o);
+    } else {
+      long long v;
+      if (!PyLong_Check(o) || !ints(&o, 1, &v)) Py_RETURN_NONE;
+      all[i] = (double)v;
+    }
+    if (i < 2) all[i] = all[i] < 0.0 ? 0.0 : all[i] > (double)N ? (double)N : all[i];
+    if (i >= 2 && !tokens && (t || all[i] != none[i])) Py_RETURN_NONE;
+  }
+  if (!(all[2] > 0.0 && all[2] <= 3.4e38)) Py_RETURN_NONE;
+  if (args[9] != Py_None || args[10] != Py_None) {
+    ids = matrix(args[9], rows, d), bias = matrix(args[10], rows, d);
+    if (!ids || !bias || ids->scalar_type() != at::kInt || bias->scalar_type() != at::kFloat ||
+        ids->size(1) != bias->size(1))
+      Py_RETURN_NONE;
+  }
+  if (args[11] != Py_None) {
+    allowed = matrix(args[11], rows, d);
+    if (!allowed || allowed->scalar_type() != at::kInt || allowed->size(1) * 32 < V) Py_RETURN_NONE;
+  }
+  const int code = dt == at::kBFloat16 ? DKV_BF16 : dt == at::kHalf ? DKV_F16 : DKV_F32;
+  int rc;
+  void* const stream = PyLong_AsVoidPtr(args[0]);
+  auto ld = [&](const at::Tensor* t) { return t && rows > 1 ? t->stride(0) : 0; };
+  Py_BEGIN_ALLOW_THREADS;
+  rc = dkv_adjust_logits(
+      stream, code, x->data_ptr(), rows > 1 ? x->stride(0) : V, (int)rows, (int)V,
+      tokens ? tokens->data_ptr() : nullptr, tokens && tokens->scalar_type() == at::kLong ? 8 : 4,
+      ld(tokens), (int)N, static_cast<const int*>(by_row[0]), (int)all[0],
+      static_cast<const int*>(by_row[1]), (int)all[1], static_cast<const float*>(by_row[2]),
+      (float)all[2], static_cast<const float*>(by_row[3]), (float)all[3],
+      static_cast<const float*>(by_row[4]), (float)all[4],
+      ids ? static_cast<const int*>(ids->data_ptr()) : nullptr, ld(ids),
+      bias ? static_cast<const float*>(bias->data_ptr()) : nullptr, ld(bias),
+      ids ? (int)ids->size(1) : 0,
+      allowed ? static_cast<const int*>(allowed->data_ptr()) : nullptr, ld(allowed));
+  Py_END_ALLOW_THREADS;
+  if (rc != DKV_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+}
+
 // (a C++ exception, of a tensor without memory or an allocation that failed: the Python function's)
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
@@ -345,7 +436,8 @@ PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<name>)), METH_FASTCALL, nullptr}
 
 PyMethodDef methods[] = {DKV_ENTRY(paged_batch), DKV_ENTRY(paged_append), DKV_ENTRY(paged_attention),
-                         DKV_ENTRY(paged_values), DKV_ENTRY(sample_tokens), {nullptr, nullptr, 0, nullptr}};
+                         DKV_ENTRY(paged_values), DKV_ENTRY(sample_tokens),
+                         DKV_ENTRY(adjust_logits), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_dkv_tensor", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

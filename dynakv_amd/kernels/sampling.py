@@ -1,10 +1,11 @@
-"""Sampling of the next token from logits (host side of ``dkv_sample.hip``).
+"""Sampling of the next token from logits (host side of ``dkv_sample.hip``, ``dkv_logits.hip``).
 
 The generators take the most probable token (the reference's benchmark decodes greedily,
 ``scripts/benchmark_throughput.py:17-30``; its models inherit transformers' ``generate`` with
 temperature, top-k, top-p and min-p). ``sample_tokens`` draws a token per row under these filters from
 a uniform number that the caller gives, so a draw can be repeated; it is one launch, or three where
-few rows of a large vocabulary are cut among workgroups.
+few rows of a large vocabulary are cut among workgroups. ``adjust_logits_`` comes before it where a
+request has penalties for the tokens it has seen, biased tokens or a mask of allowed ones.
 """
 
 from __future__ import annotations
@@ -85,3 +86,89 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
         rows, V, u.data_ptr(), t_ptr, float(t), k_ptr, int(min(max(k, 0), V)), p_ptr, float(p),
         m_ptr, float(m), _lib.ptr(ws), need, out.data_ptr()), "dkv_sample_tokens")
     return out
+
+
+def _rows_of(t: torch.Tensor, rows: int, dtypes: tuple, device: int, name: str) -> int:
+    """The row stride of (rows, n), checked."""
+    if t.dim() != 2 or t.shape[0] != rows or t.dtype not in dtypes:
+        raise ValueError(f"{name} must be ({rows}, n) of {' or '.join(str(d) for d in dtypes)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have unit last stride")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on the logits' device")
+    return t.stride(0) if rows > 1 else t.shape[1]
+
+
+def adjust_logits_(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, prompt_lens=None,
+                   lens=None, repetition=1.0, frequency=0.0, presence=0.0,
+                   bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   allowed: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties, biases and a mask on ``logits`` (rows, V), in place; returns them.
+
+    Row b's request has the tokens ``tokens[b, :lens[b]]`` (int32 or int64; ``lens`` a number or a
+    (rows,) int32 tensor, all by default), the first ``prompt_lens[b]`` of them given (0 by
+    default), the others generated. Settings are numbers or (rows,) fp32 tensors. In this order, for a
+    token that is
+
+    * in ``tokens``: x / ``repetition`` where x > 0, else x * ``repetition`` (which must be positive);
+    * generated n > 0 times: x - n * ``frequency`` - ``presence``;
+    * in ``bias_ids[b]`` ((rows, M) int32): x + its ``bias[b]`` ((rows, M) fp32), several of one token
+      added up in their order;
+    * not allowed, bit i % 32 of ``allowed[b, i // 32]`` ((rows, >= V / 32) int32) being 0: -infinity.
+
+    In fp32, rounded once to the logits' type (bf16, fp16 or fp32). Ids outside the vocabulary are
+    passed over (pad with -1); a row stride may be 0 (one row expanded to all), but for the logits'.
+    Logits that nothing concerns are neither read nor written, so the cost goes by the histories' and
+    masks' size."""
+    fast = _lib.tensor_calls()
+    if fast is not None:
+        dev = logits.get_device()
+        if _lib.is_current(dev) and fast.adjust_logits(
+                _lib.stream_on(dev), dev, logits, tokens, prompt_lens, lens, repetition, frequency,
+                presence, bias_ids, bias, allowed):
+            return logits
+    shape, st = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and st[1] != 1):
+        raise ValueError("logits must be (rows, V) with unit last stride")
+    rows, V = shape
+    if rows > 1 and st[0] < V:
+        raise ValueError("rows of logits must not share memory")
+    code, dev = _lib.dtype_code(logits.dtype), logits.get_device()
+    settings = [_setting(v, rows, torch.float32, dev, name) for v, name in (
+        (repetition, "repetition"), (frequency, "frequency"), (presence, "presence"))]
+    if not isinstance(repetition, torch.Tensor) and not 0.0 < repetition < float("inf"):
+        raise ValueError("repetition must be positive and finite")
+    if tokens is None:
+        if prompt_lens is not None or lens is not None:
+            raise ValueError("prompt_lens and lens need tokens")
+        if any(isinstance(v, torch.Tensor) or v != none
+               for v, none in ((repetition, 1.0), (frequency, 0.0), (presence, 0.0))):
+            raise ValueError("penalties need tokens")
+        N, t_ld, size = 0, 0, 4
+    else:
+        t_ld = _rows_of(tokens, rows, (torch.int32, torch.int64), dev, "tokens")
+        N, size = tokens.shape[1], tokens.element_size()
+    p_ptr, p = _setting(0 if prompt_lens is None else prompt_lens, rows, torch.int32, dev, "prompt_lens")
+    l_ptr, n = _setting(N if lens is None else lens, rows, torch.int32, dev, "lens")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("give bias_ids and bias, or neither")
+    M = i_ld = b_ld = a_ld = 0
+    if bias is not None:
+        i_ld = _rows_of(bias_ids, rows, (torch.int32,), dev, "bias_ids")
+        b_ld = _rows_of(bias, rows, (torch.float32,), dev, "bias")
+        M = bias.shape[1]
+        if bias_ids.shape != bias.shape:
+            raise ValueError("bias_ids and bias differ in shape")
+    if allowed is not None:
+        a_ld = _rows_of(allowed, rows, (torch.int32,), dev, "allowed")
+        if allowed.shape[1] * 32 < V:
+            raise ValueError(f"allowed has {allowed.shape[1]} words for {V} tokens")
+    stream = _lib.stream_of(logits)
+    _lib.check(_lib.call_on(
+        dev, _lib.calls().dkv_adjust_logits, stream, code, logits.data_ptr(),
+        st[0] if rows > 1 else V, rows, V, _lib.ptr(tokens), size, t_ld, N, p_ptr,
+        min(max(int(p), 0), N), l_ptr, min(max(int(n), 0), N),
+        *(x for ptr, v in settings for x in (ptr, float(v) if ptr is None else 1.0)),
+        _lib.ptr(bias_ids), i_ld, _lib.ptr(bias), b_ld, M, _lib.ptr(allowed), a_ld),
+        "dkv_adjust_logits")
+    return logits

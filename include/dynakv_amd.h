@@ -722,6 +722,26 @@ int dkv_sample_tokens(void* stream, int dtype, const void* logits, long long ld,
                       const float* min_p, float min_p_all,
                       void* workspace, long long workspace_bytes, long long* out);
 
+/*
+ * dkv_adjust_logits: penalties, biases and a mask on rows of logits (row stride ld >= V; bf16, fp16 or
+ * fp32), in place, in fp32 with one rounding. Row's history: tokens[0 .. len - 1] of row's N (row stride
+ * tokens_ld, 4 or 8 bytes each; null or N = 0: none), those from prompt on generated. Settings and lengths
+ * per row where the pointer is given, else the value beside it. In this order, for token i:
+ *   in the history:           x > 0 ? x / repetition : x * repetition (repetition > 0)
+ *   n > 0 times generated:    x - frequency * n - presence
+ *   in bias_ids[0 .. M - 1]:  x + the sum of its biases, in their order
+ *   bit i % 32 of allowed[i / 32] is 0 (null: no mask):  -infinity
+ * Ids outside [0, V) are passed over. Row strides may be 0 (one row for all), but for the logits'. Logits
+ * that none of it concerns are neither read nor written.
+ */
+int dkv_adjust_logits(void* stream, int dtype, void* logits, long long ld, int rows, int V,
+                      const void* tokens, int token_bytes, long long tokens_ld, int N,
+                      const int* prompt_lens, int prompt_all, const int* lens, int len_all,
+                      const float* repetition, float repetition_all, const float* frequency,
+                      float frequency_all, const float* presence, float presence_all,
+                      const int* bias_ids, long long bias_ids_ld, const float* bias, long long bias_ld,
+                      int M, const int* allowed, long long allowed_ld);
+
 #ifdef __cplusplus
 }
 #endif
