@@ -207,9 +207,9 @@ constexpr int DSLOT_BYTES = 2 * DTILE_BYTES;
 constexpr int DROWS = 16;
 constexpr int DREC = DROWS * (PG_DH + 2);   // floats of a record: m, l and acc[128] of 16 rows
 constexpr int D_COUNTERS = 16384;           // leading workspace ints
-constexpr int D_WGS = 256;                  // workgroups of 8 waves: one per CU
+constexpr int D_WAVES = 2048;               // of a launch that fills the chip: eight per CU
 constexpr int D_SPLIT_B = 256;              // requests a wave can hold the lengths of (4 a lane)
-static_assert(D_WGS <= D_SPLIT_B && D_WGS <= D_COUNTERS, "units that are cut: fewer than D_WGS");
+static_assert(D_WAVES / 4 <= D_COUNTERS, "a counter for each unit that is cut");
 constexpr int D_MIN_TILES = 16;             // least part
 template <int DT>                           // log2 units the running maximum may be exceeded by
 constexpr float D_RESCALE = DT == DKV_F16 ? PG_F16_RESCALE : 11.5f;
@@ -686,7 +686,7 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
     return __hip_atomic_load((const unsigned long long*)a, __ATOMIC_RELAXED,
                              __HIP_MEMORY_SCOPE_AGENT);
   };
-  constexpr int AHEAD = 8;  // parts whose loads are on their way together
+  constexpr int AHEAD = Q8 ? 16 : 8;  // parts whose loads are on their way together
   for (int idx = tid; idx < rows * (PG_DH / 2); idx += 64 * DW) {
     const int row = idx / (PG_DH / 2), d = 2 * (idx % (PG_DH / 2));
     float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
@@ -717,11 +717,11 @@ __device__ __forceinline__ void few_rows(const AttendParams& p, int wg, int wgs,
   if (tid == 0) p.counters[b * p.Hkv + kvh] = 0;
 }
 
-template <int DT, int ODT, bool Q8>
-__global__ __launch_bounds__(512, 2) void paged_few_kernel(AttendParams p) {
-  __shared__ __attribute__((aligned(256))) uint8_t sRing[8 * DSLOT * DSLOT_BYTES];
+template <int DT, int ODT, bool Q8, int DW>
+__global__ __launch_bounds__(64 * DW, 2) void paged_few_kernel(AttendParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t sRing[DW * DSLOT * DSLOT_BYTES];
   __shared__ int sLast;
-  few_rows<DT, ODT, Q8, 8>(p, blockIdx.x, gridDim.x, sRing, &sLast);
+  few_rows<DT, ODT, Q8, DW>(p, blockIdx.x, gridDim.x, sRing, &sLast);
 }
 
 // ---- many rows: prompts and their chunks ----
@@ -931,7 +931,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const int k_end = __builtin_amdgcn_readfirstlane(
       max(0, min(r.len, r.pos0 + quot(p.by_hpg, min(q0 + BQ, rows) - 1) + 1)));
   const int w_first = r.pos0 + quot(p.by_hpg, min(wq0, rows - 1));
-  const int w_end = wq0 < rows ? r.pos0 + quot(p.by_hpg, min(wq0 + QW, rows) - 1) + 1 : 0;
+  const int w_end = __builtin_amdgcn_readfirstlane(
+      wq0 < rows ? r.pos0 + quot(p.by_hpg, min(wq0 + QW, rows) - 1) + 1 : 0);
   const int all_tiles = (k_end + CK - 1) / CK;
   const int per = cut ? quot(c.by_splits, all_tiles + c.splits - 1) : all_tiles;
   const int t0 = min(all_tiles, split * per), n_tiles = min(all_tiles, t0 + per);
@@ -992,14 +993,17 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const uint16_t* k_head = p.k + (long long)kvh * p.pool.head_stride;
   const uint16_t* v_head = p.v + (long long)kvh * p.pool.head_stride;
   const int key_in_tile = blk * 16 + sub, slot_mask = p.pool.page_size - 1;
+  auto keys_from = [&](int key) {  // the wave's keys of a tile, 0 .. CK / NW
+    int keys;  // as scalar instructions: the compiler would clamp in a vector register
+    asm("s_max_i32 %0, %1, 0" : "=s"(keys) : "s"(k_end - key) : "scc");
+    asm("s_min_i32 %0, %1, %2" : "=s"(keys) : "s"(keys), "n"(CK / NW) : "scc");
+    return keys;
+  };
   auto issue = [&](int t, int page) {  // (scalar work, a wave's by itself: every instruction counts)
     const int key = t * CK + key_in_tile;
     const long long at = (long long)max(page, 0) * p.pool.page_stride +
                          (long long)((key & slot_mask) * PG_DH);
-    int keys;  // as scalar instructions: the compiler would clamp in a vector register
-    asm("s_max_i32 %0, %1, 0" : "=s"(keys) : "s"(k_end - key) : "scc");
-    asm("s_min_i32 %0, %1, %2" : "=s"(keys) : "s"(keys), "n"(CK / NW) : "scc");
-    const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys * (PG_DH * 2);
+    const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys_from(key) * (PG_DH * 2);
     pg_lds_loads<false>(dkv_make_rsrc(k_head + at, bytes),
                         dkv_lds_addr(sK(t & 1)) + CK / NW * wave * 256, voff);
     pg_lds_loads<false>(dkv_make_rsrc(v_head + at, bytes),
@@ -1014,10 +1018,10 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   uint32_t c_scales = 0x7f7f;
   auto fetch = [&](int t, int page, uint32_t s) {
     const int key = t * CK + key_in_tile;
-    const long long at = (long long)max(page, 0) * p.pool.page_stride +
-                         (long long)((key & slot_mask) * PG_DH);
-    const int keys = min(max(k_end - key, 0), CK / NW);
-    const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys * PG_DH;
+    // (the wave's, and told so: else every load would come in a loop over its lanes' resources)
+    const int in_page = __builtin_amdgcn_readfirstlane((key & slot_mask) * PG_DH);
+    const long long at = (long long)max(page, 0) * p.pool.page_stride + in_page;
+    const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys_from(key) * PG_DH;
     const __amdgpu_buffer_rsrc_t rk =
         dkv_make_rsrc((const uint8_t*)p.k + (long long)kvh * p.pool.head_stride + at, bytes);
     const __amdgpu_buffer_rsrc_t rv =
@@ -1029,23 +1033,40 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       cv[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, 1024 * i + 16 * lane, 0, 0);
     }
   };
-  auto place = [&](int t) {  // the fetched part, into tile t's buffers
-    const float sk = pg_scale(c_scales & 0xffu), sv = pg_scale(c_scales >> 8);
+  typedef __attribute__((address_space(3))) dkv_u32x4 lds_u32x4;
+  const uint32_t place0 = dkv_lds_addr(sKV);
+  uint32_t place_off[CW][2];
 #pragma unroll
-    for (int i = 0; i < CW; ++i) {
+  for (int i = 0; i < CW; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
       const int kk = sub + 8 * i + (lane >> 3);  // key of the block
-      const uint32_t row = (uint32_t)(blk * 16 + kk) * 256;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t to = row + 16 * ((2 * (lane & 7) + e) ^ kk);
-        auto wide = [&](const dkv_u32x4& w, float s) {
-          return dkv_u32x4{pg_pair<DT, false>(w[2 * e], s), pg_pair<DT, true>(w[2 * e], s),
-                           pg_pair<DT, false>(w[2 * e + 1], s), pg_pair<DT, true>(w[2 * e + 1], s)};
-        };
-        *(dkv_u32x4*)(sK(t & 1) + to) = wide(ck[i], sk);
-        *(dkv_u32x4*)(sV(t & 1) + to) = wide(cv[i], sv);
-      }
+      place_off[i][e] = (uint32_t)((blk * 16 + kk) * 256 + 16 * ((2 * (lane & 7) + e) ^ kk));
     }
+  // a fourth of what was fetched (or half: x of 2 CW), into tile t's buffers
+  auto place = [&](int t, int x) {
+    const int i = x >> 1;
+    const dkv_u32x4 w = x & 1 ? cv[i] : ck[i];
+    const float s = pg_scale(x & 1 ? c_scales >> 8 : c_scales & 0xffu);
+    const uint32_t base = place0 + (uint32_t)(t & 1) * CTILE_BYTES;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *(lds_u32x4*)(base + (uint32_t)(x & 1) * 2 * CTILE_BYTES + place_off[i][e]) =
+          dkv_u32x4{pg_pair<DT, false>(w[2 * e], s), pg_pair<DT, true>(w[2 * e], s),
+                    pg_pair<DT, false>(w[2 * e + 1], s), pg_pair<DT, true>(w[2 * e + 1], s)};
+  };
+  // tile t's fetch; pages and scales of the next 16 tiles come two tiles before the products need them
+  auto fetch_ahead = [&](int t) {
+    const int u = (t - t0) & 15;
+    if (u == 0) {
+      ids = ids_next;
+      scales = scales_next;
+      absent_next = absent_of(t);
+      if (t + 16 < n_tiles) ids_next = fetch_ids(t + 16);
+    }
+    if (u == 8 && t + 8 < n_tiles) scales_next = fetch_scales(t + 8, ids_next);
+    fetch(t, __builtin_amdgcn_readlane(ids, 4 * u + blk),
+          __builtin_amdgcn_readlane(scales, 4 * u + blk));
   };
 
   dkv_f32x4 acc[QB][8];
@@ -1068,7 +1089,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   // S^T of key block kb: A = K rows (lane: key 16kb + n, dims 32s + 8g .. +8), B = Q^T; lane (row n,
   // g) then holds keys 16kb + 4g + u, unscaled
   const uint32_t krd = n * 256 + 16 * (g ^ n);
-  typedef __attribute__((address_space(3))) dkv_u32x4 lds_u32x4;
   // transposed V reads: lane 4i + q of each 16 reads key 16kb + 4g + i, dims 16db + 4q .. +3; lane i
   // then holds dim 16db + i of keys 4g .. 4g + 3
   const uint32_t vrd =
@@ -1077,7 +1097,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   if constexpr (Q8) {
     if (t0 < n_tiles) {
       fetch(t0, __builtin_amdgcn_readlane(ids, blk), __builtin_amdgcn_readlane(scales, blk));
-      place(t0);
+#pragma unroll
+      for (int x = 0; x < 2 * CW; ++x) place(t0, x);
     }
     if (t0 + 1 < n_tiles)
       fetch(t0 + 1, __builtin_amdgcn_readlane(ids, 4 + blk),
@@ -1101,34 +1122,29 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         absent = absent_next;
       }
       gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
-      if (t + 1 < n_tiles) place(t + 1);
-      if (t + 2 < n_tiles) {
-        // (pages and scales of the next 16 tiles, two tiles before the products are at them)
-        const int u = t + 2 - t0;
-        if ((u & 15) == 0) {
-          ids = ids_next;
-          scales = scales_next;
-          absent_next = absent_of(t + 2);
-          if (t + 2 + 16 < n_tiles) ids_next = fetch_ids(t + 2 + 16);
-        }
-        if ((u & 15) == 8 && t + 2 + 8 < n_tiles) scales_next = fetch_scales(t + 2 + 8, ids_next);
-        fetch(t + 2, __builtin_amdgcn_readlane(ids, 4 * (u & 15) + blk),
-              __builtin_amdgcn_readlane(scales, 4 * (u & 15) + blk));
-      }
     } else {
-    gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
-    if (t + 1 < n_tiles) {
-      if (t + 1 == ids_base + 16) {
-        ids_base += 16;
-        ids = ids_next;
-        absent = absent_of(ids_base);
-        if (ids_base + 16 < n_tiles) ids_next = fetch_ids(ids_base + 16);
+      gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
+      if (t + 1 < n_tiles) {
+        if (t + 1 == ids_base + 16) {
+          ids_base += 16;
+          ids = ids_next;
+          absent = absent_of(ids_base);
+          if (ids_base + 16 < n_tiles) ids_next = fetch_ids(ids_base + 16);
+        }
+        issue(t + 1, __builtin_amdgcn_readlane(ids, 4 * (t + 1 - ids_base) + blk));
       }
-      issue(t + 1, __builtin_amdgcn_readlane(ids, 4 * (t + 1 - ids_base) + blk));
-    }
     }
     const int key0 = t * CK;
-    if (key0 >= w_end) continue;  // every key of the tile is past the wave's rows
+    if (key0 >= w_end) {  // every key of the tile is past the wave's rows
+      if constexpr (Q8) {
+        if (t + 1 < n_tiles) {
+#pragma unroll
+          for (int x = 0; x < 2 * CW; ++x) place(t + 1, x);
+        }
+        if (t + 2 < n_tiles) fetch_ahead(t + 2);
+      }
+      continue;
+    }
     const uint32_t kt = dkv_lds_addr(sK(t & 1));
     const uint32_t vt = dkv_lds_addr(sV(t & 1)) + vrd;
     dkv_f32x4 z[QB][4];
@@ -1143,8 +1159,15 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_mfma32<DT>(a, qop[qb][s], z[qb][kb]);
       }
+      // (among the products; after the last tile what was fetched before goes where nobody reads it)
+      if constexpr (Q8) {
+        if (kb < 2 * CW) place(t + 1, kb);
+      }
     }
     __builtin_amdgcn_s_setprio(0);
+    if constexpr (Q8) {
+      if (t + 2 < n_tiles) fetch_ahead(t + 2);
+    }
     if (key0 + CK - 1 > w_first || key0 + CK > r.len || gone) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
@@ -1432,7 +1455,7 @@ namespace {
 // The launches of a call, from its bounds alone.
 struct AttendPlan {
   bool few, many;          // kernels that run
-  int few_wgs, few_split;
+  int few_wgs, few_split, few_waves;
   int qb, nw, bq, splits;
   int items, more;         // row tiles cut into key ranges, and further ones that are not
   long long many_at;       // the many-row kind's records, in floats from the others'
@@ -1464,10 +1487,12 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
   a.many = (long long)max_new * hpg > DROWS;
   if (a.few) {
     const int tile = q8 ? DTILE<true> : DTILE<false>;
+    a.few_waves = q8 && units >= D_WAVES / 8 && units < D_WAVES / 4 && !a.many ? 4 : 8;
+    const int fill = D_WAVES / a.few_waves;
     const long long tiles = ((long long)max_len + tile - 1) / tile;
     const long long most = units * ((tiles + D_MIN_TILES - 1) / D_MIN_TILES);
     long long wgs = units;
-    if (wgs < D_WGS) wgs = most < D_WGS ? (most > units ? most : units) : D_WGS;
+    if (wgs < fill && B <= D_SPLIT_B) wgs = most < fill ? (most > units ? most : units) : fill;
     a.few_split = wgs > units;
     a.few_wgs = (int)wgs;
     if (a.few_split) floats = wgs * DREC;
@@ -1544,7 +1569,12 @@ void launch_attend(const AttendPlan& a, const ChunkParams& c, hipStream_t st) {
       hipLaunchKernelGGL((paged_mixed_kernel<DT, ODT, Q8, 1>), grid, dim3(256), 0, st, c, a.few_wgs,
                          many);
   } else if (a.few) {
-    hipLaunchKernelGGL((paged_few_kernel<DT, ODT, Q8>), dim3((unsigned)a.few_wgs), dim3(512), 0, st, c.a);
+    if (Q8 && a.few_waves == 4)
+      hipLaunchKernelGGL((paged_few_kernel<DT, ODT, true, 4>), dim3((unsigned)a.few_wgs), dim3(256),
+                         0, st, c.a);
+    else
+      hipLaunchKernelGGL((paged_few_kernel<DT, ODT, Q8, 8>), dim3((unsigned)a.few_wgs), dim3(512), 0,
+                         st, c.a);
   } else {
     const dim3 grid((unsigned)many);
     if (a.qb == 2)
