@@ -1134,15 +1134,15 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         issue(t + 1, __builtin_amdgcn_readlane(ids, 4 * (t + 1 - ids_base) + blk));
       }
     }
+    if constexpr (Q8) {
+      if (t + 1 < n_tiles) {
+#pragma unroll
+        for (int x = 0; x < 2 * CW; ++x) place(t + 1, x);
+      }
+      if (t + 2 < n_tiles) fetch_ahead(t + 2);
+    }
     const int key0 = t * CK;
     if (key0 >= w_end) {  // every key of the tile is past the wave's rows
-      if constexpr (Q8) {
-        if (t + 1 < n_tiles) {
-#pragma unroll
-          for (int x = 0; x < 2 * CW; ++x) place(t + 1, x);
-        }
-        if (t + 2 < n_tiles) fetch_ahead(t + 2);
-      }
       continue;
     }
     const uint32_t kt = dkv_lds_addr(sK(t & 1));
@@ -1160,14 +1160,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_mfma32<DT>(a, qop[qb][s], z[qb][kb]);
       }
       // (among the products; after the last tile what was fetched before goes where nobody reads it)
-      if constexpr (Q8) {
-        if (kb < 2 * CW) place(t + 1, kb);
-      }
     }
     __builtin_amdgcn_s_setprio(0);
-    if constexpr (Q8) {
-      if (t + 2 < n_tiles) fetch_ahead(t + 2);
-    }
     if (key0 + CK - 1 > w_first || key0 + CK > r.len || gone) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
