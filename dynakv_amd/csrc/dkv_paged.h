@@ -29,6 +29,16 @@ __device__ __forceinline__ int quot(const Divisor& v, int x) {
   return v.d == 1 ? x : (int)q;
 }
 
+__device__ __forceinline__ int pg_wave_scan(int v) {  // inclusive, as dkv_wave_scan_fast
+  v += dkv_dpp_i32<0x111>(v);
+  v += dkv_dpp_i32<0x112>(v);
+  v += dkv_dpp_i32<0x114>(v);
+  v += dkv_dpp_i32<0x118>(v);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 struct PagedPool {
   long long page_stride, head_stride;  // elements
   int num_pages, page_size, page_shift;

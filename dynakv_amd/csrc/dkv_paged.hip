@@ -215,15 +215,6 @@ template <int DT>                           // log2 units the running maximum ma
 constexpr float D_RESCALE = DT == DKV_F16 ? PG_F16_RESCALE : 11.5f;
 
 __device__ __forceinline__ int pg_wave_sum(int v) { return dkv_wave_sum_fast_i(v); }
-__device__ __forceinline__ int pg_wave_scan(int v) {  // inclusive, as dkv_wave_scan_fast
-  v += dkv_dpp_i32<0x111>(v);
-  v += dkv_dpp_i32<0x112>(v);
-  v += dkv_dpp_i32<0x114>(v);
-  v += dkv_dpp_i32<0x118>(v);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
-}
 __device__ __forceinline__ PagedRequest pg_lane(const PagedRequest& r, int l) {  // lane l's, for all
   return {__builtin_amdgcn_readlane(r.row0, l), __builtin_amdgcn_readlane(r.n, l),
           __builtin_amdgcn_readlane(r.len, l), __builtin_amdgcn_readlane(r.pos0, l)};

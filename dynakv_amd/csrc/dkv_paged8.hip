@@ -26,9 +26,10 @@ constexpr int E_HIGH = DT == DKV_F16 ? 7 : 119;
 // Keys are computed in 64 bits: which code a value gets turns over at borders, and 32-bit arithmetic with
 // the sine instruction put 350 of 8 million keys on another side of one.
 //
-// A wave has one block and head: lane (token i = lane / 8 of eight, twice; piece c = lane % 8) holds dims
-// 8c .. 8c + 7 and 64 + 8c .. 64 + 8c + 7. Eight waves (K heads, then V heads) share the block's sines and
-// cosines in LDS. Queries go to further workgroups of the launch, a wave per row and 8 heads.
+// Two waves have one block and head (a unit: K heads, then V heads), eight tokens each: lane (token
+// lane / 8, piece c = lane % 8) holds dims 8c .. 8c + 7 and 64 + 8c .. 64 + 8c + 7. The four units of a
+// workgroup share the block's sines and cosines in LDS. Queries go to further workgroups of the
+// launch, a wave per row and 8 heads.
 // ---------------------------------------------------------------------------------------
 struct Append8Params {
   const uint16_t* qkv;
@@ -44,7 +45,7 @@ struct Append8Params {
   const int* q_start;
   const int* lens;
   int B, T, Hq, Hkv;
-  int kv_wgs;      // leading workgroups: blocks times groups of eight units
+  int kv_wgs;      // leading workgroups: blocks times groups of units
   Divisor by_groups, by_q_groups;
   const uint16_t* q_norm;  // (128,), or null: no norm
   const uint16_t* k_norm;
@@ -52,7 +53,7 @@ struct Append8Params {
   double rev[PG_DH / 2];  // revolutions per position of each pair
 };
 
-constexpr int A8_WAVES = 8;
+constexpr int A8_WAVES = 8, A8_UNITS = 4;  // of a workgroup
 constexpr int A8_ROW = 72;  // pairs of doubles a token's sines and cosines take in LDS
 
 // A block with new tokens: tokens t_lo .. t_hi - 1 of request b, all in block [base, base + 16).
@@ -73,12 +74,7 @@ __device__ __forceinline__ NewBlock new_block(const Append8Params& p, int item, 
       off = r.row0 - r.pos0;
       if (r.n > 0 && hi > lo) count = (hi - 1) / PG_BLOCK - lo / PG_BLOCK + 1;
     }
-    int run = count;  // inclusive scan
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(run, o, 64);
-      if (lane >= o) run += x;
-    }
+    const int run = pg_wave_scan(count);
     const unsigned long long hit = __ballot(item < before + run);
     if (hit) {
       const int l = __ffsll((long long)hit) - 1;
@@ -164,187 +160,161 @@ __device__ __forceinline__ float float_for_e4m3(double d) {
   return f;
 }
 
+// Workgroup `wg`: one block, four units; wave w has unit w / 2, the tokens of half w % 2 of the block.
 template <int DT>
-__device__ __forceinline__ void append8_block(const Append8Params& p, int wg, double2* sTrig) {
+__device__ __forceinline__ void append8_block(const Append8Params& p, int wg, double2* sTrig,
+                                              int* sNeed) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i = lane >> 3, c = lane & 7;
+  const int c = lane & 7, slot = (wave & 1) * 8 + (lane >> 3);  // slot of the block
   const int groups = (int)p.by_groups.d;
   const int item = __builtin_amdgcn_readfirstlane(quot(p.by_groups, wg));
-  const int unit0 = (wg - item * groups) * A8_WAVES, unit = unit0 + wave;
+  const int unit0 = (wg - item * groups) * A8_UNITS, unit = unit0 + (wave >> 1);
   const NewBlock n = new_block(p, item, lane);
   if (n.b < 0) return;
+  const bool is_k = unit < p.Hkv, there = unit < 2 * p.Hkv;
+  const int t = n.base + slot;
+  const bool isnew = there && t >= n.t_lo && t < n.t_hi, isold = there && t < n.t_lo;
+  // the new row (before the page is known), then the earlier token's codes and the block's scale
+  dkv_u32x4 xa = {0u, 0u, 0u, 0u}, xb = {0u, 0u, 0u, 0u};
+  if (isnew) {
+    const uint16_t* src = p.qkv + (long long)(n.row_of_0 + t) * p.qkv_ld +
+                          (long long)(p.Hq + unit) * PG_DH + 8 * c;
+    xa = *(const dkv_u32x4*)src;
+    xb = *(const dkv_u32x4*)(src + 64);
+  }
   const int page = __builtin_amdgcn_readfirstlane(paged_page(p.pool, n.b, n.base));
   if (page < 0) return;
-  const bool is_k = unit < p.Hkv, there = unit < 2 * p.Hkv;
   const int head = is_k ? unit : unit - p.Hkv, slot0 = n.base & (p.pool.page_size - 1);
   uint8_t* codes = (is_k ? p.k : p.v) + (long long)page * p.pool.page_stride +
-                   (long long)head * p.pool.head_stride + (long long)slot0 * PG_DH + 8 * c;
+                   (long long)head * p.pool.head_stride + (long long)(slot0 + slot) * PG_DH + 8 * c;
   uint8_t* scale = (is_k ? p.k_scale : p.v_scale) + (long long)page * p.scale_page +
                    (long long)head * p.scale_head + slot0 / PG_BLOCK;
-  // the new rows, and the earlier tokens' codes
-  dkv_u32x4 xa[2], xb[2];
-  dkv_u32x2 oa[2], ob[2];
-  bool isnew[2], isold[2];
-  uint32_t old_byte = 127;
   const bool has_old = n.t_lo > n.base;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int t = n.base + 8 * s + i;
-    isnew[s] = there && t >= n.t_lo && t < n.t_hi;
-    isold[s] = there && t < n.t_lo;
-    xa[s] = xb[s] = dkv_u32x4{0u, 0u, 0u, 0u};
-    oa[s] = ob[s] = dkv_u32x2{0u, 0u};
-    if (isnew[s]) {
-      const uint16_t* src = p.qkv + (long long)(n.row_of_0 + t) * p.qkv_ld +
-                            (long long)(p.Hq + unit) * PG_DH + 8 * c;
-      xa[s] = *(const dkv_u32x4*)src;
-      xb[s] = *(const dkv_u32x4*)(src + 64);
-    }
-    if (isold[s]) {
-      oa[s] = *(const dkv_u32x2*)(codes + (8 * s + i) * PG_DH);
-      ob[s] = *(const dkv_u32x2*)(codes + (8 * s + i) * PG_DH + 64);
+  dkv_u32x2 oa = {0u, 0u}, ob = {0u, 0u};
+  uint32_t old_byte = 127;
+  if (has_old) {
+    if (there) old_byte = *scale;
+    if (isold) {
+      oa = *(const dkv_u32x2*)codes;
+      ob = *(const dkv_u32x2*)(codes + 64);
     }
   }
-  if (there && has_old) old_byte = *scale;
   if (unit0 < p.Hkv) {  // some of the waves have keys
     const int first = n.t_lo - n.base, pairs = (n.t_hi - n.t_lo) * (PG_DH / 2);
     for (int x = tid; x < pairs; x += 64 * A8_WAVES) {
-      const int t = first + x / (PG_DH / 2), j = x % (PG_DH / 2);
-      const double r = (double)(n.base + t) * p.rev[j];
+      const int s = first + x / (PG_DH / 2), j = x % (PG_DH / 2);
+      const double r = (double)(n.base + s) * p.rev[j];
       // (read below by piece j / 8 of the lanes, element j % 8)
-      sTrig[t * A8_ROW + (j % 8) * 8 + j / 8] = cos_sin_rev(r - floor(r));
+      sTrig[s * A8_ROW + (j % 8) * 8 + j / 8] = cos_sin_rev(r - floor(r));
     }
     __syncthreads();
   }
-  if (!there) return;
 
-  float f[2][16];  // y, or y scaled
-  double y[2][16];
-  double big = 0.0;
+  float f[16];  // y, then y scaled
+  double y[16], big = 0.0;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[s][2 * e] = dkv_elt_to_f32<DT>(xa[s][e] & 0xffffu);
-      f[s][2 * e + 1] = dkv_elt_to_f32<DT>(xa[s][e] >> 16);
-      f[s][8 + 2 * e] = dkv_elt_to_f32<DT>(xb[s][e] & 0xffffu);
-      f[s][8 + 2 * e + 1] = dkv_elt_to_f32<DT>(xb[s][e] >> 16);
-    }
+  for (int e = 0; e < 4; ++e) {
+    f[2 * e] = dkv_elt_to_f32<DT>(xa[e] & 0xffffu);
+    f[2 * e + 1] = dkv_elt_to_f32<DT>(xa[e] >> 16);
+    f[8 + 2 * e] = dkv_elt_to_f32<DT>(xb[e] & 0xffffu);
+    f[8 + 2 * e + 1] = dkv_elt_to_f32<DT>(xb[e] >> 16);
   }
   if (is_k) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (n.base + 8 * s + 8 <= n.t_lo || n.base + 8 * s >= n.t_hi) {  // (the wave's)
+    for (int e = 0; e < 16; ++e) y[e] = (double)f[e];
+    if (p.k_norm) {
+      double ss = 0.0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[s][e] = 0.0;
-        continue;
-      }
+      for (int e = 0; e < 16; ++e) ss = fma(y[e], y[e], ss);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) y[s][e] = (double)f[s][e];
-      if (p.k_norm) {
-        double ss = 0.0;
+      for (int o = 1; o <= 4; o <<= 1) ss += __shfl_xor(ss, o, 64);
+      const double inv = 1.0 / sqrt(ss * (1.0 / PG_DH) + (double)p.eps);
+      float wx[8], wy[8];
+      load8<DT>(p.k_norm + 8 * c, wx);
+      load8<DT>(p.k_norm + 64 + 8 * c, wy);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ss = fma(y[s][e], y[s][e], ss);
-#pragma unroll
-        for (int o = 1; o <= 4; o <<= 1) ss += __shfl_xor(ss, o, 64);
-        const double inv = 1.0 / sqrt(ss * (1.0 / PG_DH) + (double)p.eps);
-        float wx[8], wy[8];
-        load8<DT>(p.k_norm + 8 * c, wx);
-        load8<DT>(p.k_norm + 64 + 8 * c, wy);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          y[s][e] = y[s][e] * inv * (double)wx[e];
-          y[s][8 + e] = y[s][8 + e] * inv * (double)wy[e];
-        }
-      }
-      if (isnew[s]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double2 cs = sTrig[(8 * s + i) * A8_ROW + 8 * e + c];
-          const double u = y[s][e], w = y[s][8 + e];
-          y[s][e] = fma(u, cs.x, -(w * cs.y));
-          y[s][8 + e] = fma(w, cs.x, u * cs.y);
-          big = fmax(big, fmax(fabs(y[s][e]), fabs(y[s][8 + e])));
-        }
+      for (int e = 0; e < 8; ++e) {
+        y[e] = y[e] * inv * (double)wx[e];
+        y[8 + e] = y[8 + e] * inv * (double)wy[e];
       }
     }
-    if (!(big < INFINITY)) {  // without what is not finite
-      big = 0.0;
+    if (isnew) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int e = 0; e < 8; ++e) {
+        const double2 cs = sTrig[slot * A8_ROW + 8 * e + c];
+        const double u = y[e], w = y[8 + e];
+        y[e] = fma(u, cs.x, -(w * cs.y));
+        y[8 + e] = fma(w, cs.x, u * cs.y);
+        big = fmax(big, fmax(fabs(y[e]), fabs(y[8 + e])));
+      }
+      if (!(big < INFINITY)) {  // without what is not finite
+        big = 0.0;
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (isnew[s] && fabs(y[s][e]) < INFINITY) big = fmax(big, fabs(y[s][e]));
+          if (fabs(y[e]) < INFINITY) big = fmax(big, fabs(y[e]));
+      }
     }
   } else {
     float m = 0.f;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(f[s][e]));
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(f[e]));
     if (!(m < INFINITY)) {
       m = 0.f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (fabsf(f[s][e]) < INFINITY) m = fmaxf(m, fabsf(f[s][e]));
+      for (int e = 0; e < 16; ++e)
+        if (fabsf(f[e]) < INFINITY) m = fmaxf(m, fabsf(f[e]));
     }
     big = (double)m;
   }
-  const int need = (int)dkv_wave_max_fast((float)exponent_of(big));  // (small whole numbers)
+  // the block's exponent, from both halves
+  int need = (int)dkv_wave_max_fast((float)exponent_of(big));  // (small whole numbers)
+  if (lane == 0) sNeed[wave] = need;
+  __syncthreads();
+  if (!there) return;
+  need = max(need, sNeed[wave ^ 1]);
   const int old_e = min(max((int)old_byte - 127, E_LOW<DT>), E_HIGH<DT>);
   int e_new = min(max(need, E_LOW<DT>), E_HIGH<DT>);
   if (has_old) e_new = max(e_new, old_e);
   e_new = __builtin_amdgcn_readfirstlane(e_new);
 
-  if (is_k) {
-    const double by = pow2(-e_new);
+  if (isnew) {
+    if (is_k) {
+      const double by = pow2(-e_new);
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int e = 0; e < 16; ++e) f[e] = float_for_e4m3(y[e] * by);
+    } else {
+      const float by = __uint_as_float((uint32_t)(127 - e_new) << 23);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) f[s][e] = float_for_e4m3(y[s][e] * by);
-  } else {
-    const float by = __uint_as_float((uint32_t)(127 - e_new) << 23);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) f[s][e] *= by;
-  }
-  const bool lower = has_old && e_new > old_e;
-  const float down = lower ? __uint_as_float((uint32_t)max(127 + old_e - e_new, 0) << 23) : 1.f;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    uint8_t* at = codes + (8 * s + i) * PG_DH;
-    if (isnew[s]) {
-      *(dkv_u32x2*)at = encode8(f[s]);
-      *(dkv_u32x2*)(at + 64) = encode8(f[s] + 8);
-    } else if (isold[s] && lower) {
-      float g[16];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        g[4 * h] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 0) * down;
-        g[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 1) * down;
-        g[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 2) * down;
-        g[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(oa[s][h], 3) * down;
-        g[8 + 4 * h] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 0) * down;
-        g[8 + 4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 1) * down;
-        g[8 + 4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 2) * down;
-        g[8 + 4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(ob[s][h], 3) * down;
-      }
-      *(dkv_u32x2*)at = encode8(g);
-      *(dkv_u32x2*)(at + 64) = encode8(g + 8);
+      for (int e = 0; e < 16; ++e) f[e] *= by;
     }
+    *(dkv_u32x2*)codes = encode8(f);
+    *(dkv_u32x2*)(codes + 64) = encode8(f + 8);
+  } else if (isold && e_new > old_e) {
+    const float down = __uint_as_float((uint32_t)max(127 + old_e - e_new, 0) << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f[4 * h] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 0) * down;
+      f[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 1) * down;
+      f[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 2) * down;
+      f[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 3) * down;
+      f[8 + 4 * h] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 0) * down;
+      f[8 + 4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 1) * down;
+      f[8 + 4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 2) * down;
+      f[8 + 4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 3) * down;
+    }
+    *(dkv_u32x2*)codes = encode8(f);
+    *(dkv_u32x2*)(codes + 64) = encode8(f + 8);
   }
-  if (lane == 0) *scale = (uint8_t)(127 + e_new);
+  if (lane == 0 && !(wave & 1)) *scale = (uint8_t)(127 + e_new);
 }
 
 template <int DT>
 __global__ __launch_bounds__(64 * A8_WAVES) void paged_append8_kernel(Append8Params p) {
   __shared__ double2 sTrig[PG_BLOCK * A8_ROW];
+  __shared__ int sNeed[A8_WAVES];
   if ((int)blockIdx.x < p.kv_wgs) {
-    append8_block<DT>(p, blockIdx.x, sTrig);
+    append8_block<DT>(p, blockIdx.x, sTrig, sNeed);
     return;
   }
   const int lane = threadIdx.x & 63;
@@ -500,7 +470,7 @@ extern "C" int dkv_paged_append8(void* stream, int dtype, const void* qkv, long 
   for (int j = 0; j < PG_DH / 2; ++j) p.rev[j] = inv_freq[j] * 0.15915494309189533577;
   // n new tokens touch at most n blocks and at most n / 16 + 2
   const long long some = T / PG_BLOCK + 2LL * (B < T ? B : T), blocks = some < T ? some : T;
-  const int groups = (2 * Hkv + A8_WAVES - 1) / A8_WAVES, q_groups = (Hq + 7) / 8;
+  const int groups = (2 * Hkv + A8_UNITS - 1) / A8_UNITS, q_groups = (Hq + 7) / 8;
   const long long q_items = (long long)T * q_groups;
   const long long wgs = blocks * groups + (q_items + A8_WAVES - 1) / A8_WAVES;
   if (wgs > 0x7fffffffLL || q_items > 0x7fffffffLL - A8_WAVES) return DKV_E_UNSUPPORTED;
