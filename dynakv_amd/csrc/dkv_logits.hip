@@ -15,11 +15,16 @@ namespace {
 // A token that nothing of this concerns is neither read nor written: a row of 128256 logits with a history
 // of a few thousand tokens is a few thousand reads and writes.
 //
-// A workgroup has `span` tokens of a row's vocabulary and counts in LDS (a word each: the generated ones
-// below the bit that says it was seen) those of the history that fall into it; every workgroup of a row
-// reads the whole history. Biases go by their entries: the first one of a token claims it (least entry
-// by an atomic, whatever the order), sums the token's further ones in order and applies them, so that
-// the same call gives the same bits.
+// A workgroup has a row and a table in LDS of the tokens that its history and its biases name: open
+// addressing, at most three quarters full, a word for the token, one for its number (the generated ones
+// below the bit that says it was seen) and one for its biases. What it holds at the end does not depend
+// on the order of its atomics. Biases go by their entries: the first one of a token claims it (least
+// entry), sums the token's further ones in order and applies them, so that the same call gives the same
+// bits. The mask is for other workgroups of the launch, which clear the tokens that it forbids, and only
+// those; the rows' workgroups look their tokens up in it.
+//
+// Histories that no table of 64 KB holds (over 6144 tokens) are counted by vocabulary instead: a
+// workgroup has `span` tokens of a row's vocabulary, a word each, and reads the whole history.
 // ---------------------------------------------------------------------------------------
 struct LogitParams {
   void* logits;
@@ -44,6 +49,9 @@ struct LogitParams {
   const uint32_t* allowed;  // null: no mask
   long long allowed_ld;
   int span, slices;
+  int slots_log2;  // of the table; by vocabulary: 0
+  int row_wgs;     // leading workgroups, each with a row; then those of the mask
+  int mask_wgs;    // of a row
 };
 
 constexpr int L_THREADS = 512;
@@ -53,8 +61,193 @@ constexpr uint32_t L_SEEN = 0x80000000u;
 constexpr uint32_t L_NONE = 0x7fffffffu;  // no entry
 constexpr uint32_t L_MORE = 0x80000000u;  // further entries of the same token
 
+constexpr int L_MASK = 8;            // tokens of a thread in a mask's workgroup
+
 template <int DT>
-__global__ __launch_bounds__(L_THREADS) void adjust_kernel(LogitParams p) {
+__device__ __forceinline__ float load_logit(__amdgpu_buffer_rsrc_t r, int at) {
+  if constexpr (DT == DKV_F32)
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
+  else
+    return dkv_elt_to_f32<DT>(__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
+}
+template <int DT>
+__device__ __forceinline__ void store_logit(__amdgpu_buffer_rsrc_t r, int at, float y) {
+  if constexpr (DT == DKV_F32)
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y), r, at, 0, 0);
+  else if constexpr (DT == DKV_F16)
+    __builtin_amdgcn_raw_buffer_store_b16((uint16_t)dkv_f32_to_f16_bits(y), r, at, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b16((uint16_t)dkv_f32_to_bf16_bits(y), r, at, 0, 0);
+}
+
+// A row's settings, and its biases.
+struct LogitRow {
+  float rep, freq, pres;
+  int n, prompt;
+  const int* ids;
+  const float* bias;
+};
+__device__ __forceinline__ LogitRow logit_row(const LogitParams& p, int row) {
+  LogitRow r = {1.f, 0.f, 0.f, 0, 0, nullptr, nullptr};
+  if (p.tokens) {
+    r.rep = p.repetition ? p.repetition[row] : p.repetition_all;
+    r.freq = p.frequency ? p.frequency[row] : p.frequency_all;
+    r.pres = p.presence ? p.presence[row] : p.presence_all;
+    r.n = min(p.len ? p.len[row] : p.len_all, p.N);
+    r.prompt = p.prompt ? p.prompt[row] : p.prompt_all;
+  }
+  if (p.bias_ids) {
+    r.ids = p.bias_ids + (long long)row * p.bias_ids_ld;
+    r.bias = p.bias + (long long)row * p.bias_ld;
+  }
+  return r;
+}
+// Entry j of the row's history, or -1 where it is no token of the vocabulary.
+__device__ __forceinline__ int history(const LogitParams& p, int row, int j) {
+  if (p.wide) {
+    const long long t = ((const long long*)p.tokens)[(long long)row * p.tokens_ld + j];
+    return t >= 0 && t < p.V ? (int)t : -1;
+  }
+  const int t = ((const int*)p.tokens)[(long long)row * p.tokens_ld + j];
+  return t < p.V ? t : -1;
+}
+// What becomes of logit x of token id, of count c (0: not in the history) and bias entry e, bias b.
+__device__ __forceinline__ float adjusted(const LogitParams& p, const LogitRow& r, float x, int id,
+                                          uint32_t c, uint32_t e, float b) {
+  if (c) {
+    const uint32_t times = c & ~L_SEEN;
+    x = x > 0.f ? x / r.rep : x * r.rep;
+    x = x - r.freq * (float)times - (times ? r.pres : 0.f);
+  }
+  if (e != L_NONE) {
+    const int j = (int)(e & ~L_MORE);
+    float sum = b;
+    if (e & L_MORE)
+      for (int k = j + 1; k < p.M; ++k)
+        if (r.ids[k] == id) sum += r.bias[k];
+    x += sum;
+  }
+  return x;
+}
+
+template <int DT>
+__global__ __launch_bounds__(1024) void adjust_rows_kernel(LogitParams p) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  constexpr int SIZE = DT == DKV_F32 ? 4 : 2;
+  const int tid = threadIdx.x, T = blockDim.x;
+  if ((int)blockIdx.x >= p.row_wgs) {  // the mask of some tokens of a row
+    const int x = blockIdx.x - p.row_wgs, row = x / p.mask_wgs;
+    const int v0 = (x - row * p.mask_wgs) * (T * L_MASK), span = min(T * L_MASK, p.V - v0);
+    const __amdgpu_buffer_rsrc_t r = dkv_make_rsrc(
+        (uint8_t*)p.logits + ((long long)row * p.ld + v0) * SIZE, (uint32_t)span * SIZE);
+    const uint32_t* words = p.allowed + (long long)row * p.allowed_ld + v0 / 32;
+    uint32_t w[L_MASK];
+#pragma unroll
+    for (int u = 0; u < L_MASK; ++u) {
+      const int i = tid + u * T;
+      w[u] = i < span ? words[i >> 5] : 0xffffffffu;
+    }
+#pragma unroll
+    for (int u = 0; u < L_MASK; ++u) {
+      const int i = tid + u * T;
+      store_logit<DT>(r, (w[u] >> (i & 31)) & 1u ? DKV_OOB : i * SIZE, -INFINITY);
+    }
+    return;
+  }
+  const int row = blockIdx.x, slots = 1 << p.slots_log2;
+  uint32_t *key = lds, *count = lds + slots, *entry = lds + 2 * slots;
+  for (int i = 4 * tid; i < 2 * slots; i += 4 * T)  // (key: the token + 1, 0 where none is)
+    *(dkv_u32x4*)(lds + i) = dkv_u32x4{0u, 0u, 0u, 0u};
+  if (p.bias_ids)
+    for (int i = 4 * tid; i < slots; i += 4 * T)
+      *(dkv_u32x4*)(entry + i) = dkv_u32x4{L_NONE, L_NONE, L_NONE, L_NONE};
+  // the first of the history and of the biases, whose number is not known yet, beside the settings
+  int first[L_EACH], first_bias = -1;
+  if (p.tokens)
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      const int j = tid + u * T;
+      first[u] = j < p.N ? history(p, row, j) : -1;
+    }
+  if (p.bias_ids && tid < p.M) first_bias = p.bias_ids[(long long)row * p.bias_ids_ld + tid];
+  const LogitRow r = logit_row(p, row);
+  __syncthreads();
+  auto place = [&](int id) {  // the token's slot (there is a free one: fewer tokens than slots)
+    uint32_t i = (uint32_t)id * 2654435769u >> (32 - p.slots_log2);
+    for (;;) {
+      uint32_t k = *(volatile uint32_t*)(key + i);
+      if (k == 0) k = atomicCAS(key + i, 0u, (uint32_t)id + 1u);
+      if (k == 0 || k == (uint32_t)id + 1u) return i;
+      i = (i + 1) & (uint32_t)(slots - 1);
+    }
+  };
+  for (int j0 = tid; j0 < r.n; j0 += L_EACH * T) {
+    int id[L_EACH];
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      const int j = j0 + u * T;
+      id[u] = j >= r.n ? -1 : j0 == tid ? first[u] : history(p, row, j);
+    }
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      if (id[u] < 0) continue;
+      const uint32_t i = place(id[u]);
+      if (j0 + u * T < r.prompt)
+        atomicOr(count + i, L_SEEN);
+      else
+        atomicAdd(count + i, 1u);
+    }
+  }
+  if (p.bias_ids) {
+    auto biased = [&](int j) {  // entry j's token, or -1
+      const int id = j == tid ? first_bias : r.ids[j];
+      return id < p.V ? id : -1;
+    };
+    uint32_t mine = 0;  // slot of entry tid
+    for (int j = tid; j < p.M; j += T)
+      if (biased(j) >= 0) {
+        const uint32_t i = place(biased(j));
+        if (j == tid) mine = i;
+        atomicMin(entry + i, (uint32_t)j);
+      }
+    __syncthreads();
+    for (int j = tid; j < p.M; j += T)
+      if (biased(j) >= 0) {
+        const uint32_t i = j == tid ? mine : place(biased(j));
+        if ((entry[i] & ~L_MORE) != (uint32_t)j) atomicOr(entry + i, L_MORE);
+      }
+  }
+  __syncthreads();
+  const __amdgpu_buffer_rsrc_t logits =
+      dkv_make_rsrc((uint8_t*)p.logits + (long long)row * p.ld * SIZE, (uint32_t)p.V * SIZE);
+  for (int i0 = tid; i0 < slots; i0 += L_EACH * T) {
+    int id[L_EACH];
+    float x[L_EACH], b[L_EACH];
+    uint32_t word[L_EACH], e[L_EACH];
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      const int i = i0 + u * T;
+      id[u] = i < slots ? (int)key[i] - 1 : -1;
+      e[u] = p.bias_ids && id[u] >= 0 ? entry[i] : L_NONE;
+      b[u] = e[u] != L_NONE ? r.bias[e[u] & ~L_MORE] : 0.f;
+      x[u] = load_logit<DT>(logits, id[u] >= 0 ? id[u] * SIZE : DKV_OOB);
+      word[u] = 0xffffffffu;
+      if (p.allowed && id[u] >= 0)
+        word[u] = p.allowed[(long long)row * p.allowed_ld + (id[u] >> 5)];
+    }
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      if (id[u] < 0) continue;
+      const int i = i0 + u * T;
+      float y = adjusted(p, r, x[u], id[u], count[i], e[u], b[u]);
+      if (!((word[u] >> (id[u] & 31)) & 1u)) y = -INFINITY;
+      store_logit<DT>(logits, id[u] * SIZE, y);
+    }
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(L_THREADS) void adjust_vocabulary_kernel(LogitParams p) {
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   constexpr int SIZE = DT == DKV_F32 ? 4 : 2;
   const int tid = threadIdx.x;
@@ -70,63 +263,48 @@ __global__ __launch_bounds__(L_THREADS) void adjust_kernel(LogitParams p) {
   if (p.bias_ids)
     for (int i = 4 * tid; i < p.span; i += 4 * L_THREADS)
       *(dkv_u32x4*)(entry + i) = dkv_u32x4{L_NONE, L_NONE, L_NONE, L_NONE};
-  float rep = 1.f, freq = 0.f, pres = 0.f;
-  int n = 0, prompt = 0;
-  if (p.tokens) {
-    rep = p.repetition ? p.repetition[row] : p.repetition_all;
-    freq = p.frequency ? p.frequency[row] : p.frequency_all;
-    pres = p.presence ? p.presence[row] : p.presence_all;
-    n = min(p.len ? p.len[row] : p.len_all, p.N);
-    prompt = p.prompt ? p.prompt[row] : p.prompt_all;
-  }
+  int first[L_EACH], first_bias = -1;  // (as in the kernel by rows)
+  if (p.tokens)
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      const int j = tid + u * L_THREADS;
+      first[u] = j < p.N ? history(p, row, j) : -1;
+    }
+  if (p.bias_ids && tid < p.M) first_bias = p.bias_ids[(long long)row * p.bias_ids_ld + tid];
+  const LogitRow r = logit_row(p, row);
   if (p.tokens || p.bias_ids) __syncthreads();
-  // history
-  if (p.wide) {
-    const long long* t = (const long long*)p.tokens + (long long)row * p.tokens_ld;
-#pragma unroll 4
-    for (int j = tid; j < n; j += L_THREADS) {
-      const unsigned long long i = (unsigned long long)(t[j] - v0);
-      if (i < (unsigned long long)span) {
-        if (j < prompt)
-          atomicOr(count + i, L_SEEN);
-        else
-          atomicAdd(count + i, 1u);
-      }
+  for (int j0 = tid; j0 < r.n; j0 += L_EACH * L_THREADS) {
+    int at[L_EACH];
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      const int j = j0 + u * L_THREADS;
+      at[u] = (j >= r.n ? -1 : j0 == tid ? first[u] : history(p, row, j)) - v0;
     }
-  } else {
-    const int* t = (const int*)p.tokens + (long long)row * p.tokens_ld;
-#pragma unroll 4
-    for (int j = tid; j < n; j += L_THREADS) {
-      const uint32_t i = (uint32_t)t[j] - (uint32_t)v0;
-      if (t[j] >= 0 && i < (uint32_t)span) {
-        if (j < prompt)
-          atomicOr(count + i, L_SEEN);
-        else
-          atomicAdd(count + i, 1u);
-      }
+#pragma unroll
+    for (int u = 0; u < L_EACH; ++u) {
+      if (at[u] < 0 || at[u] >= span) continue;
+      if (j0 + u * L_THREADS < r.prompt)
+        atomicOr(count + at[u], L_SEEN);
+      else
+        atomicAdd(count + at[u], 1u);
     }
   }
-  // biases
-  const int* ids = nullptr;
-  const float* bias = nullptr;
   if (p.bias_ids) {
-    ids = p.bias_ids + (long long)row * p.bias_ids_ld;
-    bias = p.bias + (long long)row * p.bias_ld;
-    for (int j = tid; j < p.M; j += L_THREADS) {
-      const uint32_t i = (uint32_t)ids[j] - (uint32_t)v0;
-      if (ids[j] >= 0 && i < (uint32_t)span) atomicMin(entry + i, (uint32_t)j);
-    }
+    auto biased = [&](int j) {  // entry j's token from v0 on, or -1
+      const int id = j == tid ? first_bias : r.ids[j];
+      return id >= v0 && id - v0 < span ? id - v0 : -1;
+    };
+    for (int j = tid; j < p.M; j += L_THREADS)
+      if (biased(j) >= 0) atomicMin(entry + biased(j), (uint32_t)j);
     __syncthreads();
-    for (int j = tid; j < p.M; j += L_THREADS) {
-      const uint32_t i = (uint32_t)ids[j] - (uint32_t)v0;
-      if (ids[j] >= 0 && i < (uint32_t)span && (entry[i] & ~L_MORE) != (uint32_t)j)
-        atomicOr(entry + i, L_MORE);
-    }
+    for (int j = tid; j < p.M; j += L_THREADS)
+      if (biased(j) >= 0 && (entry[biased(j)] & ~L_MORE) != (uint32_t)j)
+        atomicOr(entry + biased(j), L_MORE);
   }
   if (p.tokens || p.bias_ids) __syncthreads();
 
   // the tokens that anything concerns (the others at an offset that neither loads nor stores)
-  const __amdgpu_buffer_rsrc_t r = dkv_make_rsrc(
+  const __amdgpu_buffer_rsrc_t logits = dkv_make_rsrc(
       (uint8_t*)p.logits + ((long long)row * p.ld + v0) * SIZE, (uint32_t)span * SIZE);
   const uint32_t* words = p.allowed ? p.allowed + (long long)row * p.allowed_ld + v0 / 32 : nullptr;
   for (int i0 = tid; i0 < span; i0 += L_THREADS * L_EACH) {
@@ -150,37 +328,15 @@ __global__ __launch_bounds__(L_THREADS) void adjust_kernel(LogitParams p) {
 #pragma unroll
     for (int u = 0; u < L_EACH; ++u) {
       const bool reads = (c[u] || e[u] != L_NONE) && !off[u];
-      const int at = reads ? (i0 + u * L_THREADS) * SIZE : DKV_OOB;
-      if constexpr (DT == DKV_F32)
-        x[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
-      else
-        x[u] = dkv_elt_to_f32<DT>(__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
+      x[u] = load_logit<DT>(logits, reads ? (i0 + u * L_THREADS) * SIZE : DKV_OOB);
     }
 #pragma unroll
     for (int u = 0; u < L_EACH; ++u) {
-      float y = x[u];
-      const uint32_t times = c[u] & ~L_SEEN;
-      if (c[u]) {
-        y = y > 0.f ? y / rep : y * rep;
-        y = y - freq * (float)times - (times ? pres : 0.f);
-      }
-      if (e[u] != L_NONE) {
-        const int j = (int)(e[u] & ~L_MORE), id = v0 + i0 + u * L_THREADS;
-        float sum = bias[j];
-        if (e[u] & L_MORE)
-          for (int k = j + 1; k < p.M; ++k)
-            if (ids[k] == id) sum += bias[k];
-        y += sum;
-      }
-      if (off[u]) y = -INFINITY;
+      const int i = i0 + u * L_THREADS;
+      const float b = e[u] != L_NONE ? r.bias[e[u] & ~L_MORE] : 0.f;
+      const float y = off[u] ? -INFINITY : adjusted(p, r, x[u], v0 + i, c[u], e[u], b);
       const bool writes = c[u] || e[u] != L_NONE || off[u];
-      const int at = writes ? (i0 + u * L_THREADS) * SIZE : DKV_OOB;
-      if constexpr (DT == DKV_F32)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y), r, at, 0, 0);
-      else if constexpr (DT == DKV_F16)
-        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)dkv_f32_to_f16_bits(y), r, at, 0, 0);
-      else
-        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)dkv_f32_to_bf16_bits(y), r, at, 0, 0);
+      store_logit<DT>(logits, writes ? i * SIZE : DKV_OOB, y);
     }
   }
 }
@@ -233,23 +389,43 @@ extern "C" int dkv_adjust_logits(void* stream, int dtype, void* logits, long lon
   p.allowed = (const uint32_t*)allowed;
   p.allowed_ld = allowed_ld;
   if (!p.tokens && !p.bias_ids && !p.allowed) return DKV_OK;
-  const int words = (p.tokens ? 1 : 0) + (p.bias_ids ? 1 : 0);
-  // spans of 2048 tokens to 64 KB of counts and entries (two workgroups a CU), as small as fills the chip
-  int span = L_SPAN;
-  const int most = words == 2 ? 8192 : 16384;
-  while (span < most && (long long)rows * ((V + 2 * span - 1) / (2 * span)) >= 512) span *= 2;
-  p.span = span;
-  p.slices = (V + span - 1) / span;
-  const long long wgs = ((long long)rows + 7) / 8 * 8 * p.slices;
-  if (wgs > 0x7fffffffLL) return DKV_E_UNSUPPORTED;
-  const size_t lds = (size_t)words * span * 4;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DKV_F32)
-    hipLaunchKernelGGL(adjust_kernel<DKV_F32>, dim3((unsigned)wgs), dim3(L_THREADS), lds, st, p);
-  else if (dtype == DKV_F16)
-    hipLaunchKernelGGL(adjust_kernel<DKV_F16>, dim3((unsigned)wgs), dim3(L_THREADS), lds, st, p);
-  else
-    hipLaunchKernelGGL(adjust_kernel<DKV_BF16>, dim3((unsigned)wgs), dim3(L_THREADS), lds, st, p);
+  const int words = (p.tokens ? 1 : 0) + (p.bias_ids ? 1 : 0);
+  auto launch = [&](auto f32, auto f16, auto bf16, long long wgs, int threads, size_t lds) {
+    const dim3 grid((unsigned)wgs);
+    if (dtype == DKV_F32)
+      hipLaunchKernelGGL(f32, grid, dim3(threads), lds, st, p);
+    else if (dtype == DKV_F16)
+      hipLaunchKernelGGL(f16, grid, dim3(threads), lds, st, p);
+    else
+      hipLaunchKernelGGL(bf16, grid, dim3(threads), lds, st, p);
+  };
+  const long long named = (p.tokens ? (long long)N : 0) + M;
+  int log2 = 9;
+  while (log2 < 30 && 3LL << log2 < 4 * named) ++log2;
+  const size_t table = ((size_t)4 << log2) * (p.bias_ids ? 3 : 2);
+  const bool few = words && (long long)rows * ((V + L_SPAN - 1) / L_SPAN) <= 256;
+  if (table <= 65536 && !few) {
+    const int threads = named > 1024 ? 1024 : L_THREADS;
+    p.slots_log2 = log2;
+    p.row_wgs = words ? rows : 0;
+    p.mask_wgs = (V + threads * L_MASK - 1) / (threads * L_MASK);
+    const long long wgs = p.row_wgs + (p.allowed ? (long long)rows * p.mask_wgs : 0);
+    if (wgs > 0x7fffffffLL) return DKV_E_UNSUPPORTED;
+    launch(adjust_rows_kernel<DKV_F32>, adjust_rows_kernel<DKV_F16>, adjust_rows_kernel<DKV_BF16>, wgs,
+           threads, words ? table : 0);
+  } else {
+    // spans of 2048 tokens to 64 KB of counts and entries (two workgroups a CU), as small as fills the chip
+    int span = L_SPAN;
+    const int most = words == 2 ? 8192 : 16384;
+    while (span < most && (long long)rows * ((V + 2 * span - 1) / (2 * span)) >= 512) span *= 2;
+    p.span = span;
+    p.slices = (V + span - 1) / span;
+    const long long wgs = ((long long)rows + 7) / 8 * 8 * p.slices;
+    if (wgs > 0x7fffffffLL) return DKV_E_UNSUPPORTED;
+    launch(adjust_vocabulary_kernel<DKV_F32>, adjust_vocabulary_kernel<DKV_F16>,
+           adjust_vocabulary_kernel<DKV_BF16>, wgs, L_THREADS, (size_t)words * span * 4);
+  }
   DKV_HIP_CHECK_LAUNCH();
   return DKV_OK;
 }

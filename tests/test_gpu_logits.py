@@ -122,6 +122,13 @@ CASES = {
     "spans_of_16384": (260, 40007, FP, 100, torch.int64, 0, True, True),
     "spans_with_biases": (260, 20011, BF, 60, torch.int32, 3, False, True),
     "long_history": (2, 3000, F32, 30000, torch.int64, 0, False, True),
+    # histories that are counted by vocabulary, in spans of 2048, 8192 and 16384 tokens
+    "long_all": (3, 4100, FP, 7000, torch.int32, 9, True, True),
+    "long_spans_of_8192": (80, 40007, BF, 6200, torch.int32, 5, True, True),
+    "long_spans_of_16384": (260, 40007, BF, 6200, torch.int64, 0, False, True),
+    "largest_table": (2, 50000, BF, 6144, torch.int64, 0, True, True),
+    "largest_table_with_biases": (2, 50000, F32, 3000, torch.int64, 72, False, True),
+    "every_token_once": (2, 6144, F32, 6144, torch.int64, 0, False, False),
 }
 
 
@@ -132,6 +139,8 @@ def test_against_the_formula(dev, name):
     print(f"[gpu] adjust {name}", flush=True)
     x, kw = _rows(dev, rows, V, dtype, seed=len(name), n=n, ids=ids, biases=biases, mask=mask,
                   settings=settings)
+    if name == "every_token_once":
+        kw["tokens"] = torch.stack([torch.randperm(V, device=dev) for _ in range(rows)])
     check(x, **kw)
 
 
