@@ -169,7 +169,11 @@ struct PagedScales {
   const uint8_t* v;
   long long page_stride, head_stride;
 };
+// As the conversions to 16 bits take it (by its exponent field), and as a factor in fp32.
 __device__ __forceinline__ float pg_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+__device__ __forceinline__ float pg_factor(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
+}
 
 // Two codes of a dword times a scale, as two 16-bit numbers (exact where they are such numbers).
 template <int DT, bool HIGH>

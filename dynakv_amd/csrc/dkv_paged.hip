@@ -847,8 +847,8 @@ __device__ __forceinline__ void attend_row_apart(const AttendParams& p, int b, i
         const long long sa = (long long)page * p.scales.page_stride +
                              (long long)kvh * p.scales.head_stride +
                              (key & (p.pool.page_size - 1)) / PG_BLOCK;
-        by_k = pg_scale(p.scales.k[sa]);
-        by_v = pg_scale(p.scales.v[sa]);
+        by_k = pg_factor(p.scales.k[sa]);
+        by_v = pg_factor(p.scales.v[sa]);
       }
     }
     if (page >= 0) {

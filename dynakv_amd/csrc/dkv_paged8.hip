@@ -384,7 +384,7 @@ __global__ __launch_bounds__(V_THREADS) void paged_values_kernel(ValuesParams p)
   for (int u = 0; u < V_EACH; ++u) {
     const long long at = at0 + u * V_THREADS;
     if (at >= p.pieces) continue;
-    const float s = pg_scale(byte[u]);
+    const float s = ODT == DKV_F32 ? pg_factor(byte[u]) : pg_scale(byte[u]);
     if constexpr (ODT == DKV_F32) {
 #pragma unroll
       for (int d = 0; d < 4; ++d) {

@@ -22,8 +22,8 @@ only the forward math):
   the same stages serve the dense baseline.
 * ``PagedLlama.generate``: the same weights over a paged uncompressed cache
   (``kernels/paged.py``), for prompts of different lengths that come and go: prompts go through
-  in chunks beside the other requests' single tokens. Generation is greedy, or drawn by a
-  ``Sampler`` (``kernels/sampling.py``), which the other generators take too.
+  in chunks beside the other requests' single tokens; its pages may be of 8 bits. Generation is
+  greedy, or drawn by a ``Sampler`` (``kernels/sampling.py``), which the other generators take too.
 * ``DenseLlama.generate``: the uncompressed-cache baseline of the same weights (K/V kept in
   full in a preallocated cache; decode attention by the same split kernel over that cache read
   as a packed cache with all 128 dims per token and an identity basis, prefill attention by
@@ -50,7 +50,7 @@ from .kernels.model_ops import linear, rmsnorm_glu, rmsnorm_linear
 from .kernels.paged import PagedBatch, PagedKVCache, paged_append, paged_attention
 from .kernels.prefill import coef_prefill_attention, rope_dense_
 from .kernels.router import KernelPolicy
-from .kernels.sampling import sample_tokens
+from .kernels.sampling import adjust_logits_, sample_tokens
 
 
 @dataclass(frozen=True)
@@ -167,28 +167,54 @@ class RandomLlama:
 
 class Sampler:
     """Draws tokens from logits: a generator's replacement for its argmax. The settings are those of
-    ``sample_tokens``, numbers or a tensor with an entry per row (of a batch, or of the requests that
-    are generated for); the uniform numbers come from a generator of its own, so a seed gives the same
-    draws for the same logits."""
+    ``sample_tokens`` and, before them, the penalties of ``adjust_logits_`` over a request's tokens:
+    numbers or a tensor with an entry per row (of a batch, or of the requests that are generated for).
+    ``bias`` maps tokens to what is added to their logits. The uniform numbers come from a generator of
+    its own, so a seed gives the same draws for the same logits."""
 
-    def __init__(self, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0,
+    _NEUTRAL = dict(repetition=1.0, frequency=0.0, presence=0.0)
+
+    def __init__(self, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, repetition=1.0,
+                 frequency=0.0, presence=0.0, bias: dict[int, float] | None = None, seed: int = 0,
                  device="cuda"):
         self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        given = dict(repetition=repetition, frequency=frequency, presence=presence)
+        self.penalties = {name: v for name, v in given.items()
+                          if torch.is_tensor(v) or v != self._NEUTRAL[name]}
+        self._bias = None
+        if bias:
+            self._bias = (torch.tensor([list(bias)], dtype=torch.int32, device=device),
+                          torch.tensor([list(bias.values())], dtype=torch.float32, device=device))
         self._gen = torch.Generator(device=device)
         self._gen.manual_seed(seed)
 
     def __call__(self, logits: torch.Tensor, *, requests: Sequence[int] | None = None,
-                 u: torch.Tensor | None = None) -> torch.Tensor:
+                 u: torch.Tensor | None = None, tokens: torch.Tensor | None = None, prompt_lens=None,
+                 lens=None, allowed: torch.Tensor | None = None) -> torch.Tensor:
         """``logits`` (..., V) -> tokens (...). ``requests``: the request of each row, whose entries the
         settings' tensors are taken from (else row i has entry i); ``u``: the rows' uniform numbers (else
-        the generator's next ones). Of a row without a token to take (all NaN or -infinity) token 0, as
-        the tokens are looked up next: ``sample_tokens`` tells them by -1."""
+        the generator's next ones). Penalties need the rows' ``tokens``, with ``prompt_lens`` and
+        ``lens``, and ``allowed`` is their mask, as ``adjust_logits_`` takes them (here on a copy of the
+        logits). Of a row without a token to take (all NaN or -infinity) token 0, as the tokens are
+        looked up next: ``sample_tokens`` tells them by -1."""
         rows = logits.reshape(-1, logits.shape[-1])
-        settings = self.settings
+        settings = self.settings | self.penalties
         if requests is not None:
             settings = self._of(requests, rows)
         if u is None:
             u = self.uniform(rows.shape[0], logits.device)
+        penalties = {name: settings.pop(name) for name in self.penalties}
+        if penalties:
+            if tokens is None:
+                raise ValueError("a sampler with penalties needs the rows' tokens")
+            penalties |= dict(tokens=tokens, prompt_lens=prompt_lens, lens=lens)
+        if self._bias is not None:
+            n = rows.shape[0]
+            penalties |= dict(bias_ids=self._bias[0].expand(n, -1), bias=self._bias[1].expand(n, -1))
+        if allowed is not None:
+            penalties["allowed"] = allowed
+        if penalties:
+            rows = adjust_logits_(rows.clone(memory_format=torch.contiguous_format), **penalties)
         return sample_tokens(rows, u, **settings).clamp_(min=0).view(logits.shape[:-1])
 
     def uniform(self, n: int, device) -> torch.Tensor:
@@ -197,7 +223,7 @@ class Sampler:
 
     def check(self, requests: int) -> None:
         """Raises where a setting's tensor has not an entry for each of so many requests."""
-        for name, v in self.settings.items():
+        for name, v in (self.settings | self.penalties).items():
             if torch.is_tensor(v) and v.shape != (requests,):
                 raise ValueError(f"{name} must be a number or have an entry for each of the {requests} "
                                  "requests")
@@ -206,7 +232,7 @@ class Sampler:
         if len(requests) != rows.shape[0]:
             raise ValueError(f"{len(requests)} requests for {rows.shape[0]} rows of logits")
         at = None
-        settings = dict(self.settings)
+        settings = self.settings | self.penalties
         for name, v in settings.items():
             if not torch.is_tensor(v):
                 continue
@@ -269,6 +295,8 @@ class _Generator:
         """Greedy decode (or tokens drawn by ``sampler``); returns tokens, timings and cache
         bytes."""
         pick = sampler if sampler is not None else lambda logits: logits.argmax(-1)
+        if isinstance(sampler, Sampler) and sampler.penalties:
+            pick = self._with_history(sampler, prompt, new_tokens)
         torch.cuda.synchronize(self.m.device)
         t0 = time.perf_counter()
         x = self.prefill(prompt)
@@ -293,6 +321,23 @@ class _Generator:
             "decode_tokens_per_s": B * (new_tokens - 1) / max(t2 - t1, 1e-9),
             "kv_bytes": self.kv_bytes(),
         }
+
+
+    def _with_history(self, sampler: Sampler, prompt: torch.Tensor, new_tokens: int):
+        """Logits (B, 1, V) -> tokens (B, 1), with the prompts' and the generated tokens' penalties."""
+        B, S = prompt.shape
+        history = torch.zeros(B, S + new_tokens, dtype=torch.long, device=prompt.device)
+        history[:, :S] = prompt
+        n = S
+
+        def pick(logits):
+            nonlocal n
+            tok = sampler(logits, tokens=history, prompt_lens=S, lens=n)
+            history[:, n:n + 1] = tok
+            n += 1
+            return tok
+
+        return pick
 
 
 class CompressedLlama(_Generator):
@@ -499,17 +544,20 @@ class PagedLlama(_Generator):
     """The same weights over a paged uncompressed cache: requests of different lengths, whose
     prompts go through in chunks beside the other requests' single tokens.
 
-    ``pages`` pages of ``page_size`` tokens per layer are shared by all requests. ``add`` starts a
+    ``pages`` pages of ``page_size`` tokens per layer are shared by all requests, in the model's type
+    or of 8 bits (``cache_dtype=torch.float8_e4m3fn``: half the bytes). ``add`` starts a
     request, ``step`` feeds tokens to some of them and returns the logits after each one's last
     token, ``end`` gives a request's pages back; ``generate`` is the loop over them."""
 
     takes_qk_norm = True
 
-    def __init__(self, model: RandomLlama, pages: int, page_size: int = 64):
+    def __init__(self, model: RandomLlama, pages: int, page_size: int = 64,
+                 cache_dtype: torch.dtype | None = None):
         super().__init__(model)
         s = self.s
         self.cache = PagedKVCache(s.layers, pages, s.kv_heads, page_size=page_size,
-                                  dtype=model.dtype, device=model.device)
+                                  dtype=model.dtype if cache_dtype is None else cache_dtype,
+                                  device=model.device)
 
     def add(self) -> int:
         return self.cache.add()
@@ -536,9 +584,11 @@ class PagedLlama(_Generator):
         x = F.embedding(torch.cat([t for _, t in feed]), self.m.embed).unsqueeze(0)
 
         def attn(i, lw, y):
-            q = paged_append(y[0], self.cache.k[i], self.cache.v[i], batch, heads=s.heads,
-                             theta=s.theta, q_norm=lw.q_norm, k_norm=lw.k_norm, eps=s.eps)
-            a = paged_attention(q, self.cache.k[i], self.cache.v[i], batch)
+            c = self.cache
+            scales = dict(k_scale=c.k_scale[i], v_scale=c.v_scale[i])
+            q = paged_append(y[0], c.k[i], c.v[i], batch, heads=s.heads, theta=s.theta,
+                             q_norm=lw.q_norm, k_norm=lw.k_norm, eps=s.eps, **scales)
+            a = paged_attention(q, c.k[i], c.v[i], batch, **scales)
             return a.view(1, -1, s.hidden)
 
         x = self._run(x, attn, "w_qkv")[0]
@@ -556,7 +606,7 @@ class PagedLlama(_Generator):
             raise ValueError("need prompts, a positive chunk and a positive number of tokens")
         if any(p.dim() != 1 or p.shape[0] < 1 for p in prompts):
             raise ValueError("prompts are (n,) tokens, n >= 1")
-        pick = self._pick(sampler, len(prompts), new_tokens)
+        pick = self._pick(sampler, prompts, new_tokens)
         torch.cuda.synchronize(self.m.device)
         t0 = time.perf_counter()
         ids: list = [self.add() for _ in prompts]  # None once ended
@@ -599,8 +649,9 @@ class PagedLlama(_Generator):
         return {"tokens": torch.stack([torch.cat(o) for o in out]), "seconds": t,
                 "tokens_per_s": len(prompts) * new_tokens / t, "pages": held}
 
-    def _pick(self, sampler: Sampler | None, requests: int, new_tokens: int):
+    def _pick(self, sampler: Sampler | None, prompts: list[torch.Tensor], new_tokens: int):
         """(logits, (request, index of its token) of each row) -> tokens."""
+        requests = len(prompts)
         if sampler is None:
             return lambda logits, at: logits.argmax(-1)
         if not isinstance(sampler, Sampler):  # any function of logits
@@ -609,6 +660,13 @@ class PagedLlama(_Generator):
         # row i: the numbers of the requests' i-th tokens, drawn when the first of them is
         u = torch.empty(new_tokens, requests, dtype=torch.float32, device=self.m.device)
         drawn = 0
+        history = None  # the requests' tokens, where there are penalties for them
+        if sampler.penalties:
+            sizes = [p.shape[0] for p in prompts]
+            history = torch.zeros(requests, max(sizes) + new_tokens, dtype=torch.long,
+                                  device=self.m.device)
+            for j, p in enumerate(prompts):
+                history[j, :sizes[j]] = p
 
         def pick(logits, at):
             nonlocal drawn
@@ -616,12 +674,21 @@ class PagedLlama(_Generator):
                 u[drawn] = sampler.uniform(requests, u.device)
                 drawn += 1
             mine = u.view(-1).index_select(0, _index([i * requests + j for j, i in at], u.device))
-            return sampler(logits, requests=[j for j, _ in at], u=mine)
+            who = [j for j, _ in at]
+            if history is None:
+                return sampler(logits, requests=who, u=mine)
+            rows = _index(who + [sizes[j] for j in who] + [sizes[j] + i for j, i in at], u.device)
+            rows, first, ends = rows.view(3, -1)
+            tok = sampler(logits, requests=who, u=mine, tokens=history.index_select(0, rows),
+                          prompt_lens=first.int(), lens=ends.int())
+            history[rows, ends] = tok
+            return tok
 
         return pick
 
     def kv_bytes(self) -> int:
-        """Bytes of the pages that requests hold, over all layers."""
-        k = self.cache.k[0]
+        """Bytes of the pages that requests hold (and of their scales), over all layers."""
+        k, scale = self.cache.k[0], self.cache.k_scale[0]
         held = self.cache.pages - self.cache.free_pages
-        return 2 * len(self.cache.k) * held * k[0].numel() * k.element_size()
+        page = k[0].numel() * k.element_size() + (0 if scale is None else scale[0].numel())
+        return 2 * len(self.cache.k) * held * page

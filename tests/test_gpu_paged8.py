@@ -38,6 +38,11 @@ def nearest(y):
     return torch.where(pick, grid[hi], grid[lo]).copysign(y)
 
 
+def two_to(e):
+    """2^e in float64 by its bits (a library's power may be off by a step)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 class Step8(Step):
     """A step over 8-bit pages: the requests' earlier tokens are held as random values are, with
     block scales some powers of two apart; the new ones too where ``data``."""
@@ -92,7 +97,7 @@ class Step8(Step):
         """(pages, hkv, ps, 128) float64 values."""
         scale = self.k_scale if codes is self.k else self.v_scale
         e = scale.contiguous().view(torch.uint8).double() - 127
-        two = torch.where(e == 128, math.nan, torch.ldexp(torch.ones_like(e), e))
+        two = torch.where(e == 128, math.nan, two_to(e))
         return codes.contiguous().double() * two.repeat_interleave(BLOCK, -1)[..., None]
 
     def tokens(self, pool, b, g):
@@ -104,7 +109,7 @@ class Step8(Step):
         if key not in self._seen:
             scale = (self.k_scale if pool is self.k else self.v_scale)[ids, g]
             e = scale.contiguous().view(torch.uint8).double() - 127
-            two = torch.where(e == 128, math.nan, torch.ldexp(torch.ones_like(e), e))
+            two = torch.where(e == 128, math.nan, two_to(e))
             x = pool[ids, g].double() * two.repeat_interleave(BLOCK, -1)[..., None]
             self._seen[key] = x.reshape(-1, DH)[:n]
         return self._seen[key]
@@ -337,7 +342,7 @@ def test_tokens_one_by_one_are_held_as_at_once(dev, dtype):
         for kind in (0, 1):
             e = held[0][2 + kind]
             assert torch.equal(other[2 + kind], e)
-            step = torch.exp2(e.float() - 127).repeat_interleave(16, 2).transpose(1, 2).reshape(
+            step = two_to(e.long() - 127).float().repeat_interleave(16, 2).transpose(1, 2).reshape(
                 -1, hkv, 1)[:n]
             a, b = other[kind], held[0][kind]
             # below 2^-6 of a scale codes are 2^-9 apart: rounded twice or more, a step at most
@@ -397,3 +402,388 @@ def test_attention(dev, name):
     new, lens, hq, hkv, ps, dt, layout = ATTEND[name]
     print(f"[gpu] paged attention8 {name}", flush=True)
     _check_attend(Step8(dev, new, lens, hkv=hkv, ps=ps, dtype=dt, layout=layout, seed=11), hq)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 1], [700, 90]), ([80, 5], [300, 200])])
+def test_attention_peaked_and_scaled(dev, new, lens):
+    """A near one-hot softmax (the running maximum rises late), and a scale of its own."""
+    print(f"[gpu] paged attention8 peaked {new}", flush=True)
+    _check_attend(Step8(dev, new, lens, hkv=2, seed=12), 8, qscale=8.0)
+    _check_attend(Step8(dev, new, lens, hkv=2, seed=13, dtype=FP), 8, scale=0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("new,lens", [([1, 1], [700, 90]), ([80, 5], [300, 200])])
+def test_attention_scales_far_apart(dev, new, lens, dtype):
+    """Blocks whose scales differ by up to 2^14 (fp16) and 2^60 (bf16) in one tile, values that are large and
+    tiny; keys small enough for the scores to stay moderate."""
+    print(f"[gpu] paged attention8 scales {new}", flush=True)
+    s = Step8(dev, new, lens, hkv=2, seed=14, dtype=dtype)
+    g = torch.Generator().manual_seed(3)
+    n = s.v_scale.numel()
+    lo, hi = (-14, 0) if dtype == FP else (-60, 0)
+    e = torch.randint(lo, hi + 1, (n,), generator=g) + 127
+    s.v_scale.view(torch.uint8).copy_(e.to(torch.uint8).view(s.v_scale.shape))
+    e = torch.randint(-14, -7, (n,), generator=g) + 127
+    s.k_scale.view(torch.uint8).copy_(e.to(torch.uint8).view(s.k_scale.shape))
+    _check_attend(s, 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1] * 3, [700, 90, 33]), ([80, 5], [300, 200])])
+def test_attention_leaves_padding_rows(dev, new, lens):
+    print(f"[gpu] paged attention8 padding {new}", flush=True)
+    s = Step8(dev, new, lens, hkv=2, seed=14, pad=9)
+    q = s.rand(s.T, 8, DH)
+    want, tol = _attend_reference(s, q)
+    whole = torch.full((s.T, 9, 2 * DH), 3.0, dtype=torch.float32, device=dev)
+    out = whole[:, :8, :DH]
+    got = paged_attention(q, s.k, s.v, s.batch, out=out, **s.both)
+    good = got.data_ptr() == out.data_ptr() and bool(
+        ((out[:s.rows].double() - want).abs() <= 2 * tol + 1e-30).all())
+    assert good
+    out[:s.rows] = 3.0
+    assert bool((whole == 3.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 3, 60])
+def test_attention_masks_pages_that_are_not_there(dev, new):
+    """A page id outside the pool: its keys are masked, as if their tokens were others'. No page at all, or
+    a length of zero: 0."""
+    print(f"[gpu] paged attention8 bad pages {new}", flush=True)
+    s = Step8(dev, [new] * 4, [150, 150, 150, 60], hkv=2, seed=15)
+    q = s.rand(s.T, 4, DH)
+    want, tol = _attend_reference(s, q)
+    s.table[1, 2], s.table[1, 5] = -1, 10**6      # tokens 32 .. 47 and 80 .. 95 of request 1
+    s.table[2] = -1                               # all of request 2
+    lens = torch.tensor([150, 150, 150, 0], dtype=torch.int32, device=dev)
+    batch = PagedBatch(s.table.to(dev), s.batch.q_start, lens, rows=s.rows, max_new=new,
+                       max_len=150, min_new=new)
+    got = paged_attention(q, s.k, s.v, batch, out_dtype=torch.float32, **s.both)
+    pos = torch.arange(150 - new, 150, device=dev)[:, None]
+    key = torch.arange(150, device=dev)[None]
+    dead = (key > pos) | ((key // 16) == 2) | ((key // 16) == 5)
+    good = [int(i) if 0 <= int(i) < s.k.shape[0] else 0 for i in s.table[1, :10]]
+    k_all, v_all = s.held(s.k).nan_to_num(), s.held(s.v).nan_to_num()
+    for h in range(4):
+        k, v = (t[good, h // 2].reshape(-1, DH)[:150] for t in (k_all, v_all))
+        z = (q[new:2 * new, h].double() @ k.T / math.sqrt(DH)).masked_fill(dead, -math.inf)
+        p = torch.softmax(z, -1)
+        # the weights' two half steps and fp32 scores of up to 2^6: 2^-7 covers both
+        fine = (got[new:2 * new, h].double() - p @ v).abs() <= 2.0**-7 * (p @ v.abs()) + 1e-30
+        assert bool(fine.all())
+    first = bool(((got[:new].double() - want[:new]).abs() <= 2 * tol[:new] + 1e-30).all())
+    assert first and bool((got[2 * new:] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,n,hkv", [(4, 300, 2), (60, 60, 2), (60, 3000, 2), (700, 700, 8)])
+def test_attention_keeps_later_tokens_out(dev, new, n, hkv):
+    """A NaN in a new token's value or key: the tokens before it have the result they have without it; the
+    ones from it on have it in theirs."""
+    print(f"[gpu] paged attention8 later {new}", flush=True)
+    s = Step8(dev, [new, 1], [n, 40], hkv=hkv, seed=17)
+    q = s.rand(s.T, 4 * hkv, DH)
+    attend = lambda: paged_attention(q, s.k, s.v, s.batch, out_dtype=torch.float32, **s.both)  # noqa: E731
+    clean = attend()
+    _, tol = _attend_reference(s, q)
+    bad = n - new + new // 2  # the position of the token
+    page, slot = int(s.table[0, bad // 16]), bad % 16
+    before, after = slice(0, new // 2), slice(new // 2, new)
+    s.v.view(torch.uint8)[page, :, slot, ::3] = 0xff
+    got = attend()
+    near = lambda a, b, t: bool(((a - b).abs() <= 4 * t).all())  # noqa: E731
+    assert near(got[before], clean[before], tol[before]) and torch.equal(got[new:], clean[new:])
+    assert bool(got[after][..., ::3].isnan().all())
+    assert near(got[after][..., 1::3], clean[after][..., 1::3], tol[after][..., 1::3])
+    s.k.view(torch.uint8)[page, :, slot] = 0x7f
+    got = attend()
+    assert near(got[before], clean[before], tol[before]) and torch.equal(got[new:], clean[new:])
+    assert bool(got[after].isnan().all())
+
+
+def _random_step(i):
+    g = torch.Generator().manual_seed(900 + i)
+    r = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
+    hkv = [1, 2, 3, 8][r(0, 3)]
+    hq = hkv * [1, 2, 4, 5, 8, 16][r(0, 5)]
+    n = r(1, 6)
+    kind = r(0, 3)
+    new = [[1, r(1, 6), r(1, 200), [0, 1, r(2, 90)][r(0, 2)]][kind] for _ in range(n)]
+    if not any(new):
+        new[0] = 1
+    lens = [m + (0 if r(0, 2) == 0 else int(math.exp(float(torch.rand(1, generator=g)) * 8)))
+            for m in new]
+    return new, lens, hq, hkv, [16, 32, 64, 128, 256][r(0, 4)], [BF, FP][r(0, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(16))
+def test_random_steps(dev, i):
+    """Append, then attention, of a random step."""
+    new, lens, hq, hkv, ps, dt = _random_step(i)
+    print(f"[gpu] random step8 {i}: {new} {lens} {hq}/{hkv} page {ps} {dt}", flush=True)
+    s = Step8(dev, new, lens, hkv=hkv, ps=ps, dtype=dt, seed=600 + i)
+    q = _check_append(s, hq, norms=i % 2 == 0)
+    _check_attend(s, hq, q=q)
+
+
+MANY = {
+    # more units than workgroups of eight waves, of four, and requests than a wave holds the lengths of
+    "four_waves": ([1] * 35, [40, 3000, 7, 500, 64] * 7, 32, 8, 16),
+    "uncut": ([1] * 70, [40, 300, 7, 500, 64] * 14, 32, 8, 16),
+    "many_requests": ([1, 1, 0] * 100, [40, 300, 7] * 100, 8, 2, 16),
+    "many_requests_one_head": ([1] * 400, [40, 300] * 200, 4, 1, 32),
+    "with_prompts": ([1, 1, 40] * 30, [40, 300, 47] * 30, 8, 2, 16),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(MANY))
+def test_attention_many_requests(dev, name):
+    new, lens, hq, hkv, ps = MANY[name]
+    print(f"[gpu] paged attention8 many {name}", flush=True)
+    s = Step8(dev, new, lens, hkv=hkv, ps=ps, seed=51)
+    q = s.rand(s.T, hq, DH)
+    got = paged_attention(q, s.k, s.v, s.batch, out_dtype=torch.float32, **s.both)
+    hpg = hq // hkv
+    k_all, v_all = s.held(s.k), s.held(s.v)
+    for b, (m, n) in enumerate(zip(new, lens)):
+        if m == 0:
+            continue
+        ids = s.table[b, :-(-n // ps)].long().to(dev)
+        k, v = (t[ids].transpose(0, 1).reshape(hkv, -1, DH)[:, :n].repeat_interleave(hpg, 0)
+                for t in (k_all, v_all))
+        x = q[s.starts[b]:s.starts[b] + m].double().transpose(0, 1)
+        z = torch.matmul(x, k.transpose(1, 2).contiguous()) / math.sqrt(DH)
+        z.masked_fill_(torch.arange(n, device=dev)[None] > torch.arange(n - m, n, device=dev)[:, None],
+                       -math.inf)
+        p = torch.softmax(z, -1)
+        want, size = torch.matmul(p, v).transpose(0, 1), torch.matmul(p, v.abs()).transpose(0, 1)
+        # two half steps of the weights, and fp32 scores: 2^-7 covers both
+        fine = (got[s.starts[b]:s.starts[b] + m].double() - want).abs() <= 2.0**-7 * size + 1e-30
+        assert bool(fine.all()), (b, m, n)
+
+
+# ---------------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_requests_that_come_and_go(dev, dtype):
+    """Three requests through a cache: prompts in chunks beside single tokens, one ended and its pages
+    reused, one cut back; every output against attention over the values that the pages hold, and these
+    against the tokens kept aside, half a step of e4m3 (2^-4, or 2^-10 of a block's scale) away."""
+    print("[gpu] paged8 chunks", flush=True)
+    hq, hkv, theta = 8, 2, 10000.0
+    cache = PagedKVCache(1, 24, hkv, page_size=16, dtype=CODES, device=dev)
+    cache.k[0].view(torch.uint8).fill_(0x7f), cache.v[0].view(torch.uint8).fill_(0x7f)
+    g = torch.Generator().manual_seed(77)
+    both = dict(k_scale=cache.k_scale[0], v_scale=cache.v_scale[0])
+    kept: dict = {}
+    a, b, c = cache.add(), cache.add(), cache.add()
+
+    def step(parts):
+        qkv = torch.randn(sum(n for _, n in parts), (hq + 2 * hkv) * DH, generator=g).to(dtype).to(dev)
+        batch = cache.batch(parts)
+        q = paged_append(qkv, cache.k[0], cache.v[0], batch, heads=hq, theta=theta, **both)
+        o = paged_attention(q, cache.k[0], cache.v[0], batch, out_dtype=torch.float32, **both)
+        at = 0
+        for r, n in parts:
+            kept[r] = torch.cat([kept[r], qkv[at:at + n]]) if r in kept else qkv[at:at + n]
+            total = kept[r].shape[0]
+            assert total == cache.length(r)
+            ids = torch.tensor(cache.page_ids(r), dtype=torch.int32, device=dev)
+            held = paged_values(cache.k[0], cache.v[0], **both, pages=ids, dtype=torch.float32)
+            k, v = (t.transpose(1, 2).reshape(-1, hkv, DH)[:total].double() for t in held)
+            x = kept[r].double().view(total, hq + 2 * hkv, DH)
+            from test_gpu_paged import _turn
+            pos = torch.arange(total, dtype=torch.float64, device=dev)
+            for got, want, scale in ((k, _turn(x[:, hq:hq + hkv], pos, _freq(dev, theta)), 0),
+                                     (v, x[:, hq + hkv:], 1)):
+                e = u8(cache.v_scale[0] if scale else cache.k_scale[0])[ids.long()].double() - 127
+                two = two_to(e).repeat_interleave(16, 2).transpose(1, 2).reshape(-1, hkv, 1)[:total]
+                # (once more where a block's scale rose later: two roundings below the normal codes)
+                fine = (got - want).abs() <= 2.0**-4 * want.abs() + 2 * 2.0**-10 * two
+                assert bool(fine.all())
+            for h in range(hq):
+                z = q[at:at + n, h].double() @ k[:, h // 4].T / math.sqrt(DH)
+                z.masked_fill_(torch.arange(total, device=dev)[None]
+                               > torch.arange(total - n, total, device=dev)[:, None], -math.inf)
+                p = torch.softmax(z, -1)
+                fine = ((o[at:at + n, h].double() - p @ v[:, h // 4]).abs()
+                        <= 2.0**-7 * (p @ v[:, h // 4].abs()) + 1e-30)
+                assert bool(fine.all()), (r, total, h)
+            at += n
+
+    step([(a, 70), (b, 5)])
+    step([(b, 40), (a, 1)])
+    step([(a, 1), (c, 100), (b, 1)])
+    cache.truncate(c, 90)
+    kept[c] = kept[c][:90]
+    step([(a, 1), (b, 0), (c, 3)])
+    cache.free(a)
+    d = cache.add()
+    step([(d, 130), (c, 1), (b, 2)])
+    step([(d, 1), (c, 1), (b, 1)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1] * 4, [700, 90, 33, 260]), ([60, 1, 9], [300, 200, 100])])
+def test_captured_step(dev, new, lens):
+    """A captured append, attention and reading back, replayed with other inputs, lengths and pages in the
+    same buffers, with eager work between the replays; two graphs replayed at once on two streams."""
+    print(f"[gpu] paged8 graph {new}", flush=True)
+    side = torch.cuda.Stream()
+    s = [Step8(dev, new, lens, hkv=2, seed=21 + i) for i in range(2)]
+    qkv = [t.rand(t.T, 12 * DH) for t in s]
+
+    def one(i):
+        t = s[i]
+        q = paged_append(qkv[i], t.k, t.v, t.batch, heads=8, theta=1e4, **t.both)
+        return (paged_attention(q, t.k, t.v, t.batch, **t.both),
+                *paged_values(t.k, t.v, **t.both, pages=t.batch.page_table.view(-1)))
+
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        for i in range(2):
+            one(i)
+        torch.cuda.synchronize()
+        for i in range(2):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=side):
+                outs.append(one(i))
+            graphs.append(gr)
+    torch.cuda.synchronize()
+    other = Step8(dev, [1], [3000], hkv=2, seed=29)
+    oq = other.rand(1, 8, DH)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        for i in range(2):
+            qkv[i].copy_(s[i].rand(s[i].T, 12 * DH))
+            if rep == 2:  # shorter, and two pages changed places
+                t = s[i]
+                t.lens = [max(m, n - 20) for m, n in zip(t.new, t.lens)]
+                t.batch.lens.copy_(torch.tensor(t.lens, dtype=torch.int32))
+                t.table[0, [0, 1]] = t.table[0, [1, 0]]
+                t.batch.page_table.copy_(t.table)
+        paged_attention(oq, other.k, other.v, other.batch, **other.both)
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            t = s[i]
+            got = [u8(x).clone() for x in (*outs[i], t.k, t.v, t.k_scale, t.v_scale)]
+            again = one(i)
+            for x, y in zip(got, (*again, t.k, t.v, t.k_scale, t.v_scale)):
+                assert torch.equal(x, u8(y)), (rep, i)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    print("[gpu] paged8 two streams", flush=True)
+    s = [Step8(dev, [1, 2], [1500, 1100 + 300 * i], hkv=2, seed=31 + i) for i in range(2)]
+    q = [t.rand(t.T, 8, DH) for t in s]
+    run = lambda i: paged_attention(q[i], s[i].k, s[i].v, s[i].batch, **s[i].both)  # noqa: E731
+    want = [run(i) for i in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            assert torch.equal(o, want[i])
+
+
+@pytest.mark.gpu
+def test_pool_past_32_bits(dev):
+    """Pages whose codes lie past 2^32 bytes of the pool's start."""
+    print("[gpu] paged8 large pool", flush=True)
+    ps, hkv, pages = 256, 2, 70000  # 4.6 GB each for keys and values
+    k = torch.empty(pages, hkv, ps, DH, dtype=torch.uint8, device=dev).view(CODES)
+    v = torch.empty_like(k)
+    ks = torch.zeros(pages, hkv, ps // 16, dtype=torch.uint8, device=dev).view(SCALES)
+    vs = torch.zeros_like(ks)
+    for new, n in ((1, 700), (70, 700)):
+        ids = [pages - 1, 3, pages - 900]
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        batch = PagedBatch(i32(*ids)[None], i32(0, new), i32(n), rows=new, max_new=new, max_len=n,
+                           min_new=new)
+        small = Step8(dev, [new], [n], hkv=hkv, ps=ps, seed=42)
+        qkv = small.rand(new, 8 * DH)
+        order = small.table[0, :3].long().to(dev)
+        for big, part in ((k, small.k), (v, small.v), (ks, small.k_scale), (vs, small.v_scale)):
+            big.view(torch.uint8)[ids] = part.view(torch.uint8)[order]
+        both = dict(k_scale=ks, v_scale=vs)
+        qa = paged_append(qkv, k, v, batch, heads=4, theta=1e4, **both)
+        qb = paged_append(qkv, small.k, small.v, small.batch, heads=4, theta=1e4, **small.both)
+        assert torch.equal(qa, qb)
+        for big, part in ((k, small.k), (v, small.v), (ks, small.k_scale), (vs, small.v_scale)):
+            assert torch.equal(big.view(torch.uint8)[ids], part.view(torch.uint8)[order])
+        assert torch.equal(paged_attention(qa, k, v, batch, **both),
+                           paged_attention(qb, small.k, small.v, small.batch, **small.both))
+        a = paged_values(k, v, **both, pages=i32(*ids))
+        b = paged_values(small.k, small.v, **small.both, pages=order.int())
+        assert torch.equal(u8(a[0]), u8(b[0])) and torch.equal(u8(a[1]), u8(b[1]))
+
+
+# ---------------------------------------------------------------------------------------------
+# pages read back
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP, torch.float32])
+@pytest.mark.parametrize("layout,ps,hkv", [("plain", 16, 1), ("heads_first", 32, 3), ("apart", 64, 2)])
+def test_values(dev, dtype, layout, ps, hkv):
+    """Every code under scales from the least to the largest that an append gives; NaN codes and scales;
+    chosen pages, some of them outside the pool; a page twice; none."""
+    print(f"[gpu] paged values {layout} {dtype}", flush=True)
+    s = Step8(dev, [1], [1], ps=ps, hkv=hkv, spare=9, layout=layout, data=False, seed=1)
+    g = torch.Generator().manual_seed(9)
+    s.k.view(torch.uint8).copy_(torch.randint(0, 256, s.k.shape, generator=g, dtype=torch.uint8))
+    s.v.view(torch.uint8).copy_(torch.randint(0, 256, s.v.shape, generator=g, dtype=torch.uint8))
+    low, high = RANGE.get(dtype, (-110, 119))
+    for t in (s.k_scale, s.v_scale):
+        e = torch.randint(low, high + 1, t.shape, generator=g) + 127
+        t.view(torch.uint8).copy_(e.to(torch.uint8))
+        t.view(torch.uint8)[2, 0, 0] = 255
+    same = lambda a, b: bool(((a.double() == b) | (a.isnan() & b.isnan())).all())  # noqa: E731
+    k, v = paged_values(s.k, s.v, **s.both, dtype=dtype)
+    assert k.dtype == dtype and k.is_contiguous() and k.shape == s.k.shape
+    assert same(k, s.held(s.k)) and same(v, s.held(s.v))
+    ids = torch.tensor([4, -1, 0, 4, s.k.shape[0], 2**30], dtype=torch.int32, device=dev)
+    k, v = paged_values(s.k, s.v, **s.both, pages=ids, dtype=dtype)
+    for got, whole in ((k, s.held(s.k)), (v, s.held(s.v))):
+        assert got.shape[0] == 6 and not bool(got[[1, 4, 5]].any())
+        assert same(got[[0, 2, 3]], whole[[4, 0, 4]])
+    k, v = paged_values(s.k, s.v, **s.both, pages=ids[:0], dtype=dtype)
+    assert k.shape == (0, hkv, ps, DH) and v.shape == k.shape
+
+
+@pytest.mark.gpu
+def test_same_with_and_without_the_tensor_module(dev, monkeypatch):
+    from dynakv_amd import _lib
+    print("[gpu] paged8 without the tensor module", flush=True)
+    out = []
+    for off in (False, True):
+        if off:
+            monkeypatch.setattr(_lib, "_tensor_calls", None)
+        got = []
+        for new, lens, dt in (([1, 1], [30, 2000], BF), ([70, 3], [100, 90], FP)):
+            s = Step8(dev, new, lens, hkv=2, seed=61, dtype=dt)
+            qkv = s.rand(s.T, 12 * DH)
+            q = paged_append(qkv, s.k, s.v, s.batch, heads=8, theta=1e4, **s.both)
+            got += [q, paged_attention(q, s.k, s.v, s.batch, **s.both), s.k, s.v, s.k_scale, s.v_scale]
+            got += paged_values(s.k, s.v, **s.both, dtype=dt)
+            got += paged_values(s.k, s.v, **s.both, pages=s.batch.page_table[0], dtype=torch.float32)
+        out.append(got)
+    for x, y in zip(*out):
+        assert x.dtype == y.dtype and torch.equal(u8(x), u8(y))
