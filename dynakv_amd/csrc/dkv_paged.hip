@@ -973,7 +973,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     }
     return s;
   };
-  if constexpr (Q8) scales = fetch_scales(t0, ids);
 
   // tile loads: wave w, instruction i stores keys 64 / NW * w + 4 i + lane / 16 of the tile, LDS piece
   // lane % 16, which holds the key's 16-byte piece (lane % 16) ^ (key % 16)
@@ -1022,7 +1021,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   constexpr uint32_t K8_BYTES = CK * PG_DH;
   auto ring_after = [](uint32_t r) { return r == 2 * K8_BYTES ? 0u : r + K8_BYTES; };
   auto ring_before = [](uint32_t r) { return r == 0 ? 2 * K8_BYTES : r - K8_BYTES; };
-  auto fetch = [&](int t, int page, uint32_t s, uint32_t ring) {
+  auto fetch = [&](int t, int page, uint32_t ring) {
     const int key = t * CK + key_in_tile;
     // (the wave's, and told so: else every load would come in a loop over its lanes' resources)
     const int in_page = __builtin_amdgcn_readfirstlane((key & slot_mask) * PG_DH);
@@ -1032,7 +1031,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         dkv_make_rsrc((const uint8_t*)p.k + (long long)kvh * p.pool.head_stride + at, bytes);
     const __amdgpu_buffer_rsrc_t rv =
         dkv_make_rsrc((const uint8_t*)p.v + (long long)kvh * p.pool.head_stride + at, bytes);
-    c_scales = s;
     if constexpr (K8) {
       pg_lds_loads<false>(rk, dkv_lds_addr(sKV) + ring + blk * 16 * PG_DH, koff);
 #pragma unroll
@@ -1056,18 +1054,18 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       const int kk = sub + 8 * i + (lane >> 3);  // key of the block
       place_off[i][e] = (uint32_t)((blk * 16 + kk) * 256 + 16 * ((2 * (lane & 7) + e) ^ kk));
     }
-  // part x of what was fetched (i = x / 2 of the keys, x even, or the values), into tile t's buffers
+  // A quarter of what was fetched (16 bytes of a load's 32: half e of load i, of the keys or the values) to
+  // tile t's buffers. K8: of the values alone, quarters 0 .. 2 CW - 1.
+  constexpr int PARTS = K8 ? 2 * CW : 4 * CW;
   auto place = [&](int t, int x) {
-    if (K8 && !(x & 1)) return;
-    const int i = x >> 1;
-    const dkv_u32x4 w = x & 1 ? cv[i] : ck[i];
-    const float s = pg_scale(x & 1 ? c_scales >> 8 : c_scales & 0xffu);
+    const bool value = K8 || (x & 1);
+    const int y = K8 ? x : x >> 1, i = y >> 1, e = y & 1;
+    const dkv_u32x4 w = value ? cv[i] : ck[i];
+    const float s = pg_scale(value ? c_scales >> 8 : c_scales & 0xffu);
     const uint32_t base = place0 + (uint32_t)(t & 1) * CTILE_BYTES;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *(lds_u32x4*)(base + (uint32_t)(x & 1) * 2 * CTILE_BYTES + place_off[i][e]) =
-          dkv_u32x4{pg_pair<DT, false>(w[2 * e], s), pg_pair<DT, true>(w[2 * e], s),
-                    pg_pair<DT, false>(w[2 * e + 1], s), pg_pair<DT, true>(w[2 * e + 1], s)};
+    *(lds_u32x4*)(base + (value ? 2 * CTILE_BYTES : 0) + place_off[i][e]) =
+        dkv_u32x4{pg_pair<DT, false>(w[2 * e], s), pg_pair<DT, true>(w[2 * e], s),
+                  pg_pair<DT, false>(w[2 * e + 1], s), pg_pair<DT, true>(w[2 * e + 1], s)};
   };
   // tile t's fetch; pages and scales of the next 16 tiles come two tiles before the products need them
   auto fetch_ahead = [&](int t, uint32_t ring) {
@@ -1079,8 +1077,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       if (t + 16 < n_tiles) ids_next = fetch_ids(t + 16);
     }
     if (u == 8 && t + 8 < n_tiles) scales_next = fetch_scales(t + 8, ids_next);
-    fetch(t, __builtin_amdgcn_readlane(ids, 4 * u + blk),
-          __builtin_amdgcn_readlane(scales, 4 * u + blk), ring);
+    c_scales = __builtin_amdgcn_readlane(scales, 4 * u + blk);
+    fetch(t, __builtin_amdgcn_readlane(ids, 4 * u + blk), ring);
   };
 
   dkv_f32x4 acc[QB][8];
@@ -1109,14 +1107,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       (4 * g + (n >> 2)) * 256 + 16 * (((n & 3) >> 1) ^ (4 * g + (n >> 2))) + 8 * (n & 1);
 
   if constexpr (Q8) {
-    if (t0 < n_tiles) {
-      fetch(t0, __builtin_amdgcn_readlane(ids, blk), __builtin_amdgcn_readlane(scales, blk), 0);
-#pragma unroll
-      for (int x = 0; x < 2 * CW; ++x) place(t0, x);
-    }
-    if (t0 + 1 < n_tiles)
-      fetch(t0 + 1, __builtin_amdgcn_readlane(ids, 4 + blk),
-            __builtin_amdgcn_readlane(scales, 4 + blk), K8_BYTES);
+    if (t0 < n_tiles) fetch(t0, __builtin_amdgcn_readlane(ids, blk), 0);
+    scales = fetch_scales(t0, ids);
   } else {
     if (t0 < n_tiles) issue(t0, __builtin_amdgcn_readlane(ids, blk));
   }
@@ -1166,10 +1158,22 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       }
     }
   }
+  if constexpr (Q8) {
+    if (t0 < n_tiles) {
+      c_scales = __builtin_amdgcn_readlane(scales, blk);
+      pg_wait_vm();
+#pragma unroll
+      for (int x = 0; x < PARTS; ++x) place(t0, x);
+    }
+    if (t0 + 1 < n_tiles) {
+      c_scales = __builtin_amdgcn_readlane(scales, 4 + blk);
+      fetch(t0 + 1, __builtin_amdgcn_readlane(ids, 4 + blk), K8_BYTES);
+    }
+  }
   uint32_t scales_now = scales;  // of the 16 tiles that the products are at
   const uint32_t krd8 = n * PG_DH + 16 * (g ^ swizzle8(n));
   for (int t = t0; t < n_tiles; ++t) {
-    if constexpr (!Q8 || K8) pg_wait_vm();
+    if constexpr (!Q8) pg_wait_vm();
     __syncthreads();  // tile t is in LDS for every wave; tile t - 1's buffer is free
     uint32_t gone;
     if constexpr (Q8) {
@@ -1191,17 +1195,18 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         issue(t + 1, __builtin_amdgcn_readlane(ids, 4 * (t + 1 - ids_base) + blk));
       }
     }
-    if constexpr (Q8) {
-      if (t + 1 < n_tiles) {
-#pragma unroll
-        for (int x = 0; x < 2 * CW; ++x) place(t + 1, x);
-      }
-      if (t + 2 < n_tiles) fetch_ahead(t + 2, ring_before(k_ring));
-    }
     const uint32_t k_tile = k_ring;
     k_ring = ring_after(k_ring);
     const int key0 = t * CK;
-    if (key0 >= w_end) continue;  // every key of the tile is past the wave's rows
+    if (key0 >= w_end) {  // every key of the tile is past the wave's rows
+      if constexpr (Q8) {
+        pg_wait_vm();
+#pragma unroll
+        for (int x = 0; x < PARTS; ++x) place(t + 1, x);
+        if (t + 2 < n_tiles) fetch_ahead(t + 2, ring_before(k_tile));
+      }
+      continue;
+    }
     const uint32_t kt = dkv_lds_addr(sK(t & 1));
     const uint32_t vt = dkv_lds_addr(sV(t & 1)) + vrd;
     dkv_f32x4 z[QB][4];
@@ -1323,7 +1328,16 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         }
         if (j == 0 && db % (4 / QB) == 4 / QB - 1)
           probs(1, db / (4 / QB) % 2, db / (8 / QB));
+        // Among the last products, which have no vector work of their own: the next tile, fetched a tile
+        // ago (after the last one what was fetched before goes where nobody reads it).
+        if constexpr (Q8) {
+          if (j == 1 && db == 0) pg_wait_vm();
+          if (j == 1 && db % (8 / PARTS) == 0) place(t + 1, db / (8 / PARTS));
+        }
       }
+    }
+    if constexpr (Q8) {
+      if (t + 2 < n_tiles) fetch_ahead(t + 2, ring_before(k_tile));
     }
   }
 
