@@ -895,8 +895,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   constexpr int QW = 16 * QB;            // rows per wave
   constexpr int BQ = NW * QW;            // rows per workgroup
   constexpr int LW = CK / 4 / NW;        // K (or V) loads per wave and tile, 4 keys each
-  // Codes of keys go to the score products as they are (below); fp16 queries would take three e4m3 parts
-  constexpr bool K8 = Q8 && DT == DKV_BF16;
   static_assert(!Q8 || NW == 4, "a wave stages a block of 16 keys");
   auto sK = [&](int i) { return sKV + i * CTILE_BYTES; };
   auto sV = [&](int i) { return sKV + (2 + i) * CTILE_BYTES; };
@@ -950,8 +948,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     const uint16_t* qp = p.q + (long long)(r.row0 + i) * p.q_st +
                          (long long)(kvh * p.hpg + h) * p.q_sh + 8 * g;
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-      qop[qb][s] = *(const dkv_u32x4*)(qp + (K8 ? 8 * g + 64 * (s >> 1) + 8 * (s & 1) : 32 * s));
+    for (int s = 0; s < 4; ++s) qop[qb][s] = *(const dkv_u32x4*)(qp + 32 * s);
     limit[qb] = min(r.pos0 + i, r.len - 1);
   }
   // blocks with keys but no page
@@ -1010,18 +1007,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   constexpr int CW = LW / 2;
   dkv_u32x4 ck[CW], cv[CW];
   uint32_t c_scales = 0x7f7f;
-  // K8: the tile's keys as codes in the first of three LDS buffers in turn (8 KB each), 16-byte pieces
-  // XOR-swizzled as in the few-row kernel; the products read pieces g and g + 4 of key 16 kb + n.
-  uint32_t koff[2] = {0, 0}, k_ring = 0;  // (ring: bytes from sKV to the buffer of the tile at hand)
-  if constexpr (K8) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      koff[i] = (uint32_t)((lane >> 3) * PG_DH + 16 * ((lane & 7) ^ swizzle8(8 * i + (lane >> 3))));
-  }
-  constexpr uint32_t K8_BYTES = CK * PG_DH;
-  auto ring_after = [](uint32_t r) { return r == 2 * K8_BYTES ? 0u : r + K8_BYTES; };
-  auto ring_before = [](uint32_t r) { return r == 0 ? 2 * K8_BYTES : r - K8_BYTES; };
-  auto fetch = [&](int t, int page, uint32_t ring) {
+  auto fetch = [&](int t, int page) {
     const int key = t * CK + key_in_tile;
     // (the wave's, and told so: else every load would come in a loop over its lanes' resources)
     const int in_page = __builtin_amdgcn_readfirstlane((key & slot_mask) * PG_DH);
@@ -1031,17 +1017,10 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         dkv_make_rsrc((const uint8_t*)p.k + (long long)kvh * p.pool.head_stride + at, bytes);
     const __amdgpu_buffer_rsrc_t rv =
         dkv_make_rsrc((const uint8_t*)p.v + (long long)kvh * p.pool.head_stride + at, bytes);
-    if constexpr (K8) {
-      pg_lds_loads<false>(rk, dkv_lds_addr(sKV) + ring + blk * 16 * PG_DH, koff);
 #pragma unroll
-      for (int i = 0; i < CW; ++i)
-        cv[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, 1024 * i + 16 * lane, 0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < CW; ++i) {
-        ck[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, 1024 * i + 16 * lane, 0, 0);
-        cv[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, 1024 * i + 16 * lane, 0, 0);
-      }
+    for (int i = 0; i < CW; ++i) {
+      ck[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, 1024 * i + 16 * lane, 0, 0);
+      cv[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, 1024 * i + 16 * lane, 0, 0);
     }
   };
   typedef __attribute__((address_space(3))) dkv_u32x4 lds_u32x4;
@@ -1054,13 +1033,12 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       const int kk = sub + 8 * i + (lane >> 3);  // key of the block
       place_off[i][e] = (uint32_t)((blk * 16 + kk) * 256 + 16 * ((2 * (lane & 7) + e) ^ kk));
     }
-  // A quarter of what was fetched (16 bytes of a load's 32: half e of load i, of the keys or the values) to
-  // tile t's buffers. K8: of the values alone, quarters 0 .. 2 CW - 1.
-  constexpr int PARTS = K8 ? 2 * CW : 4 * CW;
-  auto place = [&](int t, int x) {
-    const bool value = K8 || (x & 1);
-    const int y = K8 ? x : x >> 1, i = y >> 1, e = y & 1;
-    const dkv_u32x4 w = value ? cv[i] : ck[i];
+  // Half e of load i, of the keys or the values (part x = 4 i + 2 e + value), to tile t's buffers
+  constexpr int PARTS = 4 * CW;
+  auto place = [&](int t, int x, const dkv_u32x4* keys, const dkv_u32x4* values) {
+    const bool value = x & 1;
+    const int i = x >> 2, e = (x >> 1) & 1;
+    const dkv_u32x4 w = value ? values[i] : keys[i];
     const float s = pg_scale(value ? c_scales >> 8 : c_scales & 0xffu);
     const uint32_t base = place0 + (uint32_t)(t & 1) * CTILE_BYTES;
     *(lds_u32x4*)(base + (value ? 2 * CTILE_BYTES : 0) + place_off[i][e]) =
@@ -1068,7 +1046,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
                   pg_pair<DT, false>(w[2 * e + 1], s), pg_pair<DT, true>(w[2 * e + 1], s)};
   };
   // tile t's fetch; pages and scales of the next 16 tiles come two tiles before the products need them
-  auto fetch_ahead = [&](int t, uint32_t ring) {
+  auto fetch_ahead = [&](int t) {
     const int u = (t - t0) & 15;
     if (u == 0) {
       ids = ids_next;
@@ -1078,7 +1056,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     }
     if (u == 8 && t + 8 < n_tiles) scales_next = fetch_scales(t + 8, ids_next);
     c_scales = __builtin_amdgcn_readlane(scales, 4 * u + blk);
-    fetch(t, __builtin_amdgcn_readlane(ids, 4 * u + blk), ring);
+    fetch(t, __builtin_amdgcn_readlane(ids, 4 * u + blk));
   };
 
   dkv_f32x4 acc[QB][8];
@@ -1106,9 +1084,19 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   const uint32_t vrd =
       (4 * g + (n >> 2)) * 256 + 16 * (((n & 3) >> 1) ^ (4 * g + (n >> 2))) + 8 * (n & 1);
 
-  if constexpr (Q8) {
-    if (t0 < n_tiles) fetch(t0, __builtin_amdgcn_readlane(ids, blk), 0);
+  if constexpr (Q8) {  // the first two tiles at once: of the first, what the accumulators' registers take
+    dkv_u32x4 k0[CW], v0[CW];
+    if (t0 < n_tiles) fetch(t0, __builtin_amdgcn_readlane(ids, blk));
+#pragma unroll
+    for (int i = 0; i < CW; ++i) k0[i] = ck[i], v0[i] = cv[i];
     scales = fetch_scales(t0, ids);
+    if (t0 + 1 < n_tiles) fetch(t0 + 1, __builtin_amdgcn_readlane(ids, 4 + blk));
+    if (t0 < n_tiles) {
+      c_scales = __builtin_amdgcn_readlane(scales, blk);
+#pragma unroll
+      for (int x = 0; x < PARTS; ++x) place(t0, x, k0, v0);
+    }
+    c_scales = __builtin_amdgcn_readlane(scales, 4 + blk);
   } else {
     if (t0 < n_tiles) issue(t0, __builtin_amdgcn_readlane(ids, blk));
   }
@@ -1118,60 +1106,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
     for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(qop[qb][s]));
-  // K8: bf16 queries as two e4m3 parts, q = 2^e (hi + lo / 16), e the row's least with |q| <= 448 2^e: four
-  // bits each make up bf16's eight, so this is q but for what falls below 2^-21 of the row's largest. The
-  // products with the codes of the keys are 16x16x128 deep, two for four of 32, and take the powers of two
-  // of rows and blocks of keys as their scales: no key is converted, a tile's keys are half the bytes of LDS.
-  typedef __attribute__((ext_vector_type(8))) int i32x8;
-  i32x8 q_part[QB][2];
-  int q_scale[QB];  // of hi, and above it of lo
-  if constexpr (K8) {
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      auto q_of = [&](int x) {  // element x of the lane's 32
-        const uint32_t w = qop[qb][x >> 3][(x >> 1) & 3];
-        return dkv_elt_to_f32<DT>(x & 1 ? w >> 16 : w & 0xffffu);
-      };
-      float most = 0.f;
-#pragma unroll
-      for (int x = 0; x < 32; ++x) most = fmaxf(most, fabsf(q_of(x)));
-      const uint32_t bits = __float_as_uint(pg_max4(most));
-      const int e = min(max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u), -100), 119);
-      const float by = __uint_as_float((uint32_t)(127 - e) << 23);
-      q_scale[qb] = (127 + e) | (127 + e - 4) << 8;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        float x[4];
-        uint32_t hi, lo;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = q_of(4 * d + k) * by;
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
-        x[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8(hi, 0)) * 16.f;
-        x[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8(hi, 1)) * 16.f;
-        x[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8(hi, 2)) * 16.f;
-        x[3] = (x[3] - __builtin_amdgcn_cvt_f32_fp8(hi, 3)) * 16.f;
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
-        q_part[qb][0][d] = (int)hi;
-        q_part[qb][1][d] = (int)lo;
-      }
-    }
-  }
-  if constexpr (Q8) {
-    if (t0 < n_tiles) {
-      c_scales = __builtin_amdgcn_readlane(scales, blk);
-      pg_wait_vm();
-#pragma unroll
-      for (int x = 0; x < PARTS; ++x) place(t0, x);
-    }
-    if (t0 + 1 < n_tiles) {
-      c_scales = __builtin_amdgcn_readlane(scales, 4 + blk);
-      fetch(t0 + 1, __builtin_amdgcn_readlane(ids, 4 + blk), K8_BYTES);
-    }
-  }
-  uint32_t scales_now = scales;  // of the 16 tiles that the products are at
-  const uint32_t krd8 = n * PG_DH + 16 * (g ^ swizzle8(n));
   for (int t = t0; t < n_tiles; ++t) {
     if constexpr (!Q8) pg_wait_vm();
     __syncthreads();  // tile t is in LDS for every wave; tile t - 1's buffer is free
@@ -1180,7 +1114,6 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
       if (t == ids_base + 16) {
         ids_base += 16;
         absent = absent_next;
-        scales_now = scales;
       }
       gone = (uint32_t)(absent >> (4 * (t - ids_base))) & 15u;
     } else {
@@ -1195,15 +1128,12 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         issue(t + 1, __builtin_amdgcn_readlane(ids, 4 * (t + 1 - ids_base) + blk));
       }
     }
-    const uint32_t k_tile = k_ring;
-    k_ring = ring_after(k_ring);
     const int key0 = t * CK;
     if (key0 >= w_end) {  // every key of the tile is past the wave's rows
       if constexpr (Q8) {
-        pg_wait_vm();
 #pragma unroll
-        for (int x = 0; x < PARTS; ++x) place(t + 1, x);
-        if (t + 2 < n_tiles) fetch_ahead(t + 2, ring_before(k_tile));
+        for (int x = 0; x < PARTS; ++x) place(t + 1, x, ck, cv);
+        if (t + 2 < n_tiles) fetch_ahead(t + 2);
       }
       continue;
     }
@@ -1215,30 +1145,12 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
     for (int kb = 0; kb < 4; ++kb) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (K8) {
-        const uint32_t at = dkv_lds_addr(sKV) + k_tile + krd8;
-        const dkv_u32x4 a0 = *(const lds_u32x4*)(at + 2048 * kb);
-        const dkv_u32x4 a1 = *(const lds_u32x4*)((at ^ 64) + 2048 * kb);
-        const i32x8 a = {(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w,
-                         (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
-        const int sk = __builtin_amdgcn_readlane(scales_now, 4 * (t - ids_base) + kb);
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
-          z[qb][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              a, q_part[qb][0], z[qb][kb], 0, 0, 0, sk, 0, q_scale[qb]);
+      for (int s = 0; s < 4; ++s) {
+        const dkv_u32x4 a = *(const lds_u32x4*)(((kt + krd) ^ (64 * s)) + 4096 * kb);
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
-          z[qb][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              a, q_part[qb][1], z[qb][kb], 0, 0, 0, sk, 1, q_scale[qb]);
-      } else {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const dkv_u32x4 a = *(const lds_u32x4*)(((kt + krd) ^ (64 * s)) + 4096 * kb);
-#pragma unroll
-          for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_mfma32<DT>(a, qop[qb][s], z[qb][kb]);
-        }
+        for (int qb = 0; qb < QB; ++qb) z[qb][kb] = dkv_mfma32<DT>(a, qop[qb][s], z[qb][kb]);
       }
-      // (among the products; after the last tile what was fetched before goes where nobody reads it)
     }
     __builtin_amdgcn_s_setprio(0);
     if (key0 + CK - 1 > w_first || key0 + CK > r.len || gone) {
@@ -1331,13 +1243,13 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
         // Among the last products, which have no vector work of their own: the next tile, fetched a tile
         // ago (after the last one what was fetched before goes where nobody reads it).
         if constexpr (Q8) {
-          if (j == 1 && db == 0) pg_wait_vm();
-          if (j == 1 && db % (8 / PARTS) == 0) place(t + 1, db / (8 / PARTS));
+          static_assert(PARTS == 8, "a part for each block of dims");
+          if (j == 1) place(t + 1, db, ck, cv);
         }
       }
     }
     if constexpr (Q8) {
-      if (t + 2 < n_tiles) fetch_ahead(t + 2, ring_before(k_tile));
+      if (t + 2 < n_tiles) fetch_ahead(t + 2);
     }
   }
 
@@ -1606,8 +1518,10 @@ AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, 
       a.qb = 2, a.nw = 4, a.splits = ranges(wg128, 24);
     } else if (wg64 < 256 && ranges(wg64, 8) > 1) {
       a.qb = 1, a.nw = 4, a.splits = ranges(wg64, 8);
+    } else if (q8 && wg128 > 256) {
+      a.qb = 2, a.nw = 4;
     } else {
-      a.qb = 1, a.nw = wg128 > 256 && !a.few && !q8 ? 8 : 4;
+      a.qb = 1, a.nw = wg128 > 256 && !a.few ? 8 : 4;
     }
     a.bq = 16 * a.qb * a.nw;
     a.items = (int)items(a.bq);
