@@ -404,7 +404,8 @@ __global__ __launch_bounds__(V_THREADS) void paged_values_kernel(ValuesParams p)
       x = dkv_u32x4{pg_pair<ODT, false>(codes[u].x, s), pg_pair<ODT, true>(codes[u].x, s),
                     pg_pair<ODT, false>(codes[u].y, s), pg_pair<ODT, true>(codes[u].y, s)};
     }
-    *(dkv_u32x4*)(out + at * 16) = x;
+    // (past the caches: 35 us for 512 pages of 64 tokens, 44 through them)
+    __builtin_nontemporal_store(x, (dkv_u32x4*)(out + at * 16));
   }
 }
 
