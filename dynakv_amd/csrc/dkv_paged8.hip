@@ -129,35 +129,27 @@ __device__ __forceinline__ double pow2(int e) {
   return __builtin_bit_cast(double, (unsigned long long)(1023 + e) << 52);
 }
 
-// f rounded to e4m3, four to a dword; what is not finite becomes NaN.
-__device__ __forceinline__ uint32_t encode4(const float* f) {
-  float x[4];
-  bool odd = false;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    x[k] = __builtin_amdgcn_fmed3f(f[k], -E4M3_MAX, E4M3_MAX);
-    odd = odd || !(fabsf(f[k]) < INFINITY);
-  }
-  uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
-  if (odd) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (!(fabsf(f[k]) < INFINITY)) w = (w & ~(0xffu << (8 * k))) | (0x7fu << (8 * k));
-  }
-  return w;
-}
+// Eight numbers rounded to e4m3. ANY: what is past 448 is 448, what is not finite becomes NaN (else they
+// are neither).
+template <bool ANY>
 __device__ __forceinline__ dkv_u32x2 encode8(const float* f) {
-  return dkv_u32x2{encode4(f), encode4(f + 4)};
-}
-// d as a float from which e4m3 rounds as it would from d: where rounding to fp32 landed on a border
-// between two codes (or on a code, which has no more bits), a step to d's side of it.
-__device__ __forceinline__ float float_for_e4m3(double d) {
-  const float f = (float)d;
-  const uint32_t bits = __float_as_uint(f);
-  if ((bits & 0x7ffffu) == 0 && (double)f != d)  // (a NaN stays one)
-    return __uint_as_float(fabs(d) < fabs((double)f) ? bits - 1 : bits + 1);
-  return f;
+  uint32_t w[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = ANY ? __builtin_amdgcn_fmed3f(f[4 * k + i], -E4M3_MAX, E4M3_MAX) : f[4 * k + i];
+    w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w[k], true);
+    if constexpr (ANY) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(fabsf(f[4 * k + i]) < INFINITY))
+          w[k] = (w[k] & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
+    }
+  }
+  return dkv_u32x2{w[0], w[1]};
 }
 
 // Workgroup `wg`: one block, four units; wave w has unit w / 2, the tokens of half w % 2 of the block.
@@ -212,7 +204,8 @@ __device__ __forceinline__ void append8_block(const Append8Params& p, int wg, do
   }
 
   float f[16];  // y, then y scaled
-  double y[16], big = 0.0;
+  double y[16], big = 0.0, zeros = 0.0;
+  bool odd = false;  // something is not finite
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     f[2 * e] = dkv_elt_to_f32<DT>(xa[e] & 0xffffu);
@@ -247,8 +240,11 @@ __device__ __forceinline__ void append8_block(const Append8Params& p, int wg, do
         y[e] = fma(u, cs.x, -(w * cs.y));
         y[8 + e] = fma(w, cs.x, u * cs.y);
         big = fmax(big, fmax(fabs(y[e]), fabs(y[8 + e])));
+        zeros = fma(y[e], 0.0, fma(y[8 + e], 0.0, zeros));
       }
+      odd = !(zeros == 0.0);  // (a NaN, which is no maximum)
       if (!(big < INFINITY)) {  // without what is not finite
+        odd = true;
         big = 0.0;
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -256,10 +252,14 @@ __device__ __forceinline__ void append8_block(const Append8Params& p, int wg, do
       }
     }
   } else {
-    float m = 0.f;
+    float m = 0.f, none = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(f[e]));
-    if (!(m < INFINITY)) {
+    for (int e = 0; e < 16; ++e) {
+      m = fmaxf(m, fabsf(f[e]));
+      none = fmaf(f[e], 0.f, none);
+    }
+    if (!(none == 0.f)) {
+      odd = true;
       m = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -278,18 +278,32 @@ __device__ __forceinline__ void append8_block(const Append8Params& p, int wg, do
   if (has_old) e_new = max(e_new, old_e);
   e_new = __builtin_amdgcn_readfirstlane(e_new);
 
+  const bool any = __ballot(odd) || need > E_HIGH<DT>;
   if (isnew) {
     if (is_k) {
+      // y / 2^e as floats from which e4m3 rounds as it would from y: where rounding to fp32 landed on a
+      // border between two codes (or on a code, which has no more bits), a step to y's side of it
       const double by = pow2(-e_new);
+      uint32_t tie = 0xffffffffu;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] = float_for_e4m3(y[e] * by);
+      for (int e = 0; e < 16; ++e) {
+        y[e] *= by;
+        f[e] = (float)y[e];
+        tie = min(tie, __float_as_uint(f[e]) & 0x7ffffu);
+      }
+      if (tie == 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t bits = __float_as_uint(f[e]);
+          if ((bits & 0x7ffffu) == 0 && (double)f[e] != y[e])  // (a NaN stays one)
+            f[e] = __uint_as_float(fabs(y[e]) < fabs((double)f[e]) ? bits - 1 : bits + 1);
+        }
+      }
     } else {
       const float by = __uint_as_float((uint32_t)(127 - e_new) << 23);
 #pragma unroll
       for (int e = 0; e < 16; ++e) f[e] *= by;
     }
-    *(dkv_u32x2*)codes = encode8(f);
-    *(dkv_u32x2*)(codes + 64) = encode8(f + 8);
   } else if (isold && e_new > old_e) {
     const float down = __uint_as_float((uint32_t)max(127 + old_e - e_new, 0) << 23);
 #pragma unroll
@@ -303,14 +317,21 @@ __device__ __forceinline__ void append8_block(const Append8Params& p, int wg, do
       f[8 + 4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 2) * down;
       f[8 + 4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 3) * down;
     }
-    *(dkv_u32x2*)codes = encode8(f);
-    *(dkv_u32x2*)(codes + 64) = encode8(f + 8);
+  }
+  if (isnew || (isold && e_new > old_e)) {
+    if (any) {
+      *(dkv_u32x2*)codes = encode8<true>(f);
+      *(dkv_u32x2*)(codes + 64) = encode8<true>(f + 8);
+    } else {
+      *(dkv_u32x2*)codes = encode8<false>(f);
+      *(dkv_u32x2*)(codes + 64) = encode8<false>(f + 8);
+    }
   }
   if (lane == 0 && !(wave & 1)) *scale = (uint8_t)(127 + e_new);
 }
 
 template <int DT>
-__global__ __launch_bounds__(64 * A8_WAVES) void paged_append8_kernel(Append8Params p) {
+__global__ __launch_bounds__(64 * A8_WAVES, 6) void paged_append8_kernel(Append8Params p) {
   __shared__ double2 sTrig[PG_BLOCK * A8_ROW];
   __shared__ int sNeed[A8_WAVES];
   if ((int)blockIdx.x < p.kv_wgs) {

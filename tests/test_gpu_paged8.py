@@ -280,6 +280,21 @@ def test_append_extreme_values(dev, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_append_keeps_earlier_nans(dev, dtype):
+    """NaN codes of earlier tokens stay NaN where the block's scale rises; codes of both signs of zero and
+    the largest are rounded again as the others are."""
+    print("[gpu] paged append8 earlier NaN", flush=True)
+    s = Step8(dev, [2, 1], [14, 9], hkv=2, dtype=dtype, seed=35, data=False, spread=0, unit=-1)
+    page = int(s.table[0, 0])
+    for t in (s.k, s.v):
+        t.view(torch.uint8)[page, :, 3, :5] = torch.tensor([0x7f, 0xff, 0x80, 0x7e, 0xfe],
+                                                           dtype=torch.uint8, device=dev)
+    _check_append(s, 4, qkv=(s.rand(s.T, 8 * DH).float() * 8).to(dtype))
+    assert s.v[page, 0, 3, :2].double().isnan().all()
+
+
+@pytest.mark.gpu
 def test_append_leaves_padding_rows_and_what_has_no_place(dev):
     """Rows behind the last request, tokens whose page is outside the pool or past the table."""
     print("[gpu] paged append8 padding, bad pages", flush=True)
