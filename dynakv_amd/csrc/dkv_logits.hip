@@ -23,6 +23,11 @@ namespace {
 // bits. The mask is for other workgroups of the launch, which clear the tokens that it forbids, and only
 // those; the rows' workgroups look their tokens up in it.
 //
+// 256 rows of 128256 bf16 logits, histories of up to 4096 (400000 different tokens in all, a line of
+// memory each) 17 us, where counting by vocabulary takes 59; with a mask that forbids half 31.5. Rows so
+// few that they leave CUs idle are counted by vocabulary too: one row of 32000, a history of 1000, 4.4 us
+// against 6.2.
+//
 // Histories that no table of 64 KB holds (over 6144 tokens) are counted by vocabulary instead: a
 // workgroup has `span` tokens of a row's vocabulary, a word each, and reads the whole history.
 // ---------------------------------------------------------------------------------------

@@ -193,12 +193,22 @@ __device__ __forceinline__ int swizzle8(int t) { return (t ^ (t >> 3)) & 7; }
 // unit's last one to arrive. 16 requests of 2K to 8K tokens (8 KV heads) 63 us, 5.6 TB/s; two of 65533
 // 89 us, 6.0 TB/s; one of 96 5.0 us, the latency of lengths, page ids, one tile and the joins.
 //
-// How a step's units are cut, where there are fewer than D_WGS: requests have any lengths, which only
-// the device knows, and the launch has a fixed number of workgroups. Every wave finds the smallest part C
-// (tiles) for which sum over units of ceil(tiles / C) parts fit the launch, and takes its own from the
-// running sums. From D_WGS units on (32 requests of 8 KV heads) a unit is one workgroup's, whatever its
-// length: 32 requests of 8192 tokens 159 us (6.7 TB/s, partly from the memory-side cache), 33 of them 226,
-// a second round of workgroups; one of 65536 beside 39 of 500 570 us, beside 20 of 500, in parts, 66.
+// Of 8-bit pages (Q8) a tile is two blocks of 16 tokens, as many bytes. Codes stay codes in LDS and become
+// 16-bit numbers (one instruction for two, the block's scale in it) in the operands' registers: an eighth
+// of a wave's instructions, beside loads that are the bound. The products of values take 32 tokens' hi
+// parts, then their lo parts. 16 requests of 2K to 8K tokens 36.5 us, 4.9 TB/s (6 us of it are the start,
+// the joins and parts of unequal length); two of 131069 86 us, 6.2 TB/s; one of 96 5.3 us.
+//
+// How a step's units are cut: requests have any lengths, which only the device knows, and the launch has a
+// fixed number of workgroups. Every wave finds the smallest part C (tiles) for which sum over units of
+// ceil(tiles / C) parts fit the launch, and takes its own from the running sums. That is for fewer units
+// than the 256 workgroups of eight waves that fill the chip (32 requests of 8 KV heads); from there on a unit
+// is one workgroup's, whatever its length: 32 requests of 8192 tokens 159 us (6.7 TB/s, partly from the
+// memory-side cache), 33 of them 226, a second round of workgroups; one of 65536 beside 39 of 500 570 us,
+// beside 20 of 500, in parts, 66. Of 8-bit pages 256 to 511 units go to 512 workgroups of four waves, in
+// parts: 40 requests of 2K to 8K 76 us (87 in workgroups of eight waves), one of 65536 beside 39 of 500 37
+// (357); with fewer or more units those are the slower ones (4 requests 16.4 us against 14.6, 80 156 against
+// 142: a part more is a record more, and fewer waves share a unit's start and end).
 constexpr int DSLOT = 2;                    // tile slots per wave
 template <bool Q8>
 constexpr int DTILE = Q8 ? 32 : 16;
@@ -1001,9 +1011,14 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
                         dkv_lds_addr(sV(t & 1)) + CK / NW * wave * 256, voff);
   };
 
-  // Codes go through registers: a wave's part of a tile is fetched (two loads of 16 codes a lane, or one)
-  // while the tile before it is worked on, and stored to LDS as the 16-bit numbers that codes times scale
-  // are, where the products find them as they would a 16-bit cache's.
+  // Codes go through registers: a wave's part of a tile (two loads of 16 codes a lane) is fetched while the
+  // tile before it is worked on, and stored to LDS as the 16-bit numbers that codes times scale are, where
+  // the products find them as they would a 16-bit cache's: 32 conversions and eight stores a wave and tile,
+  // among the last products of values, which have no vector work of their own. One prompt of 8192 takes
+  // what it takes of 16-bit pages (518 us, fp16 518 to 520), four of 2048 168 (158): a workgroup's first tile
+  // waits for its scales besides its page. Tried and left: conversions before the tile's products (chunks 4%
+  // slower); eight waves a workgroup (8% slower); scores from the codes themselves, the queries in two e4m3
+  // parts and scales in the instruction (2% faster than that, not than this; 2 us a workgroup to split them).
   constexpr int CW = LW / 2;
   dkv_u32x4 ck[CW], cv[CW];
   uint32_t c_scales = 0x7f7f;
@@ -1470,7 +1485,8 @@ struct AttendPlan {
 //    (520).
 //  * otherwise one range: above 256 of 128 rows 1x8 (eight 300-token prompts 22.7, against 23.5 1x4,
 //    25.5 2x4), else 1x4 (512 tokens at 1024: 20.1, against 24.4 1x8 and 29 2x4/2: a range more
-//    costs its records, 66 KB a workgroup, written and read).
+//    costs its records, 66 KB a workgroup, written and read). Of 8-bit pages 2x4 above 256 (one
+//    2048-token prompt 57.8, against 63.5 1x4; 1x8 has no registers for codes on their way).
 AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, int max_len,
                        bool q8) {
   AttendPlan a = {};

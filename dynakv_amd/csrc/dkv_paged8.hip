@@ -24,7 +24,14 @@ constexpr int E_HIGH = DT == DKV_F16 ? 7 : 119;
 // are infinite or NaN are held as NaN and have no say in e.
 //
 // Keys are computed in 64 bits: which code a value gets turns over at borders, and 32-bit arithmetic with
-// the sine instruction put 350 of 8 million keys on another side of one.
+// the sine instruction (off by 2^-19 or so) would put some hundreds of 8 million on another side of one.
+//
+// 8192 tokens of 32 + 2 x 8 heads with norms 52 us by trace (49 in a row; a large copy takes 37 for the
+// bytes): the waves of keys have 12 us of issue slots, at three workgroups a CU (80 registers) partly
+// beside the others' traffic. 64 tokens 6.0 us, the chain of lengths, page id, scale and codes. Tried and
+// left: blocks and queries in turns on each CU (11% slower: both then have half the workgroups); a wave a
+// block and head, 134 registers (68 us); keys as fp32 only, computed again where that may not do (as fast,
+// 3.5 us more for few tokens).
 //
 // Two waves have one block and head (a unit: K heads, then V heads), eight tokens each: lane (token
 // lane / 8, piece c = lane % 8) holds dims 8c .. 8c + 7 and 64 + 8c .. 64 + 8c + 7. The four units of a

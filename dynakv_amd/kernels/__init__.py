@@ -10,6 +10,7 @@ Modules mirror the reference package ``src/dynakv/kernels/``:
 
 Beside them, for serving without compression:
 
-* :mod:`.paged` -- a paged cache for requests of different lengths, its append and its attention
-* :mod:`.sampling` -- tokens drawn from logits
+* :mod:`.paged` -- a paged cache for requests of different lengths, in 16 or 8 bits, its append and its
+  attention
+* :mod:`.sampling` -- tokens drawn from logits, and what changes logits before that
 """
