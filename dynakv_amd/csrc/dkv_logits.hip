@@ -122,7 +122,7 @@ __device__ __forceinline__ float adjusted(const LogitParams& p, const LogitRow& 
   if (c) {
     const uint32_t times = c & ~L_SEEN;
     x = x > 0.f ? x / r.rep : x * r.rep;
-    x = x - r.freq * (float)times - (times ? r.pres : 0.f);
+    if (times) x = x - r.freq * (float)times - r.pres;
   }
   if (e != L_NONE) {
     const int j = (int)(e & ~L_MORE);
@@ -380,7 +380,7 @@ extern "C" int dkv_adjust_logits(void* stream, int dtype, void* logits, long lon
   if (token_bytes != 4 && token_bytes != 8) return DKV_E_ARG;
   if (tokens_ld < 0 || bias_ids_ld < 0 || bias_ld < 0 || allowed_ld < 0) return DKV_E_ARG;
   if ((M > 0 && !bias_ids != !bias)) return DKV_E_ARG;
-  if (!repetition && !(repetition_all > 0.f)) return DKV_E_ARG;
+  if (!repetition && !(repetition_all > 0.f && repetition_all < INFINITY)) return DKV_E_ARG;
   LogitParams p;
   p.logits = logits;
   p.ld = ld;

@@ -204,6 +204,19 @@ def test_nothing_to_do(dev):
 
 
 @pytest.mark.gpu
+def test_infinite_penalties_ban_what_was_generated(dev):
+    """An infinite frequency or presence penalty takes the generated tokens out and no other."""
+    print("[gpu] adjust infinite penalties", flush=True)
+    for kw in (dict(frequency=math.inf), dict(presence=math.inf)):
+        x = torch.randn(1, 50, device=dev)
+        x0 = x.clone()
+        t = torch.tensor([[3, 4, 5, 5]], device=dev)
+        adjust_logits_(x, tokens=t, prompt_lens=2, **kw)
+        assert bool((x[0, 5] == -math.inf)) and torch.equal(x[0, :5], x0[0, :5])
+        assert torch.equal(x[0, 6:], x0[0, 6:])
+
+
+@pytest.mark.gpu
 def test_same_bits_every_time_captured_and_on_a_stream(dev):
     """Many biases of one token, repeated calls, a graph replayed with other histories in the same buffers,
     sampling after it in the graph."""
@@ -299,7 +312,7 @@ def test_c_entry_refusals():
     call = lambda **kw: lib.dkv_adjust_logits(*(base | kw).values())  # noqa: E731
     for kw in (dict(rows=-1), dict(V=-1), dict(N=-1), dict(M=-1), dict(logits=None), dict(ld=39),
                dict(size=2), dict(tld=-1), dict(al=-1), dict(M=3, bi=64), dict(M=3, b=64), dict(ra=0.0),
-               dict(ra=math.nan)):
+               dict(ra=math.nan), dict(ra=1e39), dict(ra=1e-50)):
         assert call(**kw) == _lib.DKV_E_ARG, kw
     for kw in (dict(dtype=7), dict(V=2**29, ld=2**29), dict(logits=66)):
         assert call(**kw) == _lib.DKV_E_UNSUPPORTED, kw

@@ -14,7 +14,8 @@ import torch
 
 from dynakv_amd.kernels.paged import (PagedBatch, PagedKVCache, paged_append, paged_attention,
                                       paged_values)
-from test_gpu_paged import BF, DH, FP, Step, _append_tol, _append_reference, _attend_reference, _freq
+from test_gpu_paged import (BF, DH, FP, Step, _append_reference, _append_tol, _attend_reference,
+                            _freq, _turn)
 
 CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 BLOCK = 16
@@ -615,7 +616,6 @@ def test_requests_that_come_and_go(dev, dtype):
             held = paged_values(cache.k[0], cache.v[0], **both, pages=ids, dtype=torch.float32)
             k, v = (t.transpose(1, 2).reshape(-1, hkv, DH)[:total].double() for t in held)
             x = kept[r].double().view(total, hq + 2 * hkv, DH)
-            from test_gpu_paged import _turn
             pos = torch.arange(total, dtype=torch.float64, device=dev)
             for got, want, scale in ((k, _turn(x[:, hq:hq + hkv], pos, _freq(dev, theta)), 0),
                                      (v, x[:, hq + hkv:], 1)):
