@@ -17,10 +17,10 @@ namespace {
 //
 // A workgroup has a row and a table in LDS of the tokens that its history and its biases name: open
 // addressing, at most three quarters full, a word for the token, one for its number (the generated ones
-// below the bit that says it was seen) and one for its biases. What it holds at the end does not depend
-// on the order of its atomics. Biases go by their entries: the first one of a token claims it (least
-// entry), sums the token's further ones in order and applies them, so that the same call gives the same
-// bits. The mask is for other workgroups of the launch, which clear the tokens that it forbids, and only
+// below the bit that says it was seen) and one for the sum of its biases. What it holds at the end does not
+// depend on the order of its atomics. One wave adds the biases, 64 entries at a time: of those of one token
+// the first, then the second and so on, so that sums are in the entries' order and the same call gives the
+// same bits (300 entries: 5 us a row, all on one token 67). The mask is for other workgroups of the launch, which clear the tokens that it forbids, and only
 // those; the rows' workgroups look their tokens up in it.
 //
 // 256 rows of 128256 bf16 logits, histories of up to 4096 (400000 different tokens in all, a line of
@@ -63,8 +63,7 @@ constexpr int L_THREADS = 512;
 constexpr int L_EACH = 4;            // tokens of a thread at a time
 constexpr int L_SPAN = L_THREADS * L_EACH;  // least span
 constexpr uint32_t L_SEEN = 0x80000000u;
-constexpr uint32_t L_NONE = 0x7fffffffu;  // no entry
-constexpr uint32_t L_MORE = 0x80000000u;  // further entries of the same token
+constexpr uint32_t L_NONE = 0xffffffffu;  // no bias (a NaN that no sum is kept as)
 
 constexpr int L_MASK = 8;            // tokens of a thread in a mask's workgroup
 
@@ -116,37 +115,46 @@ __device__ __forceinline__ int history(const LogitParams& p, int row, int j) {
   const int t = ((const int*)p.tokens)[(long long)row * p.tokens_ld + j];
   return t < p.V ? t : -1;
 }
-// What becomes of logit x of token id, of count c (0: not in the history) and bias entry e, bias b.
-__device__ __forceinline__ float adjusted(const LogitParams& p, const LogitRow& r, float x, int id,
-                                          uint32_t c, uint32_t e, float b) {
+// What becomes of logit x of count c (0: not in the history) and biases' sum e (bits).
+__device__ __forceinline__ float adjusted(const LogitRow& r, float x, uint32_t c, uint32_t e) {
   if (c) {
     const uint32_t times = c & ~L_SEEN;
     x = x > 0.f ? x / r.rep : x * r.rep;
     if (times) x = x - r.freq * (float)times - r.pres;
   }
-  if (e != L_NONE) {
-    const int j = (int)(e & ~L_MORE);
-    float sum = b;
-    if (e & L_MORE) {
-      // (sixteen entries' loads on their way together: 300 entries, two of one token, 40 us one by one)
-      constexpr int AHEAD = 16;
-      for (int k0 = j + 1; k0 < p.M; k0 += AHEAD) {
-        int ids[AHEAD];
-        float more[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          const int k = min(k0 + u, p.M - 1);
-          ids[u] = r.ids[k];
-          more[u] = r.bias[k];
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-          if (k0 + u < p.M && ids[u] == id) sum += more[u];
-      }
+  return e != L_NONE ? x + __uint_as_float(e) : x;
+}
+// The row's biases added to sums[slot(token)] (a slot below 0: none of this workgroup's), by one wave;
+// `turn`: a word for each slot, L_NONE before and after.
+template <class F>
+__device__ __forceinline__ void add_biases(const LogitParams& p, const LogitRow& r, uint32_t* sums,
+                                           uint32_t* turn, int lane, F&& slot) {
+  int id = lane < p.M ? r.ids[lane] : -1;
+  float b = lane < p.M ? r.bias[lane] : 0.f;
+  for (int j = 0; j < p.M; j += 64) {
+    const int s = id >= 0 && id < p.V ? slot(id) : -1;
+    const float mine = b;
+    if (j + 64 + lane < p.M) {
+      id = r.ids[j + 64 + lane];
+      b = r.bias[j + 64 + lane];
+    } else {
+      id = -1;
     }
-    x += sum;
+    // of the lanes left that have a slot, the lowest is next
+    for (bool left = s >= 0; __ballot(left);) {
+      if (left) atomicMin(turn + s, (uint32_t)lane);
+      __builtin_amdgcn_wave_barrier();
+      if (left && *(volatile uint32_t*)(turn + s) == (uint32_t)lane) {
+        volatile uint32_t* at = sums + s;
+        const uint32_t was = *at;
+        const float sum = was == L_NONE ? mine : __uint_as_float(was) + mine;
+        *at = sum == sum ? __float_as_uint(sum) : 0x7fc00000u;
+        *(volatile uint32_t*)(turn + s) = L_NONE;
+        left = false;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
   }
-  return x;
 }
 
 template <int DT>
@@ -178,17 +186,16 @@ __global__ __launch_bounds__(1024) void adjust_rows_kernel(LogitParams p) {
   for (int i = 4 * tid; i < 2 * slots; i += 4 * T)  // (key: the token + 1, 0 where none is)
     *(dkv_u32x4*)(lds + i) = dkv_u32x4{0u, 0u, 0u, 0u};
   if (p.bias_ids)
-    for (int i = 4 * tid; i < slots; i += 4 * T)
+    for (int i = 4 * tid; i < 2 * slots; i += 4 * T)  // (and the turns behind them)
       *(dkv_u32x4*)(entry + i) = dkv_u32x4{L_NONE, L_NONE, L_NONE, L_NONE};
-  // the first of the history and of the biases, whose number is not known yet, beside the settings
-  int first[L_EACH], first_bias = -1;
+  // the first of the history, whose number is not known yet, beside the settings
+  int first[L_EACH];
   if (p.tokens)
 #pragma unroll
     for (int u = 0; u < L_EACH; ++u) {
       const int j = tid + u * T;
       first[u] = j < p.N ? history(p, row, j) : -1;
     }
-  if (p.bias_ids && tid < p.M) first_bias = p.bias_ids[(long long)row * p.bias_ids_ld + tid];
   const LogitRow r = logit_row(p, row);
   __syncthreads();
   auto place = [&](int id) {  // the token's slot (there is a free one: fewer tokens than slots)
@@ -200,6 +207,8 @@ __global__ __launch_bounds__(1024) void adjust_rows_kernel(LogitParams p) {
       i = (i + 1) & (uint32_t)(slots - 1);
     }
   };
+  if (p.bias_ids && tid < 64)
+    add_biases(p, r, entry, entry + slots, tid, [&](int id) { return (int)place(id); });
   for (int j0 = tid; j0 < r.n; j0 += L_EACH * T) {
     int id[L_EACH];
 #pragma unroll
@@ -217,38 +226,18 @@ __global__ __launch_bounds__(1024) void adjust_rows_kernel(LogitParams p) {
         atomicAdd(count + i, 1u);
     }
   }
-  if (p.bias_ids) {
-    auto biased = [&](int j) {  // entry j's token, or -1
-      const int id = j == tid ? first_bias : r.ids[j];
-      return id < p.V ? id : -1;
-    };
-    uint32_t mine = 0;  // slot of entry tid
-    for (int j = tid; j < p.M; j += T)
-      if (biased(j) >= 0) {
-        const uint32_t i = place(biased(j));
-        if (j == tid) mine = i;
-        atomicMin(entry + i, (uint32_t)j);
-      }
-    __syncthreads();
-    for (int j = tid; j < p.M; j += T)
-      if (biased(j) >= 0) {
-        const uint32_t i = j == tid ? mine : place(biased(j));
-        if ((entry[i] & ~L_MORE) != (uint32_t)j) atomicOr(entry + i, L_MORE);
-      }
-  }
   __syncthreads();
   const __amdgpu_buffer_rsrc_t logits =
       dkv_make_rsrc((uint8_t*)p.logits + (long long)row * p.ld * SIZE, (uint32_t)p.V * SIZE);
   for (int i0 = tid; i0 < slots; i0 += L_EACH * T) {
     int id[L_EACH];
-    float x[L_EACH], b[L_EACH];
+    float x[L_EACH];
     uint32_t word[L_EACH], e[L_EACH];
 #pragma unroll
     for (int u = 0; u < L_EACH; ++u) {
       const int i = i0 + u * T;
       id[u] = i < slots ? (int)key[i] - 1 : -1;
       e[u] = p.bias_ids && id[u] >= 0 ? entry[i] : L_NONE;
-      b[u] = e[u] != L_NONE ? r.bias[e[u] & ~L_MORE] : 0.f;
       x[u] = load_logit<DT>(logits, id[u] >= 0 ? id[u] * SIZE : DKV_OOB);
       word[u] = 0xffffffffu;
       if (p.allowed && id[u] >= 0)
@@ -258,7 +247,7 @@ __global__ __launch_bounds__(1024) void adjust_rows_kernel(LogitParams p) {
     for (int u = 0; u < L_EACH; ++u) {
       if (id[u] < 0) continue;
       const int i = i0 + u * T;
-      float y = adjusted(p, r, x[u], id[u], count[i], e[u], b[u]);
+      float y = adjusted(r, x[u], count[i], e[u]);
       if (!((word[u] >> (id[u] & 31)) & 1u)) y = -INFINITY;
       store_logit<DT>(logits, id[u] * SIZE, y);
     }
@@ -280,16 +269,15 @@ __global__ __launch_bounds__(L_THREADS) void adjust_vocabulary_kernel(LogitParam
   if (p.tokens)
     for (int i = 4 * tid; i < p.span; i += 4 * L_THREADS) *(dkv_u32x4*)(count + i) = dkv_u32x4{0u, 0u, 0u, 0u};
   if (p.bias_ids)
-    for (int i = 4 * tid; i < p.span; i += 4 * L_THREADS)
+    for (int i = 4 * tid; i < 2 * p.span; i += 4 * L_THREADS)  // (and the turns behind them)
       *(dkv_u32x4*)(entry + i) = dkv_u32x4{L_NONE, L_NONE, L_NONE, L_NONE};
-  int first[L_EACH], first_bias = -1;  // (as in the kernel by rows)
+  int first[L_EACH];  // (as in the kernel by rows)
   if (p.tokens)
 #pragma unroll
     for (int u = 0; u < L_EACH; ++u) {
       const int j = tid + u * L_THREADS;
       first[u] = j < p.N ? history(p, row, j) : -1;
     }
-  if (p.bias_ids && tid < p.M) first_bias = p.bias_ids[(long long)row * p.bias_ids_ld + tid];
   const LogitRow r = logit_row(p, row);
   if (p.tokens || p.bias_ids) __syncthreads();
   for (int j0 = tid; j0 < r.n; j0 += L_EACH * L_THREADS) {
@@ -308,18 +296,9 @@ __global__ __launch_bounds__(L_THREADS) void adjust_vocabulary_kernel(LogitParam
         atomicAdd(count + at[u], 1u);
     }
   }
-  if (p.bias_ids) {
-    auto biased = [&](int j) {  // entry j's token from v0 on, or -1
-      const int id = j == tid ? first_bias : r.ids[j];
-      return id >= v0 && id - v0 < span ? id - v0 : -1;
-    };
-    for (int j = tid; j < p.M; j += L_THREADS)
-      if (biased(j) >= 0) atomicMin(entry + biased(j), (uint32_t)j);
-    __syncthreads();
-    for (int j = tid; j < p.M; j += L_THREADS)
-      if (biased(j) >= 0 && (entry[biased(j)] & ~L_MORE) != (uint32_t)j)
-        atomicOr(entry + biased(j), L_MORE);
-  }
+  if (p.bias_ids && tid < 64)
+    add_biases(p, r, entry, entry + p.span, tid,
+               [&](int id) { return id >= v0 && id - v0 < span ? id - v0 : -1; });
   if (p.tokens || p.bias_ids) __syncthreads();
 
   // the tokens that anything concerns (the others at an offset that neither loads nor stores)
@@ -352,8 +331,7 @@ __global__ __launch_bounds__(L_THREADS) void adjust_vocabulary_kernel(LogitParam
 #pragma unroll
     for (int u = 0; u < L_EACH; ++u) {
       const int i = i0 + u * L_THREADS;
-      const float b = e[u] != L_NONE ? r.bias[e[u] & ~L_MORE] : 0.f;
-      const float y = off[u] ? -INFINITY : adjusted(p, r, x[u], v0 + i, c[u], e[u], b);
+      const float y = off[u] ? -INFINITY : adjusted(r, x[u], c[u], e[u]);
       const bool writes = c[u] || e[u] != L_NONE || off[u];
       store_logit<DT>(logits, writes ? i * SIZE : DKV_OOB, y);
     }
@@ -409,7 +387,7 @@ extern "C" int dkv_adjust_logits(void* stream, int dtype, void* logits, long lon
   p.allowed_ld = allowed_ld;
   if (!p.tokens && !p.bias_ids && !p.allowed) return DKV_OK;
   hipStream_t st = (hipStream_t)stream;
-  const int words = (p.tokens ? 1 : 0) + (p.bias_ids ? 1 : 0);
+  const int words = (p.tokens ? 1 : 0) + (p.bias_ids ? 2 : 0);
   auto launch = [&](auto f32, auto f16, auto bf16, long long wgs, int threads, size_t lds) {
     const dim3 grid((unsigned)wgs);
     if (dtype == DKV_F32)
@@ -422,7 +400,7 @@ extern "C" int dkv_adjust_logits(void* stream, int dtype, void* logits, long lon
   const long long named = (p.tokens ? (long long)N : 0) + M;
   int log2 = 9;
   while (log2 < 30 && 3LL << log2 < 4 * named) ++log2;
-  const size_t table = ((size_t)4 << log2) * (p.bias_ids ? 3 : 2);
+  const size_t table = ((size_t)4 << log2) * (p.bias_ids ? 4 : 2);
   const bool few = words && (long long)rows * ((V + L_SPAN - 1) / L_SPAN) <= 256;
   if (table <= 65536 && !few) {
     const int threads = named > 1024 ? 1024 : L_THREADS;
@@ -436,7 +414,7 @@ extern "C" int dkv_adjust_logits(void* stream, int dtype, void* logits, long lon
   } else {
     // spans of 2048 tokens to 64 KB of counts and entries (two workgroups a CU), as small as fills the chip
     int span = L_SPAN;
-    const int most = words == 2 ? 8192 : 16384;
+    const int most = words == 3 ? 4096 : words == 2 ? 8192 : 16384;
     while (span < most && (long long)rows * ((V + 2 * span - 1) / (2 * span)) >= 512) span *= 2;
     p.span = span;
     p.slices = (V + span - 1) / span;
