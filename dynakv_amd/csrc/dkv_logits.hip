@@ -20,16 +20,18 @@ namespace {
 // below the bit that says it was seen) and one for the sum of its biases. What it holds at the end does not
 // depend on the order of its atomics. One wave adds the biases, 64 entries at a time: of those of one token
 // the first, then the second and so on, so that sums are in the entries' order and the same call gives the
-// same bits (300 entries: 5 us a row, all on one token 67). The mask is for other workgroups of the launch, which clear the tokens that it forbids, and only
-// those; the rows' workgroups look their tokens up in it.
+// same bits (300 entries: 5 us a row, all on one token 67). A token's turn is a fourth word. The mask is for
+// other workgroups of the launch, which clear the tokens that it forbids, and only those; the rows'
+// workgroups look their tokens up in it.
 //
 // 256 rows of 128256 bf16 logits, histories of up to 4096 (400000 different tokens in all, a line of
 // memory each) 17 us, where counting by vocabulary takes 59; with a mask that forbids half 31.5. Rows so
 // few that they leave CUs idle are counted by vocabulary too: one row of 32000, a history of 1000, 4.4 us
 // against 6.2.
 //
-// Histories that no table of 64 KB holds (over 6144 tokens) are counted by vocabulary instead: a
-// workgroup has `span` tokens of a row's vocabulary, a word each, and reads the whole history.
+// Histories that no table of 64 KB holds (over 6144 tokens, half of that with biases) are counted by
+// vocabulary instead: a workgroup has `span` tokens of a row's vocabulary, a word each, and reads the whole
+// history.
 // ---------------------------------------------------------------------------------------
 struct LogitParams {
   void* logits;
