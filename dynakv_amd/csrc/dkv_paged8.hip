@@ -1,6 +1,7 @@
 // Pages of 8 bits: the append of a step's keys and values to them, and pages read back as values.
 // The layout of codes and scales: dkv_paged.h. The attention over them: dkv_paged.hip.
 #include "dkv_paged.h"
+#include "dkv_paged_index.h"
 
 namespace {
 
@@ -398,23 +399,22 @@ __global__ __launch_bounds__(V_THREADS) void paged_values_kernel(ValuesParams p)
   uint32_t byte[V_EACH];
 #pragma unroll
   for (int u = 0; u < V_EACH; ++u) {
-    const long long at = at0 + u * V_THREADS, token = at / PIECES;
+    const long long at = at0 + u * V_THREADS;
     codes[u] = dkv_u32x2{0u, 0u};
     byte[u] = 127;
     if (at >= p.pieces) continue;
-    const int row = (int)(token >> p.page_shift);  // page and head
-    const int i = quot(p.by_hkv, row), h = row - i * p.Hkv;
-    const int slot = (int)token & ((1 << p.page_shift) - 1), piece = (int)at % PIECES;
+    const PagedPiece x = paged_piece<PIECES>(at, p.page_shift);  // (row: page and head)
+    const int i = quot(p.by_hkv, x.row), h = x.row - i * p.Hkv;
     const int page = p.ids ? p.ids[i] : i;
     if (page < 0 || page >= p.num_pages) continue;
     const uint8_t* src = pool + (long long)page * p.page_stride + (long long)h * p.head_stride +
-                         slot * PG_DH + CODES * piece;
+                         x.slot * PG_DH + CODES * x.piece;
     if constexpr (CODES == 8)
       codes[u] = *(const dkv_u32x2*)src;
     else
       codes[u].x = *(const uint32_t*)src;
     byte[u] = scales[(long long)page * p.scales.page_stride + (long long)h * p.scales.head_stride +
-                     slot / PG_BLOCK];
+                     x.slot / PG_BLOCK];
   }
 #pragma unroll
   for (int u = 0; u < V_EACH; ++u) {

@@ -1,0 +1,15 @@
+// Where a thread's piece of pages lies. Plain C++ (constexpr, so that kernels have it too): indexes past
+// 32 bits are checked without a device.
+#pragma once
+
+// Piece `at` of pages of 2^page_shift tokens, PIECES (a power of two) to a token: the row (of pages and
+// heads), the token's slot in it and the piece of the token.
+struct PagedPiece {
+  int row, slot, piece;
+};
+template <int PIECES>
+constexpr PagedPiece paged_piece(long long at, int page_shift) {
+  static_assert(PIECES > 0 && (PIECES & (PIECES - 1)) == 0, "");
+  const long long token = at / PIECES;
+  return {(int)(token >> page_shift), (int)token & ((1 << page_shift) - 1), (int)(at % PIECES)};
+}
