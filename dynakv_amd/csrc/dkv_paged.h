@@ -13,10 +13,12 @@
 #pragma once
 #include "dkv_common.h"
 #include "dkv_mfma_ops.h"
+#include "dkv_paged_index.h"
 
 namespace {
 
 constexpr int PG_DH = 128;
+static_assert(paged_slot_at(1) == PG_DH, "");
 
 // x / d for 0 <= x < 2^31, by a product: m = ceil(2^32 / d) gives the quotient or one more.
 struct Divisor {

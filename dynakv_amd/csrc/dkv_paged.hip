@@ -1003,7 +1003,7 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   auto issue = [&](int t, int page) {  // (scalar work, a wave's by itself: every instruction counts)
     const int key = t * CK + key_in_tile;
     const long long at = (long long)max(page, 0) * p.pool.page_stride +
-                         (long long)((key & slot_mask) * PG_DH);
+                         paged_slot_at(key & slot_mask);
     const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys_from(key) * (PG_DH * 2);
     pg_lds_loads<false>(dkv_make_rsrc(k_head + at, bytes),
                         dkv_lds_addr(sK(t & 1)) + CK / NW * wave * 256, voff);
@@ -1025,8 +1025,8 @@ __device__ __forceinline__ void many_rows(const ChunkParams& c, int wg, uint8_t*
   auto fetch = [&](int t, int page) {
     const int key = t * CK + key_in_tile;
     // (the wave's, and told so: else every load would come in a loop over its lanes' resources)
-    const int in_page = __builtin_amdgcn_readfirstlane((key & slot_mask) * PG_DH);
-    const long long at = (long long)max(page, 0) * p.pool.page_stride + in_page;
+    const int slot = __builtin_amdgcn_readfirstlane(key & slot_mask);
+    const long long at = (long long)max(page, 0) * p.pool.page_stride + paged_slot_at(slot);
     const uint32_t bytes = page < 0 ? 0u : (uint32_t)keys_from(key) * PG_DH;
     const __amdgpu_buffer_rsrc_t rk =
         dkv_make_rsrc((const uint8_t*)p.k + (long long)kvh * p.pool.head_stride + at, bytes);

@@ -1,7 +1,6 @@
 // Pages of 8 bits: the append of a step's keys and values to them, and pages read back as values.
 // The layout of codes and scales: dkv_paged.h. The attention over them: dkv_paged.hip.
 #include "dkv_paged.h"
-#include "dkv_paged_index.h"
 
 namespace {
 
@@ -408,7 +407,7 @@ __global__ __launch_bounds__(V_THREADS) void paged_values_kernel(ValuesParams p)
     const int page = p.ids ? p.ids[i] : i;
     if (page < 0 || page >= p.num_pages) continue;
     const uint8_t* src = pool + (long long)page * p.page_stride + (long long)h * p.head_stride +
-                         x.slot * PG_DH + CODES * x.piece;
+                         paged_slot_at(x.slot) + CODES * x.piece;
     if constexpr (CODES == 8)
       codes[u] = *(const dkv_u32x2*)src;
     else

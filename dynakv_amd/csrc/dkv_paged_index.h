@@ -13,3 +13,6 @@ constexpr PagedPiece paged_piece(long long at, int page_shift) {
   const long long token = at / PIECES;
   return {(int)(token >> page_shift), (int)token & ((1 << page_shift) - 1), (int)(at % PIECES)};
 }
+
+// Elements from the start of a page's head to its slot, 128 each (pages of 2^24 tokens and more pass 32 bits).
+constexpr long long paged_slot_at(int slot) { return (long long)slot * 128; }

@@ -7,7 +7,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from dynakv_amd.kernels.paged import paged_values
+from dynakv_amd.kernels.paged import PagedBatch, paged_attention, paged_values
 
 CSRC = Path(__file__).resolve().parent.parent / "dynakv_amd" / "csrc"
 CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -25,19 +25,71 @@ int main() {
 }
 """
 
+_SLOTS = r"""
+#include <cstdio>
+#include "dkv_paged_index.h"
+int main() {
+  int slot;
+  while (scanf("%d", &slot) == 1) printf("%lld\n", paged_slot_at(slot));
+}
+"""
+
+
+def _answers(tmp_path, source, text):
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    (tmp_path / "main.cpp").write_text(source)
+    subprocess.run(["g++", "-std=c++17", "-I", str(CSRC), str(tmp_path / "main.cpp"), "-o",
+                    str(tmp_path / "main")], check=True)
+    return subprocess.run([str(tmp_path / "main")], input=text, capture_output=True, text=True,
+                          check=True).stdout.split()
+
+
+def test_slots_of_large_pages(tmp_path):
+    """A slot's place in pages of 2^24 tokens and more."""
+    slots = [0, 1, 2**24 - 1, 2**24, 2**24 + 5, 2**25 - 1, 2**25, 2**29 + 7]
+    assert list(map(int, _answers(tmp_path, _SLOTS, " ".join(map(str, slots))))) == [
+        128 * s for s in slots]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 70, 1100])
+def test_a_page_of_many_tokens(dev, new):
+    """A page of 2^25 tokens, some of them past 2^31 elements of it: attention over it, in 8 and in 16 bits, and
+    its values are those of the same memory as pages of 64 tokens."""
+    print(f"[gpu] paged page of 2^25 tokens, {new} new", flush=True)
+    n, whole = 2**24 + 900, 2**25
+    g = torch.Generator(device=dev).manual_seed(6)
+    pools, i32 = [], lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for _ in range(2):
+        codes = torch.zeros(whole, 128, dtype=torch.uint8, device=dev)
+        scales = torch.zeros(whole // 16, dtype=torch.uint8, device=dev)
+        for lo, hi in ((0, 3000), (n - 2000, n)):  # the others' keys and values are 0
+            codes[lo:hi].random_(0, 127, generator=g)
+        scales.random_(116, 119, generator=g)
+        pools.append((codes.view(CODES), scales.view(SCALES)))
+    q = torch.randn(new, 4, 128, generator=g, device=dev).bfloat16()
+    got = []
+    for ps in (whole, 64):
+        k, v = (c.view(whole // ps, 1, ps, 128) for c, _ in pools)
+        ks, vs = (c.view(whole // ps, 1, ps // 16) for _, c in pools)
+        table = torch.arange(whole // ps, dtype=torch.int32, device=dev)[None]
+        batch = PagedBatch(table, i32(0, new), i32(n), rows=new, max_new=new, max_len=n, min_new=new)
+        o = paged_attention(q, k, v, batch, k_scale=ks, v_scale=vs)
+        k, v = paged_values(k, v, ks, vs)
+        part = [t.view(whole, 128)[n - 2000:n].clone() for t in (k, v)]
+        got.append((o, paged_attention(q, k, v, batch), *part))
+        del k, v
+    assert all(bool(o.any()) and not bool(o.isnan().any()) for o in got[0])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
 
 def test_split_of_a_piece(tmp_path):
     """Row, slot and piece of numbers on both sides of 2^31, 2^32 and 2^33, in Python's whole numbers."""
-    if shutil.which("g++") is None:
-        pytest.skip("g++ not available")
-    (tmp_path / "split.cpp").write_text(_MAIN)
-    exe = tmp_path / "split"
-    subprocess.run(["g++", "-std=c++17", "-I", str(CSRC), str(tmp_path / "split.cpp"), "-o", str(exe)],
-                   check=True)
     cases = [(edge + d, shift) for edge in (64, 2**31, 2**32, 2**33, 3 * 2**32)
              for d in (-33, -32, -17, -16, -1, 0, 1, 5, 15, 16, 31, 32, 100) for shift in (4, 6, 12)]
-    out = subprocess.run([str(exe)], input="".join(f"{a} {s}\n" for a, s in cases), capture_output=True,
-                         text=True, check=True).stdout.split()
+    out = _answers(tmp_path, _MAIN, "".join(f"{a} {s}\n" for a, s in cases))
     got = [list(map(int, out[i:i + 6])) for i in range(0, len(out), 6)]
     assert len(got) == len(cases)
     for (at, shift), g in zip(cases, got):
