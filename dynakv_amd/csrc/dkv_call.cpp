@@ -108,6 +108,7 @@ PyMethodDef methods[] = {
     DKV_CALL(dkv_gemv_glu),
     DKV_CALL(dkv_paged_append),
     DKV_CALL(dkv_paged_workspace_floats),
+    DKV_CALL(dkv_paged_workspace_floats_of),
     DKV_CALL(dkv_paged_attention),
     DKV_CALL(dkv_paged_append8),
     DKV_CALL(dkv_paged_attention8),

@@ -1610,14 +1610,18 @@ bool attend_sizes_ok(int B, int T, int Hq, int Hkv, int max_new) {
 
 }  // namespace
 
-extern "C" long long dkv_paged_workspace_floats(int B, int T, int Hq, int Hkv, int max_new,
-                                                int min_new, int max_len) {
+extern "C" long long dkv_paged_workspace_floats_of(int page_bits, int B, int T, int Hq, int Hkv,
+                                                   int max_new, int min_new, int max_len) {
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_new <= 0 || max_len < 0)
     return 0;
   if (!attend_sizes_ok(B, T, Hq, Hkv, max_new)) return 0;
-  // (for either kind of pages)
-  const long long a = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len, false).floats;
-  const long long c = attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len, true).floats;
+  return attend_plan(B, T, Hq, Hkv, max_new, min_new, max_len, page_bits == 8).floats;
+}
+
+extern "C" long long dkv_paged_workspace_floats(int B, int T, int Hq, int Hkv, int max_new,
+                                                int min_new, int max_len) {
+  const long long a = dkv_paged_workspace_floats_of(16, B, T, Hq, Hkv, max_new, min_new, max_len);
+  const long long c = dkv_paged_workspace_floats_of(8, B, T, Hq, Hkv, max_new, min_new, max_len);
   return a > c ? a : c;
 }
 

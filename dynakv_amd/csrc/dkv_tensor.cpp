@@ -193,8 +193,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       b.rows() > T || !aligned16(*q))
     Py_RETURN_NONE;
   at::Tensor out = at::empty({T, hq, HEAD_DIM}, q->options());
-  const long long need = dkv_paged_workspace_floats(b.requests(), b.rows(), (int)hq, (int)hkv,
-                                                    b.max_new(), b.min_new(), b.max_len());
+  const long long need =
+      dkv_paged_workspace_floats_of(pool.ks ? 8 : 16, b.requests(), b.rows(), (int)hq, (int)hkv,
+                                    b.max_new(), b.min_new(), b.max_len());
   float* ws = nullptr;
   long long ws_floats = 0;
   PyObject* held = nullptr;  // until the launch

@@ -411,7 +411,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         o_st = _row_strides(out)
     lib = _lib.calls()
     bounds = batch._args[7:10]
-    need = lib.dkv_paged_workspace_floats(batch._requests, batch._rows, hq, hkv, *bounds)
+    need = lib.dkv_paged_workspace_floats_of(8 if coded else 16, batch._requests, batch._rows, hq, hkv,
+                                             *bounds)
     ws = _attention_workspace(q, stream, need) if need else None
     name = "dkv_paged_attention8" if coded else "dkv_paged_attention"
     _lib.check(_lib.call_on(

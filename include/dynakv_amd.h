@@ -641,9 +641,10 @@ int dkv_gemv_glu(void* stream, int dtype, const void* x, long long x_ld, const v
  * q's strides) q itself. Hq / Hkv <= 16. max_new
  * and max_len bound every request's new tokens and length, min_new (from below) the new tokens of a
  * request that has any: they choose the launch, and what passes them may be left out. The workspace
- * holds dkv_paged_workspace_floats(...) floats, its first 16384 zero (and left zero), 16-byte
- * aligned; it may be null where that is 0. Calls that share it must not overlap on the device: those of one stream may share it,
- * from any threads (a call of two launches makes them together).
+ * holds dkv_paged_workspace_floats_of(16, ...) floats, its first 16384 zero (and left zero), 16-byte
+ * aligned; it may be null where that is 0. (dkv_paged_workspace_floats: enough for pages of 16 and of 8
+ * bits.) Calls that share it must not overlap on the device: those of one stream may share it, from any
+ * threads (a call of two launches makes them together).
  */
 int dkv_paged_append(void* stream, int dtype, const void* qkv, long long qkv_ld, void* q_out,
                      long long q_st, long long q_sh, void* k_pages, void* v_pages,
@@ -653,6 +654,8 @@ int dkv_paged_append(void* stream, int dtype, const void* qkv, long long qkv_ld,
                      const void* k_norm, float eps, const double* inv_freq);
 long long dkv_paged_workspace_floats(int B, int T, int Hq, int Hkv, int max_new, int min_new,
                                      int max_len);
+long long dkv_paged_workspace_floats_of(int page_bits, int B, int T, int Hq, int Hkv, int max_new,
+                                        int min_new, int max_len);
 int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st, long long q_sh,
                         const void* k_pages, const void* v_pages, long long page_stride,
                         long long head_stride, int num_pages, int page_size,
@@ -675,7 +678,8 @@ int dkv_paged_attention(void* stream, int dtype, const void* q, long long q_st, 
  * rounded to the nearest code (ties to even). What is infinite or NaN is held as NaN. New tokens of one
  * call must not share a block with another request's.
  *
- * dkv_paged_attention8: dkv_paged_attention over the pages' values; its workspace is the same.
+ * dkv_paged_attention8: dkv_paged_attention over the pages' values; its workspace holds
+ * dkv_paged_workspace_floats_of(8, ...) floats.
  *
  * dkv_paged_values: the values of pages ids[0 .. n - 1] (device; zeros for one outside the pool), or of the
  * pages 0 .. n - 1 where ids is null, to k_out and v_out, each (n, Hkv, page_size, 128) of out_dtype,
