@@ -208,7 +208,10 @@ __device__ __forceinline__ int swizzle8(int t) { return (t ^ (t >> 3)) & 7; }
 // beside 20 of 500, in parts, 66. Of 8-bit pages 256 to 511 units go to 512 workgroups of four waves, in
 // parts: 40 requests of 2K to 8K 76 us (87 in workgroups of eight waves), one of 65536 beside 39 of 500 37
 // (357); with fewer or more units those are the slower ones (4 requests 16.4 us against 14.6, 80 156 against
-// 142: a part more is a record more, and fewer waves share a unit's start and end).
+// 142: a part more is a record more, and fewer waves share a unit's start and end). Of more requests than a
+// wave holds the lengths of (257 to 511 of one KV head) they are not cut, but go to the chip at once, where
+// eight waves make a second round: 400 of 300 tokens 10 us against 13, of 2000 36.0 against 39.5, of 8000
+// 130 against 132; with one of 8000 beside 399 of 300 they are the slower ones (69 against 48).
 constexpr int DSLOT = 2;                    // tile slots per wave
 template <bool Q8>
 constexpr int DTILE = Q8 ? 32 : 16;
