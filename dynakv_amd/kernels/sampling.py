@@ -110,7 +110,8 @@ def adjust_logits_(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
     default), the others generated. Settings are numbers or (rows,) fp32 tensors. In this order, for a
     token that is
 
-    * in ``tokens``: x / ``repetition`` where x > 0, else x * ``repetition`` (which must be positive);
+    * in ``tokens``: x / ``repetition`` where x > 0, else x * ``repetition`` (which must be positive and
+      finite: a number is checked, a tensor's entries, which would have to be read back, are not);
     * generated n > 0 times: x - n * ``frequency`` - ``presence``;
     * in ``bias_ids[b]`` ((rows, M) int32): x + its ``bias[b]`` ((rows, M) fp32), several of one token
       added up in their order;

@@ -169,7 +169,7 @@ class Sampler:
     """Draws tokens from logits: a generator's replacement for its argmax. The settings are those of
     ``sample_tokens`` and, before them, the penalties of ``adjust_logits_`` over a request's tokens:
     numbers or a tensor with an entry per row (of a batch, or of the requests that are generated for).
-    ``bias`` maps tokens to what is added to their logits. The uniform numbers come from a generator of
+    ``bias`` maps tokens to what is added to their logits, for all rows. The uniform numbers come from a generator of
     its own, so a seed gives the same draws for the same logits."""
 
     _NEUTRAL = dict(repetition=1.0, frequency=0.0, presence=0.0)
@@ -178,6 +178,10 @@ class Sampler:
                  frequency=0.0, presence=0.0, bias: dict[int, float] | None = None, seed: int = 0,
                  device="cuda"):
         self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        # (here, where a tensor may be read back: the operator, which does not, divides by its entries)
+        rep = torch.as_tensor(repetition, dtype=torch.float32)
+        if not bool(((rep > 0.0) & (rep < float("inf"))).all()):
+            raise ValueError("repetition must be positive and finite")
         given = dict(repetition=repetition, frequency=frequency, presence=presence)
         self.penalties = {name: v for name, v in given.items()
                           if torch.is_tensor(v) or v != self._NEUTRAL[name]}

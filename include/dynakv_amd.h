@@ -731,7 +731,8 @@ int dkv_sample_tokens(void* stream, int dtype, const void* logits, long long ld,
  * fp32), in place, in fp32 with one rounding. Row's history: tokens[0 .. len - 1] of row's N (row stride
  * tokens_ld, 4 or 8 bytes each; null or N = 0: none), those from prompt on generated. Settings and lengths
  * per row where the pointer is given, else the value beside it. In this order, for token i:
- *   in the history:           x > 0 ? x / repetition : x * repetition (repetition > 0)
+ *   in the history:           x > 0 ? x / repetition : x * repetition (positive and finite: not
+ *                             checked where the pointer is given)
  *   n > 0 times generated:    x - frequency * n - presence
  *   in bias_ids[0 .. M - 1]:  x + the sum of its biases, in their order
  *   bit i % 32 of allowed[i / 32] is 0 (null: no mask):  -infinity
