@@ -1489,7 +1489,8 @@ struct AttendPlan {
 //  * otherwise one range: above 256 of 128 rows 1x8 (eight 300-token prompts 22.7, against 23.5 1x4,
 //    25.5 2x4), else 1x4 (512 tokens at 1024: 20.1, against 24.4 1x8 and 29 2x4/2: a range more
 //    costs its records, 66 KB a workgroup, written and read). Of 8-bit pages 2x4 above 256 (one
-//    2048-token prompt 57.8, against 63.5 1x4; 1x8 has no registers for codes on their way).
+//    2048-token prompt 57.8, against 63.5 1x4; 1x8 has no registers for codes on their way; shorter
+//    prompts and steps with single tokens beside were not measured of 8-bit pages).
 AttendPlan attend_plan(int B, int T, int Hq, int Hkv, int max_new, int min_new, int max_len,
                        bool q8) {
   AttendPlan a = {};

@@ -19,9 +19,11 @@ constexpr int E_HIGH = DT == DKV_F16 ? 7 : 119;
 //       holds earlier tokens of the request (its first slots), whose codes are then rounded again,
 //   c = y / 2^e rounded to the nearest e4m3 (ties to even), at most 448.
 // Scales are powers of two: a code moved to a larger one only loses what falls below 2^-9 of it, so
-// tokens that come one by one are held as those that come at once are, but for a last bit down there;
-// a value's relative error is that of e4m3 (2^-4) from 2^-15 of the block's largest on. Values that
-// are infinite or NaN are held as NaN and have no say in e.
+// tokens that come one by one are held as those that come at once are, but for a last bit down there.
+// A value is off by at most 2^-4 of itself from 2^-6 of the scale on, below that by 2^-10 of the scale.
+// The block's largest lies between 224 and 448 scales where the scale is its least, so that is from
+// 2^-13.8 of the largest on; a larger scale kept from earlier tokens raises the border with it. Values
+// that are infinite or NaN are held as NaN and have no say in e.
 //
 // Keys are computed in 64 bits: which code a value gets turns over at borders, and 32-bit arithmetic with
 // the sine instruction (off by 2^-19 or so) would put some hundreds of 8 million on another side of one.
@@ -381,7 +383,7 @@ struct ValuesParams {
   void* v_out;
 };
 // A thread's codes of one access: a wave's stores are whole lines (16 codes, two stores of every other 16
-// bytes: 50 us instead of 44 for 1024 pages of 64 tokens)
+// bytes: 50 us instead of 44 for 512 pages of 64 tokens, through the caches)
 template <int ODT>
 constexpr int V_CODES = ODT == DKV_F32 ? 4 : 8;
 constexpr int V_THREADS = 256, V_EACH = 8;
