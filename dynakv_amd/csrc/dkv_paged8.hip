@@ -16,7 +16,8 @@ constexpr int E_HIGH = DT == DKV_F16 ? 7 : 119;
 // Append to 8-bit pages. Queries as in the 16-bit append. Keys y (normed, rotated) and values y of one
 // block (16 tokens, one head) get one exponent
 //   e = least with max |y| <= 448 2^e, within E_LOW .. E_HIGH, and at least the block's old one where it
-//       holds earlier tokens of the request (its first slots), whose codes are then rounded again,
+//       holds earlier tokens of the request (its first slots), whose codes are rounded again where their
+//       scale changes (it rises, or lay outside the range),
 //   c = y / 2^e rounded to the nearest e4m3 (ties to even), at most 448.
 // Scales are powers of two: a code moved to a larger one only loses what falls below 2^-9 of it, so
 // tokens that come one by one are held as those that come at once are, but for a last bit down there.
@@ -282,12 +283,14 @@ __device__ __forceinline__ void append8_block(const Append8Params& p, int wg, do
   __syncthreads();
   if (!there) return;
   need = max(need, sNeed[wave ^ 1]);
-  const int old_e = min(max((int)old_byte - 127, E_LOW<DT>), E_HIGH<DT>);
+  // (the block's own exponent may lie outside the range: pages of another type's, or a user's)
+  const int old_e = __builtin_amdgcn_readfirstlane((int)old_byte) - 127;
   int e_new = min(max(need, E_LOW<DT>), E_HIGH<DT>);
-  if (has_old) e_new = max(e_new, old_e);
+  if (has_old) e_new = max(e_new, min(max(old_e, E_LOW<DT>), E_HIGH<DT>));
   e_new = __builtin_amdgcn_readfirstlane(e_new);
+  const bool again = has_old && e_new != old_e;  // earlier codes are rounded to the new scale
 
-  const bool any = __ballot(odd) || need > E_HIGH<DT>;
+  const bool any = __ballot(odd) || need > E_HIGH<DT> || (again && old_e > e_new);
   if (isnew) {
     if (is_k) {
       // y / 2^e as floats from which e4m3 rounds as it would from y: where rounding to fp32 landed on a
@@ -313,21 +316,23 @@ __device__ __forceinline__ void append8_block(const Append8Params& p, int wg, do
 #pragma unroll
       for (int e = 0; e < 16; ++e) f[e] *= by;
     }
-  } else if (isold && e_new > old_e) {
-    const float down = __uint_as_float((uint32_t)max(127 + old_e - e_new, 0) << 23);
+  } else if (isold && again) {
+    // 2^(old_e - e_new), from 2^18 on as 2^18: every code but 0 is then past 448. Byte 255 is NaN.
+    const int up = min(max(old_e - e_new, -127), 18);
+    const float by = old_e == 128 ? NAN : __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      f[4 * h] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 0) * down;
-      f[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 1) * down;
-      f[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 2) * down;
-      f[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 3) * down;
-      f[8 + 4 * h] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 0) * down;
-      f[8 + 4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 1) * down;
-      f[8 + 4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 2) * down;
-      f[8 + 4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 3) * down;
+      f[4 * h] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 0) * by;
+      f[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 1) * by;
+      f[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 2) * by;
+      f[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(oa[h], 3) * by;
+      f[8 + 4 * h] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 0) * by;
+      f[8 + 4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 1) * by;
+      f[8 + 4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 2) * by;
+      f[8 + 4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(ob[h], 3) * by;
     }
   }
-  if (isnew || (isold && e_new > old_e)) {
+  if (isnew || (isold && again)) {
     if (any) {
       *(dkv_u32x2*)codes = encode8<true>(f);
       *(dkv_u32x2*)(codes + 64) = encode8<true>(f + 8);

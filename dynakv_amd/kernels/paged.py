@@ -322,7 +322,8 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     tokens of the request keeps its scale where that is larger, and else has their codes rounded again
     to the new one (a request cut back by ``truncate`` into a block leaves that block's scale). Scales
     are 2^-15 to 2^7 for fp16 and 2^-110 to 2^119 for bf16, so that every value held is one of qkv's
-    type: what is past 448 times the largest is held as that, and what is infinite or NaN as NaN.
+    type: what is past 448 times the largest is held as that, and what is infinite or NaN as NaN. (So are
+    earlier tokens whose block had a scale outside that, from pages of another type.)
     Requests of one call must not share such a block."""
     freqs = _frequency_address(theta, inv_freq)
     fast = _lib.tensor_calls()
