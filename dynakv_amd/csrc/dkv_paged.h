@@ -108,21 +108,26 @@ __device__ __forceinline__ dkv_u32x4 round8(const float (&f)[8]) {
   return dkv_u32x4{w[0], w[1], w[2], w[3]};
 }
 
-// The request of row `row`: the last one that starts at or before it (64 starts per step, one per
-// lane), or -1 for a row of no request.
-__device__ __forceinline__ int request_of_row(const int* q_start, int B, int row, int lane) {
-  if (row < q_start[0] || row >= q_start[B]) return -1;
+// The last request for which starts(b) holds, as it does for every one before (64 a step, one per lane);
+// 0 if for none.
+template <class F>
+__device__ __forceinline__ int last_request(int B, int lane, F&& starts) {
   int lo = 0, n = B;
   while (n > 1) {
     const int step = (n + 63) / 64;
     const int i = lo + lane * step;
-    const bool at = lane * step < n && q_start[min(i, B - 1)] <= row;
+    const bool at = lane * step < n && starts(min(i, B - 1));
     const int cnt = max(1, __popcll(__ballot(at)));
     const int skip = (cnt - 1) * step;
     lo += skip;
     n = min(step, n - skip);
   }
   return lo;
+}
+// The request of row `row`: the last one that starts at or before it, or -1 for a row of no request.
+__device__ __forceinline__ int request_of_row(const int* q_start, int B, int row, int lane) {
+  if (row < q_start[0] || row >= q_start[B]) return -1;
+  return last_request(B, lane, [&](int b) { return q_start[b] <= row; });
 }
 
 // A head's 128 values at src, optionally normed with weights nw and rotated by position pos: dims

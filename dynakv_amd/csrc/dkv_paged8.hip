@@ -56,6 +56,7 @@ struct Append8Params {
   const int* lens;
   int B, T, Hq, Hkv;
   int kv_wgs;      // leading workgroups: blocks times groups of units
+  int by_row;      // an item for every row, as many as for the blocks' places
   Divisor by_groups, by_q_groups;
   const uint16_t* q_norm;  // (128,), or null: no norm
   const uint16_t* k_norm;
@@ -64,6 +65,7 @@ struct Append8Params {
 };
 
 constexpr int A8_WAVES = 8, A8_UNITS = 4;  // of a workgroup
+constexpr int A8_SCAN = 256;  // requests that one wave sums over (64 at a time)
 constexpr int A8_ROW = 72;  // pairs of doubles a token's sines and cosines take in LDS
 
 // A block with new tokens: tokens t_lo .. t_hi - 1 of request b, all in block [base, base + 16).
@@ -72,8 +74,42 @@ struct NewBlock {
   int base, t_lo, t_hi;
   int row_of_0;  // row of token t: row_of_0 + t
 };
-// The item-th block with new tokens, request by request.
+// The item-th block with new tokens, request by request. Of more than A8_SCAN requests the one at the item-th
+// place instead (paged_block_place), or the one whose first new token is row `item`, if there is one: found
+// by a search, where sums over the requests before it would make the launch's time go by their square: single
+// tokens of 512 requests 15.4 us (summed 17.2), of 1024 30.8 (42.4), of 4096 123 (370); of 256 9.4 (9.2).
 __device__ __forceinline__ NewBlock new_block(const Append8Params& p, int item, int lane) {
+  if (p.B > A8_SCAN) {
+    const NewBlock none = {-1, 0, 0, 0, 0};
+    int b, first = 0;
+    if (p.by_row) {
+      b = request_of_row(p.q_start, p.B, item, lane);
+      if (b < 0) return none;
+    } else {
+      b = last_request(p.B, lane,
+                       [&](int i) { return paged_block_place(max(p.q_start[i], 0), i) <= item; });
+      first = paged_block_place(max(p.q_start[b], 0), b);
+      if (first > item) return none;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    const PagedRequest r = uniform(paged_request(p.pool, p.q_start, p.lens, b, p.T));
+    const int lo = max(r.pos0, 0);
+    const int hi = (int)min((long long)r.pos0 + r.n, (long long)p.pool.cols << p.pool.page_shift);
+    if (r.n <= 0 || hi <= lo) return none;
+    NewBlock n = {b, 0, 0, 0, r.row0 - r.pos0};
+    if (p.by_row) {
+      const int t = item - n.row_of_0;
+      if (t < lo || t >= hi || (t != lo && t % PG_BLOCK)) return none;
+      n.base = t / PG_BLOCK * PG_BLOCK;
+    } else {
+      const long long base = (lo / PG_BLOCK + (long long)(item - first)) * PG_BLOCK;
+      if (base >= hi) return none;
+      n.base = (int)base;
+    }
+    n.t_lo = max(lo, n.base);
+    n.t_hi = min(hi, n.base + PG_BLOCK);
+    return n;
+  }
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     int count = 0, lo = 0, hi = 0, off = 0;
@@ -511,6 +547,7 @@ extern "C" int dkv_paged_append8(void* stream, int dtype, const void* qkv, long 
   const long long wgs = blocks * groups + (q_items + A8_WAVES - 1) / A8_WAVES;
   if (wgs > 0x7fffffffLL || q_items > 0x7fffffffLL - A8_WAVES) return DKV_E_UNSUPPORTED;
   p.kv_wgs = (int)(blocks * groups);
+  p.by_row = blocks == T;
   p.by_groups = divisor(groups);
   p.by_q_groups = divisor(q_groups);
   hipStream_t st = (hipStream_t)stream;

@@ -125,3 +125,28 @@ def test_values_of_more_pieces_than_31_bits(dev, dtype):
             assert torch.equal(got[a:b], held[ids[a:b].long()]), (a, b)
     del out
     torch.cuda.empty_cache()
+
+
+_BLOCKS = r"""
+#include <cstdio>
+#include "dkv_paged_index.h"
+int main() {
+  int start, b;
+  while (scanf("%d %d", &start, &b) == 2) printf("%d\n", paged_block_place(start, b));
+}
+"""
+
+
+def test_places_of_blocks(tmp_path):
+    """A request has a place for every block that its new tokens can touch, wherever its rows and its tokens
+    begin, and all of them fit the launch: rows / 16 + 2 for each request."""
+    g = torch.Generator().manual_seed(4)
+    starts = [0]
+    for n in torch.cat([torch.randint(0, 70, (500,), generator=g), torch.arange(0, 70)]).tolist():
+        starts.append(starts[-1] + n)
+    out = list(map(int, _answers(tmp_path, _BLOCKS, "".join(f"{s} {b}\n" for b, s in enumerate(starts)))))
+    for b in range(len(starts) - 1):
+        n = starts[b + 1] - starts[b]
+        most = max((pos + n - 1) // 16 - pos // 16 + 1 for pos in range(16)) if n else 0
+        assert out[b + 1] - out[b] >= most, b
+    assert out[0] == 0 and out[-1] == starts[-1] // 16 + 2 * (len(starts) - 1)
